@@ -269,7 +269,7 @@ def prepare(case, seed):
         if own:
             lib = _lib()
             st["cache"] = lib.KVCache(st["k"], st["v"], st["table"], st["ks"], st["vs"])
-            size = lib.attn_tree_workspace(st["cache"], c["heads"], c["tree"], c["ctx"] + c["tree"])
+            size = lib.attn_tree_workspace(st["cache"], c["heads"], st["q"].shape[0], c["tree"], c["ctx"] + c["tree"])
             st["ws"] = torch.empty(size, dtype=torch.uint8, device=DEV)
     else:
         st["x"], st["tok"] = _logits(c, seed)
