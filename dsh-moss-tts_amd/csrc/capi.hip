@@ -1,6 +1,7 @@
 // capi.hip -- extern "C" entry points of libmoss_hip.so (declared in include/moss_hip.h).
 // No exception crosses this boundary: failures become status codes plus a
 // thread-local message (moss_hip_last_error).
+#include <cmath>
 #include <cstdio>
 #include <map>
 #include <mutex>
@@ -10,6 +11,7 @@
 
 #include "batch_model.h"
 #include "codec.h"
+#include "paged_ops.h"
 
 using mh::Status;
 
@@ -559,6 +561,299 @@ int moss_hip_attn_paged(const float *q, const void *k_pool, const void *v_pool, 
         a.out_f16 = out_dtype == MOSS_HIP_F16;
         const auto kv = kv_dtype == MOSS_HIP_F32 ? mh::KV_F32 : mh::KV_F16;
         mh::hip_check(mh::launch_attn(a, kv, static_cast<hipStream_t>(stream)), "attention launch");
+    });
+}
+
+}  // extern "C"
+
+// ------------------------------------------------------------------ a caller's own decoding loop
+
+namespace {
+
+constexpr int kMaxRows = 1 << 22, kMaxHeads = 1024, kMaxRot = 512;
+
+void check_row_type(int dtype) {
+    if (dtype != MOSS_HIP_F32 && dtype != MOSS_HIP_F16) throw Status(MOSS_HIP_EINVAL, "dtype must be MOSS_HIP_F32 or MOSS_HIP_F16");
+}
+
+mh::RopeArgs rope_args(const moss_hip_rope *r, int head_dim) {
+    if (r->freqs == nullptr) throw Status(MOSS_HIP_EINVAL, "rope: null freqs");
+    if (r->rot_dim < 2 || r->rot_dim % 2 || r->rot_dim > kMaxRot || r->rot_dim > head_dim)
+        throw Status(MOSS_HIP_EINVAL, "rope: rot_dim must be even, 2 .. 512 and at most head_dim");
+    if (r->halves != 0 && r->halves != 1) throw Status(MOSS_HIP_EINVAL, "rope: halves must be 0 or 1");
+    mh::RopeArgs a;
+    a.freqs = r->freqs;
+    a.rot = r->rot_dim;
+    a.halves = r->halves;
+    a.mscale = r->mscale;
+    return a;
+}
+
+// The shape of a cache: what the workspace sizes need.
+mh::KvCacheArgs cache_shape(const moss_hip_kv_cache *c) {
+    if (c == nullptr) throw Status(MOSS_HIP_EINVAL, "null cache");
+    if (c->kv_dtype < MOSS_HIP_F32 || c->kv_dtype > MOSS_HIP_E4M3) throw Status(MOSS_HIP_EINVAL, "kv_dtype must be MOSS_HIP_F32, F16, I8 or E4M3");
+    if (c->head_dim != 64 && c->head_dim != 128) throw Status(MOSS_HIP_EINVAL, "head_dim must be 64 or 128");
+    if (c->kv_heads <= 0 || c->kv_heads > kMaxHeads) throw Status(MOSS_HIP_EINVAL, "need 0 < kv_heads <= 1024");
+    if (c->page_size <= 0 || c->page_size % 16 || c->page_size > mh::kTreePageMax)
+        throw Status(MOSS_HIP_EINVAL, "page_size must be a multiple of 16 and at most 32768");
+    if (c->streams < 0 || c->streams > (1 << 16)) throw Status(MOSS_HIP_EINVAL, "need 0 <= streams <= 65536");
+    mh::KvCacheArgs a;
+    a.dtype = c->kv_dtype;
+    a.heads = c->kv_heads;
+    a.dim = c->head_dim;
+    a.page_size = c->page_size;
+    a.streams = c->streams;
+    return a;
+}
+
+mh::KvCacheArgs cache_args(const moss_hip_kv_cache *c) {
+    mh::KvCacheArgs a = cache_shape(c);
+    if (!c->k || !c->v || !c->page_table) throw Status(MOSS_HIP_EINVAL, "cache: null pointer");
+    if (c->n_pages <= 0 || c->table_stride <= 0) throw Status(MOSS_HIP_EINVAL, "cache: need n_pages, table_stride > 0");
+    const bool q8 = mh::quantised(c->kv_dtype);
+    if (q8 != (c->k_scale != nullptr) || q8 != (c->v_scale != nullptr))
+        throw Status(MOSS_HIP_EINVAL, "cache: I8 and E4M3 pools have scales, F32 and F16 pools have none");
+    if (((uintptr_t)c->k | (uintptr_t)c->v | (uintptr_t)c->k_scale | (uintptr_t)c->v_scale) % 16)
+        throw Status(MOSS_HIP_EINVAL, "cache: pools and scales must be 16-byte aligned");
+    a.k = c->k;
+    a.v = c->v;
+    a.k_scale = c->k_scale;
+    a.v_scale = c->v_scale;
+    a.n_pages = c->n_pages;
+    a.table = c->page_table;
+    a.table_stride = c->table_stride;
+    return a;
+}
+
+void check_rows(int rows) {
+    if (rows < 0 || rows > kMaxRows) throw Status(MOSS_HIP_EINVAL, "need 0 <= rows <= 4194304");
+}
+
+mh::KvCacheArgs tree_shape(const moss_hip_kv_cache *c, int heads, int rows, int max_rows, int max_keys) {
+    const mh::KvCacheArgs a = cache_shape(c);
+    check_rows(rows);
+    if (heads <= 0 || heads > kMaxHeads || heads % a.heads) throw Status(MOSS_HIP_EINVAL, "heads must be a multiple of kv_heads, at most 1024");
+    if (max_rows <= 0 || max_rows > mh::kTreeMax) throw Status(MOSS_HIP_EINVAL, "need 0 < max_rows <= 64");
+    if (max_keys <= 0 || max_keys > mh::kTreeKeysMax) throw Status(MOSS_HIP_EINVAL, "need 0 < max_keys <= 2^28");
+    if ((long long)a.streams * max_rows * heads > (1 << 22)) throw Status(MOSS_HIP_EINVAL, "streams * max_rows * heads must be at most 2^22");
+    return a;
+}
+
+void logprobs_shape(int rows, int vocab, int top_k) {
+    check_rows(rows);
+    if (vocab <= 0 || vocab > mh::kVocabMax) throw Status(MOSS_HIP_EINVAL, "need 0 < vocab <= 2^20");
+    if (top_k < 0 || top_k > mh::kTopMax) throw Status(MOSS_HIP_EINVAL, "need 0 <= top_k <= 32");
+    if ((long long)rows * vocab > (1ll << 34)) throw Status(MOSS_HIP_EINVAL, "rows * vocab must be at most 2^34");
+}
+
+void check_workspace(const void *ws, size_t bytes, size_t need, const char *call) {
+    if (need == 0) return;
+    if (ws == nullptr || bytes < need)
+        throw Status(MOSS_HIP_EINVAL, std::string(call) + ": the workspace needs " + std::to_string(need) + " bytes");
+    if ((uintptr_t)ws % 16) throw Status(MOSS_HIP_EINVAL, std::string(call) + ": the workspace must be 16-byte aligned");
+}
+
+}  // namespace
+
+extern "C" {
+
+int moss_hip_rope_freqs(const moss_hip_rope_params *p, double *freqs, float *mscale) {
+    return guard([&] {
+        if (!p || !freqs || !mscale) throw Status(MOSS_HIP_EINVAL, "null argument");
+        const int d = p->rot_dim;
+        if (d < 2 || d % 2 || d > kMaxRot) throw Status(MOSS_HIP_EINVAL, "rot_dim must be even, 2 .. 512");
+        if (p->scaling < MOSS_HIP_ROPE_PLAIN || p->scaling > MOSS_HIP_ROPE_YARN) throw Status(MOSS_HIP_EINVAL, "bad scaling");
+        double base = p->base == 0.0 ? 10000.0 : p->base;
+        if (!(base > 1.0) || !std::isfinite(base)) throw Status(MOSS_HIP_EINVAL, "base must be above 1");
+        const double factor = p->scaling == MOSS_HIP_ROPE_PLAIN ? 1.0 : p->factor;
+        if (!(factor >= 1.0) || !std::isfinite(factor)) throw Status(MOSS_HIP_EINVAL, "factor must be at least 1");
+        if (p->scaling == MOSS_HIP_ROPE_NTK) {
+            if (d < 4) throw Status(MOSS_HIP_EINVAL, "MOSS_HIP_ROPE_NTK needs rot_dim >= 4");
+            base *= std::pow(factor, d / (d - 2.0));
+        }
+        const bool yarn = p->scaling == MOSS_HIP_ROPE_YARN;
+        const bool std_betas = p->beta_fast == 0.0 && p->beta_slow == 0.0;
+        const double fast = std_betas ? 32.0 : p->beta_fast, slow = std_betas ? 1.0 : p->beta_slow;
+        if (yarn && (p->orig_ctx <= 0 || !(fast > slow) || !(slow >= 0.0) || !std::isfinite(fast)))
+            throw Status(MOSS_HIP_EINVAL, "MOSS_HIP_ROPE_YARN needs orig_ctx > 0 and beta_fast > beta_slow >= 0");
+        for (int i = 0; i < d / 2; ++i) {
+            double w = std::pow(base, -2.0 * i / d);
+            if (p->scaling == MOSS_HIP_ROPE_LINEAR) w /= factor;
+            if (yarn) {
+                const double turns = p->orig_ctx * w / (2.0 * 3.14159265358979323846);
+                const double g = std::min(1.0, std::max(0.0, (turns - slow) / (fast - slow)));
+                w = g * w + (1.0 - g) * w / factor;
+            }
+            freqs[i] = w;
+        }
+        *mscale = yarn ? (float)(0.1 * std::log(factor) + 1.0) : 1.0f;
+    });
+}
+
+int moss_hip_rope_rows(const void *x, int64_t x_row_stride, int64_t x_head_stride, void *y, int64_t y_row_stride,
+                       int64_t y_head_stride, int dtype, int rows, int heads, int head_dim, const int32_t *pos,
+                       const moss_hip_rope *rope, void *stream) {
+    return guard([&] {
+        if (!x || !y || !pos || !rope) throw Status(MOSS_HIP_EINVAL, "null pointer");
+        check_row_type(dtype);
+        check_rows(rows);
+        if (heads <= 0 || heads > kMaxHeads || head_dim <= 0 || head_dim > 1024)
+            throw Status(MOSS_HIP_EINVAL, "need 0 < heads, head_dim <= 1024");
+        if (x_row_stride < 0 || x_head_stride < 0 || y_row_stride < 0 || y_head_stride < 0)
+            throw Status(MOSS_HIP_EINVAL, "strides must not be negative");
+        if (x == y && (x_row_stride != y_row_stride || x_head_stride != y_head_stride))
+            throw Status(MOSS_HIP_EINVAL, "in place, x and y must have the same strides");
+        if ((heads > 1 && y_head_stride < head_dim) || (rows > 1 && y_row_stride == 0))
+            throw Status(MOSS_HIP_EINVAL, "rows and heads of y must not overlap");
+        mh::RopeRowsArgs a;
+        a.rope = rope_args(rope, head_dim);
+        if (rows == 0) return;
+        a.x = x;
+        a.y = y;
+        a.dtype = dtype;
+        a.rows = rows;
+        a.heads = heads;
+        a.dim = head_dim;
+        a.x_row = x_row_stride;
+        a.x_head = x_head_stride;
+        a.y_row = y_row_stride;
+        a.y_head = y_head_stride;
+        a.pos = pos;
+        mh::hip_check(mh::launch_rope_rows(a, static_cast<hipStream_t>(stream)), "rope launch");
+    });
+}
+
+int moss_hip_kv_write(const moss_hip_kv_cache *cache, const void *k, int64_t k_stride, const void *v, int64_t v_stride,
+                      int dtype, int rows, const int32_t *row_stream, const int32_t *row_pos, const moss_hip_rope *rope,
+                      const int32_t *rope_pos, void *stream) {
+    return guard([&] {
+        mh::KvRowsArgs a;
+        a.c = cache_args(cache);
+        if (!k || !v || !row_stream || !row_pos) throw Status(MOSS_HIP_EINVAL, "null pointer");
+        check_row_type(dtype);
+        check_rows(rows);
+        if (k_stride < 0 || v_stride < 0) throw Status(MOSS_HIP_EINVAL, "strides must not be negative");
+        if (rope != nullptr)
+            a.rope = rope_args(rope, a.c.dim);
+        else if (rope_pos != nullptr)
+            throw Status(MOSS_HIP_EINVAL, "rope_pos without rope");
+        if (rows == 0 || a.c.streams == 0) return;
+        a.k = k;
+        a.v = v;
+        a.k_row = k_stride;
+        a.v_row = v_stride;
+        a.dtype = dtype;
+        a.rows = rows;
+        a.stream = row_stream;
+        a.pos = row_pos;
+        a.rope_pos = rope_pos;
+        mh::hip_check(mh::launch_kv_write(a, static_cast<hipStream_t>(stream)), "kv write launch");
+    });
+}
+
+int moss_hip_kv_read(const moss_hip_kv_cache *cache, const int32_t *row_stream, const int32_t *row_pos, int rows, void *k,
+                     int64_t k_stride, void *v, int64_t v_stride, int dtype, void *stream) {
+    return guard([&] {
+        mh::KvRowsArgs a;
+        a.c = cache_args(cache);
+        if (!k || !v || !row_stream || !row_pos) throw Status(MOSS_HIP_EINVAL, "null pointer");
+        check_row_type(dtype);
+        check_rows(rows);
+        const int64_t width = (int64_t)a.c.heads * a.c.dim;
+        if (rows > 1 && (k_stride < width || v_stride < width)) throw Status(MOSS_HIP_EINVAL, "rows of k and v must not overlap");
+        if (rows == 0) return;
+        a.k_out = k;
+        a.v_out = v;
+        a.k_row = k_stride;
+        a.v_row = v_stride;
+        a.dtype = dtype;
+        a.rows = rows;
+        a.stream = row_stream;
+        a.pos = row_pos;
+        mh::hip_check(mh::launch_kv_read(a, static_cast<hipStream_t>(stream)), "kv read launch");
+    });
+}
+
+int moss_hip_attn_tree_workspace(const moss_hip_kv_cache *cache, int heads, int rows, int max_rows, int max_keys, size_t *bytes) {
+    return guard([&] {
+        if (bytes == nullptr) throw Status(MOSS_HIP_EINVAL, "null output");
+        const mh::KvCacheArgs c = tree_shape(cache, heads, rows, max_rows, max_keys);
+        *bytes = rows == 0 || c.streams == 0 ? 0 : mh::tree_workspace(c, heads, rows, max_rows, max_keys);
+    });
+}
+
+int moss_hip_attn_tree(const void *q, int64_t q_stride, int q_dtype, int heads, const moss_hip_kv_cache *cache,
+                       const int32_t *row_start, const int32_t *ctx_len, const uint64_t *row_mask, int rows, int max_rows,
+                       int max_keys, float scale, void *out, int64_t out_stride, int out_dtype, float *lse, void *workspace,
+                       size_t workspace_bytes, void *stream) {
+    return guard([&] {
+        mh::TreeArgs a;
+        tree_shape(cache, heads, rows, max_rows, max_keys);
+        a.c = cache_args(cache);
+        if (!q || !row_start || !ctx_len || !out) throw Status(MOSS_HIP_EINVAL, "null pointer");
+        check_row_type(q_dtype);
+        check_row_type(out_dtype);
+        const int64_t width = (int64_t)heads * a.c.dim;
+        if (q_stride < 0) throw Status(MOSS_HIP_EINVAL, "strides must not be negative");
+        if (rows > 1 && out_stride < width) throw Status(MOSS_HIP_EINVAL, "rows of out must not overlap");
+        if (!std::isfinite(scale)) throw Status(MOSS_HIP_EINVAL, "scale must be finite");
+        if (rows == 0 || a.c.streams == 0) return;
+        check_workspace(workspace, workspace_bytes, mh::tree_workspace(a.c, heads, rows, max_rows, max_keys), "moss_hip_attn_tree");
+        a.q = q;
+        a.q_dtype = q_dtype;
+        a.q_row = q_stride;
+        a.out_row = out_stride;
+        a.heads = heads;
+        a.row_start = row_start;
+        a.ctx_len = ctx_len;
+        a.row_mask = row_mask;
+        a.rows = rows;
+        a.max_rows = max_rows;
+        a.max_keys = max_keys;
+        a.scale = scale;
+        a.out = out;
+        a.out_dtype = out_dtype;
+        a.lse = lse;
+        a.ws = workspace;
+        mh::hip_check(mh::launch_attn_tree(a, static_cast<hipStream_t>(stream)), "attention launch");
+    });
+}
+
+int moss_hip_token_logprobs_workspace(int rows, int vocab, int top_k, size_t *bytes) {
+    return guard([&] {
+        if (bytes == nullptr) throw Status(MOSS_HIP_EINVAL, "null output");
+        logprobs_shape(rows, vocab, top_k);
+        *bytes = rows == 0 ? 0 : mh::logprobs_workspace(rows, vocab, top_k);
+    });
+}
+
+int moss_hip_token_logprobs(const void *logits, int64_t row_stride, int dtype, int rows, int vocab, const int32_t *tokens,
+                            float inv_temperature, float *logprob, float *entropy, int top_k, int32_t *top_ids,
+                            float *top_logprobs, void *workspace, size_t workspace_bytes, void *stream) {
+    return guard([&] {
+        logprobs_shape(rows, vocab, top_k);
+        if (!logits || !tokens || !logprob || (top_k > 0 && (!top_ids || !top_logprobs))) throw Status(MOSS_HIP_EINVAL, "null pointer");
+        check_row_type(dtype);
+        if (row_stride < 0) throw Status(MOSS_HIP_EINVAL, "strides must not be negative");
+        if (!(inv_temperature > 0.0f) || !std::isfinite(inv_temperature)) throw Status(MOSS_HIP_EINVAL, "inv_temperature must be positive and finite");
+        if (rows == 0) return;
+        check_workspace(workspace, workspace_bytes, mh::logprobs_workspace(rows, vocab, top_k), "moss_hip_token_logprobs");
+        mh::LogprobArgs a;
+        a.x = logits;
+        a.dtype = dtype;
+        a.row = row_stride;
+        a.rows = rows;
+        a.vocab = vocab;
+        a.tokens = tokens;
+        a.inv_t = inv_temperature;
+        a.logprob = logprob;
+        a.entropy = entropy;
+        a.top_k = top_k;
+        a.top_ids = top_ids;
+        a.top_lp = top_logprobs;
+        a.ws = workspace;
+        mh::hip_check(mh::launch_logprobs(a, static_cast<hipStream_t>(stream)), "log probability launch");
     });
 }
 

@@ -14,7 +14,7 @@ PKG_DIR = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 LIB_PATH = os.path.join(PKG_DIR, "libmoss_hip.so")
 
 OK, EINVAL, EDEVICE, EFORMAT, EUNSUPPORTED, ESTATE = 0, 1, 2, 3, 4, 5
-F32, F16 = 0, 1
+F32, F16, I8, E4M3 = 0, 1, 2, 3
 
 # Quantiser capture (moss_hip_llm_capture): kinds and the per-step float offsets of a decode
 # capture, as include/moss_hip.h declares them (name -> (offset, length)).
@@ -39,6 +39,9 @@ EXPORTED = [
     "moss_hip_gemv_q8x4", "moss_hip_gemm_q8x4", "moss_hip_dequant_rows_q8x4", "moss_hip_attn_decode",
     "moss_hip_attn_decode_noalloc", "moss_hip_attn_paged",
     "moss_hip_quantize_rows", "moss_hip_gemm_q8x4_w8a8", "moss_hip_gemv_q8x4_w8a8",
+    "moss_hip_rope_freqs", "moss_hip_rope_rows", "moss_hip_kv_write", "moss_hip_kv_read",
+    "moss_hip_attn_tree", "moss_hip_attn_tree_workspace",
+    "moss_hip_token_logprobs", "moss_hip_token_logprobs_workspace",
     "moss_hip_codec_create", "moss_hip_codec_create_from_file", "moss_hip_codec_destroy",
     "moss_hip_codec_samples_per_frame", "moss_hip_codec_reset_stream", "moss_hip_codec_decode_chunk",
     "moss_hip_codec_decode", "moss_hip_codec_last_ms", "moss_hip_codec_stage_ms",
@@ -72,6 +75,24 @@ class SampleParams(C.Structure):
              min_frames=0, greedy_frames=0):
         return cls(int(greedy), temperature, top_k, top_p, repetition_penalty, int(end_greedy), min_frames,
                    greedy_frames)
+
+
+class RopeParams(C.Structure):
+    """moss_hip_rope_params."""
+    _fields_ = [("rot_dim", C.c_int), ("scaling", C.c_int), ("base", C.c_double), ("factor", C.c_double),
+                ("orig_ctx", C.c_int), ("beta_fast", C.c_double), ("beta_slow", C.c_double)]
+
+
+class RopeStruct(C.Structure):
+    """moss_hip_rope."""
+    _fields_ = [("freqs", C.c_void_p), ("rot_dim", C.c_int), ("halves", C.c_int), ("mscale", C.c_float)]
+
+
+class KVCacheStruct(C.Structure):
+    """moss_hip_kv_cache."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("kv_dtype", C.c_int), ("kv_heads", C.c_int), ("head_dim", C.c_int), ("page_size", C.c_int),
+                ("n_pages", C.c_int), ("page_table", C.c_void_p), ("table_stride", C.c_int), ("streams", C.c_int)]
 
 
 FRAME_CB = C.CFUNCTYPE(None, C.c_void_p, C.c_int, C.POINTER(C.c_int32))
@@ -132,6 +153,15 @@ def load(path: str = LIB_PATH) -> C.CDLL:
     L.moss_hip_attn_decode.argtypes = [vp, vp, vp, i32, i32, i32, i32, vp, i32, vp]
     L.moss_hip_attn_decode_noalloc.argtypes = [vp, vp, vp, i32, i32, i32, i32, vp, i32, vp]
     L.moss_hip_attn_paged.argtypes = [vp, vp, vp, i32, i32, vp, i32, i32, i32, vp, vp, i32, vp, i32, vp]
+    i64, f32, sz = C.c_int64, C.c_float, C.c_size_t
+    L.moss_hip_rope_freqs.argtypes = [C.POINTER(RopeParams), vp, C.POINTER(f32)]
+    L.moss_hip_rope_rows.argtypes = [vp, i64, i64, vp, i64, i64, i32, i32, i32, i32, vp, vp, vp]
+    L.moss_hip_kv_write.argtypes = [vp, vp, i64, vp, i64, i32, i32, vp, vp, vp, vp, vp]
+    L.moss_hip_kv_read.argtypes = [vp, vp, vp, i32, vp, i64, vp, i64, i32, vp]
+    L.moss_hip_attn_tree.argtypes = [vp, i64, i32, i32, vp, vp, vp, vp, i32, i32, i32, f32, vp, i64, i32, vp, vp, sz, vp]
+    L.moss_hip_attn_tree_workspace.argtypes = [vp, i32, i32, i32, i32, C.POINTER(sz)]
+    L.moss_hip_token_logprobs.argtypes = [vp, i64, i32, i32, i32, vp, f32, vp, vp, i32, vp, vp, vp, sz, vp]
+    L.moss_hip_token_logprobs_workspace.argtypes = [i32, i32, i32, C.POINTER(sz)]
     L.moss_hip_codec_create.argtypes = [vp, C.c_size_t, C.POINTER(CodecOptions), C.POINTER(vp)]
     L.moss_hip_codec_create_from_file.argtypes = [C.c_char_p, C.POINTER(CodecOptions), C.POINTER(vp)]
     L.moss_hip_codec_destroy.argtypes = [vp]
@@ -225,6 +255,237 @@ def attn_paged(q, k_pool, v_pool, heads: int, page_table, table_stride: int, pag
                                 rows, C.c_void_p(row_stream.data_ptr()) if row_stream is not None else None,
                                 C.c_void_p(row_pos.data_ptr()), max_keys, C.c_void_p(out.data_ptr()), dt[out.dtype],
                                 _stream(stream)))
+
+
+# ---------------------------------------------------------------- a caller's own decoding loop
+
+ROPE_SCALING = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3}
+
+
+def _types(t):
+    """Element type of a tensor of rows."""
+    import torch
+    d = t.dtype
+    if d == torch.float32:
+        return F32
+    if d == torch.float16:
+        return F16
+    raise TypeError(f"float32 or float16 rows are wanted, not {d}")
+
+
+def _whole(name, t, dtype, shape, device, optional=False):
+    """The address of a contiguous tensor of this type and shape on this device (None: NULL)."""
+    if t is None and optional:
+        return None
+    if t.dtype != dtype or t.device != device or tuple(t.shape) != shape or not t.is_contiguous():
+        raise ValueError(f"{name}: a contiguous {dtype} tensor of shape {shape} on {device} is wanted, "
+                         f"not {t.dtype} {tuple(t.shape)} on {t.device}")
+    return t.data_ptr()
+
+
+def _here(device):
+    """The calls launch on the current device: tensors of another one are refused."""
+    import torch
+    if device.type != "cuda":
+        raise ValueError(f"tensors on the GPU are wanted, not on {device}")
+    if device.index != torch.cuda.current_device():
+        raise ValueError(f"the tensors are on {device}, the current device is cuda:{torch.cuda.current_device()}")
+
+
+def _rows(name, t, heads, dim, device):
+    """(address, row stride) of rows [rows][heads][dim] (or [rows][heads * dim]) whose rows are contiguous."""
+    if t.device != device or t.numel() != t.shape[0] * heads * dim:
+        raise ValueError(f"{name}: [rows][{heads}][{dim}] on {device} is wanted, not {tuple(t.shape)} on {t.device}")
+    inner = t.stride()[1:] == ((dim, 1) if t.dim() == 3 else (1,))
+    if not (t.dim() in (2, 3) and (t.dim() == 2 or t.shape[1] == heads) and (inner or t.numel() == 0)):
+        raise ValueError(f"{name}: the heads of a row must be contiguous")
+    return t.data_ptr(), t.stride(0)
+
+
+def _workspace(given, size, device, stream):
+    """(address, bytes): the caller's, or a new one from torch's allocator, which is safe on the current stream."""
+    import torch
+    if size == 0:
+        return None, 0
+    if given is None:
+        if stream is not None and stream != torch.cuda.current_stream().cuda_stream:
+            raise ValueError("on a stream other than torch's current one, pass a workspace")
+        given = torch.empty(size, dtype=torch.uint8, device=device)
+    elif given.device != device or not given.is_contiguous():
+        raise ValueError(f"workspace: a contiguous tensor on {device} is wanted")
+    return given.data_ptr(), given.numel() * given.element_size()
+
+
+def rope_freqs(rot_dim: int, base: float = 10000.0, scaling: str = "none", factor: float = 1.0, orig_ctx: int = 0,
+               beta_fast: float = 0.0, beta_slow: float = 0.0):
+    """moss_hip_rope_freqs: (angles per position [rot_dim / 2] float64, the factor of sine and cosine)."""
+    p = RopeParams(rot_dim, ROPE_SCALING[scaling], base, factor, orig_ctx, beta_fast, beta_slow)
+    f, m = np.empty(max(rot_dim // 2, 1), np.float64), C.c_float(1.0)
+    check(load().moss_hip_rope_freqs(C.byref(p), _ptr(f), C.byref(m)))
+    return f, m.value
+
+
+class Rope:
+    """A rotation a program keeps: its angles per position on the device (moss_hip_rope).
+
+    Rope(rot_dim, ...) takes the arguments of rope_freqs; Rope(freqs=tensor) takes float64 angles of the
+    caller's own.  halves: pairs (i, i + rot_dim / 2) rather than (2i, 2i + 1)."""
+
+    def __init__(self, rot_dim: int = 64, halves: bool = False, freqs=None, mscale: float = 1.0, device=None, **scaling):
+        import torch
+        if freqs is None:
+            f, mscale = rope_freqs(rot_dim, **scaling)
+            freqs = torch.from_numpy(f).to("cuda" if device is None else device)
+        self.freqs, self.device = freqs, freqs.device
+        _whole("freqs", freqs, torch.float64, (freqs.numel(),), freqs.device)
+        self.struct = RopeStruct(freqs.data_ptr(), 2 * freqs.numel(), int(halves), mscale)
+        self.ref = C.addressof(self.struct)
+
+
+class KVCache:
+    """One layer's paged cache as the calls take it (moss_hip_kv_cache): pools [n_pages][kv_heads][page_size][head_dim]
+    (float32, float16, int8 or float8_e4m3fn; the 8-bit ones with float32 scales [n_pages][kv_heads][page_size])
+    and the block table [streams][pages of a stream] (int32).  Keeps the tensors, owns nothing else."""
+
+    def __init__(self, k, v, page_table, k_scale=None, v_scale=None):
+        import torch
+        kinds = {torch.float32: F32, torch.float16: F16, torch.int8: I8, torch.float8_e4m3fn: E4M3}
+        if k.dim() != 4 or k.dtype not in kinds or page_table.dim() != 2:
+            raise ValueError("pools [n_pages][kv_heads][page_size][head_dim] and a table [streams][pages] are wanted")
+        self.tensors, self.device = (k, v, page_table, k_scale, v_scale), k.device
+        n, h, size, dim = k.shape
+        self.kv_heads, self.head_dim, self.streams = h, dim, page_table.shape[0]
+        self.struct = KVCacheStruct(
+            _whole("k", k, k.dtype, (n, h, size, dim), k.device), _whole("v", v, k.dtype, (n, h, size, dim), k.device),
+            _whole("k_scale", k_scale, torch.float32, (n, h, size), k.device, optional=True),
+            _whole("v_scale", v_scale, torch.float32, (n, h, size), k.device, optional=True),
+            kinds[k.dtype], h, dim, size, n,
+            _whole("page_table", page_table, torch.int32, tuple(page_table.shape), k.device), page_table.shape[1],
+            page_table.shape[0])
+        self.ref = C.addressof(self.struct)
+
+
+def rope_rows(x, pos, rope: Rope, out=None, stream=None):
+    """moss_hip_rope_rows on x [rows][heads][head_dim] (any row and head strides) at positions pos [rows] int32, into
+    out (x itself by default); returns out."""
+    import torch
+    out = x if out is None else out
+    dev = x.device
+    _here(dev)
+    if x.dim() != 3 or out.shape != x.shape or out.dtype != x.dtype or out.device != dev or rope.device != dev:
+        raise ValueError("x and out must be [rows][heads][head_dim] of one type, on one device with the rotation")
+    if x.numel() == 0:
+        return out
+    if x.stride(2) != 1 or out.stride(2) != 1:
+        raise ValueError("the elements of a head must be contiguous")
+    rows, heads, dim = x.shape
+    check(load().moss_hip_rope_rows(x.data_ptr(), x.stride(0), x.stride(1), out.data_ptr(), out.stride(0), out.stride(1),
+                                    _types(x), rows, heads, dim, _whole("pos", pos, torch.int32, (rows,), dev), rope.ref,
+                                    _stream(stream)))
+    return out
+
+
+def kv_write(cache: KVCache, k, v, row_stream, row_pos, rope: Rope | None = None, rope_pos=None, stream=None) -> None:
+    """moss_hip_kv_write: rows k, v [rows][kv_heads][head_dim] to position row_pos[r] of stream row_stream[r], keys turned
+    by `rope` at rope_pos (row_pos by default)."""
+    import torch
+    dev, n = cache.device, k.shape[0]
+    _here(dev)
+    if v.shape[0] != n or v.dtype != k.dtype or (rope is not None and rope.device != dev):
+        raise ValueError("k and v must have the same rows and type, and the rotation their device")
+    if n == 0:
+        return
+    kp, ks = _rows("k", k, cache.kv_heads, cache.head_dim, dev)
+    vp, vs = _rows("v", v, cache.kv_heads, cache.head_dim, dev)
+    check(load().moss_hip_kv_write(cache.ref, kp, ks, vp, vs, _types(k), n,
+                                   _whole("row_stream", row_stream, torch.int32, (n,), dev),
+                                   _whole("row_pos", row_pos, torch.int32, (n,), dev),
+                                   None if rope is None else rope.ref,
+                                   _whole("rope_pos", rope_pos, torch.int32, (n,), dev, optional=True), _stream(stream)))
+
+
+def kv_read(cache: KVCache, row_stream, row_pos, k, v, stream=None) -> None:
+    """moss_hip_kv_read: those rows back, into k, v [rows][kv_heads][head_dim]."""
+    import torch
+    dev, n = cache.device, k.shape[0]
+    _here(dev)
+    if v.shape[0] != n or v.dtype != k.dtype:
+        raise ValueError("k and v must have the same rows and type")
+    if n == 0:
+        return
+    kp, ks = _rows("k", k, cache.kv_heads, cache.head_dim, dev)
+    vp, vs = _rows("v", v, cache.kv_heads, cache.head_dim, dev)
+    check(load().moss_hip_kv_read(cache.ref, _whole("row_stream", row_stream, torch.int32, (n,), dev),
+                                  _whole("row_pos", row_pos, torch.int32, (n,), dev), n, kp, ks, vp, vs, _types(k),
+                                  _stream(stream)))
+
+
+def attn_tree_workspace(cache: KVCache, heads: int, rows: int, max_rows: int, max_keys: int) -> int:
+    """Bytes of workspace attn_tree takes for `rows` rows in all, max_rows of one stream, max_keys keys."""
+    n = C.c_size_t(0)
+    check(load().moss_hip_attn_tree_workspace(cache.ref, heads, rows, max_rows, max_keys, C.byref(n)))
+    return n.value
+
+
+def attn_tree(q, cache: KVCache, row_start, ctx_len, out, max_rows: int, max_keys: int, row_mask=None, scale: float | None = None,
+              lse=None, workspace=None, stream=None) -> None:
+    """moss_hip_attn_tree: q [rows][heads][head_dim] against the cache, into out (float32 or float16).
+
+    row_start [streams + 1] and ctx_len [streams] int32; row_mask [rows] int64 (bit j: drafted row j of the
+    stream), None: a chain; scale: head_dim ** -0.5 by default; lse [rows][heads] float32 or None."""
+    import torch
+    dev, dim = cache.device, cache.head_dim
+    _here(dev)
+    rows = q.shape[0]
+    heads = q.shape[1] if q.dim() == 3 else q.shape[1] // dim
+    if out.shape[0] != rows:
+        raise ValueError("q and out must have the same rows")
+    if rows == 0:
+        return
+    qp, qs = _rows("q", q, heads, dim, dev)
+    op, os_ = _rows("out", out, heads, dim, dev)
+    wp, wb = _workspace(workspace, attn_tree_workspace(cache, heads, rows, max_rows, max_keys), dev, stream)
+    check(load().moss_hip_attn_tree(qp, qs, _types(q), heads, cache.ref,
+                                    _whole("row_start", row_start, torch.int32, (cache.streams + 1,), dev),
+                                    _whole("ctx_len", ctx_len, torch.int32, (cache.streams,), dev),
+                                    _whole("row_mask", row_mask, torch.int64, (rows,), dev, optional=True), rows, max_rows,
+                                    max_keys, dim ** -0.5 if scale is None else scale, op, os_, _types(out),
+                                    _whole("lse", lse, torch.float32, (rows, heads), dev, optional=True), wp, wb,
+                                    _stream(stream)))
+
+
+def token_logprobs_workspace(rows: int, vocab: int, top_k: int) -> int:
+    """Bytes of workspace token_logprobs takes."""
+    n = C.c_size_t(0)
+    check(load().moss_hip_token_logprobs_workspace(rows, vocab, top_k, C.byref(n)))
+    return n.value
+
+
+def token_logprobs(logits, tokens, logprob, entropy=None, top_ids=None, top_logprobs=None, inv_temperature: float = 1.0,
+                   workspace=None, stream=None) -> None:
+    """moss_hip_token_logprobs: of tokens [rows] int32 under logits [rows][vocab] (float32 or float16, any row stride), into
+    logprob and entropy [rows] and the alternatives top_ids (int32), top_logprobs [rows][top_k]."""
+    import torch
+    dev = logits.device
+    _here(dev)
+    if logits.dim() != 2:
+        raise ValueError("logits [rows][vocab] are wanted")
+    rows, vocab = logits.shape
+    k = 0 if top_ids is None else top_ids.shape[1]
+    if (top_ids is None) != (top_logprobs is None):
+        raise ValueError("top_ids and top_logprobs come together")
+    if rows == 0:
+        return
+    if vocab > 1 and logits.stride(1) != 1:
+        raise ValueError("the logits of a row must be contiguous")
+    wp, wb = _workspace(workspace, token_logprobs_workspace(rows, vocab, k), dev, stream)
+    check(load().moss_hip_token_logprobs(logits.data_ptr(), logits.stride(0), _types(logits), rows, vocab,
+                                         _whole("tokens", tokens, torch.int32, (rows,), dev), inv_temperature,
+                                         _whole("logprob", logprob, torch.float32, (rows,), dev),
+                                         _whole("entropy", entropy, torch.float32, (rows,), dev, optional=True), k,
+                                         _whole("top_ids", top_ids, torch.int32, (rows, k), dev, optional=True),
+                                         _whole("top_logprobs", top_logprobs, torch.float32, (rows, k), dev, optional=True),
+                                         wp, wb, _stream(stream)))
 
 
 # ---------------------------------------------------------------- model

@@ -260,7 +260,12 @@ int moss_hip_batch_capture_read(moss_hip_batch *b, void *out, size_t bytes, size
 
 /* ------------------------------------------------------------------ operator layer */
 
-enum { MOSS_HIP_F32 = 0, MOSS_HIP_F16 = 1 };
+enum {
+    MOSS_HIP_F32 = 0,
+    MOSS_HIP_F16 = 1,
+    MOSS_HIP_I8 = 2,  /* cache elements only (moss_hip_kv_cache): int8 times a scale */
+    MOSS_HIP_E4M3 = 3 /* cache elements only: 8-bit floats of 4 exponent and 3 mantissa bits (largest 448), times a scale */
+};
 
 /* y[rows] = W[rows][cols] x over Q8_0_4X4 weights -- gemv_par (csrc/include/moss/gemv.h:48,
  * csrc/src/gemv.cpp:245-274) with MOSS_A16 on (row kernel csrc/src/gemv_avx2.cpp:123-150).
@@ -335,6 +340,125 @@ int moss_hip_attn_paged(const float *q, const void *k_pool, const void *v_pool, 
  * replays) race: serialise them. */
 int moss_hip_attn_decode_noalloc(const float *q, const void *k_cache, const void *v_cache, int kv_dtype, int heads,
                                  int ctx_stride, int n_keys, void *out, int out_dtype, void *stream);
+
+/* ---- Operators of a caller's own decoding loop -----------------------------------------
+ * Rotary positions, a paged K/V cache that may hold 8-bit values, attention of one or more drafted
+ * rows per stream over it, and the log probabilities that accept or reject what was drafted.  One
+ * step of such a loop: rotate the queries (moss_hip_rope_rows), write the rows' keys and values
+ * (moss_hip_kv_write, which rotates the keys on the way), attend (moss_hip_attn_tree), score the
+ * drafted tokens under the logits (moss_hip_token_logprobs); then write the accepted rows once
+ * more at their final positions.  The reference has none of these as calls of their own: its
+ * rotation and cache write are part of its QKV step (csrc/src/llm.cpp:173-228), its cache is fp32
+ * and its decode takes one row at a time.
+ *
+ * The calls allocate nothing, wait for nothing and keep nothing: they launch one or two kernels on
+ * `stream` and may be captured.  Every pointer inside the structs but the structs' own is a device
+ * pointer of the device that is current at the call, and `stream` is a stream of that device.
+ * Arrays read while a call's kernels run must not be changed meanwhile by work on other streams.  A
+ * workspace belongs to one call at a time: calls (and replays of captured calls) that may overlap
+ * need workspaces of their own.  Where rows, streams or top_k are 0 there is nothing to do and the
+ * call returns OK.  What only the device can see (positions, page indices, row ranges) is checked
+ * there and never followed out of range; each call says what becomes of such rows. */
+
+enum {
+    MOSS_HIP_ROPE_PLAIN = 0,  /* w_i = base^(-2i / rot_dim) */
+    MOSS_HIP_ROPE_LINEAR = 1, /* w_i / factor */
+    MOSS_HIP_ROPE_NTK = 2,    /* base * factor^(rot_dim / (rot_dim - 2)) in place of base (rot_dim >= 4) */
+    MOSS_HIP_ROPE_YARN = 3    /* g w_i + (1 - g) w_i / factor, with g = (turns - beta_slow) / (beta_fast - beta_slow) within
+                                 [0, 1] and turns = orig_ctx w_i / 2pi; mscale = 0.1 ln(factor) + 1 */
+};
+typedef struct {
+    int rot_dim;  /* leading elements of a head that are rotated: even, 2 .. 512 */
+    int scaling;  /* MOSS_HIP_ROPE_* */
+    double base;  /* 0 = 10000 (the model's) */
+    double factor; /* >= 1: how much longer contexts get (not PLAIN) */
+    int orig_ctx; /* YARN: the context the frequencies were trained on */
+    double beta_fast, beta_slow; /* YARN: 0, 0 = 32, 1 */
+} moss_hip_rope_params;
+/* The rot_dim / 2 angles per position (radians) and the factor of sine and cosine that `p` describes,
+ * into host memory.  The caller keeps them on the device for moss_hip_rope; any other angles may be
+ * put there as well (negated ones undo a rotation, which is also its gradient). */
+int moss_hip_rope_freqs(const moss_hip_rope_params *p, double *freqs, float *mscale);
+
+typedef struct {
+    const double *freqs; /* device: rot_dim / 2 angles per position */
+    int rot_dim;         /* even, 2 .. 512 */
+    int halves;          /* 0 = pairs (2i, 2i + 1), the model's; 1 = pairs (i, i + rot_dim / 2) */
+    float mscale;        /* multiplies sine and cosine */
+} moss_hip_rope;
+
+/* y = x with the pairs of every head turned by pos[row] * freqs[i]; elements from rot_dim on are
+ * copied.  x, y: dtype (F32 or F16), element (row, head, e) at row * row_stride + head * head_stride + e
+ * (strides in elements, >= 0); y may be x with the same strides, and must not overlap it otherwise.
+ * Angles are formed in 64 bits: positions may be any int32.  head_dim >= rot_dim. */
+int moss_hip_rope_rows(const void *x, int64_t x_row_stride, int64_t x_head_stride, void *y, int64_t y_row_stride,
+                       int64_t y_head_stride, int dtype, int rows, int heads, int head_dim, const int32_t *pos,
+                       const moss_hip_rope *rope, void *stream);
+
+/* A paged cache of one layer.  Position p of stream s is slot p % page_size of page
+ * page_table[s * table_stride + p / page_size].  F32 and F16 pools are those of moss_hip_attn_paged;
+ * I8 and E4M3 pools have a scale per (page, head, slot): the value is the element times it. */
+typedef struct {
+    void *k, *v;              /* pools [n_pages][kv_heads][page_size][head_dim], 16-byte aligned */
+    float *k_scale, *v_scale; /* [n_pages][kv_heads][page_size], 16-byte aligned; NULL for F32 and F16 */
+    int kv_dtype;             /* MOSS_HIP_F32 / F16 / I8 / E4M3 */
+    int kv_heads, head_dim;   /* head_dim 64 or 128 */
+    int page_size;            /* a multiple of 16, at most 32768 */
+    int n_pages;
+    const int32_t *page_table; /* [streams][table_stride] */
+    int table_stride, streams;
+} moss_hip_kv_cache;
+
+/* Rows of keys and values into the cache: row r to position row_pos[r] of stream row_stream[r].  k, v:
+ * [rows][kv_heads][head_dim] of dtype (F32 or F16), row strides in elements.  With `rope`, keys are
+ * turned first, by rope_pos[r] or, when rope_pos is NULL, row_pos[r] (a drafted node's slot is not
+ * its depth).  8-bit caches: t = max|x| over the head, d = t / 127 or t / 448, the element is x * (1 / d)
+ * rounded to nearest even (of the turned key in 32 bits); d under 2^-126 is stored as 0, and a head
+ * with an Inf or NaN gets the scale NaN, so that it reads back as NaN.  A row whose position is
+ * negative or past the table, whose stream is outside [0, streams) or whose page is outside
+ * [0, n_pages) is not written.  No two rows of one call may name the same place. */
+int moss_hip_kv_write(const moss_hip_kv_cache *cache, const void *k, int64_t k_stride, const void *v, int64_t v_stride,
+                      int dtype, int rows, const int32_t *row_stream, const int32_t *row_pos, const moss_hip_rope *rope,
+                      const int32_t *rope_pos, void *stream);
+
+/* The same rows back out of the cache, in 32 bits and rounded once to dtype.  A row of negative
+ * position is left as it was; one that has no place in the cache otherwise is NaN. */
+int moss_hip_kv_read(const moss_hip_kv_cache *cache, const int32_t *row_stream, const int32_t *row_pos, int rows, void *k,
+                     int64_t k_stride, void *v, int64_t v_stride, int dtype, void *stream);
+
+/* Attention of a few rows per stream over the cache.  Stream s has rows row_start[s] .. row_start[s + 1] - 1
+ * (n of them, at most max_rows <= 64), ctx_len[s] committed positions, all of which every row attends, and its
+ * rows' own drafted keys at positions ctx_len[s] + j, j < n, of which row i attends those whose bit j is set in
+ * row_mask[row] (its ancestors and itself), or j <= i where row_mask is NULL (a chain; one row: a plain
+ * decode step).  Scores are scale * q . k; query head i reads key head i / (heads / kv_heads).
+ *   q: [rows][heads][head_dim] of q_dtype (F32 or F16), rotated; out the same shape in out_dtype; row
+ *   strides in elements.  lse [rows][heads] fp32 or NULL: the log of each row's sum of exp(score).
+ * A row that attends nothing is 0 with lse -inf.  What a row does not attend may hold anything, Inf and NaN
+ * too.  max_keys bounds every stream's ctx_len + n and sizes the launch.  A stream whose ctx_len is
+ * negative, whose keys pass max_keys or its table, or with a page outside [0, n_pages) among them, gets
+ * NaN rows; one whose row range is not within [0, rows] gets none, and rows of no stream stay as they were.
+ * The same call gives the same bits.  workspace: moss_hip_attn_tree_workspace bytes (any content, 16-byte
+ * aligned; NULL where that is 0). */
+int moss_hip_attn_tree(const void *q, int64_t q_stride, int q_dtype, int heads, const moss_hip_kv_cache *cache,
+                       const int32_t *row_start, const int32_t *ctx_len, const uint64_t *row_mask, int rows, int max_rows,
+                       int max_keys, float scale, void *out, int64_t out_stride, int out_dtype, float *lse, void *workspace,
+                       size_t workspace_bytes, void *stream);
+/* Bytes of workspace such a call takes (of the cache it reads kv_dtype, kv_heads, head_dim, page_size and
+ * streams). */
+int moss_hip_attn_tree_workspace(const moss_hip_kv_cache *cache, int heads, int rows, int max_rows, int max_keys, size_t *bytes);
+
+/* For rows of logits x [rows][vocab] (dtype F32 or F16, row stride in elements) and z = x * inv_temperature:
+ *   logprob[r] = log softmax(z)[tokens[r]]; NaN for a token outside [0, vocab).
+ *   entropy[r] = -sum p log p, or NULL.
+ *   top_ids / top_logprobs [rows][top_k]: the top_k <= 32 largest, of equal logits the lowest index first;
+ *   -1 / -inf where a row has no more.
+ * -inf logits are ruled out: probability 0, and no alternatives.  A row of nothing else has logprob -inf
+ * and entropy 0.  A NaN or +inf logit makes the row's log probabilities and entropy NaN (NaN logits are no
+ * alternatives).  vocab <= 2^20.  workspace as above: moss_hip_token_logprobs_workspace bytes. */
+int moss_hip_token_logprobs(const void *logits, int64_t row_stride, int dtype, int rows, int vocab, const int32_t *tokens,
+                            float inv_temperature, float *logprob, float *entropy, int top_k, int32_t *top_ids,
+                            float *top_logprobs, void *workspace, size_t workspace_bytes, void *stream);
+int moss_hip_token_logprobs_workspace(int rows, int vocab, int top_k, size_t *bytes);
 
 /* ---- Audio codec decoder (codes -> 48 kHz stereo PCM) --------------------------------
  * The GPU replacement of moss::AudioDecoder (reference csrc/include/moss/decoder.h:14-83,
