@@ -38,11 +38,13 @@ typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 constexpr int kWaves = 4, kThreads = 64 * kWaves;
 constexpr int kMaxSplits = 64;
 constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.69314718055994531f;
-constexpr int kWeightExp = 13;  // weights are scaled to at most 2^14
+constexpr float kSlack = 8.0f;  // log 2 of how far a weight may pass 1
+constexpr int kWeightExp = 6;   // and of what it is scaled by
 
 struct TreePlan {
-    int tiles, row_groups, splits, chunk;  // row tiles of 16, groups of MT of them, key splits of `chunk` keys
-    uint64_t page_magic;                   // block of 16 keys / blocks of a page, as a product
+    int tiles, group, row_groups;  // row tiles of 16, of which a workgroup takes `group`
+    int splits, chunk;             // key splits of `chunk` keys
+    uint64_t page_magic;           // block of 16 keys / blocks of a page, as a product
 };
 
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -76,14 +78,57 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t &hi, uint32_t 
     lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a - (float)h[0], b - (float)h[1]));
 }
 
-// 16 keys x D of one head as a lane's share of 32 keys: K as the A operand of S^T, V as that of O^T.
+// A lane's share of 32 keys x D of one head, as they lie in memory: of K the A operand of S^T (key
+// l % 16 of each block of 16), of V the lane's dims of keys 4g .. 4g + 3 of each block.
 template <int KV, int D>
 struct Keys {
     static constexpr int NW = D * elem_size(KV) / 64;
     uint4 k[2][NW];
-    uint32_t v[8][NW];
+    uint32_t v[2][4][NW];
     float4 ks[2], vs[2];
 };
+
+// Where a block of 16 keys lies: the index of its first vector, and its last key that is read.
+struct Block {
+    size_t vec;
+    int lim;
+};
+
+// The block of keys kb .. kb + 15 of a stream whose last key to read is `last`; a page outside the pools
+// sets `bad` (and page 0 is read in its place).
+__device__ __forceinline__ Block block_of(const TreeArgs &a, const TreePlan &plan, const int *table, int h, int kb, int last,
+                                          bool &bad) {
+    kb = min(kb, last & ~15);
+    const uint32_t blk = (uint32_t)kb >> 4, pg = (uint32_t)((blk * plan.page_magic) >> 40);
+    int page = __builtin_amdgcn_readfirstlane(table[pg]);
+    if (page < 0 || page >= a.c.n_pages) {
+        page = 0;
+        bad = true;
+    }
+    Block b;
+    b.vec = ((size_t)page * a.c.heads + h) * a.c.page_size + (blk - pg * (a.c.page_size >> 4)) * 16;
+    b.lim = min(15, last - kb);
+    return b;
+}
+
+// Loads of one block: K as NW 16-byte pieces of a key, V as NW words of each of 4 keys.
+template <int KV, int D>
+__device__ __forceinline__ void load_k(const TreeArgs &a, const Block &b, int c, int g, uint4 (&k)[Keys<KV, D>::NW]) {
+    const char *p = (const char *)a.c.k + b.vec * (D * elem_size(KV));
+    const int off = min(c, b.lim) * (D * elem_size(KV)) + 16 * g;
+#pragma unroll
+    for (int u = 0; u < Keys<KV, D>::NW; ++u) k[u] = *(const uint4 *)(p + off + 64 * u);
+}
+template <int KV, int D>
+__device__ __forceinline__ void load_v(const TreeArgs &a, const Block &b, int c, int g, uint32_t (&v)[4][Keys<KV, D>::NW]) {
+    constexpr int NW = Keys<KV, D>::NW;
+    const char *p = (const char *)a.c.v + b.vec * (D * elem_size(KV));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int off = min(4 * g + i, b.lim) * (D * elem_size(KV)) + c * (NW * 4);
+        __builtin_memcpy(v[i], __builtin_assume_aligned(p + off, NW < 4 ? NW * 4 : 16), NW * 4);
+    }
+}
 
 // The 8 dims of K fragment s (f16 products) start at this one, for lane group g.
 template <int KV>
@@ -108,30 +153,31 @@ __device__ __forceinline__ Frag k_frag(const uint4 (&k)[Keys<KV, D>::NW], int s)
     return f;
 }
 
-// V fragments of dims 4n .. 4n + 3 (8 bit) or 2n, 2n + 1 (fp16) of the lane's D / 16.
+// The half of V's fragments that one block of 16 keys gives: words w[0], w[1] of the fragments of dims
+// 4n .. 4n + 3 (8 bit) or 2n, 2n + 1 (fp16) of the lane's D / 16.
 template <int KV>
 constexpr int dims_per_word() {
     return KV == ELEM_F16 ? 2 : 4;
 }
 template <int KV, int NW>
-__device__ __forceinline__ void v_frags(const uint32_t (&v)[8][NW], int n, Frag (&f)[dims_per_word<KV>()]) {
+__device__ __forceinline__ void v_halves(const uint32_t (&v)[4][NW], int n, uint32_t (&f)[dims_per_word<KV>()][2]) {
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
+    for (int q = 0; q < 2; ++q) {
         const uint32_t a = v[2 * q][n], b = v[2 * q + 1][n];
         if constexpr (KV == ELEM_F16) {
-            f[0].w[q] = perm(b, a, 0x05040100u);
-            f[1].w[q] = perm(b, a, 0x07060302u);
+            f[0][q] = perm(b, a, 0x05040100u);
+            f[1][q] = perm(b, a, 0x07060302u);
         } else {
             const uint32_t x = KV == ELEM_I8 ? 0x80808080u : 0u;
             const uint32_t t01 = perm(b ^ x, a ^ x, 0x05010400u), t23 = perm(b ^ x, a ^ x, 0x07030602u);
             if constexpr (KV == ELEM_I8) {
-                f[0].w[q] = bias_off(perm(0x64646464u, t01, 0x04010400u));
-                f[1].w[q] = bias_off(perm(0x64646464u, t01, 0x04030402u));
-                f[2].w[q] = bias_off(perm(0x64646464u, t23, 0x04010400u));
-                f[3].w[q] = bias_off(perm(0x64646464u, t23, 0x04030402u));
+                f[0][q] = bias_off(perm(0x64646464u, t01, 0x04010400u));
+                f[1][q] = bias_off(perm(0x64646464u, t01, 0x04030402u));
+                f[2][q] = bias_off(perm(0x64646464u, t23, 0x04010400u));
+                f[3][q] = bias_off(perm(0x64646464u, t23, 0x04030402u));
             } else {
-                f[0].w[q] = e4m3_pair(t01, false), f[1].w[q] = e4m3_pair(t01, true);
-                f[2].w[q] = e4m3_pair(t23, false), f[3].w[q] = e4m3_pair(t23, true);
+                f[0][q] = e4m3_pair(t01, false), f[1][q] = e4m3_pair(t01, true);
+                f[2][q] = e4m3_pair(t23, false), f[3][q] = e4m3_pair(t23, true);
             }
         }
     }
@@ -159,10 +205,6 @@ __device__ __forceinline__ uint32_t finite_part(uint32_t w) {
     return w;
 }
 
-__device__ __forceinline__ float load_q(const TreeArgs &a, size_t i) {
-    return a.q_dtype == ELEM_F16 ? __half2float(((const __half *)a.q)[i]) : ((const float *)a.q)[i];
-}
-
 // A stream's rows and keys; n = 0 where there is nothing to do.
 struct Stream {
     int row0, n, ctx, total;
@@ -180,13 +222,280 @@ __device__ __forceinline__ Stream stream_of(const TreeArgs &a, int s) {
     return t;
 }
 
-// HB: spans of HB * 32 keys; MT row tiles; LO: 32-bit queries, as hi + lo.
-template <int KV, int D, int MT, int HB, bool LO>
-__global__ __launch_bounds__(kThreads) void attn_tree_kernel(TreeArgs a, TreePlan plan) {
+// N values of a query in 32 bits, at element i.
+template <int N>
+__device__ __forceinline__ void load_q(const TreeArgs &a, bool f32, size_t i, float (&x)[N]) {
+    if (f32) {
+        const float *p = (const float *)a.q + i;
+        if (a.q_vec) {
+#pragma unroll
+            for (int e = 0; e < N; e += 4) *(float4 *)&x[e] = *(const float4 *)(p + e);
+        } else {
+#pragma unroll
+            for (int e = 0; e < N; ++e) x[e] = p[e];
+        }
+    } else {
+        const __half *p = (const __half *)a.q + i;
+        if (a.q_vec) {
+            __half h[N];
+            __builtin_memcpy(h, __builtin_assume_aligned(p, N >= 8 ? 16 : 2 * N), 2 * N);
+#pragma unroll
+            for (int e = 0; e < N; ++e) x[e] = __half2float(h[e]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < N; ++e) x[e] = __half2float(p[e]);
+        }
+    }
+}
+
+// One packed query of a lane's row: fp16 fragments (hi, and lo of a 32-bit query) or 32-bit values.  Its
+// scores in units of log 2 are qs times the products; qs > 0 (the sign of the scale goes into the query, and
+// a scale of 0 is one so small that it makes no score differ from 0).
+template <int KV, int D, bool LO>
+struct Query {
+    static constexpr bool F32 = KV == ELEM_F32;
+    Frag hi[F32 ? 1 : D / 32], lo[F32 || !LO ? 1 : D / 32];
+    float f[F32 ? D / 4 : 1];
+    float qs;
+    uint64_t mask;
+
+    __device__ __forceinline__ void load(const TreeArgs &a, const Stream &st, int grp, int h, int i, int packed, int g) {
+        const bool ok = i < packed;
+        const int node = ok ? i / grp : 0, row = st.row0 + node, head = h * grp + (ok ? i - node * grp : 0);
+        const size_t base = (size_t)((int64_t)row * a.q_row + head * D);
+        mask = !ok ? 0 : (a.row_mask != nullptr ? a.row_mask[row] : (2ull << node) - 1);
+        if (st.n < 64) mask &= (1ull << st.n) - 1;
+        const bool minus = a.scale < 0.0f;
+        qs = fmaxf(fabsf(a.scale) * kLog2e, 1.17549435e-38f);
+        if constexpr (F32) {
+#pragma unroll
+            for (int u = 0; u < D / 16; ++u) {
+                float x[4];
+                load_q<4>(a, a.q_dtype == ELEM_F32, base + 16 * u + 4 * g, x);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) f[4 * u + e] = !ok ? 0.0f : (minus ? -x[e] : x[e]);
+            }
+        } else {
+            float x[D / 32][8];
+#pragma unroll
+            for (int k = 0; k < D / 32; ++k) {
+                load_q<8>(a, LO, base + frag_dim<KV>(k, g), x[k]);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[k][e] = !ok ? 0.0f : (minus ? -x[k][e] : x[k][e]);
+            }
+            if constexpr (LO) {
+                uint32_t top = 0;
+#pragma unroll
+                for (int k = 0; k < D / 32; ++k)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(x[k][e]) & 0x7fffffffu);
+                top = max(top, (uint32_t)xshfl<16>((int)top));
+                top = max(top, (uint32_t)xshfl<32>((int)top));
+                const int e2 = (int)(top >> 23) - 127;  // a power of two: exact (an Inf or NaN stays one)
+                qs = fmaxf(__builtin_amdgcn_ldexpf(qs, e2), 1.17549435e-38f);
+#pragma unroll
+                for (int k = 0; k < D / 32; ++k)
+#pragma unroll
+                    for (int e = 0; e < 8; e += 2)
+                        split2(__builtin_amdgcn_ldexpf(x[k][e], -e2), __builtin_amdgcn_ldexpf(x[k][e + 1], -e2), hi[k].w[e / 2],
+                               lo[k].w[e / 2]);
+            } else {
+#pragma unroll
+                for (int k = 0; k < D / 32; ++k)
+#pragma unroll
+                    for (int e = 0; e < 8; e += 2)
+                        hi[k].w[e / 2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x[k][e], x[k][e + 1]));
+            }
+        }
+    }
+};
+
+// The drafted positions that any row of a wave's tiles sees.
+template <class Q, int MT>
+__device__ __forceinline__ uint64_t seen_by(const Q (&q)[MT]) {
+    uint64_t seen = 0;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) seen |= q[mt].mask;
+    uint32_t lo = (uint32_t)seen, hi = (uint32_t)(seen >> 32);
+    lo |= xshfl<1>((int)lo), hi |= xshfl<1>((int)hi);
+    lo |= xshfl<2>((int)lo), hi |= xshfl<2>((int)hi);
+    lo |= xshfl<4>((int)lo), hi |= xshfl<4>((int)hi);
+    lo |= xshfl<8>((int)lo), hi |= xshfl<8>((int)hi);
+    return ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane(hi) << 32) | (uint32_t)__builtin_amdgcn_readfirstlane(lo);
+}
+
+// Whether a row whose mask is `bits` sees key `pos` (of a stream's ctx + n).
+__device__ __forceinline__ bool visible(const Stream &st, uint64_t bits, int pos) {
+    const int j = pos - st.ctx;
+    return j < 0 || (j < st.n && ((bits >> (j & 63)) & 1));
+}
+
+// Softmax state of a lane's rows, one per tile: o = sum 2^(x - m) v, l = sum 2^(x - m) over the scores x so
+// far, l of this lane's keys only.  m is `ref` less `up`, whole numbers both, so scaling by their changes is
+// exact.  ref is at most kSlack under the largest score so far: it moves (and o and l are scaled) only when a
+// score passes it by more, which after the first spans is rare, where the largest itself still moves in every
+// other span for some row of a tile.  2^up makes the weights use fp16's range: with value scales below 2^(e + 1) a
+// weight times its scale stays under 2^15.5 at up = kWeightExp - e (at most 90), slack and all.
+template <int MT, int ND>
+struct Rows {
+    float ref[MT], l[MT];
+    floatx4 o[MT][ND];
+    float up;
+
+    __device__ __forceinline__ void clear(bool scaled) {
+        up = scaled ? 90.0f : (float)kWeightExp;
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+            ref[mt] = -INFINITY;
+            l[mt] = 0.0f;
+#pragma unroll
+            for (int j = 0; j < ND; ++j) o[mt][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+        }
+    }
+    __device__ __forceinline__ float m(int mt) const { return ref[mt] - up; }
+    // A new up for all rows, before their next scores.
+    __device__ __forceinline__ void raise(float up_new) {
+        const float f = exp2_((up_new - up) * 0.5f);  // twice: the whole of it can be below what fp32 holds
+        up = up_new;
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+            l[mt] = l[mt] * f * f;
+#pragma unroll
+            for (int j = 0; j < ND; ++j) o[mt][j] = o[mt][j] * f * f;
+        }
+    }
+    // Products x (times key scales) of 32 keys, -inf where the row does not see the key, become weights.
+    __device__ __forceinline__ void weigh(int mt, float qs, float (&x)[2][4]) {
+        float mx = fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])), fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3])));
+        mx = fmaxf(mx, xshfl<16>(mx));
+        mx = fmaxf(mx, xshfl<32>(mx)) * qs;
+        if (__any(mx > ref[mt] + kSlack)) {
+            const float r = mx > ref[mt] + kSlack ? rintf(mx) : ref[mt];  // (a row's own business, whatever its tile does)
+            const float fade = r == -INFINITY ? 1.0f : exp2_(ref[mt] - r);
+            ref[mt] = r;
+            l[mt] *= fade;
+#pragma unroll
+            for (int j = 0; j < ND; ++j) o[mt][j] *= fade;
+        }
+        const float m0 = ref[mt] == -INFINITY ? 0.0f : ref[mt] - up;
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                x[b][i] = exp2_(fmaf(x[b][i], qs, -m0));
+                l[mt] += x[b][i];
+            }
+    }
+};
+
+// `up` for value scales of which the largest has these bits.
+__device__ __forceinline__ float up_of(uint32_t top) { return fminf((float)(kWeightExp + 127 - (int)(top >> 23)), 90.0f); }
+
+// x of the keys that a row does not see becomes `v` (32 keys at p0).
+template <class Q, int MT>
+__device__ __forceinline__ void hide(const Stream &st, const Q (&q)[MT], int p0, int g, float v, float (&x)[MT][2][4]) {
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (!visible(st, q[mt].mask, p0 + 16 * b + 4 * g + i)) x[mt][b][i] = v;
+}
+// Weights times value scales; 0 for what a row does not see, whatever its scale holds.
+template <class Q, int MT>
+__device__ __forceinline__ void scale_weights(const Stream &st, const Q (&q)[MT], bool tail, int p0, int g, const float4 (&vs)[2],
+                                              float (&x)[MT][2][4]) {
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+        const float v[4] = {vs[b].x, vs[b].y, vs[b].z, vs[b].w};
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[mt][b][i] *= v[i];
+    }
+    if (tail) hide(st, q, p0, g, 0.0f, x);
+}
+
+// The Inf and NaN elements of V among 32 keys, added key by key to the rows that see them (x: weights,
+// `room` the wave's [16][ >= 32] floats of LDS).
+template <int KV, int D, int MT, class Room>
+__device__ __forceinline__ void add_odd_values(const TreeArgs &a, const Stream &st, const Block (&blk)[2], int p0, int mt,
+                                               uint64_t mask, const float (&x)[2][4], Room &room, Rows<MT, D / 16> &rows) {
+    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) room[c][16 * b + 4 * g + i] = x[b][i];
+    __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+    for (int kk = 0; kk < 32; ++kk) {
+        const int b = kk >> 4;
+        const size_t at = ((b ? blk[1].vec : blk[0].vec) + min(kk & 15, b ? blk[1].lim : blk[0].lim)) * D + (D / 4) * g;
+        const float wt = room[c][kk];
+        const bool see = visible(st, mask, p0 + kk);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int j = 0; j < D / 16; ++j) {
+                const float v = v_value<KV>(a.c.v, at + (D / 16) * r + j);
+                rows.o[mt][j][r] += see && !(fabsf(v) < INFINITY) ? wt * v : 0.0f;
+            }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+// N elements from d0 on of packed row i, normalised, or, where the keys are split, as they are with the
+// row's maximum and sum (a lane of d0 = 0 writes those).
+template <int D, int N>
+__device__ __forceinline__ void put_row(const TreeArgs &a, const TreePlan &plan, const Stream &st, int z, int grp, int h, int i, int d0,
+                                        float M, float L, const float (&x)[N]) {
+    const int node = i / grp, head = h * grp + i - node * grp;
+    const size_t at = (size_t)(st.row0 + node) * a.heads + head;
+    if (plan.splits > 1) {
+        const size_t all_rows = (size_t)a.rows * a.heads;
+        if (d0 == 0) ((float2 *)a.ws)[(size_t)z * all_rows + at] = make_float2(M, L);
+        if (L == 0.0f) return;
+        float *po = (float *)a.ws + (size_t)plan.splits * all_rows * 2 + ((size_t)z * all_rows + at) * D + d0;
+#pragma unroll
+        for (int j = 0; j < N; j += 4) *(float4 *)(po + j) = make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
+        return;
+    }
+    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+    const size_t o = (size_t)((int64_t)(st.row0 + node) * a.out_row + head * D + d0);
+    if (a.out_dtype == ELEM_F16) {
+        __half *p = (__half *)a.out + o;
+        __half y[N];
+#pragma unroll
+        for (int j = 0; j < N; ++j) y[j] = __float2half_rn(x[j] * inv);
+        if (a.out_vec) {
+            __builtin_memcpy(__builtin_assume_aligned(p, N < 8 ? 2 * N : 16), y, 2 * N);
+        } else {
+#pragma unroll
+            for (int j = 0; j < N; ++j) p[j] = y[j];
+        }
+    } else {
+        float *p = (float *)a.out + o;
+        if (a.out_vec) {
+#pragma unroll
+            for (int j = 0; j < N; j += 4) *(float4 *)(p + j) = make_float4(x[j] * inv, x[j + 1] * inv, x[j + 2] * inv, x[j + 3] * inv);
+        } else {
+#pragma unroll
+            for (int j = 0; j < N; ++j) p[j] = x[j] * inv;
+        }
+    }
+    if (a.lse != nullptr && d0 == 0) a.lse[at] = L == 0.0f ? -INFINITY : (M + log2f(L)) * kLn2;
+}
+
+// Few rows (up to 2 tiles): memory bound.  Each of the 4 waves takes every 4th span of 32 keys, the next
+// span's loads in flight while one is worked on, and the waves are joined through LDS.
+// LO: 32-bit queries, as hi + lo.
+template <int KV, int D, int MT, bool LO>
+__global__ __launch_bounds__(kThreads, KV == ELEM_F32 ? (D == 64 ? 2 : 1) : (D == 64 && MT == 1 ? 3 : 2)) void attn_tree_kernel(TreeArgs a, TreePlan plan) {
     constexpr bool F32 = KV == ELEM_F32, SCALED = quantised(KV);
-    constexpr int NW = Keys<KV, D>::NW, NS = D / 32, ND = D / 16;
-    constexpr int KT = 32 * HB;
-    constexpr int ESZ = elem_size(KV);
+    constexpr int NW = Keys<KV, D>::NW, ND = D / 16;
     __shared__ float so[kWaves][16][D + 4];
     __shared__ float sm[kWaves][16], sl[kWaves][16];
 
@@ -201,363 +510,181 @@ __global__ __launch_bounds__(kThreads) void attn_tree_kernel(TreeArgs a, TreePla
     const int grp = a.heads / a.c.heads, packed = st.n * grp, first = rg * MT * 16;
     if (first >= packed) return;
     const int live = min(MT, (packed - first + 15) / 16);
+    bool bad = st.bad;
+    const int beg = z * plan.chunk, end = min(beg + plan.chunk, st.total), last = end - 1;
+    const int *table = a.c.table + (size_t)s * a.c.table_stride;
 
-    // ---- queries
-    Frag qh[MT][F32 ? 1 : NS], ql[MT][F32 || !LO ? 1 : NS];
-    float qf[MT][F32 ? D / 4 : 1];
-    float qs[MT];
-    uint64_t mask[MT];
+    Keys<KV, D> cur;
+    Block blk[2];
+    auto fetch = [&](int p, Keys<KV, D> &to, Block (&at)[2]) {
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-        const int i = first + mt * 16 + c;
-        const bool ok = i < packed;
-        const int node = ok ? i / grp : 0, row = st.row0 + node, head = h * grp + (ok ? i - node * grp : 0);
-        const size_t base = (size_t)((int64_t)row * a.q_row + head * D);
-        mask[mt] = !ok ? 0 : (a.row_mask != nullptr ? a.row_mask[row] : (2ull << node) - 1);
-        if (st.n < 64) mask[mt] &= (1ull << st.n) - 1;
-        qs[mt] = a.scale * kLog2e;
-        if constexpr (F32) {
+        for (int b = 0; b < 2; ++b) at[b] = block_of(a, plan, table, h, p + 16 * b, last, bad);
 #pragma unroll
-            for (int u = 0; u < D / 16; ++u)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) qf[mt][4 * u + e] = ok ? load_q(a, base + 16 * u + 4 * g + e) : 0.0f;
-        } else {
-            float x[NS][8];
-            uint32_t top = 0;
-#pragma unroll
-            for (int k = 0; k < NS; ++k)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    x[k][e] = ok ? load_q(a, base + frag_dim<KV>(k, g) + e) : 0.0f;
-                    top = max(top, __float_as_uint(x[k][e]) & 0x7fffffffu);
-                }
-            if constexpr (LO) {
-                top = max(top, (uint32_t)xshfl<16>((int)top));
-                top = max(top, (uint32_t)xshfl<32>((int)top));
-                const int e2 = (int)(top >> 23) - 127;  // a power of two: exact (an Inf or NaN stays one)
-                qs[mt] = ldexpf(qs[mt], e2);
-#pragma unroll
-                for (int k = 0; k < NS; ++k)
-#pragma unroll
-                    for (int e = 0; e < 8; e += 2)
-                        split2(ldexpf(x[k][e], -e2), ldexpf(x[k][e + 1], -e2), qh[mt][k].w[e / 2], ql[mt][k].w[e / 2]);
-            } else {
-#pragma unroll
-                for (int k = 0; k < NS; ++k)
-#pragma unroll
-                    for (int e = 0; e < 8; e += 2)
-                        qh[mt][k].w[e / 2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x[k][e], x[k][e + 1]));
+        for (int b = 0; b < 2; ++b) {
+            load_k<KV, D>(a, at[b], c, g, to.k[b]);
+            if constexpr (SCALED) {
+                to.ks[b] = *(const float4 *)(a.c.k_scale + at[b].vec + 4 * g);
+                to.vs[b] = *(const float4 *)(a.c.v_scale + at[b].vec + 4 * g);
             }
         }
-    }
-    uint64_t seen = 0;  // drafted positions that any of these rows sees
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) seen |= mask[mt];
-    {
-        uint32_t lo = (uint32_t)seen, hi = (uint32_t)(seen >> 32);
-        lo |= xshfl<1>((int)lo), hi |= xshfl<1>((int)hi);
-        lo |= xshfl<2>((int)lo), hi |= xshfl<2>((int)hi);
-        lo |= xshfl<4>((int)lo), hi |= xshfl<4>((int)hi);
-        lo |= xshfl<8>((int)lo), hi |= xshfl<8>((int)hi);
-        seen = ((uint64_t)hi << 32) | lo;
-    }
+        for (int b = 0; b < 2; ++b) load_v<KV, D>(a, at[b], c, g, to.v[b]);
+    };
+    int p0 = beg + 32 * w;
+    if (p0 < end) fetch(p0, cur, blk);
 
-    // ---- keys
-    float m[MT], l[MT];
-    floatx4 o[MT][ND];
+    Query<KV, D, LO> q[MT];
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-        m[mt] = -INFINITY;
-        l[mt] = 0.0f;
-#pragma unroll
-        for (int j = 0; j < ND; ++j) o[mt][j] = floatx4{0.f, 0.f, 0.f, 0.f};
-    }
-    int top_exp = 0;       // biased exponent of the largest value scale so far
-    bool bad = st.bad;
-    const int beg = z * plan.chunk, end = min(beg + plan.chunk, st.total), last = st.total - 1;
-    const int *table = a.c.table + (size_t)s * a.c.table_stride;
-    const uint32_t page16 = a.c.page_size >> 4;
+    for (int mt = 0; mt < MT; ++mt) q[mt].load(a, st, grp, h, first + mt * 16 + c, packed, g);
+    const uint64_t seen = seen_by(q);
+    Rows<MT, ND> rows;
+    rows.clear(SCALED);
 
 #pragma unroll 1
-    for (int p0 = beg + KT * w; p0 < end; p0 += KT * kWaves) {
-        const bool tail = p0 + KT > st.ctx;
-        Keys<KV, D> keys[HB];
-        size_t vec[HB][2];  // first vector of each block of 16 keys
-        int lim[HB][2];     // its last key that exists
-#pragma unroll
-        for (int hb = 0; hb < HB; ++hb)
-#pragma unroll
-            for (int b = 0; b < 2; ++b) {
-                const int kb = min(p0 + 32 * hb + 16 * b, last & ~15);
-                const uint32_t blk = (uint32_t)kb >> 4, pg = (uint32_t)((blk * plan.page_magic) >> 40);
-                int page = __builtin_amdgcn_readfirstlane(table[pg]);
-                if (page < 0 || page >= a.c.n_pages) {
-                    page = 0;
-                    bad = true;
-                }
-                vec[hb][b] = ((size_t)page * a.c.heads + h) * a.c.page_size + (blk - pg * page16) * 16;
-                lim[hb][b] = min(15, last - kb);
-            }
-#pragma unroll
-        for (int hb = 0; hb < HB; ++hb)
-#pragma unroll
-            for (int b = 0; b < 2; ++b) {
-                const char *kp = (const char *)a.c.k + vec[hb][b] * (D * ESZ);
-                const int off = min(c, lim[hb][b]) * (D * ESZ) + 16 * g;
-#pragma unroll
-                for (int u = 0; u < NW; ++u) keys[hb].k[b][u] = *(const uint4 *)(kp + off + 64 * u);
-                if constexpr (SCALED) {
-                    keys[hb].ks[b] = *(const float4 *)(a.c.k_scale + vec[hb][b] + 4 * g);
-                    keys[hb].vs[b] = *(const float4 *)(a.c.v_scale + vec[hb][b] + 4 * g);
-                }
-            }
-#pragma unroll
-        for (int hb = 0; hb < HB; ++hb)
-#pragma unroll
-            for (int b = 0; b < 2; ++b) {
-                const char *vp = (const char *)a.c.v + vec[hb][b] * (D * ESZ);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int off = min(4 * g + i, lim[hb][b]) * (D * ESZ) + c * (NW * 4);
-                    __builtin_memcpy(keys[hb].v[4 * b + i], __builtin_assume_aligned(vp + off, NW < 4 ? NW * 4 : 16), NW * 4);
-                }
-            }
+    for (; p0 < end; p0 += 32 * kWaves) {
+        const bool tail = p0 + 32 > st.ctx;
+        Keys<KV, D> next;
+        Block nblk[2];
+        fetch(p0 + 32 * kWaves, next, nblk);  // (past the end: the last block again)
 
-        // scores, in units of log 2
-        float sc[MT][HB][2][4];
+        float x[MT][2][4];
 #pragma unroll
-        for (int hb = 0; hb < HB; ++hb)
+        for (int b = 0; b < 2; ++b) {
+            floatx4 acc[MT];
 #pragma unroll
-            for (int b = 0; b < 2; ++b) {
-                floatx4 acc[MT];
+            for (int mt = 0; mt < MT; ++mt) acc[mt] = floatx4{0.f, 0.f, 0.f, 0.f};
+            if constexpr (F32) {
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt) acc[mt] = floatx4{0.f, 0.f, 0.f, 0.f};
-                if constexpr (F32) {
+                for (int u = 0; u < NW; ++u) {
+                    const float kf[4] = {__uint_as_float(cur.k[b][u].x), __uint_as_float(cur.k[b][u].y),
+                                         __uint_as_float(cur.k[b][u].z), __uint_as_float(cur.k[b][u].w)};
 #pragma unroll
-                    for (int u = 0; u < NW; ++u) {
-                        const float *kf = (const float *)&keys[hb].k[b][u];
+                    for (int e = 0; e < 4; ++e)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
+                        for (int mt = 0; mt < MT; ++mt) acc[mt] = mfma(kf[e], q[mt].f[4 * u + e], acc[mt]);
+                }
+            } else {
 #pragma unroll
-                            for (int mt = 0; mt < MT; ++mt)
-                                if (mt < live) acc[mt] = mfma(kf[e], qf[mt][4 * u + e], acc[mt]);
-                    }
-                } else {
+                for (int k = 0; k < D / 32; ++k) {
+                    const Frag f = k_frag<KV, D>(cur.k[b], k);
 #pragma unroll
-                    for (int k = 0; k < NS; ++k) {
-                        const Frag f = k_frag<KV, D>(keys[hb].k[b], k);
-#pragma unroll
-                        for (int mt = 0; mt < MT; ++mt)
-                            if (mt < live) {
-                                acc[mt] = mfma(f, qh[mt][k], acc[mt]);
-                                if constexpr (LO) acc[mt] = mfma(f, ql[mt][k], acc[mt]);
-                            }
+                    for (int mt = 0; mt < MT; ++mt) {
+                        acc[mt] = mfma(f, q[mt].hi[k], acc[mt]);
+                        if constexpr (LO) acc[mt] = mfma(f, q[mt].lo[k], acc[mt]);
                     }
                 }
-                const float *ks = (const float *)&keys[hb].ks[b];
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) sc[mt][hb][b][i] = acc[mt][i] * (SCALED ? ks[i] * qs[mt] : qs[mt]);
             }
-        auto visible = [&](uint64_t rows_mask, int key) {  // key p0 + key
-            const int j = p0 + key - st.ctx;
-            return j < 0 || (j < st.n && ((rows_mask >> (j & 63)) & 1));
-        };
-        if (tail) {
+            const float ks[4] = {cur.ks[b].x, cur.ks[b].y, cur.ks[b].z, cur.ks[b].w};
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-                for (int hb = 0; hb < HB; ++hb)
-#pragma unroll
-                    for (int b = 0; b < 2; ++b)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            if (!visible(mask[mt], 32 * hb + 16 * b + 4 * g + i)) sc[mt][hb][b][i] = -INFINITY;
+                for (int i = 0; i < 4; ++i) x[mt][b][i] = SCALED ? acc[mt][i] * ks[i] : acc[mt][i];
         }
-
-        // value scales against the largest so far
-        float vs[HB][2][4];
-        float shrink = 1.0f;
+        if (tail) hide(st, q, p0, g, -INFINITY, x);
         if constexpr (SCALED) {
             uint32_t top = 0;
 #pragma unroll
-            for (int hb = 0; hb < HB; ++hb)
+            for (int b = 0; b < 2; ++b) {
+                const float vs[4] = {cur.vs[b].x, cur.vs[b].y, cur.vs[b].z, cur.vs[b].w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t y = __float_as_uint(vs[i]) & 0x7fffffffu;
+                    const bool use = y < 0x7f800000u && (!tail || visible(st, seen, p0 + 16 * b + 4 * g + i));
+                    top = max(top, use ? y : 0u);
+                }
+            }
+            top = max(top, (uint32_t)xshfl<16>((int)top));
+            top = max(top, (uint32_t)xshfl<32>((int)top));
+            const float up = up_of((uint32_t)__builtin_amdgcn_readfirstlane((int)top));
+            if (up < rows.up) rows.raise(up);
+        }
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) rows.weigh(mt, q[mt].qs, x[mt]);
+        if constexpr (SCALED) scale_weights(st, q, tail, p0, g, cur.vs, x);
+        Frag ph[MT], pl[MT];
+        if constexpr (!F32)
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
                 for (int b = 0; b < 2; ++b)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const uint32_t x = __float_as_uint(((const float *)&keys[hb].vs[b])[i]) & 0x7fffffffu;
-                        const bool use = x < 0x7f800000u && (!tail || visible(seen, 32 * hb + 16 * b + 4 * g + i));
-                        top = max(top, use ? x : 0u);
-                    }
-            top = max(top, (uint32_t)xshfl<16>((int)top));
-            top = max(top, (uint32_t)xshfl<32>((int)top));
-            const int e = __builtin_amdgcn_readfirstlane(top >> 23);
-            if (e > top_exp) {
-                shrink = ldexpf(1.0f, top_exp - e);
-                top_exp = e;
-            }
-#pragma unroll
-            for (int hb = 0; hb < HB; ++hb)
+                    for (int i = 0; i < 4; i += 2) split2(x[mt][b][i], x[mt][b][i + 1], ph[mt].w[2 * b + i / 2], pl[mt].w[2 * b + i / 2]);
+        // drafted values that some row does not see may hold anything, and 0 times an Inf or NaN is not 0: such
+        // elements go into the products as 0, and are added to the rows that see them
+        if constexpr (KV != ELEM_I8) {
+            if (tail) {
+                bool odd = false;
 #pragma unroll
                 for (int b = 0; b < 2; ++b)
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        vs[hb][b][i] = ldexpf(((const float *)&keys[hb].vs[b])[i], kWeightExp + 127 - top_exp);
-        }
-
-        // weights
-        Frag ph[MT][HB], pl[MT][HB];
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-            float mx = -INFINITY;
-#pragma unroll
-            for (int hb = 0; hb < HB; ++hb)
-#pragma unroll
-                for (int b = 0; b < 2; ++b)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) mx = fmaxf(mx, sc[mt][hb][b][i]);
-            mx = fmaxf(mx, xshfl<16>(mx));
-            mx = fmaxf(mx, xshfl<32>(mx));
-            const float m_new = fmaxf(m[mt], mx), m0 = m_new == -INFINITY ? 0.0f : m_new;
-            const float fade = exp2_(m[mt] - m0);
-            if (__any(fade != 1.0f) || (SCALED && shrink != 1.0f)) {
-                l[mt] *= fade;
-                const float f = SCALED ? fade * shrink : fade;
-#pragma unroll
-                for (int j = 0; j < ND; ++j) o[mt][j] *= f;
-            }
-            m[mt] = m_new;
-#pragma unroll
-            for (int hb = 0; hb < HB; ++hb)
-#pragma unroll
-                for (int b = 0; b < 2; ++b)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        float &x = sc[mt][hb][b][i];
-                        const float e = exp2_(x - m0);
-                        l[mt] += e;
-                        x = SCALED ? e * vs[hb][b][i] : (F32 ? e : e * (float)(1 << kWeightExp));
-                        if (SCALED && tail && !visible(mask[mt], 32 * hb + 16 * b + 4 * g + i)) x = 0.0f;  // whatever its scale holds
-                    }
-            if constexpr (!F32) {
-#pragma unroll
-                for (int hb = 0; hb < HB; ++hb)
-#pragma unroll
-                    for (int b = 0; b < 2; ++b)
-#pragma unroll
-                        for (int i = 0; i < 4; i += 2)
-                            split2(sc[mt][hb][b][i], sc[mt][hb][b][i + 1], ph[mt][hb].w[2 * b + i / 2], pl[mt][hb].w[2 * b + i / 2]);
-            }
-        }
-
-        // values
-#pragma unroll
-        for (int hb = 0; hb < HB; ++hb) {
-            if constexpr (KV != ELEM_I8) {
-                // drafted values that some row does not see may hold anything, and 0 times an Inf or NaN
-                // is not 0: such elements go into the products as 0, and are added, key by key, to the rows
-                // that see them
-                if (tail) {
-                    bool odd = false;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
 #pragma unroll
                         for (int n = 0; n < NW; ++n) {
-                            const uint32_t x = keys[hb].v[e][n];
-                            keys[hb].v[e][n] = finite_part<KV>(x);
-                            odd |= keys[hb].v[e][n] != x;
+                            const uint32_t y = cur.v[b][i][n];
+                            cur.v[b][i][n] = finite_part<KV>(y);
+                            odd |= cur.v[b][i][n] != y;
                         }
-                    if (__any(odd)) {
+                if (__any(odd))
 #pragma unroll
-                        for (int mt = 0; mt < MT; ++mt) {
-#pragma unroll
-                            for (int b = 0; b < 2; ++b)
-#pragma unroll
-                                for (int i = 0; i < 4; ++i) so[w][c][16 * b + 4 * g + i] = sc[mt][hb][b][i];
-                            __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
-                            __builtin_amdgcn_wave_barrier();
-#pragma unroll 1
-                            for (int kk = 0; kk < 32; ++kk) {
-                                const int b = kk >> 4;
-                                const size_t at = ((b ? vec[hb][1] : vec[hb][0]) + min(kk & 15, b ? lim[hb][1] : lim[hb][0])) * D +
-                                                  (D / 4) * g;
-                                const float x = so[w][c][kk];
-                                const bool see = visible(mask[mt], 32 * hb + kk);
-#pragma unroll
-                                for (int r = 0; r < 4; ++r)
-#pragma unroll
-                                    for (int j = 0; j < ND; ++j) {
-                                        const float v = v_value<KV>(a.c.v, at + ND * r + j);
-                                        const bool add = see && !(fabsf(v) < INFINITY);
-                                        o[mt][j][r] += add ? x * v : 0.0f;
-                                    }
-                            }
-                            __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
-                            __builtin_amdgcn_wave_barrier();
-                        }
-                    }
-                }
+                    for (int mt = 0; mt < MT; ++mt) add_odd_values<KV, D>(a, st, blk, p0, mt, q[mt].mask, x[mt], so[w], rows);
             }
-            if constexpr (F32) {
+        }
+        if constexpr (F32) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
 #pragma unroll
                     for (int j = 0; j < ND; ++j)
 #pragma unroll
                         for (int mt = 0; mt < MT; ++mt)
-                            if (mt < live) o[mt][j] = mfma(__uint_as_float(keys[hb].v[e][j]), sc[mt][hb][e / 4][e % 4], o[mt][j]);
-            } else {
-                constexpr int DW = dims_per_word<KV>();
+                            rows.o[mt][j] = mfma(__uint_as_float(cur.v[b][i][j]), x[mt][b][i], rows.o[mt][j]);
+        } else {
+            constexpr int DW = dims_per_word<KV>();
 #pragma unroll
-                for (int n = 0; n < NW; ++n) {
-                    Frag f[DW];
-                    v_frags<KV, NW>(keys[hb].v, n, f);
+            for (int n = 0; n < NW; ++n) {
+                uint32_t f0[DW][2], f1[DW][2];
+                v_halves<KV, NW>(cur.v[0], n, f0);
+                v_halves<KV, NW>(cur.v[1], n, f1);
 #pragma unroll
-                    for (int d = 0; d < DW; ++d)
+                for (int d = 0; d < DW; ++d) {
+                    const Frag f{{f0[d][0], f0[d][1], f1[d][0], f1[d][1]}};
 #pragma unroll
-                        for (int mt = 0; mt < MT; ++mt)
-                            if (mt < live) {
-                                o[mt][DW * n + d] = mfma(f[d], ph[mt][hb], o[mt][DW * n + d]);
-                                o[mt][DW * n + d] = mfma(f[d], pl[mt][hb], o[mt][DW * n + d]);
-                            }
+                    for (int mt = 0; mt < MT; ++mt) {
+                        rows.o[mt][DW * n + d] = mfma(f, ph[mt], rows.o[mt][DW * n + d]);
+                        rows.o[mt][DW * n + d] = mfma(f, pl[mt], rows.o[mt][DW * n + d]);
+                    }
                 }
             }
         }
+        cur = next;
+        blk[0] = nblk[0], blk[1] = nblk[1];
     }
 
     // ---- the waves joined, one row tile at a time
     bad = __any(bad);
-    const size_t all_rows = (size_t)a.rows * a.heads;
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
         if (mt >= live) break;
-        const int unscale = F32 ? 0 : (SCALED ? top_exp - 127 - kWeightExp : -kWeightExp);
-        float sum = l[mt];
+        float sum = rows.l[mt];
         sum += xshfl<16>(sum);
         sum += xshfl<32>(sum);
         if (mt > 0) __syncthreads();
 #pragma unroll
         for (int r = 0; r < 4; ++r)
 #pragma unroll
-            for (int j = 0; j < ND; j += 4) {
-                float4 x;
-                x.x = ldexpf(o[mt][j][r], unscale);
-                x.y = ldexpf(o[mt][j + 1][r], unscale);
-                x.z = ldexpf(o[mt][j + 2][r], unscale);
-                x.w = ldexpf(o[mt][j + 3][r], unscale);
-                *(float4 *)&so[w][c][ND * (4 * g + r) + j] = x;
-            }
+            for (int j = 0; j < ND; j += 4)
+                *(float4 *)&so[w][c][ND * (4 * g + r) + j] =
+                    make_float4(rows.o[mt][j][r], rows.o[mt][j + 1][r], rows.o[mt][j + 2][r], rows.o[mt][j + 3][r]);
         if (g == 0) {
-            sm[w][c] = m[mt];
+            sm[w][c] = rows.m(mt);
             sl[w][c] = bad ? __uint_as_float(0x7fc00000u) : sum;
         }
         __syncthreads();
         const int row = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * ND;
         const int i = first + mt * 16 + row;
         if (i >= packed) continue;
-        float M = fmaxf(fmaxf(sm[0][row], sm[1][row]), fmaxf(sm[2][row], sm[3][row]));
+        const float M = fmaxf(fmaxf(sm[0][row], sm[1][row]), fmaxf(sm[2][row], sm[3][row]));
         const float M0 = M == -INFINITY ? 0.0f : M;
         float L = 0.0f, acc[ND];
 #pragma unroll
@@ -569,93 +696,302 @@ __global__ __launch_bounds__(kThreads) void attn_tree_kernel(TreeArgs a, TreePla
 #pragma unroll
             for (int j = 0; j < ND; ++j) acc[j] = fmaf(so[v][row][d0 + j], f, acc[j]);
         }
-        const int node = i / grp, head = h * grp + i - node * grp;
-        const size_t at = (size_t)(st.row0 + node) * a.heads + head;
-        if (plan.splits > 1) {
-            float *ws = (float *)a.ws + ((size_t)z * all_rows + at) * 2;
-            if (d0 == 0) *(float2 *)ws = make_float2(M, L);
-            float *po = (float *)a.ws + (size_t)plan.splits * all_rows * 2 + ((size_t)z * all_rows + at) * D + d0;
-            if (L != 0.0f)
-#pragma unroll
-                for (int j = 0; j < ND; j += 4) *(float4 *)(po + j) = make_float4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
-            continue;
-        }
-        const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-        const size_t oi = (size_t)((int64_t)(st.row0 + node) * a.out_row + head * D + d0);
-#pragma unroll
-        for (int j = 0; j < ND; ++j) {
-            if (a.out_dtype == ELEM_F16)
-                ((__half *)a.out)[oi + j] = __float2half_rn(acc[j] * inv);
-            else
-                ((float *)a.out)[oi + j] = acc[j] * inv;
-        }
-        if (a.lse != nullptr && d0 == 0) a.lse[at] = L == 0.0f ? -INFINITY : (M + log2f(L)) * kLn2;
+        put_row<D, ND>(a, plan, st, z, grp, h, i, d0, M, L, acc);
     }
 }
 
-// The key splits of each (row, head) joined in their order: one wave each, lane c holding split c's
-// maximum and sum, then D / 4 lanes a vector with 256 / D splits side by side.
+// Many rows (more than 32): bound by the matrix and vector units.  Every wave has MT row tiles of its own and all
+// of them the same keys, which they prepare together: of a stage of 16 keys a wave each turns its block into
+// fragments, K and V, and puts them into LDS in the order in which the products read them (16 bytes a lane, no
+// bank conflicts), so a key is converted once for up to 256 rows.  Two stages: while one is worked on the next
+// one's loads are in flight, and it is written before the only barrier of a stage.
+// PLO: weights as hi + lo; where the output is fp16 they are rounded to fp16 once, to nearest: an error of the
+// size of the output's own rounding, for a quarter of the products less.
+template <int KV, int D, int NWV>
+struct WideLds {
+    uint4 k[2][NWV][D / 32][64];
+    uint4 v[2][NWV / 2][D / 16][64];
+    float ks[2][NWV][16], vs[2][NWV][16];
+    uint32_t top[2][NWV];
+    int odd[2][NWV];
+    uint64_t seen[NWV];
+    int bad[NWV];
+    float room[KV == ELEM_I8 ? 1 : NWV][16][36];
+};
+
+template <int KV, int D, int NWV, int MT, bool LO, bool PLO>
+__global__ __launch_bounds__(64 * NWV, 2) void attn_tree_wide_kernel(TreeArgs a, TreePlan plan) {
+    constexpr bool SCALED = quantised(KV);
+    constexpr int NW = Keys<KV, D>::NW, NS = D / 32, ND = D / 16, DW = dims_per_word<KV>();
+    constexpr int STAGE = 16 * NWV;
+    __shared__ WideLds<KV, D, NWV> lds;
+
+    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int units = a.c.streams * a.c.heads * plan.splits;
+    const int b8 = blockIdx.x >> 3, rg = b8 % plan.row_groups, unit = (b8 / plan.row_groups) * 8 + (blockIdx.x & 7);
+    if (unit >= units) return;
+    const int z = unit % plan.splits, sh = unit / plan.splits, h = sh % a.c.heads, s = sh / a.c.heads;
+    const Stream st = stream_of(a, s);
+    const int grp = a.heads / a.c.heads, packed = st.n * grp;
+    if (rg * NWV * MT * 16 >= packed) return;
+    const int first = (rg * NWV + w) * MT * 16;
+    bool bad = st.bad;
+    const int beg = z * plan.chunk, end = min(beg + plan.chunk, st.total), last = end - 1;
+    const int *table = a.c.table + (size_t)s * a.c.table_stride;
+
+    uint4 kraw[NW];
+    uint32_t vraw[4][NW];
+    float ksr = 0.0f, vsr = 0.0f;
+    auto fetch = [&](int p) {
+        const Block b = block_of(a, plan, table, h, p + 16 * w, last, bad);
+        load_k<KV, D>(a, b, c, g, kraw);
+        load_v<KV, D>(a, b, c, g, vraw);
+        if constexpr (SCALED) {
+            ksr = a.c.k_scale[b.vec + c];
+            vsr = a.c.v_scale[b.vec + c];
+        }
+    };
+    if (beg < end) fetch(beg);
+
+    Query<KV, D, LO> q[MT];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) q[mt].load(a, st, grp, h, first + mt * 16 + c, packed, g);
+    uint64_t seen = seen_by(q);
+    if (lane == 0) lds.seen[w] = seen;
+    lds_barrier();
+    seen = 0;
+#pragma unroll
+    for (int v = 0; v < NWV; ++v) seen |= lds.seen[v];
+
+    auto put = [&](int buf, int p) {  // this wave's block of the stage at p
+        const int pos = p + 16 * w;
+#pragma unroll
+        for (int k = 0; k < NS; ++k) {
+            const Frag f = k_frag<KV, D>(kraw, k);
+            lds.k[buf][w][k][lane] = make_uint4(f.w[0], f.w[1], f.w[2], f.w[3]);
+        }
+        if constexpr (KV != ELEM_I8) {
+            bool odd = false;
+            if (pos + 16 > st.ctx) {  // (as in the kernel for few rows)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int n = 0; n < NW; ++n) {
+                        const uint32_t y = vraw[i][n];
+                        vraw[i][n] = finite_part<KV>(y);
+                        odd |= vraw[i][n] != y;
+                    }
+            }
+            odd = __any(odd);
+            if (lane == 0) lds.odd[buf][w] = odd;
+        }
+#pragma unroll
+        for (int n = 0; n < NW; ++n) {
+            uint32_t f[DW][2];
+            v_halves<KV, NW>(vraw, n, f);
+#pragma unroll
+            for (int d = 0; d < DW; ++d) ((uint2 *)&lds.v[buf][w / 2][DW * n + d][lane])[w & 1] = make_uint2(f[d][0], f[d][1]);
+        }
+        if constexpr (SCALED) {
+            uint32_t top = __float_as_uint(vsr) & 0x7fffffffu;
+            if (top >= 0x7f800000u || !visible(st, seen, pos + c)) top = 0;
+            top = max(top, (uint32_t)xshfl<1>((int)top));
+            top = max(top, (uint32_t)xshfl<2>((int)top));
+            top = max(top, (uint32_t)xshfl<4>((int)top));
+            top = max(top, (uint32_t)xshfl<8>((int)top));
+            if (lane == 0) lds.top[buf][w] = top;
+            if (g == 0) {
+                lds.ks[buf][w][c] = ksr;
+                lds.vs[buf][w][c] = vsr;
+            }
+        }
+    };
+
+    Rows<MT, ND> rows;
+    rows.clear(SCALED);
+    if (beg < end) put(0, beg);
+    lds_barrier();
+    int buf = 0;
+#pragma unroll 1
+    for (int p = beg; p < end; p += STAGE) {
+        const bool more = p + STAGE < end;
+        if (more) fetch(p + STAGE);
+        if (first < packed) {
+#pragma unroll 1
+            for (int u = 0; u < NWV / 2; ++u) {
+                const int p0 = p + 32 * u;
+                if (p0 >= end) break;
+                const bool tail = p0 + 32 > st.ctx;
+                float x[MT][2][4];
+                float4 ks[2], vs[2];
+                float up = 0.0f;
+                if constexpr (SCALED) {
+                    up = up_of((uint32_t)__builtin_amdgcn_readfirstlane((int)max(lds.top[buf][2 * u], lds.top[buf][2 * u + 1])));
+#pragma unroll
+                    for (int b = 0; b < 2; ++b) {
+                        ks[b] = *(const float4 *)&lds.ks[buf][2 * u + b][4 * g];
+                        vs[b] = *(const float4 *)&lds.vs[buf][2 * u + b][4 * g];
+                    }
+                }
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+                    floatx4 acc[MT];
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt) acc[mt] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int k = 0; k < NS; ++k) {
+                        const uint4 y = lds.k[buf][2 * u + b][k][lane];
+                        const Frag f{{y.x, y.y, y.z, y.w}};
+#pragma unroll
+                        for (int mt = 0; mt < MT; ++mt) {
+                            acc[mt] = mfma(f, q[mt].hi[k], acc[mt]);
+                            if constexpr (LO) acc[mt] = mfma(f, q[mt].lo[k], acc[mt]);
+                        }
+                    }
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) x[mt][b][i] = SCALED ? acc[mt][i] * ((const float *)&ks[b])[i] : acc[mt][i];
+                }
+                if (tail) hide(st, q, p0, g, -INFINITY, x);
+                if constexpr (SCALED) {
+                    if (up < rows.up) rows.raise(up);
+                }
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) rows.weigh(mt, q[mt].qs, x[mt]);
+                if constexpr (SCALED) scale_weights(st, q, tail, p0, g, vs, x);
+                Frag ph[MT], pl[PLO ? MT : 1];
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                    for (int b = 0; b < 2; ++b)
+#pragma unroll
+                        for (int i = 0; i < 4; i += 2) {
+                            if constexpr (PLO) {
+                                split2(x[mt][b][i], x[mt][b][i + 1], ph[mt].w[2 * b + i / 2], pl[mt].w[2 * b + i / 2]);
+                            } else {
+                                const h2 y = {(_Float16)x[mt][b][i], (_Float16)x[mt][b][i + 1]};
+                                ph[mt].w[2 * b + i / 2] = __builtin_bit_cast(uint32_t, y);
+                            }
+                        }
+                if constexpr (KV != ELEM_I8) {
+                    if (tail && (lds.odd[buf][2 * u] | lds.odd[buf][2 * u + 1])) {
+                        Block blk[2];
+#pragma unroll
+                        for (int b = 0; b < 2; ++b) blk[b] = block_of(a, plan, table, h, p0 + 16 * b, last, bad);
+#pragma unroll
+                        for (int mt = 0; mt < MT; ++mt) add_odd_values<KV, D>(a, st, blk, p0, mt, q[mt].mask, x[mt], lds.room[w], rows);
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < ND; ++j) {
+                    const uint4 y = lds.v[buf][u][j][lane];
+                    const Frag f{{y.x, y.y, y.z, y.w}};
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt) {
+                        rows.o[mt][j] = mfma(f, ph[mt], rows.o[mt][j]);
+                        if constexpr (PLO) rows.o[mt][j] = mfma(f, pl[mt], rows.o[mt][j]);
+                    }
+                }
+            }
+        }
+        buf ^= 1;
+        if (more) put(buf, p + STAGE);
+        lds_barrier();
+    }
+    bad = __any(bad);
+    if (lane == 0) lds.bad[w] = bad;
+    lds_barrier();
+#pragma unroll
+    for (int v = 0; v < NWV; ++v) bad |= lds.bad[v] != 0;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+        const int i = first + mt * 16 + c;
+        float L = rows.l[mt];
+        L += xshfl<16>(L);
+        L += xshfl<32>(L);
+        if (bad) L = __uint_as_float(0x7fc00000u);
+        float y[4 * ND];
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int j = 0; j < ND; ++j) y[ND * r + j] = rows.o[mt][j][r];
+        if (i < packed) put_row<D, 4 * ND>(a, plan, st, z, grp, h, i, (D / 4) * g, rows.m(mt), L, y);
+    }
+}
+
+// The key splits of each (row, head) joined in their order by one workgroup of 4 waves: every wave forms the
+// maximum and the sum (lane c holds split c's) and adds up a quarter of the splits, D / 4 lanes a vector with
+// 256 / D splits side by side.
 template <int D>
-__global__ __launch_bounds__(kThreads) void attn_tree_join_kernel(TreeArgs a, int splits) {
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const int per = (a.max_rows * a.heads + kWaves - 1) / kWaves;
-    const int s = blockIdx.x / per, i = (blockIdx.x - s * per) * kWaves + w;
+__global__ __launch_bounds__(kThreads) void attn_tree_join_kernel(TreeArgs a, TreePlan plan) {
+    constexpr int G = D / 4, SIDE = 64 / G, ROUNDS = kMaxSplits / (kWaves * SIDE);
+    __shared__ float4 part[kWaves][G];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, splits = plan.splits;
+    const int per = a.max_rows * a.heads, s = blockIdx.x / per, i = blockIdx.x - s * per;
     const Stream st = stream_of(a, s);
     if (i >= st.n * a.heads) return;
     const size_t all_rows = (size_t)a.rows * a.heads, at = (size_t)st.row0 * a.heads + i;
-    const float2 *ml = (const float2 *)a.ws;
     float2 mine = make_float2(-INFINITY, 0.0f);
-    if (lane < splits) mine = ml[(size_t)lane * all_rows + at];
-    const float M = wave_max(mine.x), M0 = M == -INFINITY ? 0.0f : M;
-    const float f = exp2_(mine.x - M0);
-    const float L = wave_sum(mine.y * f);
-    constexpr int G = D / 4, SIDE = 64 / G;
+    if (lane < splits) mine = ((const float2 *)a.ws)[(size_t)lane * all_rows + at];
     const int d = (lane % G) * 4, side = lane / G;
-    const float *po = (const float *)a.ws + (size_t)splits * all_rows * 2;
+    const float *po = (const float *)a.ws + (size_t)splits * all_rows * 2 + at * D + d;
+    float4 x[ROUNDS];
+#pragma unroll
+    for (int r = 0; r < ROUNDS; ++r) {  // (a split without keys has written none: what is read there is not used)
+        const int k = (r * kWaves + w) * SIDE + side;
+        if (r * kWaves * SIDE < splits) x[r] = *(const float4 *)(po + (size_t)min(k, splits - 1) * all_rows * D);
+    }
+    const float M = wave_max(mine.x), M0 = M == -INFINITY ? 0.0f : M;
+    const float f = exp2_(mine.x - M0), L = wave_sum(mine.y * f);
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int c0 = 0; c0 < splits; c0 += SIDE) {
-        const int k = c0 + side;
-        const float fk = __shfl(f, k & 63), lk = __shfl(mine.y, k & 63);
-        if (k < splits && lk != 0.0f) {
-            const float4 x = *(const float4 *)(po + ((size_t)k * all_rows + at) * D + d);
-            o.x = fmaf(x.x, fk, o.x);
-            o.y = fmaf(x.y, fk, o.y);
-            o.z = fmaf(x.z, fk, o.z);
-            o.w = fmaf(x.w, fk, o.w);
+#pragma unroll
+    for (int r = 0; r < ROUNDS; ++r) {
+        const int k = (r * kWaves + w) * SIDE + side;
+        if (r * kWaves * SIDE < splits) {
+            const float fk = __shfl(f, k & 63), lk = __shfl(mine.y, k & 63);
+            const bool use = k < splits && lk != 0.0f;
+            o.x = use ? fmaf(x[r].x, fk, o.x) : o.x;
+            o.y = use ? fmaf(x[r].y, fk, o.y) : o.y;
+            o.z = use ? fmaf(x[r].z, fk, o.z) : o.z;
+            o.w = use ? fmaf(x[r].w, fk, o.w) : o.w;
         }
     }
-#define MH_FOLD(M_) o.x += xshfl<M_>(o.x), o.y += xshfl<M_>(o.y), o.z += xshfl<M_>(o.z), o.w += xshfl<M_>(o.w)
-    if constexpr (G == 16) MH_FOLD(16);
-    MH_FOLD(32);
-#undef MH_FOLD
-    if (side != 0) return;
-    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-    const int node = i / a.heads, head = i - node * a.heads;
-    const size_t oi = (size_t)((int64_t)(st.row0 + node) * a.out_row + head * D + d);
-    const float x[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
+    if constexpr (G == 16) o.x += xshfl<16>(o.x), o.y += xshfl<16>(o.y), o.z += xshfl<16>(o.z), o.w += xshfl<16>(o.w);
+    o.x += xshfl<32>(o.x), o.y += xshfl<32>(o.y), o.z += xshfl<32>(o.z), o.w += xshfl<32>(o.w);
+    if (side == 0) part[w][lane % G] = o;
+    __syncthreads();
+    if (threadIdx.x >= G) return;
+    float y[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        if (a.out_dtype == ELEM_F16)
-            ((__half *)a.out)[oi + j] = __float2half_rn(x[j]);
-        else
-            ((float *)a.out)[oi + j] = x[j];
-    }
-    if (a.lse != nullptr && lane == 0) a.lse[at] = L == 0.0f ? -INFINITY : (M + log2f(L)) * kLn2;
+    for (int j = 0; j < 4; ++j)
+        y[j] = (((const float *)&part[0][lane])[j] + ((const float *)&part[1][lane])[j]) +
+               (((const float *)&part[2][lane])[j] + ((const float *)&part[3][lane])[j]);
+    TreePlan whole = plan;
+    whole.splits = 1;
+    put_row<D, 4>(a, whole, st, 0, a.heads, 0, i, d, M, L, y);
 }
 
-// Row tiles of a workgroup.  An fp32 cache's queries and keys take four times the registers.
-int row_tiles_of(const KvCacheArgs &c, int tiles) { return std::min(tiles >= 3 ? 4 : tiles, c.dtype == ELEM_F32 ? 2 : 4); }
+// Rows of 16 of a workgroup: 1 or 2 in the kernel for few rows (an fp32 cache, which the wide one's fp16
+// fragments cannot hold, takes it always), else 4, 8 or 16.
+int group_tiles(const KvCacheArgs &c, int tiles) {
+    if (tiles <= 2 || c.dtype == ELEM_F32) return std::min(tiles, 2);
+    return tiles <= 4 ? 4 : (tiles <= 8 ? 8 : 16);
+}
 
 TreePlan plan_of(const KvCacheArgs &c, int heads, int max_rows, int max_keys) {
     TreePlan p;
     p.tiles = (max_rows * (heads / c.heads) + 15) / 16;
-    const int mt = row_tiles_of(c, p.tiles);
-    p.row_groups = (p.tiles + mt - 1) / mt;
+    p.group = group_tiles(c, p.tiles);
+    p.row_groups = (p.tiles + p.group - 1) / p.group;
     const long long base = (long long)c.streams * c.heads * p.row_groups;
-    const int spans = (max_keys + 255) / 256;  // every wave of a split should have a span
-    int splits = base >= 512 ? 1 : (int)std::min<long long>((1024 + base - 1) / base, kMaxSplits);
+    // enough workgroups for the chip's 256 CUs, and keys enough in a split for its start and end to pay
+    const int least = 256, want = p.group <= 2 ? 512 : 256;
+    const int spans = (max_keys + least - 1) / least;
+    int splits = (int)std::min<long long>((want + base - 1) / base, kMaxSplits);
     splits = std::max(1, std::min(splits, spans));
-    p.chunk = (spans + splits - 1) / splits * 256;
+    p.chunk = ((max_keys + splits - 1) / splits + 127) / 128 * 128;
     p.splits = (max_keys + p.chunk - 1) / p.chunk;
     // blk / (page_size / 16) for blk < 2^24 and a divisor up to 2^11: 2^40 / d rounded up is off by
     // less than d, and blk * d < 2^40
@@ -664,32 +1000,43 @@ TreePlan plan_of(const KvCacheArgs &c, int heads, int max_rows, int max_keys) {
     return p;
 }
 
-template <int KV, int D, int MT, int HB>
-void launch_tiles(const TreeArgs &a, const TreePlan &p, hipStream_t s) {
+template <int KV, int D, bool LO>
+void launch_group(const TreeArgs &a, const TreePlan &p, hipStream_t s) {
     const long long units = (long long)a.c.streams * a.c.heads * p.splits;
     const dim3 grid((unsigned)((units + 7) / 8 * 8 * p.row_groups));
-    constexpr bool LO = KV != ELEM_F32;  // there is a kernel of its own for 32-bit queries
-    if (LO && a.q_dtype == ELEM_F32)
-        hipLaunchKernelGGL((attn_tree_kernel<KV, D, MT, HB, LO>), grid, dim3(kThreads), 0, s, a, p);
-    else
-        hipLaunchKernelGGL((attn_tree_kernel<KV, D, MT, HB, false>), grid, dim3(kThreads), 0, s, a, p);
+    if (p.group == 1) {
+        hipLaunchKernelGGL((attn_tree_kernel<KV, D, 1, LO>), grid, dim3(kThreads), 0, s, a, p);
+    } else if (p.group == 2) {
+        hipLaunchKernelGGL((attn_tree_kernel<KV, D, 2, LO>), grid, dim3(kThreads), 0, s, a, p);
+    } else if constexpr (KV != ELEM_F32) {
+        const bool f16 = a.out_dtype == ELEM_F16;
+        if (p.group == 4 && f16)
+            hipLaunchKernelGGL((attn_tree_wide_kernel<KV, D, 4, 1, LO, false>), grid, dim3(256), 0, s, a, p);
+        else if (p.group == 4)
+            hipLaunchKernelGGL((attn_tree_wide_kernel<KV, D, 4, 1, LO, true>), grid, dim3(256), 0, s, a, p);
+        else if (p.group == 8 && f16)
+            hipLaunchKernelGGL((attn_tree_wide_kernel<KV, D, 8, 1, LO, false>), grid, dim3(512), 0, s, a, p);
+        else if (p.group == 8)
+            hipLaunchKernelGGL((attn_tree_wide_kernel<KV, D, 8, 1, LO, true>), grid, dim3(512), 0, s, a, p);
+        else if (f16)
+            hipLaunchKernelGGL((attn_tree_wide_kernel<KV, D, 8, 2, LO, false>), grid, dim3(512), 0, s, a, p);
+        else
+            hipLaunchKernelGGL((attn_tree_wide_kernel<KV, D, 8, 2, LO, true>), grid, dim3(512), 0, s, a, p);
+    }
 }
 
 template <int KV, int D>
 hipError_t launch_kv(const TreeArgs &a, hipStream_t s) {
     const TreePlan p = plan_of(a.c, a.heads, a.max_rows, a.max_keys);
     (void)hipGetLastError();
-    constexpr int HB = KV == ELEM_F32 ? 1 : 2;
-    switch (row_tiles_of(a.c, p.tiles)) {
-        case 1: launch_tiles<KV, D, 1, HB>(a, p, s); break;
-        case 2: launch_tiles<KV, D, 2, HB>(a, p, s); break;
-        default:
-            if constexpr (KV != ELEM_F32) launch_tiles<KV, D, 4, 1>(a, p, s);
-    }
-    if (p.splits > 1) {
-        const int per = (a.max_rows * a.heads + kWaves - 1) / kWaves;
-        hipLaunchKernelGGL((attn_tree_join_kernel<D>), dim3((unsigned)a.c.streams * per), dim3(kThreads), 0, s, a, p.splits);
-    }
+    if constexpr (KV == ELEM_F32)
+        launch_group<KV, D, false>(a, p, s);
+    else if (a.q_dtype == ELEM_F32)
+        launch_group<KV, D, true>(a, p, s);
+    else
+        launch_group<KV, D, false>(a, p, s);
+    if (p.splits > 1)
+        hipLaunchKernelGGL((attn_tree_join_kernel<D>), dim3((unsigned)(a.c.streams * a.max_rows * a.heads)), dim3(kThreads), 0, s, a, p);
     return hipGetLastError();
 }
 
@@ -710,7 +1057,10 @@ size_t tree_workspace(const KvCacheArgs &c, int heads, int rows, int max_rows, i
     return p.splits == 1 ? 0 : (size_t)p.splits * rows * heads * (2 + c.dim) * sizeof(float);
 }
 
-hipError_t launch_attn_tree(const TreeArgs &a, hipStream_t s) {
+hipError_t launch_attn_tree(const TreeArgs &args, hipStream_t s) {
+    TreeArgs a = args;
+    a.q_vec = (uintptr_t)a.q % 16 == 0 && a.q_row * elem_size(a.q_dtype) % 16 == 0;
+    a.out_vec = (uintptr_t)a.out % 16 == 0 && a.out_row * elem_size(a.out_dtype) % 16 == 0;
     return a.c.dim == 64 ? launch_d<64>(a, s) : launch_d<128>(a, s);
 }
 

@@ -90,6 +90,7 @@ struct TreeArgs {
     int out_dtype = ELEM_F32;
     float *lse = nullptr;
     void *ws = nullptr;
+    bool q_vec = false, out_vec = false;  // 16-byte accesses are aligned (set at the launch)
 };
 constexpr int kTreeMax = 64;  // drafted rows of a stream
 constexpr int kTreeKeysMax = 1 << 28, kTreePageMax = 1 << 15;
