@@ -8,9 +8,10 @@
 // from there.  A row of more than one chunk leaves (m, S, U) and its k best per chunk in the
 // workspace, and a second, small launch joins them in chunk order (fixed, no atomics).
 //
-// The k best of a chunk: each wave sorts its 64 lanes' maxima (21 exchange steps); at least k
-// values reach the k-th of them, so only values at or above it are candidates -- in practice a
-// few more than k of thousands.  The candidates' rank is the number of better ones.
+// The k best of a chunk: each wave sorts its 64 lanes' maxima (21 exchange steps).  At least k values
+// reach the k-th of a wave's, and at least k reach the least of the four waves' (k / 4)-th, so only
+// values at or above the larger of those are candidates -- in practice a few more than k of
+// thousands.  A candidate's rank is the number of better ones.
 #include <algorithm>
 
 #include "paged_ops.h"
@@ -19,10 +20,12 @@ namespace mh {
 namespace {
 
 constexpr int kThreads = 256, kWaves = kThreads / 64;
-constexpr int kMergeMax = 4096;  // candidates a merge holds: chunks * k
+constexpr int kMaxChunks = 128;  // of a row: with 32 alternatives each, 16 values a thread of the join
+static_assert(kMaxChunks * kTopMax <= 16 * kThreads && kMaxChunks * 32 * kThreads >= kVocabMax, "the join holds all chunks' best");
 
-// A row's chunk in the workspace: m, S, U, then k values and k indices.
-constexpr int chunk_words(int k) { return 4 + 2 * k; }
+// A row in the workspace: (m, S, U, -) of each chunk, then the chunks' k values each, then their indices; whole
+// 16-byte pieces.
+__host__ __device__ constexpr size_t row_words(int chunks, int k) { return ((size_t)chunks * (4 + 2 * k) + 3) / 4 * 4; }
 
 // fp32 as an unsigned integer of the same order; -0 counts as +0, and -inf and NaN as 0, below all
 // others: neither is an alternative.
@@ -77,7 +80,25 @@ template <int CAP>
 struct TopLds {
     uint2 cand[kWaves][CAP];  // key, position
     int n[kWaves];
+    uint32_t kth[kWaves], quarter[kWaves];
 };
+
+// First half: the waves' sorted maxima (a barrier must follow).
+template <int EPT, int CAP>
+__device__ __forceinline__ void top_floor(const float (&x)[EPT], int k, TopLds<CAP> &lds) {
+    uint32_t best = 0;
+#pragma unroll
+    for (int i = 0; i < EPT; ++i) best = max(best, key_of(x[i]));
+    const uint32_t sorted = sort64(best);
+    const int w = threadIdx.x >> 6;
+    // read before the branch: inside it the other lanes' last exchange need not have happened
+    const uint32_t kth = __builtin_amdgcn_readlane(sorted, k - 1);
+    const uint32_t quarter = __builtin_amdgcn_readlane(sorted, (k + kWaves - 1) / kWaves - 1);
+    if ((threadIdx.x & 63) == 0) {
+        lds.kth[w] = kth;
+        lds.quarter[w] = quarter;
+    }
+}
 
 // The k best of the workgroup's values x[i], element i of thread t at position
 // ((i / V) * kThreads + t) * V + i % V: put(rank, key, position) is called once for each rank
@@ -85,11 +106,8 @@ struct TopLds {
 template <int EPT, int V, int CAP, class Put>
 __device__ __forceinline__ int top_of(const float (&x)[EPT], int k, TopLds<CAP> &lds, Put &&put) {
     const int t = threadIdx.x, lane = t & 63, w = t >> 6;
-    uint32_t best = 0;
-#pragma unroll
-    for (int i = 0; i < EPT; ++i) best = max(best, key_of(x[i]));
-    const uint32_t sorted = sort64(best);
-    const uint32_t floor_key = __builtin_amdgcn_readlane(sorted, k - 1);
+    const uint32_t least = min(min(lds.quarter[0], lds.quarter[1]), min(lds.quarter[2], lds.quarter[3]));
+    const uint32_t floor_key = max(least, max(max(lds.kth[0], lds.kth[1]), max(lds.kth[2], lds.kth[3])));
     int n = 0, equal = 0;  // of the wave
     const uint64_t below = (1ull << lane) - 1;
 #pragma unroll
@@ -117,6 +135,7 @@ __device__ __forceinline__ int top_of(const float (&x)[EPT], int k, TopLds<CAP> 
         int rank = 0;
         for (int v = 0; v < kWaves; ++v) {
             const int nv = lds.n[v];
+#pragma unroll 4
             for (int j = 0; j < nv; ++j) {
                 const uint2 o = lds.cand[v][j];
                 rank += o.x > me.x || (o.x == me.x && o.y < me.y);
@@ -131,9 +150,10 @@ struct Sums {
     float m, s, u;
 };
 
-// e^x (z - m) terms of a chunk; -inf contributes nothing, NaN and +inf make the sums NaN.
-template <int EPT>
-__device__ __forceinline__ Sums sums_of(const float (&x)[EPT], float inv_t, float (*red)[kWaves]) {
+// m, S and U of a chunk, and the first half of its k best; -inf contributes nothing, NaN and +inf make the
+// sums NaN.
+template <int EPT, int CAP>
+__device__ __forceinline__ Sums sums_of(const float (&x)[EPT], float inv_t, int k, float (*red)[kWaves], TopLds<CAP> &lds) {
     const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
     float m = -INFINITY;
 #pragma unroll
@@ -157,6 +177,7 @@ __device__ __forceinline__ Sums sums_of(const float (&x)[EPT], float inv_t, floa
         red[1][w] = s;
         red[2][w] = u;
     }
+    if (k > 0) top_floor(x, k, lds);
     __syncthreads();
     return Sums{m, (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]), (red[2][0] + red[2][1]) + (red[2][2] + red[2][3])};
 }
@@ -214,7 +235,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LogprobArgs a, int c
             for (int j = 0; j < V; ++j) x[i + j] = e + j < a.vocab ? logit(p + e + j) : -INFINITY;
         }
     }
-    const Sums q = sums_of<EPT>(x, a.inv_t, red);
+    const Sums q = sums_of(x, a.inv_t, a.top_k, red, lds);
     if (chunks == 1) {
         if (t == 0) finish_row<T>(a, r, q);
         if (a.top_k > 0) {
@@ -226,53 +247,52 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LogprobArgs a, int c
         }
         return;
     }
-    float *o = (float *)a.ws + (size_t)blockIdx.x * chunk_words(a.top_k);
-    if (t == 0) {
-        o[0] = q.m;
-        o[1] = q.s;
-        o[2] = q.u;
-    }
+    float *row = (float *)a.ws + r * row_words(chunks, a.top_k);
+    if (t == 0) *(float4 *)(row + 4 * c) = make_float4(q.m, q.s, q.u, 0.0f);
     if (a.top_k > 0) {
+        float *o = row + 4 * chunks + c * a.top_k;
         const int n = top_of<EPT, V>(x, a.top_k, lds, [&](int rank, uint32_t key, int at) {
-            o[4 + rank] = of_key(key);
-            ((int *)o)[4 + a.top_k + rank] = base + at;
+            o[rank] = of_key(key);
+            ((int *)o)[chunks * a.top_k + rank] = base + at;
         });
-        for (int i = n + t; i < a.top_k; i += kThreads) o[4 + i] = -INFINITY;
+        for (int i = n + t; i < a.top_k; i += kThreads) o[i] = -INFINITY;
     }
 }
 
-// The chunks of one row joined.
-template <class T>
+// The chunks of one row joined; EPT values a thread hold all chunks' best.
+template <class T, int EPT>
 __global__ __launch_bounds__(kThreads) void logprobs_join_kernel(LogprobArgs a, int chunks) {
-    constexpr int EPT = kMergeMax / kThreads;
     __shared__ TopLds<cand_max<EPT, 1>()> lds;
-    const int r = blockIdx.x, t = threadIdx.x, words = chunk_words(a.top_k);
-    const float *w = (const float *)a.ws + (size_t)r * chunks * words;
+    const int r = blockIdx.x, t = threadIdx.x, n = chunks * a.top_k;
+    const float *w = (const float *)a.ws + r * row_words(chunks, a.top_k), *best = w + 4 * chunks;
+    // position c * k + j: equal values of a lower index come first, as chunks and ranks do
+    float x[EPT];
+#pragma unroll
+    for (int i = 0; i < EPT; ++i) x[i] = i * kThreads + t < n ? best[i * kThreads + t] : -INFINITY;
     Sums q{-INFINITY, 0.0f, 0.0f};
-    for (int c = t & 63; c < chunks; c += 64) q.m = fmaxf(q.m, w[(size_t)c * words]);
+    float4 part[2];  // every wave joins all chunks, at most 128
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int c = (t & 63) + 64 * i;
+        part[i] = c < chunks ? *(const float4 *)(w + 4 * c) : make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
+        q.m = fmaxf(q.m, part[i].x);
+    }
     q.m = wave_max(q.m);
-    for (int c = t & 63; c < chunks; c += 64) {  // every wave joins all chunks
-        const float m = w[(size_t)c * words], s = w[(size_t)c * words + 1], u = w[(size_t)c * words + 2];
-        if (m == -INFINITY && s == 0.0f) continue;  // nothing allowed in this chunk
-        const float d = m - q.m, f = __builtin_amdgcn_exp2f(d * 1.44269504088896341f);
-        q.s += f * s;
-        q.u += f == 0.0f ? 0.0f : f * (u + s * d);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        if (part[i].x == -INFINITY && part[i].y == 0.0f) continue;  // nothing allowed in this chunk
+        const float d = part[i].x - q.m, f = __builtin_amdgcn_exp2f(d * 1.44269504088896341f);
+        q.s += f * part[i].y;
+        q.u += f == 0.0f ? 0.0f : f * (part[i].z + part[i].y * d);
     }
     q.s = wave_sum(q.s);
     q.u = wave_sum(q.u);
     if (t == 0) finish_row<T>(a, r, q);
     if (a.top_k == 0) return;
-    // position c * k + j: equal values of a lower index come first, as chunks and ranks do
-    const int n = chunks * a.top_k;
-    float x[EPT];
-#pragma unroll
-    for (int i = 0; i < EPT; ++i) {
-        const int at = i * kThreads + t, c = at / a.top_k;
-        x[i] = at < n ? w[(size_t)c * words + 4 + (at - c * a.top_k)] : -INFINITY;
-    }
+    top_floor(x, a.top_k, lds);
+    __syncthreads();
     const int got = top_of<EPT, 1>(x, a.top_k, lds, [&](int rank, uint32_t key, int at) {
-        const int c = at / a.top_k;
-        a.top_ids[(size_t)r * a.top_k + rank] = ((const int *)w)[(size_t)c * words + 4 + a.top_k + (at - c * a.top_k)];
+        a.top_ids[(size_t)r * a.top_k + rank] = ((const int *)best)[n + at];
         a.top_lp[(size_t)r * a.top_k + rank] = alt_lp(a, q, key);
     });
     no_alternatives(a, r, got);
@@ -281,9 +301,8 @@ __global__ __launch_bounds__(kThreads) void logprobs_join_kernel(LogprobArgs a, 
 // Values a thread holds.
 int ept_of(int rows, int vocab) {
     if (vocab <= 4 * kThreads) return 4;
-    if ((long long)rows * ((vocab + 8 * kThreads - 1) / (8 * kThreads)) <= 1024 && (vocab + 8 * kThreads - 1) / (8 * kThreads) <= 128)
-        return 8;
-    return 32;
+    const int chunks8 = (vocab + 8 * kThreads - 1) / (8 * kThreads);
+    return chunks8 <= kMaxChunks && (long long)rows * chunks8 <= 4096 ? 8 : 32;
 }
 int chunks_of(int rows, int vocab) {
     const int n = ept_of(rows, vocab) * kThreads;
@@ -310,7 +329,10 @@ hipError_t logprobs_t(const LogprobArgs &a, hipStream_t s) {
         launch_chunks<T, 8>(a, chunks, s);
     else
         launch_chunks<T, 32>(a, chunks, s);
-    if (chunks > 1) hipLaunchKernelGGL((logprobs_join_kernel<T>), dim3(a.rows), dim3(kThreads), 0, s, a, chunks);
+    if (chunks > 1 && chunks * a.top_k <= 2 * kThreads)
+        hipLaunchKernelGGL((logprobs_join_kernel<T, 2>), dim3(a.rows), dim3(kThreads), 0, s, a, chunks);
+    else if (chunks > 1)
+        hipLaunchKernelGGL((logprobs_join_kernel<T, 16>), dim3(a.rows), dim3(kThreads), 0, s, a, chunks);
     return hipGetLastError();
 }
 
@@ -318,7 +340,7 @@ hipError_t logprobs_t(const LogprobArgs &a, hipStream_t s) {
 
 size_t logprobs_workspace(int rows, int vocab, int top_k) {
     const int chunks = chunks_of(rows, vocab);
-    return chunks == 1 ? 0 : (size_t)rows * chunks * chunk_words(top_k) * sizeof(float);
+    return chunks == 1 ? 0 : rows * row_words(chunks, top_k) * sizeof(float);
 }
 
 hipError_t launch_logprobs(const LogprobArgs &a, hipStream_t s) {

@@ -61,6 +61,31 @@ __device__ __forceinline__ void store_n(T *p, bool vec, const float (&x)[N]) {
     }
 }
 
+// V elements as they are: one 16-byte access where they fill one (p is then 16-byte aligned).
+template <class T, int V, class P>
+__device__ __forceinline__ P load_piece(const T *p) {
+    P x;
+    if constexpr (V * sizeof(T) == 16) {
+        const uint4 raw = *(const uint4 *)p;
+        __builtin_memcpy(&x, &raw, 16);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) x.e[i] = p[i];
+    }
+    return x;
+}
+template <class T, int V, class P>
+__device__ __forceinline__ void store_piece(T *p, const P &x) {
+    if constexpr (V * sizeof(T) == 16) {
+        uint4 raw;
+        __builtin_memcpy(&raw, &x, 16);
+        *(uint4 *)p = raw;
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) p[i] = x.e[i];
+    }
+}
+
 // cos and sin (times mscale) of position p at `w` radians a position.
 __device__ __forceinline__ float2 turn(int p, double w, float mscale) {
     const double t = (double)p * w * 0.15915494309189533577;  // turns
@@ -78,41 +103,71 @@ __device__ __forceinline__ void rotate(float a, float b, float2 cs, float &x, fl
 // what one thread turns at a time: V neighbouring elements of interleaved pairs, or V elements
 // and their V partners half a rotation further; then the V-element pieces behind rot.
 // Memory bound: every element is read and written once, in 16-byte pieces where base, strides
-// and (halves) rot / 2 allow it.
-template <class T, bool HALVES, int V>
+// and (halves) rot / 2 allow it, and a thread has N units' loads in flight, the first N before the
+// angles are formed.
+template <class T, bool HALVES, int V, int N>
 __global__ __launch_bounds__(kThreads) void rope_rows_kernel(RopeRowsArgs a, int rpb, int per_head) {
     extern __shared__ float2 cs[];  // [rpb][rot / 2]
+    struct Piece {
+        T e[V];
+    };
     const int half = a.rope.rot / 2, t = threadIdx.x;
     const int row0 = blockIdx.x * rpb, nrow = min(rpb, a.rows - row0);
+    const int per_row = a.heads * per_head, units = nrow * per_row, turned = HALVES ? half / V : per_head;
+    const int step = kThreads * gridDim.y;
+    constexpr int SIDES = HALVES ? 2 : 1;
+    Piece x[N][SIDES];
+    T *to[N];
+    int at[N], angle[N];  // first element (of the lower half), and where its angles are; -1: copied
+    auto load = [&](int u0) {
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int u = min(u0 + n * step, units - 1);
+            const int r = u / per_row, hu = u - r * per_row, h = hu / per_head, p = hu - h * per_head;
+            const T *from = (const T *)a.x + (row0 + r) * a.x_row + h * a.x_head;
+            to[n] = (T *)a.y + (row0 + r) * a.y_row + h * a.y_head;
+            const bool turn_it = HALVES ? p < turned : p * V < 2 * half;
+            at[n] = HALVES && !turn_it ? 2 * half + (p - turned) * V : p * V;
+            angle[n] = turn_it ? r * half + (HALVES ? p * V : p * V / 2) : -1;
+            x[n][0] = load_piece<T, V, Piece>(from + at[n]);
+            if (HALVES) x[n][SIDES - 1] = load_piece<T, V, Piece>(from + (turn_it ? half + at[n] : at[n]));
+        }
+    };
+    const int first = blockIdx.y * kThreads + t;
+    load(first);
     for (int i = t; i < nrow * half; i += kThreads) {
         const int r = i / half;
         cs[i] = turn(a.pos[row0 + r], a.rope.freqs[i - r * half], a.rope.mscale);
     }
     __syncthreads();
-    const int units = a.heads * per_head, turned = HALVES ? half / V : per_head;
-    for (int u = blockIdx.y * kThreads + t; u < nrow * units; u += kThreads * gridDim.y) {
-        const int r = u / units, hu = u - r * units, h = hu / per_head, p = hu - h * per_head;
-        const T *x = (const T *)a.x + (row0 + r) * a.x_row + h * a.x_head;
-        T *y = (T *)a.y + (row0 + r) * a.y_row + h * a.y_head;
-        const float2 *c = cs + r * half;
-        if (HALVES && p < turned) {
-            float lo[V], hi[V];
-            load_n<T, V>(x + p * V, true, lo);
-            load_n<T, V>(x + half + p * V, true, hi);
+    for (int u0 = first; u0 < units; u0 += N * step) {
+        if (u0 != first) load(u0);
 #pragma unroll
-            for (int i = 0; i < V; ++i) rotate(lo[i], hi[i], c[p * V + i], lo[i], hi[i]);
-            store_n<T, V>(y + p * V, true, lo);
-            store_n<T, V>(y + half + p * V, true, hi);
-        } else {
-            const int e = HALVES ? 2 * half + (p - turned) * V : p * V;
-            float v[V];
-            load_n<T, V>(x + e, true, v);
-            if constexpr (!HALVES) {
+        for (int n = 0; n < N; ++n) {
+            if (u0 + n * step >= units) break;
+            if (angle[n] >= 0) {
+                const float2 *c = cs + angle[n];
+                if constexpr (HALVES) {
 #pragma unroll
-                for (int i = 0; i < V; i += 2)
-                    if (e + i < 2 * half) rotate(v[i], v[i + 1], c[(e + i) / 2], v[i], v[i + 1]);
+                    for (int i = 0; i < V; ++i) {
+                        float lo, hi;
+                        rotate(Elem<T>::get(x[n][0].e[i]), Elem<T>::get(x[n][SIDES - 1].e[i]), c[i], lo, hi);
+                        x[n][0].e[i] = Elem<T>::put(lo);
+                        x[n][SIDES - 1].e[i] = Elem<T>::put(hi);
+                    }
+                    store_piece<T, V>(to[n] + half + at[n], x[n][SIDES - 1]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < V; i += 2)
+                        if (at[n] + i < 2 * half) {
+                            float lo, hi;
+                            rotate(Elem<T>::get(x[n][0].e[i]), Elem<T>::get(x[n][0].e[i + 1]), c[i / 2], lo, hi);
+                            x[n][0].e[i] = Elem<T>::put(lo);
+                            x[n][0].e[i + 1] = Elem<T>::put(hi);
+                        }
+                }
             }
-            store_n<T, V>(y + e, true, v);
+            store_piece<T, V>(to[n] + at[n], x[n][0]);
         }
     }
 }
@@ -121,13 +176,19 @@ template <class T, bool HALVES, int V>
 hipError_t rope_rows(const RopeRowsArgs &a, hipStream_t s) {
     const int half = a.rope.rot / 2;
     const int per_head = HALVES ? half / V + (a.dim - a.rope.rot) / V : a.dim / V;
-    const long long units = (long long)a.heads * per_head;
-    const int rpb = units >= kThreads ? 1 : (int)std::min<long long>(kThreads / units, 16);
-    const int blocks = (a.rows + rpb - 1) / rpb;
-    const int split = rpb == 1 && a.rows < 512 ? (int)std::min<long long>((units + kThreads - 1) / kThreads, 64) : 1;
+    const int units = a.heads * per_head;
     (void)hipGetLastError();
-    hipLaunchKernelGGL((rope_rows_kernel<T, HALVES, V>), dim3(blocks, split), dim3(kThreads), rpb * half * sizeof(float2), s, a,
-                       rpb, per_head);
+    // 4 units a thread once that leaves 1024 workgroups
+    const int rpb4 = std::min(std::max(1, 4 * kThreads / units), 16);
+    if ((a.rows + rpb4 - 1) / rpb4 >= 1024) {
+        hipLaunchKernelGGL((rope_rows_kernel<T, HALVES, V, 4>), dim3((a.rows + rpb4 - 1) / rpb4), dim3(kThreads),
+                           rpb4 * half * sizeof(float2), s, a, rpb4, per_head);
+        return hipGetLastError();
+    }
+    const int rpb = std::min(std::max(1, kThreads / units), 16);
+    const int split = a.rows < 512 ? std::min((units + kThreads - 1) / kThreads, 64) : 1;
+    hipLaunchKernelGGL((rope_rows_kernel<T, HALVES, V, 1>), dim3((a.rows + rpb - 1) / rpb, split), dim3(kThreads),
+                       rpb * half * sizeof(float2), s, a, rpb, per_head);
     return hipGetLastError();
 }
 
@@ -179,14 +240,17 @@ __device__ __forceinline__ uint32_t group_max(uint32_t v) {
 // the scale NaN and reads back as NaN, as quantising it would otherwise hide it.  The maximum is
 // taken over the magnitudes' bit patterns, in which Inf and NaN are largest.
 // Memory bound; the rotation of the keys is done here so that they do not go through memory twice.
-template <class T, int KV, int D>
+// A thread has N units (8 elements of K or V of one head) in flight at a time.
+template <class T, int KV, int D, int N>
 __global__ __launch_bounds__(kThreads) void kv_write_kernel(KvRowsArgs a, int rpb, bool vec) {
     extern __shared__ float2 cs[];  // [rpb][rot / 2]
     constexpr int L = D / 8;
     const int t = threadIdx.x, l = t % L;
     const int row0 = blockIdx.x * rpb, nrow = min(rpb, a.rows - row0);
     const int half = a.rope.rot / 2, heads = a.c.heads;
-    if (a.rope.freqs != nullptr) {
+    const bool rope = a.rope.freqs != nullptr;
+    const int per_row = 2 * heads * L, units = nrow * per_row;  // K then V
+    if (rope) {
         const int *pos = a.rope_pos != nullptr ? a.rope_pos : a.pos;
         for (int i = t; i < nrow * half; i += kThreads) {
             const int r = i / half;
@@ -194,69 +258,94 @@ __global__ __launch_bounds__(kThreads) void kv_write_kernel(KvRowsArgs a, int rp
         }
         __syncthreads();
     }
-    const int units = 2 * heads * L;  // K then V
-    for (int u = t; u < nrow * units; u += kThreads) {
-        const int rl = u / units, g = (u - rl * units) / L, r = row0 + rl;
-        const bool is_v = g >= heads;
-        const int h = is_v ? g - heads : g;
-        const T *src = (is_v ? (const T *)a.v + r * a.v_row : (const T *)a.k + r * a.k_row) + h * D;
-        float x[8];
-        load_n<T, 8>(src + 8 * l, vec, x);
-        const Place at = place_of(a.c, a.stream[r], a.pos[r]);
-        if (!is_v && a.rope.freqs != nullptr) {
-            const float2 *c = cs + rl * half;
-            if (a.rope.halves) {
+    for (int u0 = t; u0 < units; u0 += N * kThreads) {
+        float x[N][8];
+        const T *src[N];
+        size_t vecs[N];
+        int row[N];
+        bool is_v[N], ok[N];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int e = 8 * l + i;
-                    if (e < 2 * half) {
-                        const bool up = e >= half;
-                        const float b = Elem<T>::get(src[up ? e - half : e + half]);
-                        const float2 w = c[up ? e - half : e];
-                        x[i] = up ? x[i] * w.x + b * w.y : x[i] * w.x - b * w.y;
-                    }
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; i += 2)
-                    if (8 * l + i < 2 * half) rotate(x[i], x[i + 1], c[4 * l + i / 2], x[i], x[i + 1]);
-            }
+        for (int n = 0; n < N; ++n) {  // (a unit past the last is the last, and not written: groups are whole)
+            const int u = u0 + n * kThreads < units ? u0 + n * kThreads : units - L + l;
+            row[n] = u / per_row;
+            const int g = (u - row[n] * per_row) / L, r = row0 + row[n];
+            is_v[n] = g >= heads;
+            const int h = is_v[n] ? g - heads : g;
+            src[n] = (is_v[n] ? (const T *)a.v + r * a.v_row : (const T *)a.k + r * a.k_row) + h * D;
+            load_n<T, 8>(src[n] + 8 * l, vec, x[n]);
+            const Place at = place_of(a.c, a.stream[r], a.pos[r]);
+            vecs[n] = at.at + (size_t)h * a.c.page_size;
+            ok[n] = at.ok && u0 + n * kThreads < units;
         }
-        const size_t vecs = at.at + (size_t)h * a.c.page_size;
-        const size_t o = vecs * D + 8 * l;
-        void *pool = is_v ? a.c.v : a.c.k;
-        if constexpr (KV == ELEM_F32) {
-            if (at.ok) store_n<float, 8>((float *)pool + o, true, x);
-        } else if constexpr (KV == ELEM_F16) {
-            if (at.ok) store_n<__half, 8>((__half *)pool + o, true, x);
-        } else {
-            constexpr float top = KV == ELEM_I8 ? 127.0f : 448.0f;
-            uint32_t mb = 0;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) mb = max(mb, __float_as_uint(x[i]) & 0x7fffffffu);
-            mb = group_max<L>(mb);
-            const bool bad = mb >= 0x7f800000u;
-            float d = __uint_as_float(mb) / top;
-            if (bad || d < 1.17549435e-38f) d = 0.0f;
-            const float id = d > 0.0f ? 1.0f / d : 0.0f;
-            uint32_t w[2] = {0, 0};
-            if (!bad) {
+        for (int n = 0; n < N; ++n) {
+            if (rope && !is_v[n]) {
+                const float2 *c = cs + row[n] * half;
+                if (a.rope.halves && half % 8 == 0) {
+                    if (8 * l < 2 * half) {  // the partners are the 8 elements half a rotation away
+                        const bool up = 8 * l >= half;
+                        const int e = up ? 8 * l - half : 8 * l;
+                        float b[8];
+                        load_n<T, 8>(src[n] + (up ? e : e + half), vec, b);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) x[i] = fminf(fmaxf(x[i] * id, -top), top);
-                if constexpr (KV == ELEM_I8) {
+                        for (int i = 0; i < 8; ++i) {
+                            const float2 w = c[e + i];
+                            x[n][i] = x[n][i] * w.x + (up ? b[i] : -b[i]) * w.y;
+                        }
+                    }
+                } else if (a.rope.halves) {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) w[i / 4] |= ((uint32_t)(int)rintf(x[i]) & 0xffu) << (8 * (i & 3));
+                    for (int i = 0; i < 8; ++i) {
+                        const int e = 8 * l + i;
+                        if (e < 2 * half) {
+                            const bool up = e >= half;
+                            const float b = Elem<T>::get(src[n][up ? e - half : e + half]);
+                            const float2 w = c[up ? e - half : e];
+                            x[n][i] = x[n][i] * w.x + (up ? b : -b) * w.y;
+                        }
+                    }
                 } else {
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        int p = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i], x[4 * i + 1], 0, false);
-                        w[i] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i + 2], x[4 * i + 3], p, true);
-                    }
+                    for (int i = 0; i < 8; i += 2)
+                        if (8 * l + i < 2 * half) rotate(x[n][i], x[n][i + 1], c[4 * l + i / 2], x[n][i], x[n][i + 1]);
                 }
             }
-            if (at.ok) {
-                *(uint2 *)((uint8_t *)pool + o) = make_uint2(w[0], w[1]);
-                if (l == 0) (is_v ? a.c.v_scale : a.c.k_scale)[vecs] = bad ? __uint_as_float(0x7fc00000u) : d;
+            const size_t o = vecs[n] * D + 8 * l;
+            void *pool = is_v[n] ? a.c.v : a.c.k;
+            if constexpr (KV == ELEM_F32) {
+                if (ok[n]) store_n<float, 8>((float *)pool + o, true, x[n]);
+            } else if constexpr (KV == ELEM_F16) {
+                if (ok[n]) store_n<__half, 8>((__half *)pool + o, true, x[n]);
+            } else {
+                constexpr float top = KV == ELEM_I8 ? 127.0f : 448.0f;
+                uint32_t mb = 0;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) mb = max(mb, __float_as_uint(x[n][i]) & 0x7fffffffu);
+                mb = group_max<L>(mb);
+                const bool bad = mb >= 0x7f800000u;
+                float d = __uint_as_float(mb) / top;
+                if (bad || d < 1.17549435e-38f) d = 0.0f;
+                const float id = d > 0.0f ? 1.0f / d : 0.0f;
+                uint32_t w[2] = {0, 0};
+                if (!bad) {
+                    float *y = x[n];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) y[i] = fminf(fmaxf(y[i] * id, -top), top);
+                    if constexpr (KV == ELEM_I8) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) w[i / 4] |= ((uint32_t)(int)rintf(y[i]) & 0xffu) << (8 * (i & 3));
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const int p = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * i], y[4 * i + 1], 0, false);
+                            w[i] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[4 * i + 2], y[4 * i + 3], p, true);
+                        }
+                    }
+                }
+                if (ok[n]) {
+                    *(uint2 *)((uint8_t *)pool + o) = make_uint2(w[0], w[1]);
+                    if (l == 0) (is_v[n] ? a.c.v_scale : a.c.k_scale)[vecs[n]] = bad ? __uint_as_float(0x7fc00000u) : d;
+                }
             }
         }
     }
@@ -264,50 +353,72 @@ __global__ __launch_bounds__(kThreads) void kv_write_kernel(KvRowsArgs a, int rp
 
 // Rows out of the pools: q d in 32 bits, rounded once to the output's type.  Rows with no place in
 // the cache (a position past the table, a page outside the pools) are NaN; a negative position is
-// padding and its row stays as it was.
-template <class T, int KV, int D>
+// padding and its row stays as it was.  N units of a thread in flight, as in the write.
+template <class T, int KV, int D, int N>
 __global__ __launch_bounds__(kThreads) void kv_read_kernel(KvRowsArgs a, int rpb, bool vec) {
     constexpr int L = D / 8;
-    const int units = 2 * a.c.heads * L, row0 = blockIdx.x * rpb, nrow = min(rpb, a.rows - row0);
-    for (int u = threadIdx.x; u < nrow * units; u += kThreads) {
-        const int rl = u / units, rest = u - rl * units, g = rest / L, l = rest - g * L, r = row0 + rl;
-        const bool is_v = g >= a.c.heads;
-        const int h = is_v ? g - a.c.heads : g;
-        const int pos = a.pos[r];
-        if (pos < 0) continue;
-        const Place at = place_of(a.c, a.stream[r], pos);
-        float x[8];
-        if (at.ok) {
-            const size_t vecs = at.at + (size_t)h * a.c.page_size;
-            const size_t o = vecs * D + 8 * l;
-            const void *pool = is_v ? a.c.v : a.c.k;
-            if constexpr (KV == ELEM_F32) {
-                load_n<float, 8>((const float *)pool + o, true, x);
-            } else if constexpr (KV == ELEM_F16) {
-                load_n<__half, 8>((const __half *)pool + o, true, x);
+    constexpr int RAW = KV == ELEM_F32 ? 32 : (KV == ELEM_F16 ? 16 : 8);  // bytes of a unit
+    const int row0 = blockIdx.x * rpb, nrow = min(rpb, a.rows - row0);
+    const int per_row = 2 * a.c.heads * L, units = nrow * per_row;
+    for (int u0 = threadIdx.x; u0 < units; u0 += N * kThreads) {
+        T *dst[N];
+        size_t vecs[N];
+        bool is_v[N], ok[N], put[N];
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int u = min(u0 + n * kThreads, units - 1);
+            const int rl = u / per_row, rest = u - rl * per_row, g = rest / L, l = rest - g * L, r = row0 + rl;
+            is_v[n] = g >= a.c.heads;
+            const int h = is_v[n] ? g - a.c.heads : g, pos = a.pos[r];
+            const Place at = place_of(a.c, a.stream[r], pos);
+            ok[n] = at.ok;
+            put[n] = pos >= 0 && u0 + n * kThreads < units;
+            vecs[n] = at.ok ? at.at + (size_t)h * a.c.page_size : 0;  // (0: any vector that exists)
+            dst[n] = (is_v[n] ? (T *)a.v_out + r * a.v_row : (T *)a.k_out + r * a.k_row) + h * D + 8 * l;
+        }
+        const int l = threadIdx.x % L;
+        uint4 raw[N][RAW > 16 ? 2 : 1];
+        float d[N];
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const char *p = (const char *)(is_v[n] ? a.c.v : a.c.k) + (vecs[n] * D + 8 * l) * elem_size(KV);
+            if constexpr (RAW == 8) {
+                const uint2 w = *(const uint2 *)p;
+                raw[n][0] = make_uint4(w.x, w.y, 0, 0);
+                d[n] = (is_v[n] ? a.c.v_scale : a.c.k_scale)[vecs[n]];
             } else {
-                const uint2 w = *(const uint2 *)((const uint8_t *)pool + o);
-                const float d = (is_v ? a.c.v_scale : a.c.k_scale)[vecs];
-                const uint32_t ww[2] = {w.x, w.y};
-    #pragma unroll
+#pragma unroll
+                for (int i = 0; i < RAW / 16; ++i) raw[n][i] = ((const uint4 *)p)[i];
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            float x[8];
+            if constexpr (KV == ELEM_F32) {
+                __builtin_memcpy(x, raw[n], 32);
+            } else if constexpr (KV == ELEM_F16) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[i] = __half2float(((const __half *)raw[n])[i]);
+            } else {
+                const uint32_t w[2] = {raw[n][0].x, raw[n][0].y};
+#pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     if constexpr (KV == ELEM_I8) {
-    #pragma unroll
-                        for (int j = 0; j < 4; ++j) x[4 * i + j] = (float)(int8_t)(ww[i] >> (8 * j)) * d;
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) x[4 * i + j] = (float)(int8_t)(w[i] >> (8 * j)) * d[n];
                     } else {
-                        x[4 * i] = __builtin_amdgcn_cvt_f32_fp8((int)ww[i], 0) * d;
-                        x[4 * i + 1] = __builtin_amdgcn_cvt_f32_fp8((int)ww[i], 1) * d;
-                        x[4 * i + 2] = __builtin_amdgcn_cvt_f32_fp8((int)ww[i], 2) * d;
-                        x[4 * i + 3] = __builtin_amdgcn_cvt_f32_fp8((int)ww[i], 3) * d;
+                        x[4 * i] = __builtin_amdgcn_cvt_f32_fp8((int)w[i], 0) * d[n];
+                        x[4 * i + 1] = __builtin_amdgcn_cvt_f32_fp8((int)w[i], 1) * d[n];
+                        x[4 * i + 2] = __builtin_amdgcn_cvt_f32_fp8((int)w[i], 2) * d[n];
+                        x[4 * i + 3] = __builtin_amdgcn_cvt_f32_fp8((int)w[i], 3) * d[n];
                     }
                 }
             }
-        } else {
-    #pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(0x7fc00000u);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (!ok[n]) x[i] = __uint_as_float(0x7fc00000u);
+            if (put[n]) store_n<T, 8>(dst[n], vec, x);
         }
-        T *dst = (is_v ? (T *)a.v_out + r * a.v_row : (T *)a.k_out + r * a.k_row) + h * D;
-        store_n<T, 8>(dst + 8 * l, vec, x);
     }
 }
 
@@ -317,34 +428,36 @@ bool rows_vec(const void *k, const void *v, int64_t k_row, int64_t v_row) {
     return ((uintptr_t)k | (uintptr_t)v) % 16 == 0 && k_row % V == 0 && v_row % V == 0;
 }
 
-template <class T, int KV, int D>
-hipError_t kv_write(const KvRowsArgs &a, hipStream_t s) {
-    const int units = 2 * a.c.heads * (D / 8);
-    const int rpb = units >= kThreads ? 1 : kThreads / units;
+// 4 units a thread once that leaves 512 workgroups, else one (a step's few rows).
+template <class T, bool READ, int KV, int D>
+hipError_t kv_launch(const KvRowsArgs &a, hipStream_t s) {
+    const int units = 2 * a.c.heads * (D / 8), rpb4 = std::max(1, 4 * kThreads / units), blocks4 = (a.rows + rpb4 - 1) / rpb4;
+    const bool four = blocks4 >= 512;
+    const int rpb = four ? rpb4 : std::max(1, kThreads / units), blocks = (a.rows + rpb - 1) / rpb;
     const size_t lds = a.rope.freqs ? (size_t)rpb * (a.rope.rot / 2) * sizeof(float2) : 0;
+    const bool vec = READ ? rows_vec<T>(a.k_out, a.v_out, a.k_row, a.v_row) : rows_vec<T>(a.k, a.v, a.k_row, a.v_row);
     (void)hipGetLastError();
-    hipLaunchKernelGGL((kv_write_kernel<T, KV, D>), dim3((a.rows + rpb - 1) / rpb), dim3(kThreads), lds, s, a, rpb,
-                       rows_vec<T>(a.k, a.v, a.k_row, a.v_row));
-    return hipGetLastError();
-}
-
-template <class T, int KV, int D>
-hipError_t kv_read(const KvRowsArgs &a, hipStream_t s) {
-    const int units = 2 * a.c.heads * (D / 8);
-    const int rpb = units >= kThreads ? 1 : kThreads / units;
-    (void)hipGetLastError();
-    hipLaunchKernelGGL((kv_read_kernel<T, KV, D>), dim3((a.rows + rpb - 1) / rpb), dim3(kThreads), 0, s, a, rpb,
-                       rows_vec<T>(a.k_out, a.v_out, a.k_row, a.v_row));
+    if constexpr (READ) {
+        if (four)
+            hipLaunchKernelGGL((kv_read_kernel<T, KV, D, 4>), dim3(blocks), dim3(kThreads), 0, s, a, rpb, vec);
+        else
+            hipLaunchKernelGGL((kv_read_kernel<T, KV, D, 1>), dim3(blocks), dim3(kThreads), 0, s, a, rpb, vec);
+    } else {
+        if (four)
+            hipLaunchKernelGGL((kv_write_kernel<T, KV, D, 4>), dim3(blocks), dim3(kThreads), lds, s, a, rpb, vec);
+        else
+            hipLaunchKernelGGL((kv_write_kernel<T, KV, D, 1>), dim3(blocks), dim3(kThreads), lds, s, a, rpb, vec);
+    }
     return hipGetLastError();
 }
 
 template <class T, bool READ, int D>
 hipError_t kv_rows_d(const KvRowsArgs &a, hipStream_t s) {
     switch (a.c.dtype) {
-        case ELEM_F32: return READ ? kv_read<T, ELEM_F32, D>(a, s) : kv_write<T, ELEM_F32, D>(a, s);
-        case ELEM_F16: return READ ? kv_read<T, ELEM_F16, D>(a, s) : kv_write<T, ELEM_F16, D>(a, s);
-        case ELEM_I8: return READ ? kv_read<T, ELEM_I8, D>(a, s) : kv_write<T, ELEM_I8, D>(a, s);
-        default: return READ ? kv_read<T, ELEM_E4M3, D>(a, s) : kv_write<T, ELEM_E4M3, D>(a, s);
+        case ELEM_F32: return kv_launch<T, READ, ELEM_F32, D>(a, s);
+        case ELEM_F16: return kv_launch<T, READ, ELEM_F16, D>(a, s);
+        case ELEM_I8: return kv_launch<T, READ, ELEM_I8, D>(a, s);
+        default: return kv_launch<T, READ, ELEM_E4M3, D>(a, s);
     }
 }
 

@@ -277,37 +277,49 @@ def _whole(name, t, dtype, shape, device, optional=False):
     """The address of a contiguous tensor of this type and shape on this device (None: NULL)."""
     if t is None and optional:
         return None
-    if t.dtype != dtype or t.device != device or tuple(t.shape) != shape or not t.is_contiguous():
-        raise ValueError(f"{name}: a contiguous {dtype} tensor of shape {shape} on {device} is wanted, "
+    if t.dtype != dtype or t.shape != shape or t.device != device or not t.is_contiguous():
+        raise ValueError(f"{name}: a contiguous {dtype} tensor of shape {tuple(shape)} on {device} is wanted, "
                          f"not {t.dtype} {tuple(t.shape)} on {t.device}")
     return t.data_ptr()
 
 
-def _here(device):
-    """The calls launch on the current device: tensors of another one are refused."""
+def _on(device, stream):
+    """The stream to launch on: the caller's handle, or torch's current one.  The calls launch on the current device:
+    tensors of another one are refused.  (torch.cuda.current_stream() builds an object for 2.9 us, the call of its
+    handle takes 0.1: of a small operator's 10 us in all.)"""
     import torch
     if device.type != "cuda":
         raise ValueError(f"tensors on the GPU are wanted, not on {device}")
     if device.index != torch.cuda.current_device():
         raise ValueError(f"the tensors are on {device}, the current device is cuda:{torch.cuda.current_device()}")
+    if stream is not None:
+        return stream
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return raw(device.index) if raw is not None else torch.cuda.current_stream().cuda_stream
 
 
 def _rows(name, t, heads, dim, device):
     """(address, row stride) of rows [rows][heads][dim] (or [rows][heads * dim]) whose rows are contiguous."""
-    if t.device != device or t.numel() != t.shape[0] * heads * dim:
-        raise ValueError(f"{name}: [rows][{heads}][{dim}] on {device} is wanted, not {tuple(t.shape)} on {t.device}")
-    inner = t.stride()[1:] == ((dim, 1) if t.dim() == 3 else (1,))
-    if not (t.dim() in (2, 3) and (t.dim() == 2 or t.shape[1] == heads) and (inner or t.numel() == 0)):
+    shape, st = t.shape, t.stride()
+    if len(shape) == 3:
+        fits, whole = shape[1] == heads and shape[2] == dim, st[2] == 1 and (st[1] == dim or heads == 1)
+    else:
+        fits, whole = len(shape) == 2 and shape[1] == heads * dim, st[-1] == 1
+    if not fits or t.device != device:
+        raise ValueError(f"{name}: [rows][{heads}][{dim}] on {device} is wanted, not {tuple(shape)} on {t.device}")
+    if not whole:
         raise ValueError(f"{name}: the heads of a row must be contiguous")
-    return t.data_ptr(), t.stride(0)
+    return t.data_ptr(), st[0]
 
 
-def _workspace(given, size, device, stream):
-    """(address, bytes): the caller's, or a new one from torch's allocator, which is safe on the current stream."""
+def _workspace(given, size_of, device, stream):
+    """(address, bytes): the caller's (the call checks that it is large enough), or a new one from torch's allocator,
+    which is safe on torch's current stream."""
     import torch
-    if size == 0:
-        return None, 0
     if given is None:
+        size = size_of()
+        if size == 0:
+            return None, 0
         if stream is not None and stream != torch.cuda.current_stream().cuda_stream:
             raise ValueError("on a stream other than torch's current one, pass a workspace")
         given = torch.empty(size, dtype=torch.uint8, device=device)
@@ -370,18 +382,18 @@ def rope_rows(x, pos, rope: Rope, out=None, stream=None):
     out (x itself by default); returns out."""
     import torch
     out = x if out is None else out
-    dev = x.device
-    _here(dev)
-    if x.dim() != 3 or out.shape != x.shape or out.dtype != x.dtype or out.device != dev or rope.device != dev:
+    dev, shape = x.device, x.shape
+    on = _on(dev, stream)
+    if len(shape) != 3 or out.shape != shape or out.dtype != x.dtype or out.device != dev or rope.device != dev:
         raise ValueError("x and out must be [rows][heads][head_dim] of one type, on one device with the rotation")
-    if x.numel() == 0:
+    rows, heads, dim = shape
+    if rows * heads * dim == 0:
         return out
-    if x.stride(2) != 1 or out.stride(2) != 1:
+    xs, os_ = x.stride(), out.stride()
+    if xs[2] != 1 or os_[2] != 1:
         raise ValueError("the elements of a head must be contiguous")
-    rows, heads, dim = x.shape
-    check(load().moss_hip_rope_rows(x.data_ptr(), x.stride(0), x.stride(1), out.data_ptr(), out.stride(0), out.stride(1),
-                                    _types(x), rows, heads, dim, _whole("pos", pos, torch.int32, (rows,), dev), rope.ref,
-                                    _stream(stream)))
+    check(load().moss_hip_rope_rows(x.data_ptr(), xs[0], xs[1], out.data_ptr(), os_[0], os_[1], _types(x), rows, heads, dim,
+                                    _whole("pos", pos, torch.int32, (rows,), dev), rope.ref, on))
     return out
 
 
@@ -390,7 +402,7 @@ def kv_write(cache: KVCache, k, v, row_stream, row_pos, rope: Rope | None = None
     by `rope` at rope_pos (row_pos by default)."""
     import torch
     dev, n = cache.device, k.shape[0]
-    _here(dev)
+    on = _on(dev, stream)
     if v.shape[0] != n or v.dtype != k.dtype or (rope is not None and rope.device != dev):
         raise ValueError("k and v must have the same rows and type, and the rotation their device")
     if n == 0:
@@ -401,14 +413,14 @@ def kv_write(cache: KVCache, k, v, row_stream, row_pos, rope: Rope | None = None
                                    _whole("row_stream", row_stream, torch.int32, (n,), dev),
                                    _whole("row_pos", row_pos, torch.int32, (n,), dev),
                                    None if rope is None else rope.ref,
-                                   _whole("rope_pos", rope_pos, torch.int32, (n,), dev, optional=True), _stream(stream)))
+                                   _whole("rope_pos", rope_pos, torch.int32, (n,), dev, optional=True), on))
 
 
 def kv_read(cache: KVCache, row_stream, row_pos, k, v, stream=None) -> None:
     """moss_hip_kv_read: those rows back, into k, v [rows][kv_heads][head_dim]."""
     import torch
     dev, n = cache.device, k.shape[0]
-    _here(dev)
+    on = _on(dev, stream)
     if v.shape[0] != n or v.dtype != k.dtype:
         raise ValueError("k and v must have the same rows and type")
     if n == 0:
@@ -416,8 +428,7 @@ def kv_read(cache: KVCache, row_stream, row_pos, k, v, stream=None) -> None:
     kp, ks = _rows("k", k, cache.kv_heads, cache.head_dim, dev)
     vp, vs = _rows("v", v, cache.kv_heads, cache.head_dim, dev)
     check(load().moss_hip_kv_read(cache.ref, _whole("row_stream", row_stream, torch.int32, (n,), dev),
-                                  _whole("row_pos", row_pos, torch.int32, (n,), dev), n, kp, ks, vp, vs, _types(k),
-                                  _stream(stream)))
+                                  _whole("row_pos", row_pos, torch.int32, (n,), dev), n, kp, ks, vp, vs, _types(k), on))
 
 
 def attn_tree_workspace(cache: KVCache, heads: int, rows: int, max_rows: int, max_keys: int) -> int:
@@ -435,7 +446,7 @@ def attn_tree(q, cache: KVCache, row_start, ctx_len, out, max_rows: int, max_key
     stream), None: a chain; scale: head_dim ** -0.5 by default; lse [rows][heads] float32 or None."""
     import torch
     dev, dim = cache.device, cache.head_dim
-    _here(dev)
+    on = _on(dev, stream)
     rows = q.shape[0]
     heads = q.shape[1] if q.dim() == 3 else q.shape[1] // dim
     if out.shape[0] != rows:
@@ -444,14 +455,13 @@ def attn_tree(q, cache: KVCache, row_start, ctx_len, out, max_rows: int, max_key
         return
     qp, qs = _rows("q", q, heads, dim, dev)
     op, os_ = _rows("out", out, heads, dim, dev)
-    wp, wb = _workspace(workspace, attn_tree_workspace(cache, heads, rows, max_rows, max_keys), dev, stream)
+    wp, wb = _workspace(workspace, lambda: attn_tree_workspace(cache, heads, rows, max_rows, max_keys), dev, stream)
     check(load().moss_hip_attn_tree(qp, qs, _types(q), heads, cache.ref,
                                     _whole("row_start", row_start, torch.int32, (cache.streams + 1,), dev),
                                     _whole("ctx_len", ctx_len, torch.int32, (cache.streams,), dev),
                                     _whole("row_mask", row_mask, torch.int64, (rows,), dev, optional=True), rows, max_rows,
                                     max_keys, dim ** -0.5 if scale is None else scale, op, os_, _types(out),
-                                    _whole("lse", lse, torch.float32, (rows, heads), dev, optional=True), wp, wb,
-                                    _stream(stream)))
+                                    _whole("lse", lse, torch.float32, (rows, heads), dev, optional=True), wp, wb, on))
 
 
 def token_logprobs_workspace(rows: int, vocab: int, top_k: int) -> int:
@@ -466,11 +476,11 @@ def token_logprobs(logits, tokens, logprob, entropy=None, top_ids=None, top_logp
     """moss_hip_token_logprobs: of tokens [rows] int32 under logits [rows][vocab] (float32 or float16, any row stride), into
     logprob and entropy [rows] and the alternatives top_ids (int32), top_logprobs [rows][top_k]."""
     import torch
-    dev = logits.device
-    _here(dev)
-    if logits.dim() != 2:
+    dev, shape = logits.device, logits.shape
+    on = _on(dev, stream)
+    if len(shape) != 2:
         raise ValueError("logits [rows][vocab] are wanted")
-    rows, vocab = logits.shape
+    rows, vocab = shape
     k = 0 if top_ids is None else top_ids.shape[1]
     if (top_ids is None) != (top_logprobs is None):
         raise ValueError("top_ids and top_logprobs come together")
@@ -478,14 +488,14 @@ def token_logprobs(logits, tokens, logprob, entropy=None, top_ids=None, top_logp
         return
     if vocab > 1 and logits.stride(1) != 1:
         raise ValueError("the logits of a row must be contiguous")
-    wp, wb = _workspace(workspace, token_logprobs_workspace(rows, vocab, k), dev, stream)
+    wp, wb = _workspace(workspace, lambda: token_logprobs_workspace(rows, vocab, k), dev, stream)
     check(load().moss_hip_token_logprobs(logits.data_ptr(), logits.stride(0), _types(logits), rows, vocab,
                                          _whole("tokens", tokens, torch.int32, (rows,), dev), inv_temperature,
                                          _whole("logprob", logprob, torch.float32, (rows,), dev),
                                          _whole("entropy", entropy, torch.float32, (rows,), dev, optional=True), k,
                                          _whole("top_ids", top_ids, torch.int32, (rows, k), dev, optional=True),
                                          _whole("top_logprobs", top_logprobs, torch.float32, (rows, k), dev, optional=True),
-                                         wp, wb, _stream(stream)))
+                                         wp, wb, on))
 
 
 # ---------------------------------------------------------------- model
