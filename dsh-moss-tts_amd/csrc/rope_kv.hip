@@ -30,56 +30,47 @@ struct Elem<__half> {
     static __device__ __forceinline__ __half put(float x) { return __float2half_rn(x); }
 };
 
-// N elements at p as 32-bit floats: 16-byte accesses where `vec` (p is then 16-byte aligned),
-// one element at a time elsewhere.
-template <class T, int N>
-__device__ __forceinline__ void load_n(const T *p, bool vec, float (&x)[N]) {
-    constexpr int B = N * (int)sizeof(T);
-    if (B % 16 == 0 && vec) {
-        uint4 raw[B / 16 ? B / 16 : 1];
+// Memory is read and written 16 bytes at a time at any address that an element may have (the hardware takes
+// them unaligned).
+
+// 8 values to p.
+template <class T>
+__device__ __forceinline__ void store8(T *p, const float (&x)[8]) {
+    uint32_t w[2 * sizeof(T)];  // (words: from an array of halves the compiler makes 2-byte stores)
 #pragma unroll
-        for (int i = 0; i < B / 16; ++i) raw[i] = ((const uint4 *)p)[i];
-#pragma unroll
-        for (int i = 0; i < N; ++i) x[i] = Elem<T>::get(((const T *)raw)[i]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i) x[i] = Elem<T>::get(p[i]);
+    for (int i = 0; i < 2 * (int)sizeof(T); ++i) {
+        if constexpr (sizeof(T) == 2)
+            w[i] = (uint32_t)f2h(x[2 * i]) | (uint32_t)f2h(x[2 * i + 1]) << 16;
+        else
+            w[i] = __float_as_uint(x[i]);
     }
-}
-template <class T, int N>
-__device__ __forceinline__ void store_n(T *p, bool vec, const float (&x)[N]) {
-    constexpr int B = N * (int)sizeof(T);
-    if (B % 16 == 0 && vec) {
-        uint4 raw[B / 16 ? B / 16 : 1];
-#pragma unroll
-        for (int i = 0; i < N; ++i) ((T *)raw)[i] = Elem<T>::put(x[i]);
-#pragma unroll
-        for (int i = 0; i < B / 16; ++i) ((uint4 *)p)[i] = raw[i];
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i) p[i] = Elem<T>::put(x[i]);
-    }
+    __builtin_memcpy(p, w, sizeof(w));
 }
 
-// V elements as they are: one 16-byte access where they fill one (p is then 16-byte aligned).
-template <class T, int V, class P>
-__device__ __forceinline__ P load_piece(const T *p) {
-    P x;
-    if constexpr (V * sizeof(T) == 16) {
-        const uint4 raw = *(const uint4 *)p;
-        __builtin_memcpy(&x, &raw, 16);
+// V elements as they lie in memory.
+template <class T, int V>
+struct Raw {
+    T e[V];
+};
+template <class T, int V>
+__device__ __forceinline__ Raw<T, V> load_raw(const T *p) {
+    Raw<T, V> x;
+    if constexpr (V * sizeof(T) >= 16) {
+        uint4 w[V * sizeof(T) / 16];
+        __builtin_memcpy(w, p, sizeof(w));
+        __builtin_memcpy(&x, w, sizeof(w));
     } else {
 #pragma unroll
         for (int i = 0; i < V; ++i) x.e[i] = p[i];
     }
     return x;
 }
-template <class T, int V, class P>
-__device__ __forceinline__ void store_piece(T *p, const P &x) {
-    if constexpr (V * sizeof(T) == 16) {
-        uint4 raw;
-        __builtin_memcpy(&raw, &x, 16);
-        *(uint4 *)p = raw;
+template <class T, int V>
+__device__ __forceinline__ void store_raw(T *p, const Raw<T, V> &x) {
+    if constexpr (V * sizeof(T) >= 16) {
+        uint4 w[V * sizeof(T) / 16];
+        __builtin_memcpy(w, &x, sizeof(w));
+        __builtin_memcpy(p, w, sizeof(w));
     } else {
 #pragma unroll
         for (int i = 0; i < V; ++i) p[i] = x.e[i];
@@ -102,21 +93,18 @@ __device__ __forceinline__ void rotate(float a, float b, float2 cs, float &x, fl
 // One workgroup per `rpb` rows (and a share of their units where there are few rows).  A unit is
 // what one thread turns at a time: V neighbouring elements of interleaved pairs, or V elements
 // and their V partners half a rotation further; then the V-element pieces behind rot.
-// Memory bound: every element is read and written once, in 16-byte pieces where base, strides
-// and (halves) rot / 2 allow it, and a thread has N units' loads in flight, the first N before the
+// Memory bound: every element is read and written once, in 16-byte pieces where head_dim and
+// (halves) rot / 2 are made of such, and a thread has N units' loads in flight, the first N before the
 // angles are formed.
 template <class T, bool HALVES, int V, int N>
 __global__ __launch_bounds__(kThreads) void rope_rows_kernel(RopeRowsArgs a, int rpb, int per_head) {
     extern __shared__ float2 cs[];  // [rpb][rot / 2]
-    struct Piece {
-        T e[V];
-    };
     const int half = a.rope.rot / 2, t = threadIdx.x;
     const int row0 = blockIdx.x * rpb, nrow = min(rpb, a.rows - row0);
     const int per_row = a.heads * per_head, units = nrow * per_row, turned = HALVES ? half / V : per_head;
     const int step = kThreads * gridDim.y;
     constexpr int SIDES = HALVES ? 2 : 1;
-    Piece x[N][SIDES];
+    Raw<T, V> x[N][SIDES];
     T *to[N];
     int at[N], angle[N];  // first element (of the lower half), and where its angles are; -1: copied
     auto load = [&](int u0) {
@@ -129,8 +117,8 @@ __global__ __launch_bounds__(kThreads) void rope_rows_kernel(RopeRowsArgs a, int
             const bool turn_it = HALVES ? p < turned : p * V < 2 * half;
             at[n] = HALVES && !turn_it ? 2 * half + (p - turned) * V : p * V;
             angle[n] = turn_it ? r * half + (HALVES ? p * V : p * V / 2) : -1;
-            x[n][0] = load_piece<T, V, Piece>(from + at[n]);
-            if (HALVES) x[n][SIDES - 1] = load_piece<T, V, Piece>(from + (turn_it ? half + at[n] : at[n]));
+            x[n][0] = load_raw<T, V>(from + at[n]);
+            if (HALVES) x[n][SIDES - 1] = load_raw<T, V>(from + (turn_it ? half + at[n] : at[n]));
         }
     };
     const int first = blockIdx.y * kThreads + t;
@@ -155,7 +143,7 @@ __global__ __launch_bounds__(kThreads) void rope_rows_kernel(RopeRowsArgs a, int
                         x[n][0].e[i] = Elem<T>::put(lo);
                         x[n][SIDES - 1].e[i] = Elem<T>::put(hi);
                     }
-                    store_piece<T, V>(to[n] + half + at[n], x[n][SIDES - 1]);
+                    store_raw<T, V>(to[n] + half + at[n], x[n][SIDES - 1]);
                 } else {
 #pragma unroll
                     for (int i = 0; i < V; i += 2)
@@ -167,7 +155,7 @@ __global__ __launch_bounds__(kThreads) void rope_rows_kernel(RopeRowsArgs a, int
                         }
                 }
             }
-            store_piece<T, V>(to[n] + at[n], x[n][0]);
+            store_raw<T, V>(to[n] + at[n], x[n][0]);
         }
     }
 }
@@ -195,15 +183,20 @@ hipError_t rope_rows(const RopeRowsArgs &a, hipStream_t s) {
 template <class T>
 hipError_t rope_rows_t(const RopeRowsArgs &a, hipStream_t s) {
     constexpr int V = 16 / (int)sizeof(T);
-    auto whole = [](int64_t n) { return n % V == 0; };
-    const bool vec = ((uintptr_t)a.x | (uintptr_t)a.y) % 16 == 0 && whole(a.x_row) && whole(a.x_head) && whole(a.y_row) &&
-                     whole(a.y_head) && whole(a.dim);
+    auto whole = [](int n) { return n % V == 0; };
     if (a.rope.halves)
-        return vec && whole(a.rope.rot / 2) ? rope_rows<T, true, V>(a, s) : rope_rows<T, true, 1>(a, s);
-    return vec ? rope_rows<T, false, V>(a, s) : rope_rows<T, false, 2>(a, s);
+        return whole(a.dim) && whole(a.rope.rot) && whole(a.rope.rot / 2) ? rope_rows<T, true, V>(a, s) : rope_rows<T, true, 1>(a, s);
+    return whole(a.dim) ? rope_rows<T, false, V>(a, s) : rope_rows<T, false, 2>(a, s);
 }
 
 // ---------------------------------------------------------------- the paged cache
+
+// Divisions of a launch by numbers that it does not change, as products.
+struct KvShape {
+    uint32_t row_magic;  // u / (units of a row): u times 2^32 / that, rounded up (exact while their product is under 2^32)
+    int page_shift;      // page_size = 1 << page_shift, or -1
+};
+__device__ __forceinline__ int row_of(const KvShape &k, int u) { return (int)__umulhi((uint32_t)u, k.row_magic); }
 
 // Where row r of a call lives in the pools: the index of its first vector ([page][head 0][slot]) and
 // whether there is such a place.
@@ -211,10 +204,10 @@ struct Place {
     size_t at;
     bool ok;
 };
-__device__ __forceinline__ Place place_of(const KvCacheArgs &c, int stream, int pos) {
+__device__ __forceinline__ Place place_of(const KvCacheArgs &c, const KvShape &k, int stream, int pos) {
     Place p{0, false};
     if (stream < 0 || stream >= c.streams || pos < 0) return p;
-    const int j = pos / c.page_size;
+    const int j = k.page_shift >= 0 ? pos >> k.page_shift : pos / c.page_size;
     if (j >= c.table_stride) return p;
     const int page = c.table[(size_t)stream * c.table_stride + j];
     if (page < 0 || page >= c.n_pages) return p;
@@ -240,16 +233,45 @@ __device__ __forceinline__ uint32_t group_max(uint32_t v) {
 // the scale NaN and reads back as NaN, as quantising it would otherwise hide it.  The maximum is
 // taken over the magnitudes' bit patterns, in which Inf and NaN are largest.
 // Memory bound; the rotation of the keys is done here so that they do not go through memory twice.
-// A thread has N units (8 elements of K or V of one head) in flight at a time.
+// A thread has N units (8 elements of K or V of one head) in flight at a time, the first before the angles.
 template <class T, int KV, int D, int N>
-__global__ __launch_bounds__(kThreads) void kv_write_kernel(KvRowsArgs a, int rpb, bool vec) {
+__global__ __launch_bounds__(kThreads) void kv_write_kernel(KvRowsArgs a, KvShape shape, int rpb) {
     extern __shared__ float2 cs[];  // [rpb][rot / 2]
     constexpr int L = D / 8;
     const int t = threadIdx.x, l = t % L;
     const int row0 = blockIdx.x * rpb, nrow = min(rpb, a.rows - row0);
     const int half = a.rope.rot / 2, heads = a.c.heads;
-    const bool rope = a.rope.freqs != nullptr;
+    const bool rope = a.rope.freqs != nullptr, apart = a.rope.halves && half % 8 == 0;
     const int per_row = 2 * heads * L, units = nrow * per_row;  // K then V
+    // with halves of whole pieces, the partners of this lane's 8 elements are 8 others
+    const bool upper = 8 * l >= half, turned = 8 * l < 2 * half;
+    const int mate = !turned ? 0 : (upper ? -half : half);
+    Raw<T, 8> raw[N], other[N];
+    const T *src[N];
+    size_t vecs[N];
+    int row[N];
+    bool is_v[N], ok[N];
+    auto load = [&](int u0) {
+#pragma unroll
+        for (int n = 0; n < N; ++n) {  // (a unit past the last is the last, and not written: groups are whole)
+            const int u = u0 + n * kThreads < units ? u0 + n * kThreads : units - L + l;
+            row[n] = row_of(shape, u);
+            const int g = (u - row[n] * per_row) / L, r = row0 + row[n];
+            is_v[n] = g >= heads;
+            const int h = is_v[n] ? g - heads : g;
+            src[n] = (is_v[n] ? (const T *)a.v + r * a.v_row : (const T *)a.k + r * a.k_row) + h * D;
+            raw[n] = load_raw<T, 8>(src[n] + 8 * l);
+            if (rope && apart && !is_v[n]) other[n] = load_raw<T, 8>(src[n] + 8 * l + mate);
+            vecs[n] = (size_t)h * a.c.page_size;
+        }
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const Place at = place_of(a.c, shape, a.stream[row0 + row[n]], a.pos[row0 + row[n]]);
+            vecs[n] += at.at;
+            ok[n] = at.ok && u0 + n * kThreads < units;
+        }
+    };
+    load(t);
     if (rope) {
         const int *pos = a.rope_pos != nullptr ? a.rope_pos : a.pos;
         for (int i = t; i < nrow * half; i += kThreads) {
@@ -259,68 +281,53 @@ __global__ __launch_bounds__(kThreads) void kv_write_kernel(KvRowsArgs a, int rp
         __syncthreads();
     }
     for (int u0 = t; u0 < units; u0 += N * kThreads) {
-        float x[N][8];
-        const T *src[N];
-        size_t vecs[N];
-        int row[N];
-        bool is_v[N], ok[N];
-#pragma unroll
-        for (int n = 0; n < N; ++n) {  // (a unit past the last is the last, and not written: groups are whole)
-            const int u = u0 + n * kThreads < units ? u0 + n * kThreads : units - L + l;
-            row[n] = u / per_row;
-            const int g = (u - row[n] * per_row) / L, r = row0 + row[n];
-            is_v[n] = g >= heads;
-            const int h = is_v[n] ? g - heads : g;
-            src[n] = (is_v[n] ? (const T *)a.v + r * a.v_row : (const T *)a.k + r * a.k_row) + h * D;
-            load_n<T, 8>(src[n] + 8 * l, vec, x[n]);
-            const Place at = place_of(a.c, a.stream[r], a.pos[r]);
-            vecs[n] = at.at + (size_t)h * a.c.page_size;
-            ok[n] = at.ok && u0 + n * kThreads < units;
-        }
+        if (u0 != t) load(u0);
 #pragma unroll
         for (int n = 0; n < N; ++n) {
+            float x[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = Elem<T>::get(raw[n].e[i]);
             if (rope && !is_v[n]) {
                 const float2 *c = cs + row[n] * half;
-                if (a.rope.halves && half % 8 == 0) {
-                    if (8 * l < 2 * half) {  // the partners are the 8 elements half a rotation away
-                        const bool up = 8 * l >= half;
-                        const int e = up ? 8 * l - half : 8 * l;
-                        float b[8];
-                        load_n<T, 8>(src[n] + (up ? e : e + half), vec, b);
+                if (apart) {
+                    if (turned) {
+                        c += 8 * l - (upper ? half : 0);
 #pragma unroll
                         for (int i = 0; i < 8; ++i) {
-                            const float2 w = c[e + i];
-                            x[n][i] = x[n][i] * w.x + (up ? b[i] : -b[i]) * w.y;
+                            const float b = Elem<T>::get(other[n].e[i]);
+                            x[i] = fmaf(upper ? b : -b, c[i].y, x[i] * c[i].x);
                         }
                     }
                 } else if (a.rope.halves) {
-#pragma unroll
+#pragma unroll 1
                     for (int i = 0; i < 8; ++i) {
                         const int e = 8 * l + i;
                         if (e < 2 * half) {
                             const bool up = e >= half;
                             const float b = Elem<T>::get(src[n][up ? e - half : e + half]);
                             const float2 w = c[up ? e - half : e];
-                            x[n][i] = x[n][i] * w.x + (up ? b : -b) * w.y;
+                            const float y = fmaf(up ? b : -b, w.y, Elem<T>::get(src[n][e]) * w.x);
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) x[j] = j == i ? y : x[j];
                         }
                     }
                 } else {
 #pragma unroll
                     for (int i = 0; i < 8; i += 2)
-                        if (8 * l + i < 2 * half) rotate(x[n][i], x[n][i + 1], c[4 * l + i / 2], x[n][i], x[n][i + 1]);
+                        if (8 * l + i < 2 * half) rotate(x[i], x[i + 1], c[4 * l + i / 2], x[i], x[i + 1]);
                 }
             }
             const size_t o = vecs[n] * D + 8 * l;
             void *pool = is_v[n] ? a.c.v : a.c.k;
             if constexpr (KV == ELEM_F32) {
-                if (ok[n]) store_n<float, 8>((float *)pool + o, true, x[n]);
+                if (ok[n]) store8((float *)pool + o, x);
             } else if constexpr (KV == ELEM_F16) {
-                if (ok[n]) store_n<__half, 8>((__half *)pool + o, true, x[n]);
+                if (ok[n]) store8((__half *)pool + o, x);
             } else {
                 constexpr float top = KV == ELEM_I8 ? 127.0f : 448.0f;
                 uint32_t mb = 0;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) mb = max(mb, __float_as_uint(x[n][i]) & 0x7fffffffu);
+                for (int i = 0; i < 8; ++i) mb = max(mb, __float_as_uint(x[i]) & 0x7fffffffu);
                 mb = group_max<L>(mb);
                 const bool bad = mb >= 0x7f800000u;
                 float d = __uint_as_float(mb) / top;
@@ -328,17 +335,16 @@ __global__ __launch_bounds__(kThreads) void kv_write_kernel(KvRowsArgs a, int rp
                 const float id = d > 0.0f ? 1.0f / d : 0.0f;
                 uint32_t w[2] = {0, 0};
                 if (!bad) {
-                    float *y = x[n];
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) y[i] = fminf(fmaxf(y[i] * id, -top), top);
+                    for (int i = 0; i < 8; ++i) x[i] = fminf(fmaxf(x[i] * id, -top), top);
                     if constexpr (KV == ELEM_I8) {
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) w[i / 4] |= ((uint32_t)(int)rintf(y[i]) & 0xffu) << (8 * (i & 3));
+                        for (int i = 0; i < 8; ++i) w[i / 4] |= ((uint32_t)(int)rintf(x[i]) & 0xffu) << (8 * (i & 3));
                     } else {
 #pragma unroll
                         for (int i = 0; i < 2; ++i) {
-                            const int p = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * i], y[4 * i + 1], 0, false);
-                            w[i] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[4 * i + 2], y[4 * i + 3], p, true);
+                            const int p = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i], x[4 * i + 1], 0, false);
+                            w[i] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i + 2], x[4 * i + 3], p, true);
                         }
                     }
                 }
@@ -355,7 +361,7 @@ __global__ __launch_bounds__(kThreads) void kv_write_kernel(KvRowsArgs a, int rp
 // the cache (a position past the table, a page outside the pools) are NaN; a negative position is
 // padding and its row stays as it was.  N units of a thread in flight, as in the write.
 template <class T, int KV, int D, int N>
-__global__ __launch_bounds__(kThreads) void kv_read_kernel(KvRowsArgs a, int rpb, bool vec) {
+__global__ __launch_bounds__(kThreads) void kv_read_kernel(KvRowsArgs a, KvShape shape, int rpb) {
     constexpr int L = D / 8;
     constexpr int RAW = KV == ELEM_F32 ? 32 : (KV == ELEM_F16 ? 16 : 8);  // bytes of a unit
     const int row0 = blockIdx.x * rpb, nrow = min(rpb, a.rows - row0);
@@ -367,10 +373,10 @@ __global__ __launch_bounds__(kThreads) void kv_read_kernel(KvRowsArgs a, int rpb
 #pragma unroll
         for (int n = 0; n < N; ++n) {
             const int u = min(u0 + n * kThreads, units - 1);
-            const int rl = u / per_row, rest = u - rl * per_row, g = rest / L, l = rest - g * L, r = row0 + rl;
+            const int rl = row_of(shape, u), rest = u - rl * per_row, g = rest / L, l = rest - g * L, r = row0 + rl;
             is_v[n] = g >= a.c.heads;
             const int h = is_v[n] ? g - a.c.heads : g, pos = a.pos[r];
-            const Place at = place_of(a.c, a.stream[r], pos);
+            const Place at = place_of(a.c, shape, a.stream[r], pos);
             ok[n] = at.ok;
             put[n] = pos >= 0 && u0 + n * kThreads < units;
             vecs[n] = at.ok ? at.at + (size_t)h * a.c.page_size : 0;  // (0: any vector that exists)
@@ -417,36 +423,33 @@ __global__ __launch_bounds__(kThreads) void kv_read_kernel(KvRowsArgs a, int rpb
 #pragma unroll
             for (int i = 0; i < 8; ++i)
                 if (!ok[n]) x[i] = __uint_as_float(0x7fc00000u);
-            if (put[n]) store_n<T, 8>(dst[n], vec, x);
+            if (put[n]) store8(dst[n], x);
         }
     }
 }
 
-template <class T>
-bool rows_vec(const void *k, const void *v, int64_t k_row, int64_t v_row) {
-    constexpr int V = 16 / (int)sizeof(T);
-    return ((uintptr_t)k | (uintptr_t)v) % 16 == 0 && k_row % V == 0 && v_row % V == 0;
-}
-
-// 4 units a thread once that leaves 512 workgroups, else one (a step's few rows).
+// Several units a thread once that leaves 512 workgroups, else one (a step's few rows).
+constexpr int kWriteUnits = 2;
 template <class T, bool READ, int KV, int D>
 hipError_t kv_launch(const KvRowsArgs &a, hipStream_t s) {
-    const int units = 2 * a.c.heads * (D / 8), rpb4 = std::max(1, 4 * kThreads / units), blocks4 = (a.rows + rpb4 - 1) / rpb4;
-    const bool four = blocks4 >= 512;
-    const int rpb = four ? rpb4 : std::max(1, kThreads / units), blocks = (a.rows + rpb - 1) / rpb;
+    constexpr int N = READ ? 4 : kWriteUnits;
+    const int units = 2 * a.c.heads * (D / 8), rpb_n = std::max(1, N * kThreads / units);
+    const bool many = (a.rows + rpb_n - 1) / rpb_n >= 512;
+    const int rpb = many ? rpb_n : std::max(1, kThreads / units), blocks = (a.rows + rpb - 1) / rpb;
     const size_t lds = a.rope.freqs ? (size_t)rpb * (a.rope.rot / 2) * sizeof(float2) : 0;
-    const bool vec = READ ? rows_vec<T>(a.k_out, a.v_out, a.k_row, a.v_row) : rows_vec<T>(a.k, a.v, a.k_row, a.v_row);
+    const KvShape shape{(uint32_t)(((1ull << 32) + units - 1) / units),
+                        (a.c.page_size & (a.c.page_size - 1)) == 0 ? __builtin_ctz(a.c.page_size) : -1};
     (void)hipGetLastError();
     if constexpr (READ) {
-        if (four)
-            hipLaunchKernelGGL((kv_read_kernel<T, KV, D, 4>), dim3(blocks), dim3(kThreads), 0, s, a, rpb, vec);
+        if (many)
+            hipLaunchKernelGGL((kv_read_kernel<T, KV, D, 4>), dim3(blocks), dim3(kThreads), 0, s, a, shape, rpb);
         else
-            hipLaunchKernelGGL((kv_read_kernel<T, KV, D, 1>), dim3(blocks), dim3(kThreads), 0, s, a, rpb, vec);
+            hipLaunchKernelGGL((kv_read_kernel<T, KV, D, 1>), dim3(blocks), dim3(kThreads), 0, s, a, shape, rpb);
     } else {
-        if (four)
-            hipLaunchKernelGGL((kv_write_kernel<T, KV, D, 4>), dim3(blocks), dim3(kThreads), lds, s, a, rpb, vec);
+        if (many)
+            hipLaunchKernelGGL((kv_write_kernel<T, KV, D, kWriteUnits>), dim3(blocks), dim3(kThreads), lds, s, a, shape, rpb);
         else
-            hipLaunchKernelGGL((kv_write_kernel<T, KV, D, 1>), dim3(blocks), dim3(kThreads), lds, s, a, rpb, vec);
+            hipLaunchKernelGGL((kv_write_kernel<T, KV, D, 1>), dim3(blocks), dim3(kThreads), lds, s, a, shape, rpb);
     }
     return hipGetLastError();
 }
