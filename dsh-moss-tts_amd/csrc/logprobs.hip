@@ -36,37 +36,27 @@ __device__ __forceinline__ uint32_t key_of(float x) {
 }
 __device__ __forceinline__ float of_key(uint32_t k) { return __uint_as_float(k ^ ((k & 0x80000000u) ? 0x80000000u : 0xffffffffu)); }
 
-// v of the 64 lanes in descending order
-template <int M>
-__device__ __forceinline__ uint32_t exchange(uint32_t v, bool descending) {
+// v of the 64 lanes in descending order: a bitonic sort.  Step M of runs of RUN: the lower lane of a pair keeps
+// the larger value where its run descends; which lanes those are is a constant.
+__host__ __device__ constexpr uint64_t keep_larger(int run, int m) {
+    uint64_t mask = 0;
+    for (int l = 0; l < 64; ++l) mask |= (uint64_t)(((l & m) == 0) == ((l & run) == 0)) << l;
+    return mask;
+}
+template <int RUN, int M>
+__device__ __forceinline__ uint32_t exchange(uint32_t v) {
+    constexpr uint64_t mask = keep_larger(RUN, M);
     const uint32_t o = (uint32_t)xshfl<M>((int)v);
-    const bool low = (__lane_id() & M) == 0;
-    return low == descending ? max(v, o) : min(v, o);
+    return __builtin_amdgcn_inverse_ballot_w64(mask) ? max(v, o) : min(v, o);
+}
+template <int RUN, int M = RUN / 2>
+__device__ __forceinline__ uint32_t merge_runs(uint32_t v) {
+    v = exchange<RUN, M>(v);
+    if constexpr (M > 1) v = merge_runs<RUN, M / 2>(v);
+    return v;
 }
 __device__ __forceinline__ uint32_t sort64(uint32_t v) {
-    const int l = __lane_id();
-    v = exchange<1>(v, (l & 2) == 0);
-    v = exchange<2>(v, (l & 4) == 0);
-    v = exchange<1>(v, (l & 4) == 0);
-    v = exchange<4>(v, (l & 8) == 0);
-    v = exchange<2>(v, (l & 8) == 0);
-    v = exchange<1>(v, (l & 8) == 0);
-    v = exchange<8>(v, (l & 16) == 0);
-    v = exchange<4>(v, (l & 16) == 0);
-    v = exchange<2>(v, (l & 16) == 0);
-    v = exchange<1>(v, (l & 16) == 0);
-    v = exchange<16>(v, (l & 32) == 0);
-    v = exchange<8>(v, (l & 32) == 0);
-    v = exchange<4>(v, (l & 32) == 0);
-    v = exchange<2>(v, (l & 32) == 0);
-    v = exchange<1>(v, (l & 32) == 0);
-    v = exchange<32>(v, true);
-    v = exchange<16>(v, true);
-    v = exchange<8>(v, true);
-    v = exchange<4>(v, true);
-    v = exchange<2>(v, true);
-    v = exchange<1>(v, true);
-    return v;
+    return merge_runs<64>(merge_runs<32>(merge_runs<16>(merge_runs<8>(merge_runs<4>(merge_runs<2>(v))))));
 }
 
 // Candidates one wave can have: values above the k-th lane maximum lie in at most k - 1 lanes, and
@@ -76,24 +66,24 @@ constexpr int cand_max() {
     return (kTopMax - 1) * EPT + kTopMax + 64 * V;
 }
 
+constexpr int kFastCand = 512;  // candidates that are all taken
 template <int CAP>
 struct TopLds {
-    uint2 cand[kWaves][CAP];  // key, position
-    int n[kWaves];
+    static_assert(kWaves * CAP >= kFastCand, "room for them");
+    uint2 cand[kWaves * CAP];  // key, position, in any order
+    int n;                     // how many (cleared in the first half)
     uint32_t kth[kWaves], quarter[kWaves];
 };
 
-// First half: the waves' sorted maxima (a barrier must follow).
-template <int EPT, int CAP>
-__device__ __forceinline__ void top_floor(const float (&x)[EPT], int k, TopLds<CAP> &lds) {
-    uint32_t best = 0;
-#pragma unroll
-    for (int i = 0; i < EPT; ++i) best = max(best, key_of(x[i]));
-    const uint32_t sorted = sort64(best);
+// First half: the waves' sorted maxima, `best` being the lane's (a barrier must follow).
+template <int CAP>
+__device__ __forceinline__ void top_floor(float best, int k, TopLds<CAP> &lds) {
+    const uint32_t sorted = sort64(key_of(best));
     const int w = threadIdx.x >> 6;
+    if (threadIdx.x == 0) lds.n = 0;
     // read before the branch: inside it the other lanes' last exchange need not have happened
     const uint32_t kth = __builtin_amdgcn_readlane(sorted, k - 1);
-    const uint32_t quarter = __builtin_amdgcn_readlane(sorted, (k + kWaves - 1) / kWaves - 1);
+    const uint32_t quarter = __builtin_amdgcn_readlane(sorted, (k + kWaves - 1) / (kWaves) - 1);
     if ((threadIdx.x & 63) == 0) {
         lds.kth[w] = kth;
         lds.quarter[w] = quarter;
@@ -102,44 +92,68 @@ __device__ __forceinline__ void top_floor(const float (&x)[EPT], int k, TopLds<C
 
 // The k best of the workgroup's values x[i], element i of thread t at position
 // ((i / V) * kThreads + t) * V + i % V: put(rank, key, position) is called once for each rank
-// that exists.
-template <int EPT, int V, int CAP, class Put>
-__device__ __forceinline__ int top_of(const float (&x)[EPT], int k, TopLds<CAP> &lds, Put &&put) {
-    const int t = threadIdx.x, lane = t & 63, w = t >> 6;
-    const uint32_t least = min(min(lds.quarter[0], lds.quarter[1]), min(lds.quarter[2], lds.quarter[3]));
-    const uint32_t floor_key = max(least, max(max(lds.kth[0], lds.kth[1]), max(lds.kth[2], lds.kth[3])));
-    int n = 0, equal = 0;  // of the wave
-    const uint64_t below = (1ull << lane) - 1;
+// that exists.  What reaches the floor is marked with a bit each, and read once more by position, again(position),
+// by loops of few instructions: taken out of the registers where they are found, in straight code of EPT branches
+// whose instructions are fetched for the first time, 20 of 16384 took 11 us of 16.
+template <int EPT, int V, int CAP, class Again, class Put>
+__device__ __forceinline__ int top_of(const float (&x)[EPT], int k, TopLds<CAP> &lds, Again &&again, Put &&put) {
+    const int t = threadIdx.x, lane = t & 63;
+    uint32_t floor_key = 0, least = 0xffffffffu;
 #pragma unroll
-    for (int i0 = 0; i0 < EPT; i0 += V) {
-        const bool more = equal < k;
-#pragma unroll
-        for (int i = i0; i < i0 + V; ++i) {
-            const uint32_t key = key_of(x[i]);
-            const bool eq = key == floor_key && key != 0 && more;
-            const bool take = key > floor_key || eq;
-            const uint64_t who = __ballot(take);
-            if (who == 0) continue;
-            if (take) lds.cand[w][n + __popcll(who & below)] = make_uint2(key, ((i / V) * kThreads + t) * V + i % V);
-            n += __popcll(who);
-            equal += __popcll(__ballot(eq));
-        }
+    for (int v = 0; v < kWaves; ++v) {
+        floor_key = max(floor_key, lds.kth[v]);
+        least = min(least, lds.quarter[v]);
     }
-    if (lane == 0) lds.n[w] = n;
-    __syncthreads();
-    int total = 0;
+    floor_key = max(floor_key, least);
+    const float floor = floor_key == 0 ? -3.40282347e38f : of_key(floor_key);  // comparisons leave NaN out, and -inf below
+    uint64_t bits = 0;
 #pragma unroll
-    for (int v = 0; v < kWaves; ++v) total += lds.n[v];
-    for (int c = lane; c < n; c += 64) {
-        const uint2 me = lds.cand[w][c];
-        int rank = 0;
-        for (int v = 0; v < kWaves; ++v) {
-            const int nv = lds.n[v];
-#pragma unroll 4
-            for (int j = 0; j < nv; ++j) {
-                const uint2 o = lds.cand[v][j];
-                rank += o.x > me.x || (o.x == me.x && o.y < me.y);
+    for (int i = 0; i < EPT; ++i) bits |= x[i] >= floor ? 1ull << i : 0;
+    auto place = [&](int i) { return ((i / V) * kThreads + t) * V + i % V; };
+    int at = 0;
+    if (bits) at = atomicAdd(&lds.n, __popcll(bits));
+    __syncthreads();
+    int total = lds.n;
+    if (total <= kFastCand) {
+        while (bits) {
+            const int p = place(__builtin_ctzll(bits));
+            bits &= bits - 1;
+            lds.cand[at++] = make_uint2(key_of(again(p)), p);
+        }
+    } else {  // hundreds at the floor itself: each wave's first k of those will do, in the order of their positions
+        __syncthreads();
+        if (t == 0) lds.n = 0;
+        __syncthreads();
+        int equal = 0;  // of the wave
+        const uint64_t below = (1ull << lane) - 1;
+#pragma unroll 1
+        for (int i0 = 0; i0 < EPT; i0 += V) {
+            const bool more = floor_key != 0 && equal < k;
+#pragma unroll 1
+            for (int i = i0; i < i0 + V; ++i) {
+                const bool has = (bits >> i) & 1;
+                if (!__any(has)) continue;
+                const uint32_t key = has ? key_of(again(place(i))) : 0;
+                const bool eq = has && key == floor_key && more, take = key > floor_key || eq;
+                const uint64_t who = __ballot(take);
+                int to = 0;
+                if (lane == 0) to = atomicAdd(&lds.n, __popcll(who));
+                to = __builtin_amdgcn_readfirstlane(to);
+                if (take) lds.cand[to + __popcll(who & below)] = make_uint2(key, place(i));
+                equal += __popcll(__ballot(eq));
             }
+        }
+        __syncthreads();
+        total = lds.n;
+    }
+    __syncthreads();
+    for (int c = t; c < total; c += kThreads) {
+        const uint2 me = lds.cand[c];
+        int rank = 0;
+#pragma unroll 4
+        for (int j = 0; j < total; ++j) {
+            const uint2 o = lds.cand[j];
+            rank += o.x > me.x || (o.x == me.x && o.y < me.y);
         }
         if (rank < k) put(rank, me.x, (int)me.y);
     }
@@ -155,13 +169,14 @@ struct Sums {
 template <int EPT, int CAP>
 __device__ __forceinline__ Sums sums_of(const float (&x)[EPT], float inv_t, int k, float (*red)[kWaves], TopLds<CAP> &lds) {
     const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    float m = -INFINITY;
+    float best = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < EPT; ++i) m = fmaxf(m, x[i] * inv_t);
-    m = wave_max(m);
+    for (int i = 0; i < EPT; ++i) best = fmaxf(best, x[i]);
+    float m = wave_max(best) * inv_t;  // (rounding keeps the order)
     if (lane == 0) red[0][w] = m;
     __syncthreads();
-    m = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+#pragma unroll
+    for (int v = 0; v < kWaves; ++v) m = fmaxf(m, red[0][v]);
     const float m0 = m == -INFINITY ? 0.0f : m;
     float s = 0.0f, u = 0.0f;
 #pragma unroll
@@ -177,9 +192,15 @@ __device__ __forceinline__ Sums sums_of(const float (&x)[EPT], float inv_t, int 
         red[1][w] = s;
         red[2][w] = u;
     }
-    if (k > 0) top_floor(x, k, lds);
+    if (k > 0) top_floor(best, k, lds);
     __syncthreads();
-    return Sums{m, (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]), (red[2][0] + red[2][1]) + (red[2][2] + red[2][3])};
+    Sums q{m, 0.0f, 0.0f};
+#pragma unroll
+    for (int v = 0; v < kWaves; ++v) {
+        q.s += red[1][v];
+        q.u += red[2][v];
+    }
+    return q;
 }
 
 template <class T>
@@ -190,18 +211,17 @@ __device__ __forceinline__ float logit(const T *p) {
         return *p;
 }
 
-// What a row's sums give: the token's log probability and the entropy (thread 0), and the log
-// probability of an alternative.
+// The logit of a row's token, asked for early; NaN for a token outside the vocabulary.
 template <class T>
-__device__ __forceinline__ void finish_row(const LogprobArgs &a, int r, const Sums &q) {
-    const float log_s = logf(q.s);
+__device__ __forceinline__ float token_logit(const LogprobArgs &a, int r) {
     const int tok = a.tokens[r];
-    float lp = __uint_as_float(0x7fc00000u);
-    if (tok >= 0 && tok < a.vocab) {
-        const float z = logit((const T *)a.x + r * a.row + tok) * a.inv_t;
-        lp = q.s == 0.0f ? -INFINITY : z - q.m - log_s;  // no token is allowed at all
-    }
-    a.logprob[r] = lp;
+    return tok >= 0 && tok < a.vocab ? logit((const T *)a.x + r * a.row + tok) : __uint_as_float(0x7fc00000u);
+}
+// What a row's sums give: the token's log probability and the entropy (one thread), and the log
+// probability of an alternative.
+__device__ __forceinline__ void finish_row(const LogprobArgs &a, int r, float x, const Sums &q) {
+    const float log_s = logf(q.s), z = x * a.inv_t;
+    a.logprob[r] = q.s == 0.0f && z == z ? -INFINITY : z - q.m - log_s;  // (sum 0: no token is allowed at all)
     if (a.entropy != nullptr) a.entropy[r] = q.s == 0.0f ? 0.0f : log_s - q.u / q.s;
 }
 __device__ __forceinline__ float alt_lp(const LogprobArgs &a, const Sums &q, uint32_t key) {
@@ -222,14 +242,19 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LogprobArgs a, int c
     const int r = blockIdx.x / chunks, c = blockIdx.x - r * chunks, t = threadIdx.x;
     const int base = c * EPT * kThreads;
     const T *p = (const T *)a.x + r * a.row;
+    float token = 0.0f;
+    if (chunks == 1 && t == 0) token = token_logit<T>(a, r);
     float x[EPT];
 #pragma unroll
     for (int i = 0; i < EPT; i += V) {
-        const int e = base + (i * kThreads) + t * V;
-        if (V > 1 && e + V <= a.vocab) {
-            uint4 raw = *(const uint4 *)(p + e);
+        const int e = base + i * kThreads + t * V;
+        if (e + V <= a.vocab) {
+            T raw[V];  // (16 bytes at any address that a logit may have: the hardware takes them unaligned)
+            uint32_t w[V * sizeof(T) / 4];
+            __builtin_memcpy(w, p + e, sizeof(w));
+            __builtin_memcpy(raw, w, sizeof(w));
 #pragma unroll
-            for (int j = 0; j < V; ++j) x[i + j] = logit((const T *)&raw + j);
+            for (int j = 0; j < V; ++j) x[i + j] = logit(raw + j);
         } else {
 #pragma unroll
             for (int j = 0; j < V; ++j) x[i + j] = e + j < a.vocab ? logit(p + e + j) : -INFINITY;
@@ -237,9 +262,9 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LogprobArgs a, int c
     }
     const Sums q = sums_of(x, a.inv_t, a.top_k, red, lds);
     if (chunks == 1) {
-        if (t == 0) finish_row<T>(a, r, q);
+        if (t == 0) finish_row(a, r, token, q);
         if (a.top_k > 0) {
-            const int n = top_of<EPT, V>(x, a.top_k, lds, [&](int rank, uint32_t key, int at) {
+            const int n = top_of<EPT, V>(x, a.top_k, lds, [&](int at) { return logit(p + base + at); }, [&](int rank, uint32_t key, int at) {
                 a.top_ids[(size_t)r * a.top_k + rank] = at;
                 a.top_lp[(size_t)r * a.top_k + rank] = alt_lp(a, q, key);
             });
@@ -251,7 +276,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LogprobArgs a, int c
     if (t == 0) *(float4 *)(row + 4 * c) = make_float4(q.m, q.s, q.u, 0.0f);
     if (a.top_k > 0) {
         float *o = row + 4 * chunks + c * a.top_k;
-        const int n = top_of<EPT, V>(x, a.top_k, lds, [&](int rank, uint32_t key, int at) {
+        const int n = top_of<EPT, V>(x, a.top_k, lds, [&](int at) { return logit(p + base + at); }, [&](int rank, uint32_t key, int at) {
             o[rank] = of_key(key);
             ((int *)o)[chunks * a.top_k + rank] = base + at;
         });
@@ -265,6 +290,8 @@ __global__ __launch_bounds__(kThreads) void logprobs_join_kernel(LogprobArgs a, 
     __shared__ TopLds<cand_max<EPT, 1>()> lds;
     const int r = blockIdx.x, t = threadIdx.x, n = chunks * a.top_k;
     const float *w = (const float *)a.ws + r * row_words(chunks, a.top_k), *best = w + 4 * chunks;
+    float token = 0.0f;
+    if (t == 0) token = token_logit<T>(a, r);
     // position c * k + j: equal values of a lower index come first, as chunks and ranks do
     float x[EPT];
 #pragma unroll
@@ -287,22 +314,27 @@ __global__ __launch_bounds__(kThreads) void logprobs_join_kernel(LogprobArgs a, 
     }
     q.s = wave_sum(q.s);
     q.u = wave_sum(q.u);
-    if (t == 0) finish_row<T>(a, r, q);
+    if (t == 0) finish_row(a, r, token, q);
     if (a.top_k == 0) return;
-    top_floor(x, a.top_k, lds);
+    float most = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < EPT; ++i) most = fmaxf(most, x[i]);
+    top_floor(most, a.top_k, lds);
     __syncthreads();
-    const int got = top_of<EPT, 1>(x, a.top_k, lds, [&](int rank, uint32_t key, int at) {
+    const int got = top_of<EPT, 1>(x, a.top_k, lds, [&](int at) { return best[at]; }, [&](int rank, uint32_t key, int at) {
         a.top_ids[(size_t)r * a.top_k + rank] = ((const int *)best)[n + at];
         a.top_lp[(size_t)r * a.top_k + rank] = alt_lp(a, q, key);
     });
     no_alternatives(a, r, got);
 }
 
-// Values a thread holds.
+// Values a thread holds.  Up to 16384 logits a row is one chunk: one launch and no join.  A longer one is cut finely
+// while there are few, so that they fill the chip.
 int ept_of(int rows, int vocab) {
-    if (vocab <= 4 * kThreads) return 4;
+    for (int ept = 4; ept <= 64; ept *= 2)
+        if (vocab <= ept * kThreads) return ept;
     const int chunks8 = (vocab + 8 * kThreads - 1) / (8 * kThreads);
-    return chunks8 <= kMaxChunks && (long long)rows * chunks8 <= 4096 ? 8 : 32;
+    return chunks8 <= kMaxChunks && (long long)rows * chunks8 <= 1024 ? 8 : 32;
 }
 int chunks_of(int rows, int vocab) {
     const int n = ept_of(rows, vocab) * kThreads;
@@ -312,23 +344,20 @@ int chunks_of(int rows, int vocab) {
 template <class T, int EPT>
 void launch_chunks(const LogprobArgs &a, int chunks, hipStream_t s) {
     constexpr int V = std::min<int>(16 / (int)sizeof(T), EPT);
-    const dim3 grid((unsigned)a.rows * chunks);
-    if (V * sizeof(T) == 16 && (uintptr_t)a.x % 16 == 0 && a.row % V == 0)
-        hipLaunchKernelGGL((logprobs_kernel<T, EPT, V>), grid, dim3(kThreads), 0, s, a, chunks);
-    else
-        hipLaunchKernelGGL((logprobs_kernel<T, EPT, 1>), grid, dim3(kThreads), 0, s, a, chunks);
+    hipLaunchKernelGGL((logprobs_kernel<T, EPT, V>), dim3((unsigned)a.rows * chunks), dim3(kThreads), 0, s, a, chunks);
 }
 
 template <class T>
 hipError_t logprobs_t(const LogprobArgs &a, hipStream_t s) {
-    const int chunks = chunks_of(a.rows, a.vocab), ept = ept_of(a.rows, a.vocab);
+    const int chunks = chunks_of(a.rows, a.vocab);
     (void)hipGetLastError();
-    if (ept == 4)
-        launch_chunks<T, 4>(a, chunks, s);
-    else if (ept == 8)
-        launch_chunks<T, 8>(a, chunks, s);
-    else
-        launch_chunks<T, 32>(a, chunks, s);
+    switch (ept_of(a.rows, a.vocab)) {
+        case 4: launch_chunks<T, 4>(a, chunks, s); break;
+        case 8: launch_chunks<T, 8>(a, chunks, s); break;
+        case 16: launch_chunks<T, 16>(a, chunks, s); break;
+        case 32: launch_chunks<T, 32>(a, chunks, s); break;
+        default: launch_chunks<T, 64>(a, chunks, s); break;
+    }
     if (chunks > 1 && chunks * a.top_k <= 2 * kThreads)
         hipLaunchKernelGGL((logprobs_join_kernel<T, 2>), dim3(a.rows), dim3(kThreads), 0, s, a, chunks);
     else if (chunks > 1)
