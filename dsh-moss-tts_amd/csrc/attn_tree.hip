@@ -75,7 +75,7 @@ __device__ __forceinline__ floatx4 mfma(float a, float b, floatx4 c) {
 __device__ __forceinline__ void split2(float a, float b, uint32_t &hi, uint32_t &lo) {
     const auto h = __builtin_amdgcn_cvt_pkrtz(a, b);
     hi = __builtin_bit_cast(uint32_t, h);
-    lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a - (float)h[0], b - (float)h[1]));
+    lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(fmaf((float)h[0], -1.0f, a), fmaf((float)h[1], -1.0f, b)));
 }
 
 // A lane's share of 32 keys x D of one head, as they lie in memory: of K the A operand of S^T (key
@@ -88,16 +88,11 @@ struct Keys {
     float4 ks[2], vs[2];
 };
 
-// Where a block of 16 keys lies: the index of its first vector, and its last key that is read.
-struct Block {
-    size_t vec;
-    int lim;
-};
-
-// The block of keys kb .. kb + 15 of a stream whose last key to read is `last`; a page outside the pools
-// sets `bad` (and page 0 is read in its place).
-__device__ __forceinline__ Block block_of(const TreeArgs &a, const TreePlan &plan, const int *table, int h, int kb, int last,
-                                          bool &bad) {
+// The block of keys kb .. kb + 15 of a stream, or of the last one that has any up to key `last`: the index of its
+// first vector.  A block lies in one page, so all of it can be read; what lies behind the last key is masked like a key
+// that no row sees.  A page outside the pools sets `bad` (and page 0 is read in its place).
+__device__ __forceinline__ size_t block_of(const TreeArgs &a, const TreePlan &plan, const int *table, int h, int kb, int last,
+                                           bool &bad) {
     kb = min(kb, last & ~15);
     const uint32_t blk = (uint32_t)kb >> 4, pg = (uint32_t)((blk * plan.page_magic) >> 40);
     int page = __builtin_amdgcn_readfirstlane(table[pg]);
@@ -105,29 +100,25 @@ __device__ __forceinline__ Block block_of(const TreeArgs &a, const TreePlan &pla
         page = 0;
         bad = true;
     }
-    Block b;
-    b.vec = ((size_t)page * a.c.heads + h) * a.c.page_size + (blk - pg * (a.c.page_size >> 4)) * 16;
-    b.lim = min(15, last - kb);
-    return b;
+    return ((size_t)page * a.c.heads + h) * a.c.page_size + (blk - pg * (a.c.page_size >> 4)) * 16;
 }
 
-// Loads of one block: K as NW 16-byte pieces of a key, V as NW words of each of 4 keys.
+// Loads of the block at vector `at`: K as NW 16-byte pieces of a key, V as NW words of each of 4 keys; a lane's
+// offsets are the same for every block.
 template <int KV, int D>
-__device__ __forceinline__ void load_k(const TreeArgs &a, const Block &b, int c, int g, uint4 (&k)[Keys<KV, D>::NW]) {
-    const char *p = (const char *)a.c.k + b.vec * (D * elem_size(KV));
-    const int off = min(c, b.lim) * (D * elem_size(KV)) + 16 * g;
+__device__ __forceinline__ void load_k(const TreeArgs &a, size_t at, int c, int g, uint4 (&k)[Keys<KV, D>::NW]) {
+    const char *p = (const char *)a.c.k + at * (D * elem_size(KV));
 #pragma unroll
-    for (int u = 0; u < Keys<KV, D>::NW; ++u) k[u] = *(const uint4 *)(p + off + 64 * u);
+    for (int u = 0; u < Keys<KV, D>::NW; ++u) k[u] = *(const uint4 *)(p + (unsigned)(c * (D * elem_size(KV)) + 16 * g + 64 * u));
 }
 template <int KV, int D>
-__device__ __forceinline__ void load_v(const TreeArgs &a, const Block &b, int c, int g, uint32_t (&v)[4][Keys<KV, D>::NW]) {
+__device__ __forceinline__ void load_v(const TreeArgs &a, size_t at, int c, int g, uint32_t (&v)[4][Keys<KV, D>::NW]) {
     constexpr int NW = Keys<KV, D>::NW;
-    const char *p = (const char *)a.c.v + b.vec * (D * elem_size(KV));
+    const char *p = (const char *)a.c.v + at * (D * elem_size(KV));
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int off = min(4 * g + i, b.lim) * (D * elem_size(KV)) + c * (NW * 4);
-        __builtin_memcpy(v[i], __builtin_assume_aligned(p + off, NW < 4 ? NW * 4 : 16), NW * 4);
-    }
+    for (int i = 0; i < 4; ++i)
+        __builtin_memcpy(v[i], __builtin_assume_aligned(p + (unsigned)((4 * g + i) * (D * elem_size(KV)) + c * (NW * 4)), NW < 4 ? NW * 4 : 16),
+                         NW * 4);
 }
 
 // The 8 dims of K fragment s (f16 products) start at this one, for lane group g.
@@ -420,7 +411,7 @@ __device__ __forceinline__ void scale_weights(const Stream &st, const Q (&q)[MT]
 // The Inf and NaN elements of V among 32 keys, added key by key to the rows that see them (x: weights,
 // `room` the wave's [16][ >= 32] floats of LDS).
 template <int KV, int D, int MT, class Room>
-__device__ __forceinline__ void add_odd_values(const TreeArgs &a, const Stream &st, const Block (&blk)[2], int p0, int mt,
+__device__ __forceinline__ void add_odd_values(const TreeArgs &a, const Stream &st, const size_t (&blk)[2], int p0, int mt,
                                                uint64_t mask, const float (&x)[2][4], Room &room, Rows<MT, D / 16> &rows) {
     const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
 #pragma unroll
@@ -432,7 +423,7 @@ __device__ __forceinline__ void add_odd_values(const TreeArgs &a, const Stream &
 #pragma unroll 1
     for (int kk = 0; kk < 32; ++kk) {
         const int b = kk >> 4;
-        const size_t at = ((b ? blk[1].vec : blk[0].vec) + min(kk & 15, b ? blk[1].lim : blk[0].lim)) * D + (D / 4) * g;
+        const size_t at = ((b ? blk[1] : blk[0]) + (kk & 15)) * D + (D / 4) * g;
         const float wt = room[c][kk];
         const bool see = visible(st, mask, p0 + kk);
 #pragma unroll
@@ -515,16 +506,16 @@ __global__ __launch_bounds__(kThreads, KV == ELEM_F32 ? (D == 64 ? 2 : 1) : (D =
     const int *table = a.c.table + (size_t)s * a.c.table_stride;
 
     Keys<KV, D> cur;
-    Block blk[2];
-    auto fetch = [&](int p, Keys<KV, D> &to, Block (&at)[2]) {
+    size_t blk[2];
+    auto fetch = [&](int p, Keys<KV, D> &to, size_t (&at)[2]) {
 #pragma unroll
         for (int b = 0; b < 2; ++b) at[b] = block_of(a, plan, table, h, p + 16 * b, last, bad);
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
             load_k<KV, D>(a, at[b], c, g, to.k[b]);
             if constexpr (SCALED) {
-                to.ks[b] = *(const float4 *)(a.c.k_scale + at[b].vec + 4 * g);
-                to.vs[b] = *(const float4 *)(a.c.v_scale + at[b].vec + 4 * g);
+                to.ks[b] = *(const float4 *)(a.c.k_scale + at[b] + 4 * g);
+                to.vs[b] = *(const float4 *)(a.c.v_scale + at[b] + 4 * g);
             }
         }
 #pragma unroll
@@ -544,7 +535,7 @@ __global__ __launch_bounds__(kThreads, KV == ELEM_F32 ? (D == 64 ? 2 : 1) : (D =
     for (; p0 < end; p0 += 32 * kWaves) {
         const bool tail = p0 + 32 > st.ctx;
         Keys<KV, D> next;
-        Block nblk[2];
+        size_t nblk[2];
         fetch(p0 + 32 * kWaves, next, nblk);  // (past the end: the last block again)
 
         float x[MT][2][4];
@@ -583,15 +574,20 @@ __global__ __launch_bounds__(kThreads, KV == ELEM_F32 ? (D == 64 ? 2 : 1) : (D =
         if (tail) hide(st, q, p0, g, -INFINITY, x);
         if constexpr (SCALED) {
             uint32_t top = 0;
+            if (tail) {
 #pragma unroll
-            for (int b = 0; b < 2; ++b) {
-                const float vs[4] = {cur.vs[b].x, cur.vs[b].y, cur.vs[b].z, cur.vs[b].w};
+                for (int b = 0; b < 2; ++b) {
+                    const float vs[4] = {cur.vs[b].x, cur.vs[b].y, cur.vs[b].z, cur.vs[b].w};
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const uint32_t y = __float_as_uint(vs[i]) & 0x7fffffffu;
-                    const bool use = y < 0x7f800000u && (!tail || visible(st, seen, p0 + 16 * b + 4 * g + i));
-                    top = max(top, use ? y : 0u);
+                    for (int i = 0; i < 4; ++i) {
+                        const uint32_t y = __float_as_uint(vs[i]) & 0x7fffffffu;
+                        top = max(top, y < 0x7f800000u && visible(st, seen, p0 + 16 * b + 4 * g + i) ? y : 0u);
+                    }
                 }
+            } else {  // (an Inf or NaN here is every row's)
+                const float v = fmaxf(fmaxf(fmaxf(fabsf(cur.vs[0].x), fabsf(cur.vs[0].y)), fmaxf(fabsf(cur.vs[0].z), fabsf(cur.vs[0].w))),
+                                      fmaxf(fmaxf(fabsf(cur.vs[1].x), fabsf(cur.vs[1].y)), fmaxf(fabsf(cur.vs[1].z), fabsf(cur.vs[1].w))));
+                top = __float_as_uint(v);
             }
             top = max(top, (uint32_t)xshfl<16>((int)top));
             top = max(top, (uint32_t)xshfl<32>((int)top));
@@ -744,12 +740,12 @@ __global__ __launch_bounds__(64 * NWV, 2) void attn_tree_wide_kernel(TreeArgs a,
     uint32_t vraw[4][NW];
     float ksr = 0.0f, vsr = 0.0f;
     auto fetch = [&](int p) {
-        const Block b = block_of(a, plan, table, h, p + 16 * w, last, bad);
+        const size_t b = block_of(a, plan, table, h, p + 16 * w, last, bad);
         load_k<KV, D>(a, b, c, g, kraw);
         load_v<KV, D>(a, b, c, g, vraw);
         if constexpr (SCALED) {
-            ksr = a.c.k_scale[b.vec + c];
-            vsr = a.c.v_scale[b.vec + c];
+            ksr = a.c.k_scale[b + c];
+            vsr = a.c.v_scale[b + c];
         }
     };
     if (beg < end) fetch(beg);
@@ -877,7 +873,7 @@ __global__ __launch_bounds__(64 * NWV, 2) void attn_tree_wide_kernel(TreeArgs a,
                         }
                 if constexpr (KV != ELEM_I8) {
                     if (tail && (lds.odd[buf][2 * u] | lds.odd[buf][2 * u + 1])) {
-                        Block blk[2];
+                        size_t blk[2];
 #pragma unroll
                         for (int b = 0; b < 2; ++b) blk[b] = block_of(a, plan, table, h, p0 + 16 * b, last, bad);
 #pragma unroll
@@ -921,35 +917,36 @@ __global__ __launch_bounds__(64 * NWV, 2) void attn_tree_wide_kernel(TreeArgs a,
     }
 }
 
-// The key splits of each (row, head) joined in their order by one workgroup of 4 waves: every wave forms the
-// maximum and the sum (lane c holds split c's) and adds up a quarter of the splits, D / 4 lanes a vector with
-// 256 / D splits side by side.
-template <int D>
+// The key splits of each (row, head) joined in their order: lane c holds split c's maximum and sum, and D / 4
+// lanes add up a vector with SIDE = 256 / D splits side by side, all of a wave's splits loaded at once.  Up to 4 SIDE
+// splits one wave does a row; more are shared out to the 4 waves of a workgroup and joined through LDS.
+template <int D, bool ONE_WAVE>
 __global__ __launch_bounds__(kThreads) void attn_tree_join_kernel(TreeArgs a, TreePlan plan) {
-    constexpr int G = D / 4, SIDE = 64 / G, ROUNDS = kMaxSplits / (kWaves * SIDE);
+    constexpr int G = D / 4, SIDE = 64 / G, ROUNDS = ONE_WAVE ? 4 : kMaxSplits / (kWaves * SIDE);
     __shared__ float4 part[kWaves][G];
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, splits = plan.splits;
-    const int per = a.max_rows * a.heads, s = blockIdx.x / per, i = blockIdx.x - s * per;
+    const int lane = threadIdx.x & 63, splits = plan.splits;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int of_stream = a.max_rows * a.heads, per = ONE_WAVE ? (of_stream + kWaves - 1) / kWaves : of_stream;
+    const int s = blockIdx.x / per, i = ONE_WAVE ? (blockIdx.x - s * per) * kWaves + w : blockIdx.x - s * per;
     const Stream st = stream_of(a, s);
     if (i >= st.n * a.heads) return;
     const size_t all_rows = (size_t)a.rows * a.heads, at = (size_t)st.row0 * a.heads + i;
     float2 mine = make_float2(-INFINITY, 0.0f);
     if (lane < splits) mine = ((const float2 *)a.ws)[(size_t)lane * all_rows + at];
     const int d = (lane % G) * 4, side = lane / G;
+    const int first = ONE_WAVE ? side : w * SIDE + side, step = ONE_WAVE ? SIDE : kWaves * SIDE;
     const float *po = (const float *)a.ws + (size_t)splits * all_rows * 2 + at * D + d;
     float4 x[ROUNDS];
 #pragma unroll
-    for (int r = 0; r < ROUNDS; ++r) {  // (a split without keys has written none: what is read there is not used)
-        const int k = (r * kWaves + w) * SIDE + side;
-        if (r * kWaves * SIDE < splits) x[r] = *(const float4 *)(po + (size_t)min(k, splits - 1) * all_rows * D);
-    }
+    for (int r = 0; r < ROUNDS; ++r)  // (a split without keys has written none: what is read there is not used)
+        if (r * step < splits) x[r] = *(const float4 *)(po + (size_t)min(first + r * step, splits - 1) * all_rows * D);
     const float M = wave_max(mine.x), M0 = M == -INFINITY ? 0.0f : M;
     const float f = exp2_(mine.x - M0), L = wave_sum(mine.y * f);
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int r = 0; r < ROUNDS; ++r) {
-        const int k = (r * kWaves + w) * SIDE + side;
-        if (r * kWaves * SIDE < splits) {
+    for (int r = 0; r < ROUNDS; ++r)
+        if (r * step < splits) {
+            const int k = first + r * step;
             const float fk = __shfl(f, k & 63), lk = __shfl(mine.y, k & 63);
             const bool use = k < splits && lk != 0.0f;
             o.x = use ? fmaf(x[r].x, fk, o.x) : o.x;
@@ -957,17 +954,19 @@ __global__ __launch_bounds__(kThreads) void attn_tree_join_kernel(TreeArgs a, Tr
             o.z = use ? fmaf(x[r].z, fk, o.z) : o.z;
             o.w = use ? fmaf(x[r].w, fk, o.w) : o.w;
         }
-    }
     if constexpr (G == 16) o.x += xshfl<16>(o.x), o.y += xshfl<16>(o.y), o.z += xshfl<16>(o.z), o.w += xshfl<16>(o.w);
     o.x += xshfl<32>(o.x), o.y += xshfl<32>(o.y), o.z += xshfl<32>(o.z), o.w += xshfl<32>(o.w);
-    if (side == 0) part[w][lane % G] = o;
-    __syncthreads();
-    if (threadIdx.x >= G) return;
-    float y[4];
+    float y[4] = {o.x, o.y, o.z, o.w};
+    if constexpr (!ONE_WAVE) {
+        if (side == 0) part[w][lane % G] = o;
+        __syncthreads();
+        if (w != 0) return;
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-        y[j] = (((const float *)&part[0][lane])[j] + ((const float *)&part[1][lane])[j]) +
-               (((const float *)&part[2][lane])[j] + ((const float *)&part[3][lane])[j]);
+        for (int j = 0; j < 4; ++j)
+            y[j] = (((const float *)&part[0][lane % G])[j] + ((const float *)&part[1][lane % G])[j]) +
+                   (((const float *)&part[2][lane % G])[j] + ((const float *)&part[3][lane % G])[j]);
+    }
+    if (side != 0) return;
     TreePlan whole = plan;
     whole.splits = 1;
     put_row<D, 4>(a, whole, st, 0, a.heads, 0, i, d, M, L, y);
@@ -1035,8 +1034,11 @@ hipError_t launch_kv(const TreeArgs &a, hipStream_t s) {
         launch_group<KV, D, true>(a, p, s);
     else
         launch_group<KV, D, false>(a, p, s);
-    if (p.splits > 1)
-        hipLaunchKernelGGL((attn_tree_join_kernel<D>), dim3((unsigned)(a.c.streams * a.max_rows * a.heads)), dim3(kThreads), 0, s, a, p);
+    const unsigned rows = (unsigned)(a.max_rows * a.heads), streams = (unsigned)a.c.streams;
+    if (p.splits > 1024 / D)
+        hipLaunchKernelGGL((attn_tree_join_kernel<D, false>), dim3(streams * rows), dim3(kThreads), 0, s, a, p);
+    else if (p.splits > 1)
+        hipLaunchKernelGGL((attn_tree_join_kernel<D, true>), dim3(streams * ((rows + kWaves - 1) / kWaves)), dim3(kThreads), 0, s, a, p);
     return hipGetLastError();
 }
 
