@@ -43,7 +43,8 @@ constexpr int kWeightExp = 6;   // and of what it is scaled by
 
 struct TreePlan {
     int tiles, group, row_groups;  // row tiles of 16, of which a workgroup takes `group`
-    int splits, chunk;             // key splits of `chunk` keys
+    int slots;                     // pieces that all streams' keys are cut into; streams: no cuts, and no workspace
+    int chunk;                     // keys of a piece where every stream has as many slots
     uint64_t page_magic;           // block of 16 keys / blocks of a page, as a product
 };
 
@@ -201,18 +202,76 @@ struct Stream {
     int row0, n, ctx, total;
     bool bad;  // more keys than the launch or the table has room for
 };
-__device__ __forceinline__ Stream stream_of(const TreeArgs &a, int s) {
+__device__ __forceinline__ Stream stream_at(const TreeArgs &a, int row0, int end, int ctx) {
     Stream t;
-    t.row0 = __builtin_amdgcn_readfirstlane(a.row_start[s]);
-    const int end = __builtin_amdgcn_readfirstlane(a.row_start[s + 1]);
-    t.n = t.row0 < 0 || end > a.rows || end <= t.row0 ? 0 : min(end - t.row0, a.max_rows);
-    t.ctx = __builtin_amdgcn_readfirstlane(a.ctx_len[s]);
+    t.row0 = row0;
+    t.n = row0 < 0 || end > a.rows || end <= row0 ? 0 : min(end - row0, a.max_rows);
+    t.ctx = ctx;
     const long long room = min((long long)a.c.table_stride * a.c.page_size, (long long)a.max_keys);
-    t.bad = t.ctx < 0 || (long long)t.ctx + t.n > room;
-    t.total = t.bad ? 0 : t.ctx + t.n;
+    t.bad = ctx < 0 || (long long)ctx + t.n > room;
+    t.total = t.bad ? 0 : ctx + t.n;
     return t;
 }
+__device__ __forceinline__ Stream stream_of(const TreeArgs &a, int s) {
+    return stream_at(a, __builtin_amdgcn_readfirstlane(a.row_start[s]), __builtin_amdgcn_readfirstlane(a.row_start[s + 1]),
+                     __builtin_amdgcn_readfirstlane(a.ctx_len[s]));
+}
 
+// One piece of the keys: those from beg to end of a stream (-1: none), whose pieces are the slots from `first` on.
+struct Cut {
+    int stream, beg, end, first, pieces;
+};
+// Up to 64 streams share the slots out by their lengths: pieces of the fewest keys (a multiple of 128, at least 256)
+// of which there are no more than slots, so that no workgroup has much more to do than another, however
+// ragged the streams (8 of 8192 to 16384 keys and one just begun: 204 us with as many pieces each, 168 so).  Every
+// wave finds that size for itself, lane s holding stream s.  More streams: as many slots each.
+__device__ __forceinline__ int even_chunk(const TreeArgs &a, const TreePlan &plan, int &mine) {
+    const int lane = threadIdx.x & 63;
+    mine = 0;
+    if (lane < a.c.streams) {
+        const Stream st = stream_at(a, a.row_start[lane], a.row_start[lane + 1], a.ctx_len[lane]);
+        mine = st.n == 0 ? 0 : max(st.total, 1);  // (rows that are to be NaN need a piece too)
+    }
+    int most = mine;
+    most = max(most, xshfl<1>(most)), most = max(most, xshfl<2>(most)), most = max(most, xshfl<4>(most));
+    most = max(most, xshfl<8>(most)), most = max(most, xshfl<16>(most)), most = max(most, xshfl<32>(most));
+    long long sum = mine;
+    for (int m = 1; m < 64; m *= 2) sum += __shfl_xor(sum, m);
+    const long long even = (sum + plan.slots - 1) / plan.slots;
+    int chunk = max(max((int)min(even, 1ll << 30), (most + kMaxSplits - 1) / kMaxSplits), 256);
+    chunk = __builtin_amdgcn_readfirstlane((chunk + 127) / 128 * 128);
+    const int step = (chunk / 16 + 127) / 128 * 128;
+    while (true) {  // (ends at the longest stream's keys at the latest: then there are no more pieces than streams)
+        int pieces = ((uint32_t)mine + chunk - 1) / (uint32_t)chunk;
+        for (int m = 1; m < 64; m *= 2) pieces += __shfl_xor(pieces, m);
+        if (__builtin_amdgcn_readfirstlane(pieces) <= plan.slots) return chunk;
+        chunk += step;
+    }
+}
+__device__ __forceinline__ bool even_cuts(const TreeArgs &a, const TreePlan &plan) { return a.c.streams > 1 && a.c.streams <= 64; }
+// Slots before lane's stream, when its pieces are so many.
+__device__ __forceinline__ int slots_before(int pieces) {
+    int sum = pieces;
+    for (int m = 1; m < 64; m *= 2) {
+        const int below = __shfl_up(sum, m);
+        if ((int)(threadIdx.x & 63) >= m) sum += below;
+    }
+    return sum - pieces;
+}
+__device__ __forceinline__ Cut cut_of_slot(const TreeArgs &a, const TreePlan &plan, int slot) {
+    if (plan.slots == a.c.streams) return Cut{slot, 0, 0x7fffffff, slot, 1};
+    if (!even_cuts(a, plan)) {
+        const int per = plan.slots / a.c.streams, s = slot / per, z = slot - s * per;
+        return Cut{s, z * plan.chunk, (z + 1) * plan.chunk, s * per, per};
+    }
+    int mine;
+    const int chunk = even_chunk(a, plan, mine);
+    const int pieces = ((uint32_t)mine + chunk - 1) / (uint32_t)chunk, before = slots_before(pieces);
+    const uint64_t who = __ballot(slot >= before && slot < before + pieces);
+    if (who == 0) return Cut{-1, 0, 0, 0, 0};
+    const int s = __builtin_ctzll(who), first = __builtin_amdgcn_readlane(before, s), z = slot - first;
+    return Cut{s, z * chunk, (z + 1) * chunk, first, __builtin_amdgcn_readlane(pieces, s)};
+}
 // N values of a query in 32 bits, at element i.
 template <int N>
 __device__ __forceinline__ void load_q(const TreeArgs &a, bool f32, size_t i, float (&x)[N]) {
@@ -438,22 +497,33 @@ __device__ __forceinline__ void add_odd_values(const TreeArgs &a, const Stream &
     __builtin_amdgcn_wave_barrier();
 }
 
-// N elements from d0 on of packed row i, normalised, or, where the keys are split, as they are with the
-// row's maximum and sum (a lane of d0 = 0 writes those).
+// The workspace: each stream's first slot and how many it has (4 words a stream), (maximum, sum) of each slot's
+// rows, [slots][max_rows][heads], then their unnormalised outputs.
+__device__ __forceinline__ float2 *row_sums(const TreeArgs &a) { return (float2 *)((int4 *)a.ws + a.c.streams); }
+__device__ __forceinline__ float *partials(const TreeArgs &a, const TreePlan &plan) {
+    return (float *)(row_sums(a) + ((size_t)plan.slots * a.max_rows * a.heads + 1) / 2 * 2);
+}
+// Says so to the join: by the first piece's workgroup of the first head and rows.
+__device__ __forceinline__ void put_cut(const TreeArgs &a, const TreePlan &plan, const Cut &cut, int slot, int h, int rg) {
+    if (plan.slots > a.c.streams && slot == cut.first && h == 0 && rg == 0 && threadIdx.x == 0)
+        *((int4 *)a.ws + cut.stream) = make_int4(cut.first, cut.pieces, 0, 0);
+}
+// N elements from d0 on of packed row i, normalised, or, where the keys are cut, as they are with the
+// row's maximum and sum (a lane of d0 = 0 writes those) for the slot.
 template <int D, int N>
-__device__ __forceinline__ void put_row(const TreeArgs &a, const TreePlan &plan, const Stream &st, int z, int grp, int h, int i, int d0,
-                                        float M, float L, const float (&x)[N]) {
+__device__ __forceinline__ void put_row(const TreeArgs &a, const TreePlan &plan, const Stream &st, int slot, int grp, int h, int i,
+                                        int d0, float M, float L, const float (&x)[N]) {
     const int node = i / grp, head = h * grp + i - node * grp;
-    const size_t at = (size_t)(st.row0 + node) * a.heads + head;
-    if (plan.splits > 1) {
-        const size_t all_rows = (size_t)a.rows * a.heads;
-        if (d0 == 0) ((float2 *)a.ws)[(size_t)z * all_rows + at] = make_float2(M, L);
+    if (slot >= 0 && plan.slots > a.c.streams) {
+        const size_t at = (size_t)slot * a.max_rows * a.heads + node * a.heads + head;
+        if (d0 == 0) row_sums(a)[at] = make_float2(M, L);
         if (L == 0.0f) return;
-        float *po = (float *)a.ws + (size_t)plan.splits * all_rows * 2 + ((size_t)z * all_rows + at) * D + d0;
+        float *po = partials(a, plan) + at * D + d0;
 #pragma unroll
         for (int j = 0; j < N; j += 4) *(float4 *)(po + j) = make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
         return;
     }
+    const size_t at = (size_t)(st.row0 + node) * a.heads + head;
     const float inv = L == 0.0f ? 0.0f : 1.0f / L;
     const size_t o = (size_t)((int64_t)(st.row0 + node) * a.out_row + head * D + d0);
     if (a.out_dtype == ELEM_F16) {
@@ -493,16 +563,18 @@ __global__ __launch_bounds__(kThreads, KV == ELEM_F32 ? (D == 64 ? 2 : 1) : (D =
     const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // workgroups that read the same keys follow each other on one XCD, whose L2 then serves them
-    const int units = a.c.streams * a.c.heads * plan.splits;
     const int b8 = blockIdx.x >> 3, rg = b8 % plan.row_groups, unit = (b8 / plan.row_groups) * 8 + (blockIdx.x & 7);
-    if (unit >= units) return;
-    const int z = unit % plan.splits, sh = unit / plan.splits, h = sh % a.c.heads, s = sh / a.c.heads;
+    if (unit >= plan.slots * a.c.heads) return;
+    const int slot = unit / a.c.heads, h = unit - slot * a.c.heads;
+    const Cut cut = cut_of_slot(a, plan, slot);
+    const int s = cut.stream;
+    if (s < 0) return;
     const Stream st = stream_of(a, s);
     const int grp = a.heads / a.c.heads, packed = st.n * grp, first = rg * MT * 16;
     if (first >= packed) return;
     const int live = min(MT, (packed - first + 15) / 16);
     bool bad = st.bad;
-    const int beg = z * plan.chunk, end = min(beg + plan.chunk, st.total), last = end - 1;
+    const int beg = cut.beg, end = min(cut.end, st.total), last = end - 1;
     const int *table = a.c.table + (size_t)s * a.c.table_stride;
 
     Keys<KV, D> cur;
@@ -658,6 +730,7 @@ __global__ __launch_bounds__(kThreads, KV == ELEM_F32 ? (D == 64 ? 2 : 1) : (D =
     }
 
     // ---- the waves joined, one row tile at a time
+    put_cut(a, plan, cut, slot, h, rg);
     bad = __any(bad);
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
@@ -692,7 +765,7 @@ __global__ __launch_bounds__(kThreads, KV == ELEM_F32 ? (D == 64 ? 2 : 1) : (D =
 #pragma unroll
             for (int j = 0; j < ND; ++j) acc[j] = fmaf(so[v][row][d0 + j], f, acc[j]);
         }
-        put_row<D, ND>(a, plan, st, z, grp, h, i, d0, M, L, acc);
+        put_row<D, ND>(a, plan, st, slot, grp, h, i, d0, M, L, acc);
     }
 }
 
@@ -724,16 +797,18 @@ __global__ __launch_bounds__(64 * NWV, 2) void attn_tree_wide_kernel(TreeArgs a,
 
     const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int units = a.c.streams * a.c.heads * plan.splits;
     const int b8 = blockIdx.x >> 3, rg = b8 % plan.row_groups, unit = (b8 / plan.row_groups) * 8 + (blockIdx.x & 7);
-    if (unit >= units) return;
-    const int z = unit % plan.splits, sh = unit / plan.splits, h = sh % a.c.heads, s = sh / a.c.heads;
+    if (unit >= plan.slots * a.c.heads) return;
+    const int slot = unit / a.c.heads, h = unit - slot * a.c.heads;
+    const Cut cut = cut_of_slot(a, plan, slot);
+    const int s = cut.stream;
+    if (s < 0) return;
     const Stream st = stream_of(a, s);
     const int grp = a.heads / a.c.heads, packed = st.n * grp;
     if (rg * NWV * MT * 16 >= packed) return;
     const int first = (rg * NWV + w) * MT * 16;
     bool bad = st.bad;
-    const int beg = z * plan.chunk, end = min(beg + plan.chunk, st.total), last = end - 1;
+    const int beg = cut.beg, end = min(cut.end, st.total), last = end - 1;
     const int *table = a.c.table + (size_t)s * a.c.table_stride;
 
     uint4 kraw[NW];
@@ -896,6 +971,7 @@ __global__ __launch_bounds__(64 * NWV, 2) void attn_tree_wide_kernel(TreeArgs a,
         if (more) put(buf, p + STAGE);
         lds_barrier();
     }
+    put_cut(a, plan, cut, slot, h, rg);
     bad = __any(bad);
     if (lane == 0) lds.bad[w] = bad;
     lds_barrier();
@@ -913,47 +989,51 @@ __global__ __launch_bounds__(64 * NWV, 2) void attn_tree_wide_kernel(TreeArgs a,
         for (int r = 0; r < 4; ++r)
 #pragma unroll
             for (int j = 0; j < ND; ++j) y[ND * r + j] = rows.o[mt][j][r];
-        if (i < packed) put_row<D, 4 * ND>(a, plan, st, z, grp, h, i, (D / 4) * g, rows.m(mt), L, y);
+        if (i < packed) put_row<D, 4 * ND>(a, plan, st, slot, grp, h, i, (D / 4) * g, rows.m(mt), L, y);
     }
 }
 
-// The key splits of each (row, head) joined in their order: lane c holds split c's maximum and sum, and D / 4
-// lanes add up a vector with SIDE = 256 / D splits side by side, all of a wave's splits loaded at once.  Up to 4 SIDE
-// splits one wave does a row; more are shared out to the 4 waves of a workgroup and joined through LDS.
+// The pieces of each (row, head) joined in their order: lane c holds piece c's maximum and sum, and D / 4
+// lanes add up a vector with SIDE = 256 / D pieces side by side, several loads of a wave at once.  One wave does a
+// row where pieces are few, else they are shared out to the 4 waves of a workgroup and joined through LDS.
 template <int D, bool ONE_WAVE>
 __global__ __launch_bounds__(kThreads) void attn_tree_join_kernel(TreeArgs a, TreePlan plan) {
-    constexpr int G = D / 4, SIDE = 64 / G, ROUNDS = ONE_WAVE ? 4 : kMaxSplits / (kWaves * SIDE);
+    constexpr int G = D / 4, SIDE = 64 / G, ROUNDS = kMaxSplits / (kWaves * SIDE);
     __shared__ float4 part[kWaves][G];
-    const int lane = threadIdx.x & 63, splits = plan.splits;
+    const int lane = threadIdx.x & 63;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int of_stream = a.max_rows * a.heads, per = ONE_WAVE ? (of_stream + kWaves - 1) / kWaves : of_stream;
     const int s = blockIdx.x / per, i = ONE_WAVE ? (blockIdx.x - s * per) * kWaves + w : blockIdx.x - s * per;
     const Stream st = stream_of(a, s);
     if (i >= st.n * a.heads) return;
-    const size_t all_rows = (size_t)a.rows * a.heads, at = (size_t)st.row0 * a.heads + i;
+    const int4 cut = ((const int4 *)a.ws)[s];
+    const int splits = __builtin_amdgcn_readfirstlane(cut.y);
+    const size_t slot_rows = (size_t)of_stream, at = cut.x * slot_rows + i;
     float2 mine = make_float2(-INFINITY, 0.0f);
-    if (lane < splits) mine = ((const float2 *)a.ws)[(size_t)lane * all_rows + at];
+    if (lane < splits) mine = row_sums(a)[lane * slot_rows + at];
     const int d = (lane % G) * 4, side = lane / G;
     const int first = ONE_WAVE ? side : w * SIDE + side, step = ONE_WAVE ? SIDE : kWaves * SIDE;
-    const float *po = (const float *)a.ws + (size_t)splits * all_rows * 2 + at * D + d;
-    float4 x[ROUNDS];
-#pragma unroll
-    for (int r = 0; r < ROUNDS; ++r)  // (a split without keys has written none: what is read there is not used)
-        if (r * step < splits) x[r] = *(const float4 *)(po + (size_t)min(first + r * step, splits - 1) * all_rows * D);
+    const float *po = partials(a, plan) + at * D + d;
     const float M = wave_max(mine.x), M0 = M == -INFINITY ? 0.0f : M;
     const float f = exp2_(mine.x - M0), L = wave_sum(mine.y * f);
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k0 = 0; k0 < splits; k0 += ROUNDS * step) {  // (one wave: more rounds where a stream has most of the slots)
+        float4 x[ROUNDS];
 #pragma unroll
-    for (int r = 0; r < ROUNDS; ++r)
-        if (r * step < splits) {
-            const int k = first + r * step;
-            const float fk = __shfl(f, k & 63), lk = __shfl(mine.y, k & 63);
-            const bool use = k < splits && lk != 0.0f;
-            o.x = use ? fmaf(x[r].x, fk, o.x) : o.x;
-            o.y = use ? fmaf(x[r].y, fk, o.y) : o.y;
-            o.z = use ? fmaf(x[r].z, fk, o.z) : o.z;
-            o.w = use ? fmaf(x[r].w, fk, o.w) : o.w;
-        }
+        for (int r = 0; r < ROUNDS; ++r)  // (a piece without keys has written none: what is read there is not used)
+            if (k0 + r * step < splits) x[r] = *(const float4 *)(po + (size_t)min(k0 + first + r * step, splits - 1) * slot_rows * D);
+#pragma unroll
+        for (int r = 0; r < ROUNDS; ++r)
+            if (k0 + r * step < splits) {
+                const int k = k0 + first + r * step;
+                const float fk = __shfl(f, k & 63), lk = __shfl(mine.y, k & 63);
+                const bool use = k < splits && lk != 0.0f;
+                o.x = use ? fmaf(x[r].x, fk, o.x) : o.x;
+                o.y = use ? fmaf(x[r].y, fk, o.y) : o.y;
+                o.z = use ? fmaf(x[r].z, fk, o.z) : o.z;
+                o.w = use ? fmaf(x[r].w, fk, o.w) : o.w;
+            }
+    }
     if constexpr (G == 16) o.x += xshfl<16>(o.x), o.y += xshfl<16>(o.y), o.z += xshfl<16>(o.z), o.w += xshfl<16>(o.w);
     o.x += xshfl<32>(o.x), o.y += xshfl<32>(o.y), o.z += xshfl<32>(o.z), o.w += xshfl<32>(o.w);
     float y[4] = {o.x, o.y, o.z, o.w};
@@ -967,9 +1047,7 @@ __global__ __launch_bounds__(kThreads) void attn_tree_join_kernel(TreeArgs a, Tr
                    (((const float *)&part[2][lane % G])[j] + ((const float *)&part[3][lane % G])[j]);
     }
     if (side != 0) return;
-    TreePlan whole = plan;
-    whole.splits = 1;
-    put_row<D, 4>(a, whole, st, 0, a.heads, 0, i, d, M, L, y);
+    put_row<D, 4>(a, plan, st, -1, a.heads, 0, i, d, M, L, y);
 }
 
 // Rows of 16 of a workgroup: 1 or 2 in the kernel for few rows (an fp32 cache, which the wide one's fp16
@@ -985,13 +1063,13 @@ TreePlan plan_of(const KvCacheArgs &c, int heads, int max_rows, int max_keys) {
     p.group = group_tiles(c, p.tiles);
     p.row_groups = (p.tiles + p.group - 1) / p.group;
     const long long base = (long long)c.streams * c.heads * p.row_groups;
-    // enough workgroups for the chip's 256 CUs, and keys enough in a split for its start and end to pay
-    const int least = 256, want = p.group <= 2 ? 512 : 256;
-    const int spans = (max_keys + least - 1) / least;
-    int splits = (int)std::min<long long>((want + base - 1) / base, kMaxSplits);
-    splits = std::max(1, std::min(splits, spans));
+    // as many workgroups as are resident at once (3 or 2 of the kernel for few rows on a CU, one wide one), and keys
+    // enough in a piece for its start and end to pay
+    const int least = 256, want = 256 * (p.group > 2 ? 1 : (c.dim == 64 && p.group == 1 ? 3 : 2));
+    int splits = (int)std::min<long long>(want / base, kMaxSplits);
+    splits = std::max(1, std::min(splits, (max_keys + least - 1) / least));
     p.chunk = ((max_keys + splits - 1) / splits + 127) / 128 * 128;
-    p.splits = (max_keys + p.chunk - 1) / p.chunk;
+    p.slots = splits * c.streams;
     // blk / (page_size / 16) for blk < 2^24 and a divisor up to 2^11: 2^40 / d rounded up is off by
     // less than d, and blk * d < 2^40
     const uint64_t d = (uint64_t)c.page_size / 16;
@@ -1001,7 +1079,7 @@ TreePlan plan_of(const KvCacheArgs &c, int heads, int max_rows, int max_keys) {
 
 template <int KV, int D, bool LO>
 void launch_group(const TreeArgs &a, const TreePlan &p, hipStream_t s) {
-    const long long units = (long long)a.c.streams * a.c.heads * p.splits;
+    const long long units = (long long)p.slots * a.c.heads;
     const dim3 grid((unsigned)((units + 7) / 8 * 8 * p.row_groups));
     if (p.group == 1) {
         hipLaunchKernelGGL((attn_tree_kernel<KV, D, 1, LO>), grid, dim3(kThreads), 0, s, a, p);
@@ -1035,9 +1113,9 @@ hipError_t launch_kv(const TreeArgs &a, hipStream_t s) {
     else
         launch_group<KV, D, false>(a, p, s);
     const unsigned rows = (unsigned)(a.max_rows * a.heads), streams = (unsigned)a.c.streams;
-    if (p.splits > 1024 / D)
+    if (p.slots > 1024 / D * a.c.streams)
         hipLaunchKernelGGL((attn_tree_join_kernel<D, false>), dim3(streams * rows), dim3(kThreads), 0, s, a, p);
-    else if (p.splits > 1)
+    else if (p.slots > a.c.streams)
         hipLaunchKernelGGL((attn_tree_join_kernel<D, true>), dim3(streams * ((rows + kWaves - 1) / kWaves)), dim3(kThreads), 0, s, a, p);
     return hipGetLastError();
 }
@@ -1055,12 +1133,14 @@ hipError_t launch_d(const TreeArgs &a, hipStream_t s) {
 }  // namespace
 
 size_t tree_workspace(const KvCacheArgs &c, int heads, int rows, int max_rows, int max_keys) {
+    max_rows = std::min(max_rows, rows);
     const TreePlan p = plan_of(c, heads, max_rows, max_keys);
-    return p.splits == 1 ? 0 : (size_t)p.splits * rows * heads * (2 + c.dim) * sizeof(float);
+    return p.slots == c.streams ? 0 : c.streams * sizeof(int4) + ((size_t)p.slots * max_rows * heads * (2 + c.dim) + 2) * sizeof(float);
 }
 
 hipError_t launch_attn_tree(const TreeArgs &args, hipStream_t s) {
     TreeArgs a = args;
+    a.max_rows = std::min(a.max_rows, a.rows);
     a.q_vec = (uintptr_t)a.q % 16 == 0 && a.q_row * elem_size(a.q_dtype) % 16 == 0;
     a.out_vec = (uintptr_t)a.out % 16 == 0 && a.out_row * elem_size(a.out_dtype) % 16 == 0;
     return a.c.dim == 64 ? launch_d<64>(a, s) : launch_d<128>(a, s);
