@@ -1,6 +1,7 @@
 // capi.hip -- extern "C" entry points of libmoss_hip.so (declared in include/moss_hip.h).
 // No exception crosses this boundary: failures become status codes plus a
 // thread-local message (moss_hip_last_error).
+#include <algorithm>
 #include <cmath>
 #include <cstdio>
 #include <map>
@@ -698,13 +699,16 @@ int moss_hip_rope_rows(const void *x, int64_t x_row_stride, int64_t x_head_strid
         if (!x || !y || !pos || !rope) throw Status(MOSS_HIP_EINVAL, "null pointer");
         check_row_type(dtype);
         check_rows(rows);
-        if (heads <= 0 || heads > kMaxHeads || head_dim <= 0 || head_dim > 1024)
-            throw Status(MOSS_HIP_EINVAL, "need 0 < heads, head_dim <= 1024");
+        if (heads <= 0 || heads > kMaxHeads || head_dim <= 0 || head_dim > 1024 || head_dim % 2)
+            throw Status(MOSS_HIP_EINVAL, "need 0 < heads, head_dim <= 1024, and an even head_dim");
         if (x_row_stride < 0 || x_head_stride < 0 || y_row_stride < 0 || y_head_stride < 0)
             throw Status(MOSS_HIP_EINVAL, "strides must not be negative");
         if (x == y && (x_row_stride != y_row_stride || x_head_stride != y_head_stride))
             throw Status(MOSS_HIP_EINVAL, "in place, x and y must have the same strides");
-        if ((heads > 1 && y_head_stride < head_dim) || (rows > 1 && y_row_stride == 0))
+        // one of the two dimensions lies within the other's steps
+        const bool rows_apart = rows <= 1 || y_row_stride >= (heads - 1) * y_head_stride + head_dim;
+        const bool heads_apart = heads == 1 || y_head_stride >= (std::max(rows, 1) - 1) * y_row_stride + head_dim;
+        if (!(rows_apart && (heads == 1 || y_head_stride >= head_dim)) && !(heads_apart && (rows <= 1 || y_row_stride >= head_dim)))
             throw Status(MOSS_HIP_EINVAL, "rows and heads of y must not overlap");
         mh::RopeRowsArgs a;
         a.rope = rope_args(rope, head_dim);

@@ -390,7 +390,8 @@ typedef struct {
 /* y = x with the pairs of every head turned by pos[row] * freqs[i]; elements from rot_dim on are
  * copied.  x, y: dtype (F32 or F16), element (row, head, e) at row * row_stride + head * head_stride + e
  * (strides in elements, >= 0); y may be x with the same strides, and must not overlap it otherwise.
- * Angles are formed in 64 bits: positions may be any int32.  head_dim >= rot_dim. */
+ * Angles are formed in 64 bits: positions may be any int32.  head_dim is even and >= rot_dim; the rows and heads
+ * of y lie apart (rows within heads or heads within rows). */
 int moss_hip_rope_rows(const void *x, int64_t x_row_stride, int64_t x_head_stride, void *y, int64_t y_row_stride,
                        int64_t y_head_stride, int dtype, int rows, int heads, int head_dim, const int32_t *pos,
                        const moss_hip_rope *rope, void *stream);
@@ -436,7 +437,9 @@ int moss_hip_kv_read(const moss_hip_kv_cache *cache, const int32_t *row_stream, 
  * A row that attends nothing is 0 with lse -inf.  What a row does not attend may hold anything, Inf and NaN
  * too.  max_keys bounds every stream's ctx_len + n and sizes the launch.  A stream whose ctx_len is
  * negative, whose keys pass max_keys or its table, or with a page outside [0, n_pages) among them, gets
- * NaN rows; one whose row range is not within [0, rows] gets none, and rows of no stream stay as they were.
+ * NaN rows; one whose row range is not within [0, rows] gets none.  Rows of no stream, and a stream's rows past
+ * max_rows, stay as they were.  With an fp16 output and more than 32 rows * heads per key head of a stream, the softmax
+ * weights are rounded to fp16 (once, to nearest); otherwise sums, weights and statistics have 22 bits or more.
  * The same call gives the same bits.  workspace: moss_hip_attn_tree_workspace bytes (any content, 16-byte
  * aligned; NULL where that is 0). */
 int moss_hip_attn_tree(const void *q, int64_t q_stride, int q_dtype, int heads, const moss_hip_kv_cache *cache,

@@ -106,6 +106,17 @@ def test_rope_strides_and_in_place(torch_gpu, halves, dtype, pad, first):
     assert torch.equal(flat[rest], before[rest])
 
 
+def test_rope_heads_outside_rows(torch_gpu):
+    """[heads][rows][dim] in memory: rows within the steps of the heads."""
+    torch = torch_gpu
+    x = torch.randn(7, 5, 64, generator=torch.Generator().manual_seed(1)).cuda()
+    pos = torch.arange(7, dtype=torch.int32, device="cuda") * 11
+    rope = lib.Rope(64)
+    want = lib.rope_rows(x, pos, rope, torch.empty_like(x))
+    turned = torch.full((5, 7, 64), 3.0, device="cuda").transpose(0, 1)
+    assert torch.equal(lib.rope_rows(x, pos, rope, turned), want)
+
+
 def test_rope_undone_by_negated_angles(torch_gpu):
     """Negated angles are the inverse, and the gradient: <rope(x), y> = <x, rope^-1(y)>, as differences of
     the 64-bit form say too."""
@@ -417,6 +428,41 @@ def test_attn_long_context(torch_gpu, cache, dim, n):
     _check_attn(torch, c, q, start, ctx, masks, max_rows=64, max_keys=20011 + 64)
 
 
+@pytest.mark.parametrize("streams,heads,kvh,dim", [(70, 2, 1, 64), (66, 16, 1, 128), (5, 2, 2, 64), (9, 8, 1, 128)])
+def test_attn_cuts_of_ragged_streams(torch_gpu, streams, heads, kvh, dim):
+    """Keys cut into pieces over up to 64 streams by their lengths, and over more as many each: streams without rows, without
+    a context and with a bad one among long and short ones."""
+    torch = torch_gpu
+    rng = np.random.default_rng(streams)
+    ctx = [int(x) for x in rng.integers(0, 2600, streams)]
+    n = [int(x) for x in rng.integers(0, 4, streams)]
+    ctx[0], n[0], ctx[1], n[1], ctx[2] = 2600, 3, 0, 2, 1
+    n[-1] = 1
+    print(f"attn cuts {streams} {heads}/{kvh} {dim}", flush=True)
+    c, start, rows, masks, q = _attn_case(torch, "i8", dim, heads, kvh, 64, ctx, n, False, streams)
+    assert lib.attn_tree_workspace(c, heads, rows, 3, 2603) > 0
+    a = _check_attn(torch, c, q, start, ctx, masks, max_rows=3, max_keys=2603)
+    bad = list(ctx)
+    bad[-1] = -5
+    b = _run_attn(torch, c, q, start, bad, masks, 3, 2603)
+    assert np.isnan(b[0][-1]).all() and (streams > 64 or np.abs(b[0][:-1] - a[0][:-1]).max() < 1e-5)
+    # a workspace of the size that was asked for, with guards around it, full of NaN
+    size = lib.attn_tree_workspace(c, heads, rows, 3, 2603)
+    ws = torch.full((size + 512,), 255, dtype=torch.uint8, device="cuda")
+    d = _run_attn(torch, c, q, start, ctx, masks, 3, 2603, workspace=ws[256:256 + size])
+    assert np.array_equal(d[0], a[0]) and (ws[:256] == 255).all() and (ws[256 + size:] == 255).all()
+
+
+def test_attn_more_rows_than_max_rows(torch_gpu):
+    """A stream's rows past max_rows stay as they were, and are no keys."""
+    torch = torch_gpu
+    c, start, rows, masks, q = _attn_case(torch, "f16", 64, 2, 2, 16, [20, 3], [5, 2], True, 8)
+    got, lse = _run_attn(torch, c, q, start, [20, 3], None, 3, 25)
+    want, _, tol, _, _ = _attn_ref(q.numpy(), c, start, [20, 3], None, 0.125, rows, 2)
+    keep = [0, 1, 2, 5, 6]
+    assert (np.abs(got - want) <= tol)[keep].all() and (got[3:5] == 9).all() and (lse[3:5] == 9).all()
+
+
 def test_attn_empty_rows_and_masks(torch_gpu):
     """Rows that see nothing, bits beyond the stream's rows, rows of no stream, a stream without rows."""
     torch = torch_gpu
@@ -622,11 +668,11 @@ def _check_lp(torch, x, tokens, k, inv_t=1.0):
     assert np.array_equal(ids, wids), (ids[(ids != wids).any(1)][:2], wids[(ids != wids).any(1)][:2])
     assert np.array_equal(np.isnan(lp), np.isnan(wlp))
     fin = np.isfinite(wlp)
-    assert (np.abs(lp - wlp)[fin] <= tol[fin]).all(), np.max(np.abs(lp - wlp)[fin] - tol[fin])
+    assert (np.abs(lp[fin] - wlp[fin]) <= tol[fin]).all(), np.max(np.abs(lp[fin] - wlp[fin]) - tol[fin])
     assert (lp[wlp == -np.inf] == -np.inf).all()
     assert (np.abs(ent - went) <= tol).all()
     fin = np.isfinite(wtop)
-    assert np.array_equal(fin, np.isfinite(top)) and (np.abs(top - wtop)[fin] <= np.broadcast_to(tol[:, None], top.shape)[fin]).all()
+    assert np.array_equal(fin, np.isfinite(top)) and (np.abs(top[fin] - wtop[fin]) <= np.broadcast_to(tol[:, None], top.shape)[fin]).all()
 
 
 @pytest.mark.parametrize("dtype", ["f32", "f16"])
@@ -677,6 +723,19 @@ def test_token_logprobs_nan_and_inf(torch_gpu, vocab):
     assert (ids[3] == -1).all() and (top[3] == -np.inf).all() and np.isnan(top[1:3]).all()
     wlp, went, _, wtop, tol = _lp_ref(x[[0, 4]], [7, 7], 1.0, 3)
     assert (np.abs(lp[[0, 4]] - wlp) <= tol).all() and (np.abs(top[[0, 4]] - wtop) <= tol[:, None]).all()
+
+
+def test_token_logprobs_stays_in_its_workspace(torch_gpu):
+    """Guards around a workspace of the size that was asked for, odd numbers of chunks and alternatives."""
+    torch = torch_gpu
+    x = torch.randn(3, 21003, generator=torch.Generator().manual_seed(3)).cuda()
+    for k in (0, 1, 5, 32):
+        size = lib.token_logprobs_workspace(3, 21003, k)
+        assert size > 0
+        ws = torch.full((size + 512,), 255, dtype=torch.uint8, device="cuda")
+        a = _run_lp(torch, x, [1, 2, 3], k, workspace=ws[256:256 + size])
+        b = _run_lp(torch, x, [1, 2, 3], k)
+        assert all(np.array_equal(p, q) for p, q in zip(a, b)) and (ws[:256] == 255).all() and (ws[256 + size:] == 255).all()
 
 
 def test_token_logprobs_strides_and_no_extras(torch_gpu):

@@ -61,11 +61,12 @@ def test_null_structs():
 
 @pytest.mark.parametrize("i,value,word", [
     (0, None, "null"), (3, None, "null"), (10, None, "null"), (6, lib.I8, "dtype"), (7, -1, "rows"), (7, (1 << 22) + 1, "rows"),
-    (8, 0, "heads"), (9, 0, "head_dim"), (1, -1, "negative"), (4, 768, "same strides"), (5, 32, "overlap")])
+    (8, 0, "heads"), (9, 0, "head_dim"), (9, 65, "even"), (1, -1, "negative"), (4, 768, "same strides"), (5, 32, "overlap"), (4, 700, "overlap"),
+    (4, 0, "overlap"), (4, 32, "overlap")])
 def test_rope_rows_refusals(i, value, word):
     a = [P, 1024, 64, P, 1024, 64, lib.F32, 4, 12, 64, P]
     a[i] = value
-    if i == 5:
+    if word == "overlap":
         a[3] = P + 0x10000
     _refused(lib.load().moss_hip_rope_rows(*a, C.addressof(_rope()), None), word)
 
