@@ -191,25 +191,18 @@ hipError_t rope_rows_t(const RopeRowsArgs &a, hipStream_t s) {
 
 // ---------------------------------------------------------------- the paged cache
 
-// Divisions of a launch by numbers that it does not change, as products.
-struct KvShape {
-    uint32_t row_magic;  // u / (units of a row): u times 2^32 / that, rounded up (exact while their product is under 2^32)
-    int page_shift;      // page_size = 1 << page_shift, or -1
-};
-__device__ __forceinline__ int row_of(const KvShape &k, int u) { return (int)__umulhi((uint32_t)u, k.row_magic); }
-
 // Where row r of a call lives in the pools: the index of its first vector ([page][head 0][slot]) and
-// whether there is such a place.
+// whether there is such a place.  A wave has one row at a time, so all of this is scalar work.
 struct Place {
     size_t at;
     bool ok;
 };
-__device__ __forceinline__ Place place_of(const KvCacheArgs &c, const KvShape &k, int stream, int pos) {
+__device__ __forceinline__ Place place_of(const KvCacheArgs &c, int stream, int pos) {
     Place p{0, false};
     if (stream < 0 || stream >= c.streams || pos < 0) return p;
-    const int j = k.page_shift >= 0 ? pos >> k.page_shift : pos / c.page_size;
+    const int j = pos / c.page_size;
     if (j >= c.table_stride) return p;
-    const int page = c.table[(size_t)stream * c.table_stride + j];
+    const int page = __builtin_amdgcn_readfirstlane(c.table[(size_t)stream * c.table_stride + j]);
     if (page < 0 || page >= c.n_pages) return p;
     p.at = (size_t)page * c.heads * c.page_size + (pos - j * c.page_size);
     p.ok = true;
@@ -226,87 +219,88 @@ __device__ __forceinline__ uint32_t group_max(uint32_t v) {
     return v;
 }
 
-// Rows into the pools.  A group of D / 8 lanes holds one (row, head) of K or V, 8 elements a lane.
+constexpr int kUnits = 4;  // of a lane at a time
+
+// Rows into the pools: a wave a row.  A unit is 8 elements of K or V; the row's units, K's heads then V's, go to the
+// lanes in turn, kUnits a lane at a time and their loads before the angles are formed, which lane p keeps
+// in LDS for the row.  A group of D / 8 lanes holds one head.
 // 8-bit caches: with t = max|x| over the head and d = t / 127 (int8) or t / 448 (e4m3), the stored
 // value is x (1 / d) rounded to nearest even, so |x - q d| <= d / 2 (int8) or |q d| 2^-4 (e4m3).  A d
 // under 2^-126 is stored as 0 (its reciprocal would not be finite).  A head with an Inf or NaN gets
 // the scale NaN and reads back as NaN, as quantising it would otherwise hide it.  The maximum is
 // taken over the magnitudes' bit patterns, in which Inf and NaN are largest.
 // Memory bound; the rotation of the keys is done here so that they do not go through memory twice.
-// A thread has N units (8 elements of K or V of one head) in flight at a time, the first before the angles.
-template <class T, int KV, int D, int N>
-__global__ __launch_bounds__(kThreads) void kv_write_kernel(KvRowsArgs a, KvShape shape, int rpb) {
-    extern __shared__ float2 cs[];  // [rpb][rot / 2]
+template <class T, int KV, int D>
+__global__ __launch_bounds__(kThreads) void kv_write_kernel(KvRowsArgs a, int table_words) {
+    extern __shared__ float2 cs[];  // [waves][rot / 2], rounded up to what lanes read at once
     constexpr int L = D / 8;
-    const int t = threadIdx.x, l = t % L;
-    const int row0 = blockIdx.x * rpb, nrow = min(rpb, a.rows - row0);
-    const int half = a.rope.rot / 2, heads = a.c.heads;
+    const int lane = threadIdx.x & 63, l = lane % L;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = blockIdx.x * (blockDim.x >> 6) + w;
+    if (r >= a.rows) return;
+    const int half = a.rope.rot / 2, of_k = a.c.heads * L, units = 2 * of_k;
     const bool rope = a.rope.freqs != nullptr, apart = a.rope.halves && half % 8 == 0;
-    const int per_row = 2 * heads * L, units = nrow * per_row;  // K then V
+    const T *k = (const T *)a.k + r * a.k_row, *v = (const T *)a.v + r * a.v_row - (size_t)of_k * 8;
     // with halves of whole pieces, the partners of this lane's 8 elements are 8 others
     const bool upper = 8 * l >= half, turned = 8 * l < 2 * half;
     const int mate = !turned ? 0 : (upper ? -half : half);
-    Raw<T, 8> raw[N], other[N];
-    const T *src[N];
-    size_t vecs[N];
-    int row[N];
-    bool is_v[N], ok[N];
+    // a lane reads the angles of its 8 elements (4 pairs): angle p is kept at (p % per lane) * pitch + p / per lane, so that
+    // lanes read neighbouring words
+    const int lanes_at = apart ? 3 : (a.rope.halves ? 0 : 2), pitch = (half + (1 << lanes_at) - 1) >> lanes_at;
+    float2 *angles = cs + w * table_words;
+    Raw<T, 8> raw[kUnits], other[kUnits];
     auto load = [&](int u0) {
 #pragma unroll
-        for (int n = 0; n < N; ++n) {  // (a unit past the last is the last, and not written: groups are whole)
-            const int u = u0 + n * kThreads < units ? u0 + n * kThreads : units - L + l;
-            row[n] = row_of(shape, u);
-            const int g = (u - row[n] * per_row) / L, r = row0 + row[n];
-            is_v[n] = g >= heads;
-            const int h = is_v[n] ? g - heads : g;
-            src[n] = (is_v[n] ? (const T *)a.v + r * a.v_row : (const T *)a.k + r * a.k_row) + h * D;
-            raw[n] = load_raw<T, 8>(src[n] + 8 * l);
-            if (rope && apart && !is_v[n]) other[n] = load_raw<T, 8>(src[n] + 8 * l + mate);
-            vecs[n] = (size_t)h * a.c.page_size;
-        }
-#pragma unroll
-        for (int n = 0; n < N; ++n) {
-            const Place at = place_of(a.c, shape, a.stream[row0 + row[n]], a.pos[row0 + row[n]]);
-            vecs[n] += at.at;
-            ok[n] = at.ok && u0 + n * kThreads < units;
+        for (int n = 0; n < kUnits; ++n) {
+            const int u = u0 + 64 * n;
+            if (u < units) {
+                raw[n] = load_raw<T, 8>((u < of_k ? k : v) + 8 * u);
+                if (rope && apart && u < of_k) other[n] = load_raw<T, 8>(k + 8 * u + mate);
+            }
         }
     };
-    load(t);
+    load(lane);
+    const Place place = place_of(a.c, __builtin_amdgcn_readfirstlane(a.stream[r]), __builtin_amdgcn_readfirstlane(a.pos[r]));
+    if (!place.ok) return;
     if (rope) {
-        const int *pos = a.rope_pos != nullptr ? a.rope_pos : a.pos;
-        for (int i = t; i < nrow * half; i += kThreads) {
-            const int r = i / half;
-            cs[i] = turn(pos[row0 + r], a.rope.freqs[i - r * half], a.rope.mscale);
-        }
-        __syncthreads();
+        const int pos = __builtin_amdgcn_readfirstlane(a.rope_pos != nullptr ? a.rope_pos[r] : a.pos[r]);
+        for (int p = lane; p < half; p += 64)
+            angles[(p & ((1 << lanes_at) - 1)) * pitch + (p >> lanes_at)] = turn(pos, a.rope.freqs[p], a.rope.mscale);
+        // written and read by lanes of this one wave
+        __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+        __builtin_amdgcn_wave_barrier();
     }
-    for (int u0 = t; u0 < units; u0 += N * kThreads) {
-        if (u0 != t) load(u0);
+    for (int u0 = lane; u0 < units; u0 += 64 * kUnits) {
+        if (u0 != lane) load(u0);
 #pragma unroll
-        for (int n = 0; n < N; ++n) {
+        for (int n = 0; n < kUnits; ++n) {
+            const int u = u0 + 64 * n;
+            if (u >= units) break;  // (whole groups of lanes)
+            const bool is_v = u >= of_k;
+            const int h = (is_v ? u - of_k : u) / L;
             float x[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) x[i] = Elem<T>::get(raw[n].e[i]);
-            if (rope && !is_v[n]) {
-                const float2 *c = cs + row[n] * half;
+            if (rope && !is_v) {
                 if (apart) {
                     if (turned) {
-                        c += 8 * l - (upper ? half : 0);
+                        const float2 *c = angles + l - (upper ? half / 8 : 0);
 #pragma unroll
                         for (int i = 0; i < 8; ++i) {
                             const float b = Elem<T>::get(other[n].e[i]);
-                            x[i] = fmaf(upper ? b : -b, c[i].y, x[i] * c[i].x);
+                            const float2 t = c[i * pitch];
+                            x[i] = fmaf(upper ? b : -b, t.y, x[i] * t.x);
                         }
                     }
                 } else if (a.rope.halves) {
+                    const T *src = k + h * D;
 #pragma unroll 1
                     for (int i = 0; i < 8; ++i) {
                         const int e = 8 * l + i;
                         if (e < 2 * half) {
                             const bool up = e >= half;
-                            const float b = Elem<T>::get(src[n][up ? e - half : e + half]);
-                            const float2 w = c[up ? e - half : e];
-                            const float y = fmaf(up ? b : -b, w.y, Elem<T>::get(src[n][e]) * w.x);
+                            const float b = Elem<T>::get(src[up ? e - half : e + half]);
+                            const float2 t = angles[up ? e - half : e];
+                            const float y = fmaf(up ? b : -b, t.y, Elem<T>::get(src[e]) * t.x);
 #pragma unroll
                             for (int j = 0; j < 8; ++j) x[j] = j == i ? y : x[j];
                         }
@@ -314,15 +308,15 @@ __global__ __launch_bounds__(kThreads) void kv_write_kernel(KvRowsArgs a, KvShap
                 } else {
 #pragma unroll
                     for (int i = 0; i < 8; i += 2)
-                        if (8 * l + i < 2 * half) rotate(x[i], x[i + 1], c[4 * l + i / 2], x[i], x[i + 1]);
+                        if (8 * l + i < 2 * half) rotate(x[i], x[i + 1], angles[i / 2 * pitch + l], x[i], x[i + 1]);
                 }
             }
-            const size_t o = vecs[n] * D + 8 * l;
-            void *pool = is_v[n] ? a.c.v : a.c.k;
+            const size_t vec = place.at + (size_t)(unsigned)(h * a.c.page_size), o = vec * D + 8 * l;
+            void *pool = is_v ? a.c.v : a.c.k;
             if constexpr (KV == ELEM_F32) {
-                if (ok[n]) store8((float *)pool + o, x);
+                store8((float *)pool + o, x);
             } else if constexpr (KV == ELEM_F16) {
-                if (ok[n]) store8((__half *)pool + o, x);
+                store8((__half *)pool + o, x);
             } else {
                 constexpr float top = KV == ELEM_I8 ? 127.0f : 448.0f;
                 uint32_t mb = 0;
@@ -333,124 +327,106 @@ __global__ __launch_bounds__(kThreads) void kv_write_kernel(KvRowsArgs a, KvShap
                 float d = __uint_as_float(mb) / top;
                 if (bad || d < 1.17549435e-38f) d = 0.0f;
                 const float id = d > 0.0f ? 1.0f / d : 0.0f;
-                uint32_t w[2] = {0, 0};
-                if (!bad) {
+                // |x id| passes the top by 2^-22 of it at most (three roundings), which rounds back to it: no clamp
+                uint32_t q[2];
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) x[i] = fminf(fmaxf(x[i] * id, -top), top);
+                for (int i = 0; i < 2; ++i) {
+#pragma clang fp contract(off)  // the product is rounded before it is rounded to a whole number
+                    float y[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) y[j] = x[4 * i + j] * id;
                     if constexpr (KV == ELEM_I8) {
+                        // 1.5 * 2^23 + y: the sum's low byte is y rounded to nearest even
+                        uint32_t b[4];
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) w[i / 4] |= ((uint32_t)(int)rintf(x[i]) & 0xffu) << (8 * (i & 3));
+                        for (int j = 0; j < 4; ++j) b[j] = __float_as_uint(y[j] + 12582912.0f);
+                        q[i] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(b[3], b[2], 0x0c0c0400u), __builtin_amdgcn_perm(b[1], b[0], 0x0c0c0400u),
+                                                     0x05040100u);
                     } else {
-#pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            const int p = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i], x[4 * i + 1], 0, false);
-                            w[i] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i + 2], x[4 * i + 3], p, true);
-                        }
+                        const int p = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
+                        q[i] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], p, true);
                     }
+                    if (bad) q[i] = 0;
                 }
-                if (ok[n]) {
-                    *(uint2 *)((uint8_t *)pool + o) = make_uint2(w[0], w[1]);
-                    if (l == 0) (is_v[n] ? a.c.v_scale : a.c.k_scale)[vecs[n]] = bad ? __uint_as_float(0x7fc00000u) : d;
-                }
+                *(uint2 *)((uint8_t *)pool + o) = make_uint2(q[0], q[1]);
+                if (l == 0) (is_v ? a.c.v_scale : a.c.k_scale)[vec] = bad ? __uint_as_float(0x7fc00000u) : d;
             }
         }
     }
 }
 
-// Rows out of the pools: q d in 32 bits, rounded once to the output's type.  Rows with no place in
+// Rows out of the pools, a wave a row: q d in 32 bits, rounded once to the output's type.  Rows with no place in
 // the cache (a position past the table, a page outside the pools) are NaN; a negative position is
-// padding and its row stays as it was.  N units of a thread in flight, as in the write.
-template <class T, int KV, int D, int N>
-__global__ __launch_bounds__(kThreads) void kv_read_kernel(KvRowsArgs a, KvShape shape, int rpb) {
+// padding and its row stays as it was.
+template <class T, int KV, int D>
+__global__ __launch_bounds__(kThreads) void kv_read_kernel(KvRowsArgs a) {
     constexpr int L = D / 8;
-    constexpr int RAW = KV == ELEM_F32 ? 32 : (KV == ELEM_F16 ? 16 : 8);  // bytes of a unit
-    const int row0 = blockIdx.x * rpb, nrow = min(rpb, a.rows - row0);
-    const int per_row = 2 * a.c.heads * L, units = nrow * per_row;
-    for (int u0 = threadIdx.x; u0 < units; u0 += N * kThreads) {
-        T *dst[N];
-        size_t vecs[N];
-        bool is_v[N], ok[N], put[N];
+    constexpr int E = KV == ELEM_F32 ? 4 : (KV == ELEM_F16 ? 2 : 1);
+    const int lane = threadIdx.x & 63;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = blockIdx.x * (blockDim.x >> 6) + w;
+    if (r >= a.rows) return;
+    const int of_k = a.c.heads * L, units = 2 * of_k;
+    const int pos = __builtin_amdgcn_readfirstlane(a.pos[r]);
+    if (pos < 0) return;
+    const Place place = place_of(a.c, __builtin_amdgcn_readfirstlane(a.stream[r]), pos);
+    T *k = (T *)a.k_out + r * a.k_row, *v = (T *)a.v_out + r * a.v_row - (size_t)of_k * 8;
+    for (int u0 = lane; u0 < units; u0 += 64 * kUnits) {
+        uint32_t raw[kUnits][2 * E];
+        float d[kUnits];
 #pragma unroll
-        for (int n = 0; n < N; ++n) {
-            const int u = min(u0 + n * kThreads, units - 1);
-            const int rl = row_of(shape, u), rest = u - rl * per_row, g = rest / L, l = rest - g * L, r = row0 + rl;
-            is_v[n] = g >= a.c.heads;
-            const int h = is_v[n] ? g - a.c.heads : g, pos = a.pos[r];
-            const Place at = place_of(a.c, shape, a.stream[r], pos);
-            ok[n] = at.ok;
-            put[n] = pos >= 0 && u0 + n * kThreads < units;
-            vecs[n] = at.ok ? at.at + (size_t)h * a.c.page_size : 0;  // (0: any vector that exists)
-            dst[n] = (is_v[n] ? (T *)a.v_out + r * a.v_row : (T *)a.k_out + r * a.k_row) + h * D + 8 * l;
-        }
-        const int l = threadIdx.x % L;
-        uint4 raw[N][RAW > 16 ? 2 : 1];
-        float d[N];
-#pragma unroll
-        for (int n = 0; n < N; ++n) {
-            const char *p = (const char *)(is_v[n] ? a.c.v : a.c.k) + (vecs[n] * D + 8 * l) * elem_size(KV);
-            if constexpr (RAW == 8) {
-                const uint2 w = *(const uint2 *)p;
-                raw[n][0] = make_uint4(w.x, w.y, 0, 0);
-                d[n] = (is_v[n] ? a.c.v_scale : a.c.k_scale)[vecs[n]];
-            } else {
-#pragma unroll
-                for (int i = 0; i < RAW / 16; ++i) raw[n][i] = ((const uint4 *)p)[i];
+        for (int n = 0; n < kUnits; ++n) {
+            const int u = u0 + 64 * n;
+            if (u < units && place.ok) {
+                const bool is_v = u >= of_k;
+                const int h = (is_v ? u - of_k : u) / L;
+                const size_t vec = place.at + (size_t)(unsigned)(h * a.c.page_size);
+                __builtin_memcpy(raw[n], __builtin_assume_aligned((const char *)(is_v ? a.c.v : a.c.k) + (vec * D + 8 * (u % L)) * E, 8 * E > 16 ? 16 : 8 * E),
+                                 8 * E);
+                if constexpr (E == 1) d[n] = (is_v ? a.c.v_scale : a.c.k_scale)[vec];
             }
         }
 #pragma unroll
-        for (int n = 0; n < N; ++n) {
+        for (int n = 0; n < kUnits; ++n) {
+            const int u = u0 + 64 * n;
+            if (u >= units) break;
             float x[8];
             if constexpr (KV == ELEM_F32) {
                 __builtin_memcpy(x, raw[n], 32);
             } else if constexpr (KV == ELEM_F16) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) x[i] = __half2float(((const __half *)raw[n])[i]);
+                for (int i = 0; i < 8; ++i) x[i] = h2f((uint16_t)(raw[n][i / 2] >> (16 * (i & 1))));
             } else {
-                const uint32_t w[2] = {raw[n][0].x, raw[n][0].y};
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     if constexpr (KV == ELEM_I8) {
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) x[4 * i + j] = (float)(int8_t)(w[i] >> (8 * j)) * d[n];
+                        for (int j = 0; j < 4; ++j) x[4 * i + j] = (float)(int8_t)(raw[n][i] >> (8 * j)) * d[n];
                     } else {
-                        x[4 * i] = __builtin_amdgcn_cvt_f32_fp8((int)w[i], 0) * d[n];
-                        x[4 * i + 1] = __builtin_amdgcn_cvt_f32_fp8((int)w[i], 1) * d[n];
-                        x[4 * i + 2] = __builtin_amdgcn_cvt_f32_fp8((int)w[i], 2) * d[n];
-                        x[4 * i + 3] = __builtin_amdgcn_cvt_f32_fp8((int)w[i], 3) * d[n];
+                        x[4 * i] = __builtin_amdgcn_cvt_f32_fp8((int)raw[n][i], 0) * d[n];
+                        x[4 * i + 1] = __builtin_amdgcn_cvt_f32_fp8((int)raw[n][i], 1) * d[n];
+                        x[4 * i + 2] = __builtin_amdgcn_cvt_f32_fp8((int)raw[n][i], 2) * d[n];
+                        x[4 * i + 3] = __builtin_amdgcn_cvt_f32_fp8((int)raw[n][i], 3) * d[n];
                     }
                 }
             }
+            if (!place.ok)
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (!ok[n]) x[i] = __uint_as_float(0x7fc00000u);
-            if (put[n]) store8(dst[n], x);
+                for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(0x7fc00000u);
+            store8((u < of_k ? k : v) + 8 * u, x);
         }
     }
 }
 
-// Several units a thread once that leaves 512 workgroups, else one (a step's few rows).
-constexpr int kWriteUnits = 2;
+// A workgroup of 4 rows, or of one where rows are few (a step's).
 template <class T, bool READ, int KV, int D>
 hipError_t kv_launch(const KvRowsArgs &a, hipStream_t s) {
-    constexpr int N = READ ? 4 : kWriteUnits;
-    const int units = 2 * a.c.heads * (D / 8), rpb_n = std::max(1, N * kThreads / units);
-    const bool many = (a.rows + rpb_n - 1) / rpb_n >= 512;
-    const int rpb = many ? rpb_n : std::max(1, kThreads / units), blocks = (a.rows + rpb - 1) / rpb;
-    const size_t lds = a.rope.freqs ? (size_t)rpb * (a.rope.rot / 2) * sizeof(float2) : 0;
-    const KvShape shape{(uint32_t)(((1ull << 32) + units - 1) / units),
-                        (a.c.page_size & (a.c.page_size - 1)) == 0 ? __builtin_ctz(a.c.page_size) : -1};
+    const int waves = a.rows >= 2048 ? kThreads / 64 : 1, blocks = (a.rows + waves - 1) / waves;
+    const int words = a.rope.freqs ? (a.rope.rot / 2 + 7) / 8 * 8 : 0;
     (void)hipGetLastError();
-    if constexpr (READ) {
-        if (many)
-            hipLaunchKernelGGL((kv_read_kernel<T, KV, D, 4>), dim3(blocks), dim3(kThreads), 0, s, a, shape, rpb);
-        else
-            hipLaunchKernelGGL((kv_read_kernel<T, KV, D, 1>), dim3(blocks), dim3(kThreads), 0, s, a, shape, rpb);
-    } else {
-        if (many)
-            hipLaunchKernelGGL((kv_write_kernel<T, KV, D, kWriteUnits>), dim3(blocks), dim3(kThreads), lds, s, a, shape, rpb);
-        else
-            hipLaunchKernelGGL((kv_write_kernel<T, KV, D, 1>), dim3(blocks), dim3(kThreads), lds, s, a, shape, rpb);
-    }
+    if constexpr (READ)
+        hipLaunchKernelGGL((kv_read_kernel<T, KV, D>), dim3(blocks), dim3(64 * waves), 0, s, a);
+    else
+        hipLaunchKernelGGL((kv_write_kernel<T, KV, D>), dim3(blocks), dim3(64 * waves), waves * words * sizeof(float2), s, a, words);
     return hipGetLastError();
 }
 
