@@ -223,7 +223,7 @@ struct Cut {
 };
 // Up to 64 streams share the slots out by their lengths: pieces of the fewest keys (a multiple of 128, at least 256)
 // of which there are no more than slots, so that no workgroup has much more to do than another, however
-// ragged the streams (8 of 8192 to 16384 keys and one just begun: 204 us with as many pieces each, 168 so).  Every
+// ragged the streams (7 of 8192 to 16384 keys and one just begun: 203 us with as many pieces each, 172 so).  Every
 // wave finds that size for itself, lane s holding stream s.  More streams: as many slots each.
 __device__ __forceinline__ int even_chunk(const TreeArgs &a, const TreePlan &plan, int &mine) {
     const int lane = threadIdx.x & 63;
@@ -550,9 +550,13 @@ __device__ __forceinline__ void put_row(const TreeArgs &a, const TreePlan &plan,
     if (a.lse != nullptr && d0 == 0) a.lse[at] = L == 0.0f ? -INFINITY : (M + log2f(L)) * kLn2;
 }
 
-// Few rows (up to 2 tiles): memory bound.  Each of the 4 waves takes every 4th span of 32 keys, the next
+// Few rows (up to 4 tiles, 2 of a workgroup): memory bound.  Each of the 4 waves takes every 4th span of 32 keys, the next
 // span's loads in flight while one is worked on, and the waves are joined through LDS.
 // LO: 32-bit queries, as hi + lo.
+// One row over 130001 e4m3 keys of 8 x 128, 32 heads: 51.6 us and 4.8 of the join, 5.3 TB/s.  64 streams of 270 to 541
+// int8 keys of 12 x 64: 15.5 us; 16 trees of 14 to 27 over 507 to 1015 fp16 keys of 12 x 64: 17.0 and 4.1.  The last two are
+// short of it by their chain of dependent loads (row range, page, keys, then 4 or 5 spans a wave) and by vector work, about
+// 300 instructions a span.
 template <int KV, int D, int MT, bool LO>
 __global__ __launch_bounds__(kThreads, KV == ELEM_F32 ? (D == 64 ? 2 : 1) : (D == 64 && MT == 1 ? 3 : 2)) void attn_tree_kernel(TreeArgs a, TreePlan plan) {
     constexpr bool F32 = KV == ELEM_F32, SCALED = quantised(KV);
@@ -769,13 +773,18 @@ __global__ __launch_bounds__(kThreads, KV == ELEM_F32 ? (D == 64 ? 2 : 1) : (D =
     }
 }
 
-// Many rows (more than 32): bound by the matrix and vector units.  Every wave has MT row tiles of its own and all
+// Many rows (more than 64): bound by the matrix and vector units.  Every wave has MT row tiles of its own and all
 // of them the same keys, which they prepare together: of a stage of 16 keys a wave each turns its block into
 // fragments, K and V, and puts them into LDS in the order in which the products read them (16 bytes a lane, no
 // bank conflicts), so a key is converted once for up to 256 rows.  Two stages: while one is worked on the next
 // one's loads are in flight, and it is written before the only barrier of a stage.
 // PLO: weights as hi + lo; where the output is fp16 they are rounded to fp16 once, to nearest: an error of the
-// size of the output's own rounding, for a quarter of the products less.
+// size of the output's own rounding (2.9e-4 in all where rounding the output alone gives 2.1e-4), for a third of the
+// products less: 211 and 255 us when that was measured.
+// 8 streams with trees of 33 to 64, 32 heads of 128 on 8 key heads, 8192 to 16384 int8 keys: 172 us and 9.3 of the join.
+// The vector unit is what is busy most: 72 us of the softmax (a score: scale, maximum, exponential of 4 slots, sum, value
+// scale, packing) and the conversions, 33 of the matrix unit, and little of the one falls under the other with two
+// waves to a SIMD.  Products of the next span issued ahead of the weights of one: 182.
 template <int KV, int D, int NWV>
 struct WideLds {
     uint4 k[2][NWV][D / 32][64];
@@ -995,7 +1004,8 @@ __global__ __launch_bounds__(64 * NWV, 2) void attn_tree_wide_kernel(TreeArgs a,
 
 // The pieces of each (row, head) joined in their order: lane c holds piece c's maximum and sum, and D / 4
 // lanes add up a vector with SIDE = 256 / D pieces side by side, several loads of a wave at once.  One wave does a
-// row where pieces are few, else they are shared out to the 4 waves of a workgroup and joined through LDS.
+// row where pieces are few (about 4 of 12400 rows of 128: 9.3 us; a workgroup a row: 16.8), else they are shared out to the
+// 4 waves of a workgroup and joined through LDS (64 of 32 rows: 4.8 us; one wave a row: 14).
 template <int D, bool ONE_WAVE>
 __global__ __launch_bounds__(kThreads) void attn_tree_join_kernel(TreeArgs a, TreePlan plan) {
     constexpr int G = D / 4, SIDE = 64 / G, ROUNDS = kMaxSplits / (kWaves * SIDE);
@@ -1050,11 +1060,14 @@ __global__ __launch_bounds__(kThreads) void attn_tree_join_kernel(TreeArgs a, Tr
     put_row<D, 4>(a, plan, st, -1, a.heads, 0, i, d, M, L, y);
 }
 
-// Rows of 16 of a workgroup: 1 or 2 in the kernel for few rows (an fp32 cache, which the wide one's fp16
-// fragments cannot hold, takes it always), else 4, 8 or 16.
+// Rows of 16 of a workgroup: 1 or 2 in the kernel for few rows, 8 or 16 in the wide one.  With 3 and 4 tiles the keys are
+// read twice by the one and still sooner done (16 trees of 64 over 1015 fp16 keys of 12 x 64: 21.9 us, a wide workgroup of 4
+// waves 27.4; 4 over 4000 int8 keys 22.6 and 25.1); with 8 they are not (8 trees of 32 x 4 heads a key head over 16384 int8
+// keys of 128: 165 and 122; over 8000 fp16 keys, 80 rows: 104 and 61).  An fp32 cache, which the wide one's fp16 fragments
+// cannot hold, takes the first always.
 int group_tiles(const KvCacheArgs &c, int tiles) {
-    if (tiles <= 2 || c.dtype == ELEM_F32) return std::min(tiles, 2);
-    return tiles <= 4 ? 4 : (tiles <= 8 ? 8 : 16);
+    if (tiles <= 4 || c.dtype == ELEM_F32) return std::min(tiles, 2);
+    return tiles <= 8 ? 8 : 16;
 }
 
 TreePlan plan_of(const KvCacheArgs &c, int heads, int max_rows, int max_keys) {
@@ -1087,11 +1100,7 @@ void launch_group(const TreeArgs &a, const TreePlan &p, hipStream_t s) {
         hipLaunchKernelGGL((attn_tree_kernel<KV, D, 2, LO>), grid, dim3(kThreads), 0, s, a, p);
     } else if constexpr (KV != ELEM_F32) {
         const bool f16 = a.out_dtype == ELEM_F16;
-        if (p.group == 4 && f16)
-            hipLaunchKernelGGL((attn_tree_wide_kernel<KV, D, 4, 1, LO, false>), grid, dim3(256), 0, s, a, p);
-        else if (p.group == 4)
-            hipLaunchKernelGGL((attn_tree_wide_kernel<KV, D, 4, 1, LO, true>), grid, dim3(256), 0, s, a, p);
-        else if (p.group == 8 && f16)
+        if (p.group == 8 && f16)
             hipLaunchKernelGGL((attn_tree_wide_kernel<KV, D, 8, 1, LO, false>), grid, dim3(512), 0, s, a, p);
         else if (p.group == 8)
             hipLaunchKernelGGL((attn_tree_wide_kernel<KV, D, 8, 1, LO, true>), grid, dim3(512), 0, s, a, p);

@@ -12,6 +12,10 @@
 // reach the k-th of a wave's, and at least k reach the least of the four waves' (k / 4)-th, so only
 // values at or above the larger of those are candidates -- in practice a few more than k of
 // thousands.  A candidate's rank is the number of better ones.
+//
+// 16 rows of 1024 with 5 alternatives 5.0 us; 181 of 16384 with 20 12.0 us, of which the sums alone take 5.0 (2.4 TB/s) and
+// the rest is the chain of sort, marks, second reads and ranks; 3 fp16 rows of 130001 with 8 6.1 and 4.8 of the join.
+// Few rows are a chain of dependent steps, not memory.
 #include <algorithm>
 
 #include "paged_ops.h"
@@ -329,7 +333,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_join_kernel(LogprobArgs a, 
 }
 
 // Values a thread holds.  Up to 16384 logits a row is one chunk: one launch and no join.  A longer one is cut finely
-// while there are few, so that they fill the chip.
+// while there are few, so that they fill the chip (3 rows of 130001: 10.6 us, in chunks of 8192 11.9).
 int ept_of(int rows, int vocab) {
     for (int ept = 4; ept <= 64; ept *= 2)
         if (vocab <= ept * kThreads) return ept;

@@ -95,7 +95,8 @@ __device__ __forceinline__ void rotate(float a, float b, float2 cs, float &x, fl
 // and their V partners half a rotation further; then the V-element pieces behind rot.
 // Memory bound: every element is read and written once, in 16-byte pieces where head_dim and
 // (halves) rot / 2 are made of such, and a thread has N units' loads in flight, the first N before the
-// angles are formed.
+// angles are formed.  8191 rows of 40 heads x 128 fp16, three quarters of each turned: 33.5 us, 5.0 TB/s,
+// what a 1 GiB copy reaches (5.08); one unit at a time, a row a workgroup: 51.
 template <class T, bool HALVES, int V, int N>
 __global__ __launch_bounds__(kThreads) void rope_rows_kernel(RopeRowsArgs a, int rpb, int per_head) {
     extern __shared__ float2 cs[];  // [rpb][rot / 2]
@@ -229,7 +230,10 @@ constexpr int kUnits = 4;  // of a lane at a time
 // under 2^-126 is stored as 0 (its reciprocal would not be finite).  A head with an Inf or NaN gets
 // the scale NaN and reads back as NaN, as quantising it would otherwise hide it.  The maximum is
 // taken over the magnitudes' bit patterns, in which Inf and NaN are largest.
-// Memory bound; the rotation of the keys is done here so that they do not go through memory twice.
+// Memory and vector work are near each other (about 180 instructions a unit: the quotients, the rotation, the
+// packing); the rotation of the keys is done here so that they do not go through memory twice.  16001 rows of
+// 8 x 128 fp16 into e4m3, keys turned: 30.4 us, 3.3 TB/s (a thread a unit of any row, its place in vector
+// registers: 42.8).  2603 rows of 12 x 64 into int8: 7.9 us.
 template <class T, int KV, int D>
 __global__ __launch_bounds__(kThreads) void kv_write_kernel(KvRowsArgs a, int table_words) {
     extern __shared__ float2 cs[];  // [waves][rot / 2], rounded up to what lanes read at once
@@ -357,7 +361,7 @@ __global__ __launch_bounds__(kThreads) void kv_write_kernel(KvRowsArgs a, int ta
 
 // Rows out of the pools, a wave a row: q d in 32 bits, rounded once to the output's type.  Rows with no place in
 // the cache (a position past the table, a page outside the pools) are NaN; a negative position is
-// padding and its row stays as it was.
+// padding and its row stays as it was.  Memory bound: 16001 rows of 8 x 128 out of e4m3 as fp16 17.9 us, 5.5 TB/s.
 template <class T, int KV, int D>
 __global__ __launch_bounds__(kThreads) void kv_read_kernel(KvRowsArgs a) {
     constexpr int L = D / 8;
@@ -417,7 +421,8 @@ __global__ __launch_bounds__(kThreads) void kv_read_kernel(KvRowsArgs a) {
     }
 }
 
-// A workgroup of 4 rows, or of one where rows are few (a step's).
+// A workgroup of 4 rows, or of one where rows are few (a step's 64 rows of
+// 12 x 64, written and read: 5.8 us, by fours 6.1).
 template <class T, bool READ, int KV, int D>
 hipError_t kv_launch(const KvRowsArgs &a, hipStream_t s) {
     const int waves = a.rows >= 2048 ? kThreads / 64 : 1, blocks = (a.rows + waves - 1) / waves;

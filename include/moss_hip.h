@@ -438,7 +438,7 @@ int moss_hip_kv_read(const moss_hip_kv_cache *cache, const int32_t *row_stream, 
  * too.  max_keys bounds every stream's ctx_len + n and sizes the launch.  A stream whose ctx_len is
  * negative, whose keys pass max_keys or its table, or with a page outside [0, n_pages) among them, gets
  * NaN rows; one whose row range is not within [0, rows] gets none.  Rows of no stream, and a stream's rows past
- * max_rows, stay as they were.  With an fp16 output and more than 32 rows * heads per key head of a stream, the softmax
+ * max_rows, stay as they were.  With an fp16 output and max_rows * (heads / kv_heads) > 64, the softmax
  * weights are rounded to fp16 (once, to nearest); otherwise sums, weights and statistics have 22 bits or more.
  * The same call gives the same bits.  workspace: moss_hip_attn_tree_workspace bytes (any content, 16-byte
  * aligned; NULL where that is 0). */

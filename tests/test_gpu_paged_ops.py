@@ -377,9 +377,9 @@ def _check_attn(torch, c, q, start, ctx, masks, odt="f32", max_rows=None, max_ke
     want, wl, tol, ltol, avg = _attn_ref(q.float().numpy(), c, start, ctx, masks, c.head_dim ** -0.5 if scale is None else scale,
                                          q.shape[0], q.shape[1])
     if odt == "f16":
-        # the output's rounding, 2^-11 of it; with more than 32 packed rows the weights are fp16 too, each off by up to
+        # the output's rounding, 2^-11 of it; with more than 64 packed rows the weights are fp16 too, each off by up to
         # 2^-11 of itself (times a value scale, as the sum is), so sum p v by up to 2^-11 sum p |v|
-        tol = tol + np.abs(want) * U16 + 2.0 ** -25 + (avg * U16 if n.max() * q.shape[1] // c.kv_heads > 32 and c.tensors[0].dtype != torch.float32 else 0)
+        tol = tol + np.abs(want) * U16 + 2.0 ** -25 + (avg * U16 if (max_rows or n.max()) * q.shape[1] // c.kv_heads > 64 and c.tensors[0].dtype != torch.float32 else 0)
     bad = np.abs(got - want) > tol
     assert not bad.any(), (np.argwhere(bad)[:5], np.max(np.abs(got - want)), tol[bad][:5])
     fin = np.isfinite(wl)
