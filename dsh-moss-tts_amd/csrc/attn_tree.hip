@@ -405,13 +405,15 @@ struct Rows {
     __device__ __forceinline__ float m(int mt) const { return ref[mt] - up; }
     // A new up for all rows, before their next scores.
     __device__ __forceinline__ void raise(float up_new) {
-        const float f = exp2_((up_new - up) * 0.5f);  // twice: the whole of it can be below what fp32 holds
+        const int by = (int)(up_new - up);  // (2^by itself can be below what fp32 holds)
         up = up_new;
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
-            l[mt] = l[mt] * f * f;
+            l[mt] = __builtin_amdgcn_ldexpf(l[mt], by);
 #pragma unroll
-            for (int j = 0; j < ND; ++j) o[mt][j] = o[mt][j] * f * f;
+            for (int j = 0; j < ND; ++j)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) o[mt][j][r] = __builtin_amdgcn_ldexpf(o[mt][j][r], by);
         }
     }
     // Products x (times key scales) of 32 keys, -inf where the row does not see the key, become weights.
@@ -784,7 +786,8 @@ __global__ __launch_bounds__(kThreads, KV == ELEM_F32 ? (D == 64 ? 2 : 1) : (D =
 // 8 streams with trees of 33 to 64, 32 heads of 128 on 8 key heads, 8192 to 16384 int8 keys: 172 us and 9.3 of the join.
 // The vector unit is what is busy most: 72 us of the softmax (a score: scale, maximum, exponential of 4 slots, sum, value
 // scale, packing) and the conversions, 33 of the matrix unit, and little of the one falls under the other with two
-// waves to a SIMD.  Products of the next span issued ahead of the weights of one: 182.
+// waves to a SIMD.  Products of the next span issued ahead of the weights of one: 182; the row tiles dealt to the waves in
+// turn, so that none is idle where rows are fewer than 256: 184, as each then reads all fragments for half the rows.
 template <int KV, int D, int NWV>
 struct WideLds {
     uint4 k[2][NWV][D / 32][64];
