@@ -225,48 +225,60 @@ struct Cut {
 // of which there are no more than slots, so that no workgroup has much more to do than another, however
 // ragged the streams (7 of 8192 to 16384 keys and one just begun: 203 us with as many pieces each, 172 so).  Every
 // wave finds that size for itself, lane s holding stream s.  More streams: as many slots each.
-__device__ __forceinline__ int even_chunk(const TreeArgs &a, const TreePlan &plan, int &mine) {
+__device__ __forceinline__ int sum64(int v) {
+    v += xshfl<32>(v);
+    v += xshfl<16>(v);
+    v += xshfl<8>(v);
+    v += xshfl<4>(v);
+    v += xshfl<2>(v);
+    v += xshfl<1>(v);
+    return v;
+}
+__device__ __forceinline__ int max64(int v) {
+    v = max(v, xshfl<32>(v));
+    v = max(v, xshfl<16>(v));
+    v = max(v, xshfl<8>(v));
+    v = max(v, xshfl<4>(v));
+    v = max(v, xshfl<2>(v));
+    return max(v, xshfl<1>(v));
+}
+// The sum over the lanes below: shifts within rows of 16, then row ends handed on.
+__device__ __forceinline__ int sum_below(int v) {
+    int sum = v;
+    sum += __builtin_amdgcn_update_dpp(0, sum, 0x111, 0xF, 0xF, false);  // row_shr:1
+    sum += __builtin_amdgcn_update_dpp(0, sum, 0x112, 0xF, 0xF, false);
+    sum += __builtin_amdgcn_update_dpp(0, sum, 0x114, 0xF, 0xF, false);
+    sum += __builtin_amdgcn_update_dpp(0, sum, 0x118, 0xF, 0xF, false);
+    sum += __builtin_amdgcn_update_dpp(0, sum, 0x142, 0xA, 0xF, false);  // row_bcast:15 into rows 1 and 3
+    sum += __builtin_amdgcn_update_dpp(0, sum, 0x143, 0xC, 0xF, false);  // row_bcast:31 into rows 2 and 3
+    return sum - v;
+}
+// The size of a piece and how many of it the lane's stream has, in blocks of 128 keys.
+__device__ __forceinline__ int even_chunk(const TreeArgs &a, const TreePlan &plan, int &pieces) {
     const int lane = threadIdx.x & 63;
-    mine = 0;
+    int mine = 0;
     if (lane < a.c.streams) {
         const Stream st = stream_at(a, a.row_start[lane], a.row_start[lane + 1], a.ctx_len[lane]);
-        mine = st.n == 0 ? 0 : max(st.total, 1);  // (rows that are to be NaN need a piece too)
+        mine = st.n == 0 ? 0 : (max(st.total, 1) + 127) / 128;  // (rows that are to be NaN need a piece too)
     }
-    int most = mine;
-    most = max(most, xshfl<1>(most)), most = max(most, xshfl<2>(most)), most = max(most, xshfl<4>(most));
-    most = max(most, xshfl<8>(most)), most = max(most, xshfl<16>(most)), most = max(most, xshfl<32>(most));
-    long long sum = mine;
-    for (int m = 1; m < 64; m *= 2) sum += __shfl_xor(sum, m);
-    const long long even = (sum + plan.slots - 1) / plan.slots;
-    int chunk = max(max((int)min(even, 1ll << 30), (most + kMaxSplits - 1) / kMaxSplits), 256);
-    chunk = __builtin_amdgcn_readfirstlane((chunk + 127) / 128 * 128);
-    const int step = (chunk / 16 + 127) / 128 * 128;
+    const int most = max64(mine), even = (sum64(mine) + plan.slots - 1) / plan.slots;
+    int chunk = __builtin_amdgcn_readfirstlane(max(max(even, (most + kMaxSplits - 1) / kMaxSplits), 2));
+    const int step = (chunk + 15) / 16;
     while (true) {  // (ends at the longest stream's keys at the latest: then there are no more pieces than streams)
-        int pieces = ((uint32_t)mine + chunk - 1) / (uint32_t)chunk;
-        for (int m = 1; m < 64; m *= 2) pieces += __shfl_xor(pieces, m);
-        if (__builtin_amdgcn_readfirstlane(pieces) <= plan.slots) return chunk;
+        pieces = (mine + chunk - 1) / chunk;
+        if (__builtin_amdgcn_readfirstlane(sum64(pieces)) <= plan.slots) return chunk * 128;
         chunk += step;
     }
 }
 __device__ __forceinline__ bool even_cuts(const TreeArgs &a, const TreePlan &plan) { return a.c.streams > 1 && a.c.streams <= 64; }
-// Slots before lane's stream, when its pieces are so many.
-__device__ __forceinline__ int slots_before(int pieces) {
-    int sum = pieces;
-    for (int m = 1; m < 64; m *= 2) {
-        const int below = __shfl_up(sum, m);
-        if ((int)(threadIdx.x & 63) >= m) sum += below;
-    }
-    return sum - pieces;
-}
 __device__ __forceinline__ Cut cut_of_slot(const TreeArgs &a, const TreePlan &plan, int slot) {
     if (plan.slots == a.c.streams) return Cut{slot, 0, 0x7fffffff, slot, 1};
     if (!even_cuts(a, plan)) {
         const int per = plan.slots / a.c.streams, s = slot / per, z = slot - s * per;
         return Cut{s, z * plan.chunk, (z + 1) * plan.chunk, s * per, per};
     }
-    int mine;
-    const int chunk = even_chunk(a, plan, mine);
-    const int pieces = ((uint32_t)mine + chunk - 1) / (uint32_t)chunk, before = slots_before(pieces);
+    int pieces;
+    const int chunk = even_chunk(a, plan, pieces), before = sum_below(pieces);
     const uint64_t who = __ballot(slot >= before && slot < before + pieces);
     if (who == 0) return Cut{-1, 0, 0, 0, 0};
     const int s = __builtin_ctzll(who), first = __builtin_amdgcn_readlane(before, s), z = slot - first;

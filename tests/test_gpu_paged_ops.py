@@ -428,7 +428,8 @@ def test_attn_long_context(torch_gpu, cache, dim, n):
     _check_attn(torch, c, q, start, ctx, masks, max_rows=64, max_keys=20011 + 64)
 
 
-@pytest.mark.parametrize("streams,heads,kvh,dim", [(70, 2, 1, 64), (66, 16, 1, 128), (5, 2, 2, 64), (9, 8, 1, 128)])
+@pytest.mark.parametrize("streams,heads,kvh,dim", [(70, 2, 1, 64), (66, 16, 1, 128), (5, 2, 2, 64), (9, 8, 1, 128), (64, 2, 1, 64), (33, 3, 1, 128),
+                                                     (17, 2, 2, 64)])
 def test_attn_cuts_of_ragged_streams(torch_gpu, streams, heads, kvh, dim):
     """Keys cut into pieces over up to 64 streams by their lengths, and over more as many each: streams without rows, without
     a context and with a bad one among long and short ones."""
