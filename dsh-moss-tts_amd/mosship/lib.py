@@ -262,40 +262,52 @@ def attn_paged(q, k_pool, v_pool, heads: int, page_table, table_stride: int, pag
 ROPE_SCALING = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3}
 
 
+# These calls are a few microseconds long, so their Python is kept short: torch is looked up once, devices are
+# compared as numbers, and a stream is asked for as its handle.
+_torch = None
+
+
+def _t():
+    global _torch
+    if _torch is None:
+        import torch
+        _torch = torch
+    return _torch
+
+
 def _types(t):
     """Element type of a tensor of rows."""
-    import torch
-    d = t.dtype
-    if d == torch.float32:
+    torch, d = _t(), t.dtype
+    if d is torch.float32:
         return F32
-    if d == torch.float16:
+    if d is torch.float16:
         return F16
     raise TypeError(f"float32 or float16 rows are wanted, not {d}")
 
 
 def _whole(name, t, dtype, shape, device, optional=False):
-    """The address of a contiguous tensor of this type and shape on this device (None: NULL)."""
+    """The address of a contiguous tensor of this type and shape on this device's number (None: NULL)."""
     if t is None and optional:
         return None
-    if t.dtype != dtype or t.shape != shape or t.device != device or not t.is_contiguous():
-        raise ValueError(f"{name}: a contiguous {dtype} tensor of shape {tuple(shape)} on {device} is wanted, "
-                         f"not {t.dtype} {tuple(t.shape)} on {t.device}")
-    return t.data_ptr()
+    if t.dtype is dtype and t.shape == shape and t.get_device() == device and t.is_contiguous():
+        return t.data_ptr()
+    raise ValueError(f"{name}: a contiguous {dtype} tensor of shape {tuple(shape)} on device {device} is wanted, "
+                     f"not {t.dtype} {tuple(t.shape)} on {t.device}")
 
 
 def _on(device, stream):
     """The stream to launch on: the caller's handle, or torch's current one.  The calls launch on the current device:
-    tensors of another one are refused.  (torch.cuda.current_stream() builds an object for 2.9 us, the call of its
-    handle takes 0.1: of a small operator's 10 us in all.)"""
-    import torch
-    if device.type != "cuda":
-        raise ValueError(f"tensors on the GPU are wanted, not on {device}")
-    if device.index != torch.cuda.current_device():
-        raise ValueError(f"the tensors are on {device}, the current device is cuda:{torch.cuda.current_device()}")
+    tensors of another one are refused."""
+    torch = _t()
+    if device < 0:
+        raise ValueError("tensors on the GPU are wanted")
+    if device != torch.cuda.current_device():
+        raise ValueError(f"the tensors are on cuda:{device}, the current device is cuda:{torch.cuda.current_device()}")
     if stream is not None:
         return stream
+    # (torch.cuda.current_stream() makes an object first: 2.9 us, where the handle takes 0.1)
     raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-    return raw(device.index) if raw is not None else torch.cuda.current_stream().cuda_stream
+    return raw(device) if raw is not None else torch.cuda.current_stream().cuda_stream
 
 
 def _rows(name, t, heads, dim, device):
@@ -305,8 +317,8 @@ def _rows(name, t, heads, dim, device):
         fits, whole = shape[1] == heads and shape[2] == dim, st[2] == 1 and (st[1] == dim or heads == 1)
     else:
         fits, whole = len(shape) == 2 and shape[1] == heads * dim, st[-1] == 1
-    if not fits or t.device != device:
-        raise ValueError(f"{name}: [rows][{heads}][{dim}] on {device} is wanted, not {tuple(shape)} on {t.device}")
+    if not fits or t.get_device() != device:
+        raise ValueError(f"{name}: [rows][{heads}][{dim}] on device {device} is wanted, not {tuple(shape)} on {t.device}")
     if not whole:
         raise ValueError(f"{name}: the heads of a row must be contiguous")
     return t.data_ptr(), st[0]
@@ -315,16 +327,16 @@ def _rows(name, t, heads, dim, device):
 def _workspace(given, size_of, device, stream):
     """(address, bytes): the caller's (the call checks that it is large enough), or a new one from torch's allocator,
     which is safe on torch's current stream."""
-    import torch
+    torch = _t()
     if given is None:
         size = size_of()
         if size == 0:
             return None, 0
         if stream is not None and stream != torch.cuda.current_stream().cuda_stream:
             raise ValueError("on a stream other than torch's current one, pass a workspace")
-        given = torch.empty(size, dtype=torch.uint8, device=device)
-    elif given.device != device or not given.is_contiguous():
-        raise ValueError(f"workspace: a contiguous tensor on {device} is wanted")
+        given = torch.empty(size, dtype=torch.uint8, device=torch.device("cuda", device))
+    elif given.get_device() != device or not given.is_contiguous():
+        raise ValueError(f"workspace: a contiguous tensor on device {device} is wanted")
     return given.data_ptr(), given.numel() * given.element_size()
 
 
@@ -348,8 +360,8 @@ class Rope:
         if freqs is None:
             f, mscale = rope_freqs(rot_dim, **scaling)
             freqs = torch.from_numpy(f).to("cuda" if device is None else device)
-        self.freqs, self.device = freqs, freqs.device
-        _whole("freqs", freqs, torch.float64, (freqs.numel(),), freqs.device)
+        self.freqs, self.device = freqs, freqs.get_device()
+        _whole("freqs", freqs, torch.float64, (freqs.numel(),), self.device)
         self.struct = RopeStruct(freqs.data_ptr(), 2 * freqs.numel(), int(halves), mscale)
         self.ref = C.addressof(self.struct)
 
@@ -364,15 +376,15 @@ class KVCache:
         kinds = {torch.float32: F32, torch.float16: F16, torch.int8: I8, torch.float8_e4m3fn: E4M3}
         if k.dim() != 4 or k.dtype not in kinds or page_table.dim() != 2:
             raise ValueError("pools [n_pages][kv_heads][page_size][head_dim] and a table [streams][pages] are wanted")
-        self.tensors, self.device = (k, v, page_table, k_scale, v_scale), k.device
+        self.tensors, self.device = (k, v, page_table, k_scale, v_scale), k.get_device()
         n, h, size, dim = k.shape
         self.kv_heads, self.head_dim, self.streams = h, dim, page_table.shape[0]
         self.struct = KVCacheStruct(
-            _whole("k", k, k.dtype, (n, h, size, dim), k.device), _whole("v", v, k.dtype, (n, h, size, dim), k.device),
-            _whole("k_scale", k_scale, torch.float32, (n, h, size), k.device, optional=True),
-            _whole("v_scale", v_scale, torch.float32, (n, h, size), k.device, optional=True),
+            _whole("k", k, k.dtype, (n, h, size, dim), self.device), _whole("v", v, k.dtype, (n, h, size, dim), self.device),
+            _whole("k_scale", k_scale, torch.float32, (n, h, size), self.device, optional=True),
+            _whole("v_scale", v_scale, torch.float32, (n, h, size), self.device, optional=True),
             kinds[k.dtype], h, dim, size, n,
-            _whole("page_table", page_table, torch.int32, tuple(page_table.shape), k.device), page_table.shape[1],
+            _whole("page_table", page_table, torch.int32, tuple(page_table.shape), self.device), page_table.shape[1],
             page_table.shape[0])
         self.ref = C.addressof(self.struct)
 
@@ -380,11 +392,10 @@ class KVCache:
 def rope_rows(x, pos, rope: Rope, out=None, stream=None):
     """moss_hip_rope_rows on x [rows][heads][head_dim] (any row and head strides) at positions pos [rows] int32, into
     out (x itself by default); returns out."""
-    import torch
     out = x if out is None else out
-    dev, shape = x.device, x.shape
+    dev, shape = x.get_device(), x.shape
     on = _on(dev, stream)
-    if len(shape) != 3 or out.shape != shape or out.dtype != x.dtype or out.device != dev or rope.device != dev:
+    if len(shape) != 3 or out.shape != shape or out.dtype is not x.dtype or out.get_device() != dev or rope.device != dev:
         raise ValueError("x and out must be [rows][heads][head_dim] of one type, on one device with the rotation")
     rows, heads, dim = shape
     if rows * heads * dim == 0:
@@ -393,42 +404,40 @@ def rope_rows(x, pos, rope: Rope, out=None, stream=None):
     if xs[2] != 1 or os_[2] != 1:
         raise ValueError("the elements of a head must be contiguous")
     check(load().moss_hip_rope_rows(x.data_ptr(), xs[0], xs[1], out.data_ptr(), os_[0], os_[1], _types(x), rows, heads, dim,
-                                    _whole("pos", pos, torch.int32, (rows,), dev), rope.ref, on))
+                                    _whole("pos", pos, _torch.int32, (rows,), dev), rope.ref, on))
     return out
 
 
 def kv_write(cache: KVCache, k, v, row_stream, row_pos, rope: Rope | None = None, rope_pos=None, stream=None) -> None:
     """moss_hip_kv_write: rows k, v [rows][kv_heads][head_dim] to position row_pos[r] of stream row_stream[r], keys turned
     by `rope` at rope_pos (row_pos by default)."""
-    import torch
     dev, n = cache.device, k.shape[0]
     on = _on(dev, stream)
-    if v.shape[0] != n or v.dtype != k.dtype or (rope is not None and rope.device != dev):
+    if v.shape[0] != n or v.dtype is not k.dtype or (rope is not None and rope.device != dev):
         raise ValueError("k and v must have the same rows and type, and the rotation their device")
     if n == 0:
         return
     kp, ks = _rows("k", k, cache.kv_heads, cache.head_dim, dev)
     vp, vs = _rows("v", v, cache.kv_heads, cache.head_dim, dev)
     check(load().moss_hip_kv_write(cache.ref, kp, ks, vp, vs, _types(k), n,
-                                   _whole("row_stream", row_stream, torch.int32, (n,), dev),
-                                   _whole("row_pos", row_pos, torch.int32, (n,), dev),
+                                   _whole("row_stream", row_stream, _torch.int32, (n,), dev),
+                                   _whole("row_pos", row_pos, _torch.int32, (n,), dev),
                                    None if rope is None else rope.ref,
-                                   _whole("rope_pos", rope_pos, torch.int32, (n,), dev, optional=True), on))
+                                   _whole("rope_pos", rope_pos, _torch.int32, (n,), dev, optional=True), on))
 
 
 def kv_read(cache: KVCache, row_stream, row_pos, k, v, stream=None) -> None:
     """moss_hip_kv_read: those rows back, into k, v [rows][kv_heads][head_dim]."""
-    import torch
     dev, n = cache.device, k.shape[0]
     on = _on(dev, stream)
-    if v.shape[0] != n or v.dtype != k.dtype:
+    if v.shape[0] != n or v.dtype is not k.dtype:
         raise ValueError("k and v must have the same rows and type")
     if n == 0:
         return
     kp, ks = _rows("k", k, cache.kv_heads, cache.head_dim, dev)
     vp, vs = _rows("v", v, cache.kv_heads, cache.head_dim, dev)
-    check(load().moss_hip_kv_read(cache.ref, _whole("row_stream", row_stream, torch.int32, (n,), dev),
-                                  _whole("row_pos", row_pos, torch.int32, (n,), dev), n, kp, ks, vp, vs, _types(k), on))
+    check(load().moss_hip_kv_read(cache.ref, _whole("row_stream", row_stream, _torch.int32, (n,), dev),
+                                  _whole("row_pos", row_pos, _torch.int32, (n,), dev), n, kp, ks, vp, vs, _types(k), on))
 
 
 def attn_tree_workspace(cache: KVCache, heads: int, rows: int, max_rows: int, max_keys: int) -> int:
@@ -444,7 +453,6 @@ def attn_tree(q, cache: KVCache, row_start, ctx_len, out, max_rows: int, max_key
 
     row_start [streams + 1] and ctx_len [streams] int32; row_mask [rows] int64 (bit j: drafted row j of the
     stream), None: a chain; scale: head_dim ** -0.5 by default; lse [rows][heads] float32 or None."""
-    import torch
     dev, dim = cache.device, cache.head_dim
     on = _on(dev, stream)
     rows = q.shape[0]
@@ -457,11 +465,11 @@ def attn_tree(q, cache: KVCache, row_start, ctx_len, out, max_rows: int, max_key
     op, os_ = _rows("out", out, heads, dim, dev)
     wp, wb = _workspace(workspace, lambda: attn_tree_workspace(cache, heads, rows, max_rows, max_keys), dev, stream)
     check(load().moss_hip_attn_tree(qp, qs, _types(q), heads, cache.ref,
-                                    _whole("row_start", row_start, torch.int32, (cache.streams + 1,), dev),
-                                    _whole("ctx_len", ctx_len, torch.int32, (cache.streams,), dev),
-                                    _whole("row_mask", row_mask, torch.int64, (rows,), dev, optional=True), rows, max_rows,
+                                    _whole("row_start", row_start, _torch.int32, (cache.streams + 1,), dev),
+                                    _whole("ctx_len", ctx_len, _torch.int32, (cache.streams,), dev),
+                                    _whole("row_mask", row_mask, _torch.int64, (rows,), dev, optional=True), rows, max_rows,
                                     max_keys, dim ** -0.5 if scale is None else scale, op, os_, _types(out),
-                                    _whole("lse", lse, torch.float32, (rows, heads), dev, optional=True), wp, wb, on))
+                                    _whole("lse", lse, _torch.float32, (rows, heads), dev, optional=True), wp, wb, on))
 
 
 def token_logprobs_workspace(rows: int, vocab: int, top_k: int) -> int:
@@ -475,8 +483,7 @@ def token_logprobs(logits, tokens, logprob, entropy=None, top_ids=None, top_logp
                    workspace=None, stream=None) -> None:
     """moss_hip_token_logprobs: of tokens [rows] int32 under logits [rows][vocab] (float32 or float16, any row stride), into
     logprob and entropy [rows] and the alternatives top_ids (int32), top_logprobs [rows][top_k]."""
-    import torch
-    dev, shape = logits.device, logits.shape
+    dev, shape = logits.get_device(), logits.shape
     on = _on(dev, stream)
     if len(shape) != 2:
         raise ValueError("logits [rows][vocab] are wanted")
@@ -490,11 +497,11 @@ def token_logprobs(logits, tokens, logprob, entropy=None, top_ids=None, top_logp
         raise ValueError("the logits of a row must be contiguous")
     wp, wb = _workspace(workspace, lambda: token_logprobs_workspace(rows, vocab, k), dev, stream)
     check(load().moss_hip_token_logprobs(logits.data_ptr(), logits.stride(0), _types(logits), rows, vocab,
-                                         _whole("tokens", tokens, torch.int32, (rows,), dev), inv_temperature,
-                                         _whole("logprob", logprob, torch.float32, (rows,), dev),
-                                         _whole("entropy", entropy, torch.float32, (rows,), dev, optional=True), k,
-                                         _whole("top_ids", top_ids, torch.int32, (rows, k), dev, optional=True),
-                                         _whole("top_logprobs", top_logprobs, torch.float32, (rows, k), dev, optional=True),
+                                         _whole("tokens", tokens, _torch.int32, (rows,), dev), inv_temperature,
+                                         _whole("logprob", logprob, _torch.float32, (rows,), dev),
+                                         _whole("entropy", entropy, _torch.float32, (rows,), dev, optional=True), k,
+                                         _whole("top_ids", top_ids, _torch.int32, (rows, k), dev, optional=True),
+                                         _whole("top_logprobs", top_logprobs, _torch.float32, (rows, k), dev, optional=True),
                                          wp, wb, on))
 
 
