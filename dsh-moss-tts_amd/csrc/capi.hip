@@ -4,6 +4,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstdio>
+#include <initializer_list>
 #include <map>
 #include <mutex>
 #include <string>
@@ -627,6 +628,12 @@ mh::KvCacheArgs cache_args(const moss_hip_kv_cache *c) {
     return a;
 }
 
+// Strides of which no multiple by a row or a head leaves 64 bits.
+void check_strides(std::initializer_list<int64_t> strides) {
+    for (const int64_t n : strides)
+        if (n < 0 || n > (1ll << 40)) throw Status(MOSS_HIP_EINVAL, "strides must not be negative, nor past 2^40");
+}
+
 void check_rows(int rows) {
     if (rows < 0 || rows > kMaxRows) throw Status(MOSS_HIP_EINVAL, "need 0 <= rows <= 4194304");
 }
@@ -701,8 +708,7 @@ int moss_hip_rope_rows(const void *x, int64_t x_row_stride, int64_t x_head_strid
         check_rows(rows);
         if (heads <= 0 || heads > kMaxHeads || head_dim <= 0 || head_dim > 1024 || head_dim % 2)
             throw Status(MOSS_HIP_EINVAL, "need 0 < heads, head_dim <= 1024, and an even head_dim");
-        if (x_row_stride < 0 || x_head_stride < 0 || y_row_stride < 0 || y_head_stride < 0)
-            throw Status(MOSS_HIP_EINVAL, "strides must not be negative");
+        check_strides({x_row_stride, x_head_stride, y_row_stride, y_head_stride});
         if (x == y && (x_row_stride != y_row_stride || x_head_stride != y_head_stride))
             throw Status(MOSS_HIP_EINVAL, "in place, x and y must have the same strides");
         // one of the two dimensions lies within the other's steps
@@ -737,7 +743,7 @@ int moss_hip_kv_write(const moss_hip_kv_cache *cache, const void *k, int64_t k_s
         if (!k || !v || !row_stream || !row_pos) throw Status(MOSS_HIP_EINVAL, "null pointer");
         check_row_type(dtype);
         check_rows(rows);
-        if (k_stride < 0 || v_stride < 0) throw Status(MOSS_HIP_EINVAL, "strides must not be negative");
+        check_strides({k_stride, v_stride});
         if (rope != nullptr)
             a.rope = rope_args(rope, a.c.dim);
         else if (rope_pos != nullptr)
@@ -765,6 +771,7 @@ int moss_hip_kv_read(const moss_hip_kv_cache *cache, const int32_t *row_stream, 
         check_row_type(dtype);
         check_rows(rows);
         const int64_t width = (int64_t)a.c.heads * a.c.dim;
+        check_strides({k_stride, v_stride});
         if (rows > 1 && (k_stride < width || v_stride < width)) throw Status(MOSS_HIP_EINVAL, "rows of k and v must not overlap");
         if (rows == 0) return;
         a.k_out = k;
@@ -799,7 +806,7 @@ int moss_hip_attn_tree(const void *q, int64_t q_stride, int q_dtype, int heads, 
         check_row_type(q_dtype);
         check_row_type(out_dtype);
         const int64_t width = (int64_t)heads * a.c.dim;
-        if (q_stride < 0) throw Status(MOSS_HIP_EINVAL, "strides must not be negative");
+        check_strides({q_stride, out_stride});
         if (rows > 1 && out_stride < width) throw Status(MOSS_HIP_EINVAL, "rows of out must not overlap");
         if (!std::isfinite(scale)) throw Status(MOSS_HIP_EINVAL, "scale must be finite");
         if (rows == 0 || a.c.streams == 0) return;
@@ -839,7 +846,7 @@ int moss_hip_token_logprobs(const void *logits, int64_t row_stride, int dtype, i
         logprobs_shape(rows, vocab, top_k);
         if (!logits || !tokens || !logprob || (top_k > 0 && (!top_ids || !top_logprobs))) throw Status(MOSS_HIP_EINVAL, "null pointer");
         check_row_type(dtype);
-        if (row_stride < 0) throw Status(MOSS_HIP_EINVAL, "strides must not be negative");
+        check_strides({row_stride});
         if (!(inv_temperature > 0.0f) || !std::isfinite(inv_temperature)) throw Status(MOSS_HIP_EINVAL, "inv_temperature must be positive and finite");
         if (rows == 0) return;
         check_workspace(workspace, workspace_bytes, mh::logprobs_workspace(rows, vocab, top_k), "moss_hip_token_logprobs");

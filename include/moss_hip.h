@@ -356,7 +356,7 @@ int moss_hip_attn_decode_noalloc(const float *q, const void *k_cache, const void
  * pointer of the device that is current at the call, and `stream` is a stream of that device.
  * Arrays read while a call's kernels run must not be changed meanwhile by work on other streams.  A
  * workspace belongs to one call at a time: calls (and replays of captured calls) that may overlap
- * need workspaces of their own.  Where rows, streams or top_k are 0 there is nothing to do and the
+ * need workspaces of their own.  Strides are 0 .. 2^40 elements.  Where rows, streams or top_k are 0 there is nothing to do and the
  * call returns OK.  What only the device can see (positions, page indices, row ranges) is checked
  * there and never followed out of range; each call says what becomes of such rows. */
 

@@ -135,6 +135,22 @@ def test_token_logprobs_refusals():
     assert L.moss_hip_token_logprobs_workspace(4, 1024, 5, C.byref(n)) == lib.OK and n.value == 0
 
 
+def test_strides_whose_multiples_leave_64_bits():
+    """11 head strides of 2^62 are negative in 64 bits, which once passed for rows that lie apart."""
+    L, c = lib.load(), _cache(streams=1)
+    far, r = 1 << 62, C.addressof(c)
+    for i in (1, 2, 4, 5):
+        a = [P, 1024, 64, P + 0x10000, 1024, 64, lib.F32, 4, 12, 64, P]
+        a[i] = far
+        _refused(L.moss_hip_rope_rows(*a, C.addressof(_rope()), None), "2^40")
+    for k, v in ((far, 256), (256, far)):
+        _refused(L.moss_hip_kv_write(r, P, k, P, v, lib.F32, 4, P, P, None, None, None), "2^40")
+        _refused(L.moss_hip_kv_read(r, P, P, 4, P, k, P, v, lib.F32, None), "2^40")
+    for q, o in ((far, 1024), (1024, far)):
+        _refused(L.moss_hip_attn_tree(P, q, lib.F32, 16, r, P, P, None, 4, 4, 256, 0.125, P, o, lib.F32, None, P, 1 << 30, None), "2^40")
+    _refused(L.moss_hip_token_logprobs(P, far, lib.F32, 4, 1024, P, 1.0, P, P, 5, P, P, P, 1 << 30, None), "2^40")
+
+
 def test_nothing_to_do_is_ok():
     """No rows, no streams: OK before any device call."""
     L, c = lib.load(), _cache(streams=0)
