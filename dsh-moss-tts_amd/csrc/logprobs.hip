@@ -1,8 +1,9 @@
 // logprobs.hip -- log probabilities of given tokens, the entropy and the top alternatives of rows of
 // logits (gfx950).
 //
-// Of a row z = x / T: with m = max z, S = sum e^(z - m) and U = sum e^(z - m) (z - m),
-//   log p(t) = z_t - m - log S,     entropy = -sum p log p = log S - U / S,
+// Of a row: with m = max x, z = (x - m) / T, S = sum e^z and U = sum e^z z,
+//   log p(t) = z_t - log S,     entropy = -sum p log p = log S - U / S,
+// the differences first, so that a row of the type's lowest value does not leave its range when it is scaled;
 // and the k largest x, of equal values the lowest index first.  One pass: a workgroup takes a
 // chunk of a row into registers, so memory is read once; m, S, U and the alternatives all come
 // from there.  A row of more than one chunk leaves (m, S, U) and its k best per chunk in the
@@ -176,7 +177,7 @@ __device__ __forceinline__ Sums sums_of(const float (&x)[EPT], float inv_t, int 
     float best = -INFINITY;
 #pragma unroll
     for (int i = 0; i < EPT; ++i) best = fmaxf(best, x[i]);
-    float m = wave_max(best) * inv_t;  // (rounding keeps the order)
+    float m = wave_max(best);
     if (lane == 0) red[0][w] = m;
     __syncthreads();
 #pragma unroll
@@ -185,7 +186,7 @@ __device__ __forceinline__ Sums sums_of(const float (&x)[EPT], float inv_t, int 
     float s = 0.0f, u = 0.0f;
 #pragma unroll
     for (int i = 0; i < EPT; ++i) {
-        const float z = x[i] * inv_t - m0;
+        const float z = (x[i] - m0) * inv_t;
         const float e = __builtin_amdgcn_exp2f(z * 1.44269504088896341f);
         s += e;
         u += e == 0.0f ? 0.0f : e * z;
@@ -224,12 +225,12 @@ __device__ __forceinline__ float token_logit(const LogprobArgs &a, int r) {
 // What a row's sums give: the token's log probability and the entropy (one thread), and the log
 // probability of an alternative.
 __device__ __forceinline__ void finish_row(const LogprobArgs &a, int r, float x, const Sums &q) {
-    const float log_s = logf(q.s), z = x * a.inv_t;
-    a.logprob[r] = q.s == 0.0f && z == z ? -INFINITY : z - q.m - log_s;  // (sum 0: no token is allowed at all)
+    const float log_s = logf(q.s);
+    a.logprob[r] = q.s == 0.0f && x == x ? -INFINITY : (x - q.m) * a.inv_t - log_s;  // (sum 0: no token is allowed at all)
     if (a.entropy != nullptr) a.entropy[r] = q.s == 0.0f ? 0.0f : log_s - q.u / q.s;
 }
 __device__ __forceinline__ float alt_lp(const LogprobArgs &a, const Sums &q, uint32_t key) {
-    return of_key(key) * a.inv_t - q.m - logf(q.s);
+    return (of_key(key) - q.m) * a.inv_t - logf(q.s);
 }
 __device__ __forceinline__ void no_alternatives(const LogprobArgs &a, int r, int from) {
     for (int i = from + (int)threadIdx.x; i < a.top_k; i += kThreads) {
@@ -312,7 +313,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_join_kernel(LogprobArgs a, 
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         if (part[i].x == -INFINITY && part[i].y == 0.0f) continue;  // nothing allowed in this chunk
-        const float d = part[i].x - q.m, f = __builtin_amdgcn_exp2f(d * 1.44269504088896341f);
+        const float d = (part[i].x - q.m) * a.inv_t, f = __builtin_amdgcn_exp2f(d * 1.44269504088896341f);
         q.s += f * part[i].y;
         q.u += f == 0.0f ? 0.0f : f * (part[i].z + part[i].y * d);
     }

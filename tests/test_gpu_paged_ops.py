@@ -709,6 +709,32 @@ def test_token_logprobs_ties_and_ruled_out(torch_gpu, vocab):
     _check_lp(torch, torch.from_numpy(x).cuda(), tokens, 32)
 
 
+@pytest.mark.parametrize("vocab", [700, 5000, 70001])
+@pytest.mark.parametrize("inv_t", [1.5, 1e-38, 3e38])
+def test_token_logprobs_scaled_past_the_range(torch_gpu, vocab, inv_t):
+    """The type's lowest value everywhere, in all places but one and in all but two, under temperatures that scale it past
+    the type's range, or everything to nothing.  The exact results are log vocab, log 2 and 0: the sum of vocab equal
+    terms is off by vocab / 256 + 16 units at most, the logarithm by 4."""
+    torch = torch_gpu
+    low = float(np.finfo(np.float32).min)
+    x = np.full((4, vocab), low, np.float32)
+    x[1, 17] = x[2, [17, vocab - 1]] = 2.0
+    x[3] = 0.0
+    lp, ent, ids, top = _run_lp(torch, torch.from_numpy(x).cuda(), [vocab - 1, 17, 17, 5], 3, inv_t)
+    assert np.array_equal(ids, [[0, 1, 2], [17, 0, 1], [17, vocab - 1, 0], [0, 1, 2]])
+    even = math.log(vocab)
+    tol = U32 * (vocab / 256 + 16 + 4 * even)
+    for r in (0, 3):
+        assert abs(lp[r] + even) <= tol and abs(ent[r] - even) <= tol and (np.abs(top[r] + even) <= tol).all()
+    if inv_t < 1:  # differences of 3.4 * (1 +- 2^-24), each rounded twice, in 64 bits
+        z = np.where(np.arange(vocab) == 17, 0.0, low * np.float64(np.float32(inv_t)))
+        p = np.exp(z - np.log(np.exp(z).sum()))
+        assert abs(lp[1] - math.log(p[17])) <= tol + 16 * U32 and abs(ent[1] + (p * np.log(p)).sum()) <= 16 * (tol + 16 * U32)
+    else:
+        assert lp[1] == 0 and ent[1] == 0 and top[1, 0] == 0 and (top[1, 1:] == -np.inf).all()
+        assert abs(lp[2] + math.log(2)) <= 8 * U32 and abs(ent[2] - math.log(2)) <= 8 * U32 and top[2, 2] == -np.inf
+
+
 @pytest.mark.parametrize("vocab", [1000, 40000])
 def test_token_logprobs_nan_and_inf(torch_gpu, vocab):
     """A NaN or +inf makes the row's probabilities NaN; NaN is no alternative; rows beside it are as ever."""
