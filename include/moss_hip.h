@@ -433,7 +433,8 @@ int moss_hip_kv_read(const moss_hip_kv_cache *cache, const int32_t *row_stream, 
  * row_mask[row] (its ancestors and itself), or j <= i where row_mask is NULL (a chain; one row: a plain
  * decode step).  Scores are scale * q . k; query head i reads key head i / (heads / kv_heads).
  *   q: [rows][heads][head_dim] of q_dtype (F32 or F16), rotated; out the same shape in out_dtype; row
- *   strides in elements.  lse [rows][heads] fp32 or NULL: the log of each row's sum of exp(score).
+ *   strides in elements, out q itself (same type and stride) or apart from it.  lse [rows][heads] fp32 or
+ *   NULL: the log of each row's sum of exp(score).  The streams' row ranges lie apart.
  * A row that attends nothing is 0 with lse -inf.  What a row does not attend may hold anything, Inf and NaN
  * too.  max_keys bounds every stream's ctx_len + n and sizes the launch.  A stream whose ctx_len is
  * negative, whose keys pass max_keys or its table, or with a page outside [0, n_pages) among them, gets
@@ -447,7 +448,8 @@ int moss_hip_attn_tree(const void *q, int64_t q_stride, int q_dtype, int heads, 
                        int max_keys, float scale, void *out, int64_t out_stride, int out_dtype, float *lse, void *workspace,
                        size_t workspace_bytes, void *stream);
 /* Bytes of workspace such a call takes (of the cache it reads kv_dtype, kv_heads, head_dim, page_size and
- * streams). */
+ * streams).  Fewer rows can take more, as their keys are cut finer: a workspace for calls of several shapes
+ * is the largest of theirs. */
 int moss_hip_attn_tree_workspace(const moss_hip_kv_cache *cache, int heads, int rows, int max_rows, int max_keys, size_t *bytes);
 
 /* For rows of logits x [rows][vocab] (dtype F32 or F16, row stride in elements) and z = x * inv_temperature:

@@ -571,6 +571,29 @@ def test_attn_large_queries_and_scores(torch_gpu):
     _check_attn(torch, c, q, start, ctx, None, scale=-0.3)
 
 
+@pytest.mark.parametrize("cache", ["f16", "i8", "e4m3", "f32"])
+@pytest.mark.parametrize("n", [1, 5, 40])
+def test_attn_inf_and_nan_queries(torch_gpu, cache, n):
+    """A head of a row with a NaN or an Inf in its query is NaN; not a bit of any other changes, those packed with it
+    among them.  In place, the output over the query, gives the same."""
+    torch = torch_gpu
+    print(f"attn queries {cache} {n}", flush=True)
+    ctx = [700, 45]
+    c, start, rows, masks, q = _attn_case(torch, cache, 64, 8, 2, 32, ctx, [n, n], False, 40 + n)
+    a, la = _run_attn(torch, c, q, start, ctx, masks, n, 700 + n)
+    odd = q.clone()
+    odd[0, 1, 5], odd[rows - 1, 4, 63], odd[rows - 1, 7, 0] = math.nan, math.inf, -math.inf
+    b, lb = _run_attn(torch, c, odd, start, ctx, masks, n, 700 + n)
+    bad = np.zeros((rows, 8), bool)
+    bad[0, 1] = bad[rows - 1, 4] = bad[rows - 1, 7] = True
+    assert np.isnan(b[bad]).all() and np.isnan(lb[bad]).all()
+    assert np.array_equal(a[~bad], b[~bad]) and np.array_equal(la[~bad], lb[~bad])
+    x = q.cuda()
+    lib.attn_tree(x, c, torch.from_numpy(start).cuda(), torch.tensor(ctx, dtype=torch.int32, device="cuda"), x, n, 700 + n,
+                  row_mask=_dev_masks(torch, masks))
+    assert np.array_equal(x.double().cpu().numpy(), a)
+
+
 def test_attn_strided_rows(torch_gpu):
     """Queries inside wider rows and at odd addresses, outputs inside wider rows; nothing beside them is written."""
     torch = torch_gpu
