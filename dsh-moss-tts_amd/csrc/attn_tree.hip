@@ -223,7 +223,7 @@ struct Cut {
 };
 // Up to 64 streams share the slots out by their lengths: pieces of the fewest keys (a multiple of 128, at least 256)
 // of which there are no more than slots, so that no workgroup has much more to do than another, however
-// ragged the streams (7 of 8192 to 16384 keys and one just begun: 203 us with as many pieces each, 172 so).  Every
+// ragged the streams (7 of 8192 to 16384 keys and one just begun: 203 us with as many pieces each, 172 so, both before later steps).  Every
 // wave finds that size for itself, lane s holding stream s.  More streams: as many slots each.
 __device__ __forceinline__ int sum64(int v) {
     v += xshfl<32>(v);
@@ -567,8 +567,8 @@ __device__ __forceinline__ void put_row(const TreeArgs &a, const TreePlan &plan,
 // Few rows (up to 4 tiles, 2 of a workgroup): memory bound.  Each of the 4 waves takes every 4th span of 32 keys, the next
 // span's loads in flight while one is worked on, and the waves are joined through LDS.
 // LO: 32-bit queries, as hi + lo.
-// One row over 130001 e4m3 keys of 8 x 128, 32 heads: 51.6 us and 4.8 of the join, 5.3 TB/s.  64 streams of 270 to 541
-// int8 keys of 12 x 64: 15.5 us; 16 trees of 14 to 27 over 507 to 1015 fp16 keys of 12 x 64: 17.0 and 4.1.  The last two are
+// One row over 130001 e4m3 keys of 8 x 128, 32 heads: 51.8 us and 4.9 of the join, 5.3 TB/s.  64 streams of 270 to 541
+// int8 keys of 12 x 64: 15.7 us; 16 trees of 14 to 27 over 507 to 1015 fp16 keys of 12 x 64: 16.5 and 4.1.  The last two are
 // short of it by their chain of dependent loads (row range, page, keys, then 4 or 5 spans a wave) and by vector work, about
 // 300 instructions a span.
 template <int KV, int D, int MT, bool LO>
@@ -795,11 +795,11 @@ __global__ __launch_bounds__(kThreads, KV == ELEM_F32 ? (D == 64 ? 2 : 1) : (D =
 // PLO: weights as hi + lo; where the output is fp16 they are rounded to fp16 once, to nearest: an error of the
 // size of the output's own rounding (2.9e-4 in all where rounding the output alone gives 2.1e-4), for a third of the
 // products less: 211 and 255 us when that was measured.
-// 8 streams with trees of 33 to 64, 32 heads of 128 on 8 key heads, 8192 to 16384 int8 keys: 172 us and 9.3 of the join.
+// 8 streams with trees of 33 to 64, 32 heads of 128 on 8 key heads, 8192 to 16384 int8 keys: 162 us and 9.2 of the join.
 // The vector unit is what is busy most: 72 us of the softmax (a score: scale, maximum, exponential of 4 slots, sum, value
 // scale, packing) and the conversions, 33 of the matrix unit, and little of the one falls under the other with two
-// waves to a SIMD.  Products of the next span issued ahead of the weights of one: 182; the row tiles dealt to the waves in
-// turn, so that none is idle where rows are fewer than 256: 184, as each then reads all fragments for half the rows.
+// waves to a SIMD.  Tried when it took 172: products of the next span issued ahead of the weights of one, 182; the row tiles dealt to
+// the waves in turn, so that none is idle where rows are fewer than 256, 184, as each then reads all fragments for half the rows.
 template <int KV, int D, int NWV>
 struct WideLds {
     uint4 k[2][NWV][D / 32][64];
