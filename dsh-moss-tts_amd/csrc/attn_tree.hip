@@ -795,11 +795,13 @@ __global__ __launch_bounds__(kThreads, KV == ELEM_F32 ? (D == 64 ? 2 : 1) : (D =
 // PLO: weights as hi + lo; where the output is fp16 they are rounded to fp16 once, to nearest: an error of the
 // size of the output's own rounding (2.9e-4 in all where rounding the output alone gives 2.1e-4), for a third of the
 // products less: 211 and 255 us when that was measured.
-// 8 streams with trees of 33 to 64, 32 heads of 128 on 8 key heads, 8192 to 16384 int8 keys: 162 us and 9.2 of the join.
+// 8 streams with trees of 33 to 64, 32 heads of 128 on 8 key heads, 8192 to 16384 int8 keys: 162 to 175 us from run to
+// run, and 9.3 of the join.
 // The vector unit is what is busy most: 72 us of the softmax (a score: scale, maximum, exponential of 4 slots, sum, value
 // scale, packing) and the conversions, 33 of the matrix unit, and little of the one falls under the other with two
-// waves to a SIMD.  Tried when it took 172: products of the next span issued ahead of the weights of one, 182; the row tiles dealt to
-// the waves in turn, so that none is idle where rows are fewer than 256, 184, as each then reads all fragments for half the rows.
+// waves to a SIMD.  Tried when it took 172: products of the next span issued ahead of the weights of one, 182; the row
+// tiles dealt to the waves in turn, so that none is idle where rows are fewer than 256, 184, as each then reads all
+// fragments for half the rows.
 template <int KV, int D, int NWV>
 struct WideLds {
     uint4 k[2][NWV][D / 32][64];
