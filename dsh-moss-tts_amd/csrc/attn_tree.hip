@@ -7,8 +7,8 @@
 // A row that sees nothing is 0 with lse = -inf.
 //
 // The n rows x (heads / kv_heads) queries that share a key head are packed into tiles of 16, the
-// columns of the matrix instructions, so a key is loaded once for all of them.  A workgroup's 4 waves
-// take every 4th span of keys with a running maximum and sum each, and are joined through LDS; with
+// columns of the matrix instructions, so a key is loaded once for all of them.  A workgroup's 4 or 8
+// waves take every 4th or 8th span of keys with a running maximum and sum each, and are joined through LDS; with
 // few workgroups the keys are also cut over workgroups, whose partial results a second launch
 // joins in their order (no atomics: the same call gives the same bits).
 //
@@ -43,6 +43,7 @@ constexpr int kWeightExp = 6;   // and of what it is scaled by
 
 struct TreePlan {
     int tiles, group, row_groups;  // row tiles of 16, of which a workgroup takes `group`
+    int waves;                     // of a workgroup of the kernel for few rows
     int slots;                     // pieces that all streams' keys are cut into; streams: no cuts, and no workspace
     int chunk;                     // keys of a piece where every stream has as many slots
     uint64_t page_magic;           // block of 16 keys / blocks of a page, as a product
@@ -564,19 +565,19 @@ __device__ __forceinline__ void put_row(const TreeArgs &a, const TreePlan &plan,
     if (a.lse != nullptr && d0 == 0) a.lse[at] = L == 0.0f ? -INFINITY : (M + log2f(L)) * kLn2;
 }
 
-// Few rows (up to 4 tiles, 2 of a workgroup): memory bound.  Each of the 4 waves takes every 4th span of 32 keys, the next
-// span's loads in flight while one is worked on, and the waves are joined through LDS.
+// Few rows (up to 4 tiles, 2 of a workgroup): memory bound.  Each of the W = 4 or 8 waves takes every W-th span of 32 keys,
+// the next span's loads in flight while one is worked on, and the waves are joined through LDS.
 // LO: 32-bit queries, as hi + lo.
 // One row over 130001 e4m3 keys of 8 x 128, 32 heads: 51.8 us and 4.9 of the join, 5.3 TB/s.  64 streams of 270 to 541
-// int8 keys of 12 x 64: 15.7 us; 16 trees of 14 to 27 over 507 to 1015 fp16 keys of 12 x 64: 16.5 and 4.1.  The last two are
-// short of it by their chain of dependent loads (row range, page, keys, then 4 or 5 spans a wave) and by vector work, about
-// 300 instructions a span.
-template <int KV, int D, int MT, bool LO>
-__global__ __launch_bounds__(kThreads, KV == ELEM_F32 ? (D == 64 ? 2 : 1) : (D == 64 && MT == 1 ? 3 : 2)) void attn_tree_kernel(TreeArgs a, TreePlan plan) {
+// int8 keys of 12 x 64: 15.5 us; 16 trees of 14 to 27 over 507 to 1015 fp16 keys of 12 x 64, by 8 waves: 15.6.  The last two
+// are short of it by their chain of dependent loads (row range, page, keys, then 4 or 5 spans a wave) and by vector work,
+// about 300 instructions a span.
+template <int KV, int D, int MT, bool LO, int W>
+__global__ __launch_bounds__(64 * W, W > kWaves ? 2 : KV == ELEM_F32 ? (D == 64 ? 2 : 1) : (D == 64 && MT == 1 ? 3 : 2)) void attn_tree_kernel(TreeArgs a, TreePlan plan) {
     constexpr bool F32 = KV == ELEM_F32, SCALED = quantised(KV);
     constexpr int NW = Keys<KV, D>::NW, ND = D / 16;
-    __shared__ float so[kWaves][16][D + 4];
-    __shared__ float sm[kWaves][16], sl[kWaves][16];
+    __shared__ float so[W][16][D + 4];
+    __shared__ float sm[W][16], sl[W][16];
 
     const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -622,11 +623,11 @@ __global__ __launch_bounds__(kThreads, KV == ELEM_F32 ? (D == 64 ? 2 : 1) : (D =
     rows.clear(SCALED);
 
 #pragma unroll 1
-    for (; p0 < end; p0 += 32 * kWaves) {
+    for (; p0 < end; p0 += 32 * W) {
         const bool tail = p0 + 32 > st.ctx;
         Keys<KV, D> next;
         size_t nblk[2];
-        fetch(p0 + 32 * kWaves, next, nblk);  // (past the end: the last block again)
+        fetch(p0 + 32 * W, next, nblk);  // (past the end: the last block again)
 
         float x[MT][2][4];
 #pragma unroll
@@ -770,14 +771,16 @@ __global__ __launch_bounds__(kThreads, KV == ELEM_F32 ? (D == 64 ? 2 : 1) : (D =
         __syncthreads();
         const int row = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * ND;
         const int i = first + mt * 16 + row;
-        if (i >= packed) continue;
-        const float M = fmaxf(fmaxf(sm[0][row], sm[1][row]), fmaxf(sm[2][row], sm[3][row]));
+        if (row >= 16 || i >= packed) continue;
+        float M = sm[0][row];
+#pragma unroll
+        for (int v = 1; v < W; ++v) M = fmaxf(M, sm[v][row]);
         const float M0 = M == -INFINITY ? 0.0f : M;
         float L = 0.0f, acc[ND];
 #pragma unroll
         for (int j = 0; j < ND; ++j) acc[j] = 0.0f;
 #pragma unroll
-        for (int v = 0; v < kWaves; ++v) {
+        for (int v = 0; v < W; ++v) {
             const float f = exp2_(sm[v][row] - M0);
             L = fmaf(sl[v][row], f, L);
 #pragma unroll
@@ -1098,6 +1101,18 @@ TreePlan plan_of(const KvCacheArgs &c, int heads, int max_rows, int max_keys) {
     const int least = 256, want = 256 * (p.group > 2 ? 1 : (c.dim == 64 && p.group == 1 ? 3 : 2));
     int splits = (int)std::min<long long>(want / base, kMaxSplits);
     splits = std::max(1, std::min(splits, (max_keys + least - 1) / least));
+    // Short keys that would be cut are given to 8 waves of a workgroup instead, without the join: 16 trees of 27 over 1000
+    // fp16 keys of 12 x 64 19.9 -> 15.2 us, 64 rows over 300 int8 keys of 4 x 128 14.4 -> 9.1.  That pays while the cuts
+    // that the workgroups leave room for are few and the spans of a wave are few: where one stream is much longer than
+    // the others, cuts serve it better (1500 keys among 100s: 13.5 us cut, 16.4 so).  Two tiles of 128 dims cost most a
+    // span (16 x 27 over 500 keys of 8 x 128: 22.0 cut in 4, 24.4 so).
+    const int room = (int)std::min<long long>(want / base, kMaxSplits);
+    const int eight_to = c.dim == 128 && p.group == 2 ? (room <= 2 ? 512 : 0) : (room <= 2 ? 1536 : (room <= 4 ? 1024 : 512));
+    p.waves = kWaves;
+    if (p.group <= 2 && c.dtype != ELEM_F32 && splits > 1 && max_keys <= eight_to) {
+        p.waves = 2 * kWaves;
+        splits = 1;
+    }
     p.chunk = ((max_keys + splits - 1) / splits + 127) / 128 * 128;
     p.slots = splits * c.streams;
     // blk / (page_size / 16) for blk < 2^24 and a divisor up to 2^11: 2^40 / d rounded up is off by
@@ -1107,14 +1122,25 @@ TreePlan plan_of(const KvCacheArgs &c, int heads, int max_rows, int max_keys) {
     return p;
 }
 
+template <int KV, int D, int MT, bool LO>
+void launch_few(dim3 grid, const TreeArgs &a, const TreePlan &p, hipStream_t s) {
+    if constexpr (KV != ELEM_F32) {
+        if (p.waves > kWaves) {
+            hipLaunchKernelGGL((attn_tree_kernel<KV, D, MT, LO, 2 * kWaves>), grid, dim3(2 * kThreads), 0, s, a, p);
+            return;
+        }
+    }
+    hipLaunchKernelGGL((attn_tree_kernel<KV, D, MT, LO, kWaves>), grid, dim3(kThreads), 0, s, a, p);
+}
+
 template <int KV, int D, bool LO>
 void launch_group(const TreeArgs &a, const TreePlan &p, hipStream_t s) {
     const long long units = (long long)p.slots * a.c.heads;
     const dim3 grid((unsigned)((units + 7) / 8 * 8 * p.row_groups));
     if (p.group == 1) {
-        hipLaunchKernelGGL((attn_tree_kernel<KV, D, 1, LO>), grid, dim3(kThreads), 0, s, a, p);
+        launch_few<KV, D, 1, LO>(grid, a, p, s);
     } else if (p.group == 2) {
-        hipLaunchKernelGGL((attn_tree_kernel<KV, D, 2, LO>), grid, dim3(kThreads), 0, s, a, p);
+        launch_few<KV, D, 2, LO>(grid, a, p, s);
     } else if constexpr (KV != ELEM_F32) {
         const bool f16 = a.out_dtype == ELEM_F16;
         if (p.group == 8 && f16)

@@ -413,6 +413,21 @@ def test_attn_trees(torch_gpu, cache, dim, heads, kvh, page, n):
     _check_attn(torch, c, q.float() * 1.37, start, ctx, None, odt="f16")
 
 
+@pytest.mark.parametrize("cache", ["f16", "i8", "e4m3"])
+@pytest.mark.parametrize("dim,heads,kvh,n", [(64, 12, 12, [1] * 16), (64, 12, 12, [27, 1, 0, 14] * 4), (128, 8, 2, [4, 2] * 24), (128, 4, 4, [32, 7]),
+                                             (64, 8, 8, [33, 64, 5])])
+def test_attn_under_other_bounds(torch_gpu, cache, dim, heads, kvh, n):
+    """The bound on the keys chooses how they are shared out (by waves of one workgroup, or cut and joined): the same rows
+    under their own bound, one key more than short lengths, and a far one."""
+    torch = torch_gpu
+    print(f"attn bounds {cache} {dim} {heads}/{kvh} {n[:4]}", flush=True)
+    ctx = [int(k) for k in np.random.default_rng(len(n)).integers(0, 480, len(n))]
+    ctx[0], ctx[-1] = 470, 0
+    c, start, rows, masks, q = _attn_case(torch, cache, dim, heads, kvh, 32, ctx, n, False, sum(n))
+    for bound in (None, 513, 1025, 1537, 9000):
+        _check_attn(torch, c, q, start, ctx, masks, max_keys=bound)
+
+
 @pytest.mark.parametrize("cache,dim,n", [("f16", 64, 1), ("i8", 128, 1), ("e4m3", 64, 3), ("f32", 64, 2), ("i8", 64, 40)])
 def test_attn_long_context(torch_gpu, cache, dim, n):
     """Keys cut over workgroups and joined; a short stream beside a long one leaves whole splits without keys."""
