@@ -224,8 +224,8 @@ struct Cut {
 };
 // Up to 64 streams share the slots out by their lengths: pieces of the fewest keys (a multiple of 128, at least 256)
 // of which there are no more than slots, so that no workgroup has much more to do than another, however
-// ragged the streams (7 of 8192 to 16384 keys and one just begun: 203 us with as many pieces each, 172 so, both before later steps).  Every
-// wave finds that size for itself, lane s holding stream s.  More streams: as many slots each.
+// ragged the streams (7 of 8192 to 16384 keys and one just begun: 203 us with as many pieces each, 172 so, both
+// before later steps).  Every wave finds that size for itself, lane s holding stream s.  More streams: as many slots each.
 __device__ __forceinline__ int sum64(int v) {
     v += xshfl<32>(v);
     v += xshfl<16>(v);
