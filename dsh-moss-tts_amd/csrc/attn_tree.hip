@@ -795,9 +795,7 @@ __global__ __launch_bounds__(64 * W, W > kWaves ? 2 : KV == ELEM_F32 ? (D == 64 
 // fragments, K and V, and puts them into LDS in the order in which the products read them (16 bytes a lane, no
 // bank conflicts), so a key is converted once for up to 256 rows.  Two stages: while one is worked on the next
 // one's loads are in flight, and it is written before the only barrier of a stage.
-// PLO: weights as hi + lo; where the output is fp16 they are rounded to fp16 once, to nearest: an error of the
-// size of the output's own rounding (2.9e-4 in all where rounding the output alone gives 2.1e-4), for a third of the
-// products less: 211 and 255 us when that was measured.
+// LO: 32-bit queries, as hi + lo; the weights are hi + lo whatever the output's type is.
 // 8 streams with trees of 33 to 64, 32 heads of 128 on 8 key heads, 8192 to 16384 int8 keys: 162 to 175 us from run to
 // run, and 9.3 of the join.
 // The vector unit is what is busy most: 72 us of the softmax (a score: scale, maximum, exponential of 4 slots, sum, value
@@ -817,7 +815,7 @@ struct WideLds {
     float room[KV == ELEM_I8 ? 1 : NWV][16][36];
 };
 
-template <int KV, int D, int NWV, int MT, bool LO, bool PLO>
+template <int KV, int D, int NWV, int MT, bool LO>
 __global__ __launch_bounds__(64 * NWV, 2) void attn_tree_wide_kernel(TreeArgs a, TreePlan plan) {
     constexpr bool SCALED = quantised(KV);
     constexpr int NW = Keys<KV, D>::NW, NS = D / 32, ND = D / 16, DW = dims_per_word<KV>();
@@ -961,20 +959,13 @@ __global__ __launch_bounds__(64 * NWV, 2) void attn_tree_wide_kernel(TreeArgs a,
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt) rows.weigh(mt, q[mt].qs, x[mt]);
                 if constexpr (SCALED) scale_weights(st, q, tail, p0, g, vs, x);
-                Frag ph[MT], pl[PLO ? MT : 1];
+                Frag ph[MT], pl[MT];
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
                     for (int b = 0; b < 2; ++b)
 #pragma unroll
-                        for (int i = 0; i < 4; i += 2) {
-                            if constexpr (PLO) {
-                                split2(x[mt][b][i], x[mt][b][i + 1], ph[mt].w[2 * b + i / 2], pl[mt].w[2 * b + i / 2]);
-                            } else {
-                                const h2 y = {(_Float16)x[mt][b][i], (_Float16)x[mt][b][i + 1]};
-                                ph[mt].w[2 * b + i / 2] = __builtin_bit_cast(uint32_t, y);
-                            }
-                        }
+                        for (int i = 0; i < 4; i += 2) split2(x[mt][b][i], x[mt][b][i + 1], ph[mt].w[2 * b + i / 2], pl[mt].w[2 * b + i / 2]);
                 if constexpr (KV != ELEM_I8) {
                     if (tail && (lds.odd[buf][2 * u] | lds.odd[buf][2 * u + 1])) {
                         size_t blk[2];
@@ -991,7 +982,7 @@ __global__ __launch_bounds__(64 * NWV, 2) void attn_tree_wide_kernel(TreeArgs a,
 #pragma unroll
                     for (int mt = 0; mt < MT; ++mt) {
                         rows.o[mt][j] = mfma(f, ph[mt], rows.o[mt][j]);
-                        if constexpr (PLO) rows.o[mt][j] = mfma(f, pl[mt], rows.o[mt][j]);
+                        rows.o[mt][j] = mfma(f, pl[mt], rows.o[mt][j]);
                     }
                 }
             }
@@ -1142,15 +1133,10 @@ void launch_group(const TreeArgs &a, const TreePlan &p, hipStream_t s) {
     } else if (p.group == 2) {
         launch_few<KV, D, 2, LO>(grid, a, p, s);
     } else if constexpr (KV != ELEM_F32) {
-        const bool f16 = a.out_dtype == ELEM_F16;
-        if (p.group == 8 && f16)
-            hipLaunchKernelGGL((attn_tree_wide_kernel<KV, D, 8, 1, LO, false>), grid, dim3(512), 0, s, a, p);
-        else if (p.group == 8)
-            hipLaunchKernelGGL((attn_tree_wide_kernel<KV, D, 8, 1, LO, true>), grid, dim3(512), 0, s, a, p);
-        else if (f16)
-            hipLaunchKernelGGL((attn_tree_wide_kernel<KV, D, 8, 2, LO, false>), grid, dim3(512), 0, s, a, p);
+        if (p.group == 8)
+            hipLaunchKernelGGL((attn_tree_wide_kernel<KV, D, 8, 1, LO>), grid, dim3(512), 0, s, a, p);
         else
-            hipLaunchKernelGGL((attn_tree_wide_kernel<KV, D, 8, 2, LO, true>), grid, dim3(512), 0, s, a, p);
+            hipLaunchKernelGGL((attn_tree_wide_kernel<KV, D, 8, 2, LO>), grid, dim3(512), 0, s, a, p);
     }
 }
 

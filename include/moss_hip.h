@@ -439,10 +439,9 @@ int moss_hip_kv_read(const moss_hip_kv_cache *cache, const int32_t *row_stream, 
  * too.  max_keys bounds every stream's ctx_len + n and sizes the launch.  A stream whose ctx_len is
  * negative, whose keys pass max_keys or its table, or with a page outside [0, n_pages) among them, gets
  * NaN rows; one whose row range is not within [0, rows] gets none.  Rows of no stream, and a stream's rows past
- * max_rows, stay as they were.  With an fp16 output and max_rows * (heads / kv_heads) > 64, the softmax
- * weights are rounded to fp16 (once, to nearest); otherwise sums, weights and statistics have 22 bits or more.
- * The same call gives the same bits.  workspace: moss_hip_attn_tree_workspace bytes (any content, 16-byte
- * aligned; NULL where that is 0). */
+ * max_rows, stay as they were.  Sums, weights and statistics have 22 bits or more whatever the types of
+ * q and out are; out is rounded once.  The same call gives the same bits.  workspace:
+ * moss_hip_attn_tree_workspace bytes (any content, 16-byte aligned; NULL where that is 0). */
 int moss_hip_attn_tree(const void *q, int64_t q_stride, int q_dtype, int heads, const moss_hip_kv_cache *cache,
                        const int32_t *row_start, const int32_t *ctx_len, const uint64_t *row_mask, int rows, int max_rows,
                        int max_keys, float scale, void *out, int64_t out_stride, int out_dtype, float *lse, void *workspace,
