@@ -23,8 +23,8 @@
 // Arithmetic: fp16, int8 and e4m3 values are exact in the fp16 products; a 32-bit query (scaled by a
 // power of two to below 2) and the softmax weights go in as fp16 hi + lo, 22 bits, so results are as
 // good as 32-bit ones.  int8 / e4m3 scales multiply the scores and the weights; weights are kept in
-// fp16's range by the largest value scale seen, a power of two E that is wave-uniform and rises like the
-// running maximum.  An fp32 cache runs on the fp32 matrix instructions.
+// fp16's range by a power of two of each row's own, which falls as the row's largest weight times value scale
+// rises.  An fp32 cache runs on the fp32 matrix instructions.
 #include <algorithm>
 
 #include "paged_ops.h"
@@ -38,8 +38,9 @@ typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 constexpr int kWaves = 4, kThreads = 64 * kWaves;
 constexpr int kMaxSplits = 64;
 constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.69314718055994531f;
-constexpr float kSlack = 8.0f;  // log 2 of how far a weight may pass 1
-constexpr int kWeightExp = 6;   // and of what it is scaled by
+constexpr float kSlack = 8.0f;  // log 2 of how far below its place a row's largest weight may lie
+constexpr float kPlace = 15.0f;  // log 2 of that place in fp16's range
+constexpr float kLeast = -109.0f;  // log 2 of the least product of weight and value scale that is put there (2^(kPlace - kLeast) is a float)
 
 struct TreePlan {
     int tiles, group, row_groups;  // row tiles of 16, of which a workgroup takes `group`
@@ -373,88 +374,102 @@ struct Query {
     }
 };
 
-// The drafted positions that any row of a wave's tiles sees.
-template <class Q, int MT>
-__device__ __forceinline__ uint64_t seen_by(const Q (&q)[MT]) {
-    uint64_t seen = 0;
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt) seen |= q[mt].mask;
-    uint32_t lo = (uint32_t)seen, hi = (uint32_t)(seen >> 32);
-    lo |= xshfl<1>((int)lo), hi |= xshfl<1>((int)hi);
-    lo |= xshfl<2>((int)lo), hi |= xshfl<2>((int)hi);
-    lo |= xshfl<4>((int)lo), hi |= xshfl<4>((int)hi);
-    lo |= xshfl<8>((int)lo), hi |= xshfl<8>((int)hi);
-    return ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane(hi) << 32) | (uint32_t)__builtin_amdgcn_readfirstlane(lo);
-}
-
 // Whether a row whose mask is `bits` sees key `pos` (of a stream's ctx + n).
 __device__ __forceinline__ bool visible(const Stream &st, uint64_t bits, int pos) {
     const int j = pos - st.ctx;
     return j < 0 || (j < st.n && ((bits >> (j & 63)) & 1));
 }
 
-// Softmax state of a lane's rows, one per tile: o = sum 2^(x - m) v, l = sum 2^(x - m) over the scores x so
-// far, l of this lane's keys only.  m is `ref` less `up`, whole numbers both, so scaling by their changes is
-// exact.  ref is at most kSlack under the largest score so far: it moves (and o and l are scaled) only when a
-// score passes it by more, which after the first spans is rare, where the largest itself still moves in every
-// other span for some row of a tile.  2^up makes the weights use fp16's range: with value scales below 2^(e + 1) a
-// weight times its scale stays under 2^15.5 at up = kWeightExp - e (at most 90), slack and all.
-template <int MT, int ND>
+// Softmax state of a lane's rows, one per tile: l = sum w, o = sum w v with weights w = 2^(x - ref) of the scores x so far,
+// l of this lane's keys only.  ref is a whole number, so scaling by its changes is exact; no score passes it by more
+// than 1/2, and the largest is at most kSlack + 1/2 below it: it moves (and o and l are scaled) only when a score passes it,
+// which after the first spans is rare, where the largest itself still moves in every other span for some row of a tile.
+// For the fp16 products the weights are multiplied by 2^kPlace; with value scales (SCALED) a weight times its scale
+// is, by 2^(kPlace - top), where no such product of the row so far has passed 2^top: top moves like ref.  Both are a
+// row's own business: what other rows of a tile see changes nothing.  `settle` takes these factors out.
+template <int MT, int ND, bool SCALED, bool F32>
 struct Rows {
+    static constexpr float kUp = F32 || SCALED ? 0.0f : kPlace;  // log 2 of what w itself is multiplied by
     float ref[MT], l[MT];
+    float top[SCALED ? MT : 1], g[SCALED ? MT : 1];  // g = 2^(kPlace - top)
     floatx4 o[MT][ND];
-    float up;
 
-    __device__ __forceinline__ void clear(bool scaled) {
-        up = scaled ? 90.0f : (float)kWeightExp;
+    __device__ __forceinline__ void clear() {
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
             ref[mt] = -INFINITY;
             l[mt] = 0.0f;
+            if constexpr (SCALED) {
+                top[mt] = kLeast;
+                g[mt] = exp2_(kPlace - kLeast);
+            }
 #pragma unroll
             for (int j = 0; j < ND; ++j) o[mt][j] = floatx4{0.f, 0.f, 0.f, 0.f};
         }
     }
-    __device__ __forceinline__ float m(int mt) const { return ref[mt] - up; }
-    // A new up for all rows, before their next scores.
-    __device__ __forceinline__ void raise(float up_new) {
-        const int by = (int)(up_new - up);  // (2^by itself can be below what fp32 holds)
-        up = up_new;
+    __device__ __forceinline__ void settle(int mt) {
+        if constexpr (!SCALED) l[mt] *= exp2_(-kUp);
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-            l[mt] = __builtin_amdgcn_ldexpf(l[mt], by);
+        for (int j = 0; j < ND; ++j)
 #pragma unroll
-            for (int j = 0; j < ND; ++j)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) o[mt][j][r] = __builtin_amdgcn_ldexpf(o[mt][j][r], by);
-        }
+            for (int r = 0; r < 4; ++r)  // (2^(top - kPlace) itself can be below what fp32 holds)
+                o[mt][j][r] = SCALED ? __builtin_amdgcn_ldexpf(o[mt][j][r], (int)(top[mt] - kPlace)) : o[mt][j][r] * exp2_(-kUp);
     }
-    // Products x (times key scales) of 32 keys, -inf where the row does not see the key, become weights.
-    __device__ __forceinline__ void weigh(int mt, float qs, float (&x)[2][4]) {
+    // Products x (times key scales) of 32 keys, -inf where the row does not see the key, become weights (times 2^kUp).
+    // Returns how far the largest of these scores is from ref.
+    __device__ __forceinline__ float weigh(int mt, float qs, float (&x)[2][4]) {
         float mx = fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])), fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3])));
         mx = fmaxf(mx, xshfl<16>(mx));
         mx = fmaxf(mx, xshfl<32>(mx)) * qs;
-        if (__any(mx > ref[mt] + kSlack)) {
-            const float r = mx > ref[mt] + kSlack ? rintf(mx) : ref[mt];  // (a row's own business, whatever its tile does)
-            const float fade = r == -INFINITY ? 1.0f : exp2_(ref[mt] - r);
+        if (__any(mx > ref[mt])) {
+            const bool up = mx > ref[mt];
+            const float r = up ? rintf(mx) + kSlack : ref[mt], by = up ? ref[mt] - r : 0.0f;
             ref[mt] = r;
-            l[mt] *= fade;
+            l[mt] *= exp2_(by);
+            float fade = exp2_(by);
+            if constexpr (SCALED) {  // top stays where it was, unless it would fall under kLeast
+                const float t = fmaxf(top[mt] + by, kLeast);
+                fade = exp2_(top[mt] + by - t);
+                top[mt] = t;
+                g[mt] = exp2_(kPlace - t);
+            }
 #pragma unroll
             for (int j = 0; j < ND; ++j) o[mt][j] *= fade;
         }
-        const float m0 = ref[mt] == -INFINITY ? 0.0f : ref[mt] - up;
+        const float r0 = ref[mt] == -INFINITY ? 0.0f : ref[mt];
 #pragma unroll
         for (int b = 0; b < 2; ++b)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                x[b][i] = exp2_(fmaf(x[b][i], qs, -m0));
+                x[b][i] = exp2_(fmaf(x[b][i], qs, kUp - r0));
                 l[mt] += x[b][i];
             }
+        return mx - r0;
+    }
+    // Weights times value scales, 0 where the row does not see the key, are put in place: `most` is what weigh returned and
+    // `vmax` log 2 of what no scale of the 32 keys reaches, seen or not.
+    __device__ __forceinline__ void place(int mt, float most, float vmax, float (&y)[2][4]) {
+        if (__any(most + vmax > top[mt] - 0.015625f)) {  // (less a margin for the roundings of `most`: where this is false, no product passes top)
+            float m = fmaxf(fmaxf(fmaxf(fabsf(y[0][0]), fabsf(y[0][1])), fmaxf(fabsf(y[0][2]), fabsf(y[0][3]))),
+                            fmaxf(fmaxf(fabsf(y[1][0]), fabsf(y[1][1])), fmaxf(fabsf(y[1][2]), fabsf(y[1][3]))));
+            m = fmaxf(m, xshfl<16>(m));
+            m = fmaxf(m, xshfl<32>(m));
+            const float e = (float)((int)(__float_as_uint(m) >> 23) - 126);  // m < 2^e
+            const float t = e > top[mt] ? e + kSlack : top[mt], fade = exp2_(top[mt] - t);
+            top[mt] = t;
+            g[mt] = exp2_(kPlace - t);
+#pragma unroll
+            for (int j = 0; j < ND; ++j) o[mt][j] *= fade;
+        }
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) y[b][i] *= g[mt];
     }
 };
 
-// `up` for value scales of which the largest has these bits.
-__device__ __forceinline__ float up_of(uint32_t top) { return fminf((float)(kWeightExp + 127 - (int)(top >> 23)), 90.0f); }
+// log 2 of what no value with a magnitude up to this one's reaches.
+__device__ __forceinline__ float above(uint32_t bits) { return (float)((int)(bits >> 23) - 126); }
 
 // x of the keys that a row does not see becomes `v` (32 keys at p0).
 template <class Q, int MT>
@@ -484,9 +499,9 @@ __device__ __forceinline__ void scale_weights(const Stream &st, const Q (&q)[MT]
 
 // The Inf and NaN elements of V among 32 keys, added key by key to the rows that see them (x: weights,
 // `room` the wave's [16][ >= 32] floats of LDS).
-template <int KV, int D, int MT, class Room>
+template <int KV, int D, class Room, class R>
 __device__ __forceinline__ void add_odd_values(const TreeArgs &a, const Stream &st, const size_t (&blk)[2], int p0, int mt,
-                                               uint64_t mask, const float (&x)[2][4], Room &room, Rows<MT, D / 16> &rows) {
+                                               uint64_t mask, const float (&x)[2][4], Room &room, R &rows) {
     const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
 #pragma unroll
     for (int b = 0; b < 2; ++b)
@@ -618,9 +633,8 @@ __global__ __launch_bounds__(64 * W, W > kWaves ? 2 : KV == ELEM_F32 ? (D == 64 
     Query<KV, D, LO> q[MT];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) q[mt].load(a, st, grp, h, first + mt * 16 + c, packed, g);
-    const uint64_t seen = seen_by(q);
-    Rows<MT, ND> rows;
-    rows.clear(SCALED);
+    Rows<MT, ND, SCALED, F32> rows;
+    rows.clear();
 
 #pragma unroll 1
     for (; p0 < end; p0 += 32 * W) {
@@ -663,31 +677,19 @@ __global__ __launch_bounds__(64 * W, W > kWaves ? 2 : KV == ELEM_F32 ? (D == 64 
                 for (int i = 0; i < 4; ++i) x[mt][b][i] = SCALED ? acc[mt][i] * ks[i] : acc[mt][i];
         }
         if (tail) hide(st, q, p0, g, -INFINITY, x);
+        float most[MT];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) most[mt] = rows.weigh(mt, q[mt].qs, x[mt]);
         if constexpr (SCALED) {
-            uint32_t top = 0;
-            if (tail) {
+            scale_weights(st, q, tail, p0, g, cur.vs, x);
+            float v = fmaxf(fmaxf(fmaxf(fabsf(cur.vs[0].x), fabsf(cur.vs[0].y)), fmaxf(fabsf(cur.vs[0].z), fabsf(cur.vs[0].w))),
+                            fmaxf(fmaxf(fabsf(cur.vs[1].x), fabsf(cur.vs[1].y)), fmaxf(fabsf(cur.vs[1].z), fabsf(cur.vs[1].w))));
+            v = fmaxf(v, xshfl<16>(v));
+            v = fmaxf(v, xshfl<32>(v));
+            const float vmax = above((uint32_t)__builtin_amdgcn_readfirstlane((int)__float_as_uint(v)));
 #pragma unroll
-                for (int b = 0; b < 2; ++b) {
-                    const float vs[4] = {cur.vs[b].x, cur.vs[b].y, cur.vs[b].z, cur.vs[b].w};
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const uint32_t y = __float_as_uint(vs[i]) & 0x7fffffffu;
-                        top = max(top, y < 0x7f800000u && visible(st, seen, p0 + 16 * b + 4 * g + i) ? y : 0u);
-                    }
-                }
-            } else {  // (an Inf or NaN here is every row's)
-                const float v = fmaxf(fmaxf(fmaxf(fabsf(cur.vs[0].x), fabsf(cur.vs[0].y)), fmaxf(fabsf(cur.vs[0].z), fabsf(cur.vs[0].w))),
-                                      fmaxf(fmaxf(fabsf(cur.vs[1].x), fabsf(cur.vs[1].y)), fmaxf(fabsf(cur.vs[1].z), fabsf(cur.vs[1].w))));
-                top = __float_as_uint(v);
-            }
-            top = max(top, (uint32_t)xshfl<16>((int)top));
-            top = max(top, (uint32_t)xshfl<32>((int)top));
-            const float up = up_of((uint32_t)__builtin_amdgcn_readfirstlane((int)top));
-            if (up < rows.up) rows.raise(up);
+            for (int mt = 0; mt < MT; ++mt) rows.place(mt, most[mt], vmax, x[mt]);
         }
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) rows.weigh(mt, q[mt].qs, x[mt]);
-        if constexpr (SCALED) scale_weights(st, q, tail, p0, g, cur.vs, x);
         Frag ph[MT], pl[MT];
         if constexpr (!F32)
 #pragma unroll
@@ -754,6 +756,7 @@ __global__ __launch_bounds__(64 * W, W > kWaves ? 2 : KV == ELEM_F32 ? (D == 64 
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
         if (mt >= live) break;
+        rows.settle(mt);
         float sum = rows.l[mt];
         sum += xshfl<16>(sum);
         sum += xshfl<32>(sum);
@@ -765,7 +768,7 @@ __global__ __launch_bounds__(64 * W, W > kWaves ? 2 : KV == ELEM_F32 ? (D == 64 
                 *(float4 *)&so[w][c][ND * (4 * g + r) + j] =
                     make_float4(rows.o[mt][j][r], rows.o[mt][j + 1][r], rows.o[mt][j + 2][r], rows.o[mt][j + 3][r]);
         if (g == 0) {
-            sm[w][c] = rows.m(mt);
+            sm[w][c] = rows.ref[mt];
             sl[w][c] = bad ? __uint_as_float(0x7fc00000u) : sum;
         }
         __syncthreads();
@@ -810,7 +813,6 @@ struct WideLds {
     float ks[2][NWV][16], vs[2][NWV][16];
     uint32_t top[2][NWV];
     int odd[2][NWV];
-    uint64_t seen[NWV];
     int bad[NWV];
     float room[KV == ELEM_I8 ? 1 : NWV][16][36];
 };
@@ -855,12 +857,6 @@ __global__ __launch_bounds__(64 * NWV, 2) void attn_tree_wide_kernel(TreeArgs a,
     Query<KV, D, LO> q[MT];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) q[mt].load(a, st, grp, h, first + mt * 16 + c, packed, g);
-    uint64_t seen = seen_by(q);
-    if (lane == 0) lds.seen[w] = seen;
-    lds_barrier();
-    seen = 0;
-#pragma unroll
-    for (int v = 0; v < NWV; ++v) seen |= lds.seen[v];
 
     auto put = [&](int buf, int p) {  // this wave's block of the stage at p
         const int pos = p + 16 * w;
@@ -893,7 +889,6 @@ __global__ __launch_bounds__(64 * NWV, 2) void attn_tree_wide_kernel(TreeArgs a,
         }
         if constexpr (SCALED) {
             uint32_t top = __float_as_uint(vsr) & 0x7fffffffu;
-            if (top >= 0x7f800000u || !visible(st, seen, pos + c)) top = 0;
             top = max(top, (uint32_t)xshfl<1>((int)top));
             top = max(top, (uint32_t)xshfl<2>((int)top));
             top = max(top, (uint32_t)xshfl<4>((int)top));
@@ -906,8 +901,8 @@ __global__ __launch_bounds__(64 * NWV, 2) void attn_tree_wide_kernel(TreeArgs a,
         }
     };
 
-    Rows<MT, ND> rows;
-    rows.clear(SCALED);
+    Rows<MT, ND, SCALED, false> rows;
+    rows.clear();
     if (beg < end) put(0, beg);
     lds_barrier();
     int buf = 0;
@@ -923,9 +918,9 @@ __global__ __launch_bounds__(64 * NWV, 2) void attn_tree_wide_kernel(TreeArgs a,
                 const bool tail = p0 + 32 > st.ctx;
                 float x[MT][2][4];
                 float4 ks[2], vs[2];
-                float up = 0.0f;
+                float vmax = 0.0f;
                 if constexpr (SCALED) {
-                    up = up_of((uint32_t)__builtin_amdgcn_readfirstlane((int)max(lds.top[buf][2 * u], lds.top[buf][2 * u + 1])));
+                    vmax = above((uint32_t)__builtin_amdgcn_readfirstlane((int)max(lds.top[buf][2 * u], lds.top[buf][2 * u + 1])));
 #pragma unroll
                     for (int b = 0; b < 2; ++b) {
                         ks[b] = *(const float4 *)&lds.ks[buf][2 * u + b][4 * g];
@@ -953,12 +948,14 @@ __global__ __launch_bounds__(64 * NWV, 2) void attn_tree_wide_kernel(TreeArgs a,
                         for (int i = 0; i < 4; ++i) x[mt][b][i] = SCALED ? acc[mt][i] * ((const float *)&ks[b])[i] : acc[mt][i];
                 }
                 if (tail) hide(st, q, p0, g, -INFINITY, x);
-                if constexpr (SCALED) {
-                    if (up < rows.up) rows.raise(up);
-                }
+                float most[MT];
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt) rows.weigh(mt, q[mt].qs, x[mt]);
-                if constexpr (SCALED) scale_weights(st, q, tail, p0, g, vs, x);
+                for (int mt = 0; mt < MT; ++mt) most[mt] = rows.weigh(mt, q[mt].qs, x[mt]);
+                if constexpr (SCALED) {
+                    scale_weights(st, q, tail, p0, g, vs, x);
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt) rows.place(mt, most[mt], vmax, x[mt]);
+                }
                 Frag ph[MT], pl[MT];
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt)
@@ -1000,6 +997,7 @@ __global__ __launch_bounds__(64 * NWV, 2) void attn_tree_wide_kernel(TreeArgs a,
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
         const int i = first + mt * 16 + c;
+        rows.settle(mt);
         float L = rows.l[mt];
         L += xshfl<16>(L);
         L += xshfl<32>(L);
@@ -1009,7 +1007,7 @@ __global__ __launch_bounds__(64 * NWV, 2) void attn_tree_wide_kernel(TreeArgs a,
         for (int r = 0; r < 4; ++r)
 #pragma unroll
             for (int j = 0; j < ND; ++j) y[ND * r + j] = rows.o[mt][j][r];
-        if (i < packed) put_row<D, 4 * ND>(a, plan, st, slot, grp, h, i, (D / 4) * g, rows.m(mt), L, y);
+        if (i < packed) put_row<D, 4 * ND>(a, plan, st, slot, grp, h, i, (D / 4) * g, rows.ref[mt], L, y);
     }
 }
 

@@ -34,3 +34,138 @@ def test_attn_many_rows(torch_gpu, cache, dim, heads, kvh, n, ctx, qdt, odt):
         tol = tol + np.abs(want) * U16 + 2.0 ** -25
     assert (np.abs(got - want) <= tol).all(), np.max(np.abs(got - want) / tol)
     assert (np.abs(lse - wl) <= ltol).all()
+
+
+# ---------------------------------------------------------------- weights and value scales
+
+def _put(c, s, pos, k=None, v=None, ks=None, vs=None):
+    """Elements (as the pools hold them) and scales of positions `pos` of stream s, every head."""
+    import torch
+    page = c.tensors[0].shape[2]
+    for p in pos:
+        at = (int(c.tensors[2][s, p // page]), slice(None), p % page)
+        for pool, scale, x, d in ((c.tensors[0], c.tensors[3], k, ks), (c.tensors[1], c.tensors[4], v, vs)):
+            if x is not None:
+                x = torch.as_tensor(x).expand(pool[at].shape)
+                pool[at] = x.to(pool.dtype).to(pool.device)
+            if d is not None and scale is not None:
+                scale[at] = d
+
+
+def _raw(c, which, s, n):
+    """The first n positions of stream s in 64 bits: elements [heads][n][dim] and their scales [heads][n]."""
+    import torch
+    pool, scale = c.tensors[which], c.tensors[3 + which]
+    page = pool.shape[2]
+    pages = c.tensors[2][s, :(n + page - 1) // page].long()
+    x = pool.view(torch.int8)[pages].view(pool.dtype).double().transpose(0, 1).flatten(1, 2)[:, :n].cpu().numpy()
+    if scale is None:
+        return x, np.ones(x.shape[:2])
+    return x, scale[pages].double().transpose(0, 1).flatten(1, 2)[:, :n].cpu().numpy()
+
+
+def _fine_ref(q, c, start, ctx, mask, scale, heads, exact_products=False):
+    """out and lse in 64 bits, and tolerances key by key.
+
+    A score is off by 24 roundings of scale * sum |q k| (none where the products are exact), a weight by 4 roundings of the
+    scores it is the difference of, exp2's and the weight's own 2^-22 (with the value scale's product 2^-21); sums chain
+    keys / 16 + 64 roundings.  Below its 22 bits a weight (times its value scale) has a step: it is off by up to 2^-29 of the
+    row's largest."""
+    rows = len(q)
+    out, tol = np.zeros((rows, heads, c.head_dim)), np.zeros((rows, heads, c.head_dim))
+    lse, ltol = np.full((rows, heads), -np.inf), np.zeros((rows, heads))
+    for s in range(len(ctx)):
+        a, b, n = int(start[s]), int(start[s + 1]), int(ctx[s] + start[s + 1] - start[s])
+        if b == a:
+            continue
+        (k, ks), (v, vs) = _raw(c, 0, s, n), _raw(c, 1, s, n)
+        for r in range(a, b):
+            m = (2 << (r - a)) - 1 if mask is None else int(mask[r])
+            see = np.array([j < ctx[s] or (m >> (j - int(ctx[s]))) & 1 for j in range(n)], bool)
+            if not see.any():
+                continue
+            for h in range(heads):
+                g = h * c.kv_heads // heads
+                kk, u, d, qq = k[g][see] * ks[g][see][:, None], v[g][see], vs[g][see], q[r, h].astype(np.float64)
+                x = scale * (kk @ qq)
+                e = np.exp(x - x.max())
+                p = e / e.sum()
+                w = p * np.abs(d)
+                err = 4 * U32 * (np.abs(x) + np.abs(x.max())) + 2.0 ** -21
+                if not exact_products:
+                    err = err + 24 * U32 * abs(scale) * (np.abs(kk) @ np.abs(qq))
+                chain = (n / 16 + 64) * U32
+                norm = (p * err).sum() + chain
+                out[r, h] = (p * d) @ u
+                tol[r, h] = ((err + norm + chain) * w) @ np.abs(u) + 2.0 ** -29 * w.max() * np.abs(u).sum(0) + 2 * U32 * np.abs(out[r, h])
+                lse[r, h] = x.max() + np.log(e.sum())
+                ltol[r, h] = norm + 4 * U32 * (np.abs(lse[r, h]) + np.abs(x.max()))
+    return out, lse, tol, ltol
+
+
+def _check_fine(torch, c, q, start, ctx, masks, heads, exact_products=False, scale=None, **kw):
+    n = np.diff(start)
+    got, lse = _run_attn(torch, c, q, start, ctx, masks, int(n.max()), int((np.array(ctx) + n).max()), scale=scale, **kw)
+    want, wl, tol, ltol = _fine_ref(q.float().numpy(), c, start, ctx, masks, c.head_dim ** -0.5 if scale is None else scale, heads,
+                                    exact_products)
+    bad = ~(np.abs(got - want) <= tol)
+    assert not bad.any(), (np.argwhere(bad)[:3], got[bad][:3], want[bad][:3], tol[bad][:3])
+    fin = np.isfinite(wl)
+    assert np.array_equal(fin, np.isfinite(lse)) and (np.abs(lse[fin] - wl[fin]) <= ltol[fin]).all()
+    return got, lse
+
+
+@pytest.mark.parametrize("cache", ["i8", "e4m3"])
+@pytest.mark.parametrize("dim,heads,kvh,n", [(64, 4, 2, 6), (128, 8, 2, 6), (64, 4, 1, 40), (128, 8, 2, 20)])
+def test_attn_finite_scales_behind_the_mask(torch_gpu, cache, dim, heads, kvh, n):
+    """A drafted key's value scale, however large, changes not a bit of the rows that do not see it: roots beside it without
+    a context, and rows with one.  A row that does see it is as good as ever."""
+    torch = torch_gpu
+    print(f"attn scales behind the mask {cache} {dim} {heads}/{kvh} {n}", flush=True)
+    ctx = [37, 0]
+    c, start, rows, masks, q = _attn_case(torch, cache, dim, heads, kvh, 16, ctx, [n, n], False, 78)
+    masks = [m & ~(1 << 2) for m in masks]
+    masks = [m | (1 << 2) if r in (1, n + 3) else m for r, m in enumerate(masks)]
+    hit = np.isin(np.arange(rows), (1, n + 3))
+    clean, lse = _check_fine(torch, c, q, start, ctx, masks, heads)
+    for big in (1e4, 1e6, 1e8, 1e30):
+        for s in (0, 1):
+            _put(c, s, [ctx[s] + 2], vs=big)
+        got, l = _check_fine(torch, c, q, start, ctx, masks, heads)
+        assert np.array_equal(got[~hit], clean[~hit]) and np.array_equal(l, lse), big
+
+
+@pytest.mark.parametrize("cache", ["i8", "e4m3"])
+@pytest.mark.parametrize("dim,heads,kvh,n", [(64, 2, 1, 1), (64, 4, 1, 40), (128, 8, 2, 20)])
+@pytest.mark.parametrize("big", [2.0 ** 6, 1e4, 1e12, 1e30])
+def test_attn_scale_of_a_key_without_weight(torch_gpu, cache, dim, heads, kvh, n, big):
+    """One value scale of the context far above the others, on a key with next to no weight."""
+    torch = torch_gpu
+    print(f"attn scale without weight {cache} {dim} {heads}/{kvh} {n} {big}", flush=True)
+    ctx = [541]
+    c, start, rows, masks, q = _attn_case(torch, cache, dim, heads, kvh, 64, ctx, [n], False, 79)
+    q[..., 0] = 8.0
+    k = torch.zeros(dim)
+    k[0] = -64.0
+    _put(c, 0, [100], k=k, ks=2.0 if dim == 128 else 1.5, vs=big)  # a score of -90 or -96
+    _check_fine(torch, c, q, start, ctx, masks, heads)
+
+
+@pytest.mark.parametrize("cache", ["i8", "e4m3"])
+@pytest.mark.parametrize("scale", [1e-33, 1e-25, 1e25, 1e34])
+@pytest.mark.parametrize("n", [1, 40])
+def test_attn_scales_at_the_ends(torch_gpu, cache, n, scale):
+    """All value scales tiny or huge: the bits are kept."""
+    torch = torch_gpu
+    c, start, rows, masks, q = _attn_case(torch, cache, 64, 4, 1, 64, [300], [n], False, 80)
+    c.tensors[4].mul_(scale / float(c.tensors[4].mean()))
+    _check_fine(torch, c, q, start, [300], masks, 4)
+
+
+@pytest.mark.parametrize("n", [1, 30])
+def test_attn_fp32_values_near_the_largest(torch_gpu, n):
+    """Values of an fp32 cache within a hundredth of the type's largest: no weight is more than 1, so sums are in range."""
+    torch = torch_gpu
+    c, start, rows, masks, q = _attn_case(torch, "f32", 64, 2, 2, 16, [100], [n], False, 101)
+    c.tensors[1].clamp_(-3, 3).mul_(1e36)
+    _check_fine(torch, c, q, start, [100], masks, 2)
