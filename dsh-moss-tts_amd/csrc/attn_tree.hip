@@ -21,8 +21,9 @@
 // row c of the j-th product.
 //
 // Arithmetic: fp16, int8 and e4m3 values are exact in the fp16 products; a 32-bit query (scaled by a
-// power of two to below 2) and the softmax weights go in as fp16 hi + lo, 22 bits, so results are as
-// good as 32-bit ones.  int8 / e4m3 scales multiply the scores and the weights; weights are kept in
+// power of two to below 2) and the softmax weights go in as fp16 hi + lo: 22 bits, but no finer than 2^-35 of the
+// largest (fp16's smallest step, with the largest near its range's end), which shows where nearly all the weight is
+// on keys whose values are 0.  int8 / e4m3 scales multiply the scores and the weights; weights are kept in
 // fp16's range by a power of two of each row's own, which falls as the row's largest weight times value scale
 // rises.  An fp32 cache runs on the fp32 matrix instructions.
 #include <algorithm>
@@ -38,8 +39,8 @@ typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 constexpr int kWaves = 4, kThreads = 64 * kWaves;
 constexpr int kMaxSplits = 64;
 constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.69314718055994531f;
-constexpr float kSlack = 8.0f;  // log 2 of how far below its place a row's largest weight may lie
-constexpr float kPlace = 15.0f;  // log 2 of that place in fp16's range
+constexpr float kSlack = 5.0f;  // log 2 of how far below its place a row's largest weight may lie
+constexpr float kPlace = 16.0f;  // log 2 of that place: what passes fp16's 65504 is left to lo
 constexpr float kLeast = -109.0f;  // log 2 of the least product of weight and value scale that is put there (2^(kPlace - kLeast) is a float)
 
 struct TreePlan {
@@ -74,11 +75,14 @@ __device__ __forceinline__ floatx4 mfma(float a, float b, floatx4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
 }
 
-// x as hi + lo halves, both towards zero: 22 bits
+// x as hi + lo halves, hi towards zero and lo to nearest: off by half of 2^-21 of it, or of 2^-24 where that is more
 __device__ __forceinline__ void split2(float a, float b, uint32_t &hi, uint32_t &lo) {
     const auto h = __builtin_amdgcn_cvt_pkrtz(a, b);
     hi = __builtin_bit_cast(uint32_t, h);
-    lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(fmaf((float)h[0], -1.0f, a), fmaf((float)h[1], -1.0f, b)));
+    float x = fmaf((float)h[0], -1.0f, a), y = fmaf((float)h[1], -1.0f, b);
+    asm("" : "+v"(x), "+v"(y));  // (as fma_mixlo and fma_mixhi these are 5 % of the kernel for many rows)
+    const h2 l = {(_Float16)x, (_Float16)y};
+    lo = __builtin_bit_cast(uint32_t, l);
 }
 
 // A lane's share of 32 keys x D of one head, as they lie in memory: of K the A operand of S^T (key

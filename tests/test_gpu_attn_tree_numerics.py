@@ -69,7 +69,7 @@ def _fine_ref(q, c, start, ctx, mask, scale, heads, exact_products=False):
 
     A score is off by 24 roundings of scale * sum |q k| (none where the products are exact), a weight by 4 roundings of the
     scores it is the difference of, exp2's and the weight's own 2^-22 (with the value scale's product 2^-21); sums chain
-    keys / 16 + 64 roundings.  Below its 22 bits a weight (times its value scale) has a step: it is off by up to 2^-29 of the
+    keys / 16 + 64 roundings.  Below its 22 bits a weight (times its value scale) has a step: it is off by up to 2^-35 of the
     row's largest."""
     rows = len(q)
     out, tol = np.zeros((rows, heads, c.head_dim)), np.zeros((rows, heads, c.head_dim))
@@ -97,7 +97,7 @@ def _fine_ref(q, c, start, ctx, mask, scale, heads, exact_products=False):
                 chain = (n / 16 + 64) * U32
                 norm = (p * err).sum() + chain
                 out[r, h] = (p * d) @ u
-                tol[r, h] = ((err + norm + chain) * w) @ np.abs(u) + 2.0 ** -29 * w.max() * np.abs(u).sum(0) + 2 * U32 * np.abs(out[r, h])
+                tol[r, h] = ((err + norm + chain) * w) @ np.abs(u) + 2.0 ** -35 * w.max() * np.abs(u).sum(0) + 2 * U32 * np.abs(out[r, h])
                 lse[r, h] = x.max() + np.log(e.sum())
                 ltol[r, h] = norm + 4 * U32 * (np.abs(lse[r, h]) + np.abs(x.max()))
     return out, lse, tol, ltol
@@ -160,6 +160,40 @@ def test_attn_scales_at_the_ends(torch_gpu, cache, n, scale):
     c, start, rows, masks, q = _attn_case(torch, cache, 64, 4, 1, 64, [300], [n], False, 80)
     c.tensors[4].mul_(scale / float(c.tensors[4].mean()))
     _check_fine(torch, c, q, start, [300], masks, 4)
+
+
+@pytest.mark.parametrize("cache", ["f16", "i8", "e4m3", "f32"])
+@pytest.mark.parametrize("ctx,heads,n", [(541, 2, 1), (541, 2, 20), (541, 2, 40), (4096, 2, 1), (4096, 3, 64)])
+@pytest.mark.parametrize("gap", [8.0, 11.0, 14.0, 17.0])
+def test_attn_sink(torch_gpu, cache, ctx, heads, n, gap):
+    """A first key that takes nearly all the weight and has values of zero: the output is made of the small weights, e^-gap
+    of the largest each, with values of one sign.  Queries with one element, so that the scores' products are exact."""
+    torch = torch_gpu
+    print(f"attn sink {cache} ctx {ctx} rows {n * heads} gap {gap}", flush=True)
+    rng = np.random.default_rng(ctx + n)
+    total = ctx + n
+    c = _make_cache(torch, cache, 1, total, 1, 64, 64)
+    k = rng.integers(-100, 100, (total, 64)).astype(np.float32)
+    k[:, 0] = rng.integers(0, 5, total)
+    k[0, 0] = 112
+    v = rng.integers(64, 128, (total, 64)).astype(np.float32)
+    if cache == "e4m3":
+        k, v = torch.from_numpy(k).to(torch.float8_e4m3fn).float().numpy(), torch.from_numpy(v).to(torch.float8_e4m3fn).float().numpy()
+    v[0] = 0
+    table = c.tensors[2].cpu().numpy()[0]
+    at = (torch.from_numpy(table[np.arange(total) // 64].astype(np.int64)), 0, torch.arange(total) % 64)
+    for pool, x in ((c.tensors[0], k), (c.tensors[1], v)):
+        host = pool.float().cpu()
+        host[at] = torch.from_numpy(x)
+        pool.copy_(host.to(pool.dtype))
+    if cache in ("i8", "e4m3"):
+        c.tensors[3].fill_(2.0 ** -4)
+        c.tensors[4].fill_(2.0 ** -6)
+    q = torch.zeros(n, heads, 64)
+    q[..., 0] = 2.0 ** -8
+    scale = gap / (112 * 2.0 ** -8 * (2.0 ** -4 if cache in ("i8", "e4m3") else 1))
+    start = np.array([0, n], np.int32)
+    _check_fine(torch, c, q, start, [ctx], None, heads, exact_products=True, scale=float(np.float32(scale)))
 
 
 @pytest.mark.parametrize("n", [1, 30])
