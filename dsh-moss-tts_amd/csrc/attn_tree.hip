@@ -385,7 +385,8 @@ __device__ __forceinline__ bool visible(const Stream &st, uint64_t bits, int pos
 }
 
 // Softmax state of a lane's rows, one per tile: l = sum w, o = sum w v with weights w = 2^(x - ref) of the scores x so far,
-// l of this lane's keys only.  ref is a whole number, so scaling by its changes is exact; no score passes it by more
+// l of this lane's keys only, summed span by span with what each addition rounds off kept in `lost` (a wave can have 4096
+// spans, and equal weights round the same way each time: 2e-4 where they were added one by one).  ref is a whole number, so scaling by its changes is exact; no score passes it by more
 // than 1/2, and the largest is at most kSlack + 1/2 below it: it moves (and o and l are scaled) only when a score passes it,
 // which after the first spans is rare, where the largest itself still moves in every other span for some row of a tile.
 // For the fp16 products the weights are multiplied by 2^kPlace; with value scales (SCALED) a weight times its scale
@@ -394,7 +395,7 @@ __device__ __forceinline__ bool visible(const Stream &st, uint64_t bits, int pos
 template <int MT, int ND, bool SCALED, bool F32>
 struct Rows {
     static constexpr float kUp = F32 || SCALED ? 0.0f : kPlace;  // log 2 of what w itself is multiplied by
-    float ref[MT], l[MT];
+    float ref[MT], l[MT], lost[MT];
     float top[SCALED ? MT : 1], g[SCALED ? MT : 1];  // g = 2^(kPlace - top)
     floatx4 o[MT][ND];
 
@@ -402,7 +403,7 @@ struct Rows {
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
             ref[mt] = -INFINITY;
-            l[mt] = 0.0f;
+            l[mt] = lost[mt] = 0.0f;
             if constexpr (SCALED) {
                 top[mt] = kLeast;
                 g[mt] = exp2_(kPlace - kLeast);
@@ -412,7 +413,7 @@ struct Rows {
         }
     }
     __device__ __forceinline__ void settle(int mt) {
-        if constexpr (!SCALED) l[mt] *= exp2_(-kUp);
+        l[mt] = (l[mt] - lost[mt]) * exp2_(-kUp);
 #pragma unroll
         for (int j = 0; j < ND; ++j)
 #pragma unroll
@@ -429,8 +430,9 @@ struct Rows {
             const bool up = mx > ref[mt];
             const float r = up ? rintf(mx) + kSlack : ref[mt], by = up ? ref[mt] - r : 0.0f;
             ref[mt] = r;
-            l[mt] *= exp2_(by);
             float fade = exp2_(by);
+            l[mt] *= fade;
+            lost[mt] *= fade;
             if constexpr (SCALED) {  // top stays where it was, unless it would fall under kLeast
                 const float t = fmaxf(top[mt] + by, kLeast);
                 fade = exp2_(top[mt] + by - t);
@@ -444,10 +446,11 @@ struct Rows {
 #pragma unroll
         for (int b = 0; b < 2; ++b)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                x[b][i] = exp2_(fmaf(x[b][i], qs, kUp - r0));
-                l[mt] += x[b][i];
-            }
+            for (int i = 0; i < 4; ++i) x[b][i] = exp2_(fmaf(x[b][i], qs, kUp - r0));
+        const float add = (((x[0][0] + x[0][1]) + (x[0][2] + x[0][3])) + ((x[1][0] + x[1][1]) + (x[1][2] + x[1][3]))) - lost[mt];
+        const float sum = l[mt] + add;
+        lost[mt] = (sum - l[mt]) - add;
+        l[mt] = sum;
         return mx - r0;
     }
     // Weights times value scales, 0 where the row does not see the key, are put in place: `most` is what weigh returned and
