@@ -545,6 +545,11 @@ __device__ __forceinline__ void put_cut(const TreeArgs &a, const TreePlan &plan,
     if (plan.slots > a.c.streams && slot == cut.first && h == 0 && rg == 0 && threadIdx.x == 0)
         *((int4 *)a.ws + cut.stream) = make_int4(cut.first, cut.pieces, 0, 0);
 }
+// Whether a row attends anything.
+__device__ __forceinline__ bool sees_any(const TreeArgs &a, const Stream &st, int node) {
+    const uint64_t m = a.row_mask != nullptr ? a.row_mask[st.row0 + node] : 1;
+    return st.ctx > 0 || (m << (64 - st.n)) != 0;
+}
 // N elements from d0 on of packed row i, normalised, or, where the keys are cut, as they are with the
 // row's maximum and sum (a lane of d0 = 0 writes those) for the slot.
 template <int D, int N>
@@ -561,6 +566,7 @@ __device__ __forceinline__ void put_row(const TreeArgs &a, const TreePlan &plan,
         return;
     }
     const size_t at = (size_t)(st.row0 + node) * a.heads + head;
+    if (L == 0.0f && sees_any(a, st, node)) L = __uint_as_float(0x7fc00000u);  // (no score above -inf: 0 / 0, not a row that sees nothing)
     const float inv = L == 0.0f ? 0.0f : 1.0f / L;
     const size_t o = (size_t)((int64_t)(st.row0 + node) * a.out_row + head * D + d0);
     if (a.out_dtype == ELEM_F16) {

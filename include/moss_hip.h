@@ -435,14 +435,15 @@ int moss_hip_kv_read(const moss_hip_kv_cache *cache, const int32_t *row_stream, 
  *   q: [rows][heads][head_dim] of q_dtype (F32 or F16), rotated; out the same shape in out_dtype; row
  *   strides in elements, out q itself (same type and stride) or apart from it.  lse [rows][heads] fp32 or
  *   NULL: the log of each row's sum of exp(score).  The streams' row ranges lie apart.
- * A row that attends nothing is 0 with lse -inf.  What a row does not attend may hold anything, Inf and NaN
- * too.  max_keys bounds every stream's ctx_len + n and sizes the launch.  A stream whose ctx_len is
- * negative, whose keys pass max_keys or its table, or with a page outside [0, n_pages) among them, gets
- * NaN rows; one whose row range is not within [0, rows] gets none.  Rows of no stream, and a stream's rows past
- * max_rows, stay as they were.  Scores, sums and statistics are held in 32 bits and out is
- * rounded once.  A weight (times its key's value scale) goes into the products with 22 bits, but is off by up to 2^-35 of
- * the row's largest: that is more than 2^-22 of itself for weights under 2^-13 of the largest.  The same call gives the same bits.  workspace:
- * moss_hip_attn_tree_workspace bytes (any content, 16-byte aligned; NULL where that is 0). */
+ * A row that attends nothing is 0 with lse -inf; one that attends keys, but none with a score above -inf, is NaN, and so
+ * is one with an Inf or NaN in its query.  What a row does not attend may hold anything, Inf and NaN too.  max_keys
+ * bounds every stream's ctx_len + n and sizes the launch.  A stream whose ctx_len is negative, whose keys pass max_keys or
+ * its table, or with a page outside [0, n_pages) among them, gets NaN rows; one whose row range is not within [0, rows]
+ * gets none.  Rows of no stream, and a stream's rows past max_rows, stay as they were.  Scores, sums and statistics are
+ * held in 32 bits and out is rounded once.  A weight (times its key's value scale) goes into the products with 22 bits,
+ * but is off by up to 2^-35 of the row's largest: that is more than 2^-22 of itself for weights under 2^-13 of the largest.
+ * The same call gives the same bits.  workspace: moss_hip_attn_tree_workspace bytes (any content, 16-byte aligned; NULL
+ * where that is 0). */
 int moss_hip_attn_tree(const void *q, int64_t q_stride, int q_dtype, int heads, const moss_hip_kv_cache *cache,
                        const int32_t *row_start, const int32_t *ctx_len, const uint64_t *row_mask, int rows, int max_rows,
                        int max_keys, float scale, void *out, int64_t out_stride, int out_dtype, float *lse, void *workspace,

@@ -232,3 +232,31 @@ def test_attn_long_sums(torch_gpu, cache, streams, heads, kvh, most):
     want = 0.125 * q[..., 0].double().numpy() + math.log(ctx + 1)
     assert (np.abs(lse - want) <= 72 * U32 + 4 * U32 * (np.abs(want) + 0.5)).all(), np.max(np.abs(lse - want)) / U32
     assert (np.abs(got - 1) <= 2 * (ctx / 16 + 64) * U32).all()
+
+
+# ---------------------------------------------------------------- what is not finite, and what is far out
+
+@pytest.mark.parametrize("cache", ["f16", "i8", "e4m3", "f32"])
+@pytest.mark.parametrize("qdt", ["f32", "f16"])
+@pytest.mark.parametrize("n", [1, 2, 40])
+def test_attn_inf_queries_over_few_keys(torch_gpu, cache, qdt, n):
+    """An Inf or NaN in a query makes its head NaN also where one key is all it sees (its products may then all be -Inf), and
+    one that sees nothing is 0 all the same."""
+    torch = torch_gpu
+    print(f"attn inf queries {cache} {qdt} {n}", flush=True)
+    ctx = [0, 1, 2, 0]
+    c, start, rows, masks, q = _attn_case(torch, cache, 64, 8, 2, 16, ctx, [n] * 4, False, 90 + n, qdt=qdt)
+    masks = [1 << (r % n) for r in range(rows)]
+    for r in range(3 * n, rows):
+        masks[r] = 0
+    clean, cl = _run_attn(torch, c, q, start, ctx, masks, n, n + 2)
+    odd, bad = q.clone(), np.zeros((rows, 8), bool)
+    for i in range(8 * rows):
+        r, h = divmod(i, 8)
+        if i % 3:
+            odd[r, h, (7 * i) % 64] = (math.inf, -math.inf, math.nan)[i // 3 % 3]
+            bad[r, h] = r < 3 * n
+    got, lse = _run_attn(torch, c, odd, start, ctx, masks, n, n + 2)
+    assert np.isnan(got[bad]).all() and np.isnan(lse[bad]).all()
+    assert np.array_equal(got[~bad], clean[~bad]) and np.array_equal(lse[~bad], cl[~bad])
+    assert (got[3 * n:] == 0).all() and (lse[3 * n:] == -np.inf).all()
