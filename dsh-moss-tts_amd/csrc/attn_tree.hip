@@ -1115,6 +1115,11 @@ TreePlan plan_of(const KvCacheArgs &c, int heads, int max_rows, int max_keys) {
         p.waves = 2 * kWaves;
         splits = 1;
     }
+    // The matrix instructions cut what they add towards zero, so a sum of one sign falls short by about 2^-25 for each (1.6e-4
+    // and, of equal weights, 4.8e-4 over 131072 keys of a wide workgroup).  No wave gets more than 1024 in a row: two for 32
+    // keys, or eight in fp32; the wide workgroup's waves see every key, the others a fourth.
+    const int most = p.group > 2 || c.dtype == ELEM_F32 ? 16384 : 65536;
+    splits = std::max(splits, std::min((max_keys + most - 1) / most, kMaxSplits));
     p.chunk = ((max_keys + splits - 1) / splits + 127) / 128 * 128;
     p.slots = splits * c.streams;
     // blk / (page_size / 16) for blk < 2^24 and a divisor up to 2^11: 2^40 / d rounded up is off by

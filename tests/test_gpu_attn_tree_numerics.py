@@ -207,10 +207,11 @@ def test_attn_fp32_values_near_the_largest(torch_gpu, n):
 
 # ---------------------------------------------------------------- long sums
 
-@pytest.mark.parametrize("cache,streams,heads,kvh,most", [("i8", 17, 16, 8, 40), ("f16", 17, 16, 8, 40), ("e4m3", 97, 8, 8, 1), ("f16", 97, 8, 8, 1)])
+@pytest.mark.parametrize("cache,streams,heads,kvh,most", [("i8", 17, 16, 8, 40), ("f16", 17, 16, 8, 40), ("e4m3", 97, 8, 8, 1), ("f16", 97, 8, 8, 1), ("f32", 97, 8, 8, 1)])
 def test_attn_long_sums(torch_gpu, cache, streams, heads, kvh, most):
-    """131072 equal weights that no cut shares out (so many streams and heads there are): the normaliser does not drift.
-    lse is the score plus log 131073 within 72 roundings of the sum, and those of the result's own size."""
+    """131072 equal weights under so many streams and heads that nothing is cut to fill the chip: neither sum drifts.  lse is
+    the score plus log 131073 within 72 roundings of the sum, and those of the result's own size.  The values' sum is a chain
+    of up to 1024 products' results, each cut by up to 2^-23 of the sum so far (2^-24 of the whole on average), and 64 roundings."""
     torch = torch_gpu
     print(f"attn long sums {cache} {streams} {heads}/{kvh}", flush=True)
     ctx, page = 131072, 1024
@@ -224,14 +225,13 @@ def test_attn_long_sums(torch_gpu, cache, streams, heads, kvh, most):
     n = [most] + [1] * (streams - 1)
     start = np.concatenate([[0], np.cumsum(n)]).astype(np.int32)
     rows = int(start[-1])
-    assert lib.attn_tree_workspace(c, heads, rows, most, ctx + most) == 0
     q = torch.zeros(rows, heads, 64)
     q[..., 0] = 8 * torch.rand(rows, heads, generator=torch.Generator().manual_seed(1)) - 4
     masks = [1 << (r if r < most else 0) for r in range(rows)]  # itself
     got, lse = _run_attn(torch, c, q, start, [ctx] * streams, masks, most, ctx + most)
     want = 0.125 * q[..., 0].double().numpy() + math.log(ctx + 1)
     assert (np.abs(lse - want) <= 72 * U32 + 4 * U32 * (np.abs(want) + 0.5)).all(), np.max(np.abs(lse - want)) / U32
-    assert (np.abs(got - 1) <= 2 * (ctx / 16 + 64) * U32).all()
+    assert (np.abs(got - 1) <= (1024 + 64 + 72) * U32).all(), np.max(np.abs(got - 1)) / U32
 
 
 # ---------------------------------------------------------------- what is not finite, and what is far out
