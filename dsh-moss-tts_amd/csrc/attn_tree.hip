@@ -41,6 +41,7 @@ constexpr int kMaxSplits = 64;
 constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.69314718055994531f;
 constexpr float kSlack = 5.0f;  // log 2 of how far below its place a row's largest weight may lie
 constexpr float kPlace = 16.0f;  // log 2 of that place: what passes fp16's 65504 is left to lo
+constexpr float kFar = 16384.0f;  // scores past it are rounded before ref is taken off: past 2^31 a product's last bits alone can leave exp2's range
 constexpr float kLeast = -109.0f;  // log 2 of the least product of weight and value scale that is put there (2^(kPlace - kLeast) is a float)
 
 struct TreePlan {
@@ -443,10 +444,22 @@ struct Rows {
             for (int j = 0; j < ND; ++j) o[mt][j] *= fade;
         }
         const float r0 = ref[mt] == -INFINITY ? 0.0f : ref[mt];
+        const bool far = fabsf(mx) > kFar && fabsf(mx) < INFINITY;
+        if (__any(far)) {
+#pragma clang fp contract(off)  // rounded as mx was
 #pragma unroll
-        for (int b = 0; b < 2; ++b)
+            for (int b = 0; b < 2; ++b)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x[b][i] = exp2_(fmaf(x[b][i], qs, kUp - r0));
+                for (int i = 0; i < 4; ++i) {
+                    const float z = x[b][i] * qs;
+                    x[b][i] = exp2_(far ? (z - r0) + kUp : fmaf(x[b][i], qs, kUp - r0));
+                }
+        } else {
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[b][i] = exp2_(fmaf(x[b][i], qs, kUp - r0));
+        }
         const float add = (((x[0][0] + x[0][1]) + (x[0][2] + x[0][3])) + ((x[1][0] + x[1][1]) + (x[1][2] + x[1][3]))) - lost[mt];
         const float sum = l[mt] + add;
         lost[mt] = (sum - l[mt]) - add;

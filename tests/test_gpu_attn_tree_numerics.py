@@ -260,3 +260,36 @@ def test_attn_inf_queries_over_few_keys(torch_gpu, cache, qdt, n):
     assert np.isnan(got[bad]).all() and np.isnan(lse[bad]).all()
     assert np.array_equal(got[~bad], clean[~bad]) and np.array_equal(lse[~bad], cl[~bad])
     assert (got[3 * n:] == 0).all() and (lse[3 * n:] == -np.inf).all()
+
+
+@pytest.mark.parametrize("cache", ["f16", "i8", "e4m3", "f32"])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+@pytest.mark.parametrize("n", [1, 40])
+def test_attn_scores_past_whole_numbers(torch_gpu, cache, sign, n):
+    """Scores of 1e10, whose last bits are worth hundreds: the keys of the largest take all the weight, two equal ones
+    half each, and rows with ordinary scores beside them do not change by a bit."""
+    torch = torch_gpu
+    print(f"attn far scores {cache} {sign} {n}", flush=True)
+    ctx = [70]
+    c, start, rows, masks, q = _attn_case(torch, cache, 64, 4, 1, 16, ctx, [n], False, 100)
+    step, scale = {"f16": (2000.0, 1.0), "f32": (2000.0, 1.0), "i8": (2.0, 60000.0), "e4m3": (16.0, 300.0)}[cache]
+    for p in range(ctx[0] + n):  # of 17 sizes, each several times
+        _put(c, 0, [p], k=(1.0 + p % 17) * step, ks=scale)
+    q *= 1e-5
+    clean, cl = _run_attn(torch, c, q, start, ctx, masks, n, ctx[0] + n)
+    far = q.clone()
+    far[:, 1] = sign * 60000.0
+    far[:, 2] = sign * 30000.0
+    got, lse = _run_attn(torch, c, far, start, ctx, masks, n, ctx[0] + n)
+    assert np.array_equal(got[:, [0, 3]], clean[:, [0, 3]]) and np.array_equal(lse[:, [0, 3]], cl[:, [0, 3]])
+    (kr, ks), (v, vs) = _raw(c, 0, 0, ctx[0] + n), _raw(c, 1, 0, ctx[0] + n)
+    key, val = kr[0, :, 0] * ks[0], v[0] * vs[0][:, None]
+    for r in range(n):
+        see = np.array([j < ctx[0] or (masks[r] >> (j - ctx[0])) & 1 for j in range(ctx[0] + n)], bool)
+        for h in (1, 2):
+            score = 0.125 * 64 * float(far[r, h, 0]) * key
+            assert abs(score).max() > 2.0 ** 33 or h == 2
+            top = see & (score == score[see].max())
+            want = val[top].mean(0)
+            assert (np.abs(got[r, h] - want) <= 64 * U32 * np.abs(val[top]).mean(0) + 1e-30).all(), (r, h, got[r, h][:3], want[:3])
+            assert abs(lse[r, h] - score[top][0]) <= 16 * U32 * abs(score[top][0])
