@@ -3,7 +3,8 @@
 //
 // Of a row: with m = max x, z = (x - m) / T, S = sum e^z and U = sum e^z z,
 //   log p(t) = z_t - log S,     entropy = -sum p log p = log S - U / S,
-// the differences first, so that a row of the type's lowest value does not leave its range when it is scaled;
+// the differences first, so that a row of the type's lowest value does not leave its range when it is scaled, and as half
+// of themselves (z / 2 = (x / 2 - m / 2) / T, exact but for subnormal x), so that those of the type's two ends do not either;
 // and the k largest x, of equal values the lowest index first.  One pass: a workgroup takes a
 // chunk of a row into registers, so memory is read once; m, S, U and the alternatives all come
 // from there.  A row of more than one chunk leaves (m, S, U) and its k best per chunk in the
@@ -169,6 +170,8 @@ struct Sums {
     float m, s, u;
 };
 
+__device__ __forceinline__ float half_diff(float x, float m) { return fmaf(x, 0.5f, -0.5f * m); }
+
 // m, S and U of a chunk, and the first half of its k best; -inf contributes nothing, NaN and +inf make the
 // sums NaN.
 template <int EPT, int CAP>
@@ -186,8 +189,8 @@ __device__ __forceinline__ Sums sums_of(const float (&x)[EPT], float inv_t, int 
     float s = 0.0f, u = 0.0f;
 #pragma unroll
     for (int i = 0; i < EPT; ++i) {
-        const float z = (x[i] - m0) * inv_t;
-        const float e = __builtin_amdgcn_exp2f(z * 1.44269504088896341f);
+        const float z = half_diff(x[i], m0) * inv_t;
+        const float e = __builtin_amdgcn_exp2f(z * (2.0f * 1.44269504088896341f));
         s += e;
         u += e == 0.0f ? 0.0f : e * z;
     }
@@ -205,6 +208,7 @@ __device__ __forceinline__ Sums sums_of(const float (&x)[EPT], float inv_t, int 
         q.s += red[1][v];
         q.u += red[2][v];
     }
+    q.u *= 2.0f;
     return q;
 }
 
@@ -226,11 +230,11 @@ __device__ __forceinline__ float token_logit(const LogprobArgs &a, int r) {
 // probability of an alternative.
 __device__ __forceinline__ void finish_row(const LogprobArgs &a, int r, float x, const Sums &q) {
     const float log_s = logf(q.s);
-    a.logprob[r] = q.s == 0.0f && x == x ? -INFINITY : (x - q.m) * a.inv_t - log_s;  // (sum 0: no token is allowed at all)
+    a.logprob[r] = q.s == 0.0f && x == x ? -INFINITY : 2.0f * (half_diff(x, q.m) * a.inv_t) - log_s;  // (sum 0: no token is allowed at all)
     if (a.entropy != nullptr) a.entropy[r] = q.s == 0.0f ? 0.0f : log_s - q.u / q.s;
 }
 __device__ __forceinline__ float alt_lp(const LogprobArgs &a, const Sums &q, uint32_t key) {
-    return (of_key(key) - q.m) * a.inv_t - logf(q.s);
+    return 2.0f * (half_diff(of_key(key), q.m) * a.inv_t) - logf(q.s);
 }
 __device__ __forceinline__ void no_alternatives(const LogprobArgs &a, int r, int from) {
     for (int i = from + (int)threadIdx.x; i < a.top_k; i += kThreads) {
@@ -313,7 +317,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_join_kernel(LogprobArgs a, 
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         if (part[i].x == -INFINITY && part[i].y == 0.0f) continue;  // nothing allowed in this chunk
-        const float d = (part[i].x - q.m) * a.inv_t, f = __builtin_amdgcn_exp2f(d * 1.44269504088896341f);
+        const float d = 2.0f * (half_diff(part[i].x, q.m) * a.inv_t), f = __builtin_amdgcn_exp2f(d * 1.44269504088896341f);
         q.s += f * part[i].y;
         q.u += f == 0.0f ? 0.0f : f * (part[i].z + part[i].y * d);
     }
