@@ -353,13 +353,20 @@ class Rope:
     """A rotation a program keeps: its angles per position on the device (moss_hip_rope).
 
     Rope(rot_dim, ...) takes the arguments of rope_freqs; Rope(freqs=tensor) takes float64 angles of the
-    caller's own.  halves: pairs (i, i + rot_dim / 2) rather than (2i, 2i + 1)."""
+    caller's own, where they are, and no scaling.  halves: pairs (i, i + rot_dim / 2) rather than (2i, 2i + 1);
+    mscale: the factor of sine and cosine, by default what the scaling asks for."""
 
-    def __init__(self, rot_dim: int = 64, halves: bool = False, freqs=None, mscale: float = 1.0, device=None, **scaling):
+    def __init__(self, rot_dim: int | None = None, halves: bool = False, freqs=None, mscale: float | None = None, device=None, **scaling):
         import torch
         if freqs is None:
-            f, mscale = rope_freqs(rot_dim, **scaling)
+            f, m = rope_freqs(64 if rot_dim is None else rot_dim, **scaling)
             freqs = torch.from_numpy(f).to("cuda" if device is None else device)
+            mscale = m if mscale is None else mscale
+        elif scaling or rot_dim not in (None, 2 * freqs.numel()):
+            raise ValueError("freqs say the angles and their number: no scaling or other rot_dim besides")
+        elif device is not None and torch.empty(0, device=device).device != freqs.device:
+            raise ValueError(f"freqs are on {freqs.device}, not {device}")
+        mscale = 1.0 if mscale is None else mscale
         self.freqs, self.device = freqs, freqs.get_device()
         _whole("freqs", freqs, torch.float64, (freqs.numel(),), self.device)
         self.struct = RopeStruct(freqs.data_ptr(), 2 * freqs.numel(), int(halves), mscale)

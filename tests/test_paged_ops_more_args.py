@@ -1,0 +1,24 @@
+"""More of the decoding-loop operators' checks of their arguments, without a GPU."""
+import math
+
+import pytest
+
+from mosship import lib
+
+
+def test_rope_takes_mscale_as_given():
+    """With frequencies of the library's own it is used too, and what frequencies given already say is refused besides them."""
+    import torch
+    assert lib.Rope(64, device="cpu").struct.mscale == 1.0
+    assert lib.Rope(64, mscale=0.5, device="cpu").struct.mscale == 0.5
+    yarn = dict(scaling="yarn", factor=16.0, orig_ctx=4096, device="cpu")
+    assert abs(lib.Rope(64, **yarn).struct.mscale - (0.1 * math.log(16.0) + 1.0)) < 2.0 ** -22
+    assert lib.Rope(64, mscale=2.0, **yarn).struct.mscale == 2.0
+    f = torch.ones(24, dtype=torch.float64)
+    own = lib.Rope(freqs=f, halves=True)
+    assert (own.struct.rot_dim, own.struct.mscale, own.struct.halves) == (48, 1.0, 1)
+    assert lib.Rope(48, freqs=f, mscale=0.5).struct.mscale == 0.5
+    assert lib.Rope(freqs=f, device="cpu").device == -1
+    for kw in (dict(rot_dim=64), dict(scaling="linear", factor=2.0), dict(device="meta")):
+        with pytest.raises(ValueError, match="freqs"):
+            lib.Rope(freqs=f, **kw)
