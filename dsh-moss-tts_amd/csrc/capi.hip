@@ -808,6 +808,8 @@ int moss_hip_attn_tree(const void *q, int64_t q_stride, int q_dtype, int heads, 
         const int64_t width = (int64_t)heads * a.c.dim;
         check_strides({q_stride, out_stride});
         if (rows > 1 && out_stride < width) throw Status(MOSS_HIP_EINVAL, "rows of out must not overlap");
+        if (q == out && (q_dtype != out_dtype || (rows > 1 && q_stride != out_stride)))
+            throw Status(MOSS_HIP_EINVAL, "in place, q and out must have the same type and stride");
         if (!std::isfinite(scale)) throw Status(MOSS_HIP_EINVAL, "scale must be finite");
         if (rows == 0 || a.c.streams == 0) return;
         check_workspace(workspace, workspace_bytes, mh::tree_workspace(a.c, heads, rows, max_rows, max_keys), "moss_hip_attn_tree");

@@ -1,9 +1,11 @@
 """More of the decoding-loop operators' checks of their arguments, without a GPU."""
+import ctypes as C
 import math
 
 import pytest
 
 from mosship import lib
+from test_paged_ops_args import P, _cache, _refused
 
 
 def test_rope_takes_mscale_as_given():
@@ -22,3 +24,11 @@ def test_rope_takes_mscale_as_given():
     for kw in (dict(rot_dim=64), dict(scaling="linear", factor=2.0), dict(device="meta")):
         with pytest.raises(ValueError, match="freqs"):
             lib.Rope(freqs=f, **kw)
+
+
+def test_attention_in_place_of_another_layout_is_refused():
+    """Over the query itself, with rows that would lie elsewhere than the query's: one row's output in another's query."""
+    L, c = lib.load(), _cache(streams=1)
+    for q_stride, qdt, o_stride, odt in ((1024, lib.F32, 2048, lib.F32), (1024, lib.F32, 1024, lib.F16), (1024, lib.F16, 1024, lib.F32)):
+        _refused(L.moss_hip_attn_tree(P, q_stride, qdt, 16, C.addressof(c), P, P, None, 4, 4, 256, 0.125, P, o_stride, odt, None, P,
+                                      1 << 30, None), "same type and stride")
