@@ -611,7 +611,7 @@ mh::KvCacheArgs cache_shape(const moss_hip_kv_cache *c) {
 
 mh::KvCacheArgs cache_args(const moss_hip_kv_cache *c) {
     mh::KvCacheArgs a = cache_shape(c);
-    if (!c->k || !c->v || !c->page_table) throw Status(MOSS_HIP_EINVAL, "cache: null pointer");
+    if (!c->k || !c->v || (!c->page_table && c->streams > 0)) throw Status(MOSS_HIP_EINVAL, "cache: null pointer");
     if (c->n_pages <= 0 || c->table_stride <= 0) throw Status(MOSS_HIP_EINVAL, "cache: need n_pages, table_stride > 0");
     const bool q8 = mh::quantised(c->kv_dtype);
     if (q8 != (c->k_scale != nullptr) || q8 != (c->v_scale != nullptr))

@@ -356,9 +356,10 @@ int moss_hip_attn_decode_noalloc(const float *q, const void *k_cache, const void
  * pointer of the device that is current at the call, and `stream` is a stream of that device.
  * Arrays read while a call's kernels run must not be changed meanwhile by work on other streams.  A
  * workspace belongs to one call at a time: calls (and replays of captured calls) that may overlap
- * need workspaces of their own.  Strides are 0 .. 2^40 elements.  Where rows, streams or top_k are 0 there is nothing to do and the
- * call returns OK.  What only the device can see (positions, page indices, row ranges) is checked
- * there and never followed out of range; each call says what becomes of such rows. */
+ * need workspaces of their own.  Strides are 0 .. 2^40 elements.  Without rows, or over a cache without streams (page_table
+ * may be NULL then), there is nothing to do and a call returns OK, but for moss_hip_kv_read, whose rows have no place then.
+ * What only the device can see (positions, page indices, row ranges) is checked there and never followed out of range; each
+ * call says what becomes of such rows. */
 
 enum {
     MOSS_HIP_ROPE_PLAIN = 0,  /* w_i = base^(-2i / rot_dim) */
@@ -406,7 +407,7 @@ typedef struct {
     int kv_heads, head_dim;   /* head_dim 64 or 128 */
     int page_size;            /* a multiple of 16, at most 32768 */
     int n_pages;
-    const int32_t *page_table; /* [streams][table_stride] */
+    const int32_t *page_table; /* [streams][table_stride]; NULL where streams is 0 */
     int table_stride, streams;
 } moss_hip_kv_cache;
 

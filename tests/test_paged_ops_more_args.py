@@ -32,3 +32,18 @@ def test_attention_in_place_of_another_layout_is_refused():
     for q_stride, qdt, o_stride, odt in ((1024, lib.F32, 2048, lib.F32), (1024, lib.F32, 1024, lib.F16), (1024, lib.F16, 1024, lib.F32)):
         _refused(L.moss_hip_attn_tree(P, q_stride, qdt, 16, C.addressof(c), P, P, None, 4, 4, 256, 0.125, P, o_stride, odt, None, P,
                                       1 << 30, None), "same type and stride")
+
+
+def test_a_cache_without_streams_has_no_table():
+    """An empty tensor's address is NULL: writing and attending are nothing to do, whatever the rows."""
+    import torch
+    pool = torch.zeros(4, 2, 16, 64)
+    c = lib.KVCache(pool, pool, torch.zeros(0, 4, dtype=torch.int32))
+    assert c.struct.page_table is None and c.streams == 0
+    L = lib.load()
+    assert L.moss_hip_kv_write(c.ref, P, 128, P, 128, lib.F32, 3, P, P, None, None, None) == lib.OK
+    assert L.moss_hip_kv_read(c.ref, P, P, 0, P, 128, P, 128, lib.F32, None) == lib.OK
+    assert L.moss_hip_attn_tree(P, 256, lib.F32, 4, c.ref, P, P, None, 2, 1, 64, 0.125, P, 256, lib.F32, None, None, 0, None) == lib.OK
+    assert lib.attn_tree_workspace(c, 4, 2, 1, 64) == 0
+    bad = _cache(page_table=None, streams=1)
+    _refused(L.moss_hip_kv_write(C.addressof(bad), P, 256, P, 256, lib.F32, 3, P, P, None, None, None), "null")
