@@ -1132,7 +1132,9 @@ TreePlan plan_of(const KvCacheArgs &c, int heads, int max_rows, int max_keys) {
     // and, of equal weights, 4.8e-4 over 131072 keys of a wide workgroup).  No wave gets more than 1024 in a row: two for 32
     // keys, or eight in fp32; the wide workgroup's waves see every key, the others a fourth.
     const int most = p.group > 2 || c.dtype == ELEM_F32 ? 16384 : 65536;
-    splits = std::max(splits, std::min((max_keys + most - 1) / most, kMaxSplits));
+    // That is as far as it goes with partial results of 2^20 rows (0.5 GB of 128 dims), and so with a grid that can be launched.
+    const int room_for = (int)std::max<long long>(1, (1 << 20) / ((long long)c.streams * max_rows * heads));
+    splits = std::max(splits, std::min({(max_keys + most - 1) / most, kMaxSplits, room_for}));
     p.chunk = ((max_keys + splits - 1) / splits + 127) / 128 * 128;
     p.slots = splits * c.streams;
     // blk / (page_size / 16) for blk < 2^24 and a divisor up to 2^11: 2^40 / d rounded up is off by

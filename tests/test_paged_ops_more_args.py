@@ -47,3 +47,15 @@ def test_a_cache_without_streams_has_no_table():
     assert lib.attn_tree_workspace(c, 4, 2, 1, 64) == 0
     bad = _cache(page_table=None, streams=1)
     _refused(L.moss_hip_kv_write(C.addressof(bad), P, 256, P, 256, lib.F32, 3, P, P, None, None, None), "null")
+
+
+@pytest.mark.parametrize("streams,heads,kvh,rows", [(65536, 64, 64, 1), (1024, 64, 8, 64), (4096, 16, 16, 64), (64, 32, 8, 64), (97, 8, 8, 1)])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_workspaces_of_far_bounds_stay_small(streams, heads, kvh, rows, dim):
+    """However many rows and far the bound: partial results of 2^20 rows at most, but for a batch so small that its keys are
+    cut to fill the chip (64 pieces of each stream)."""
+    c = _cache(kv_dtype=lib.I8, k_scale=P, v_scale=P, kv_heads=kvh, head_dim=dim, streams=streams)
+    n = C.c_size_t()
+    for keys in (1000, 16384, 65537, 131072, 1 << 20, 1 << 28):
+        assert lib.load().moss_hip_attn_tree_workspace(C.addressof(c), heads, streams * rows, rows, keys, C.byref(n)) == lib.OK
+        assert n.value <= (1 << 20) * (2 + dim) * 4 + 16 * streams + 8, (keys, n.value)
