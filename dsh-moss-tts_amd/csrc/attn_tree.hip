@@ -609,10 +609,10 @@ __device__ __forceinline__ void put_row(const TreeArgs &a, const TreePlan &plan,
 // Few rows (up to 4 tiles, 2 of a workgroup): memory bound.  Each of the W = 4 or 8 waves takes every W-th span of 32 keys,
 // the next span's loads in flight while one is worked on, and the waves are joined through LDS.
 // LO: 32-bit queries, as hi + lo.
-// One row over 130001 e4m3 keys of 8 x 128, 32 heads: 51.8 us and 4.9 of the join, 5.3 TB/s.  64 streams of 270 to 541
-// int8 keys of 12 x 64: 15.5 us; 16 trees of 14 to 27 over 507 to 1015 fp16 keys of 12 x 64, by 8 waves: 15.6.  The last two
-// are short of it by their chain of dependent loads (row range, page, keys, then 4 or 5 spans a wave) and by vector work,
-// about 300 instructions a span.
+// One row over 130001 e4m3 keys of 8 x 128, 32 heads: 51.7 us and 4.8 of the join, 5.3 TB/s.  64 streams of 270 to 541
+// int8 keys of 12 x 64: 16.1 us; 16 trees of 14 to 27 over 507 to 1015 fp16 keys of 12 x 64, by 8 waves: 15.8.  The last two
+// are short of it by their chain of dependent loads (row range, page, keys, then 4 or 5 spans a wave), by the longest of
+// the streams, which are not cut there, and by vector work, about 310 instructions a span.
 template <int KV, int D, int MT, bool LO, int W>
 __global__ __launch_bounds__(64 * W, W > kWaves ? 2 : KV == ELEM_F32 ? (D == 64 ? 2 : 1) : (D == 64 && MT == 1 ? 3 : 2)) void attn_tree_kernel(TreeArgs a, TreePlan plan) {
     constexpr bool F32 = KV == ELEM_F32, SCALED = quantised(KV);
@@ -821,15 +821,15 @@ __global__ __launch_bounds__(64 * W, W > kWaves ? 2 : KV == ELEM_F32 ? (D == 64 
 
 // Many rows (more than 64): bound by the matrix and vector units.  Every wave has MT row tiles of its own and all
 // of them the same keys, which they prepare together: of a stage of 16 keys a wave each turns its block into
-// fragments, K and V, and puts them into LDS in the order in which the products read them (16 bytes a lane, no
-// bank conflicts), so a key is converted once for up to 256 rows.  Two stages: while one is worked on the next
+// fragments, K and V, and puts them into LDS in the order in which the products read them (16 bytes a lane, without
+// bank conflicts; the few that are counted are likely V's stores, 8 bytes at a stride of 16), so a key is converted once for up to 256 rows.  Two stages: while one is worked on the next
 // one's loads are in flight, and it is written before the only barrier of a stage.
 // LO: 32-bit queries, as hi + lo; the weights are hi + lo whatever the output's type is.
-// 8 streams with trees of 33 to 64, 32 heads of 128 on 8 key heads, 8192 to 16384 int8 keys: 162 to 175 us from run to
-// run, and 9.3 of the join.
-// The vector unit is what is busy most: 72 us of the softmax (a score: scale, maximum, exponential of 4 slots, sum, value
-// scale, packing) and the conversions, 33 of the matrix unit, and little of the one falls under the other with two
-// waves to a SIMD.  Tried when it took 172: products of the next span issued ahead of the weights of one, 182; the row
+// 8 streams with trees of 33 to 64, 32 heads of 128 on 8 key heads, 8192 to 16384 int8 keys: 185 to 214 us from run to
+// run, and 9.5 of the join.
+// The vector unit is what is busy most: 218 thousand cycles of the softmax (a score: scale, maximum, exponential of 4 slots,
+// sum, value scale, packing) and the conversions, 117 of the matrix unit, of 394 that a wave lives: little of the one falls
+// under the other with two waves to a SIMD.  Tried when it took 172, with weights of 11 bits: products of the next span issued ahead of the weights of one, 182; the row
 // tiles dealt to the waves in turn, so that none is idle where rows are fewer than 256, 184, as each then reads all
 // fragments for half the rows.
 template <int KV, int D, int NWV>
@@ -1097,8 +1097,8 @@ __global__ __launch_bounds__(kThreads) void attn_tree_join_kernel(TreeArgs a, Tr
 
 // Rows of 16 of a workgroup: 1 or 2 in the kernel for few rows, 8 or 16 in the wide one.  With 3 and 4 tiles the keys are
 // read twice by the one and still sooner done (16 trees of 64 over 1015 fp16 keys of 12 x 64: 21.9 us, a wide workgroup of 4
-// waves 27.4; 4 over 4000 int8 keys 22.6 and 25.1); with 8 they are not (8 trees of 32 x 4 heads a key head over 16384 int8
-// keys of 128: 165 and 122; over 8000 fp16 keys, 80 rows: 104 and 61).  An fp32 cache, which the wide one's fp16 fragments
+// waves 27.4; 4 over 4000 int8 keys 22.6 and 25.1); with 5 to 8 they are not (8 trees of 32 x 4 heads a key head over 16384
+// int8 keys of 128: 172 and 142; 80 rows over 8000 fp16 keys: 162 and 67 of 128 dims, 56 and 46 of 64).  An fp32 cache, which the wide one's fp16 fragments
 // cannot hold, takes the first always.
 int group_tiles(const KvCacheArgs &c, int tiles) {
     if (tiles <= 4 || c.dtype == ELEM_F32) return std::min(tiles, 2);

@@ -15,7 +15,7 @@
 // values at or above the larger of those are candidates -- in practice a few more than k of
 // thousands.  A candidate's rank is the number of better ones.
 //
-// 16 rows of 1024 with 5 alternatives 5.0 us; 181 of 16384 with 20 12.0 us, of which the sums alone take 5.0 (2.4 TB/s) and
+// 16 rows of 1024 with 5 alternatives 5.0 us; 181 of 16384 with 20 12.2 us, of which the sums alone take 5.8 (2.0 TB/s) and
 // the rest is the chain of sort, marks, second reads and ranks; 3 fp16 rows of 130001 with 8 6.1 and 4.8 of the join.
 // Few rows are a chain of dependent steps, not memory.
 #include <algorithm>

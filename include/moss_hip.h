@@ -366,7 +366,8 @@ enum {
     MOSS_HIP_ROPE_LINEAR = 1, /* w_i / factor */
     MOSS_HIP_ROPE_NTK = 2,    /* base * factor^(rot_dim / (rot_dim - 2)) in place of base (rot_dim >= 4) */
     MOSS_HIP_ROPE_YARN = 3    /* g w_i + (1 - g) w_i / factor, with g = (turns - beta_slow) / (beta_fast - beta_slow) within
-                                 [0, 1] and turns = orig_ctx w_i / 2pi; mscale = 0.1 ln(factor) + 1 */
+                                 [0, 1] and turns = orig_ctx w_i / 2pi; mscale = 0.1 ln(factor) + 1.  A model trained with a ramp over
+                                 i between two rounded bounds has other angles inside it: give those to moss_hip_rope */
 };
 typedef struct {
     int rot_dim;  /* leading elements of a head that are rotated: even, 2 .. 512 */
@@ -437,7 +438,8 @@ int moss_hip_kv_read(const moss_hip_kv_cache *cache, const int32_t *row_stream, 
  *   strides in elements, out q itself (same type and stride) or apart from it.  lse [rows][heads] fp32 or
  *   NULL: the log of each row's sum of exp(score).  The streams' row ranges lie apart.
  * A row that attends nothing is 0 with lse -inf; one that attends keys, but none with a score above -inf, is NaN, and so
- * is one with an Inf or NaN in its query.  What a row does not attend may hold anything, Inf and NaN too.  max_keys
+ * is one with an Inf or NaN in its query.  What a row does not attend may hold anything, Inf and NaN too;
+ * one in a key or value that it does attend may make the row, or that element of it, Inf or NaN.  max_keys
  * bounds every stream's ctx_len + n and sizes the launch.  A stream whose ctx_len is negative, whose keys pass max_keys or
  * its table, or with a page outside [0, n_pages) among them, gets NaN rows; one whose row range is not within [0, rows]
  * gets none.  Rows of no stream, and a stream's rows past max_rows, stay as they were.  Scores, sums and statistics are
