@@ -41,8 +41,10 @@ constexpr int kMaxSplits = 64;
 constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.69314718055994531f;
 constexpr float kSlack = 5.0f;  // log 2 of how far below its place a row's largest weight may lie
 constexpr float kPlace = 16.0f;  // log 2 of that place: what passes fp16's 65504 is left to lo
-constexpr float kFar = 16384.0f;  // scores past it are rounded before ref is taken off: past 2^31 a product's last bits alone can leave exp2's range
-constexpr float kLeast = -109.0f;  // log 2 of the least product of weight and value scale that is put there (2^(kPlace - kLeast) is a float)
+// Scores past this are rounded before ref is taken off: past 2^31 a product's last bits alone can leave exp2's range.
+constexpr float kFar = 16384.0f;
+// log 2 of the least product of weight and value scale that is put in its place: 2^(kPlace - kLeast) has to be a float.
+constexpr float kLeast = -109.0f;
 
 struct TreePlan {
     int tiles, group, row_groups;  // row tiles of 16, of which a workgroup takes `group`
@@ -386,10 +388,12 @@ __device__ __forceinline__ bool visible(const Stream &st, uint64_t bits, int pos
 }
 
 // Softmax state of a lane's rows, one per tile: l = sum w, o = sum w v with weights w = 2^(x - ref) of the scores x so far,
-// l of this lane's keys only, summed span by span with what each addition rounds off kept in `lost` (a wave can have 4096
-// spans, and equal weights round the same way each time: 2e-4 where they were added one by one).  ref is a whole number, so scaling by its changes is exact; no score passes it by more
-// than 1/2, and the largest is at most kSlack + 1/2 below it: it moves (and o and l are scaled) only when a score passes it,
-// which after the first spans is rare, where the largest itself still moves in every other span for some row of a tile.
+// l of this lane's keys only, summed span by span with what each addition rounds off kept in `lost` (equal weights round
+// the same way each time: 2e-4 of 131072 that were added one by one).  ref is a whole number, so scaling by its changes is
+// exact.  No score passes it, and the largest is at most kSlack + 1/2 below: it moves (and o and l are scaled) only when a
+// score passes it, which after the first spans is rare, where the largest itself still moves in every other span for some
+// row of a tile.  kSlack is what a weight's place costs in bits: with 3 the kernel for many rows takes 10 % longer, with 8
+// no less than with 5.
 // For the fp16 products the weights are multiplied by 2^kPlace; with value scales (SCALED) a weight times its scale
 // is, by 2^(kPlace - top), where no such product of the row so far has passed 2^top: top moves like ref.  Both are a
 // row's own business: what other rows of a tile see changes nothing.  `settle` takes these factors out.
@@ -469,7 +473,8 @@ struct Rows {
     // Weights times value scales, 0 where the row does not see the key, are put in place: `most` is what weigh returned and
     // `vmax` log 2 of what no scale of the 32 keys reaches, seen or not.
     __device__ __forceinline__ void place(int mt, float most, float vmax, float (&y)[2][4]) {
-        if (__any(most + vmax > top[mt] - 0.015625f)) {  // (less a margin for the roundings of `most`: where this is false, no product passes top)
+        // (less a margin for the roundings of `most`: where this is false, no product passes top)
+        if (__any(most + vmax > top[mt] - 0.015625f)) {
             float m = fmaxf(fmaxf(fmaxf(fabsf(y[0][0]), fabsf(y[0][1])), fmaxf(fabsf(y[0][2]), fabsf(y[0][3]))),
                             fmaxf(fmaxf(fabsf(y[1][0]), fabsf(y[1][1])), fmaxf(fabsf(y[1][2]), fabsf(y[1][3]))));
             m = fmaxf(m, xshfl<16>(m));
@@ -579,7 +584,7 @@ __device__ __forceinline__ void put_row(const TreeArgs &a, const TreePlan &plan,
         return;
     }
     const size_t at = (size_t)(st.row0 + node) * a.heads + head;
-    if (L == 0.0f && sees_any(a, st, node)) L = __uint_as_float(0x7fc00000u);  // (no score above -inf: 0 / 0, not a row that sees nothing)
+    if (L == 0.0f && sees_any(a, st, node)) L = __uint_as_float(0x7fc00000u);  // (no score above -inf: 0 / 0)
     const float inv = L == 0.0f ? 0.0f : 1.0f / L;
     const size_t o = (size_t)((int64_t)(st.row0 + node) * a.out_row + head * D + d0);
     if (a.out_dtype == ELEM_F16) {
@@ -822,16 +827,17 @@ __global__ __launch_bounds__(64 * W, W > kWaves ? 2 : KV == ELEM_F32 ? (D == 64 
 // Many rows (more than 64): bound by the matrix and vector units.  Every wave has MT row tiles of its own and all
 // of them the same keys, which they prepare together: of a stage of 16 keys a wave each turns its block into
 // fragments, K and V, and puts them into LDS in the order in which the products read them (16 bytes a lane, without
-// bank conflicts; the few that are counted are likely V's stores, 8 bytes at a stride of 16), so a key is converted once for up to 256 rows.  Two stages: while one is worked on the next
-// one's loads are in flight, and it is written before the only barrier of a stage.
+// bank conflicts; the few that are counted are likely V's stores, 8 bytes at a stride of 16), so a key is converted once
+// for up to 256 rows.  Two stages: while one is worked on the next one's loads are in flight, and it is written before
+// the only barrier of a stage.
 // LO: 32-bit queries, as hi + lo; the weights are hi + lo whatever the output's type is.
 // 8 streams with trees of 33 to 64, 32 heads of 128 on 8 key heads, 8192 to 16384 int8 keys: 185 to 214 us from run to
 // run, and 9.5 of the join.
 // The vector unit is what is busy most: 218 thousand cycles of the softmax (a score: scale, maximum, exponential of 4 slots,
 // sum, value scale, packing) and the conversions, 117 of the matrix unit, of 394 that a wave lives: little of the one falls
-// under the other with two waves to a SIMD.  Tried when it took 172, with weights of 11 bits: products of the next span issued ahead of the weights of one, 182; the row
-// tiles dealt to the waves in turn, so that none is idle where rows are fewer than 256, 184, as each then reads all
-// fragments for half the rows.
+// under the other with two waves to a SIMD.  Tried when it took 172, with weights of 11 bits: products of the next span
+// issued ahead of the weights of one, 182; the row tiles dealt to the waves in turn, so that none is idle where rows are
+// fewer than 256, 184, as each then reads all fragments for half the rows.
 template <int KV, int D, int NWV>
 struct WideLds {
     uint4 k[2][NWV][D / 32][64];
