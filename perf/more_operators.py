@@ -1,0 +1,520 @@
+"""Operators that a serving loop needs around its attention, as cases that can be timed and checked.
+
+Three families, in the order in which a step meets them:
+
+adapt    low-rank adapters of many requests beside a shared projection: rows of different requests, each with an
+         adapter of its own or none, added to what the projection gave;
+verify   drafted tokens against the target's probabilities, from given random numbers: chains drafted with
+         probabilities of their own, trees of tokens picked outright, greedy; the accepted path and the next token;
+beams    pages of a paged cache shared between streams: a reordering of beams (fork) and room for the next rows, with
+         copies of the pages that others still hold (reserve), over all layers;
+compact  accepted nodes of drafted trees moved to their final positions, over all layers.
+
+``run`` is the plain torch form in 32 bits (64 for probabilities that a random number is compared with), or with ``own``
+the calls of ``mosship.lib``.  Both take the state that ``prepare`` makes, and write into its pools and output buffers.
+
+Sizes: 12 layers of 12 heads of 64, 768 columns and 2304 rows of the projection, 64 streams, vocabularies of 1024 and 16384
+and a prompt of 181 are this repository's model and batch; the others are generic (rows of 4096, a vocabulary of about 2^17,
+8 heads of 128).
+"""
+from __future__ import annotations
+
+import math
+import os
+import sys
+
+import numpy as np
+import torch
+
+own = False
+DEV = "cuda"
+DTYPES = {"f32": torch.float32, "f16": torch.float16, "i8": torch.int8, "e4m3": torch.float8_e4m3fn}
+
+
+def _lib():
+    pkg = os.path.abspath("dsh-moss-tts_amd")
+    if pkg not in sys.path:
+        sys.path.insert(0, pkg)
+    from mosship import lib
+    return lib
+
+
+def listed():
+    return [
+        # one decode step of one request with its own voice
+        {"name": "adapt_step", "op": "adapt", "rows": 1, "each": 1, "cols": 768, "out": 2304, "rank": 8, "max_rank": 16, "adapters": 4,
+         "dtype": "f32"},
+        # one decode step of 64 requests, nearly every one with another adapter
+        {"name": "adapt_step_64", "op": "adapt", "rows": 64, "each": 1, "cols": 768, "out": 2304, "rank": 16, "max_rank": 16,
+         "adapters": 64, "dtype": "f32"},
+        # 16 prompts at once
+        {"name": "adapt_prompts", "op": "adapt", "rows": 2896, "each": 181, "cols": 768, "out": 2304, "rank": 16, "max_rank": 16,
+         "adapters": 16, "dtype": "f32"},
+        # long prompts over a wide projection, fp16 rows, adapters of different ranks
+        {"name": "adapt_wide", "op": "adapt", "rows": 8191, "each": 1021, "cols": 4096, "out": 4096, "rank": 64, "max_rank": 64,
+         "adapters": 8, "dtype": "f16"},
+        # one stream's four drafted audio codes, picked outright
+        {"name": "verify_step", "op": "verify", "streams": 1, "tree": 5, "vocab": 1024, "dtype": "f32", "draft": False, "chain": True,
+         "greedy": False, "temp": 1.0, "banned": False},
+        # chains of 64 streams, drafted by a model of its own
+        {"name": "verify_64", "op": "verify", "streams": 64, "tree": 6, "vocab": 16384, "dtype": "f32", "draft": True, "chain": True,
+         "greedy": False, "temp": 1.0, "banned": False},
+        # trees of 27 tokens, some of the vocabulary ruled out
+        {"name": "verify_tree", "op": "verify", "streams": 16, "tree": 27, "vocab": 16384, "dtype": "f32", "draft": False, "chain": False,
+         "greedy": False, "temp": 1.0, "banned": True},
+        # a large vocabulary, fp16 logits
+        {"name": "verify_wide", "op": "verify", "streams": 24, "tree": 9, "vocab": 130001, "dtype": "f16", "draft": True, "chain": True,
+         "greedy": False, "temp": 0.8, "banned": False},
+        # the four beams of one request
+        {"name": "beams_4", "op": "beams", "streams": 4, "width": 4, "ctx": 181, "new": 1, "layers": 12, "kvh": 12, "dim": 64, "page": 64,
+         "cache": "f16"},
+        # 16 requests of four beams each, far into their texts, an 8-bit cache of more layers
+        {"name": "beams_64", "op": "beams", "streams": 64, "width": 4, "ctx": 541, "new": 1, "layers": 32, "kvh": 8, "dim": 128, "page": 64,
+         "cache": "i8"},
+        # one stream's accepted nodes
+        {"name": "compact_1", "op": "compact", "streams": 1, "tree": 27, "ctx": 1015, "layers": 12, "kvh": 12, "dim": 64, "page": 64,
+         "cache": "f16"},
+        # 64 streams' accepted nodes
+        {"name": "compact_64", "op": "compact", "streams": 64, "tree": 64, "ctx": 181, "layers": 32, "kvh": 8, "dim": 128, "page": 64,
+         "cache": "e4m3"},
+    ]
+
+
+def _log(rng, lo, hi):
+    return max(lo, min(hi, int(round(math.exp(rng.uniform(math.log(lo), math.log(hi + 1)))))))
+
+
+def draw(rng):
+    op = rng.choice(["adapt", "adapt", "verify", "verify", "beams", "compact"])
+    if op == "adapt":
+        cols, out = rng.choice([(768, 2304), (768, 768), (4096, 4096), (32 * _log(rng, 1, 160), 16 * _log(rng, 1, 640))])
+        top = rng.choice([16, 16, 32, 64, 128])
+        n = _log(rng, 1, 64)
+        rows = _log(rng, 1, max(1, min(8192, (1 << 35) // (n * top * (cols + out)), (1 << 25) // max(cols, out))))
+        return {"op": op, "rows": rows, "each": rng.choice([1, 1, _log(rng, 1, 1024)]), "cols": cols, "out": out,
+                "rank": rng.choice([top, top, rng.randint(1, top)]), "max_rank": top, "adapters": n, "dtype": rng.choice(["f32", "f16"])}
+    if op == "verify":
+        vocab = rng.choice([1024, 16384, _log(rng, 2, 200000)])
+        draft = rng.random() < 0.4
+        tree = _log(rng, 1, 12 if draft else 64)
+        streams = _log(rng, 1, max(1, min(128, (1 << 25) // (vocab * tree))))
+        return {"op": op, "streams": streams, "tree": tree, "vocab": vocab, "dtype": rng.choice(["f32", "f16"]), "draft": draft,
+                "chain": draft or rng.random() < 0.3, "greedy": not draft and rng.random() < 0.25, "temp": rng.choice([1.0, 0.7, 1.3]),
+                "banned": rng.random() < 0.4}
+    cache = rng.choice(["f32", "f16", "i8", "e4m3"])
+    layers, (kvh, dim) = _log(rng, 1, 32), rng.choice([(12, 64), (8, 128), (1, 64), (2, 128), (5, 64)])
+    page = rng.choice([16, 48, 64, 128])
+    per_token = 2 * layers * kvh * dim * {"f32": 4, "f16": 2}.get(cache, 1)
+    most = (1 << 29) // per_token  # positions that the pools may hold
+    if op == "beams":
+        width = rng.choice([2, 4, 5, 8])
+        groups = _log(rng, 1, max(1, min(16, most // (4 * width * page))))
+        ctx = _log(rng, 1, max(1, min(2048, most // groups - 3 * width * page)))
+        return {"op": op, "streams": groups * width, "width": width, "ctx": ctx, "new": rng.choice([1, 1, _log(rng, 1, 64)]),
+                "layers": layers, "kvh": kvh, "dim": dim, "page": page, "cache": cache}
+    tree = _log(rng, 4, 64)
+    streams = _log(rng, 1, max(1, min(96, most // (2 * (tree + page)))))
+    return {"op": op, "streams": streams, "tree": tree, "ctx": _log(rng, 1, max(1, min(2048, most // streams - tree - page))),
+            "layers": layers, "kvh": kvh, "dim": dim, "page": page, "cache": cache}
+
+
+# ---------------------------------------------------------------- inputs
+
+def _gen(seed):
+    return torch.Generator(device=DEV).manual_seed(int(seed) * 2 + 1)
+
+
+def _randn(g, *shape, dtype=torch.float32):
+    return torch.randn(*shape, generator=g, device=DEV).to(dtype)
+
+
+def _randint(g, lo, hi, *shape):
+    """Whole numbers in [lo, hi)."""
+    return torch.randint(lo, hi, shape, generator=g, device=DEV)
+
+
+def _adapt_inputs(c, seed):
+    g = _gen(seed)
+    n, top, dt = c["adapters"], c["max_rank"], DTYPES[c["dtype"]]
+    st = {"x": _randn(g, c["rows"], c["cols"], dtype=dt), "base": _randn(g, c["rows"], c["out"], dtype=dt),
+          "a": _randn(g, n, top, c["cols"]).mul_(c["cols"] ** -0.5).half(), "b": _randn(g, n, c["out"], top).mul_(0.3).half()}
+    rank = torch.full((n,), c["rank"], device=DEV) if c["rank"] == top else _randint(g, 1, c["rank"] + 1, n)
+    scale = 0.5 + 1.5 * torch.rand(n, generator=g, device=DEV)
+    which = _randint(g, 0, n, (c["rows"] + c["each"] - 1) // c["each"])
+    which[1:][torch.rand(which.numel() - 1, generator=g, device=DEV) < 0.1] = -1  # requests without an adapter
+    st |= {"rank": rank.to(torch.int32), "scale": scale, "which": which.repeat_interleave(c["each"])[:c["rows"]].to(torch.int32).contiguous()}
+    return st
+
+
+def _rows_per_stream(c):
+    return [c["tree"] - s * 5 % (c["tree"] // 2 + 1) for s in range(c["streams"])]
+
+
+def _tree(g, streams, tree, chain):
+    """Parents and ancestor masks [streams][tree] of trees whose nodes come after their parents; bit j is node j, node 0 the root."""
+    up = (_randint(g, 0, 1 << 30, streams, tree) % torch.arange(1, tree + 1, device=DEV).clamp(max=8)).cpu().numpy()
+    m, par = np.zeros((streams, tree), np.uint64), np.zeros((streams, tree), np.int64)
+    for i in range(tree):
+        par[:, i] = max(i - 1, 0) if chain else np.maximum(i - 1 - up[:, i], 0)
+        m[:, i] = (m[np.arange(streams), par[:, i]] if i else np.uint64(0)) | np.uint64(1 << i)
+    return torch.from_numpy(par).to(DEV), torch.from_numpy(m.view(np.int64)).to(DEV)
+
+
+def _verify_inputs(c, seed):
+    """Logits of every node, tokens that a draft picked near them, and the random numbers."""
+    g = _gen(seed)
+    s, t, vocab = c["streams"], c["tree"], c["vocab"]
+    n = torch.tensor(_rows_per_stream(c), device=DEV)
+    start = torch.cat([torch.zeros(1, dtype=torch.int64, device=DEV), n.cumsum(0)])
+    rows = sum(_rows_per_stream(c))
+    stream = torch.repeat_interleave(torch.arange(s, device=DEV), n)
+    node = torch.arange(rows, device=DEV) - start[stream]
+    par, mask = (x[stream, node] for x in _tree(g, s, t, c["chain"]))
+    row = torch.arange(rows, device=DEV)
+    x = 2.0 * _randn(g, rows, vocab)
+    peak = _randint(g, 0, vocab, rows)
+    x[row, peak] += 5.0 + 8.0 * torch.rand(rows, generator=g, device=DEV)
+    if c["banned"]:
+        x[torch.rand(rows, vocab, generator=g, device=DEV) < 0.3] = -math.inf
+        x[row, peak] = 9.0
+    x = x.to(DTYPES[c["dtype"]])
+    st = {"x": x, "mask": mask, "start": start.to(torch.int32), "u": torch.rand(rows, generator=g, device=DEV, dtype=torch.float64),
+          "stream": stream, "node": node, "par": start[stream] + par}
+    up = st["par"]
+    if c["draft"]:  # the draft's opinion after each node, and the token drawn from it
+        y = (x.float() + 0.7 * _randn(g, rows, vocab)).to(x.dtype)
+        z = y.float() / c["temp"] - torch.log(-torch.log(torch.rand(rows, vocab, generator=g, device=DEV).clamp(1e-9, 1 - 1e-7)))
+        st["y"], tok = y, z.argmax(-1)[up]
+    else:  # often the likeliest token after the parent, else some other one
+        tok = torch.where(torch.rand(rows, generator=g, device=DEV) < 0.7, peak[up], _randint(g, 0, vocab, rows))
+    st["tok"] = tok.to(torch.int32)
+    return st
+
+
+def _pools(g, c, n_pages):
+    shape = (c["layers"], n_pages, c["kvh"], c["page"], c["dim"])
+    st = {}
+    for name in ("k", "v"):
+        if c["cache"] == "i8":
+            st[name] = torch.randint(-127, 128, shape, generator=g, device=DEV, dtype=torch.int8)
+        else:
+            st[name] = torch.randn(shape, generator=g, device=DEV, dtype=torch.float16 if c["cache"] != "f32" else torch.float32)
+            st[name] = st[name].to(DTYPES[c["cache"]])
+        st[name + "s"] = torch.rand(shape[:4], generator=g, device=DEV) if c["cache"] in ("i8", "e4m3") else None
+    return st
+
+
+def _beam_ctx(c):
+    """Committed positions of each stream: those of its group."""
+    return [c["ctx"] - s // c["width"] * 37 % (c["ctx"] // 2 + 1) for s in range(c["streams"])]
+
+
+def _beams_inputs(c, seed):
+    """Groups of beams over one prompt: whole pages are shared, each beam has its last page for itself."""
+    g = _gen(seed)
+    s, page, width = c["streams"], c["page"], c["width"]
+    ctx = _beam_ctx(c)
+    per = (c["ctx"] + c["new"] + page - 1) // page + 1
+    own_pages = (c["new"] + page - 2) // page + 2
+    n_pages = sum(x // page for x in ctx[::width]) + s * own_pages + 3
+    order = torch.randperm(n_pages, generator=g, device=DEV).cpu().numpy()
+    table, at = np.full((s, per), -1, np.int64), 0
+    for b in range(0, s, width):
+        whole = ctx[b] // page
+        table[b:b + width, :whole] = order[at:at + whole]
+        at += whole
+        if ctx[b] % page:
+            table[b:b + width, whole] = order[at:at + width]
+            at += width
+    refs = np.bincount(table[table >= 0], minlength=n_pages)
+    keep = (width + 1) // 2  # beams that go on; the others take one of theirs
+    i = torch.arange(s, device=DEV)
+    parent = torch.where(i % width < keep, i, i // width * width + _randint(g, 0, keep, s))
+    st = _pools(g, c, n_pages)
+    to = lambda x: torch.as_tensor(x).to(torch.int32).to(DEV)  # noqa: E731
+    return st | {"table": to(table), "refs": to(refs), "parent": to(parent), "ctx": to(ctx), "start": to(np.arange(s + 1) * c["new"]),
+                 "ok": torch.zeros(s, dtype=torch.int32, device=DEV)}
+
+
+def _kept_counts(c):
+    """Rows that each stream keeps, its root among them."""
+    return [1 + s * 7 % max(1, n // 2) if c["streams"] > 1 else max(1, n // 2) for s, n in enumerate(_rows_per_stream(c))]
+
+
+def _compact_inputs(c, seed):
+    g = _gen(seed)
+    s, page = c["streams"], c["page"]
+    n, m = _rows_per_stream(c), _kept_counts(c)
+    per = (c["ctx"] + c["tree"] + page - 1) // page
+    order = torch.randperm(s * per + 3, generator=g, device=DEV)[:s * per].view(s, per)
+    ctx = _randint(g, c["ctx"] // 2, c["ctx"] + 1, s)
+    pick = torch.rand(s, c["tree"], generator=g, device=DEV).cpu().numpy()
+    kept = np.full(sum(n), -1, np.int64)
+    for i, at in enumerate(np.cumsum([0] + n[:-1])):
+        # accepted nodes lie behind their final positions, as in trees numbered level by level
+        kept[at:at + m[i]] = np.concatenate([[0], np.sort(m[i] + np.argsort(pick[i, m[i]:n[i]])[:m[i] - 1])])
+    st = _pools(g, c, s * per + 3)
+    start = np.concatenate([[0], np.cumsum(n)])
+    to = lambda x: torch.as_tensor(x).to(torch.int32).to(DEV)  # noqa: E731
+    return st | {"table": to(order), "ctx": to(ctx), "kept": to(kept), "start": to(start),
+                 "stream": to(np.repeat(np.arange(s), n)), "node": to(np.concatenate([np.arange(x) for x in n]))}
+
+
+def prepare(case, seed):
+    c = case
+    if c["op"] == "adapt":
+        st = _adapt_inputs(c, seed)
+        st["out"] = torch.empty_like(st["base"])
+        if own:
+            st["ad"] = _lib().Adapters(st["a"], st["b"], st["rank"], st["scale"])
+    elif c["op"] == "verify":
+        st = _verify_inputs(c, seed)
+        rows, s = st["x"].shape[0], c["streams"]
+        st["accepted"], st["next"] = (torch.empty(s, dtype=torch.int32, device=DEV) for _ in range(2))
+        st["path"] = torch.empty(rows, dtype=torch.int32, device=DEV)
+        if own:
+            size = _lib().verify_tokens_workspace(s, c["tree"], rows, c["vocab"], draft=c["draft"])
+            st["ws"] = torch.empty(size, dtype=torch.uint8, device=DEV)
+    else:
+        st = _beams_inputs(c, seed) if c["op"] == "beams" else _compact_inputs(c, seed)
+        if own:
+            lib, scale = _lib(), lambda t, i: None if t is None else t[i]
+            st["layers"] = lib.KVLayers([lib.KVCache(st["k"][i], st["v"][i], st["table"], scale(st["ks"], i), scale(st["vs"], i))
+                                         for i in range(c["layers"])])
+            if c["op"] == "beams":
+                st["pages"] = lib.KVPages(st["table"], st["refs"], c["page"])
+                size = max(lib.kv_fork_workspace(st["pages"]), lib.kv_reserve_workspace(st["pages"], c["new"]))
+                st["ws"] = torch.empty(size, dtype=torch.uint8, device=DEV)
+    st["c"] = c
+    torch.cuda.synchronize()
+    return st
+
+
+# ---------------------------------------------------------------- one pass
+
+def run(st):
+    c, op = st["c"], st["c"]["op"]
+    if own:
+        lib = _lib()
+        if op == "adapt":
+            lib.adapter_rows(st["x"], st["ad"], st["which"], st["out"], base=st["base"])
+        elif op == "verify":
+            temp = 1.0 / c["temp"]
+            lib.verify_tokens(st["x"], st["tok"], st["start"], st["accepted"], st["path"], st["next"], max_rows=c["tree"],
+                              uniforms=None if c["greedy"] else st["u"], draft_logits=st.get("y"),
+                              row_mask=None if c["chain"] else st["mask"], inv_temperature=temp, draft_inv_temperature=temp,
+                              greedy=c["greedy"], workspace=st["ws"])
+        elif op == "beams":
+            lib.kv_fork(st["pages"], st["parent"], st["ctx"], workspace=st["ws"])
+            lib.kv_reserve(st["pages"], st["layers"], st["start"], st["ctx"], st["ok"], max_rows=c["new"], workspace=st["ws"])
+        else:
+            lib.kv_compact(st["layers"], st["start"], st["ctx"], st["kept"], max_rows=c["tree"])
+    else:
+        {"adapt": _adapt_plain, "verify": _verify_plain, "beams": _beams_plain, "compact": _compact_plain}[op](st, c)
+    if op == "adapt":
+        return st["out"]
+    if op == "verify":
+        return {"accepted": st["accepted"], "path": st["path"], "next": st["next"]}
+    pools = {name: st[name] for name in ("k", "v", "ks", "vs") if st[name] is not None}
+    return pools | {"table": st["table"], "refs": st["refs"], "ok": st["ok"]} if op == "beams" else pools
+
+
+def _adapt_plain(st, c):
+    """Every row through every adapter, and all but its own dropped in between: two products."""
+    n, top = c["adapters"], c["max_rank"]
+    k = torch.arange(top, device=DEV)
+    a = torch.where(k[None, :, None] < st["rank"][:, None, None], st["a"].float(), 0.0)
+    b = torch.where(k[None, None] < st["rank"][:, None, None], st["b"].float(), 0.0) * st["scale"][:, None, None]
+    t = torch.matmul(st["x"].float(), a.view(n * top, c["cols"]).T).view(-1, n, top)
+    t = torch.where(st["which"][:, None, None] == torch.arange(n, device=DEV)[None, :, None], t, 0.0)
+    st["out"].copy_(st["base"].float() + torch.matmul(t.view(-1, n * top), b.transpose(1, 2).reshape(n * top, c["out"])))
+
+
+def _scaled(x, temp):
+    """z in 64 bits: the temperature's reciprocal is a 32-bit number."""
+    return x.double() * float(np.float32(1.0 / temp))
+
+
+def _verify_plain(st, c):
+    s, t, vocab = c["streams"], c["tree"], c["vocab"]
+    up, stream, node, tok = st["par"], st["stream"], st["node"], st["tok"].long()
+    root, rows = node == 0, st["x"].shape[0]
+    if c["greedy"]:
+        x = st["x"].float()
+        best = torch.where(x == x.amax(-1, keepdim=True), torch.arange(vocab, device=DEV)[None], vocab).amin(-1)
+        ok = tok == best[up]
+    else:
+        z = _scaled(st["x"], c["temp"])
+        lse = torch.logsumexp(z, -1)
+        p = torch.exp(z[up, tok] - lse[up])
+        if c["draft"]:
+            zq = _scaled(st["y"], c["temp"])
+            lq = torch.logsumexp(zq, -1)
+            ok = st["u"] * torch.exp(zq[up, tok] - lq[up]) < p
+    grid = torch.full((s, t), -1, dtype=torch.int64, device=DEV)  # row of each node
+    grid[stream, node] = torch.arange(rows, device=DEV)
+    at = grid[stream]  # [rows][t]: the rows of this row's stream
+    other = at.clamp(min=0)
+    # earlier children of the same parent (the root is nobody's child)
+    elder = (at >= 0) & ~root[other] & ~root[:, None] & (up[other] == up[:, None]) & (node[other] < node[:, None])
+    if not c["greedy"] and not c["draft"]:
+        first = ~(elder & (tok[other] == tok[:, None])).any(1)
+        left = 1.0 - torch.where(elder & first[other], p[other], 0.0).sum(1)
+        ok = first & (st["u"] * left.clamp(min=0.0) < p)
+    taken = root | (ok & ~(elder & ok[other]).any(1))
+    bit = (st["mask"][:, None] >> torch.arange(t, device=DEV)[None]) & 1
+    on = ((bit == 0) | taken[other]).all(1)  # the node and all its ancestors
+    count = torch.zeros(s, dtype=torch.int64, device=DEV).index_add_(0, stream, on.long())
+    st["accepted"].copy_(count - 1)
+    depth = bit.sum(1) - 1
+    start = st["start"].long()
+    to = torch.where(on, start[stream] + depth, rows)  # rows off the path go behind the end
+    path = torch.full((rows + 1,), -1, dtype=torch.int64, device=DEV)
+    path[to] = torch.where(on, node, -1)
+    st["path"].copy_(path[:rows])
+    last = grid.gather(1, torch.where(on[grid.clamp(min=0)] & (grid >= 0), torch.arange(t, device=DEV)[None], 0).amax(1, keepdim=True))[:, 0]
+    if c["greedy"]:
+        st["next"].copy_(best[last])
+        return
+    w = torch.exp(z[last] - lse[last][:, None])
+    if c["draft"]:
+        rest = (w - torch.exp(zq[last] - lq[last][:, None])).clamp(min=0.0)
+        w = torch.where((last + 1 < start[1:])[:, None] & (rest.sum(1, keepdim=True) > 0), rest, w)
+    else:
+        child = ~root & (up == last[stream])  # all of them rejected
+        drop = torch.zeros(s, vocab + 1, dtype=torch.bool, device=DEV)
+        drop[stream, torch.where(child, tok, vocab)] = True
+        rest = torch.where(drop[:, :vocab], 0.0, w)
+        w = torch.where(rest.sum(1, keepdim=True) > 0, rest, w)
+    cdf = w.cumsum(1)
+    st["next"].copy_((cdf <= (st["u"][start[:-1]] * cdf[:, -1])[:, None]).sum(1).clamp(max=vocab - 1))
+
+
+def _beams_plain(st, c):
+    s, page = c["streams"], c["page"]
+    table, refs = st["table"].long(), st["refs"].long()
+    n_pages, per = refs.numel(), table.shape[1]
+    # fork
+    ctx = st["ctx"].long()
+    j = torch.arange(per, device=DEV)
+    new = torch.where(j[None] < ((ctx + page - 1) // page)[:, None], table[st["parent"].long()], -1)
+    uses = lambda t: torch.zeros(n_pages + 1, dtype=torch.int64, device=DEV).index_add_(  # noqa: E731
+        0, torch.where(t < 0, n_pages, t).view(-1), torch.ones(t.numel(), dtype=torch.int64, device=DEV))[:n_pages]
+    refs = refs + uses(new) - uses(table)
+    # reserve: the pages that the new rows go to
+    r = torch.arange((c["new"] + page - 2) // page + 1, device=DEV)
+    at = ctx[:, None] // page + r[None]
+    there = at <= ((ctx + c["new"] - 1) // page)[:, None]
+    e = torch.where(there, new.gather(1, at.clamp(max=per - 1)), -1)
+    i = torch.arange(s, device=DEV)
+    same = (e[:, None, :, None] == e[None, :, None, :]) & (at[:, None, :, None] == at[None, :, None, :]) & (e >= 0)[:, None, :, None]
+    earlier = (same & (i[None] < i[:, None])[:, :, None, None]).sum((1, 3))
+    shared = (e >= 0) & (refs[e.clamp(min=0)] - earlier > 1)
+    need = there & ((e < 0) | shared)
+    # the lowest free pages, in the order of streams and positions
+    order = (need.view(-1).long().cumsum(0) - 1).view(need.shape)
+    free = (refs != 0).to(torch.int8).sort(stable=True).indices
+    take = torch.where(need, free[order.clamp(0, n_pages - 1)], e)
+    refs = refs + uses(torch.where(need, take, -1)) - uses(torch.where(shared, e, -1))
+    new = new.scatter(1, torch.where(there, at, per - 1), torch.where(there, take, new[:, -1:]))
+    st["ok"].fill_(1)
+    st["table"].copy_(new)
+    st["refs"].copy_(refs)
+    # the committed positions of a page that others hold go along
+    copies, dst = shared[:, 0], take[:, 0]  # (no two streams have the same one)
+    src, below = torch.where(copies, e[:, 0], dst), torch.where(copies, ctx % page, 0)
+    slot = torch.arange(page, device=DEV)
+    for name in ("k", "v", "ks", "vs"):
+        if st[name] is not None:
+            raw = st[name].view(torch.int8) if st[name].dtype == torch.float8_e4m3fn else st[name]
+            see = (slot[None] < below[:, None]).view((1, s, 1, page) + (1,) * (raw.dim() - 4))
+            raw[:, dst] = torch.where(see, raw[:, src], raw[:, dst])
+
+
+def _compact_plain(st, c):
+    page, stream = c["page"], st["stream"].long()
+    ctx = st["ctx"].long()[stream]
+    moved = st["kept"] >= 0
+    to = ctx + st["node"].long()
+    src = torch.where(moved, ctx + st["kept"].long(), to)
+    table = st["table"].long()
+    for name in ("k", "v", "ks", "vs"):
+        if st[name] is not None:
+            raw = st[name].view(torch.int8) if st[name].dtype == torch.float8_e4m3fn else st[name]
+            x = raw[:, table[stream, src // page], :, src % page]
+            raw[:, table[stream, to // page], :, to % page] = x
+
+
+# ---------------------------------------------------------------- what a pass cannot do without
+
+def work(case):
+    c = case
+    if c["op"] == "adapt":
+        e = 4 if c["dtype"] == "f32" else 2
+        requests = (c["rows"] + c["each"] - 1) // c["each"]
+        n, used = c["adapters"], 0.9 * requests
+        used = max(1.0, n * (1.0 - (1.0 - 1.0 / n) ** used))  # different ones among them
+        rank = c["rank"] if c["rank"] == c["max_rank"] else (c["rank"] + 1) / 2
+        by = c["rows"] * (c["cols"] + 2 * c["out"]) * e + used * rank * (c["cols"] + c["out"]) * 2 + 4 * c["rows"]
+        return {"bytes": float(by), "flops": 2.0 * c["rows"] * rank * (c["cols"] + c["out"])}
+    if c["op"] == "verify":
+        rows = sum(_rows_per_stream(c))
+        n = (rows + (rows - c["streams"] if c["draft"] else 0)) * c["vocab"]  # a last node has no children that its draft drew
+        return {"bytes": float(n * (4 if c["dtype"] == "f32" else 2) + 24 * rows), "flops": 4.0 * n}
+    e = {"f32": 4, "f16": 2}.get(c["cache"], 1)
+    row = 2.0 * c["layers"] * c["kvh"] * (c["dim"] * e + (4 if e == 1 else 0))
+    if c["op"] == "beams":
+        slots = sum(x % c["page"] for s, x in enumerate(_beam_ctx(c)) if s % c["width"] >= (c["width"] + 1) // 2)
+        per = (c["ctx"] + c["new"] + c["page"] - 1) // c["page"] + 1
+        return {"bytes": 2.0 * row * slots + 8.0 * c["streams"] * per, "flops": 0.0}
+    rows = sum(m - 1 for m in _kept_counts(c))
+    return {"bytes": 2.0 * row * rows + 12.0 * c["streams"] * c["tree"], "flops": 0.0}
+
+
+# ---------------------------------------------------------------- the definitions in 64 bits
+
+def exact(case, seed):
+    c = case
+    if c["op"] == "verify":
+        return None  # whole numbers
+    if c["op"] == "adapt":
+        st = _adapt_inputs(c, seed)
+        out = st["base"].double()
+        which, rank, scale = st["which"].tolist(), st["rank"].tolist(), st["scale"].double()
+        for a in sorted(set(which) - {-1}):
+            rows = (st["which"] == a).nonzero()[:, 0]
+            t = st["x"][rows].double() @ st["a"][a, :rank[a]].double().T
+            out[rows] += scale[a] * (t @ st["b"][a, :, :rank[a]].double().T)
+        return out
+    if c["cache"] == "i8":
+        return None  # bytes are moved
+    st = _beams_inputs(c, seed) if c["op"] == "beams" else _compact_inputs(c, seed)
+    page = c["page"]
+    k, v = (st[name].view(torch.int8) if c["cache"] == "e4m3" else st[name] for name in ("k", "v"))
+    pools = [x for x in (k, v, st["ks"], st["vs"]) if x is not None]
+    table, ctx, moves = st["table"].tolist(), st["ctx"].tolist(), []  # (page, slot) to (page, slot)
+    if c["op"] == "beams":
+        new = [[p if j * page < ctx[s] else -1 for j, p in enumerate(table[a])] for s, a in enumerate(st["parent"].tolist())]
+        refs = [0] * st["refs"].numel()
+        for p in (p for t in new for p in t if p >= 0):
+            refs[p] += 1
+        for s, t in enumerate(new):  # one stream after the other
+            for j in range(ctx[s] // page, (ctx[s] + c["new"] - 1) // page + 1):
+                if t[j] >= 0 and refs[t[j]] <= 1:
+                    continue
+                old, t[j] = t[j], refs.index(0)
+                refs[t[j]] = 1
+                if old >= 0:
+                    refs[old] -= 1
+                    moves += [((old, i), (t[j], i)) for i in range(ctx[s] - j * page)]
+    else:
+        start, kept = st["start"].tolist(), st["kept"].tolist()
+        for s, t in enumerate(table):
+            place = lambda p: (t[p // page], p % page)  # noqa: E731
+            moves += [(place(ctx[s] + m), place(ctx[s] + j)) for j, m in enumerate(kept[start[s]:start[s + 1]]) if m >= 0]
+    if moves:
+        (p, i), (q, j) = (torch.tensor(x, device=DEV).T for x in zip(*moves))
+        for x in pools:
+            x[:, q, :, j] = x[:, p, :, i]
+    names = [name for name in ("k", "v", "ks", "vs") if st[name] is not None]
+    return {name: st[name].float().double() for name in names} | ({"table": None, "refs": None, "ok": None} if c["op"] == "beams" else {})
