@@ -273,7 +273,7 @@ def prepare(case, seed):
         st["accepted"], st["next"] = (torch.empty(s, dtype=torch.int32, device=DEV) for _ in range(2))
         st["path"] = torch.empty(rows, dtype=torch.int32, device=DEV)
         if own:
-            size = _lib().verify_tokens_workspace(s, c["tree"], rows, c["vocab"], draft=c["draft"])
+            size = _lib().verify_tokens_workspace(s, c["tree"], c["vocab"], draft=c["draft"])
             st["ws"] = torch.empty(size, dtype=torch.uint8, device=DEV)
     else:
         st = _beams_inputs(c, seed) if c["op"] == "beams" else _compact_inputs(c, seed)
