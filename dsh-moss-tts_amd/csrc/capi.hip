@@ -572,7 +572,7 @@ int moss_hip_attn_paged(const float *q, const void *k_pool, const void *v_pool, 
 
 namespace {
 
-constexpr int kMaxRows = 1 << 22, kMaxHeads = 1024, kMaxRot = 512;
+constexpr int kMaxRows = 1 << 22, kMaxHeads = 1024, kMaxRot = 512, kMaxStreams = 1 << 16;
 
 void check_row_type(int dtype) {
     if (dtype != MOSS_HIP_F32 && dtype != MOSS_HIP_F16) throw Status(MOSS_HIP_EINVAL, "dtype must be MOSS_HIP_F32 or MOSS_HIP_F16");
@@ -599,7 +599,7 @@ mh::KvCacheArgs cache_shape(const moss_hip_kv_cache *c) {
     if (c->kv_heads <= 0 || c->kv_heads > kMaxHeads) throw Status(MOSS_HIP_EINVAL, "need 0 < kv_heads <= 1024");
     if (c->page_size <= 0 || c->page_size % 16 || c->page_size > mh::kTreePageMax)
         throw Status(MOSS_HIP_EINVAL, "page_size must be a multiple of 16 and at most 32768");
-    if (c->streams < 0 || c->streams > (1 << 16)) throw Status(MOSS_HIP_EINVAL, "need 0 <= streams <= 65536");
+    if (c->streams < 0 || c->streams > kMaxStreams) throw Status(MOSS_HIP_EINVAL, "need 0 <= streams <= 65536");
     mh::KvCacheArgs a;
     a.dtype = c->kv_dtype;
     a.heads = c->kv_heads;
@@ -660,6 +660,78 @@ void check_workspace(const void *ws, size_t bytes, size_t need, const char *call
     if (ws == nullptr || bytes < need)
         throw Status(MOSS_HIP_EINVAL, std::string(call) + ": the workspace needs " + std::to_string(need) + " bytes");
     if ((uintptr_t)ws % 16) throw Status(MOSS_HIP_EINVAL, std::string(call) + ": the workspace must be 16-byte aligned");
+}
+
+void verify_shape(int streams, int max_rows, int vocab) {
+    if (streams < 0 || streams > kMaxStreams) throw Status(MOSS_HIP_EINVAL, "need 0 <= streams <= 65536");
+    if (max_rows <= 0 || max_rows > mh::kTreeMax) throw Status(MOSS_HIP_EINVAL, "need 0 < max_rows <= 64");
+    if (vocab <= 0 || vocab > mh::kVocabMax) throw Status(MOSS_HIP_EINVAL, "need 0 < vocab <= 2^20");
+    if ((long long)streams * max_rows * vocab > (1ll << 34)) throw Status(MOSS_HIP_EINVAL, "streams * max_rows * vocab must be at most 2^34");
+}
+
+mh::PagesArgs pages_args(const moss_hip_kv_pages *p) {
+    if (p == nullptr) throw Status(MOSS_HIP_EINVAL, "null pages");
+    if (p->streams < 0 || p->streams > kMaxStreams) throw Status(MOSS_HIP_EINVAL, "need 0 <= streams <= 65536");
+    if (p->table_stride <= 0 || (long long)p->streams * p->table_stride > (1 << 26))
+        throw Status(MOSS_HIP_EINVAL, "need table_stride > 0, streams * table_stride at most 2^26");
+    if (p->page_size <= 0 || p->page_size % 16 || p->page_size > mh::kTreePageMax)
+        throw Status(MOSS_HIP_EINVAL, "page_size must be a multiple of 16 and at most 32768");
+    if (p->n_pages <= 0) throw Status(MOSS_HIP_EINVAL, "need n_pages > 0");
+    mh::PagesArgs a;
+    a.table = p->page_table;
+    a.table_stride = p->table_stride;
+    a.streams = p->streams;
+    a.refs = p->refs;
+    a.n_pages = p->n_pages;
+    a.page_size = p->page_size;
+    return a;
+}
+void check_page_arrays(const moss_hip_kv_pages *p) {
+    if (!p->refs || (!p->page_table && p->streams > 0)) throw Status(MOSS_HIP_EINVAL, "pages: null pointer");
+}
+
+void reserve_shape(const mh::PagesArgs &p, int max_rows) {
+    if (max_rows <= 0 || max_rows > (long long)p.table_stride * p.page_size)
+        throw Status(MOSS_HIP_EINVAL, "need 0 < max_rows, at most table_stride * page_size");
+}
+
+// Caches of one shape over one table.
+mh::KvCacheArgs layer_args(const moss_hip_kv_cache *layers, int n_layers, mh::KvLayers &l) {
+    if (layers == nullptr) throw Status(MOSS_HIP_EINVAL, "null layers");
+    if (n_layers <= 0 || n_layers > mh::kLayersMax) throw Status(MOSS_HIP_EINVAL, "need 0 < n_layers <= 64");
+    const mh::KvCacheArgs c = cache_args(layers);
+    for (int i = 0; i < n_layers; ++i) {
+        const mh::KvCacheArgs o = cache_args(layers + i);
+        if (o.dtype != c.dtype || o.heads != c.heads || o.dim != c.dim || o.page_size != c.page_size || o.n_pages != c.n_pages ||
+            o.table != c.table || o.table_stride != c.table_stride || o.streams != c.streams)
+            throw Status(MOSS_HIP_EINVAL, "layers must have one shape, type and page table");
+        l.k[i] = o.k;
+        l.v[i] = o.v;
+        l.k_scale[i] = o.k_scale;
+        l.v_scale[i] = o.v_scale;
+    }
+    return c;
+}
+
+mh::AdapterArgs adapter_args(const moss_hip_adapters *p) {
+    if (p == nullptr) throw Status(MOSS_HIP_EINVAL, "null adapters");
+    if (p->n_adapters <= 0 || p->n_adapters > (1 << 20)) throw Status(MOSS_HIP_EINVAL, "need 0 < n_adapters <= 2^20");
+    if (p->max_rank <= 0 || p->max_rank % 16 || p->max_rank > mh::kAdapterRankMax)
+        throw Status(MOSS_HIP_EINVAL, "max_rank must be a multiple of 16 and at most 128");
+    if (p->cols <= 0 || p->cols % 32 || p->cols > 65536) throw Status(MOSS_HIP_EINVAL, "cols must be a multiple of 32 and at most 65536");
+    if (p->out <= 0 || p->out % 16 || p->out > 65536) throw Status(MOSS_HIP_EINVAL, "out must be a multiple of 16 and at most 65536");
+    if (!p->a || !p->b) throw Status(MOSS_HIP_EINVAL, "adapters: null pointer");
+    if (((uintptr_t)p->a | (uintptr_t)p->b) % 16) throw Status(MOSS_HIP_EINVAL, "adapters: weights must be 16-byte aligned");
+    mh::AdapterArgs a;
+    a.a = p->a;
+    a.b = p->b;
+    a.rank = p->rank;
+    a.scale = p->scale;
+    a.n = p->n_adapters;
+    a.max_rank = p->max_rank;
+    a.cols = p->cols;
+    a.out = p->out;
+    return a;
 }
 
 }  // namespace
@@ -867,6 +939,166 @@ int moss_hip_token_logprobs(const void *logits, int64_t row_stride, int dtype, i
         a.top_lp = top_logprobs;
         a.ws = workspace;
         mh::hip_check(mh::launch_logprobs(a, static_cast<hipStream_t>(stream)), "log probability launch");
+    });
+}
+
+int moss_hip_verify_tokens_workspace(int streams, int max_rows, int vocab, int draft, size_t *bytes) {
+    return guard([&] {
+        if (bytes == nullptr) throw Status(MOSS_HIP_EINVAL, "null output");
+        verify_shape(streams, max_rows, vocab);
+        *bytes = streams == 0 ? 0 : mh::verify_workspace(streams, max_rows, vocab, draft != 0);
+    });
+}
+
+int moss_hip_verify_tokens(const void *logits, int64_t row_stride, int dtype, const void *draft_logits, int64_t draft_stride,
+                           int rows, int vocab, const int32_t *tokens, const int32_t *row_start, const uint64_t *row_mask,
+                           int streams, int max_rows, const double *uniforms, float inv_temperature, float draft_inv_temperature,
+                           int greedy, int32_t *accepted, int32_t *path, int32_t *next_token, void *workspace,
+                           size_t workspace_bytes, void *stream) {
+    return guard([&] {
+        verify_shape(streams, max_rows, vocab);
+        check_rows(rows);
+        if (greedy != 0 && greedy != 1) throw Status(MOSS_HIP_EINVAL, "greedy must be 0 or 1");
+        if (!row_start || !accepted || !next_token || (rows > 0 && (!logits || !tokens || !path))) throw Status(MOSS_HIP_EINVAL, "null pointer");
+        if (greedy && (draft_logits || uniforms)) throw Status(MOSS_HIP_EINVAL, "greedy takes no draft_logits and no uniforms");
+        if (!greedy && !uniforms && rows > 0) throw Status(MOSS_HIP_EINVAL, "null uniforms");
+        if (draft_logits && row_mask) throw Status(MOSS_HIP_EINVAL, "draft_logits are for chains: no row_mask besides");
+        check_row_type(dtype);
+        check_strides({row_stride, draft_stride});
+        for (const float t : {inv_temperature, draft_inv_temperature})
+            if (!(t > 0.0f) || !std::isfinite(t)) throw Status(MOSS_HIP_EINVAL, "inverse temperatures must be positive and finite");
+        if (streams == 0) return;
+        check_workspace(workspace, workspace_bytes, mh::verify_workspace(streams, max_rows, vocab, draft_logits != nullptr), "moss_hip_verify_tokens");
+        mh::VerifyArgs a;
+        a.x = logits;
+        a.y = draft_logits;
+        a.dtype = dtype;
+        a.x_row = row_stride;
+        a.y_row = draft_stride;
+        a.rows = rows;
+        a.vocab = vocab;
+        a.tokens = tokens;
+        a.row_start = row_start;
+        a.row_mask = row_mask;
+        a.streams = streams;
+        a.max_rows = max_rows;
+        a.uniforms = uniforms;
+        a.inv_t = inv_temperature;
+        a.draft_inv_t = draft_inv_temperature;
+        a.greedy = greedy != 0;
+        a.accepted = accepted;
+        a.path = path;
+        a.next = next_token;
+        a.ws = workspace;
+        mh::hip_check(mh::launch_verify(a, static_cast<hipStream_t>(stream)), "verification launch");
+    });
+}
+
+int moss_hip_kv_fork_workspace(const moss_hip_kv_pages *pages, size_t *bytes) {
+    return guard([&] {
+        if (bytes == nullptr) throw Status(MOSS_HIP_EINVAL, "null output");
+        *bytes = mh::fork_workspace(pages_args(pages));
+    });
+}
+
+int moss_hip_kv_fork(const moss_hip_kv_pages *pages, const int32_t *parent, const int32_t *len, void *workspace,
+                     size_t workspace_bytes, void *stream) {
+    return guard([&] {
+        mh::ForkArgs a;
+        a.p = pages_args(pages);
+        check_page_arrays(pages);
+        if (!parent) throw Status(MOSS_HIP_EINVAL, "null pointer");
+        if (a.p.streams == 0) return;
+        check_workspace(workspace, workspace_bytes, mh::fork_workspace(a.p), "moss_hip_kv_fork");
+        a.parent = parent;
+        a.len = len;
+        a.ws = static_cast<int *>(workspace);
+        mh::hip_check(mh::launch_kv_fork(a, static_cast<hipStream_t>(stream)), "page launch");
+    });
+}
+
+int moss_hip_kv_reserve_workspace(const moss_hip_kv_pages *pages, int max_rows, size_t *bytes) {
+    return guard([&] {
+        if (bytes == nullptr) throw Status(MOSS_HIP_EINVAL, "null output");
+        const mh::PagesArgs p = pages_args(pages);
+        reserve_shape(p, max_rows);
+        *bytes = mh::reserve_workspace(p, max_rows);
+    });
+}
+
+int moss_hip_kv_reserve(const moss_hip_kv_pages *pages, const moss_hip_kv_cache *layers, int n_layers, const int32_t *row_start,
+                        const int32_t *ctx_len, int max_rows, int32_t *ok, void *workspace, size_t workspace_bytes, void *stream) {
+    return guard([&] {
+        mh::ReserveArgs a;
+        mh::KvLayers l{};
+        a.p = pages_args(pages);
+        check_page_arrays(pages);
+        reserve_shape(a.p, max_rows);
+        const mh::KvCacheArgs c = layer_args(layers, n_layers, l);
+        if (c.table != a.p.table || c.table_stride != a.p.table_stride || c.streams != a.p.streams || c.n_pages != a.p.n_pages ||
+            c.page_size != a.p.page_size)
+            throw Status(MOSS_HIP_EINVAL, "the layers' page table and page sizes must be those of the pages");
+        if (!row_start || !ctx_len || !ok) throw Status(MOSS_HIP_EINVAL, "null pointer");
+        if (a.p.streams == 0) return;
+        check_workspace(workspace, workspace_bytes, mh::reserve_workspace(a.p, max_rows), "moss_hip_kv_reserve");
+        a.layers = n_layers;
+        a.heads = c.heads;
+        a.vec_bytes = c.dim * mh::elem_size(c.dtype);
+        a.scales = mh::quantised(c.dtype);
+        a.row_start = row_start;
+        a.ctx_len = ctx_len;
+        a.max_rows = max_rows;
+        a.ok = ok;
+        a.ws = workspace;
+        mh::hip_check(mh::launch_kv_reserve(a, l, static_cast<hipStream_t>(stream)), "page launch");
+    });
+}
+
+int moss_hip_kv_compact(const moss_hip_kv_cache *layers, int n_layers, const int32_t *row_start, const int32_t *ctx_len,
+                        const int32_t *kept, int rows, int max_rows, void *stream) {
+    return guard([&] {
+        mh::CompactArgs a;
+        mh::KvLayers l{};
+        a.c = layer_args(layers, n_layers, l);
+        check_rows(rows);
+        if (max_rows <= 0 || max_rows > mh::kTreeMax) throw Status(MOSS_HIP_EINVAL, "need 0 < max_rows <= 64");
+        if (!row_start || !ctx_len || (!kept && rows > 0)) throw Status(MOSS_HIP_EINVAL, "null pointer");
+        if (rows == 0 || a.c.streams == 0) return;
+        a.layers = n_layers;
+        a.vec_bytes = a.c.dim * mh::elem_size(a.c.dtype);
+        a.row_start = row_start;
+        a.ctx_len = ctx_len;
+        a.kept = kept;
+        a.rows = rows;
+        a.max_rows = max_rows;
+        mh::hip_check(mh::launch_kv_compact(a, l, static_cast<hipStream_t>(stream)), "page launch");
+    });
+}
+
+int moss_hip_adapter_rows(const void *x, int64_t x_stride, int x_dtype, const moss_hip_adapters *adapters, const int32_t *adapter,
+                          int rows, const void *base, int64_t base_stride, void *y, int64_t y_stride, int y_dtype, void *stream) {
+    return guard([&] {
+        mh::AdapterArgs a = adapter_args(adapters);
+        if (!x || !adapter || !base || !y) throw Status(MOSS_HIP_EINVAL, "null pointer");
+        check_row_type(x_dtype);
+        check_row_type(y_dtype);
+        check_rows(rows);
+        check_strides({x_stride, base_stride, y_stride});
+        if (rows > 1 && y_stride < a.out) throw Status(MOSS_HIP_EINVAL, "rows of y must not overlap");
+        if (y == base && rows > 1 && y_stride != base_stride) throw Status(MOSS_HIP_EINVAL, "in place, base and y must have the same stride");
+        if (y == x) throw Status(MOSS_HIP_EINVAL, "y must not be x");
+        if (rows == 0) return;
+        a.x = x;
+        a.x_dtype = x_dtype;
+        a.x_row = x_stride;
+        a.which = adapter;
+        a.rows = rows;
+        a.base = base;
+        a.base_row = base_stride;
+        a.y = y;
+        a.y_dtype = y_dtype;
+        a.y_row = y_stride;
+        mh::hip_check(mh::launch_adapter_rows(a, static_cast<hipStream_t>(stream)), "adapter launch");
     });
 }
 

@@ -1,0 +1,366 @@
+// kv_pages.hip -- the pages of a paged K/V cache: streams that share them, room for new rows, and
+// accepted rows moved to their final positions (gfx950).
+//
+// A page is held by the table entries that name it, and refs[page] counts those (and whatever holds the
+// caller adds); a page with 0 is free.  Everything is decided on the device, by rules whose outcome does
+// not depend on the order in which workgroups run: sums of counts, and prefix sums in the order of streams.
+// What a table or a list names outside its range is never followed.
+#include <algorithm>
+
+#include "paged_ops.h"
+
+namespace mh {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kBookThreads = 1024;  // of the workgroup that keeps the books
+
+// ---------------------------------------------------------------- fork
+
+// Entry (s, j) afterwards: the parent's, where it lies within the length.
+__device__ __forceinline__ int forked(const ForkArgs &a, int s, int j) {
+    const int p = a.parent[s];
+    if (p < 0 || p >= a.p.streams) return -1;
+    if (a.len != nullptr && (long long)j * a.p.page_size >= a.len[s]) return -1;
+    const int e = a.p.table[(size_t)p * a.p.table_stride + j];
+    return e >= 0 && e < a.p.n_pages ? e : -1;
+}
+__device__ __forceinline__ void count_change(const PagesArgs &p, int from, int to) {
+    if (from == to) return;
+    if (from >= 0 && from < p.n_pages) atomicAdd(p.refs + from, -1);
+    if (to >= 0) atomicAdd(p.refs + to, 1);
+}
+
+// Tables of up to N * 1024 entries: one workgroup holds all of them, so the old ones are read before
+// the first new one is written.
+template <int N>
+__global__ __launch_bounds__(kBookThreads) void fork_kernel(ForkArgs a) {
+    const int n = a.p.streams * a.p.table_stride;
+    int from[N], to[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int e = i * kBookThreads + (int)threadIdx.x;
+        if (e >= n) break;
+        const int s = e / a.p.table_stride;
+        from[i] = a.p.table[e];
+        to[i] = forked(a, s, e - s * a.p.table_stride);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int e = i * kBookThreads + (int)threadIdx.x;
+        if (e >= n) break;
+        if (from[i] != to[i]) a.p.table[e] = to[i];
+        count_change(a.p, from[i], to[i]);
+    }
+}
+
+// Larger ones by two launches, the new table in the workspace between them.
+__global__ __launch_bounds__(kThreads) void fork_read_kernel(ForkArgs a, long long n) {
+    const long long e = (long long)blockIdx.x * kThreads + threadIdx.x;
+    if (e >= n) return;
+    const int s = (int)(e / a.p.table_stride);
+    const int to = forked(a, s, (int)(e - (long long)s * a.p.table_stride));
+    a.ws[e] = to;
+    count_change(a.p, a.p.table[e], to);
+}
+__global__ __launch_bounds__(kThreads) void fork_write_kernel(ForkArgs a, long long n) {
+    const long long e = (long long)blockIdx.x * kThreads + threadIdx.x;
+    if (e < n) a.p.table[e] = a.ws[e];
+}
+
+constexpr int kForkEntries = 16;  // of a thread of the one workgroup
+
+// ---------------------------------------------------------------- reserve
+
+// Pages j0 .. j1 are those that stream s writes (none where j1 < j0); ok: its rows have places at all.
+struct Range {
+    int j0, j1;
+    bool ok;
+};
+__device__ __forceinline__ Range range_of(const ReserveArgs &a, int s) {
+    const long long n = (long long)a.row_start[s + 1] - a.row_start[s], ctx = a.ctx_len[s];
+    Range r{0, -1, ctx >= 0 && n >= 0 && n <= a.max_rows && ctx + n <= (long long)a.p.table_stride * a.p.page_size};
+    if (r.ok && n > 0) {
+        r.j0 = (int)(ctx / a.p.page_size);
+        r.j1 = (int)((ctx + n - 1) / a.p.page_size);
+    }
+    return r;
+}
+
+// What becomes of an entry: it is missing, it is shared and gets a page of its own, it stays, or (from 0 on) it
+// stays if every earlier holder, up to that stream, takes another page.
+enum { MISSING = -3, SHARED = -2, STAYS = -1 };
+
+// Streams are served one after the other: an earlier stream of this call that writes the same page has
+// given it up by then, so the last of a page's holders keeps it.
+__device__ int fate_of(const ReserveArgs &a, int s, int j) {
+    const int e = a.p.table[(size_t)s * a.p.table_stride + j];
+    if (e < 0 || e >= a.p.n_pages) return MISSING;
+    const int held = a.p.refs[e];
+    if (held <= 1) return STAYS;
+    int earlier = 0, last = 0;
+    for (int o = 0; o < s; ++o) {
+        const Range r = range_of(a, o);
+        if (j >= r.j0 && j <= r.j1 && a.p.table[(size_t)o * a.p.table_stride + j] == e) {
+            ++earlier;
+            last = o;
+        }
+    }
+    return held - earlier > 1 ? SHARED : last;
+}
+
+// Pages that one stream's rows can touch.
+__host__ __device__ __forceinline__ int pages_of(int max_rows, int page_size) { return (max_rows + page_size - 2) / page_size + 1; }
+
+struct ReserveWs {
+    int4 *copies;  // [streams]: from page, to page, slots
+    int *free_pages;   // the lowest free ones
+    int *fate;    // [streams][pages]
+};
+__host__ __device__ __forceinline__ ReserveWs reserve_ws(const PagesArgs &p, int max_rows, void *ws) {
+    ReserveWs w;
+    w.copies = (int4 *)ws;
+    w.free_pages = (int *)(w.copies + p.streams);
+    w.fate = w.free_pages + (size_t)p.streams * pages_of(max_rows, p.page_size);
+    return w;
+}
+
+__global__ __launch_bounds__(kThreads) void fate_kernel(ReserveArgs a, long long n, int per) {
+    const long long e = (long long)blockIdx.x * kThreads + threadIdx.x;
+    if (e >= n) return;
+    const int s = (int)(e / per), r = (int)(e - (long long)s * per);
+    const Range g = range_of(a, s);
+    reserve_ws(a.p, a.max_rows, a.ws).fate[e] = g.j0 + r <= g.j1 ? fate_of(a, s, g.j0 + r) : STAYS;
+}
+
+// Sum over the workgroup's earlier threads, and over all of them.
+__device__ __forceinline__ int2 block_scan(int v, int *lds) {
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    int sum = v;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        const int o = __shfl_up(sum, d);
+        if (lane >= d) sum += o;
+    }
+    __syncthreads();
+    if (lane == 63) lds[w] = sum;
+    __syncthreads();
+    int before = 0, all = 0;
+    for (int i = 0; i < kBookThreads / 64; ++i) {
+        if (i < w) before += lds[i];
+        all += lds[i];
+    }
+    return make_int2(before + sum - v, all);
+}
+
+// The books of one call, by one workgroup, a thread a stream.
+__global__ __launch_bounds__(kBookThreads) void reserve_kernel(ReserveArgs a, int per) {
+    __shared__ int lds[kBookThreads / 64], unserved;
+    const ReserveWs w = reserve_ws(a.p, a.max_rows, a.ws);
+    const int t = threadIdx.x;
+    if (t == 0) unserved = a.p.streams;
+    // how many pages are wanted
+    int mine = 0;
+    for (long long e = t; e < (long long)a.p.streams * per; e += kBookThreads) mine += w.fate[e] <= SHARED;
+    const int wanted = block_scan(mine, lds).y;
+    // the lowest free ones, as many as that
+    int found = 0;
+    for (int p0 = 0; p0 < a.p.n_pages && found < wanted; p0 += 4 * kBookThreads) {
+        bool is[4];
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int p = p0 + 4 * t + i;
+            is[i] = p < a.p.n_pages && a.p.refs[p] == 0;
+            n += is[i];
+        }
+        const int2 at = block_scan(n, lds);
+        int k = found + at.x;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (is[i]) {
+                if (k < wanted) w.free_pages[k] = p0 + 4 * t + i;
+                ++k;
+            }
+        found += at.y;
+    }
+    __syncthreads();  // (the list is read by other threads of this workgroup)
+    // Streams in their order: those before the first that finds too few are served.
+    int given = 0;
+    for (int s0 = 0; s0 < a.p.streams; s0 += kBookThreads) {
+        const int s = s0 + t;
+        int need = 0, left = -1;
+        if (s < a.p.streams)
+            for (int r = 0; r < per; ++r) {
+                const int f = w.fate[(size_t)s * per + r];
+                need += f <= SHARED;
+                left = max(left, f);
+            }
+        const int2 at = block_scan(need, lds);
+        if (need > 0 && given + at.x + need > found) atomicMin(&unserved, s);
+        __syncthreads();
+        if (s < a.p.streams) {
+            const Range g = range_of(a, s);
+            const bool ok = g.ok && left < unserved && (need == 0 || s < unserved);
+            int4 copy = make_int4(0, 0, 0, 0);
+            if (ok && need > 0) {
+                int k = given + at.x;
+                for (int j = g.j0; j <= g.j1; ++j) {
+                    const int f = w.fate[(size_t)s * per + (j - g.j0)];
+                    if (f > SHARED) continue;
+                    int *entry = a.p.table + (size_t)s * a.p.table_stride + j;
+                    const int page = w.free_pages[k++];
+                    if (f == SHARED) {
+                        const int old = *entry;
+                        atomicAdd(a.p.refs + old, -1);
+                        if (j == g.j0) copy = make_int4(old, page, a.ctx_len[s] - j * a.p.page_size, 0);
+                    }
+                    a.p.refs[page] = 1;
+                    *entry = page;
+                }
+            }
+            a.ok[s] = ok;
+            w.copies[s] = copy;
+        }
+        given += at.y;
+    }
+}
+
+// 16-byte pieces and scales of one head's first `slots` positions.
+__global__ __launch_bounds__(kThreads) void copy_kernel(ReserveArgs a, KvLayers l) {
+    const int4 c = reserve_ws(a.p, a.max_rows, a.ws).copies[blockIdx.x];
+    if (c.z <= 0) return;
+    const int layer = blockIdx.y >> 1;
+    const bool is_v = blockIdx.y & 1;
+    char *pool = (char *)(is_v ? l.v[layer] : l.k[layer]);
+    const int units = c.z * a.vec_bytes / 16;
+    const size_t head = (size_t)a.p.page_size * a.vec_bytes;
+    for (int h = blockIdx.z; h < a.heads; h += gridDim.z) {
+        const uint4 *from = (const uint4 *)(pool + ((size_t)c.x * a.heads + h) * head);
+        uint4 *to = (uint4 *)(pool + ((size_t)c.y * a.heads + h) * head);
+        for (int u = threadIdx.x; u < units; u += kThreads) to[u] = from[u];
+        if (a.scales) {
+            float *scale = is_v ? l.v_scale[layer] : l.k_scale[layer];
+            const float *fs = scale + ((size_t)c.x * a.heads + h) * a.p.page_size;
+            float *ts = scale + ((size_t)c.y * a.heads + h) * a.p.page_size;
+            for (int u = threadIdx.x; u < c.z; u += kThreads) ts[u] = fs[u];
+        }
+    }
+}
+
+// ---------------------------------------------------------------- compact
+
+constexpr int kMovesPerThread = 8;  // 16-byte pieces in flight
+
+// One workgroup: the rows of one stream in one layer's K or V, a range of heads.  All rows of a head are in registers
+// before the first is stored, so any row may take any other's place.
+__global__ __launch_bounds__(kThreads) void compact_kernel(CompactArgs a, KvLayers l, int heads_each) {
+    __shared__ uint2 from[kTreeMax], to[kTreeMax];  // page, slot
+    __shared__ int moves;
+    const int s = blockIdx.x, t = threadIdx.x;
+    if (t < 64) {
+        const int r0 = a.row_start[s], r1 = a.row_start[s + 1], ctx = a.ctx_len[s];
+        bool move = false;
+        uint2 src{}, dst{};
+        if (r0 >= 0 && r1 <= a.rows && ctx >= 0 && t < min(r1 - r0, a.max_rows)) {
+            const int k = a.kept[r0 + t];
+            if (k >= 0 && k < r1 - r0 && k != t) {
+                const long long ps = (long long)ctx + k, pd = (long long)ctx + t;
+                const long long js = ps / a.c.page_size, jd = pd / a.c.page_size;
+                if (js < a.c.table_stride && jd < a.c.table_stride) {
+                    const int *row = a.c.table + (size_t)s * a.c.table_stride;
+                    src = make_uint2(row[js], (unsigned)(ps - js * a.c.page_size));
+                    dst = make_uint2(row[jd], (unsigned)(pd - jd * a.c.page_size));
+                    move = src.x < (unsigned)a.c.n_pages && dst.x < (unsigned)a.c.n_pages;
+                }
+            }
+        }
+        const uint64_t who = __ballot(move);
+        if (move) {
+            const int at = __popcll(who & ((1ull << t) - 1));
+            from[at] = src;
+            to[at] = dst;
+        }
+        if (t == 0) moves = __popcll(who);
+    }
+    __syncthreads();
+    const int m = moves;
+    if (m == 0) return;
+    const int layer = blockIdx.y >> 1;
+    const bool is_v = blockIdx.y & 1;
+    char *pool = (char *)(is_v ? l.v[layer] : l.k[layer]);
+    float *scale = is_v ? l.v_scale[layer] : l.k_scale[layer];
+    const int per = a.vec_bytes / 16, of_head = m * per;
+    const int first = blockIdx.z * heads_each, last = min(first + heads_each, a.c.heads);
+    const int group = max(1, kMovesPerThread * kThreads / of_head);  // heads at a time
+    auto place = [&](uint2 p, int h) { return ((size_t)p.x * a.c.heads + h) * a.c.page_size + p.y; };
+    for (int h0 = first; h0 < last; h0 += group) {
+        const int n = min(group, last - h0), units = n * of_head;
+        uint4 x[kMovesPerThread];
+        float d[kMovesPerThread];
+#pragma unroll
+        for (int i = 0; i < kMovesPerThread; ++i) {
+            const int u = i * kThreads + t;
+            if (u < units) {
+                const int h = u / of_head, r = (u - h * of_head) / per, e = u % per;
+                x[i] = *(const uint4 *)(pool + place(from[r], h0 + h) * a.vec_bytes + 16 * e);
+            }
+            if (scale != nullptr && u < n * m) d[i] = scale[place(from[u % m], h0 + u / m)];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kMovesPerThread; ++i) {
+            const int u = i * kThreads + t;
+            if (u < units) {
+                const int h = u / of_head, r = (u - h * of_head) / per, e = u % per;
+                *(uint4 *)(pool + place(to[r], h0 + h) * a.vec_bytes + 16 * e) = x[i];
+            }
+            if (scale != nullptr && u < n * m) scale[place(to[u % m], h0 + u / m)] = d[i];
+        }
+    }
+}
+
+}  // namespace
+
+size_t fork_workspace(const PagesArgs &p) {
+    const size_t n = (size_t)p.streams * p.table_stride;
+    return n <= kForkEntries * kBookThreads ? 0 : n * sizeof(int);
+}
+
+hipError_t launch_kv_fork(const ForkArgs &a, hipStream_t s) {
+    const long long n = (long long)a.p.streams * a.p.table_stride;
+    (void)hipGetLastError();
+    if (n <= kBookThreads) {
+        hipLaunchKernelGGL(fork_kernel<1>, dim3(1), dim3(kBookThreads), 0, s, a);
+    } else if (n <= kForkEntries * kBookThreads) {
+        hipLaunchKernelGGL(fork_kernel<kForkEntries>, dim3(1), dim3(kBookThreads), 0, s, a);
+    } else {
+        const unsigned blocks = (unsigned)((n + kThreads - 1) / kThreads);
+        hipLaunchKernelGGL(fork_read_kernel, dim3(blocks), dim3(kThreads), 0, s, a, n);
+        hipLaunchKernelGGL(fork_write_kernel, dim3(blocks), dim3(kThreads), 0, s, a, n);
+    }
+    return hipGetLastError();
+}
+
+size_t reserve_workspace(const PagesArgs &p, int max_rows) {
+    return p.streams * (sizeof(int4) + 2 * sizeof(int) * (size_t)pages_of(max_rows, p.page_size));
+}
+
+hipError_t launch_kv_reserve(const ReserveArgs &a, const KvLayers &l, hipStream_t s) {
+    const int per = pages_of(a.max_rows, a.p.page_size);
+    const long long n = (long long)a.p.streams * per;
+    (void)hipGetLastError();
+    hipLaunchKernelGGL(fate_kernel, dim3((unsigned)((n + kThreads - 1) / kThreads)), dim3(kThreads), 0, s, a, n, per);
+    hipLaunchKernelGGL(reserve_kernel, dim3(1), dim3(kBookThreads), 0, s, a, per);
+    hipLaunchKernelGGL(copy_kernel, dim3(a.p.streams, 2 * a.layers, a.heads), dim3(kThreads), 0, s, a, l);
+    return hipGetLastError();
+}
+
+hipError_t launch_kv_compact(const CompactArgs &a, const KvLayers &l, hipStream_t s) {
+    (void)hipGetLastError();
+    hipLaunchKernelGGL(compact_kernel, dim3(a.c.streams, 2 * a.layers, a.c.heads), dim3(kThreads), 0, s, a, l, 1);
+    return hipGetLastError();
+}
+
+}  // namespace mh

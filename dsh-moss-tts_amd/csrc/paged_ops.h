@@ -1,6 +1,7 @@
 // paged_ops.h -- launchers of the operators of a caller's own decoding loop: rotary positions, a
-// paged K/V cache in fp32, fp16, int8 or e4m3, attention of drafted rows over it, and token
-// log probabilities (internal C++ API; the C entry points check the arguments).
+// paged K/V cache in fp32, fp16, int8 or e4m3 and its pages, attention of drafted rows over it, token
+// log probabilities, verification of drafted tokens, and adapters beside a projection (internal C++
+// API; the C entry points check the arguments).
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -96,5 +97,83 @@ constexpr int kTreeMax = 64;  // drafted rows of a stream
 constexpr int kTreeKeysMax = 1 << 28, kTreePageMax = 1 << 15;
 size_t tree_workspace(const KvCacheArgs &c, int heads, int rows, int max_rows, int max_keys);
 hipError_t launch_attn_tree(const TreeArgs &a, hipStream_t s);
+
+// ---- pages of the cache
+
+// The pools of all layers, by value: what one launch works on.
+constexpr int kLayersMax = 64;
+struct KvLayers {
+    void *k[kLayersMax], *v[kLayersMax];
+    float *k_scale[kLayersMax], *v_scale[kLayersMax];
+};
+struct PagesArgs {
+    int *table = nullptr;  // [streams][table_stride]
+    int table_stride = 0, streams = 0;
+    int *refs = nullptr;  // [n_pages]
+    int n_pages = 0, page_size = 0;
+};
+struct ForkArgs {
+    PagesArgs p;
+    const int *parent = nullptr, *len = nullptr;
+    int *ws = nullptr;
+};
+size_t fork_workspace(const PagesArgs &p);
+hipError_t launch_kv_fork(const ForkArgs &a, hipStream_t s);
+
+struct ReserveArgs {
+    PagesArgs p;
+    int layers = 0, heads = 0, vec_bytes = 0;  // vec_bytes: of one head of one position
+    bool scales = false;
+    const int *row_start = nullptr, *ctx_len = nullptr;
+    int max_rows = 0;
+    int *ok = nullptr;
+    void *ws = nullptr;
+};
+size_t reserve_workspace(const PagesArgs &p, int max_rows);
+hipError_t launch_kv_reserve(const ReserveArgs &a, const KvLayers &l, hipStream_t s);
+
+struct CompactArgs {
+    KvCacheArgs c;  // of one layer: its shape and the table
+    int layers = 0, vec_bytes = 0;
+    const int *row_start = nullptr, *ctx_len = nullptr, *kept = nullptr;
+    int rows = 0, max_rows = 0;
+};
+hipError_t launch_kv_compact(const CompactArgs &a, const KvLayers &l, hipStream_t s);
+
+// ---- verification of drafted tokens
+
+struct VerifyArgs {
+    const void *x = nullptr, *y = nullptr;  // logits [rows][vocab] of the target, and of the draft or null
+    int dtype = ELEM_F32;
+    int64_t x_row = 0, y_row = 0;  // row strides in elements
+    int rows = 0, vocab = 0;
+    const int *tokens = nullptr, *row_start = nullptr;
+    const uint64_t *row_mask = nullptr;
+    int streams = 0, max_rows = 0;
+    const double *uniforms = nullptr;
+    float inv_t = 1.0f, draft_inv_t = 1.0f;
+    bool greedy = false;
+    int *accepted = nullptr, *path = nullptr, *next = nullptr;
+    void *ws = nullptr;
+};
+size_t verify_workspace(int streams, int max_rows, int vocab, bool draft);
+hipError_t launch_verify(const VerifyArgs &a, hipStream_t s);
+
+// ---- low-rank adapters beside a projection
+
+struct AdapterArgs {
+    const void *a = nullptr, *b = nullptr;  // fp16 [n][max_rank][cols], [n][out][max_rank]
+    const int *rank = nullptr;   // [n], null: max_rank
+    const float *scale = nullptr;  // [n], null: 1
+    int n = 0, max_rank = 0, cols = 0, out = 0;
+    const void *x = nullptr, *base = nullptr;
+    void *y = nullptr;
+    int x_dtype = ELEM_F32, y_dtype = ELEM_F32;
+    int64_t x_row = 0, base_row = 0, y_row = 0;  // row strides in elements
+    const int *which = nullptr;  // [rows]
+    int rows = 0;
+};
+constexpr int kAdapterRankMax = 128;
+hipError_t launch_adapter_rows(const AdapterArgs &a, hipStream_t s);
 
 }  // namespace mh

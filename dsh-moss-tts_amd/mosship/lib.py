@@ -42,6 +42,9 @@ EXPORTED = [
     "moss_hip_rope_freqs", "moss_hip_rope_rows", "moss_hip_kv_write", "moss_hip_kv_read",
     "moss_hip_attn_tree", "moss_hip_attn_tree_workspace",
     "moss_hip_token_logprobs", "moss_hip_token_logprobs_workspace",
+    "moss_hip_verify_tokens", "moss_hip_verify_tokens_workspace",
+    "moss_hip_kv_fork", "moss_hip_kv_fork_workspace", "moss_hip_kv_reserve", "moss_hip_kv_reserve_workspace",
+    "moss_hip_kv_compact", "moss_hip_adapter_rows",
     "moss_hip_codec_create", "moss_hip_codec_create_from_file", "moss_hip_codec_destroy",
     "moss_hip_codec_samples_per_frame", "moss_hip_codec_reset_stream", "moss_hip_codec_decode_chunk",
     "moss_hip_codec_decode", "moss_hip_codec_last_ms", "moss_hip_codec_stage_ms",
@@ -93,6 +96,18 @@ class KVCacheStruct(C.Structure):
     _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
                 ("kv_dtype", C.c_int), ("kv_heads", C.c_int), ("head_dim", C.c_int), ("page_size", C.c_int),
                 ("n_pages", C.c_int), ("page_table", C.c_void_p), ("table_stride", C.c_int), ("streams", C.c_int)]
+
+
+class KVPagesStruct(C.Structure):
+    """moss_hip_kv_pages."""
+    _fields_ = [("page_table", C.c_void_p), ("table_stride", C.c_int), ("streams", C.c_int), ("refs", C.c_void_p),
+                ("n_pages", C.c_int), ("page_size", C.c_int)]
+
+
+class AdaptersStruct(C.Structure):
+    """moss_hip_adapters."""
+    _fields_ = [("a", C.c_void_p), ("b", C.c_void_p), ("rank", C.c_void_p), ("scale", C.c_void_p), ("n_adapters", C.c_int),
+                ("max_rank", C.c_int), ("cols", C.c_int), ("out", C.c_int)]
 
 
 FRAME_CB = C.CFUNCTYPE(None, C.c_void_p, C.c_int, C.POINTER(C.c_int32))
@@ -162,6 +177,14 @@ def load(path: str = LIB_PATH) -> C.CDLL:
     L.moss_hip_attn_tree_workspace.argtypes = [vp, i32, i32, i32, i32, C.POINTER(sz)]
     L.moss_hip_token_logprobs.argtypes = [vp, i64, i32, i32, i32, vp, f32, vp, vp, i32, vp, vp, vp, sz, vp]
     L.moss_hip_token_logprobs_workspace.argtypes = [i32, i32, i32, C.POINTER(sz)]
+    L.moss_hip_verify_tokens.argtypes = [vp, i64, i32, vp, i64, i32, i32, vp, vp, vp, i32, i32, vp, f32, f32, i32, vp, vp, vp, vp, sz, vp]
+    L.moss_hip_verify_tokens_workspace.argtypes = [i32, i32, i32, i32, C.POINTER(sz)]
+    L.moss_hip_kv_fork.argtypes = [vp, vp, vp, vp, sz, vp]
+    L.moss_hip_kv_fork_workspace.argtypes = [vp, C.POINTER(sz)]
+    L.moss_hip_kv_reserve.argtypes = [vp, vp, i32, vp, vp, i32, vp, vp, sz, vp]
+    L.moss_hip_kv_reserve_workspace.argtypes = [vp, i32, C.POINTER(sz)]
+    L.moss_hip_kv_compact.argtypes = [vp, i32, vp, vp, vp, i32, i32, vp]
+    L.moss_hip_adapter_rows.argtypes = [vp, i64, i32, vp, vp, i32, vp, i64, vp, i64, i32, vp]
     L.moss_hip_codec_create.argtypes = [vp, C.c_size_t, C.POINTER(CodecOptions), C.POINTER(vp)]
     L.moss_hip_codec_create_from_file.argtypes = [C.c_char_p, C.POINTER(CodecOptions), C.POINTER(vp)]
     L.moss_hip_codec_destroy.argtypes = [vp]
@@ -510,6 +533,160 @@ def token_logprobs(logits, tokens, logprob, entropy=None, top_ids=None, top_logp
                                          _whole("top_ids", top_ids, _torch.int32, (rows, k), dev, optional=True),
                                          _whole("top_logprobs", top_logprobs, _torch.float32, (rows, k), dev, optional=True),
                                          wp, wb, on))
+
+
+def verify_tokens_workspace(streams: int, max_rows: int, vocab: int, draft: bool = False) -> int:
+    """Bytes of workspace verify_tokens takes (draft: with draft_logits)."""
+    n = C.c_size_t(0)
+    check(load().moss_hip_verify_tokens_workspace(streams, max_rows, vocab, int(draft), C.byref(n)))
+    return n.value
+
+
+def verify_tokens(logits, tokens, row_start, accepted, path, next_token, max_rows: int, uniforms=None, draft_logits=None, row_mask=None,
+                  inv_temperature: float = 1.0, draft_inv_temperature: float | None = None, greedy: bool = False, workspace=None,
+                  stream=None) -> None:
+    """moss_hip_verify_tokens: drafted tokens [rows] int32 under the target's logits [rows][vocab] (float32 or float16, any row
+    stride), into accepted and next_token [streams] and path [rows] int32.
+
+    row_start [streams + 1] int32; uniforms [rows] float64 (None: greedy); draft_logits [rows][vocab] of the same type, of chains
+    drawn from them, at draft_inv_temperature (inv_temperature by default); row_mask [rows] int64 as attn_tree takes it,
+    None: chains."""
+    dev, shape = logits.get_device(), logits.shape
+    on = _on(dev, stream)
+    if len(shape) != 2:
+        raise ValueError("logits [rows][vocab] are wanted")
+    rows, vocab = shape
+    streams = accepted.shape[0]
+    if streams == 0:
+        return
+    dp, ds = None, 0
+    if draft_logits is not None:
+        if draft_logits.shape != shape or draft_logits.dtype is not logits.dtype or draft_logits.get_device() != dev:
+            raise ValueError("draft_logits must have the shape, type and device of logits")
+        dp, ds = draft_logits.data_ptr(), draft_logits.stride(0)
+    if vocab > 1 and (logits.stride(1) != 1 or (dp is not None and draft_logits.stride(1) != 1)):
+        raise ValueError("the logits of a row must be contiguous")
+    wp, wb = _workspace(workspace, lambda: verify_tokens_workspace(streams, max_rows, vocab, dp is not None), dev, stream)
+    i32 = _torch.int32
+    check(load().moss_hip_verify_tokens(logits.data_ptr(), logits.stride(0), _types(logits), dp, ds, rows, vocab,
+                                        _whole("tokens", tokens, i32, (rows,), dev), _whole("row_start", row_start, i32, (streams + 1,), dev),
+                                        _whole("row_mask", row_mask, _torch.int64, (rows,), dev, optional=True), streams, max_rows,
+                                        _whole("uniforms", uniforms, _torch.float64, (rows,), dev, optional=True), inv_temperature,
+                                        inv_temperature if draft_inv_temperature is None else draft_inv_temperature, int(greedy),
+                                        _whole("accepted", accepted, i32, (streams,), dev), _whole("path", path, i32, (rows,), dev),
+                                        _whole("next_token", next_token, i32, (streams,), dev), wp, wb, on))
+
+
+class KVPages:
+    """The pages behind a block table as the calls take them (moss_hip_kv_pages): page_table [streams][pages of a stream] and refs
+    [n_pages], int32.  Keeps the tensors, owns nothing else."""
+
+    def __init__(self, page_table, refs, page_size: int):
+        import torch
+        if page_table.dim() != 2 or refs.dim() != 1:
+            raise ValueError("a table [streams][pages] and refs [n_pages] are wanted")
+        self.tensors, self.device = (page_table, refs), refs.get_device()
+        self.streams = page_table.shape[0]
+        self.struct = KVPagesStruct(_whole("page_table", page_table, torch.int32, tuple(page_table.shape), self.device), page_table.shape[1],
+                                    page_table.shape[0], _whole("refs", refs, torch.int32, (refs.numel(),), self.device), refs.numel(), page_size)
+        self.ref = C.addressof(self.struct)
+
+
+class KVLayers:
+    """The caches of a model's layers, of one shape and over one block table, for the calls that work on all of them."""
+
+    def __init__(self, caches):
+        self.caches = list(caches)
+        if not self.caches:
+            raise ValueError("at least one cache is wanted")
+        self.device, self.streams = self.caches[0].device, self.caches[0].streams
+        if any(c.device != self.device for c in self.caches):
+            raise ValueError("the caches must be on one device")
+        self.structs = (KVCacheStruct * len(self.caches))(*(c.struct for c in self.caches))
+        self.ref = C.addressof(self.structs)
+
+
+def kv_fork_workspace(pages: KVPages) -> int:
+    """Bytes of workspace kv_fork takes."""
+    n = C.c_size_t(0)
+    check(load().moss_hip_kv_fork_workspace(pages.ref, C.byref(n)))
+    return n.value
+
+
+def kv_fork(pages: KVPages, parent, len=None, workspace=None, stream=None) -> None:
+    """moss_hip_kv_fork: stream s becomes the first len[s] positions (int32; None: all) of stream parent[s] (int32; -1: of none)."""
+    dev, i32, n = pages.device, _t().int32, (pages.streams,)
+    on = _on(dev, stream)
+    if pages.streams == 0:
+        return
+    wp, wb = _workspace(workspace, lambda: kv_fork_workspace(pages), dev, stream)
+    check(load().moss_hip_kv_fork(pages.ref, _whole("parent", parent, i32, n, dev), _whole("len", len, i32, n, dev, optional=True), wp, wb, on))
+
+
+def kv_reserve_workspace(pages: KVPages, max_rows: int) -> int:
+    """Bytes of workspace kv_reserve takes."""
+    n = C.c_size_t(0)
+    check(load().moss_hip_kv_reserve_workspace(pages.ref, max_rows, C.byref(n)))
+    return n.value
+
+
+def kv_reserve(pages: KVPages, layers: KVLayers, row_start, ctx_len, ok, max_rows: int, workspace=None, stream=None) -> None:
+    """moss_hip_kv_reserve: pages for row_start[s + 1] - row_start[s] new positions of stream s behind its ctx_len[s] (int32), into
+    the block table and refs; ok [streams] int32: which streams have theirs."""
+    dev, i32, s = pages.device, _t().int32, pages.streams
+    on = _on(dev, stream)
+    if layers.device != dev:
+        raise ValueError("the layers must be on the pages' device")
+    if s == 0:
+        return
+    wp, wb = _workspace(workspace, lambda: kv_reserve_workspace(pages, max_rows), dev, stream)
+    check(load().moss_hip_kv_reserve(pages.ref, layers.ref, len(layers.caches), _whole("row_start", row_start, i32, (s + 1,), dev),
+                                     _whole("ctx_len", ctx_len, i32, (s,), dev), max_rows, _whole("ok", ok, i32, (s,), dev), wp, wb, on))
+
+
+def kv_compact(layers: KVLayers, row_start, ctx_len, kept, max_rows: int, stream=None) -> None:
+    """moss_hip_kv_compact: position ctx_len[s] + j becomes what ctx_len[s] + kept[row_start[s] + j] was, in all layers."""
+    dev, i32, s = layers.device, _t().int32, layers.streams
+    on = _on(dev, stream)
+    rows = kept.shape[0]
+    if rows == 0:
+        return
+    check(load().moss_hip_kv_compact(layers.ref, len(layers.caches), _whole("row_start", row_start, i32, (s + 1,), dev),
+                                     _whole("ctx_len", ctx_len, i32, (s,), dev), _whole("kept", kept, i32, (rows,), dev), rows, max_rows, on))
+
+
+class Adapters:
+    """Low-rank adapters as the calls take them (moss_hip_adapters): a [n][max_rank][cols] and b [n][out][max_rank] float16,
+    rank [n] int32 (None: max_rank), scale [n] float32 (None: 1).  Keeps the tensors, owns nothing else."""
+
+    def __init__(self, a, b, rank=None, scale=None):
+        import torch
+        if a.dim() != 3 or b.dim() != 3:
+            raise ValueError("a [n][max_rank][cols] and b [n][out][max_rank] are wanted")
+        (n, top, cols), out = a.shape, b.shape[1]
+        self.tensors, self.device, self.cols, self.out = (a, b, rank, scale), a.get_device(), cols, out
+        self.struct = AdaptersStruct(
+            _whole("a", a, torch.float16, (n, top, cols), self.device), _whole("b", b, torch.float16, (n, out, top), self.device),
+            _whole("rank", rank, torch.int32, (n,), self.device, optional=True),
+            _whole("scale", scale, torch.float32, (n,), self.device, optional=True), n, top, cols, out)
+        self.ref = C.addressof(self.struct)
+
+
+def adapter_rows(x, adapters: Adapters, adapter, out, base=None, stream=None) -> None:
+    """moss_hip_adapter_rows: out[r] = base[r] + scale B (A x[r]) of adapter[r] (int32; -1: none), rows of float32 or float16;
+    base: out itself by default."""
+    dev, base = adapters.device, out if base is None else base
+    on = _on(dev, stream)
+    rows = x.shape[0]
+    if out.shape[0] != rows or base.shape[0] != rows or base.dtype is not out.dtype:
+        raise ValueError("x, base and out must have the same rows, base and out one type")
+    if rows == 0:
+        return
+    xp, xs = _rows("x", x, 1, adapters.cols, dev)
+    bp, bs = _rows("base", base, 1, adapters.out, dev)
+    op, os_ = _rows("out", out, 1, adapters.out, dev)
+    check(load().moss_hip_adapter_rows(xp, xs, _types(x), adapters.ref, _whole("adapter", adapter, _torch.int32, (rows,), dev), rows,
+                                       bp, bs, op, os_, _types(out), on))
 
 
 # ---------------------------------------------------------------- model

@@ -469,6 +469,89 @@ int moss_hip_token_logprobs(const void *logits, int64_t row_stride, int dtype, i
                             float *top_logprobs, void *workspace, size_t workspace_bytes, void *stream);
 int moss_hip_token_logprobs_workspace(int rows, int vocab, int top_k, size_t *bytes);
 
+/* Drafted tokens against the target's probabilities p = softmax(logits * inv_temperature), from the random numbers given.
+ * Stream s has rows row_start[s] .. row_start[s + 1] - 1 (n of them; those past max_rows <= 64 take no part), its nodes: row 0
+ * is the last committed token, the others were drafted.  logits [rows][vocab] (dtype F32 or F16, row stride in elements) are
+ * the target's after each node.  A node's parent is the row before it (row_mask NULL: a chain), or, of the row_mask that
+ * moss_hip_attn_tree takes (its ancestors and itself), the highest ancestor; a node whose mask lacks its own bit, or
+ * has no ancestor, is never accepted.  From row 0 on, the walk goes to the first child that is accepted:
+ *   draft_logits given (chains only): node i is accepted where u_i q(t_i) < p(t_i), with q = softmax(draft_logits * draft_inv_temperature)
+ *     of its parent's row, which it was drawn from; the token behind a rejected one is drawn from max(p - q, 0).
+ *   draft_logits NULL: the tokens were picked outright.  Of a node's children, in the order of their rows, c is accepted
+ *     where u_c (1 - p of the different tokens rejected before it) < p(t_c); the token behind them is drawn from p without the
+ *     rejected tokens.  A child whose token an earlier one had is rejected.
+ *   greedy: accepted where it is the likeliest (of equal logits the lowest index; NaN is none), which also follows.
+ * uniforms [rows]: u of each node, numbers of [0, 1) (others count as the nearest of 0 and 1, NaN as 1); row 0's draws the next token: the
+ * first whose cumulative sum, in the order of the vocabulary, passes u times the whole.  Where nothing is left over,
+ * it is drawn from p.  Probabilities are formed and summed in 64 bits.  greedy takes no uniforms and no draft_logits.
+ *   accepted [streams]: drafted nodes accepted.
+ *   path [rows]: entry row_start[s] + j is the node that the walk took as its j-th (0 first), -1 past the last: what
+ *     moss_hip_kv_compact takes.  Rows of no stream, and a stream's rows past max_rows, stay as they were.
+ *   next_token [streams]: the token behind the last node of the path.
+ * -inf logits are ruled out.  A row with a NaN or +inf, or of nothing but -inf, is no distribution: no child of it is
+ * accepted, and no token (-1) follows; a draft's row like that rejects its child and the next token is drawn from p.  A token
+ * outside [0, vocab) is rejected.  Without rows, or with a row range not within [0, rows], a stream has accepted 0 and
+ * next_token -1.  vocab <= 2^20.  workspace as above: moss_hip_verify_tokens_workspace bytes (draft: whether draft_logits are given). */
+int moss_hip_verify_tokens(const void *logits, int64_t row_stride, int dtype, const void *draft_logits, int64_t draft_stride,
+                           int rows, int vocab, const int32_t *tokens, const int32_t *row_start, const uint64_t *row_mask,
+                           int streams, int max_rows, const double *uniforms, float inv_temperature, float draft_inv_temperature,
+                           int greedy, int32_t *accepted, int32_t *path, int32_t *next_token, void *workspace,
+                           size_t workspace_bytes, void *stream);
+int moss_hip_verify_tokens_workspace(int streams, int max_rows, int vocab, int draft, size_t *bytes);
+
+/* The pages behind the block table, shared between streams.  A page is free where refs is 0; each table entry that names it
+ * holds it once, and a caller may hold pages itself by adding to refs (a prompt kept for later streams).  Entries outside
+ * [0, n_pages) name no page; the calls write -1 there.  All layers of a model go by the same table. */
+typedef struct {
+    int32_t *page_table; /* [streams][table_stride] */
+    int table_stride, streams;
+    int32_t *refs; /* [n_pages] */
+    int n_pages;
+    int page_size; /* a multiple of 16, at most 32768 */
+} moss_hip_kv_pages;
+
+/* Stream s becomes the first len[s] positions of what stream parent[s] was before the call: it shares those pages, and gives up
+ * its own that are not among them.  One call does a reordering of beams, new streams over a prompt (parent[s] = p), cuts
+ * (parent[s] = s) and ends (parent[s] outside [0, streams), or len[s] <= 0).  len NULL: whole streams.  streams * table_stride <= 2^26.
+ * workspace: moss_hip_kv_fork_workspace bytes. */
+int moss_hip_kv_fork(const moss_hip_kv_pages *pages, const int32_t *parent, const int32_t *len, void *workspace,
+                     size_t workspace_bytes, void *stream);
+int moss_hip_kv_fork_workspace(const moss_hip_kv_pages *pages, size_t *bytes);
+
+/* Pages for rows that are about to be written: those of stream s, n = row_start[s + 1] - row_start[s] (at most max_rows), go to
+ * positions ctx_len[s] .. ctx_len[s] + n - 1.  Pages that are missing there are taken from the free ones, the lowest first; a page that
+ * others hold too is replaced by one of the stream's own, into which its positions below ctx_len[s] are copied in every
+ * layer (K, V and scales).  Streams are served in their order, so that of a page that several of them write the last one keeps it
+ * where nobody else holds it.  ok [streams]: 1, or 0 where the stream's rows have no places (ctx_len negative, more than
+ * max_rows, past the table) or too few pages are left for it: then it, and every later stream that needs one, gets
+ * none, and its entries stay.  layers: n_layers <= 64 caches of one shape over this table.  workspace:
+ * moss_hip_kv_reserve_workspace bytes. */
+int moss_hip_kv_reserve(const moss_hip_kv_pages *pages, const moss_hip_kv_cache *layers, int n_layers, const int32_t *row_start,
+                        const int32_t *ctx_len, int max_rows, int32_t *ok, void *workspace, size_t workspace_bytes, void *stream);
+int moss_hip_kv_reserve_workspace(const moss_hip_kv_pages *pages, int max_rows, size_t *bytes);
+
+/* Accepted rows to their final positions: position ctx_len[s] + j of stream s becomes what ctx_len[s] + kept[row_start[s] + j] was
+ * before the call, for j < row_start[s + 1] - row_start[s] (at most max_rows <= 64), in every layer's K, V and scales, bit for bit.  kept
+ * [rows] are row numbers within the stream; where one is negative or not below the stream's rows, or a position has no
+ * place in the cache, the position stays as it was.  Streams must not share the pages that they write. */
+int moss_hip_kv_compact(const moss_hip_kv_cache *layers, int n_layers, const int32_t *row_start, const int32_t *ctx_len,
+                        const int32_t *kept, int rows, int max_rows, void *stream);
+
+/* Low-rank adapters of many requests, beside a projection that they share (moss_hip_gemm_q8x4, moss_hip_gemv_q8x4):
+ *   y[r] = base[r] + scale_a B_a (A_a x[r]),  a = adapter[r];  y[r] = base[r] for an adapter outside [0, n_adapters).
+ * x [rows][cols] of x_dtype, base and y [rows][out] of y_dtype (F32 or F16), row strides in elements; y may be base itself (same
+ * stride), and must not overlap x, or base otherwise.  Weights and rows are multiplied exactly, with 32-bit rows held to 22 bits of the
+ * largest in 128 neighbouring columns; sums are held in 32 bits and y is rounded once. */
+typedef struct {
+    const void *a, *b;    /* fp16 [n_adapters][max_rank][cols] and [n_adapters][out][max_rank], 16-byte aligned */
+    const int32_t *rank;  /* [n_adapters], each within 0 .. max_rank (others count as the nearest); NULL: max_rank.  Weights past it may hold anything */
+    const float *scale;   /* [n_adapters]; NULL: 1 */
+    int n_adapters, max_rank; /* max_rank a multiple of 16, at most 128 */
+    int cols, out;        /* multiples of 32 and of 16, at most 65536 */
+} moss_hip_adapters;
+int moss_hip_adapter_rows(const void *x, int64_t x_stride, int x_dtype, const moss_hip_adapters *adapters, const int32_t *adapter,
+                          int rows, const void *base, int64_t base_stride, void *y, int64_t y_stride, int y_dtype, void *stream);
+
 /* ---- Audio codec decoder (codes -> 48 kHz stereo PCM) --------------------------------
  * The GPU replacement of moss::AudioDecoder (reference csrc/include/moss/decoder.h:14-83,
  * csrc/src/decoder.cpp:26-281): the MOSS-Audio-Tokenizer-Nano decoder of a decoder .moss
