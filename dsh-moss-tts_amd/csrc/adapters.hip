@@ -2,6 +2,18 @@
 //
 // y_r = base_r + s_a B_a (A_a x_r), with a = which[r] the row's own adapter, A_a of rank x cols and B_a of
 // out x rank.  Rows without an adapter are base_r.
+//
+// One launch: a workgroup takes a tile of 16 or 32 neighbouring rows and one of the adapters among them, forms
+// t = A x for the tile's rows of that adapter, and goes from there to its share of the outputs; t stays on the
+// chip.  Both products are matrix instructions with the weights as the one operand and the rows as the other, so
+// a lane keeps one row throughout: what scales a row is one number of the lane.  With one row of an adapter, 15
+// of 16 columns of a product idle; the instructions are still fewer than the vector unit would need.
+//
+// Weights are fp16.  fp16 rows are multiplied as they are.  32-bit rows, and t, go in as two fp16 numbers, hi + lo,
+// 22 bits: of 128 columns of a row (of all ranks of t) the largest is put at 2^14 by a power of two, which leaves
+// 2^-39 of the largest as the finest step, and the power is taken out again in 32 bits.  The matrix
+// instructions cut their sums towards zero, so no more than 8 of them go into one sum before it is added up in 32
+// bits with rounding.  A row's sums do not depend on where in a tile it stands, nor on the other rows.
 #include <algorithm>
 
 #include "paged_ops.h"
@@ -9,64 +21,268 @@
 namespace mh {
 namespace {
 
-constexpr int kThreads = 256;
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+
+constexpr int kSlices = 4;    // of the columns: a wave each
+constexpr int kChunk = 128;   // columns under one power of two
+constexpr int kTPitch = 17;   // of t in LDS, 16 rows wide
 
 template <class T>
-__device__ __forceinline__ float get(const T *p) {
+__device__ __forceinline__ float get(T x) {
     if constexpr (sizeof(T) == 2)
-        return __half2float(*(const __half *)p);
+        return __half2float(x);
     else
-        return *p;
-}
-template <class T>
-__device__ __forceinline__ void put(T *p, float x) {
-    if constexpr (sizeof(T) == 2)
-        *p = __float2half_rn(x);
-    else
-        *p = x;
+        return x;
 }
 
-// A workgroup a row and a share of its outputs.
-template <class X, class Y>
-__global__ __launch_bounds__(kThreads) void adapter_kernel(AdapterArgs a) {
-    __shared__ float t[kAdapterRankMax];
-    const int r = blockIdx.x, w = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const int id = a.which[r];
-    const bool has = id >= 0 && id < a.n;
-    const int rank = !has ? 0 : (a.rank == nullptr ? a.max_rank : min(max(a.rank[id], 0), a.max_rank));
-    const X *x = (const X *)a.x + r * a.x_row;
-    for (int k = w; k < rank; k += kThreads / 64) {
-        const __half *row = (const __half *)a.a + ((size_t)id * a.max_rank + k) * a.cols;
-        float sum = 0.0f;
-        for (int c = lane; c < a.cols; c += 64) sum = fmaf(get(x + c), __half2float(row[c]), sum);
-        sum = wave_sum(sum);
-        if (lane == 0) t[k] = sum;
+union Frag {
+    uint4 u;
+    half8 h;
+    __half e[8];
+};
+
+// The power of two that puts `top` at 2^14 .. 2^15, and its reciprocal; 1 where there is none.
+struct Power {
+    float up, down;
+};
+__device__ __forceinline__ Power power_of(float top) {
+    const int e = (int)(__float_as_uint(top) >> 23);  // biased exponent of a number >= 0
+    if (e == 0 && top == 0.0f) return Power{1.0f, 1.0f};
+    if (e == 255) return Power{1.0f, 1.0f};
+    const int up = min(127 + 14 + 127 - e, 253);
+    return Power{__uint_as_float((unsigned)up << 23), __uint_as_float((unsigned)(254 - up) << 23)};
+}
+// 8 values times a power of two as hi + lo.
+__device__ __forceinline__ void split8(const float (&x)[8], float up, Frag &hi, Frag &lo) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float v = x[i] * up;
+        hi.e[i] = __float2half_rn(v);
+        lo.e[i] = __float2half_rn(v - __half2float(hi.e[i]));
     }
-    __syncthreads();
-    const float scale = !has || a.scale == nullptr ? 1.0f : a.scale[id];
-    for (int o = blockIdx.y * kThreads + threadIdx.x; o < a.out; o += gridDim.y * kThreads) {
-        float sum = 0.0f;
-        if (has) {
-            const __half *row = (const __half *)a.b + ((size_t)id * a.out + o) * a.max_rank;
-            for (int k = 0; k < rank; ++k) sum = fmaf(t[k], __half2float(row[k]), sum);
+}
+__device__ __forceinline__ float row_max(float v) {  // over the lanes of one row
+    v = fmaxf(v, xshfl<16>(v));
+    return fmaxf(v, xshfl<32>(v));
+}
+
+// 8 elements of a row at any address that an element may have.
+template <class X>
+__device__ __forceinline__ void load8(const X *p, uint4 (&raw)[sizeof(X) / 2]) {
+    __builtin_memcpy(raw, p, sizeof(raw));
+}
+
+// RK: ranks of 16 that max_rank has; RT: tiles of 16 rows.
+template <class X, class Y, int RK, int RT>
+__global__ __launch_bounds__(64 * kSlices * RT) void adapter_kernel(AdapterArgs a, int outs_each) {
+    constexpr int kWaves = kSlices * RT, kThreads = 64 * kWaves;
+    constexpr int KS = RK == 1 ? 1 : RK / 2;  // steps of 32 ranks (RK 1: one half of a step)
+    constexpr int kTop = 32 * KS;
+    __shared__ float part[RT][kSlices][16 * RK][kTPitch];
+    const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6);
+    const int m = lane & 15, g = lane >> 4;
+    const int row0 = blockIdx.x * 16 * RT;
+    const int out0 = blockIdx.z * outs_each, out1 = min(out0 + outs_each, a.out);
+    // the tile's adapters: this workgroup takes the blockIdx.y-th and so on
+    int id = -2;
+    if (lane < 16 * RT && row0 + lane < a.rows) {
+        id = a.which[row0 + lane];
+        if (id < 0 || id >= a.n) id = -1;
+    }
+    uint64_t todo = __ballot(id != -2);
+    for (int j = 0; todo; ++j) {
+        const int mine = __builtin_amdgcn_readlane(id, __builtin_ctzll(todo));
+        const uint64_t who = __ballot(id == mine);
+        todo &= ~who;
+        if (j % gridDim.y != blockIdx.y) continue;
+        const int rank = mine < 0 ? 0 : (a.rank == nullptr ? a.max_rank : min(max(a.rank[mine], 0), a.max_rank));
+        if (rank == 0) {  // y is base
+            if (a.y == a.base) continue;
+            const int units = (out1 - out0) * (int)sizeof(Y) / 16;
+            for (int r = w; r < 16 * RT; r += kWaves) {
+                if (!(who >> r & 1)) continue;
+                const char *from = (const char *)((const Y *)a.base + (row0 + r) * a.base_row + out0);
+                char *to = (char *)((Y *)a.y + (row0 + r) * a.y_row + out0);
+                for (int u = lane; u < units; u += 64) {
+                    uint4 v;
+                    __builtin_memcpy(&v, from + 16 * u, 16);
+                    __builtin_memcpy(to + 16 * u, &v, 16);
+                }
+            }
+            continue;
         }
-        const float base = get((const Y *)a.base + r * a.base_row + o);
-        put((Y *)a.y + r * a.y_row + o, has ? fmaf(scale, sum, base) : base);
+        const float scale = a.scale == nullptr ? 1.0f : a.scale[mine];
+        // t = A x: a wave one tile of rows and a quarter of the chunks of columns
+        {
+            const int rt = w / kSlices, sl = w % kSlices;
+            const bool has = who >> (16 * rt + m) & 1;
+            f32x4_t sum[RK] = {};
+            if (who >> (16 * rt) & 0xffff) {
+                const X *x = (const X *)a.x + (row0 + 16 * rt + (has ? m : 0)) * a.x_row + 8 * g;
+                const __half *wa = (const __half *)a.a + ((size_t)mine * a.max_rank + m) * a.cols + 8 * g;
+                for (int c = kChunk * sl; c < a.cols; c += kChunk * kSlices) {
+                    uint4 raw[4][sizeof(X) / 2];
+#pragma unroll
+                    for (int s = 0; s < 4; ++s) {
+#pragma unroll
+                        for (int i = 0; i < (int)sizeof(X) / 2; ++i) raw[s][i] = uint4{};
+                        if (has && c + 32 * s < a.cols) load8(x + c + 32 * s, raw[s]);
+                    }
+                    f32x4_t acc[RK] = {};
+                    float down = 1.0f;
+                    if constexpr (sizeof(X) == 2) {
+#pragma unroll
+                        for (int s = 0; s < 4; ++s) {
+                            if (c + 32 * s >= a.cols) break;
+                            const Frag v{raw[s][0]};
+#pragma unroll
+                            for (int k = 0; k < RK; ++k) {
+                                Frag f{uint4{}};
+                                if (16 * k + m < rank) f.u = *(const uint4 *)(wa + (size_t)16 * k * a.cols + c + 32 * s);
+                                acc[k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.h, v.h, acc[k], 0, 0, 0);
+                            }
+                        }
+                    } else {
+                        float v[4][8], top = 0.0f;
+#pragma unroll
+                        for (int s = 0; s < 4; ++s) {
+                            __builtin_memcpy(v[s], raw[s], sizeof(v[s]));
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[s][i]));
+                        }
+                        const Power p = power_of(row_max(top));
+                        down = p.down;
+#pragma unroll
+                        for (int s = 0; s < 4; ++s) {
+                            if (c + 32 * s >= a.cols) break;
+                            Frag hi, lo;
+                            split8(v[s], p.up, hi, lo);
+#pragma unroll
+                            for (int k = 0; k < RK; ++k) {
+                                Frag f{uint4{}};
+                                if (16 * k + m < rank) f.u = *(const uint4 *)(wa + (size_t)16 * k * a.cols + c + 32 * s);
+                                acc[k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.h, hi.h, acc[k], 0, 0, 0);
+                                acc[k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.h, lo.h, acc[k], 0, 0, 0);
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int k = 0; k < RK; ++k)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) sum[k][i] = fmaf(acc[k][i], down, sum[k][i]);
+                }
+            }
+            __syncthreads();  // (the last adapter's t is no longer read)
+#pragma unroll
+            for (int k = 0; k < RK; ++k)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) part[rt][sl][16 * k + 4 * g + i][m] = sum[k][i];
+        }
+        __syncthreads();
+        // this lane's row of t in each tile: the operands of B t
+        Frag hi[RT][KS], lo[RT][KS];
+        float factor[RT];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            float v[KS][8], top = 0.0f;
+#pragma unroll
+            for (int s = 0; s < KS; ++s)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int k = 32 * s + 8 * g + i;
+                    v[s][i] = 0.0f;
+                    if (k < 16 * RK) v[s][i] = (part[rt][0][k][m] + part[rt][1][k][m]) + (part[rt][2][k][m] + part[rt][3][k][m]);
+                    top = fmaxf(top, fabsf(v[s][i]));
+                }
+            const Power p = power_of(row_max(top));
+            factor[rt] = p.down * scale;
+#pragma unroll
+            for (int s = 0; s < KS; ++s) split8(v[s], p.up, hi[rt][s], lo[rt][s]);
+        }
+        // B t: a wave 64 outputs of all rows
+        constexpr int P = 16 / (int)sizeof(Y);  // outputs of a lane that lie together: output i of tile q is the lane's q * 4 + i-th
+        for (int o = out0 + 64 * w; o < out1; o += 64 * kWaves) {
+            f32x4_t acc[RT][4] = {};
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                // row m of the product's tile q is this output
+                const int at = P == 4 ? o + 16 * q + m : o + 32 * (q >> 1) + 8 * (m >> 2) + 4 * (q & 1) + (m & 3);
+                const __half *wb = (const __half *)a.b + ((size_t)mine * a.out + min(at, a.out - 1)) * a.max_rank + 8 * g;
+#pragma unroll
+                for (int s = 0; s < KS; ++s) {
+                    const int k = 32 * s + 8 * g;
+                    Frag f{uint4{}};
+                    if (k < rank) {
+                        f.u = *(const uint4 *)(wb + 32 * s);
+                        if (k + 8 > rank) {  // what stands behind the rank may be anything
+#pragma unroll
+                            for (int i = 0; i < 8; ++i)
+                                if (k + i >= rank) f.e[i] = __half(0.0f);
+                        }
+                    }
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt) {
+                        acc[rt][q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.h, hi[rt][s].h, acc[rt][q], 0, 0, 0);
+                        acc[rt][q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.h, lo[rt][s].h, acc[rt][q], 0, 0, 0);
+                    }
+                }
+            }
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+                if (!(who >> (16 * rt + m) & 1)) continue;
+                const int64_t r = row0 + 16 * rt + m;
+#pragma unroll
+                for (int q = 0; q < 16 / P; ++q) {
+                    const int at = P == 4 ? o + 16 * q + 4 * g : o + 32 * q + 8 * g;
+                    if (at >= out1) continue;
+                    Y v[P];
+                    __builtin_memcpy(v, (const Y *)a.base + r * a.base_row + at, 16);
+#pragma unroll
+                    for (int i = 0; i < P; ++i) {
+                        const float y = fmaf(acc[rt][q * (P / 4) + i / 4][i & 3], factor[rt], get(v[i]));
+                        if constexpr (sizeof(Y) == 2)
+                            v[i] = __float2half_rn(y);
+                        else
+                            v[i] = y;
+                    }
+                    __builtin_memcpy((Y *)a.y + r * a.y_row + at, v, 16);
+                }
+            }
+        }
     }
+    (void)kTop;
+    (void)kThreads;
 }
 
-template <class X, class Y>
+template <class X, class Y, int RK>
 hipError_t launch(const AdapterArgs &a, hipStream_t s) {
     (void)hipGetLastError();
-    hipLaunchKernelGGL((adapter_kernel<X, Y>), dim3(a.rows, std::min((a.out + kThreads - 1) / kThreads, 16)), dim3(kThreads), 0, s, a);
+    const int tiles = (a.rows + 15) / 16, groups = (a.out + 63) / 64;
+    const bool wide = tiles >= 512;
+    const int blocks = wide ? (a.rows + 31) / 32 : tiles;
+    const int of_tile = std::min({wide ? 32 : 16, a.rows, a.n + 1});
+    const int each = blocks >= 256 ? 1 : of_tile;  // workgroups for the adapters of a tile
+    const int want = std::max(1, 512 / (blocks * each));
+    const int slices = std::min(want, std::max(1, groups / 4));
+    const int outs = (groups + slices - 1) / slices * 64;
+    const dim3 grid(blocks, each, (a.out + outs - 1) / outs);
+    if (wide)
+        hipLaunchKernelGGL((adapter_kernel<X, Y, RK, 2>), grid, dim3(512), 0, s, a, outs);
+    else
+        hipLaunchKernelGGL((adapter_kernel<X, Y, RK, 1>), grid, dim3(256), 0, s, a, outs);
     return hipGetLastError();
+}
+
+template <class X, class Y>
+hipError_t launch_xy(const AdapterArgs &a, hipStream_t s) {
+    return a.max_rank <= 16 ? launch<X, Y, 1>(a, s) : a.max_rank <= 32 ? launch<X, Y, 2>(a, s) : a.max_rank <= 64 ? launch<X, Y, 4>(a, s) : launch<X, Y, 8>(a, s);
 }
 
 }  // namespace
 
 hipError_t launch_adapter_rows(const AdapterArgs &a, hipStream_t s) {
-    if (a.x_dtype == ELEM_F16) return a.y_dtype == ELEM_F16 ? launch<__half, __half>(a, s) : launch<__half, float>(a, s);
-    return a.y_dtype == ELEM_F16 ? launch<float, __half>(a, s) : launch<float, float>(a, s);
+    if (a.x_dtype == ELEM_F16) return a.y_dtype == ELEM_F16 ? launch_xy<__half, __half>(a, s) : launch_xy<__half, float>(a, s);
+    return a.y_dtype == ELEM_F16 ? launch_xy<float, __half>(a, s) : launch_xy<float, float>(a, s);
 }
 
 }  // namespace mh
