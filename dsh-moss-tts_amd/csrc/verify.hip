@@ -7,8 +7,13 @@
 // target's own distribution.  A draw with u is the first token whose cumulative sum passes u times the whole.
 //
 // A draw compares u with as many borders as the vocabulary has tokens, and sums of 32 bits move each by up to
-// 2^-24: one draw in a hundred over 2^17 tokens.  So probabilities are formed and summed in 64 bits; that is about
-// 20 instructions a logit, near what reading one takes.
+// 2^-24: one draw in a hundred over 2^17 tokens.  So probabilities are formed and summed in 64 bits, which
+// takes 17 instructions a logit, near what reading one takes.
+//
+// A row is cut into pieces of 64 lanes' values.  One launch reads all rows, a wave a piece, and leaves the
+// pieces' maxima and sums; a second one walks, a workgroup a stream, and draws: it finds the piece that u falls into by
+// the pieces' sums, and reads that one piece again.  What is drawn from (p - q)+ needs that row's two sums first: there the
+// second launch has workgroups for all pieces of a stream, each of which walks by itself, and a third one draws.
 #include <algorithm>
 
 #include "paged_ops.h"
@@ -17,10 +22,10 @@ namespace mh {
 namespace {
 
 constexpr int kThreads = 256, kWaves = kThreads / 64;
-constexpr int kMaxChunks = 128;  // of a row
+constexpr int kMaxPieces = 512;  // of a row
 constexpr double kLog2e = 1.4426950408889634074;
 
-// Of a chunk of a row, or of a row: the largest logit, where it is first, and sum of e^{(x - m) / T}.  Nothing
+// Of a piece of a row, or of a row: the largest logit, where it is first, and sum of e^{(x - m) / T}.  Nothing
 // above -inf: s is 0; a NaN or +inf among them: s is NaN.
 struct Stat {
     float m;
@@ -28,31 +33,43 @@ struct Stat {
     double s;
 };
 
-// 2^x for x <= 0, or NaN: the series of 2^f, |f| <= 1/2, to f^12 (2^-52 of the result).
-__device__ __forceinline__ double exp2_64(double x) {
-    x = x < -1100.0 ? -1100.0 : x;
-    const double n = rint(x), f = (x - n) * 0.69314718055994530942;
-    double y = 1.0 / 479001600;
-    y = fma(y, f, 1.0 / 39916800);
-    y = fma(y, f, 1.0 / 3628800);
-    y = fma(y, f, 1.0 / 362880);
-    y = fma(y, f, 1.0 / 40320);
-    y = fma(y, f, 1.0 / 5040);
-    y = fma(y, f, 1.0 / 720);
-    y = fma(y, f, 1.0 / 120);
-    y = fma(y, f, 1.0 / 24);
-    y = fma(y, f, 1.0 / 6);
-    y = fma(y, f, 0.5);
+// 2^a for a <= 0, as 2^n 2^f with a polynomial through Chebyshev's nodes of |f| <= 1/2, within 2^-45; under
+// 2^-1000 it is 2^-1000.  n comes out of the low bits of a + 1.5 * 2^52 and goes into the exponent as an integer.
+__device__ __forceinline__ double exp2_64(double a) {
+    constexpr double magic = 6755399441055744.0;
+    a = a < -1000.0 ? -1000.0 : a;
+    const double t = a + magic, f = a - (t - magic);
+    double y = 1.0205905320493103e-07;
+    y = fma(y, f, 1.3259645243929057e-06);
+    y = fma(y, f, 1.5252672925346873e-05);
+    y = fma(y, f, 0.00015403433751254997);
+    y = fma(y, f, 0.0013333558200793719);
+    y = fma(y, f, 0.009618129193934304);
+    y = fma(y, f, 0.05550410866465168);
+    y = fma(y, f, 0.2402265069564034);
+    y = fma(y, f, 0.6931471805599462);
     y = fma(y, f, 1.0);
-    y = fma(y, f, 1.0);
-    return ldexp(y, (int)n);
+    return __hiloint2double(__double2hiint(y) + (__double2loint(t) << 20), __double2loint(y));
 }
-// e^{(x - m) / T}, k = log2(e) / T
-__device__ __forceinline__ double weight(float x, float m, double k) { return exp2_64(((double)x - (double)m) * k); }
+// e^{(x - m) / T}, k = log2(e) / T.  The difference first: logits may be far from 0.
+__device__ __forceinline__ double raw_weight(float x, float m, double k) { return exp2_64(((double)x - (double)m) * k); }
+// The same with 0 for what is under 2^-1000, -inf among it.
+__device__ __forceinline__ double weight(float x, float m, double k) {
+    const double a = ((double)x - (double)m) * k;
+    return a >= -1000.0 ? exp2_64(a) : 0.0;
+}
 
+template <int M>
+__device__ __forceinline__ double xshfl64(double v) {
+    return __hiloint2double(xshfl<M>(__double2hiint(v)), xshfl<M>(__double2loint(v)));
+}
 __device__ __forceinline__ double wave_sum64(double v) {
-#pragma unroll
-    for (int d = 32; d > 0; d /= 2) v += __shfl_xor(v, d);
+    v += xshfl64<32>(v);
+    v += xshfl64<16>(v);
+    v += xshfl64<8>(v);
+    v += xshfl64<4>(v);
+    v += xshfl64<2>(v);
+    v += xshfl64<1>(v);
     return v;
 }
 
@@ -63,9 +80,22 @@ __device__ __forceinline__ float logit(const T *p) {
     else
         return *p;
 }
+// N neighbouring logits from place e of a row on, at any address that a logit may have; -inf behind the row.
+template <class T, int N>
+__device__ __forceinline__ void load_logits(const T *p, int e, int vocab, float (&x)[N]) {
+    if (e + N <= vocab) {
+        T raw[N];
+        __builtin_memcpy(raw, p + e, sizeof(raw));
+#pragma unroll
+        for (int j = 0; j < N; ++j) x[j] = logit(raw + j);
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j) x[j] = e + j < vocab ? logit(p + e + j) : -INFINITY;
+    }
+}
 
-// The workspace: statistics [streams][max_rows][chunks] of the target, then of the draft; then of draws from
-// (p - q)+ the mass of each chunk [streams][chunks], and [streams] what is drawn from.
+// The workspace: statistics [streams][max_rows][pieces] of the target, then of the draft; then of draws from
+// (p - q)+ the mass of each piece [streams][pieces], and [streams] what is drawn from.
 struct Draw {
     Stat p, q;  // of the row
     int row, mode;
@@ -76,13 +106,13 @@ struct VerifyWs {
     double *mass;
     Draw *draw;
 };
-__host__ __device__ __forceinline__ VerifyWs verify_ws(int streams, int max_rows, int chunks, bool draft, void *ws) {
+__host__ __device__ __forceinline__ VerifyWs verify_ws(int streams, int max_rows, int pieces, bool draft, void *ws) {
     VerifyWs w;
-    const size_t n = (size_t)streams * max_rows * chunks;
+    const size_t n = (size_t)streams * max_rows * pieces;
     w.p = (Stat *)ws;
     w.q = w.p + n;
     w.mass = (double *)(w.q + (draft ? n : 0));
-    w.draw = (Draw *)(w.mass + (size_t)streams * chunks);
+    w.draw = (Draw *)(w.mass + (draft ? (size_t)streams * pieces : 0));
     return w;
 }
 
@@ -92,98 +122,95 @@ __device__ __forceinline__ int2 nodes_of(const VerifyArgs &a, int s) {
     return r0 >= 0 && r1 >= r0 && r1 <= a.rows ? make_int2(r0, min(r1 - r0, a.max_rows)) : make_int2(0, 0);
 }
 
-// One chunk of one row of the target (y: 0) or the draft (1); EPT values a thread, read V at a time.
-template <class T, int EPT, int V, bool GREEDY>
-__global__ __launch_bounds__(kThreads) void stat_kernel(VerifyArgs a, int chunks) {
-    __shared__ float lm[kWaves];
-    __shared__ int li[kWaves];
-    __shared__ double ls[kWaves];
-    const int at = blockIdx.x / chunks, c = blockIdx.x - at * chunks;
+// One piece of one row of the target (blockIdx.y 0) or the draft (1), a wave each: EPT values a lane, read V at a time.
+template <class T, int EPT, bool GREEDY>
+__global__ __launch_bounds__(kThreads) void stat_kernel(VerifyArgs a, int pieces) {
+    constexpr int V = std::min<int>(16 / (int)sizeof(T), EPT);
+    const int lane = threadIdx.x & 63;
+    const int unit = __builtin_amdgcn_readfirstlane(blockIdx.x * kWaves + (threadIdx.x >> 6));
+    const int at = unit / pieces, c = unit - at * pieces;
     const int s = at / a.max_rows, node = at - s * a.max_rows;
+    if (s >= a.streams) return;
     const bool of_draft = blockIdx.y == 1;
     const int2 rows = nodes_of(a, s);
     if (node >= rows.y - of_draft) return;  // (nothing was drawn behind the last row)
     const T *p = of_draft ? (const T *)a.y + (rows.x + node) * a.y_row : (const T *)a.x + (rows.x + node) * a.x_row;
-    const int base = c * EPT * kThreads, t = threadIdx.x, w = t >> 6;
-    float x[EPT];
+    const int base = c * EPT * 64 + lane * V;
+    float x[EPT / V][V];
 #pragma unroll
-    for (int i = 0; i < EPT; i += V) {
-        const int e = base + i * kThreads + t * V;
-        if (e + V <= a.vocab) {
-            T raw[V];  // (16 bytes at any address that a logit may have)
-            uint32_t u[V * sizeof(T) / 4];
-            __builtin_memcpy(u, p + e, sizeof(u));
-            __builtin_memcpy(raw, u, sizeof(u));
-#pragma unroll
-            for (int j = 0; j < V; ++j) x[i + j] = logit(raw + j);
-        } else {
-#pragma unroll
-            for (int j = 0; j < V; ++j) x[i + j] = e + j < a.vocab ? logit(p + e + j) : -INFINITY;
-        }
-    }
+    for (int i = 0; i < EPT / V; ++i) load_logits<T, V>(p, base + i * 64 * V, a.vocab, x[i]);
     float m = -INFINITY;
     int best = 0x7fffffff;
-#pragma unroll
-    for (int i = 0; i < EPT; ++i)
-        if (x[i] > m) {
-            m = x[i];
-            best = base + (i / V) * V * kThreads + t * V + i % V;
-        }
+    double sum = 0.0;
     if constexpr (GREEDY) {
+#pragma unroll
+        for (int i = 0; i < EPT / V; ++i)
+#pragma unroll
+            for (int j = 0; j < V; ++j)
+                if (x[i][j] > m) {
+                    m = x[i][j];
+                    best = base + i * 64 * V + j;
+                }
         wave_argmax(m, best);
     } else {
-        m = wave_max(m);
-    }
-    if ((t & 63) == 0) {
-        lm[w] = m;
-        li[w] = best;
-    }
-    __syncthreads();
-    for (int v = 0; v < kWaves; ++v)
-        if (lm[v] > m || (lm[v] == m && li[v] < best)) {
-            m = lm[v];
-            best = li[v];
-        }
-    double sum = 0.0;
-    if constexpr (!GREEDY) {
-        const double k = (double)(of_draft ? a.draft_inv_t : a.inv_t) * kLog2e;
-        const float m0 = m == -INFINITY ? 0.0f : m;
-        bool bad = false;
 #pragma unroll
-        for (int i = 0; i < EPT; ++i) {
-            bad |= !(x[i] < INFINITY);
-            sum += weight(x[i], m0, k);
+        for (int i = 0; i < EPT / V; ++i)
+#pragma unroll
+            for (int j = 0; j < V; ++j) m = fmaxf(m, x[i][j]);
+        m = wave_max(m);
+        if (m > -INFINITY) {
+            const double k = (double)(of_draft ? a.draft_inv_t : a.inv_t) * kLog2e;
+            bool bad = !(m < INFINITY);
+            double more[2] = {};
+#pragma unroll
+            for (int i = 0; i < EPT / V; ++i)
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    bad |= x[i][j] != x[i][j];
+                    more[j & 1] += raw_weight(x[i][j], m, k);
+                }
+            sum = wave_sum64(bad ? __builtin_nan("") : more[0] + more[1]);
+        } else {  // nothing but -inf, or NaN
+            bool bad = false;
+#pragma unroll
+            for (int i = 0; i < EPT / V; ++i)
+#pragma unroll
+                for (int j = 0; j < V; ++j) bad |= x[i][j] != x[i][j];
+            if (__any(bad)) sum = __builtin_nan("");
         }
-        sum = wave_sum64(bad ? __builtin_nan("") : sum);
-        if ((t & 63) == 0) ls[w] = sum;
-        __syncthreads();
-        sum = 0.0;
-        for (int v = 0; v < kWaves; ++v) sum += ls[v];
     }
-    if (t == 0) {
-        const VerifyWs ws = verify_ws(a.streams, a.max_rows, chunks, a.y != nullptr, a.ws);
-        (of_draft ? ws.q : ws.p)[(size_t)at * chunks + c] = Stat{m, m > -INFINITY ? best : -1, sum};
+    if (lane == 0) {
+        const VerifyWs ws = verify_ws(a.streams, a.max_rows, pieces, a.y != nullptr, a.ws);
+        (of_draft ? ws.q : ws.p)[(size_t)at * pieces + c] = Stat{m, m > -INFINITY ? best : -1, sum};
     }
 }
 
-// The chunks of a row together.
-__device__ __forceinline__ Stat row_stat(const Stat *c, int chunks, double k) {
-    Stat r{-INFINITY, -1, 0.0};
-    for (int i = 0; i < chunks; ++i) {
+// The pieces of a row together, by one wave; every lane has the result.
+template <bool GREEDY>
+__device__ __forceinline__ Stat row_stat(const Stat *c, int pieces, double k) {
+    const int lane = threadIdx.x & 63;
+    float m = -INFINITY;
+    int best = 0x7fffffff;
+    for (int i = lane; i < pieces; i += 64) {
         const Stat o = c[i];
-        if (o.m > r.m) {  // (the first of equal ones stays)
-            r.m = o.m;
-            r.best = o.best;
+        if (o.m > m) {
+            m = o.m;
+            best = o.best;
         }
     }
-    const float m0 = r.m == -INFINITY ? 0.0f : r.m;
-    for (int i = 0; i < chunks; ++i) {
-        const Stat o = c[i];
-        r.s += o.s == 0.0 ? 0.0 : o.s * weight(o.m, m0, k);
+    if constexpr (GREEDY) {
+        wave_argmax(m, best);
+        return Stat{m, m > -INFINITY ? best : -1, 0.0};
+    } else {
+        m = wave_max(m);
+        double s = 0.0;
+        for (int i = lane; i < pieces; i += 64) {
+            const Stat o = c[i];
+            if (!(o.s == 0.0)) s += o.s * weight(o.m, m, k);
+        }
+        return Stat{m, -1, wave_sum64(s)};
     }
-    return r;
 }
-__device__ __forceinline__ bool fine(const Stat &s) { return s.s > 0.0; }  // (not of NaN)
 
 // Inclusive sums over the workgroup in 64 bits: what earlier threads hold, this thread's among them.
 __device__ __forceinline__ double scan64(double v, double *lds, double &all) {
@@ -198,6 +225,7 @@ __device__ __forceinline__ double scan64(double v, double *lds, double &all) {
     __syncthreads();
     double before = 0.0;
     all = 0.0;
+#pragma unroll
     for (int i = 0; i < kWaves; ++i) {
         if (i < w) before += lds[i];
         all += lds[i];
@@ -206,131 +234,171 @@ __device__ __forceinline__ double scan64(double v, double *lds, double &all) {
 }
 
 struct PickLds {
-    double mass[kMaxChunks];
+    double mass[kMaxPieces];
     double scan[kWaves];
-    uint32_t gone[32 * kThreads / 32];  // a bit per token of one chunk: rejected
+    double before;
     int found, last;
 };
 
-// What token e of the row weighs, up to a factor of the row.
-template <class T>
-struct Weights {
-    const T *x, *y;
-    Stat p, q;
-    double kp, kq;
-    bool rest;  // (p - q)+
-    __device__ __forceinline__ double of(int e) const {
-        const double wp = weight(logit(x + e), p.m, kp);
-        if (!rest) return wp;
-        const double d = wp / p.s - weight(logit(y + e), q.m, kq) / q.s;
-        return d > 0.0 ? d : 0.0;
-    }
-};
-
-// The token drawn with u: lds.mass holds the chunks' masses.  `rejected` says of a token whether it is left out.
-template <class T, int EPT, class Gone>
-__device__ int pick(const Weights<T> &w, int vocab, int chunks, double u, PickLds &lds, Gone &&gone) {
+// Of values in order, N a thread: the first whose cumulative sum, on top of `before`, passes u of `whole` (or, whole < 0, of
+// their own sum), else the last above 0; -1 where there is none.  `before` becomes the sum in front of it, whole theirs.
+template <int N>
+__device__ __forceinline__ int pick_of(const double (&v)[N], double u, double &before, double &whole, PickLds &lds) {
     const int t = threadIdx.x;
-    double all = 0.0;
-    for (int c = 0; c < chunks; ++c) all += lds.mass[c];
-    if (!(all > 0.0)) return -1;
-    const double aim = u * all;
-    double before = 0.0;
-    int at = -1;
-    for (int c = 0; c < chunks; ++c) {  // the first that passes it; where rounding lets none, the last with any mass
-        if (!(lds.mass[c] > 0.0)) continue;
-        if (at >= 0) before += lds.mass[at];
-        at = c;
-        if (before + lds.mass[c] > aim) break;
-    }
-    const int first = at * EPT * kThreads + t * EPT;  // neighbouring tokens of a thread
-    double sum = 0.0;
-    for (int i = 0; i < EPT; ++i)
-        if (first + i < vocab && !gone(first + i)) sum += w.of(first + i);
-    double total;
-    double run = before + scan64(sum, lds.scan, total) - sum;
+    double sum = 0.0, all;
+#pragma unroll
+    for (int i = 0; i < N; ++i) sum += v[i];
     if (t == 0) {
         lds.found = 0x7fffffff;
         lds.last = -1;
     }
-    __syncthreads();
+    double run = before + scan64(sum, lds.scan, all) - sum;
+    if (whole < 0.0) whole = all;
+    const double aim = u * whole;
     int found = -1, last = -1;
-    if (sum > 0.0)
-        for (int i = 0; i < EPT; ++i) {
-            if (first + i >= vocab || gone(first + i)) continue;
-            const double v = w.of(first + i);
-            run += v;
-            if (v > 0.0) last = first + i;
-            if (v > 0.0 && run > aim && found < 0) found = first + i;
-        }
+    double front[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        front[i] = run;
+        run += v[i];
+        if (v[i] > 0.0) last = t * N + i;
+        if (v[i] > 0.0 && run > aim && found < 0) found = t * N + i;
+    }
     if (found >= 0) atomicMin(&lds.found, found);
     if (last >= 0) atomicMax(&lds.last, last);
     __syncthreads();
-    return lds.found < vocab ? lds.found : lds.last;
+    const int got = lds.found != 0x7fffffff ? lds.found : lds.last;
+    if (got >= 0 && got / N == t) {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (got % N == i) lds.before = front[i];
+    }
+    __syncthreads();
+    before = lds.before;
+    return got;
 }
+
+// What the tokens of a row weigh, up to a factor of the row.
+template <class T>
+struct Weights {
+    const T *x, *y;
+    float pm, qm;
+    double kp, kq, ps, qs;  // ps, qs: 1 / sum
+    bool rest;              // (p - q)+
+    __device__ __forceinline__ Weights(const VerifyArgs &a, const Draw &d)
+        : x((const T *)a.x + d.row * a.x_row), y((const T *)a.y + d.row * a.y_row), pm(d.p.m), qm(d.q.m), kp((double)a.inv_t * kLog2e),
+          kq((double)a.draft_inv_t * kLog2e), ps(1.0 / d.p.s), qs(1.0 / d.q.s), rest(d.mode == DRAW_REST) {}
+    // of N tokens from e on
+    template <int N>
+    __device__ __forceinline__ void of(int e, int vocab, double (&v)[N]) const {
+        float lx[N];
+        load_logits<T, N>(x, e, vocab, lx);
+        if (rest) {
+            float ly[N];
+            load_logits<T, N>(y, e, vocab, ly);
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const double d = weight(lx[i], pm, kp) * ps - weight(ly[i], qm, kq) * qs;
+                v[i] = d > 0.0 ? d : 0.0;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[i] = weight(lx[i], pm, kp);
+        }
+    }
+};
+
+// The token drawn with u; lds.mass holds the pieces' masses, -1 where there are none.  drop(first, v) leaves tokens out.
+template <class T, int EPT, class Drop>
+__device__ __forceinline__ int pick(const Weights<T> &w, int vocab, int pieces, double u, PickLds &lds, Drop &&drop) {
+    constexpr int N = EPT * 64 / kThreads, NP = kMaxPieces / kThreads;
+    const int t = threadIdx.x;
+    double mass[NP];
+#pragma unroll
+    for (int i = 0; i < NP; ++i) mass[i] = t * NP + i < pieces ? lds.mass[t * NP + i] : 0.0;
+    double before = 0.0, whole = -1.0;
+    const int c = pick_of<NP>(mass, u, before, whole, lds);
+    if (c < 0) return -1;
+    const int first = c * EPT * 64 + t * N;
+    double v[N];
+    w.template of<N>(first, vocab, v);
+    drop(first, v);
+    const int got = pick_of<N>(v, u, before, whole, lds);
+    return got < 0 ? -1 : c * EPT * 64 + got;
+}
+struct KeepAll {
+    template <int N>
+    __device__ __forceinline__ void operator()(int, double (&)[N]) const {}
+};
 
 __device__ __forceinline__ double uniform(double u) { return u < 1.0 ? (u > 0.0 ? u : 0.0) : 1.0; }  // (NaN: 1)
 
-// One workgroup a stream: the walk, by its first wave, a lane a node; and, but for draws from (p - q)+, the draw.
-template <class T, int EPT>
-__global__ __launch_bounds__(kThreads) void walk_kernel(VerifyArgs a, int chunks) {
-    __shared__ PickLds lds;
-    __shared__ Draw draw;
-    __shared__ int gone[kTreeMax], n_gone;
-    const int s = blockIdx.x, t = threadIdx.x;
-    const int2 rows = nodes_of(a, s);
-    const int n = rows.y;
-    const VerifyWs ws = verify_ws(a.streams, a.max_rows, chunks, a.y != nullptr, a.ws);
+struct WalkLds {
+    Stat p[kTreeMax], q[kTreeMax];
+    Draw draw;
+    int gone[kTreeMax], n_gone;  // the children of the last node, all rejected
+    double gone_weight[kTreeMax];
+};
+
+// The walk of one stream, by one workgroup: the rows' sums by all waves, then a lane a node.  `writes`: whether this
+// workgroup leaves the outputs.  A barrier follows.
+template <class T, bool GREEDY>
+__device__ __forceinline__ void walk(const VerifyArgs &a, int s, int2 rows, const VerifyWs &ws, int pieces, bool writes, WalkLds &lds) {
+    const int t = threadIdx.x, n = rows.y;
     const bool drafted = a.y != nullptr;
     const double kp = (double)a.inv_t * kLog2e, kq = (double)a.draft_inv_t * kLog2e;
-    if (n == 0) {
-        if (t == 0) {
-            a.accepted[s] = 0;
-            a.next[s] = -1;
-            if (drafted) ws.draw[s].mode = DRAW_NONE;
-        }
-        return;
+    // what a lane needs of its node, asked for early
+    const bool in = t < n;
+    const int tok = in ? a.tokens[rows.x + t] : -1;
+    int parent = t - 1;
+    if (in && a.row_mask != nullptr) {
+        const uint64_t mask = a.row_mask[rows.x + t], up = mask & ((1ull << t) - 1);
+        parent = (mask >> t & 1) && up ? 63 - __builtin_clzll(up) : -1;
     }
-    if (t < 64) {
-        const bool in = t < n;
-        Stat p{-INFINITY, -1, 0.0}, q = p;
-        if (in) p = row_stat(ws.p + ((size_t)s * a.max_rows + t) * chunks, chunks, kp);
-        if (drafted && t < n - 1) q = row_stat(ws.q + ((size_t)s * a.max_rows + t) * chunks, chunks, kq);
-        int parent = t - 1;
-        if (in && a.row_mask != nullptr) {
-            const uint64_t mask = a.row_mask[rows.x + t], up = mask & ((1ull << t) - 1);
-            parent = (mask >> t & 1) && up ? 63 - __builtin_clzll(up) : -1;
+    if (!in || t == 0) parent = -1;
+    const int of = max(parent, 0);
+    const bool known = tok >= 0 && tok < a.vocab && parent >= 0;
+    double u = 0.0;
+    float lx = -INFINITY, ly = -INFINITY;
+    if (!GREEDY && known) {
+        u = uniform(a.uniforms[rows.x + t]);
+        lx = logit((const T *)a.x + (rows.x + of) * a.x_row + tok);
+        if (drafted) ly = logit((const T *)a.y + (rows.x + of) * a.y_row + tok);
+    }
+    for (int i = t >> 6; i < n; i += kWaves) {
+        const Stat p = row_stat<GREEDY>(ws.p + ((size_t)s * a.max_rows + i) * pieces, pieces, kp);
+        if ((t & 63) == 0) lds.p[i] = p;
+        if (!GREEDY && drafted && i < n - 1) {
+            const Stat q = row_stat<GREEDY>(ws.q + ((size_t)s * a.max_rows + i) * pieces, pieces, kq);
+            if ((t & 63) == 0) lds.q[i] = q;
         }
-        if (!in || t == 0) parent = -1;
-        const int of = max(parent, 0);
-        const int tok = in ? a.tokens[rows.x + t] : -1;
-        const bool known = tok >= 0 && tok < a.vocab && parent >= 0;
-        const double u = in && a.uniforms != nullptr ? uniform(a.uniforms[rows.x + t]) : 0.0;
+    }
+    __syncthreads();
+    if (t < 64) {
         bool accept = false;
-        if (a.greedy) {
-            const int best = __shfl(p.best, of);  // (by all lanes: a parent need not have a token itself)
-            accept = known && tok == best;
+        const Stat p = lds.p[of];
+        double prob = 0.0;
+        if constexpr (GREEDY) {
+            accept = known && tok == p.best;
         } else {
-            const float pm = __shfl(p.m, of), qm = __shfl(q.m, of);
-            const double psum = __shfl(p.s, of), qsum = __shfl(q.s, of);
-            const bool p_fine = psum > 0.0;
-            double prob = 0.0;
-            if (known && p_fine) prob = weight(logit((const T *)a.x + (rows.x + of) * a.x_row + tok), pm, kp) / psum;
+            const bool fine = known && p.s > 0.0;  // (not NaN)
+            if (fine) prob = weight(lx, p.m, kp) / p.s;
             if (drafted) {
-                if (known && p_fine && qsum > 0.0)
-                    accept = u * (weight(logit((const T *)a.y + (rows.x + of) * a.y_row + tok), qm, kq) / qsum) < prob;
+                const Stat q = lds.q[of];
+                if (fine && q.s > 0.0) accept = u * (weight(ly, q.m, kq) / q.s) < prob;
             } else {
                 double left = 1.0;
                 bool again = false;  // an elder sibling is the same token
-                for (int j = 1; j < n; ++j) {
-                    const int pj = __builtin_amdgcn_readlane(parent, j), tj = __builtin_amdgcn_readlane(tok, j);
-                    const bool aj = __builtin_amdgcn_readlane((int)again, j);
-                    const double bj = __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(prob), j), __builtin_amdgcn_readlane(__double2loint(prob), j));
-                    if (t > j && parent == pj && pj >= 0) {
-                        again |= tok == tj;
-                        if (!aj) left -= bj;
+                if (a.row_mask != nullptr)
+                    for (int j = 1; j < n; ++j) {
+                        const int pj = __builtin_amdgcn_readlane(parent, j), tj = __builtin_amdgcn_readlane(tok, j);
+                        const bool aj = __builtin_amdgcn_readlane((int)again, j);
+                        const double bj = __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(prob), j), __builtin_amdgcn_readlane(__double2loint(prob), j));
+                        if (t > j && parent == pj && pj >= 0) {
+                            again |= tok == tj;
+                            if (!aj) left -= bj;
+                        }
                     }
-                }
                 accept = !again && known && u * (left > 0.0 ? left : 0.0) < prob;
             }
         }
@@ -343,163 +411,205 @@ __global__ __launch_bounds__(kThreads) void walk_kernel(VerifyArgs a, int chunks
             cur = __builtin_ctzll(next);
             on |= 1ull << cur;
         }
-        if (in) {  // entry j of the path is the j-th node on it
+        if (in && writes) {  // entry j of the path is the j-th node on it
             const int taken = __popcll(on);
             if (on >> t & 1) a.path[rows.x + __popcll(on & ((1ull << t) - 1))] = t;
             if (t >= taken) a.path[rows.x + t] = -1;
         }
-        const int best = __shfl(p.best, cur);
-        const Stat pl{__shfl(p.m, cur), 0, __shfl(p.s, cur)}, ql{__shfl(q.m, cur), 0, __shfl(q.s, cur)};
-        const bool child = parent == cur && known && !drafted;
+        const bool child = !GREEDY && !drafted && parent == cur && known;
         const uint64_t children = __ballot(child);
-        if (child) gone[__popcll(children & ((1ull << t) - 1))] = tok;
+        if (child) {
+            const int i = __popcll(children & ((1ull << t) - 1));
+            lds.gone[i] = tok;
+            lds.gone_weight[i] = weight(lx, p.m, kp);
+        }
         if (t == 0) {
-            n_gone = __popcll(children);
-            a.accepted[s] = __popcll(on) - 1;
-            if (a.greedy) a.next[s] = best;
-            draw.p = pl;
-            draw.q = ql;
-            draw.row = rows.x + cur;
-            draw.mode = !fine(pl) ? DRAW_NONE : (drafted && cur < n - 1 && fine(ql) ? DRAW_REST : DRAW_P);
-            if (drafted) ws.draw[s] = draw;
+            const Stat pl = lds.p[cur];
+            Stat ql{};
+            if (drafted && cur < n - 1) ql = lds.q[cur];
+            lds.n_gone = __popcll(children);
+            lds.draw = Draw{pl, ql, rows.x + cur, !(pl.s > 0.0) ? DRAW_NONE : (ql.s > 0.0 ? DRAW_REST : DRAW_P)};
+            if (writes) {
+                a.accepted[s] = __popcll(on) - 1;
+                if (GREEDY) a.next[s] = pl.best;
+            }
         }
     }
-    if (a.greedy || drafted) return;
     __syncthreads();
-    if (draw.mode == DRAW_NONE) {
-        if (t == 0) a.next[s] = -1;
+}
+
+// The pieces' masses of the row, relative to its largest logit.
+__device__ __forceinline__ void masses_of(const Stat *row, int pieces, float m, double k, PickLds &lds) {
+    for (int c = threadIdx.x; c < pieces; c += kThreads) lds.mass[c] = row[c].s == 0.0 ? 0.0 : row[c].s * weight(row[c].m, m, k);
+}
+
+// One workgroup a stream of tokens picked outright: the walk and the draw.
+template <class T, int EPT, bool GREEDY>
+__global__ __launch_bounds__(kThreads) void walk_kernel(VerifyArgs a, int pieces) {
+    __shared__ PickLds lds;
+    __shared__ WalkLds wl;
+    const int s = blockIdx.x, t = threadIdx.x;
+    const int2 rows = nodes_of(a, s);
+    if (rows.y == 0) {
+        if (t == 0) {
+            a.accepted[s] = 0;
+            a.next[s] = -1;
+        }
         return;
     }
-    const T *x = (const T *)a.x + draw.row * a.x_row;
-    const Weights<T> w{x, nullptr, draw.p, draw.q, kp, kq, false};
-    const Stat *row = ws.p + ((size_t)s * a.max_rows + (draw.row - rows.x)) * chunks;
-    auto masses = [&] {
-        __syncthreads();
-        for (int c = t; c < chunks; c += kThreads) lds.mass[c] = row[c].s == 0.0 ? 0.0 : row[c].s * weight(row[c].m, draw.p.m, kp);
-        __syncthreads();
-    };
-    auto bits_of = [&](int c) {  // those of chunk c that were rejected
-        for (int i = t; i < EPT * kThreads / 32; i += kThreads) lds.gone[i] = 0;
-        __syncthreads();
-        if (t < n_gone && gone[t] / (EPT * kThreads) == c) {
-            const int b = gone[t] - c * EPT * kThreads;
-            atomicOr(&lds.gone[b / 32], 1u << (b % 32));
+    const VerifyWs ws = verify_ws(a.streams, a.max_rows, pieces, false, a.ws);
+    walk<T, GREEDY>(a, s, rows, ws, pieces, true, wl);
+    if constexpr (!GREEDY) {
+        if (wl.draw.mode == DRAW_NONE) {
+            if (t == 0) a.next[s] = -1;
+            return;
         }
+        constexpr int PIECE = EPT * 64, N = PIECE / kThreads;
+        const Weights<T> w(a, wl.draw);
+        const Stat *row = ws.p + ((size_t)s * a.max_rows + (wl.draw.row - rows.x)) * pieces;
+        const int n_gone = wl.n_gone;
+        const double u = uniform(a.uniforms[rows.x]);
+        auto drop = [&](int first, double(&v)[N]) {
+            for (int i = 0; i < n_gone; ++i) {
+                const unsigned d = (unsigned)(wl.gone[i] - first);
+                if (d < (unsigned)N)
+#pragma unroll
+                    for (int j = 0; j < N; ++j) v[j] = (int)d == j ? 0.0 : v[j];
+            }
+        };
+        masses_of(row, pieces, wl.draw.p.m, w.kp, lds);
         __syncthreads();
-    };
-    auto is_gone = [&](int e) {
-        const int b = e % (EPT * kThreads);
-        return (lds.gone[b / 32] >> (b % 32) & 1) != 0;
-    };
-    masses();
-    // chunks that lose tokens are summed again (a difference of sums would lose what little is left)
-    for (int i = 0; i < n_gone; ++i) {
-        const int c = gone[i] / (EPT * kThreads);
-        bool seen = false;
-        for (int j = 0; j < i; ++j) seen |= gone[j] / (EPT * kThreads) == c;
-        if (seen) continue;
-        bits_of(c);
-        double sum = 0.0, all;
-        for (int e = c * EPT * kThreads + t; e < min(a.vocab, (c + 1) * EPT * kThreads); e += kThreads)
-            if (!is_gone(e)) sum += w.of(e);
-        scan64(sum, lds.scan, all);
-        if (t == 0) lds.mass[c] = all;
-        __syncthreads();
+        if (n_gone > 0) {
+            // The rejected tokens' weights come off their pieces' sums, each token once.  Where less than 2^-12 is left, the
+            // difference would be coarser than 2^-40 of it, and the piece is summed again.
+            for (int c = t; c < pieces; c += kThreads) {
+                const double all = lds.mass[c];
+                double off = 0.0;
+                for (int i = 0; i < n_gone; ++i) {
+                    if (wl.gone[i] / PIECE != c) continue;
+                    bool seen = false;
+                    for (int j = 0; j < i; ++j) seen |= wl.gone[j] == wl.gone[i];
+                    if (!seen) off += wl.gone_weight[i];
+                }
+                if (off > 0.0) lds.mass[c] = all - off >= all * 0x1p-12 ? all - off : -1.0;
+            }
+            __syncthreads();
+            for (int i = 0; i < n_gone; ++i) {
+                const int c = wl.gone[i] / PIECE;
+                if (!(lds.mass[c] < 0.0)) continue;  // (of the whole workgroup)
+                double v[N], sum = 0.0, all;
+                w.template of<N>(c * PIECE + t * N, a.vocab, v);
+                drop(c * PIECE + t * N, v);
+#pragma unroll
+                for (int j = 0; j < N; ++j) sum += v[j];
+                scan64(sum, lds.scan, all);
+                if (t == 0) lds.mass[c] = all;
+                __syncthreads();
+            }
+        }
+        int got = pick<T, EPT>(w, a.vocab, pieces, u, lds, drop);
+        if (got < 0) {  // nothing is left: p itself
+            __syncthreads();
+            masses_of(row, pieces, wl.draw.p.m, w.kp, lds);
+            __syncthreads();
+            got = pick<T, EPT>(w, a.vocab, pieces, u, lds, KeepAll());
+        }
+        if (t == 0) a.next[s] = got;
     }
-    double all = 0.0;
-    for (int c = 0; c < chunks; ++c) all += lds.mass[c];
-    const double u = uniform(a.uniforms[rows.x]);
-    int got;
-    if (all > 0.0) {
-        // the chunk's bits depend on which chunk the draw falls into: all rejected tokens are looked up there
-        got = pick<T, EPT>(w, a.vocab, chunks, u, lds, [&](int e) {
-            for (int i = 0; i < n_gone; ++i)
-                if (gone[i] == e) return true;
-            return false;
-        });
-    } else {
-        masses();
-        got = pick<T, EPT>(w, a.vocab, chunks, u, lds, [](int) { return false; });
-    }
-    if (t == 0) a.next[s] = got;
 }
 
-// The mass of (p - q)+ in one chunk of the row behind a rejected token.
+// Chains with the draft's logits: every workgroup of a stream walks; where a token is rejected, each wave has the mass of
+// (p - q)+ in one piece of the row in front of it.
 template <class T, int EPT>
-__global__ __launch_bounds__(kThreads) void rest_kernel(VerifyArgs a, int chunks) {
-    __shared__ double lds[kWaves];
-    const int s = blockIdx.x / chunks, c = blockIdx.x - s * chunks;
-    const VerifyWs ws = verify_ws(a.streams, a.max_rows, chunks, true, a.ws);
-    const Draw d = ws.draw[s];
-    if (d.mode != DRAW_REST) return;
-    const Weights<T> w{(const T *)a.x + d.row * a.x_row, (const T *)a.y + d.row * a.y_row, d.p, d.q, (double)a.inv_t * kLog2e,
-                       (double)a.draft_inv_t * kLog2e, true};
-    double sum = 0.0, all;
-    for (int e = c * EPT * kThreads + (int)threadIdx.x; e < min(a.vocab, (c + 1) * EPT * kThreads); e += kThreads) sum += w.of(e);
-    scan64(sum, lds, all);
-    if (threadIdx.x == 0) ws.mass[(size_t)s * chunks + c] = all;
+__global__ __launch_bounds__(kThreads) void walk_draft_kernel(VerifyArgs a, int pieces, int parts) {
+    __shared__ WalkLds wl;
+    const int s = blockIdx.x / parts, part = blockIdx.x - s * parts, t = threadIdx.x;
+    const int2 rows = nodes_of(a, s);
+    const VerifyWs ws = verify_ws(a.streams, a.max_rows, pieces, true, a.ws);
+    if (rows.y == 0) {
+        if (t == 0 && part == 0) {
+            a.accepted[s] = 0;
+            ws.draw[s].mode = DRAW_NONE;
+        }
+        return;
+    }
+    walk<T, false>(a, s, rows, ws, pieces, part == 0, wl);
+    if (t == 0 && part == 0) ws.draw[s] = wl.draw;
+    const int c = part * kWaves + (t >> 6);
+    if (wl.draw.mode != DRAW_REST || c >= pieces) return;
+    constexpr int V = std::min<int>(16 / (int)sizeof(T), EPT);
+    const Weights<T> w(a, wl.draw);
+    double sum = 0.0;
+#pragma unroll 2
+    for (int i = 0; i < EPT / V; ++i) {
+        double v[V];
+        w.template of<V>(c * EPT * 64 + (i * 64 + (t & 63)) * V, a.vocab, v);
+#pragma unroll
+        for (int j = 0; j < V; ++j) sum += v[j];
+    }
+    sum = wave_sum64(sum);
+    if ((t & 63) == 0) ws.mass[(size_t)s * pieces + c] = sum;
 }
 
-// The draw of a chain with the draft's logits.
+// Their draw.
 template <class T, int EPT>
-__global__ __launch_bounds__(kThreads) void draw_kernel(VerifyArgs a, int chunks) {
+__global__ __launch_bounds__(kThreads) void draw_kernel(VerifyArgs a, int pieces) {
     __shared__ PickLds lds;
     const int s = blockIdx.x, t = threadIdx.x;
-    const VerifyWs ws = verify_ws(a.streams, a.max_rows, chunks, true, a.ws);
+    const VerifyWs ws = verify_ws(a.streams, a.max_rows, pieces, true, a.ws);
     const Draw d = ws.draw[s];
     if (d.mode == DRAW_NONE) {
         if (t == 0) a.next[s] = -1;
         return;
     }
     const int2 rows = nodes_of(a, s);
-    const double kp = (double)a.inv_t * kLog2e, u = uniform(a.uniforms[rows.x]);
-    Weights<T> w{(const T *)a.x + d.row * a.x_row, (const T *)a.y + d.row * a.y_row, d.p, d.q, kp, (double)a.draft_inv_t * kLog2e,
-                 d.mode == DRAW_REST};
+    const double u = uniform(a.uniforms[rows.x]);
+    Weights<T> w(a, d);
     int got = -1;
     if (w.rest) {
-        for (int c = t; c < chunks; c += kThreads) lds.mass[c] = ws.mass[(size_t)s * chunks + c];
+        for (int c = t; c < pieces; c += kThreads) lds.mass[c] = ws.mass[(size_t)s * pieces + c];
         __syncthreads();
-        got = pick<T, EPT>(w, a.vocab, chunks, u, lds, [](int) { return false; });
+        got = pick<T, EPT>(w, a.vocab, pieces, u, lds, KeepAll());
         __syncthreads();
     }
-    if (got < 0) {  // nothing was left over: from p itself
+    if (got < 0) {  // all were accepted, or nothing is left over: from p itself
         w.rest = false;
-        const Stat *row = ws.p + ((size_t)s * a.max_rows + (d.row - rows.x)) * chunks;
-        for (int c = t; c < chunks; c += kThreads) lds.mass[c] = row[c].s == 0.0 ? 0.0 : row[c].s * weight(row[c].m, d.p.m, kp);
+        masses_of(ws.p + ((size_t)s * a.max_rows + (d.row - rows.x)) * pieces, pieces, d.p.m, w.kp, lds);
         __syncthreads();
-        got = pick<T, EPT>(w, a.vocab, chunks, u, lds, [](int) { return false; });
+        got = pick<T, EPT>(w, a.vocab, pieces, u, lds, KeepAll());
     }
     if (t == 0) a.next[s] = got;
 }
 
-// Values of a thread of a chunk: few while that fills the chip.
+// Values of a lane of a piece: few while that fills the chip, many where the pieces' sums would be much work themselves.
 int ept_of(int rows, int vocab) {
-    for (const int ept : {4, 16}) {
-        const int chunks = (vocab + ept * kThreads - 1) / (ept * kThreads);
-        if (chunks <= (ept == 4 ? 16 : 32) && (chunks == 1 || (long long)rows * chunks <= 2048)) return ept;
-    }
-    return 32;
+    const int small = (vocab + 255) / 256;
+    if (small <= 64 && (long long)rows * small <= 4096) return 4;
+    return vocab <= 64 * 1024 ? 16 : 32;
 }
-int chunks_of(int rows, int vocab) {
-    const int n = ept_of(rows, vocab) * kThreads;
+int pieces_of(int rows, int vocab) {
+    const int n = ept_of(rows, vocab) * 64;
     return (vocab + n - 1) / n;
 }
-static_assert(kMaxChunks * 32 * kThreads >= kVocabMax, "a row's chunks");
+static_assert(kMaxPieces * 32 * 64 >= kVocabMax, "a row's pieces");
 
 template <class T, int EPT>
 hipError_t verify_e(const VerifyArgs &a, hipStream_t s) {
-    constexpr int V = std::min<int>(16 / (int)sizeof(T), EPT);
-    const int chunks = chunks_of(a.streams * a.max_rows, a.vocab);
-    const dim3 grid((unsigned)a.streams * a.max_rows * chunks, a.y != nullptr ? 2 : 1);
+    const int pieces = pieces_of(a.streams * a.max_rows, a.vocab);
+    const dim3 grid((unsigned)(((long long)a.streams * a.max_rows * pieces + kWaves - 1) / kWaves), a.y != nullptr ? 2 : 1);
     (void)hipGetLastError();
-    if (a.greedy)
-        hipLaunchKernelGGL((stat_kernel<T, EPT, V, true>), grid, dim3(kThreads), 0, s, a, chunks);
-    else
-        hipLaunchKernelGGL((stat_kernel<T, EPT, V, false>), grid, dim3(kThreads), 0, s, a, chunks);
-    hipLaunchKernelGGL((walk_kernel<T, EPT>), dim3(a.streams), dim3(kThreads), 0, s, a, chunks);
-    if (a.y != nullptr && !a.greedy) {
-        hipLaunchKernelGGL((rest_kernel<T, EPT>), dim3((unsigned)a.streams * chunks), dim3(kThreads), 0, s, a, chunks);
-        hipLaunchKernelGGL((draw_kernel<T, EPT>), dim3(a.streams), dim3(kThreads), 0, s, a, chunks);
+    if (a.greedy) {
+        hipLaunchKernelGGL((stat_kernel<T, EPT, true>), grid, dim3(kThreads), 0, s, a, pieces);
+        hipLaunchKernelGGL((walk_kernel<T, EPT, true>), dim3(a.streams), dim3(kThreads), 0, s, a, pieces);
+        return hipGetLastError();
+    }
+    hipLaunchKernelGGL((stat_kernel<T, EPT, false>), grid, dim3(kThreads), 0, s, a, pieces);
+    if (a.y != nullptr) {
+        const int parts = (pieces + kWaves - 1) / kWaves;
+        hipLaunchKernelGGL((walk_draft_kernel<T, EPT>), dim3((unsigned)a.streams * parts), dim3(kThreads), 0, s, a, pieces, parts);
+        hipLaunchKernelGGL((draw_kernel<T, EPT>), dim3(a.streams), dim3(kThreads), 0, s, a, pieces);
+    } else {
+        hipLaunchKernelGGL((walk_kernel<T, EPT, false>), dim3(a.streams), dim3(kThreads), 0, s, a, pieces);
     }
     return hipGetLastError();
 }
@@ -516,8 +626,8 @@ hipError_t verify_t(const VerifyArgs &a, hipStream_t s) {
 }  // namespace
 
 size_t verify_workspace(int streams, int max_rows, int vocab, bool draft) {
-    const VerifyWs w = verify_ws(streams, max_rows, chunks_of(streams * max_rows, vocab), draft, nullptr);
-    return (size_t)(uintptr_t)(w.draw + streams);
+    const VerifyWs w = verify_ws(streams, max_rows, pieces_of(streams * max_rows, vocab), draft, nullptr);
+    return (size_t)(uintptr_t)(w.draw + (draft ? streams : 0));
 }
 
 hipError_t launch_verify(const VerifyArgs &a, hipStream_t s) { return a.dtype == ELEM_F16 ? verify_t<__half>(a, s) : verify_t<float>(a, s); }
