@@ -6,14 +6,16 @@
 // u_c (1 - the rejected ones' p) < p(t_c), and the token behind them is drawn from p without them.  Both leave the
 // target's own distribution.  A draw with u is the first token whose cumulative sum passes u times the whole.
 //
-// A draw compares u with as many borders as the vocabulary has tokens, and sums of 32 bits move each by up to
-// 2^-24: one draw in a hundred over 2^17 tokens.  So probabilities are formed and summed in 64 bits, which
-// takes 17 instructions a logit, near what reading one takes.
+// A draw compares u with as many borders as the vocabulary has tokens, and sums of 32-bit exponentials move each by up
+// to 2^-24: one draw in a hundred over 2^17 tokens.  So the row that is drawn from is weighed in 64 bits, at
+// 20 instructions of 8 cycles a logit; all others, of which only the sum is wanted, with the hardware's exponential (the sum's
+// error is some 2^-26 of it), which hides behind the reading.
 //
-// A row is cut into pieces of 64 lanes' values.  One launch reads all rows, a wave a piece, and leaves the
-// pieces' maxima and sums; a second one walks, a workgroup a stream, and draws: it finds the piece that u falls into by
-// the pieces' sums, and reads that one piece again.  What is drawn from (p - q)+ needs that row's two sums first: there the
-// second launch has workgroups for all pieces of a stream, each of which walks by itself, and a third one draws.
+// A row is cut into pieces of a wave's values, four pieces a part.  First launch: every row, a workgroup a part, leaves each
+// part's maximum and sum.  Second: a workgroup for each part of a stream; each one walks by itself, weighs its part of the row that
+// the walk ended at, and the last one to finish draws: it finds the piece that u falls into by the pieces' masses and reads
+// that one again.  What is drawn from (p - q)+ needs the exact sums of p and q first, and gets its masses and its
+// draw in a third launch.  Which workgroup finishes last changes nothing but who draws.
 #include <algorithm>
 
 #include "paged_ops.h"
@@ -25,7 +27,7 @@ constexpr int kThreads = 256, kWaves = kThreads / 64;
 constexpr int kMaxPieces = 512;  // of a row
 constexpr double kLog2e = 1.4426950408889634074;
 
-// Of a piece of a row, or of a row: the largest logit, where it is first, and sum of e^{(x - m) / T}.  Nothing
+// Of a part of a row, or of a row: the largest logit, where it is first, and sum of e^{(x - m) / T}.  Nothing
 // above -inf: s is 0; a NaN or +inf among them: s is NaN.
 struct Stat {
     float m;
@@ -34,29 +36,44 @@ struct Stat {
 };
 
 // 2^a for a <= 0, as 2^n 2^f with a polynomial through Chebyshev's nodes of |f| <= 1/2, within 2^-45; under
-// 2^-1000 it is 2^-1000.  n comes out of the low bits of a + 1.5 * 2^52 and goes into the exponent as an integer.
-__device__ __forceinline__ double exp2_64(double a) {
+// 2^-1000, and for NaN, it is 2^-1000.  n comes out of the low bits of a + 1.5 * 2^52 and goes into the exponent as an
+// integer.
+template <int N>
+__device__ __forceinline__ void exp2_64(double (&a)[N]) {
     constexpr double magic = 6755399441055744.0;
-    a = a < -1000.0 ? -1000.0 : a;
-    const double t = a + magic, f = a - (t - magic);
-    double y = 1.0205905320493103e-07;
-    y = fma(y, f, 1.3259645243929057e-06);
-    y = fma(y, f, 1.5252672925346873e-05);
-    y = fma(y, f, 0.00015403433751254997);
-    y = fma(y, f, 0.0013333558200793719);
-    y = fma(y, f, 0.009618129193934304);
-    y = fma(y, f, 0.05550410866465168);
-    y = fma(y, f, 0.2402265069564034);
-    y = fma(y, f, 0.6931471805599462);
-    y = fma(y, f, 1.0);
-    return __hiloint2double(__double2hiint(y) + (__double2loint(t) << 20), __double2loint(y));
+    constexpr double c[] = {1.3259645243929057e-06, 1.5252672925346873e-05, 0.00015403433751254997, 0.0013333558200793719, 0.009618129193934304,
+                            0.05550410866465168, 0.2402265069564034, 0.6931471805599462, 1.0};
+    double t[N], y[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        a[i] = fmax(a[i], -1000.0);
+        t[i] = a[i] + magic;
+        a[i] -= t[i] - magic;
+        y[i] = 1.0205905320493103e-07;
+    }
+#pragma unroll
+    for (int j = 0; j < 9; ++j)
+#pragma unroll
+        for (int i = 0; i < N; ++i) y[i] = fma(y[i], a[i], c[j]);
+#pragma unroll
+    for (int i = 0; i < N; ++i) a[i] = __hiloint2double(__double2hiint(y[i]) + (__double2loint(t[i]) << 20), __double2loint(y[i]));
 }
-// e^{(x - m) / T}, k = log2(e) / T.  The difference first: logits may be far from 0.
-__device__ __forceinline__ double raw_weight(float x, float m, double k) { return exp2_64(((double)x - (double)m) * k); }
-// The same with 0 for what is under 2^-1000, -inf among it.
+// e^{(x - m) / T}, k = log2(e) / T, and 0 for what is under 2^-1000, -inf among it.  The difference first: logits may be
+// far from 0.
+template <int N>
+__device__ __forceinline__ void weights(const float (&x)[N], float m, double k, double (&v)[N]) {
+    double a[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = a[i] = ((double)x[i] - (double)m) * k;
+    exp2_64(v);
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = a[i] >= -1000.0 ? v[i] : 0.0;
+}
 __device__ __forceinline__ double weight(float x, float m, double k) {
-    const double a = ((double)x - (double)m) * k;
-    return a >= -1000.0 ? exp2_64(a) : 0.0;
+    const float in[1] = {x};
+    double v[1];
+    weights<1>(in, m, k, v);
+    return v[0];
 }
 
 template <int M>
@@ -94,25 +111,23 @@ __device__ __forceinline__ void load_logits(const T *p, int e, int vocab, float 
     }
 }
 
-// The workspace: statistics [streams][max_rows][pieces] of the target, then of the draft; then of draws from
-// (p - q)+ the mass of each piece [streams][pieces], and [streams] what is drawn from.
-struct Draw {
-    Stat p, q;  // of the row
-    int row, mode;
-};
-enum { DRAW_NONE = 0, DRAW_P = 1, DRAW_REST = 2 };
+// The workspace: statistics [streams][max_rows][parts] of the target, then of the draft; the masses [streams][pieces] of the row
+// that is drawn from, and with a draft those of q and of (p - q)+; how many workgroups of a stream are done, in the second and the
+// third launch.
 struct VerifyWs {
     Stat *p, *q;
-    double *mass;
-    Draw *draw;
+    double *mass, *mass_q, *rest;
+    int2 *done;
 };
-__host__ __device__ __forceinline__ VerifyWs verify_ws(int streams, int max_rows, int pieces, bool draft, void *ws) {
+__host__ __device__ __forceinline__ VerifyWs verify_ws(int streams, int max_rows, int parts, bool draft, void *ws) {
     VerifyWs w;
-    const size_t n = (size_t)streams * max_rows * pieces;
+    const size_t n = (size_t)streams * max_rows * parts, m = (size_t)streams * parts * kWaves;
     w.p = (Stat *)ws;
     w.q = w.p + n;
     w.mass = (double *)(w.q + (draft ? n : 0));
-    w.draw = (Draw *)(w.mass + (draft ? (size_t)streams * pieces : 0));
+    w.mass_q = w.mass + m;
+    w.rest = w.mass_q + (draft ? m : 0);
+    w.done = (int2 *)(w.rest + (draft ? m : 0));
     return w;
 }
 
@@ -122,228 +137,129 @@ __device__ __forceinline__ int2 nodes_of(const VerifyArgs &a, int s) {
     return r0 >= 0 && r1 >= r0 && r1 <= a.rows ? make_int2(r0, min(r1 - r0, a.max_rows)) : make_int2(0, 0);
 }
 
-// One piece of one row of the target (blockIdx.y 0) or the draft (1), a wave each: EPT values a lane, read V at a time.
+// ---------------------------------------------------------------- all rows
+
+// One part of one row of the target (blockIdx.y 0) or the draft (1), a wave a piece: EPT values a lane, read V at a time.
 template <class T, int EPT, bool GREEDY>
-__global__ __launch_bounds__(kThreads) void stat_kernel(VerifyArgs a, int pieces) {
+__global__ __launch_bounds__(kThreads) void stat_kernel(VerifyArgs a, int parts) {
     constexpr int V = std::min<int>(16 / (int)sizeof(T), EPT);
-    const int lane = threadIdx.x & 63;
-    const int unit = __builtin_amdgcn_readfirstlane(blockIdx.x * kWaves + (threadIdx.x >> 6));
-    const int at = unit / pieces, c = unit - at * pieces;
+    __shared__ float lm[kWaves];
+    __shared__ int lb[kWaves];
+    __shared__ double ls[kWaves];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int at = blockIdx.x / parts, part = blockIdx.x - at * parts;
     const int s = at / a.max_rows, node = at - s * a.max_rows;
-    if (s >= a.streams) return;
     const bool of_draft = blockIdx.y == 1;
+    const VerifyWs ws = verify_ws(a.streams, a.max_rows, parts, a.y != nullptr, a.ws);
+    if (node == 0 && part == 0 && !of_draft && threadIdx.x == 0) ws.done[s] = make_int2(0, 0);
     const int2 rows = nodes_of(a, s);
     if (node >= rows.y - of_draft) return;  // (nothing was drawn behind the last row)
     const T *p = of_draft ? (const T *)a.y + (rows.x + node) * a.y_row : (const T *)a.x + (rows.x + node) * a.x_row;
-    const int base = c * EPT * 64 + lane * V;
+    const int base = (part * kWaves + w) * EPT * 64 + lane * V;
     float x[EPT / V][V];
 #pragma unroll
     for (int i = 0; i < EPT / V; ++i) load_logits<T, V>(p, base + i * 64 * V, a.vocab, x[i]);
     float m = -INFINITY;
     int best = 0x7fffffff;
-    double sum = 0.0;
-    if constexpr (GREEDY) {
 #pragma unroll
-        for (int i = 0; i < EPT / V; ++i)
+    for (int i = 0; i < EPT / V; ++i)
 #pragma unroll
-            for (int j = 0; j < V; ++j)
-                if (x[i][j] > m) {
-                    m = x[i][j];
-                    best = base + i * 64 * V + j;
-                }
-        wave_argmax(m, best);
-    } else {
-#pragma unroll
-        for (int i = 0; i < EPT / V; ++i)
-#pragma unroll
-            for (int j = 0; j < V; ++j) m = fmaxf(m, x[i][j]);
-        m = wave_max(m);
-        if (m > -INFINITY) {
-            const double k = (double)(of_draft ? a.draft_inv_t : a.inv_t) * kLog2e;
-            bool bad = !(m < INFINITY);
-            double more[2] = {};
-#pragma unroll
-            for (int i = 0; i < EPT / V; ++i)
-#pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    bad |= x[i][j] != x[i][j];
-                    more[j & 1] += raw_weight(x[i][j], m, k);
-                }
-            sum = wave_sum64(bad ? __builtin_nan("") : more[0] + more[1]);
-        } else {  // nothing but -inf, or NaN
-            bool bad = false;
-#pragma unroll
-            for (int i = 0; i < EPT / V; ++i)
-#pragma unroll
-                for (int j = 0; j < V; ++j) bad |= x[i][j] != x[i][j];
-            if (__any(bad)) sum = __builtin_nan("");
+        for (int j = 0; j < V; ++j) {
+            if (GREEDY && x[i][j] > m) best = base + i * 64 * V + j;
+            m = fmaxf(m, x[i][j]);
         }
+    if constexpr (GREEDY)
+        wave_argmax(m, best);
+    else
+        m = wave_max(m);
+    double sum = 0.0;
+    if constexpr (!GREEDY) {
+        // half of the difference: that of a type's two ends stays within it
+        const float h = m == -INFINITY ? 0.0f : -0.5f * m, inv_t = of_draft ? a.draft_inv_t : a.inv_t;
+        float more[4] = {};
+#pragma unroll
+        for (int i = 0; i < EPT / V; ++i)
+#pragma unroll
+            for (int j = 0; j < V; ++j) more[j & 3] += __builtin_amdgcn_exp2f(fmaf(x[i][j], 0.5f, h) * inv_t * (float)(2.0 * kLog2e));
+        sum = wave_sum64(((double)more[0] + more[1]) + ((double)more[2] + more[3]));
     }
     if (lane == 0) {
-        const VerifyWs ws = verify_ws(a.streams, a.max_rows, pieces, a.y != nullptr, a.ws);
-        (of_draft ? ws.q : ws.p)[(size_t)at * pieces + c] = Stat{m, m > -INFINITY ? best : -1, sum};
-    }
-}
-
-// The pieces of a row together, by one wave; every lane has the result.
-template <bool GREEDY>
-__device__ __forceinline__ Stat row_stat(const Stat *c, int pieces, double k) {
-    const int lane = threadIdx.x & 63;
-    float m = -INFINITY;
-    int best = 0x7fffffff;
-    for (int i = lane; i < pieces; i += 64) {
-        const Stat o = c[i];
-        if (o.m > m) {
-            m = o.m;
-            best = o.best;
-        }
-    }
-    if constexpr (GREEDY) {
-        wave_argmax(m, best);
-        return Stat{m, m > -INFINITY ? best : -1, 0.0};
-    } else {
-        m = wave_max(m);
-        double s = 0.0;
-        for (int i = lane; i < pieces; i += 64) {
-            const Stat o = c[i];
-            if (!(o.s == 0.0)) s += o.s * weight(o.m, m, k);
-        }
-        return Stat{m, -1, wave_sum64(s)};
-    }
-}
-
-// Inclusive sums over the workgroup in 64 bits: what earlier threads hold, this thread's among them.
-__device__ __forceinline__ double scan64(double v, double *lds, double &all) {
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const double o = __shfl_up(v, d);
-        if (lane >= d) v += o;
+        lm[w] = m;
+        lb[w] = best;
+        ls[w] = sum;
     }
     __syncthreads();
-    if (lane == 63) lds[w] = v;
-    __syncthreads();
-    double before = 0.0;
-    all = 0.0;
+    if (threadIdx.x == 0) {
+        const double k = (double)(of_draft ? a.draft_inv_t : a.inv_t) * kLog2e;
+        Stat r{-INFINITY, -1, 0.0};
 #pragma unroll
-    for (int i = 0; i < kWaves; ++i) {
-        if (i < w) before += lds[i];
-        all += lds[i];
-    }
-    return before + v;
-}
-
-struct PickLds {
-    double mass[kMaxPieces];
-    double scan[kWaves];
-    double before;
-    int found, last;
-};
-
-// Of values in order, N a thread: the first whose cumulative sum, on top of `before`, passes u of `whole` (or, whole < 0, of
-// their own sum), else the last above 0; -1 where there is none.  `before` becomes the sum in front of it, whole theirs.
-template <int N>
-__device__ __forceinline__ int pick_of(const double (&v)[N], double u, double &before, double &whole, PickLds &lds) {
-    const int t = threadIdx.x;
-    double sum = 0.0, all;
-#pragma unroll
-    for (int i = 0; i < N; ++i) sum += v[i];
-    if (t == 0) {
-        lds.found = 0x7fffffff;
-        lds.last = -1;
-    }
-    double run = before + scan64(sum, lds.scan, all) - sum;
-    if (whole < 0.0) whole = all;
-    const double aim = u * whole;
-    int found = -1, last = -1;
-    double front[N];
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-        front[i] = run;
-        run += v[i];
-        if (v[i] > 0.0) last = t * N + i;
-        if (v[i] > 0.0 && run > aim && found < 0) found = t * N + i;
-    }
-    if (found >= 0) atomicMin(&lds.found, found);
-    if (last >= 0) atomicMax(&lds.last, last);
-    __syncthreads();
-    const int got = lds.found != 0x7fffffff ? lds.found : lds.last;
-    if (got >= 0 && got / N == t) {
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-            if (got % N == i) lds.before = front[i];
-    }
-    __syncthreads();
-    before = lds.before;
-    return got;
-}
-
-// What the tokens of a row weigh, up to a factor of the row.
-template <class T>
-struct Weights {
-    const T *x, *y;
-    float pm, qm;
-    double kp, kq, ps, qs;  // ps, qs: 1 / sum
-    bool rest;              // (p - q)+
-    __device__ __forceinline__ Weights(const VerifyArgs &a, const Draw &d)
-        : x((const T *)a.x + d.row * a.x_row), y((const T *)a.y + d.row * a.y_row), pm(d.p.m), qm(d.q.m), kp((double)a.inv_t * kLog2e),
-          kq((double)a.draft_inv_t * kLog2e), ps(1.0 / d.p.s), qs(1.0 / d.q.s), rest(d.mode == DRAW_REST) {}
-    // of N tokens from e on
-    template <int N>
-    __device__ __forceinline__ void of(int e, int vocab, double (&v)[N]) const {
-        float lx[N];
-        load_logits<T, N>(x, e, vocab, lx);
-        if (rest) {
-            float ly[N];
-            load_logits<T, N>(y, e, vocab, ly);
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const double d = weight(lx[i], pm, kp) * ps - weight(ly[i], qm, kq) * qs;
-                v[i] = d > 0.0 ? d : 0.0;
+        for (int i = 0; i < kWaves; ++i)
+            if (lm[i] > r.m) {
+                r.m = lm[i];
+                r.best = lb[i];
             }
-        } else {
+        if constexpr (!GREEDY)
 #pragma unroll
-            for (int i = 0; i < N; ++i) v[i] = weight(lx[i], pm, kp);
-        }
+            for (int i = 0; i < kWaves; ++i)
+                if (!(ls[i] == 0.0)) r.s += lm[i] == r.m ? ls[i] : ls[i] * weight(lm[i], r.m, k);
+        (of_draft ? ws.q : ws.p)[(size_t)at * parts + part] = r;
     }
-};
-
-// The token drawn with u; lds.mass holds the pieces' masses, -1 where there are none.  drop(first, v) leaves tokens out.
-template <class T, int EPT, class Drop>
-__device__ __forceinline__ int pick(const Weights<T> &w, int vocab, int pieces, double u, PickLds &lds, Drop &&drop) {
-    constexpr int N = EPT * 64 / kThreads, NP = kMaxPieces / kThreads;
-    const int t = threadIdx.x;
-    double mass[NP];
-#pragma unroll
-    for (int i = 0; i < NP; ++i) mass[i] = t * NP + i < pieces ? lds.mass[t * NP + i] : 0.0;
-    double before = 0.0, whole = -1.0;
-    const int c = pick_of<NP>(mass, u, before, whole, lds);
-    if (c < 0) return -1;
-    const int first = c * EPT * 64 + t * N;
-    double v[N];
-    w.template of<N>(first, vocab, v);
-    drop(first, v);
-    const int got = pick_of<N>(v, u, before, whole, lds);
-    return got < 0 ? -1 : c * EPT * 64 + got;
 }
-struct KeepAll {
-    template <int N>
-    __device__ __forceinline__ void operator()(int, double (&)[N]) const {}
-};
 
-__device__ __forceinline__ double uniform(double u) { return u < 1.0 ? (u > 0.0 ? u : 0.0) : 1.0; }  // (NaN: 1)
+// ---------------------------------------------------------------- the walk
+
+struct Draw {
+    Stat p, q;  // of the row
+    int row, mode;
+};
+enum { DRAW_NONE = 0, DRAW_P = 1, DRAW_REST = 2 };
 
 struct WalkLds {
     Stat p[kTreeMax], q[kTreeMax];
     Draw draw;
     int gone[kTreeMax], n_gone;  // the children of the last node, all rejected
-    double gone_weight[kTreeMax];
 };
 
-// The walk of one stream, by one workgroup: the rows' sums by all waves, then a lane a node.  `writes`: whether this
-// workgroup leaves the outputs.  A barrier follows.
+// The parts of a row together, by the 8 lanes that ask for it.
+template <bool GREEDY>
+__device__ __forceinline__ Stat row_stat(const Stat *c, int parts, double k) {
+    const int l = threadIdx.x & 7;
+    float m = -INFINITY;
+    int best = 0x7fffffff;
+    double s = 0.0;
+    Stat mine{-INFINITY, -1, 0.0};
+    if (l < parts) mine = c[l];
+    m = mine.m;
+    if (GREEDY && m > -INFINITY) best = mine.best;
+    for (int i = l + 8; i < parts; i += 8) {
+        if (GREEDY && c[i].m > m) best = c[i].best;
+        m = fmaxf(m, c[i].m);
+    }
+    if constexpr (GREEDY) {
+        argmax_step<4>(m, best);
+        argmax_step<2>(m, best);
+        argmax_step<1>(m, best);
+        return Stat{m, m > -INFINITY ? best : -1, 0.0};
+    } else {
+        m = fmaxf(m, xshfl<4>(m));
+        m = fmaxf(m, xshfl<2>(m));
+        m = fmaxf(m, xshfl<1>(m));
+        if (!(mine.s == 0.0)) s = mine.s * weight(mine.m, m, k);
+        for (int i = l + 8; i < parts; i += 8)
+            if (!(c[i].s == 0.0)) s += c[i].s * weight(c[i].m, m, k);
+        s += xshfl64<4>(s);
+        s += xshfl64<2>(s);
+        s += xshfl64<1>(s);
+        return Stat{m, -1, s};
+    }
+}
+
+__device__ __forceinline__ double uniform(double u) { return u < 1.0 ? (u > 0.0 ? u : 0.0) : 1.0; }  // (NaN: 1)
+
+// The walk of one stream, by one workgroup: the rows' sums by all threads, then a lane a node.  `writes`: whether this
+// workgroup leaves the outputs.
 template <class T, bool GREEDY>
-__device__ __forceinline__ void walk(const VerifyArgs &a, int s, int2 rows, const VerifyWs &ws, int pieces, bool writes, WalkLds &lds) {
+__device__ __forceinline__ void walk(const VerifyArgs &a, int s, int2 rows, const VerifyWs &ws, int parts, bool writes, WalkLds &lds) {
     const int t = threadIdx.x, n = rows.y;
     const bool drafted = a.y != nullptr;
     const double kp = (double)a.inv_t * kLog2e, kq = (double)a.draft_inv_t * kLog2e;
@@ -365,22 +281,20 @@ __device__ __forceinline__ void walk(const VerifyArgs &a, int s, int2 rows, cons
         lx = logit((const T *)a.x + (rows.x + of) * a.x_row + tok);
         if (drafted) ly = logit((const T *)a.y + (rows.x + of) * a.y_row + tok);
     }
-    for (int i = t >> 6; i < n; i += kWaves) {
-        const Stat p = row_stat<GREEDY>(ws.p + ((size_t)s * a.max_rows + i) * pieces, pieces, kp);
-        if ((t & 63) == 0) lds.p[i] = p;
-        if (!GREEDY && drafted && i < n - 1) {
-            const Stat q = row_stat<GREEDY>(ws.q + ((size_t)s * a.max_rows + i) * pieces, pieces, kq);
-            if ((t & 63) == 0) lds.q[i] = q;
-        }
+    const int all = GREEDY || !drafted ? n : 2 * n - 1;  // the target's rows, then the draft's
+    for (int i = t >> 3; i < all; i += kThreads / 8) {
+        const bool q = i >= n;
+        const Stat r = row_stat<GREEDY>((q ? ws.q : ws.p) + ((size_t)s * a.max_rows + (q ? i - n : i)) * parts, parts, q ? kq : kp);
+        if ((t & 7) == 0) (q ? lds.q[i - n] : lds.p[i]) = r;
     }
     __syncthreads();
     if (t < 64) {
         bool accept = false;
         const Stat p = lds.p[of];
-        double prob = 0.0;
         if constexpr (GREEDY) {
             accept = known && tok == p.best;
         } else {
+            double prob = 0.0;
             const bool fine = known && p.s > 0.0;  // (not NaN)
             if (fine) prob = weight(lx, p.m, kp) / p.s;
             if (drafted) {
@@ -418,11 +332,7 @@ __device__ __forceinline__ void walk(const VerifyArgs &a, int s, int2 rows, cons
         }
         const bool child = !GREEDY && !drafted && parent == cur && known;
         const uint64_t children = __ballot(child);
-        if (child) {
-            const int i = __popcll(children & ((1ull << t) - 1));
-            lds.gone[i] = tok;
-            lds.gone_weight[i] = weight(lx, p.m, kp);
-        }
+        if (child) lds.gone[__popcll(children & ((1ull << t) - 1))] = tok;
         if (t == 0) {
             const Stat pl = lds.p[cur];
             Stat ql{};
@@ -438,178 +348,324 @@ __device__ __forceinline__ void walk(const VerifyArgs &a, int s, int2 rows, cons
     __syncthreads();
 }
 
-// The pieces' masses of the row, relative to its largest logit.
-__device__ __forceinline__ void masses_of(const Stat *row, int pieces, float m, double k, PickLds &lds) {
-    for (int c = threadIdx.x; c < pieces; c += kThreads) lds.mass[c] = row[c].s == 0.0 ? 0.0 : row[c].s * weight(row[c].m, m, k);
+// ---------------------------------------------------------------- the draw
+
+// Inclusive sums over a wave, and over the workgroup: what earlier threads hold, this thread's among them.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp_add(double v) {
+    return v + __hiloint2double(__builtin_amdgcn_update_dpp(0, __double2hiint(v), CTRL, ROWS, 0xf, false),
+                                __builtin_amdgcn_update_dpp(0, __double2loint(v), CTRL, ROWS, 0xf, false));
+}
+__device__ __forceinline__ double scan64(double v, double *lds, double &all) {
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    v = dpp_add<0x111, 0xf>(v);  // one lane up, two, four, eight, within rows of 16
+    v = dpp_add<0x112, 0xf>(v);
+    v = dpp_add<0x114, 0xf>(v);
+    v = dpp_add<0x118, 0xf>(v);
+    v = dpp_add<0x142, 0xa>(v);  // the last lane of rows 0 and 2 to rows 1 and 3, of row 1 to the upper half
+    v = dpp_add<0x143, 0xc>(v);
+    __syncthreads();
+    if (lane == 63) lds[w] = v;
+    __syncthreads();
+    double before = 0.0;
+    all = 0.0;
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) {
+        if (i < w) before += lds[i];
+        all += lds[i];
+    }
+    return before + v;
 }
 
-// One workgroup a stream of tokens picked outright: the walk and the draw.
-template <class T, int EPT, bool GREEDY>
-__global__ __launch_bounds__(kThreads) void walk_kernel(VerifyArgs a, int pieces) {
-    __shared__ PickLds lds;
+struct PickLds {
+    double scan[kWaves];
+    double before;
+    int found, last;
+};
+
+// Of values in order, N a thread: the first whose cumulative sum, on top of `before`, passes u of `whole` (or, whole < 0, of
+// their own sum), else the last above 0; -1 where there is none.  `before` becomes the sum in front of it, whole theirs.
+template <int N>
+__device__ __forceinline__ int pick_of(const double (&v)[N], double u, double &before, double &whole, PickLds &lds) {
+    const int t = threadIdx.x;
+    double sum = 0.0, all;
+#pragma unroll
+    for (int i = 0; i < N; ++i) sum += v[i];
+    if (t == 0) {
+        lds.found = 0x7fffffff;
+        lds.last = -1;
+    }
+    double run = before + (scan64(sum, lds.scan, all) - sum);
+    if (whole < 0.0) whole = all;
+    const double aim = u * whole;
+    int found = -1, last = -1;
+    double front = 0.0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        if (v[i] > 0.0) {
+            last = t * N + i;
+            if (found < 0) front = run;
+            if (run + v[i] > aim && found < 0) found = t * N + i;
+        }
+        run += v[i];
+    }
+    if (found >= 0) atomicMin(&lds.found, found);
+    if (last >= 0) atomicMax(&lds.last, last);
+    __syncthreads();
+    const int got = lds.found != 0x7fffffff ? lds.found : lds.last;
+    if (got >= 0 && got / N == t) lds.before = front;  // (the last positive value's, where none was found)
+    __syncthreads();
+    before = lds.before;
+    return got;
+}
+
+// Masses go from workgroup to workgroup of one launch by stores and loads that are coherent across the XCDs' L2 caches; a
+// fence instead (which writes a whole L2 back, and empties it) took 20 us with 256 workgroups.
+__device__ __forceinline__ void put_mass(double *p, double v) {
+    __hip_atomic_store((uint64_t *)p, (uint64_t)__double_as_longlong(v), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ double get_mass(const double *p) {
+    return __longlong_as_double((long long)__hip_atomic_load((const uint64_t *)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+}
+
+// What the tokens of a row weigh, up to a factor of the row.
+template <class T>
+struct Weights {
+    const T *x, *y;
+    float pm, qm;
+    double kp, kq, ps = 1.0, qs = 1.0;  // ps, qs: 1 / sum
+    bool rest = false;                  // (p - q)+
+    __device__ __forceinline__ Weights(const VerifyArgs &a, const Draw &d)
+        : x((const T *)a.x + d.row * a.x_row), y((const T *)a.y + d.row * a.y_row), pm(d.p.m), qm(d.q.m), kp((double)a.inv_t * kLog2e),
+          kq((double)a.draft_inv_t * kLog2e) {}
+    // of N tokens from e on
+    template <int N>
+    __device__ __forceinline__ void of(int e, int vocab, double (&v)[N]) const {
+        float lx[N], ly[N];
+        load_logits<T, N>(x, e, vocab, lx);
+        if (rest) load_logits<T, N>(y, e, vocab, ly);
+        weights<N>(lx, pm, kp, v);
+        if (rest) {
+            double q[N];
+            weights<N>(ly, qm, kq, q);
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const double d = v[i] * ps - q[i] * qs;
+                v[i] = d > 0.0 ? d : 0.0;
+            }
+        }
+    }
+};
+
+struct KeepAll {
+    template <int N>
+    __device__ __forceinline__ void operator()(int, double (&)[N]) const {}
+};
+// Leaves the rejected tokens out.
+struct Drop {
+    const int *gone;
+    int n;
+    template <int N>
+    __device__ __forceinline__ void operator()(int first, double (&v)[N]) const {
+        for (int i = 0; i < n; ++i) {
+            const unsigned d = (unsigned)(gone[i] - first);
+            if (d < (unsigned)N)
+#pragma unroll
+                for (int j = 0; j < N; ++j) v[j] = (int)d == j ? 0.0 : v[j];
+        }
+    }
+};
+
+// The mass of piece c, by one wave; every lane has it.
+template <class T, int EPT, class D>
+__device__ __forceinline__ double piece_mass(const Weights<T> &w, int vocab, int c, const D &drop) {
+    constexpr int V = std::min<int>(16 / (int)sizeof(T), EPT);
+    double sum = 0.0;
+#pragma unroll
+    for (int i = 0; i < EPT / V; ++i) {
+        const int e = c * EPT * 64 + (i * 64 + ((int)threadIdx.x & 63)) * V;
+        double v[V];
+        w.template of<V>(e, vocab, v);
+        drop(e, v);
+#pragma unroll
+        for (int j = 0; j < V; ++j) sum += v[j];
+    }
+    return wave_sum64(sum);
+}
+
+// The token drawn with u; mass: the pieces'.  -1 where they are all 0.
+template <class T, int EPT, class D>
+__device__ __forceinline__ int pick(const Weights<T> &w, const double *mass, int vocab, int pieces, double u, PickLds &lds, const D &drop) {
+    constexpr int N = EPT * 64 / kThreads, NP = kMaxPieces / kThreads;
+    const int t = threadIdx.x;
+    double m[NP];
+#pragma unroll
+    for (int i = 0; i < NP; ++i) m[i] = t * NP + i < pieces ? get_mass(mass + t * NP + i) : 0.0;
+    double before = 0.0, whole = -1.0;
+    const int c = pick_of<NP>(m, u, before, whole, lds);
+    if (c < 0) return -1;
+    const int first = c * EPT * 64 + t * N;
+    double v[N];
+    w.template of<N>(first, vocab, v);
+    drop(first, v);
+    const int got = pick_of<N>(v, u, before, whole, lds);
+    return got < 0 ? -1 : c * EPT * 64 + got;
+}
+
+// Sum of a stream's pieces, the same in every workgroup: by one wave.
+__device__ __forceinline__ double sum_of(const double *mass, int pieces) {
+    double s = 0.0;
+    for (int i = threadIdx.x & 63; i < pieces; i += 64) s += mass[i];
+    return wave_sum64(s);
+}
+
+// Whether this workgroup is the last of `all` to come here: then get_mass has what the others put before.
+__device__ __forceinline__ bool last_of(int *done, int all, int *lds) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's masses have arrived
+    __syncthreads();
+    if (threadIdx.x == 0) *lds = __hip_atomic_fetch_add(done, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == all - 1;
+    __syncthreads();
+    return *lds != 0;
+}
+
+// A workgroup for each part of a stream.  With a draft, what has to come from (p - q)+ is left to the next launch.
+template <class T, int EPT, bool DRAFT>
+__global__ __launch_bounds__(kThreads) void walk_kernel(VerifyArgs a, int pieces, int parts) {
     __shared__ WalkLds wl;
-    const int s = blockIdx.x, t = threadIdx.x;
+    __shared__ PickLds lds;
+    __shared__ int last;
+    const int s = blockIdx.x / parts, part = blockIdx.x - s * parts, t = threadIdx.x;
     const int2 rows = nodes_of(a, s);
     if (rows.y == 0) {
-        if (t == 0) {
+        if (t == 0 && part == 0) {
             a.accepted[s] = 0;
             a.next[s] = -1;
         }
         return;
     }
-    const VerifyWs ws = verify_ws(a.streams, a.max_rows, pieces, false, a.ws);
-    walk<T, GREEDY>(a, s, rows, ws, pieces, true, wl);
-    if constexpr (!GREEDY) {
-        if (wl.draw.mode == DRAW_NONE) {
-            if (t == 0) a.next[s] = -1;
-            return;
-        }
-        constexpr int PIECE = EPT * 64, N = PIECE / kThreads;
-        const Weights<T> w(a, wl.draw);
-        const Stat *row = ws.p + ((size_t)s * a.max_rows + (wl.draw.row - rows.x)) * pieces;
-        const int n_gone = wl.n_gone;
-        const double u = uniform(a.uniforms[rows.x]);
-        auto drop = [&](int first, double(&v)[N]) {
-            for (int i = 0; i < n_gone; ++i) {
-                const unsigned d = (unsigned)(wl.gone[i] - first);
-                if (d < (unsigned)N)
-#pragma unroll
-                    for (int j = 0; j < N; ++j) v[j] = (int)d == j ? 0.0 : v[j];
-            }
-        };
-        masses_of(row, pieces, wl.draw.p.m, w.kp, lds);
-        __syncthreads();
-        if (n_gone > 0) {
-            // The rejected tokens' weights come off their pieces' sums, each token once.  Where less than 2^-12 is left, the
-            // difference would be coarser than 2^-40 of it, and the piece is summed again.
-            for (int c = t; c < pieces; c += kThreads) {
-                const double all = lds.mass[c];
-                double off = 0.0;
-                for (int i = 0; i < n_gone; ++i) {
-                    if (wl.gone[i] / PIECE != c) continue;
-                    bool seen = false;
-                    for (int j = 0; j < i; ++j) seen |= wl.gone[j] == wl.gone[i];
-                    if (!seen) off += wl.gone_weight[i];
-                }
-                if (off > 0.0) lds.mass[c] = all - off >= all * 0x1p-12 ? all - off : -1.0;
-            }
-            __syncthreads();
-            for (int i = 0; i < n_gone; ++i) {
-                const int c = wl.gone[i] / PIECE;
-                if (!(lds.mass[c] < 0.0)) continue;  // (of the whole workgroup)
-                double v[N], sum = 0.0, all;
-                w.template of<N>(c * PIECE + t * N, a.vocab, v);
-                drop(c * PIECE + t * N, v);
-#pragma unroll
-                for (int j = 0; j < N; ++j) sum += v[j];
-                scan64(sum, lds.scan, all);
-                if (t == 0) lds.mass[c] = all;
-                __syncthreads();
-            }
-        }
-        int got = pick<T, EPT>(w, a.vocab, pieces, u, lds, drop);
-        if (got < 0) {  // nothing is left: p itself
-            __syncthreads();
-            masses_of(row, pieces, wl.draw.p.m, w.kp, lds);
-            __syncthreads();
-            got = pick<T, EPT>(w, a.vocab, pieces, u, lds, KeepAll());
-        }
-        if (t == 0) a.next[s] = got;
-    }
-}
-
-// Chains with the draft's logits: every workgroup of a stream walks; where a token is rejected, each wave has the mass of
-// (p - q)+ in one piece of the row in front of it.
-template <class T, int EPT>
-__global__ __launch_bounds__(kThreads) void walk_draft_kernel(VerifyArgs a, int pieces, int parts) {
-    __shared__ WalkLds wl;
-    const int s = blockIdx.x / parts, part = blockIdx.x - s * parts, t = threadIdx.x;
-    const int2 rows = nodes_of(a, s);
-    const VerifyWs ws = verify_ws(a.streams, a.max_rows, pieces, true, a.ws);
-    if (rows.y == 0) {
-        if (t == 0 && part == 0) {
-            a.accepted[s] = 0;
-            ws.draw[s].mode = DRAW_NONE;
-        }
-        return;
-    }
-    walk<T, false>(a, s, rows, ws, pieces, part == 0, wl);
-    if (t == 0 && part == 0) ws.draw[s] = wl.draw;
-    const int c = part * kWaves + (t >> 6);
-    if (wl.draw.mode != DRAW_REST || c >= pieces) return;
-    constexpr int V = std::min<int>(16 / (int)sizeof(T), EPT);
-    const Weights<T> w(a, wl.draw);
-    double sum = 0.0;
-#pragma unroll 2
-    for (int i = 0; i < EPT / V; ++i) {
-        double v[V];
-        w.template of<V>(c * EPT * 64 + (i * 64 + (t & 63)) * V, a.vocab, v);
-#pragma unroll
-        for (int j = 0; j < V; ++j) sum += v[j];
-    }
-    sum = wave_sum64(sum);
-    if ((t & 63) == 0) ws.mass[(size_t)s * pieces + c] = sum;
-}
-
-// Their draw.
-template <class T, int EPT>
-__global__ __launch_bounds__(kThreads) void draw_kernel(VerifyArgs a, int pieces) {
-    __shared__ PickLds lds;
-    const int s = blockIdx.x, t = threadIdx.x;
-    const VerifyWs ws = verify_ws(a.streams, a.max_rows, pieces, true, a.ws);
-    const Draw d = ws.draw[s];
+    const VerifyWs ws = verify_ws(a.streams, a.max_rows, parts, DRAFT, a.ws);
+    walk<T, false>(a, s, rows, ws, parts, part == 0, wl);
+    const Draw d = wl.draw;
     if (d.mode == DRAW_NONE) {
-        if (t == 0) a.next[s] = -1;
+        if (t == 0 && part == 0) a.next[s] = -1;
         return;
     }
-    const int2 rows = nodes_of(a, s);
-    const double u = uniform(a.uniforms[rows.x]);
+    const int c = part * kWaves + (t >> 6);
     Weights<T> w(a, d);
-    int got = -1;
-    if (w.rest) {
-        for (int c = t; c < pieces; c += kThreads) lds.mass[c] = ws.mass[(size_t)s * pieces + c];
-        __syncthreads();
-        got = pick<T, EPT>(w, a.vocab, pieces, u, lds, KeepAll());
-        __syncthreads();
+    double *mass = ws.mass + (size_t)s * parts * kWaves;
+    const Drop drop{wl.gone, DRAFT ? 0 : wl.n_gone};
+    if (c < pieces) {
+        const double v = piece_mass<T, EPT>(w, a.vocab, c, drop);
+        if ((t & 63) == 0) put_mass(mass + c, v);
+        if (DRAFT && d.mode == DRAW_REST) {
+            Weights<T> q = w;
+            q.x = w.y;
+            q.pm = w.qm;
+            q.kp = w.kq;
+            const double vq = piece_mass<T, EPT>(q, a.vocab, c, KeepAll());
+            if ((t & 63) == 0) put_mass(ws.mass_q + (size_t)s * parts * kWaves + c, vq);
+        }
     }
-    if (got < 0) {  // all were accepted, or nothing is left over: from p itself
-        w.rest = false;
-        masses_of(ws.p + ((size_t)s * a.max_rows + (d.row - rows.x)) * pieces, pieces, d.p.m, w.kp, lds);
+    if (DRAFT && d.mode == DRAW_REST) return;
+    if (!last_of(&ws.done[s].x, parts, &last)) return;
+    const double u = uniform(a.uniforms[rows.x]);
+    int got = pick<T, EPT>(w, mass, a.vocab, pieces, u, lds, drop);
+    if (!DRAFT && got < 0) {  // nothing is left: p itself
         __syncthreads();
-        got = pick<T, EPT>(w, a.vocab, pieces, u, lds, KeepAll());
+        for (int i = t >> 6; i < pieces; i += kWaves) {
+            const double v = piece_mass<T, EPT>(w, a.vocab, i, KeepAll());
+            if ((t & 63) == 0) put_mass(mass + i, v);
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        got = pick<T, EPT>(w, mass, a.vocab, pieces, u, lds, KeepAll());
     }
     if (t == 0) a.next[s] = got;
 }
 
-// Values of a lane of a piece: few while that fills the chip, many where the pieces' sums would be much work themselves.
+template <class T, int EPT>
+__global__ __launch_bounds__(kThreads) void greedy_kernel(VerifyArgs a, int parts) {
+    __shared__ WalkLds wl;
+    const int s = blockIdx.x;
+    const int2 rows = nodes_of(a, s);
+    if (rows.y == 0) {
+        if (threadIdx.x == 0) {
+            a.accepted[s] = 0;
+            a.next[s] = -1;
+        }
+        return;
+    }
+    walk<T, true>(a, s, rows, verify_ws(a.streams, a.max_rows, parts, false, a.ws), parts, true, wl);
+}
+
+// The draw behind a rejected token: a workgroup for each part of a stream has its masses of (p - q)+, the last one draws.
+template <class T, int EPT>
+__global__ __launch_bounds__(kThreads) void rest_kernel(VerifyArgs a, int pieces, int parts) {
+    __shared__ PickLds lds;
+    __shared__ int last;
+    const int s = blockIdx.x / parts, part = blockIdx.x - s * parts, t = threadIdx.x;
+    const int2 rows = nodes_of(a, s);
+    if (rows.y == 0) return;
+    const VerifyWs ws = verify_ws(a.streams, a.max_rows, parts, true, a.ws);
+    const int node = a.accepted[s];  // (a chain's)
+    if (node >= rows.y - 1) return;
+    Draw d{};
+    d.row = rows.x + node;
+    // what the walk saw, once more
+    const size_t at = ((size_t)s * a.max_rows + node) * parts;
+    d.p = row_stat<false>(ws.p + at, parts, (double)a.inv_t * kLog2e);
+    d.q = row_stat<false>(ws.q + at, parts, (double)a.draft_inv_t * kLog2e);
+    if (!(d.p.s > 0.0) || !(d.q.s > 0.0)) return;
+    Weights<T> w(a, d);
+    const double *mass = ws.mass + (size_t)s * parts * kWaves;
+    double *rest = ws.rest + (size_t)s * parts * kWaves;
+    w.ps = 1.0 / sum_of(mass, pieces);
+    w.qs = 1.0 / sum_of(ws.mass_q + (size_t)s * parts * kWaves, pieces);
+    w.rest = true;
+    const int c = part * kWaves + (t >> 6);
+    if (c < pieces) {
+        const double v = piece_mass<T, EPT>(w, a.vocab, c, KeepAll());
+        if ((t & 63) == 0) put_mass(rest + c, v);
+    }
+    if (!last_of(&ws.done[s].y, parts, &last)) return;
+    const double u = uniform(a.uniforms[rows.x]);
+    int got = pick<T, EPT>(w, rest, a.vocab, pieces, u, lds, KeepAll());
+    if (got < 0) {  // nothing is left over: p itself
+        __syncthreads();
+        w.rest = false;
+        got = pick<T, EPT>(w, mass, a.vocab, pieces, u, lds, KeepAll());
+    }
+    if (t == 0) a.next[s] = got;
+}
+
+// Values of a lane of a piece: few while that fills the chip, many where the parts' sums would be much work themselves.
 int ept_of(int rows, int vocab) {
-    const int small = (vocab + 255) / 256;
-    if (small <= 64 && (long long)rows * small <= 4096) return 4;
+    const int small = (vocab + 1023) / 1024;  // parts of 4 values a lane
+    if (small <= 16 && (long long)rows * small <= 1024) return 4;
     return vocab <= 64 * 1024 ? 16 : 32;
 }
-int pieces_of(int rows, int vocab) {
-    const int n = ept_of(rows, vocab) * 64;
+int parts_of(int rows, int vocab) {
+    const int n = ept_of(rows, vocab) * kThreads;
     return (vocab + n - 1) / n;
 }
 static_assert(kMaxPieces * 32 * 64 >= kVocabMax, "a row's pieces");
 
 template <class T, int EPT>
 hipError_t verify_e(const VerifyArgs &a, hipStream_t s) {
-    const int pieces = pieces_of(a.streams * a.max_rows, a.vocab);
-    const dim3 grid((unsigned)(((long long)a.streams * a.max_rows * pieces + kWaves - 1) / kWaves), a.y != nullptr ? 2 : 1);
+    const int parts = parts_of(a.streams * a.max_rows, a.vocab), pieces = (a.vocab + EPT * 64 - 1) / (EPT * 64);
+    const dim3 rows((unsigned)a.streams * a.max_rows * parts, a.y != nullptr ? 2 : 1), of_streams((unsigned)a.streams * parts);
     (void)hipGetLastError();
     if (a.greedy) {
-        hipLaunchKernelGGL((stat_kernel<T, EPT, true>), grid, dim3(kThreads), 0, s, a, pieces);
-        hipLaunchKernelGGL((walk_kernel<T, EPT, true>), dim3(a.streams), dim3(kThreads), 0, s, a, pieces);
+        hipLaunchKernelGGL((stat_kernel<T, EPT, true>), rows, dim3(kThreads), 0, s, a, parts);
+        hipLaunchKernelGGL((greedy_kernel<T, EPT>), dim3(a.streams), dim3(kThreads), 0, s, a, parts);
         return hipGetLastError();
     }
-    hipLaunchKernelGGL((stat_kernel<T, EPT, false>), grid, dim3(kThreads), 0, s, a, pieces);
+    hipLaunchKernelGGL((stat_kernel<T, EPT, false>), rows, dim3(kThreads), 0, s, a, parts);
     if (a.y != nullptr) {
-        const int parts = (pieces + kWaves - 1) / kWaves;
-        hipLaunchKernelGGL((walk_draft_kernel<T, EPT>), dim3((unsigned)a.streams * parts), dim3(kThreads), 0, s, a, pieces, parts);
-        hipLaunchKernelGGL((draw_kernel<T, EPT>), dim3(a.streams), dim3(kThreads), 0, s, a, pieces);
+        hipLaunchKernelGGL((walk_kernel<T, EPT, true>), of_streams, dim3(kThreads), 0, s, a, pieces, parts);
+        hipLaunchKernelGGL((rest_kernel<T, EPT>), of_streams, dim3(kThreads), 0, s, a, pieces, parts);
     } else {
-        hipLaunchKernelGGL((walk_kernel<T, EPT, false>), dim3(a.streams), dim3(kThreads), 0, s, a, pieces);
+        hipLaunchKernelGGL((walk_kernel<T, EPT, false>), of_streams, dim3(kThreads), 0, s, a, pieces, parts);
     }
     return hipGetLastError();
 }
@@ -626,8 +682,8 @@ hipError_t verify_t(const VerifyArgs &a, hipStream_t s) {
 }  // namespace
 
 size_t verify_workspace(int streams, int max_rows, int vocab, bool draft) {
-    const VerifyWs w = verify_ws(streams, max_rows, pieces_of(streams * max_rows, vocab), draft, nullptr);
-    return (size_t)(uintptr_t)(w.draw + (draft ? streams : 0));
+    const VerifyWs w = verify_ws(streams, max_rows, parts_of(streams * max_rows, vocab), draft, nullptr);
+    return (size_t)(uintptr_t)(w.done + streams);
 }
 
 hipError_t launch_verify(const VerifyArgs &a, hipStream_t s) { return a.dtype == ELEM_F16 ? verify_t<__half>(a, s) : verify_t<float>(a, s); }
