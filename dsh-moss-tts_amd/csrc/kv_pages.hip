@@ -253,26 +253,29 @@ __global__ __launch_bounds__(kThreads) void copy_kernel(ReserveArgs a, KvLayers 
 
 constexpr int kMovesPerThread = 8;  // 16-byte pieces in flight
 
-// One workgroup: the rows of one stream in one layer's K or V, a range of heads.  All rows of a head are in registers
-// before the first is stored, so any row may take any other's place.
-__global__ __launch_bounds__(kThreads) void compact_kernel(CompactArgs a, KvLayers l, int heads_each) {
-    __shared__ uint2 from[kTreeMax], to[kTreeMax];  // page, slot
+// One workgroup: the rows of one stream in pools_each of the layers' K's and V's, heads_each heads.  The list of moves is made
+// once; then, pool by pool and a group of heads at a time, all rows of a head are in registers before the first is
+// stored, so any row may take any other's place.
+template <bool SCALES>
+__global__ __launch_bounds__(kThreads) void compact_kernel(CompactArgs a, KvLayers l, int pools_each, int heads_each) {
+    __shared__ size_t from[kTreeMax], to[kTreeMax];  // vectors of head 0
     __shared__ int moves;
     const int s = blockIdx.x, t = threadIdx.x;
     if (t < 64) {
         const int r0 = a.row_start[s], r1 = a.row_start[s + 1], ctx = a.ctx_len[s];
         bool move = false;
-        uint2 src{}, dst{};
+        size_t src = 0, dst = 0;
         if (r0 >= 0 && r1 <= a.rows && ctx >= 0 && t < min(r1 - r0, a.max_rows)) {
             const int k = a.kept[r0 + t];
             if (k >= 0 && k < r1 - r0 && k != t) {
-                const long long ps = (long long)ctx + k, pd = (long long)ctx + t;
-                const long long js = ps / a.c.page_size, jd = pd / a.c.page_size;
-                if (js < a.c.table_stride && jd < a.c.table_stride) {
+                const unsigned ps = (unsigned)ctx + k, pd = (unsigned)ctx + t;  // (below 2^31 + 2^23)
+                const unsigned js = ps / (unsigned)a.c.page_size, jd = pd / (unsigned)a.c.page_size;
+                if (js < (unsigned)a.c.table_stride && jd < (unsigned)a.c.table_stride) {
                     const int *row = a.c.table + (size_t)s * a.c.table_stride;
-                    src = make_uint2(row[js], (unsigned)(ps - js * a.c.page_size));
-                    dst = make_uint2(row[jd], (unsigned)(pd - jd * a.c.page_size));
-                    move = src.x < (unsigned)a.c.n_pages && dst.x < (unsigned)a.c.n_pages;
+                    const int pf = row[js], pt = row[jd];
+                    move = pf >= 0 && pf < a.c.n_pages && pt >= 0 && pt < a.c.n_pages;
+                    src = (size_t)pf * a.c.heads * a.c.page_size + (ps - js * a.c.page_size);
+                    dst = (size_t)pt * a.c.heads * a.c.page_size + (pd - jd * a.c.page_size);
                 }
             }
         }
@@ -287,36 +290,36 @@ __global__ __launch_bounds__(kThreads) void compact_kernel(CompactArgs a, KvLaye
     __syncthreads();
     const int m = moves;
     if (m == 0) return;
-    const int layer = blockIdx.y >> 1;
-    const bool is_v = blockIdx.y & 1;
-    char *pool = (char *)(is_v ? l.v[layer] : l.k[layer]);
-    float *scale = is_v ? l.v_scale[layer] : l.k_scale[layer];
-    const int per = a.vec_bytes / 16, of_head = m * per;
+    const int shift = __builtin_ctz(a.vec_bytes) - 4, per = 1 << shift, of_head = m << shift;  // 16-byte pieces
     const int first = blockIdx.z * heads_each, last = min(first + heads_each, a.c.heads);
     const int group = max(1, kMovesPerThread * kThreads / of_head);  // heads at a time
-    auto place = [&](uint2 p, int h) { return ((size_t)p.x * a.c.heads + h) * a.c.page_size + p.y; };
-    for (int h0 = first; h0 < last; h0 += group) {
-        const int n = min(group, last - h0), units = n * of_head;
-        uint4 x[kMovesPerThread];
-        float d[kMovesPerThread];
+    for (int pool = blockIdx.y * pools_each; pool < min((int)(blockIdx.y + 1) * pools_each, 2 * a.layers); ++pool) {
+        char *data = (char *)(pool & 1 ? l.v[pool >> 1] : l.k[pool >> 1]);
+        float *scale = pool & 1 ? l.v_scale[pool >> 1] : l.k_scale[pool >> 1];
+        for (int h0 = first; h0 < last; h0 += group) {
+            const int units = min(group, last - h0) * of_head;
+            uint4 x[kMovesPerThread];
+            float d[kMovesPerThread];
+            size_t at[kMovesPerThread];
 #pragma unroll
-        for (int i = 0; i < kMovesPerThread; ++i) {
-            const int u = i * kThreads + t;
-            if (u < units) {
-                const int h = u / of_head, r = (u - h * of_head) / per, e = u % per;
-                x[i] = *(const uint4 *)(pool + place(from[r], h0 + h) * a.vec_bytes + 16 * e);
+            for (int i = 0; i < kMovesPerThread; ++i) {
+                const int u = i * kThreads + t;
+                if (u >= units) break;
+                const int hr = u >> shift, h = hr / m, r = hr - h * m, e = u & (per - 1);
+                const size_t head = (size_t)(unsigned)((h0 + h) * a.c.page_size);
+                x[i] = *(const uint4 *)(data + (from[r] + head) * a.vec_bytes + 16 * e);
+                if (SCALES && e == 0) d[i] = scale[from[r] + head];
+                at[i] = to[r] + head;
             }
-            if (scale != nullptr && u < n * m) d[i] = scale[place(from[u % m], h0 + u / m)];
-        }
-        __syncthreads();
+            __syncthreads();
 #pragma unroll
-        for (int i = 0; i < kMovesPerThread; ++i) {
-            const int u = i * kThreads + t;
-            if (u < units) {
-                const int h = u / of_head, r = (u - h * of_head) / per, e = u % per;
-                *(uint4 *)(pool + place(to[r], h0 + h) * a.vec_bytes + 16 * e) = x[i];
+            for (int i = 0; i < kMovesPerThread; ++i) {
+                const int u = i * kThreads + t;
+                if (u >= units) break;
+                const int e = u & (per - 1);
+                *(uint4 *)(data + at[i] * a.vec_bytes + 16 * e) = x[i];
+                if (SCALES && e == 0) scale[at[i]] = d[i];
             }
-            if (scale != nullptr && u < n * m) scale[place(to[u % m], h0 + u / m)] = d[i];
         }
     }
 }
@@ -359,7 +362,17 @@ hipError_t launch_kv_reserve(const ReserveArgs &a, const KvLayers &l, hipStream_
 
 hipError_t launch_kv_compact(const CompactArgs &a, const KvLayers &l, hipStream_t s) {
     (void)hipGetLastError();
-    hipLaunchKernelGGL(compact_kernel, dim3(a.c.streams, 2 * a.layers, a.c.heads), dim3(kThreads), 0, s, a, l, 1);
+    // a workgroup all heads of a pool, of several pools where that leaves 2048, or fewer heads of one where streams are few
+    const int pools = 2 * a.layers;
+    int pools_each = 1, parts = 1;
+    while (pools_each < 8 && (long long)a.c.streams * ((pools + 2 * pools_each - 1) / (2 * pools_each)) >= 2048) pools_each *= 2;
+    while (parts < a.c.heads && (long long)a.c.streams * pools * parts < 512) parts *= 2;
+    const int heads_each = (a.c.heads + parts - 1) / parts;
+    const dim3 grid(a.c.streams, (pools + pools_each - 1) / pools_each, (a.c.heads + heads_each - 1) / heads_each);
+    if (quantised(a.c.dtype))
+        hipLaunchKernelGGL(compact_kernel<true>, grid, dim3(kThreads), 0, s, a, l, pools_each, heads_each);
+    else
+        hipLaunchKernelGGL(compact_kernel<false>, grid, dim3(kThreads), 0, s, a, l, pools_each, heads_each);
     return hipGetLastError();
 }
 
