@@ -72,12 +72,64 @@ __device__ __forceinline__ void load8(const X *p, uint4 (&raw)[sizeof(X) / 2]) {
     __builtin_memcpy(raw, p, sizeof(raw));
 }
 
+// One step of 32 columns: x as it is, or as hi + lo, times the ranks' weights.
+template <class X, int RK>
+__device__ __forceinline__ void shrink_step(const Frag (&x)[sizeof(X) / 2], const Frag (&w)[RK], f32x4_t (&acc)[RK]) {
+#pragma unroll
+    for (int k = 0; k < RK; ++k)
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(X) / 2; ++i) acc[k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[k].h, x[i].h, acc[k], 0, 0, 0);
+}
+
+// STEPS * 32 columns from x and the weights' rows on (STEPS <= 4), added to sum.  No load depends on a rank or on which rows are
+// the adapter's: ranks past the last give rows of t that are dropped later, and lanes of other rows read one that is.
+template <class X, int RK, int STEPS>
+__device__ __forceinline__ void shrink_chunk(const X *x, const __half *const (&w)[RK], int c, f32x4_t (&sum)[RK]) {
+    constexpr int W = sizeof(X) / 2;  // 16-byte loads, and operands, of 8 elements
+    uint4 raw[STEPS][W];
+    Frag f[STEPS][RK];
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) load8(x + c + 32 * s, raw[s]);
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+        for (int k = 0; k < RK; ++k) f[s][k].u = *(const uint4 *)(w[k] + c + 32 * s);
+    f32x4_t acc[RK] = {};
+    float down = 1.0f;
+    if constexpr (W == 1) {
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) {
+            const Frag v[1] = {{raw[s][0]}};
+            shrink_step<X, RK>(v, f[s], acc);
+        }
+    } else {
+        float v[STEPS][8], top = 0.0f;
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) {
+            __builtin_memcpy(v[s], raw[s], sizeof(v[s]));
+#pragma unroll
+            for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[s][i]));
+        }
+        const Power p = power_of(row_max(top));
+        down = p.down;
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) {
+            Frag h[W];
+            split8(v[s], p.up, h[0], h[1]);
+            shrink_step<X, RK>(h, f[s], acc);
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < RK; ++k)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum[k][i] = fmaf(acc[k][i], down, sum[k][i]);
+}
+
 // RK: ranks of 16 that max_rank has; RT: tiles of 16 rows.
 template <class X, class Y, int RK, int RT>
 __global__ __launch_bounds__(64 * kSlices * RT) void adapter_kernel(AdapterArgs a, int outs_each) {
-    constexpr int kWaves = kSlices * RT, kThreads = 64 * kWaves;
+    constexpr int kWaves = kSlices * RT;
     constexpr int KS = RK == 1 ? 1 : RK / 2;  // steps of 32 ranks (RK 1: one half of a step)
-    constexpr int kTop = 32 * KS;
     __shared__ float part[RT][kSlices][16 * RK][kTPitch];
     const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6);
     const int m = lane & 15, g = lane >> 4;
@@ -115,62 +167,24 @@ __global__ __launch_bounds__(64 * kSlices * RT) void adapter_kernel(AdapterArgs 
         // t = A x: a wave one tile of rows and a quarter of the chunks of columns
         {
             const int rt = w / kSlices, sl = w % kSlices;
-            const bool has = who >> (16 * rt + m) & 1;
+            const unsigned here = who >> (16 * rt) & 0xffff;
             f32x4_t sum[RK] = {};
-            if (who >> (16 * rt) & 0xffff) {
-                const X *x = (const X *)a.x + (row0 + 16 * rt + (has ? m : 0)) * a.x_row + 8 * g;
-                const __half *wa = (const __half *)a.a + ((size_t)mine * a.max_rank + m) * a.cols + 8 * g;
-                for (int c = kChunk * sl; c < a.cols; c += kChunk * kSlices) {
-                    uint4 raw[4][sizeof(X) / 2];
+            if (here) {
+                const int r = here >> m & 1 ? m : __builtin_ctz(here);
+                const X *x = (const X *)a.x + (row0 + 16 * rt + r) * a.x_row + 8 * g;
+                const __half *wa[RK];
 #pragma unroll
-                    for (int s = 0; s < 4; ++s) {
-#pragma unroll
-                        for (int i = 0; i < (int)sizeof(X) / 2; ++i) raw[s][i] = uint4{};
-                        if (has && c + 32 * s < a.cols) load8(x + c + 32 * s, raw[s]);
-                    }
-                    f32x4_t acc[RK] = {};
-                    float down = 1.0f;
-                    if constexpr (sizeof(X) == 2) {
-#pragma unroll
-                        for (int s = 0; s < 4; ++s) {
-                            if (c + 32 * s >= a.cols) break;
-                            const Frag v{raw[s][0]};
-#pragma unroll
-                            for (int k = 0; k < RK; ++k) {
-                                Frag f{uint4{}};
-                                if (16 * k + m < rank) f.u = *(const uint4 *)(wa + (size_t)16 * k * a.cols + c + 32 * s);
-                                acc[k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.h, v.h, acc[k], 0, 0, 0);
-                            }
-                        }
-                    } else {
-                        float v[4][8], top = 0.0f;
-#pragma unroll
-                        for (int s = 0; s < 4; ++s) {
-                            __builtin_memcpy(v[s], raw[s], sizeof(v[s]));
-#pragma unroll
-                            for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[s][i]));
-                        }
-                        const Power p = power_of(row_max(top));
-                        down = p.down;
-#pragma unroll
-                        for (int s = 0; s < 4; ++s) {
-                            if (c + 32 * s >= a.cols) break;
-                            Frag hi, lo;
-                            split8(v[s], p.up, hi, lo);
-#pragma unroll
-                            for (int k = 0; k < RK; ++k) {
-                                Frag f{uint4{}};
-                                if (16 * k + m < rank) f.u = *(const uint4 *)(wa + (size_t)16 * k * a.cols + c + 32 * s);
-                                acc[k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.h, hi.h, acc[k], 0, 0, 0);
-                                acc[k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.h, lo.h, acc[k], 0, 0, 0);
-                            }
-                        }
-                    }
-#pragma unroll
-                    for (int k = 0; k < RK; ++k)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) sum[k][i] = fmaf(acc[k][i], down, sum[k][i]);
-                }
+                for (int k = 0; k < RK; ++k)
+                    wa[k] = (const __half *)a.a + ((size_t)mine * a.max_rank + min(16 * k + m, a.max_rank - 1)) * a.cols + 8 * g;
+                int c = kChunk * sl;
+                for (; c + kChunk <= a.cols; c += kChunk * kSlices) shrink_chunk<X, RK, 4>(x, wa, c, sum);
+                const int left = (a.cols - c) / 32;  // of this wave's last chunk
+                if (left == 1)
+                    shrink_chunk<X, RK, 1>(x, wa, c, sum);
+                else if (left == 2)
+                    shrink_chunk<X, RK, 2>(x, wa, c, sum);
+                else if (left == 3)
+                    shrink_chunk<X, RK, 3>(x, wa, c, sum);
             }
             __syncthreads();  // (the last adapter's t is no longer read)
 #pragma unroll
@@ -189,9 +203,9 @@ __global__ __launch_bounds__(64 * kSlices * RT) void adapter_kernel(AdapterArgs 
             for (int s = 0; s < KS; ++s)
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    const int k = 32 * s + 8 * g + i;
-                    v[s][i] = 0.0f;
-                    if (k < 16 * RK) v[s][i] = (part[rt][0][k][m] + part[rt][1][k][m]) + (part[rt][2][k][m] + part[rt][3][k][m]);
+                    const int k = 32 * s + 8 * g + i, at = min(k, 16 * RK - 1);
+                    v[s][i] = (part[rt][0][at][m] + part[rt][1][at][m]) + (part[rt][2][at][m] + part[rt][3][at][m]);
+                    v[s][i] = k < rank ? v[s][i] : 0.0f;
                     top = fmaxf(top, fabsf(v[s][i]));
                 }
             const Power p = power_of(row_max(top));
@@ -199,44 +213,60 @@ __global__ __launch_bounds__(64 * kSlices * RT) void adapter_kernel(AdapterArgs 
 #pragma unroll
             for (int s = 0; s < KS; ++s) split8(v[s], p.up, hi[rt][s], lo[rt][s]);
         }
+        // B's elements past the rank may be anything: the bits of a lane's 8 that count
+        uint4 keep[KS];
+        int at_k[KS];
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            const int k = 32 * s + 8 * g;
+            at_k[s] = min(k, a.max_rank - 8);
+            auto two = [&](int i) { return (k + i < rank ? 0xffffu : 0u) | (k + i + 1 < rank ? 0xffff0000u : 0u); };
+            keep[s] = make_uint4(two(0), two(2), two(4), two(6));
+        }
         // B t: a wave 64 outputs of all rows
         constexpr int P = 16 / (int)sizeof(Y);  // outputs of a lane that lie together: output i of tile q is the lane's q * 4 + i-th
         for (int o = out0 + 64 * w; o < out1; o += 64 * kWaves) {
-            f32x4_t acc[RT][4] = {};
+            Frag f[4][KS];
+            uint4 raw[RT][16 / P];
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 // row m of the product's tile q is this output
                 const int at = P == 4 ? o + 16 * q + m : o + 32 * (q >> 1) + 8 * (m >> 2) + 4 * (q & 1) + (m & 3);
-                const __half *wb = (const __half *)a.b + ((size_t)mine * a.out + min(at, a.out - 1)) * a.max_rank + 8 * g;
+                const __half *wb = (const __half *)a.b + ((size_t)mine * a.out + min(at, a.out - 1)) * a.max_rank;
 #pragma unroll
-                for (int s = 0; s < KS; ++s) {
-                    const int k = 32 * s + 8 * g;
-                    Frag f{uint4{}};
-                    if (k < rank) {
-                        f.u = *(const uint4 *)(wb + 32 * s);
-                        if (k + 8 > rank) {  // what stands behind the rank may be anything
-#pragma unroll
-                            for (int i = 0; i < 8; ++i)
-                                if (k + i >= rank) f.e[i] = __half(0.0f);
-                        }
-                    }
-#pragma unroll
-                    for (int rt = 0; rt < RT; ++rt) {
-                        acc[rt][q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.h, hi[rt][s].h, acc[rt][q], 0, 0, 0);
-                        acc[rt][q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.h, lo[rt][s].h, acc[rt][q], 0, 0, 0);
-                    }
-                }
+                for (int s = 0; s < KS; ++s) f[q][s].u = *(const uint4 *)(wb + at_k[s]);
             }
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt) {
-                if (!(who >> (16 * rt + m) & 1)) continue;
-                const int64_t r = row0 + 16 * rt + m;
+            for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
                 for (int q = 0; q < 16 / P; ++q) {
                     const int at = P == 4 ? o + 16 * q + 4 * g : o + 32 * q + 8 * g;
-                    if (at >= out1) continue;
+                    if ((who >> (16 * rt + m) & 1) && at < out1)
+                        __builtin_memcpy(&raw[rt][q], (const Y *)a.base + (row0 + 16 * rt + m) * a.base_row + at, 16);
+                }
+            f32x4_t acc[RT][4] = {};
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+#pragma unroll
+                for (int s = 0; s < KS; ++s) {
+                    f[q][s].u.x &= keep[s].x;
+                    f[q][s].u.y &= keep[s].y;
+                    f[q][s].u.z &= keep[s].z;
+                    f[q][s].u.w &= keep[s].w;
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt) {
+                        acc[rt][q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f[q][s].h, hi[rt][s].h, acc[rt][q], 0, 0, 0);
+                        acc[rt][q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f[q][s].h, lo[rt][s].h, acc[rt][q], 0, 0, 0);
+                    }
+                }
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                for (int q = 0; q < 16 / P; ++q) {
+                    const int at = P == 4 ? o + 16 * q + 4 * g : o + 32 * q + 8 * g;
+                    if (!(who >> (16 * rt + m) & 1) || at >= out1) continue;
                     Y v[P];
-                    __builtin_memcpy(v, (const Y *)a.base + r * a.base_row + at, 16);
+                    __builtin_memcpy(v, &raw[rt][q], 16);
 #pragma unroll
                     for (int i = 0; i < P; ++i) {
                         const float y = fmaf(acc[rt][q * (P / 4) + i / 4][i & 3], factor[rt], get(v[i]));
@@ -245,13 +275,10 @@ __global__ __launch_bounds__(64 * kSlices * RT) void adapter_kernel(AdapterArgs 
                         else
                             v[i] = y;
                     }
-                    __builtin_memcpy((Y *)a.y + r * a.y_row + at, v, 16);
+                    __builtin_memcpy((Y *)a.y + (row0 + 16 * rt + m) * a.y_row + at, v, 16);
                 }
-            }
         }
     }
-    (void)kTop;
-    (void)kThreads;
 }
 
 template <class X, class Y, int RK>
