@@ -23,7 +23,8 @@ namespace {
 
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
-constexpr int kSlices = 4;    // of the columns: a wave each
+constexpr int kSlices = 8;    // of the columns: a wave each
+constexpr int kThreads = 64 * kSlices;
 constexpr int kChunk = 128;   // columns under one power of two
 constexpr int kTPitch = 17;   // of t in LDS, 16 rows wide
 
@@ -72,63 +73,64 @@ __device__ __forceinline__ void load8(const X *p, uint4 (&raw)[sizeof(X) / 2]) {
     __builtin_memcpy(raw, p, sizeof(raw));
 }
 
-// One step of 32 columns: x as it is, or as hi + lo, times the ranks' weights.
-template <class X, int RK>
-__device__ __forceinline__ void shrink_step(const Frag (&x)[sizeof(X) / 2], const Frag (&w)[RK], f32x4_t (&acc)[RK]) {
-#pragma unroll
-    for (int k = 0; k < RK; ++k)
-#pragma unroll
-        for (int i = 0; i < (int)sizeof(X) / 2; ++i) acc[k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[k].h, x[i].h, acc[k], 0, 0, 0);
-}
-
-// STEPS * 32 columns from x and the weights' rows on (STEPS <= 4), added to sum.  No load depends on a rank or on which rows are
-// the adapter's: ranks past the last give rows of t that are dropped later, and lanes of other rows read one that is.
-template <class X, int RK, int STEPS>
-__device__ __forceinline__ void shrink_chunk(const X *x, const __half *const (&w)[RK], int c, f32x4_t (&sum)[RK]) {
+// STEPS * 32 columns of RT tiles of rows from x and the weights' rows on (STEPS <= 4), added to sum.  No load depends on a rank or
+// on which rows are the adapter's: ranks past the last give rows of t that are dropped later, and lanes of other rows
+// read one that is.
+template <class X, int RK, int RT, int STEPS>
+__device__ __forceinline__ void shrink_chunk(const X *const (&x)[RT], const __half *const (&w)[RK], int c, f32x4_t (&sum)[RT][RK]) {
     constexpr int W = sizeof(X) / 2;  // 16-byte loads, and operands, of 8 elements
-    uint4 raw[STEPS][W];
+    uint4 raw[RT][STEPS][W];
     Frag f[STEPS][RK];
 #pragma unroll
-    for (int s = 0; s < STEPS; ++s) load8(x + c + 32 * s, raw[s]);
+    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) load8(x[rt] + c + 32 * s, raw[rt][s]);
 #pragma unroll
     for (int s = 0; s < STEPS; ++s)
 #pragma unroll
         for (int k = 0; k < RK; ++k) f[s][k].u = *(const uint4 *)(w[k] + c + 32 * s);
-    f32x4_t acc[RK] = {};
-    float down = 1.0f;
-    if constexpr (W == 1) {
 #pragma unroll
-        for (int s = 0; s < STEPS; ++s) {
-            const Frag v[1] = {{raw[s][0]}};
-            shrink_step<X, RK>(v, f[s], acc);
+    for (int rt = 0; rt < RT; ++rt) {
+        f32x4_t acc[RK] = {};
+        float down = 1.0f;
+        Power p{1.0f, 1.0f};
+        if constexpr (W == 2) {
+            float top = 0.0f;
+#pragma unroll
+            for (int s = 0; s < STEPS; ++s) {
+                float v[8];
+                __builtin_memcpy(v, raw[rt][s], sizeof(v));
+#pragma unroll
+                for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[i]));
+            }
+            p = power_of(row_max(top));
+            down = p.down;
         }
-    } else {
-        float v[STEPS][8], top = 0.0f;
-#pragma unroll
-        for (int s = 0; s < STEPS; ++s) {
-            __builtin_memcpy(v[s], raw[s], sizeof(v[s]));
-#pragma unroll
-            for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[s][i]));
-        }
-        const Power p = power_of(row_max(top));
-        down = p.down;
 #pragma unroll
         for (int s = 0; s < STEPS; ++s) {
             Frag h[W];
-            split8(v[s], p.up, h[0], h[1]);
-            shrink_step<X, RK>(h, f[s], acc);
+            if constexpr (W == 1) {
+                h[0].u = raw[rt][s][0];
+            } else {
+                float v[8];
+                __builtin_memcpy(v, raw[rt][s], sizeof(v));
+                split8(v, p.up, h[0], h[W - 1]);
+            }
+#pragma unroll
+            for (int k = 0; k < RK; ++k)
+#pragma unroll
+                for (int i = 0; i < W; ++i) acc[k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f[s][k].h, h[i].h, acc[k], 0, 0, 0);
         }
+#pragma unroll
+        for (int k = 0; k < RK; ++k)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sum[rt][k][i] = fmaf(acc[k][i], down, sum[rt][k][i]);
     }
-#pragma unroll
-    for (int k = 0; k < RK; ++k)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) sum[k][i] = fmaf(acc[k][i], down, sum[k][i]);
 }
 
 // RK: ranks of 16 that max_rank has; RT: tiles of 16 rows.
 template <class X, class Y, int RK, int RT>
-__global__ __launch_bounds__(64 * kSlices * RT) void adapter_kernel(AdapterArgs a, int outs_each) {
-    constexpr int kWaves = kSlices * RT;
+__global__ __launch_bounds__(kThreads) void adapter_kernel(AdapterArgs a, int outs_each) {
     constexpr int KS = RK == 1 ? 1 : RK / 2;  // steps of 32 ranks (RK 1: one half of a step)
     __shared__ float part[RT][kSlices][16 * RK][kTPitch];
     const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6);
@@ -151,7 +153,7 @@ __global__ __launch_bounds__(64 * kSlices * RT) void adapter_kernel(AdapterArgs 
         if (rank == 0) {  // y is base
             if (a.y == a.base) continue;
             const int units = (out1 - out0) * (int)sizeof(Y) / 16;
-            for (int r = w; r < 16 * RT; r += kWaves) {
+            for (int r = w; r < 16 * RT; r += kSlices) {
                 if (!(who >> r & 1)) continue;
                 const char *from = (const char *)((const Y *)a.base + (row0 + r) * a.base_row + out0);
                 char *to = (char *)((Y *)a.y + (row0 + r) * a.y_row + out0);
@@ -164,33 +166,34 @@ __global__ __launch_bounds__(64 * kSlices * RT) void adapter_kernel(AdapterArgs 
             continue;
         }
         const float scale = a.scale == nullptr ? 1.0f : a.scale[mine];
-        // t = A x: a wave one tile of rows and a quarter of the chunks of columns
+        // t = A x: a wave an eighth of the chunks of columns
         {
-            const int rt = w / kSlices, sl = w % kSlices;
-            const unsigned here = who >> (16 * rt) & 0xffff;
-            f32x4_t sum[RK] = {};
-            if (here) {
-                const int r = here >> m & 1 ? m : __builtin_ctz(here);
-                const X *x = (const X *)a.x + (row0 + 16 * rt + r) * a.x_row + 8 * g;
-                const __half *wa[RK];
+            f32x4_t sum[RT][RK] = {};
+            const X *x[RT];
+            const int some = __builtin_ctzll(who);
 #pragma unroll
-                for (int k = 0; k < RK; ++k)
-                    wa[k] = (const __half *)a.a + ((size_t)mine * a.max_rank + min(16 * k + m, a.max_rank - 1)) * a.cols + 8 * g;
-                int c = kChunk * sl;
-                for (; c + kChunk <= a.cols; c += kChunk * kSlices) shrink_chunk<X, RK, 4>(x, wa, c, sum);
-                const int left = (a.cols - c) / 32;  // of this wave's last chunk
-                if (left == 1)
-                    shrink_chunk<X, RK, 1>(x, wa, c, sum);
-                else if (left == 2)
-                    shrink_chunk<X, RK, 2>(x, wa, c, sum);
-                else if (left == 3)
-                    shrink_chunk<X, RK, 3>(x, wa, c, sum);
-            }
-            __syncthreads();  // (the last adapter's t is no longer read)
+            for (int rt = 0; rt < RT; ++rt)
+                x[rt] = (const X *)a.x + (row0 + (who >> (16 * rt + m) & 1 ? 16 * rt + m : some)) * a.x_row + 8 * g;
+            const __half *wa[RK];
 #pragma unroll
             for (int k = 0; k < RK; ++k)
+                wa[k] = (const __half *)a.a + ((size_t)mine * a.max_rank + min(16 * k + m, a.max_rank - 1)) * a.cols + 8 * g;
+            int c = kChunk * w;
+            for (; c + kChunk <= a.cols; c += kChunk * kSlices) shrink_chunk<X, RK, RT, 4>(x, wa, c, sum);
+            const int left = (a.cols - c) / 32;  // of this wave's last chunk
+            if (left == 1)
+                shrink_chunk<X, RK, RT, 1>(x, wa, c, sum);
+            else if (left == 2)
+                shrink_chunk<X, RK, RT, 2>(x, wa, c, sum);
+            else if (left == 3)
+                shrink_chunk<X, RK, RT, 3>(x, wa, c, sum);
+            __syncthreads();  // (the last adapter's t is no longer read)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) part[rt][sl][16 * k + 4 * g + i][m] = sum[k][i];
+            for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                for (int k = 0; k < RK; ++k)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) part[rt][w][16 * k + 4 * g + i][m] = sum[rt][k][i];
         }
         __syncthreads();
         // this lane's row of t in each tile: the operands of B t
@@ -204,8 +207,10 @@ __global__ __launch_bounds__(64 * kSlices * RT) void adapter_kernel(AdapterArgs 
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     const int k = 32 * s + 8 * g + i, at = min(k, 16 * RK - 1);
-                    v[s][i] = (part[rt][0][at][m] + part[rt][1][at][m]) + (part[rt][2][at][m] + part[rt][3][at][m]);
-                    v[s][i] = k < rank ? v[s][i] : 0.0f;
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int j = 0; j < kSlices; ++j) sum += part[rt][j][at][m];
+                    v[s][i] = k < rank ? sum : 0.0f;
                     top = fmaxf(top, fabsf(v[s][i]));
                 }
             const Power p = power_of(row_max(top));
@@ -225,7 +230,7 @@ __global__ __launch_bounds__(64 * kSlices * RT) void adapter_kernel(AdapterArgs 
         }
         // B t: a wave 64 outputs of all rows
         constexpr int P = 16 / (int)sizeof(Y);  // outputs of a lane that lie together: output i of tile q is the lane's q * 4 + i-th
-        for (int o = out0 + 64 * w; o < out1; o += 64 * kWaves) {
+        for (int o = out0 + 64 * w; o < out1; o += 64 * kSlices) {
             Frag f[4][KS];
             uint4 raw[RT][16 / P];
 #pragma unroll
@@ -285,18 +290,19 @@ template <class X, class Y, int RK>
 hipError_t launch(const AdapterArgs &a, hipStream_t s) {
     (void)hipGetLastError();
     const int tiles = (a.rows + 15) / 16, groups = (a.out + 63) / 64;
-    const bool wide = tiles >= 512;
-    const int blocks = wide ? (a.rows + 31) / 32 : tiles;
-    const int of_tile = std::min({wide ? 32 : 16, a.rows, a.n + 1});
-    const int each = blocks >= 256 ? 1 : of_tile;  // workgroups for the adapters of a tile
+    constexpr int kMost = RK == 8 ? 1 : 2;  // (t of two tiles of 128 ranks takes a whole unit's LDS)
+    const int rt = tiles >= 512 ? kMost : 1;
+    const int blocks = (tiles + rt - 1) / rt;
+    const int of_tile = std::min({16 * rt, a.rows, a.n + 1});
+    const int each = std::min(of_tile, std::max(2, 2048 / blocks));  // workgroups for the adapters of a tile
     const int want = std::max(1, 512 / (blocks * each));
-    const int slices = std::min(want, std::max(1, groups / 4));
+    const int slices = std::min(want, std::max(1, groups / kSlices));
     const int outs = (groups + slices - 1) / slices * 64;
     const dim3 grid(blocks, each, (a.out + outs - 1) / outs);
-    if (wide)
-        hipLaunchKernelGGL((adapter_kernel<X, Y, RK, 2>), grid, dim3(512), 0, s, a, outs);
+    if (rt == kMost)
+        hipLaunchKernelGGL((adapter_kernel<X, Y, RK, kMost>), grid, dim3(kThreads), 0, s, a, outs);
     else
-        hipLaunchKernelGGL((adapter_kernel<X, Y, RK, 1>), grid, dim3(256), 0, s, a, outs);
+        hipLaunchKernelGGL((adapter_kernel<X, Y, RK, 1>), grid, dim3(kThreads), 0, s, a, outs);
     return hipGetLastError();
 }
 
