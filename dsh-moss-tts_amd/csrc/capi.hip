@@ -713,6 +713,11 @@ mh::KvCacheArgs layer_args(const moss_hip_kv_cache *layers, int n_layers, mh::Kv
     return c;
 }
 
+void check_adapter_weights(const void *a, const void *b) {
+    if (!a || !b) throw Status(MOSS_HIP_EINVAL, "adapters: null pointer");
+    if (((uintptr_t)a | (uintptr_t)b) % 16) throw Status(MOSS_HIP_EINVAL, "adapters: weights must be 16-byte aligned");
+}
+
 mh::AdapterArgs adapter_args(const moss_hip_adapters *p) {
     if (p == nullptr) throw Status(MOSS_HIP_EINVAL, "null adapters");
     if (p->n_adapters <= 0 || p->n_adapters > (1 << 20)) throw Status(MOSS_HIP_EINVAL, "need 0 < n_adapters <= 2^20");
@@ -720,12 +725,9 @@ mh::AdapterArgs adapter_args(const moss_hip_adapters *p) {
         throw Status(MOSS_HIP_EINVAL, "max_rank must be a multiple of 16 and at most 128");
     if (p->cols <= 0 || p->cols % 32 || p->cols > 65536) throw Status(MOSS_HIP_EINVAL, "cols must be a multiple of 32 and at most 65536");
     if (p->out <= 0 || p->out % 16 || p->out > 65536) throw Status(MOSS_HIP_EINVAL, "out must be a multiple of 16 and at most 65536");
-    if (!p->a || !p->b) throw Status(MOSS_HIP_EINVAL, "adapters: null pointer");
-    if (((uintptr_t)p->a | (uintptr_t)p->b) % 16) throw Status(MOSS_HIP_EINVAL, "adapters: weights must be 16-byte aligned");
     mh::AdapterArgs a;
     a.a = p->a;
     a.b = p->b;
-    a.rank = p->rank;
     a.scale = p->scale;
     a.n = p->n_adapters;
     a.max_rank = p->max_rank;
@@ -1075,10 +1077,53 @@ int moss_hip_kv_compact(const moss_hip_kv_cache *layers, int n_layers, const int
     });
 }
 
+int moss_hip_adapter_sizes(const moss_hip_adapters *adapters, size_t *a_bytes, size_t *b_bytes) {
+    return guard([&] {
+        if (a_bytes == nullptr || b_bytes == nullptr) throw Status(MOSS_HIP_EINVAL, "null output");
+        mh::adapter_sizes(adapter_args(adapters), a_bytes, b_bytes);
+    });
+}
+
+int moss_hip_adapter_pack(const moss_hip_adapters *adapters, int first, int count, const void *a, const void *b, const int32_t *rank,
+                          void *stream) {
+    return guard([&] {
+        const mh::AdapterArgs to = adapter_args(adapters);
+        check_adapter_weights(to.a, to.b);
+        check_adapter_weights(a, b);
+        if (first < 0 || count < 0 || count > to.n || first > to.n - count || count > 65535)
+            throw Status(MOSS_HIP_EINVAL, "need first, count >= 0 within the adapters, count at most 65535");
+        if (count == 0) return;
+        mh::AdapterPackArgs p;
+        p.a = a;
+        p.b = b;
+        p.rank = rank;
+        p.count = count;
+        p.first = first;
+        p.max_rank = to.max_rank;
+        p.cols = to.cols;
+        p.out = to.out;
+        p.to_a = adapters->a;
+        p.to_b = adapters->b;
+        mh::hip_check(mh::launch_adapter_pack(p, static_cast<hipStream_t>(stream)), "adapter launch");
+    });
+}
+
+int moss_hip_adapter_rows_workspace(const moss_hip_adapters *adapters, int rows, size_t *bytes) {
+    return guard([&] {
+        if (bytes == nullptr) throw Status(MOSS_HIP_EINVAL, "null output");
+        mh::AdapterArgs a = adapter_args(adapters);
+        check_rows(rows);
+        a.rows = rows;
+        *bytes = mh::adapter_workspace(a);
+    });
+}
+
 int moss_hip_adapter_rows(const void *x, int64_t x_stride, int x_dtype, const moss_hip_adapters *adapters, const int32_t *adapter,
-                          int rows, const void *base, int64_t base_stride, void *y, int64_t y_stride, int y_dtype, void *stream) {
+                          int rows, const void *base, int64_t base_stride, void *y, int64_t y_stride, int y_dtype, void *workspace,
+                          size_t workspace_bytes, void *stream) {
     return guard([&] {
         mh::AdapterArgs a = adapter_args(adapters);
+        check_adapter_weights(a.a, a.b);
         if (!x || !adapter || !base || !y) throw Status(MOSS_HIP_EINVAL, "null pointer");
         check_row_type(x_dtype);
         check_row_type(y_dtype);
@@ -1093,6 +1138,8 @@ int moss_hip_adapter_rows(const void *x, int64_t x_stride, int x_dtype, const mo
         a.x_row = x_stride;
         a.which = adapter;
         a.rows = rows;
+        check_workspace(workspace, workspace_bytes, mh::adapter_workspace(a), "moss_hip_adapter_rows");
+        a.t = static_cast<float *>(workspace);
         a.base = base;
         a.base_row = base_stride;
         a.y = y;

@@ -162,8 +162,7 @@ hipError_t launch_verify(const VerifyArgs &a, hipStream_t s);
 // ---- low-rank adapters beside a projection
 
 struct AdapterArgs {
-    const void *a = nullptr, *b = nullptr;  // fp16 [n][max_rank][cols], [n][out][max_rank]
-    const int *rank = nullptr;   // [n], null: max_rank
+    const void *a = nullptr, *b = nullptr;  // packed weights of n adapters
     const float *scale = nullptr;  // [n], null: 1
     int n = 0, max_rank = 0, cols = 0, out = 0;
     const void *x = nullptr, *base = nullptr;
@@ -172,8 +171,20 @@ struct AdapterArgs {
     int64_t x_row = 0, base_row = 0, y_row = 0;  // row strides in elements
     const int *which = nullptr;  // [rows]
     int rows = 0;
+    float *t = nullptr;  // the workspace: A x of each row
 };
 constexpr int kAdapterRankMax = 128;
+size_t adapter_workspace(const AdapterArgs &a);                                // of ranks and rows
+void adapter_sizes(const AdapterArgs &a, size_t *a_bytes, size_t *b_bytes);  // of the packed weights
 hipError_t launch_adapter_rows(const AdapterArgs &a, hipStream_t s);
+
+struct AdapterPackArgs {
+    const void *a = nullptr, *b = nullptr;  // fp16 [count][max_rank][cols], [count][out][max_rank]
+    const int *rank = nullptr;  // [count], null: max_rank
+    int count = 0, first = 0;
+    int max_rank = 0, cols = 0, out = 0;
+    void *to_a = nullptr, *to_b = nullptr;
+};
+hipError_t launch_adapter_pack(const AdapterPackArgs &p, hipStream_t s);
 
 }  // namespace mh

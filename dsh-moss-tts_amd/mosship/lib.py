@@ -44,7 +44,8 @@ EXPORTED = [
     "moss_hip_token_logprobs", "moss_hip_token_logprobs_workspace",
     "moss_hip_verify_tokens", "moss_hip_verify_tokens_workspace",
     "moss_hip_kv_fork", "moss_hip_kv_fork_workspace", "moss_hip_kv_reserve", "moss_hip_kv_reserve_workspace",
-    "moss_hip_kv_compact", "moss_hip_adapter_rows",
+    "moss_hip_kv_compact", "moss_hip_adapter_rows", "moss_hip_adapter_rows_workspace",
+    "moss_hip_adapter_sizes", "moss_hip_adapter_pack",
     "moss_hip_codec_create", "moss_hip_codec_create_from_file", "moss_hip_codec_destroy",
     "moss_hip_codec_samples_per_frame", "moss_hip_codec_reset_stream", "moss_hip_codec_decode_chunk",
     "moss_hip_codec_decode", "moss_hip_codec_last_ms", "moss_hip_codec_stage_ms",
@@ -106,7 +107,7 @@ class KVPagesStruct(C.Structure):
 
 class AdaptersStruct(C.Structure):
     """moss_hip_adapters."""
-    _fields_ = [("a", C.c_void_p), ("b", C.c_void_p), ("rank", C.c_void_p), ("scale", C.c_void_p), ("n_adapters", C.c_int),
+    _fields_ = [("a", C.c_void_p), ("b", C.c_void_p), ("scale", C.c_void_p), ("n_adapters", C.c_int),
                 ("max_rank", C.c_int), ("cols", C.c_int), ("out", C.c_int)]
 
 
@@ -184,7 +185,10 @@ def load(path: str = LIB_PATH) -> C.CDLL:
     L.moss_hip_kv_reserve.argtypes = [vp, vp, i32, vp, vp, i32, vp, vp, sz, vp]
     L.moss_hip_kv_reserve_workspace.argtypes = [vp, i32, C.POINTER(sz)]
     L.moss_hip_kv_compact.argtypes = [vp, i32, vp, vp, vp, i32, i32, vp]
-    L.moss_hip_adapter_rows.argtypes = [vp, i64, i32, vp, vp, i32, vp, i64, vp, i64, i32, vp]
+    L.moss_hip_adapter_rows.argtypes = [vp, i64, i32, vp, vp, i32, vp, i64, vp, i64, i32, vp, sz, vp]
+    L.moss_hip_adapter_sizes.argtypes = [vp, C.POINTER(sz), C.POINTER(sz)]
+    L.moss_hip_adapter_pack.argtypes = [vp, i32, i32, vp, vp, vp, vp]
+    L.moss_hip_adapter_rows_workspace.argtypes = [vp, i32, C.POINTER(sz)]
     L.moss_hip_codec_create.argtypes = [vp, C.c_size_t, C.POINTER(CodecOptions), C.POINTER(vp)]
     L.moss_hip_codec_create_from_file.argtypes = [C.c_char_p, C.POINTER(CodecOptions), C.POINTER(vp)]
     L.moss_hip_codec_destroy.argtypes = [vp]
@@ -656,23 +660,41 @@ def kv_compact(layers: KVLayers, row_start, ctx_len, kept, max_rows: int, stream
 
 
 class Adapters:
-    """Low-rank adapters as the calls take them (moss_hip_adapters): a [n][max_rank][cols] and b [n][out][max_rank] float16,
-    rank [n] int32 (None: max_rank), scale [n] float32 (None: 1).  Keeps the tensors, owns nothing else."""
+    """Low-rank adapters a program keeps (moss_hip_adapters): a [n][max_rank][cols] and b [n][out][max_rank] float16, rank [n] int32
+    (None: max_rank), scale [n] float32 (None: 1).  Holds a copy of the weights, in the order in which the calls read them, laid out
+    on torch's current stream, and keeps the scales."""
 
     def __init__(self, a, b, rank=None, scale=None):
-        import torch
+        torch = _t()
         if a.dim() != 3 or b.dim() != 3:
             raise ValueError("a [n][max_rank][cols] and b [n][out][max_rank] are wanted")
         (n, top, cols), out = a.shape, b.shape[1]
-        self.tensors, self.device, self.cols, self.out = (a, b, rank, scale), a.get_device(), cols, out
-        self.struct = AdaptersStruct(
-            _whole("a", a, torch.float16, (n, top, cols), self.device), _whole("b", b, torch.float16, (n, out, top), self.device),
-            _whole("rank", rank, torch.int32, (n,), self.device, optional=True),
-            _whole("scale", scale, torch.float32, (n,), self.device, optional=True), n, top, cols, out)
+        self.device, self.cols, self.out, self.max_rank = a.get_device(), cols, out, top
+        self.struct = AdaptersStruct(None, None, _whole("scale", scale, torch.float32, (n,), self.device, optional=True), n, top, cols, out)
         self.ref = C.addressof(self.struct)
+        sizes = C.c_size_t(0), C.c_size_t(0)
+        check(load().moss_hip_adapter_sizes(self.ref, *(C.byref(x) for x in sizes)))
+        self.tensors = (*(torch.empty(x.value, dtype=torch.uint8, device=a.device) for x in sizes), scale)
+        self.struct.a, self.struct.b = (t.data_ptr() for t in self.tensors[:2])
+        self.set(0, a, b, rank)
+
+    def set(self, first: int, a, b, rank=None, stream=None) -> None:
+        """moss_hip_adapter_pack: adapters first .. first + len(a) - 1 take these weights."""
+        torch, dev, n = _t(), self.device, a.shape[0]
+        on = _on(dev, stream)
+        check(load().moss_hip_adapter_pack(self.ref, first, n, _whole("a", a, torch.float16, (n, self.max_rank, self.cols), dev),
+                                           _whole("b", b, torch.float16, (n, self.out, self.max_rank), dev),
+                                           _whole("rank", rank, torch.int32, (n,), dev, optional=True), on))
 
 
-def adapter_rows(x, adapters: Adapters, adapter, out, base=None, stream=None) -> None:
+def adapter_rows_workspace(adapters: Adapters, rows: int) -> int:
+    """Bytes of workspace adapter_rows takes."""
+    n = C.c_size_t(0)
+    check(load().moss_hip_adapter_rows_workspace(adapters.ref, rows, C.byref(n)))
+    return n.value
+
+
+def adapter_rows(x, adapters: Adapters, adapter, out, base=None, workspace=None, stream=None) -> None:
     """moss_hip_adapter_rows: out[r] = base[r] + scale B (A x[r]) of adapter[r] (int32; -1: none), rows of float32 or float16;
     base: out itself by default."""
     dev, base = adapters.device, out if base is None else base
@@ -685,8 +707,9 @@ def adapter_rows(x, adapters: Adapters, adapter, out, base=None, stream=None) ->
     xp, xs = _rows("x", x, 1, adapters.cols, dev)
     bp, bs = _rows("base", base, 1, adapters.out, dev)
     op, os_ = _rows("out", out, 1, adapters.out, dev)
+    wp, wb = _workspace(workspace, lambda: adapter_rows_workspace(adapters, rows), dev, stream)
     check(load().moss_hip_adapter_rows(xp, xs, _types(x), adapters.ref, _whole("adapter", adapter, _torch.int32, (rows,), dev), rows,
-                                       bp, bs, op, os_, _types(out), on))
+                                       bp, bs, op, os_, _types(out), wp, wb, on))
 
 
 # ---------------------------------------------------------------- model

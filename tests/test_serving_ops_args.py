@@ -23,7 +23,7 @@ def _pages(**kw):
 
 
 def _adapters(**kw):
-    f = dict(a=P, b=P, rank=None, scale=None, n_adapters=2, max_rank=16, cols=64, out=32)
+    f = dict(a=P, b=P, scale=None, n_adapters=2, max_rank=16, cols=64, out=32)
     f.update(kw)
     return lib.AdaptersStruct(**f)
 
@@ -133,16 +133,44 @@ def test_layers_of_one_shape():
     (dict(cols=0), "cols"), (dict(cols=48), "cols"), (dict(cols=65568), "cols"), (dict(out=0), "out"), (dict(out=24), "out"), (dict(out=65552), "out")])
 def test_bad_adapters(kw, word):
     L, a = lib.load(), _adapters(**kw)
-    _refused(L.moss_hip_adapter_rows(P, 64, lib.F32, C.addressof(a), P, 1, P, 32, P, 32, lib.F32, None), word)
+    _refused(L.moss_hip_adapter_rows(P, 64, lib.F32, C.addressof(a), P, 1, P, 32, P, 32, lib.F32, None, 0, None), word)
+    _refused(L.moss_hip_adapter_pack(C.addressof(a), 0, 1, P, P, None, None), word)
+    n = C.c_size_t()
+    if word not in ("null", "aligned"):
+        _refused(L.moss_hip_adapter_rows_workspace(C.addressof(a), 1, C.byref(n)), word)
+        _refused(L.moss_hip_adapter_sizes(C.addressof(a), C.byref(n), C.byref(n)), word)
+
+
+def test_adapter_pack_refusals():
+    L, a = lib.load(), _adapters()
+    _each(L.moss_hip_adapter_pack, [C.addressof(a), 0, 2, P, P, None, None], [
+        (0, None, "null"), (1, -1, "first"), (1, 1, "first"), (1, 1 << 31 - 1, "first"), (2, -1, "count"), (2, 3, "count"), (3, None, "null"),
+        (4, None, "null"), (3, P + 8, "aligned"), (4, P + 2, "aligned")])
+    assert L.moss_hip_adapter_pack(C.addressof(a), 2, 0, P, P, None, None) == lib.OK
+    x, y = C.c_size_t(), C.c_size_t()
+    for kw, sizes in ((dict(), (2 * 16 * 64 * 2, 2 * 64 * 16 * 2)), (dict(max_rank=48, out=80), (2 * 64 * 64 * 2, 2 * 128 * 64 * 2))):
+        b = _adapters(**kw)
+        assert L.moss_hip_adapter_sizes(C.addressof(b), C.byref(x), C.byref(y)) == lib.OK and (x.value, y.value) == sizes
+    _refused(L.moss_hip_adapter_sizes(C.addressof(a), None, C.byref(y)), "null")
 
 
 def test_adapter_rows_refusals():
     L, a = lib.load(), _adapters()
     Q = P + (1 << 20)
-    ok = [P, 64, lib.F32, C.addressof(a), P, 4, Q, 32, Q, 32, lib.F32, None]
+    ok = [P, 64, lib.F32, C.addressof(a), P, 4, Q, 32, Q, 32, lib.F32, None, 0, None]
     _each(L.moss_hip_adapter_rows, ok, [
         (0, None, "null"), (3, None, "null"), (4, None, "null"), (6, None, "null"), (8, None, "null"), (2, lib.I8, "dtype"), (10, lib.E4M3, "dtype"),
         (5, -1, "rows"), (1, -1, "negative"), (7, -1, "negative"), (9, 31, "overlap"), (7, 64, "same stride"), (8, P, "must not be x")])
     none = list(ok)
     none[5] = 0
     assert L.moss_hip_adapter_rows(*none) == lib.OK
+    n = C.c_size_t()
+    assert L.moss_hip_adapter_rows_workspace(C.addressof(a), 100, C.byref(n)) == lib.OK and n.value == 0
+    assert L.moss_hip_adapter_rows_workspace(C.addressof(a), 10000, C.byref(n)) == lib.OK and n.value == 10000 * 16 * 4
+    _refused(L.moss_hip_adapter_rows_workspace(C.addressof(a), -1, C.byref(n)), "rows")
+    _refused(L.moss_hip_adapter_rows_workspace(C.addressof(a), 1, None), "null")
+    many = list(ok)
+    many[5] = 10000
+    for ws, size, word in ((None, 0, "workspace needs"), (P, n.value - 1, "workspace needs"), (P + 8, n.value, "aligned")):
+        many[11], many[12] = ws, size
+        _refused(L.moss_hip_adapter_rows(*many), word)
