@@ -129,40 +129,36 @@ struct Tile {
     static __device__ __forceinline__ int piece_of() { return threadIdx.x & (16 * W - 1); }
 };
 
-template <class X, int RK, int RT>
+template <class X, int RK>
 struct Shrink {
     using T = Tile<X>;
     static constexpr int W = T::W;
-    const X *x[RT][T::N];  // this lane's pieces of the tiles' rows
+    const X *x[T::N];  // the rows of this lane's pieces
     const __half *w;
     int cols;
 
     __device__ __forceinline__ Shrink(const AdapterArgs &a, int id, int row0, uint64_t who) : cols(a.cols) {
         const int some = __builtin_ctzll(who);  // rows of others are not read: their lanes read this one
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-            for (int i = 0; i < T::N; ++i) {
-                const int r = 16 * rt + T::row_of(i);
-                x[rt][i] = (const X *)a.x + (row0 + (who >> r & 1 ? r : some)) * a.x_row;
-            }
+        for (int i = 0; i < T::N; ++i) {
+            const int r = T::row_of(i);
+            x[i] = (const X *)a.x + (row0 + (who >> r & 1 ? r : some)) * a.x_row;
+        }
         w = (const __half *)a.a + id * a_size(a.max_rank, a.cols) + 8 * (threadIdx.x & 63);
     }
-    __device__ __forceinline__ void load(int c, uint4 (&raw)[RT][T::N]) const {
+    __device__ __forceinline__ void load(int c, uint4 (&raw)[T::N]) const {
         const int col = c + T::piece_of() * (8 / W);
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-            for (int i = 0; i < T::N; ++i) {
-                __builtin_memcpy(&raw[rt][i], x[rt][i] + min(col, cols - 8 / W), 16);
-                if (col >= cols) raw[rt][i] = uint4{};  // (of the last chunk)
-            }
+        for (int i = 0; i < T::N; ++i) {
+            __builtin_memcpy(&raw[i], x[i] + min(col, cols - 8 / W), 16);
+            if (col >= cols) raw[i] = uint4{};  // (of the last chunk)
+        }
     }
     // Chunks c, c + step, ... of the columns, into sum.  The rows' loads run a chunk ahead.
-    __device__ __forceinline__ void run(int c, int step, uint4 *lds, f32x4_t (&sum)[RT][RK]) const {
+    __device__ __forceinline__ void run(int c, int step, uint4 *lds, f32x4_t (&sum)[RK]) const {
         if (c >= cols) return;
         const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
-        uint4 raw[RT][T::N];
+        uint4 raw[T::N];
         load(c, raw);
         while (true) {
             Frag f[4][RK];
@@ -172,51 +168,45 @@ struct Shrink {
                 for (int k = 0; k < RK; ++k) f[s][k].u = *(const uint4 *)(w + ((size_t)min(c / 32 + s, cols / 32 - 1) * RK + k) * 512);
             wave_fence();  // (the last chunk has been read)
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-                for (int i = 0; i < T::N; ++i) lds[rt * T::kBytes / 16 + T::at(T::row_of(i), T::piece_of())] = raw[rt][i];
+            for (int i = 0; i < T::N; ++i) lds[T::at(T::row_of(i), T::piece_of())] = raw[i];
             wave_fence();
             const int next = c + step;
             if (next < cols) load(next, raw);
+            f32x4_t acc[RK] = {};
+            float down = 1.0f;
+            if constexpr (W == 1) {
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt) {
-                const uint4 *tile = lds + rt * T::kBytes / 16;
-                f32x4_t acc[RK] = {};
-                float down = 1.0f;
-                if constexpr (W == 1) {
+                for (int s = 0; s < 4; ++s) {
+                    const Frag v{lds[T::at(m, 4 * s + g)]};
 #pragma unroll
-                    for (int s = 0; s < 4; ++s) {
-                        const Frag v{tile[T::at(m, 4 * s + g)]};
+                    for (int k = 0; k < RK; ++k) acc[k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f[s][k].h, v.h, acc[k], 0, 0, 0);
+                }
+            } else {
+                float v[4][8], top = 0.0f;
 #pragma unroll
-                        for (int k = 0; k < RK; ++k) acc[k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f[s][k].h, v.h, acc[k], 0, 0, 0);
-                    }
-                } else {
-                    float v[4][8], top = 0.0f;
+                for (int s = 0; s < 4; ++s) {
+                    const uint4 two[2] = {lds[T::at(m, 8 * s + 2 * g)], lds[T::at(m, 8 * s + 2 * g + 1)]};
+                    __builtin_memcpy(v[s], two, 32);
 #pragma unroll
-                    for (int s = 0; s < 4; ++s) {
-                        const uint4 two[2] = {tile[T::at(m, 8 * s + 2 * g)], tile[T::at(m, 8 * s + 2 * g + 1)]};
-                        __builtin_memcpy(v[s], two, 32);
+                    for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[s][i]));
+                }
+                const Power p = power_of(row_max(top));
+                down = p.down;
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[s][i]));
-                    }
-                    const Power p = power_of(row_max(top));
-                    down = p.down;
+                for (int s = 0; s < 4; ++s) {
+                    Frag hi, lo;
+                    split(v[s], p.up, hi, lo);
 #pragma unroll
-                    for (int s = 0; s < 4; ++s) {
-                        Frag hi, lo;
-                        split(v[s], p.up, hi, lo);
-#pragma unroll
-                        for (int k = 0; k < RK; ++k) {
-                            acc[k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f[s][k].h, hi.h, acc[k], 0, 0, 0);
-                            acc[k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f[s][k].h, lo.h, acc[k], 0, 0, 0);
-                        }
+                    for (int k = 0; k < RK; ++k) {
+                        acc[k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f[s][k].h, hi.h, acc[k], 0, 0, 0);
+                        acc[k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f[s][k].h, lo.h, acc[k], 0, 0, 0);
                     }
                 }
-#pragma unroll
-                for (int k = 0; k < RK; ++k)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) sum[rt][k][i] = fmaf(acc[k][i], down, sum[rt][k][i]);
             }
+#pragma unroll
+            for (int k = 0; k < RK; ++k)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sum[k][i] = fmaf(acc[k][i], down, sum[k][i]);
             if (next >= cols) break;
             c = next;
         }
@@ -400,15 +390,15 @@ __global__ __launch_bounds__(kThreads) void adapter_kernel(AdapterArgs a, int ou
     const int row0 = blockIdx.x * 16, out0 = blockIdx.z * outs_each, out1 = min(out0 + outs_each, a.out);
     each_adapter(a, row0, 16, [&](int id, uint64_t who) {
         if (id < 0) return copy_rows<Y>(a, row0, 16, who, out0, out1);
-        f32x4_t sum[1][RK] = {};
-        const Shrink<X, RK, 1> shrink(a, id, row0, who);
+        f32x4_t sum[RK] = {};
+        const Shrink<X, RK> shrink(a, id, row0, who);
         __syncthreads();  // (the last adapter's outputs have left LDS)
         shrink.run(kChunk * w, kChunk * kSlices, lds + w * Tile<X>::kBytes / 16, sum);
         __syncthreads();
 #pragma unroll
         for (int k = 0; k < RK; ++k)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) part[(w * 16 * RK + 16 * k + 4 * g + i) * kTPitch + m] = sum[0][k][i];
+            for (int i = 0; i < 4; ++i) part[(w * 16 * RK + 16 * k + 4 * g + i) * kTPitch + m] = sum[k][i];
         __syncthreads();
         Rows<RK> t;
         t.set(a.scale == nullptr ? 1.0f : a.scale[id], [&](int k, auto &v) {
@@ -421,78 +411,15 @@ __global__ __launch_bounds__(kThreads) void adapter_kernel(AdapterArgs a, int ou
     });
 }
 
-// The first product alone, of RT tiles of 16 rows, into t [rows][ranks].
-template <class X, int RK, int RT>
-__global__ __launch_bounds__(kThreads) void shrink_kernel(AdapterArgs a) {
-    constexpr int kPart = kSlices * RT * 16 * RK * kTPitch * 4, kTiles = kSlices * RT * Tile<X>::kBytes;
-    __shared__ uint4 lds[std::max(kPart, kTiles) / 16];
-    float *part = (float *)lds;  // [slice][tile][rank][row]
-    const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6), m = lane & 15, g = lane >> 4;
-    const int row0 = blockIdx.x * 16 * RT;
-    each_adapter(a, row0, 16 * RT, [&](int id, uint64_t who) {
-        if (id < 0) return;
-        f32x4_t sum[RT][RK] = {};
-        const Shrink<X, RK, RT> shrink(a, id, row0, who);
-        __syncthreads();
-        shrink.run(kChunk * w, kChunk * kSlices, lds + w * RT * Tile<X>::kBytes / 16, sum);
-        __syncthreads();
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-            for (int k = 0; k < RK; ++k)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) part[((w * RT + rt) * 16 * RK + 16 * k + 4 * g + i) * kTPitch + m] = sum[rt][k][i];
-        __syncthreads();
-        for (int i = t; i < RT * 256 * RK; i += kThreads) {
-            const int r = i / (16 * RK), k = i % (16 * RK);
-            if (who >> r & 1) a.t[(size_t)(row0 + r) * 16 * RK + k] = sum8(part + ((r >> 4) * 16 * RK + k) * kTPitch + (r & 15), RT * 16 * RK * kTPitch);
-        }
-    });
-}
-
-// The second one, of a tile of 16 rows and outs_each outputs, from t.
-template <class Y, int RK>
-__global__ __launch_bounds__(256) void expand_kernel(AdapterArgs a, int outs_each) {
-    __shared__ uint4 lds[4 * 256];
-    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), m = lane & 15;
-    const int row0 = blockIdx.x * 16, out0 = blockIdx.z * outs_each, out1 = min(out0 + outs_each, a.out);
-    each_adapter(a, row0, 16, [&](int id, uint64_t who) {
-        if (id < 0) return copy_rows<Y>(a, row0, 16, who, out0, out1);
-        Rows<RK> t;
-        const float *row = a.t + (size_t)(row0 + (who >> m & 1 ? m : __builtin_ctzll(who))) * 16 * RK;
-        t.set(a.scale == nullptr ? 1.0f : a.scale[id], [&](int k, auto &v) { __builtin_memcpy(v, row + k, sizeof(v)); });
-        const Expand<Y, RK> expand(a, id, row0, who, out1);
-        expand.run(out0 + 64 * w, 64 * 4, t, lds + w * 256);
-    });
-}
-
-#ifndef KRT
-#define KRT 2
-#endif
-#ifndef OUTS
-#define OUTS 1024
-#endif
-#ifndef EACH
-#define EACH 1
-#endif
-constexpr int kTwoLaunches = 1024;  // rows from which on the products are launches of their own
-
 template <class X, class Y, int RK>
 hipError_t launch(const AdapterArgs &a, hipStream_t s) {
     (void)hipGetLastError();
     const int tiles = (a.rows + 15) / 16, groups = (a.out + 63) / 64;
-    if (a.rows < kTwoLaunches) {
-        const int of_tile = std::min({16, a.rows, a.n + 1});
-        const int each = std::min(of_tile, std::max(2, 2048 / tiles));  // workgroups for the adapters of a tile
-        const int slices = std::min(std::max(1, 512 / (tiles * each)), std::max(1, groups / kSlices));
-        const int outs = (groups + slices - 1) / slices * 64;
-        hipLaunchKernelGGL((adapter_kernel<X, Y, RK>), dim3(tiles, each, (a.out + outs - 1) / outs), dim3(kThreads), 0, s, a, outs);
-        return hipGetLastError();
-    }
-    constexpr int RT = RK == 8 || sizeof(X) == 4 ? 1 : KRT;
-    hipLaunchKernelGGL((shrink_kernel<X, RK, RT>), dim3((tiles + RT - 1) / RT, EACH), dim3(kThreads), 0, s, a);
-    const int outs = OUTS;
-    hipLaunchKernelGGL((expand_kernel<Y, RK>), dim3(tiles, 1, (a.out + outs - 1) / outs), dim3(256), 0, s, a, outs);
+    const int of_tile = std::min({16, a.rows, a.n + 1});
+    const int each = std::min(of_tile, std::max(2, 512 / tiles));  // workgroups for the adapters of a tile
+    const int slices = std::min(std::max(1, 512 / (tiles * each)), std::max(1, groups / kSlices));
+    const int outs = (groups + slices - 1) / slices * 64;
+    hipLaunchKernelGGL((adapter_kernel<X, Y, RK>), dim3(tiles, each, (a.out + outs - 1) / outs), dim3(kThreads), 0, s, a, outs);
     return hipGetLastError();
 }
 
@@ -507,8 +434,6 @@ hipError_t launch_xy(const AdapterArgs &a, hipStream_t s) {
 }
 
 }  // namespace
-
-size_t adapter_workspace(const AdapterArgs &a) { return a.rows < kTwoLaunches ? 0 : (size_t)a.rows * ranks_of(a.max_rank) * sizeof(float); }
 
 void adapter_sizes(const AdapterArgs &a, size_t *a_bytes, size_t *b_bytes) {
     *a_bytes = a.n * a_size(a.max_rank, a.cols) * 2;

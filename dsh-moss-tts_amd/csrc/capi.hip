@@ -1108,19 +1108,8 @@ int moss_hip_adapter_pack(const moss_hip_adapters *adapters, int first, int coun
     });
 }
 
-int moss_hip_adapter_rows_workspace(const moss_hip_adapters *adapters, int rows, size_t *bytes) {
-    return guard([&] {
-        if (bytes == nullptr) throw Status(MOSS_HIP_EINVAL, "null output");
-        mh::AdapterArgs a = adapter_args(adapters);
-        check_rows(rows);
-        a.rows = rows;
-        *bytes = mh::adapter_workspace(a);
-    });
-}
-
 int moss_hip_adapter_rows(const void *x, int64_t x_stride, int x_dtype, const moss_hip_adapters *adapters, const int32_t *adapter,
-                          int rows, const void *base, int64_t base_stride, void *y, int64_t y_stride, int y_dtype, void *workspace,
-                          size_t workspace_bytes, void *stream) {
+                          int rows, const void *base, int64_t base_stride, void *y, int64_t y_stride, int y_dtype, void *stream) {
     return guard([&] {
         mh::AdapterArgs a = adapter_args(adapters);
         check_adapter_weights(a.a, a.b);
@@ -1138,8 +1127,6 @@ int moss_hip_adapter_rows(const void *x, int64_t x_stride, int x_dtype, const mo
         a.x_row = x_stride;
         a.which = adapter;
         a.rows = rows;
-        check_workspace(workspace, workspace_bytes, mh::adapter_workspace(a), "moss_hip_adapter_rows");
-        a.t = static_cast<float *>(workspace);
         a.base = base;
         a.base_row = base_stride;
         a.y = y;

@@ -171,10 +171,8 @@ struct AdapterArgs {
     int64_t x_row = 0, base_row = 0, y_row = 0;  // row strides in elements
     const int *which = nullptr;  // [rows]
     int rows = 0;
-    float *t = nullptr;  // the workspace: A x of each row
 };
 constexpr int kAdapterRankMax = 128;
-size_t adapter_workspace(const AdapterArgs &a);                                // of ranks and rows
 void adapter_sizes(const AdapterArgs &a, size_t *a_bytes, size_t *b_bytes);  // of the packed weights
 hipError_t launch_adapter_rows(const AdapterArgs &a, hipStream_t s);
 

@@ -44,7 +44,7 @@ EXPORTED = [
     "moss_hip_token_logprobs", "moss_hip_token_logprobs_workspace",
     "moss_hip_verify_tokens", "moss_hip_verify_tokens_workspace",
     "moss_hip_kv_fork", "moss_hip_kv_fork_workspace", "moss_hip_kv_reserve", "moss_hip_kv_reserve_workspace",
-    "moss_hip_kv_compact", "moss_hip_adapter_rows", "moss_hip_adapter_rows_workspace",
+    "moss_hip_kv_compact", "moss_hip_adapter_rows",
     "moss_hip_adapter_sizes", "moss_hip_adapter_pack",
     "moss_hip_codec_create", "moss_hip_codec_create_from_file", "moss_hip_codec_destroy",
     "moss_hip_codec_samples_per_frame", "moss_hip_codec_reset_stream", "moss_hip_codec_decode_chunk",
@@ -185,10 +185,9 @@ def load(path: str = LIB_PATH) -> C.CDLL:
     L.moss_hip_kv_reserve.argtypes = [vp, vp, i32, vp, vp, i32, vp, vp, sz, vp]
     L.moss_hip_kv_reserve_workspace.argtypes = [vp, i32, C.POINTER(sz)]
     L.moss_hip_kv_compact.argtypes = [vp, i32, vp, vp, vp, i32, i32, vp]
-    L.moss_hip_adapter_rows.argtypes = [vp, i64, i32, vp, vp, i32, vp, i64, vp, i64, i32, vp, sz, vp]
+    L.moss_hip_adapter_rows.argtypes = [vp, i64, i32, vp, vp, i32, vp, i64, vp, i64, i32, vp]
     L.moss_hip_adapter_sizes.argtypes = [vp, C.POINTER(sz), C.POINTER(sz)]
     L.moss_hip_adapter_pack.argtypes = [vp, i32, i32, vp, vp, vp, vp]
-    L.moss_hip_adapter_rows_workspace.argtypes = [vp, i32, C.POINTER(sz)]
     L.moss_hip_codec_create.argtypes = [vp, C.c_size_t, C.POINTER(CodecOptions), C.POINTER(vp)]
     L.moss_hip_codec_create_from_file.argtypes = [C.c_char_p, C.POINTER(CodecOptions), C.POINTER(vp)]
     L.moss_hip_codec_destroy.argtypes = [vp]
@@ -687,14 +686,7 @@ class Adapters:
                                            _whole("rank", rank, torch.int32, (n,), dev, optional=True), on))
 
 
-def adapter_rows_workspace(adapters: Adapters, rows: int) -> int:
-    """Bytes of workspace adapter_rows takes."""
-    n = C.c_size_t(0)
-    check(load().moss_hip_adapter_rows_workspace(adapters.ref, rows, C.byref(n)))
-    return n.value
-
-
-def adapter_rows(x, adapters: Adapters, adapter, out, base=None, workspace=None, stream=None) -> None:
+def adapter_rows(x, adapters: Adapters, adapter, out, base=None, stream=None) -> None:
     """moss_hip_adapter_rows: out[r] = base[r] + scale B (A x[r]) of adapter[r] (int32; -1: none), rows of float32 or float16;
     base: out itself by default."""
     dev, base = adapters.device, out if base is None else base
@@ -707,9 +699,8 @@ def adapter_rows(x, adapters: Adapters, adapter, out, base=None, workspace=None,
     xp, xs = _rows("x", x, 1, adapters.cols, dev)
     bp, bs = _rows("base", base, 1, adapters.out, dev)
     op, os_ = _rows("out", out, 1, adapters.out, dev)
-    wp, wb = _workspace(workspace, lambda: adapter_rows_workspace(adapters, rows), dev, stream)
     check(load().moss_hip_adapter_rows(xp, xs, _types(x), adapters.ref, _whole("adapter", adapter, _torch.int32, (rows,), dev), rows,
-                                       bp, bs, op, os_, _types(out), wp, wb, on))
+                                       bp, bs, op, os_, _types(out), on))
 
 
 # ---------------------------------------------------------------- model

@@ -541,8 +541,7 @@ int moss_hip_kv_compact(const moss_hip_kv_cache *layers, int n_layers, const int
  *   y[r] = base[r] + scale_a B_a (A_a x[r]),  a = adapter[r];  y[r] = base[r] for an adapter outside [0, n_adapters).
  * x [rows][cols] of x_dtype, base and y [rows][out] of y_dtype (F32 or F16), row strides in elements; y may be base itself (same
  * stride), and must not overlap x, or base otherwise.  Weights (fp16) and rows are multiplied exactly, but for 32-bit rows, and A x,
- * held to 22 bits and 2^-39 of the largest (in 128 neighbouring columns); sums are held in 32 bits and y is rounded once.  workspace:
- * moss_hip_adapter_rows_workspace bytes (0 for few rows). */
+ * held to 22 bits and 2^-39 of the largest (in 128 neighbouring columns); sums are held in 32 bits and y is rounded once. */
 typedef struct {
     void *a, *b;          /* the weights, of the sizes that moss_hip_adapter_sizes says, 16-byte aligned: filled by moss_hip_adapter_pack */
     const float *scale;   /* [n_adapters]; NULL: 1 */
@@ -556,9 +555,7 @@ int moss_hip_adapter_sizes(const moss_hip_adapters *adapters, size_t *a_bytes, s
 int moss_hip_adapter_pack(const moss_hip_adapters *adapters, int first, int count, const void *a, const void *b, const int32_t *rank,
                           void *stream);
 int moss_hip_adapter_rows(const void *x, int64_t x_stride, int x_dtype, const moss_hip_adapters *adapters, const int32_t *adapter,
-                          int rows, const void *base, int64_t base_stride, void *y, int64_t y_stride, int y_dtype, void *workspace,
-                          size_t workspace_bytes, void *stream);
-int moss_hip_adapter_rows_workspace(const moss_hip_adapters *adapters, int rows, size_t *bytes);
+                          int rows, const void *base, int64_t base_stride, void *y, int64_t y_stride, int y_dtype, void *stream);
 
 /* ---- Audio codec decoder (codes -> 48 kHz stereo PCM) --------------------------------
  * The GPU replacement of moss::AudioDecoder (reference csrc/include/moss/decoder.h:14-83,

@@ -133,11 +133,10 @@ def test_layers_of_one_shape():
     (dict(cols=0), "cols"), (dict(cols=48), "cols"), (dict(cols=65568), "cols"), (dict(out=0), "out"), (dict(out=24), "out"), (dict(out=65552), "out")])
 def test_bad_adapters(kw, word):
     L, a = lib.load(), _adapters(**kw)
-    _refused(L.moss_hip_adapter_rows(P, 64, lib.F32, C.addressof(a), P, 1, P, 32, P, 32, lib.F32, None, 0, None), word)
+    _refused(L.moss_hip_adapter_rows(P, 64, lib.F32, C.addressof(a), P, 1, P, 32, P, 32, lib.F32, None), word)
     _refused(L.moss_hip_adapter_pack(C.addressof(a), 0, 1, P, P, None, None), word)
     n = C.c_size_t()
     if word not in ("null", "aligned"):
-        _refused(L.moss_hip_adapter_rows_workspace(C.addressof(a), 1, C.byref(n)), word)
         _refused(L.moss_hip_adapter_sizes(C.addressof(a), C.byref(n), C.byref(n)), word)
 
 
@@ -157,20 +156,10 @@ def test_adapter_pack_refusals():
 def test_adapter_rows_refusals():
     L, a = lib.load(), _adapters()
     Q = P + (1 << 20)
-    ok = [P, 64, lib.F32, C.addressof(a), P, 4, Q, 32, Q, 32, lib.F32, None, 0, None]
+    ok = [P, 64, lib.F32, C.addressof(a), P, 4, Q, 32, Q, 32, lib.F32, None]
     _each(L.moss_hip_adapter_rows, ok, [
         (0, None, "null"), (3, None, "null"), (4, None, "null"), (6, None, "null"), (8, None, "null"), (2, lib.I8, "dtype"), (10, lib.E4M3, "dtype"),
         (5, -1, "rows"), (1, -1, "negative"), (7, -1, "negative"), (9, 31, "overlap"), (7, 64, "same stride"), (8, P, "must not be x")])
     none = list(ok)
     none[5] = 0
     assert L.moss_hip_adapter_rows(*none) == lib.OK
-    n = C.c_size_t()
-    assert L.moss_hip_adapter_rows_workspace(C.addressof(a), 100, C.byref(n)) == lib.OK and n.value == 0
-    assert L.moss_hip_adapter_rows_workspace(C.addressof(a), 10000, C.byref(n)) == lib.OK and n.value == 10000 * 16 * 4
-    _refused(L.moss_hip_adapter_rows_workspace(C.addressof(a), -1, C.byref(n)), "rows")
-    _refused(L.moss_hip_adapter_rows_workspace(C.addressof(a), 1, None), "null")
-    many = list(ok)
-    many[5] = 10000
-    for ws, size, word in ((None, 0, "workspace needs"), (P, n.value - 1, "workspace needs"), (P + 8, n.value, "aligned")):
-        many[11], many[12] = ws, size
-        _refused(L.moss_hip_adapter_rows(*many), word)
