@@ -93,19 +93,24 @@ __device__ __forceinline__ Range range_of(const ReserveArgs &a, int s) {
 enum { MISSING = -3, SHARED = -2, STAYS = -1 };
 
 // Streams are served one after the other: an earlier stream of this call that writes the same page has
-// given it up by then, so the last of a page's holders keeps it.
-__device__ int fate_of(const ReserveArgs &a, int s, int j) {
+// given it up by then, so the last of a page's holders keeps it.  By one wave, its lanes an earlier stream each.
+__device__ __forceinline__ int fate_of(const ReserveArgs &a, int s, int j) {
     const int e = a.p.table[(size_t)s * a.p.table_stride + j];
     if (e < 0 || e >= a.p.n_pages) return MISSING;
     const int held = a.p.refs[e];
     if (held <= 1) return STAYS;
     int earlier = 0, last = 0;
-    for (int o = 0; o < s; ++o) {
-        const Range r = range_of(a, o);
-        if (j >= r.j0 && j <= r.j1 && a.p.table[(size_t)o * a.p.table_stride + j] == e) {
-            ++earlier;
-            last = o;
+    for (int o0 = 0; o0 < s; o0 += 64) {
+        const int o = o0 + ((int)threadIdx.x & 63);
+        bool same = false;
+        if (o < s) {
+            const int theirs = a.p.table[(size_t)o * a.p.table_stride + j];  // (asked for together with the range)
+            const Range r = range_of(a, o);
+            same = j >= r.j0 && j <= r.j1 && theirs == e;
         }
+        const uint64_t who = __ballot(same);
+        earlier += __popcll(who);
+        if (who) last = o0 + 63 - __builtin_clzll(who);
     }
     return held - earlier > 1 ? SHARED : last;
 }
@@ -113,25 +118,13 @@ __device__ int fate_of(const ReserveArgs &a, int s, int j) {
 // Pages that one stream's rows can touch.
 __host__ __device__ __forceinline__ int pages_of(int max_rows, int page_size) { return (max_rows + page_size - 2) / page_size + 1; }
 
-struct ReserveWs {
-    int4 *copies;  // [streams]: from page, to page, slots
-    int *free_pages;   // the lowest free ones
-    int *fate;    // [streams][pages]
-};
-__host__ __device__ __forceinline__ ReserveWs reserve_ws(const PagesArgs &p, int max_rows, void *ws) {
-    ReserveWs w;
-    w.copies = (int4 *)ws;
-    w.free_pages = (int *)(w.copies + p.streams);
-    w.fate = w.free_pages + (size_t)p.streams * pages_of(max_rows, p.page_size);
-    return w;
-}
-
-__global__ __launch_bounds__(kThreads) void fate_kernel(ReserveArgs a, long long n, int per) {
-    const long long e = (long long)blockIdx.x * kThreads + threadIdx.x;
+__global__ __launch_bounds__(kThreads) void fate_kernel(ReserveArgs a, int n, int per) {
+    const int e = __builtin_amdgcn_readfirstlane(blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6));
     if (e >= n) return;
-    const int s = (int)(e / per), r = (int)(e - (long long)s * per);
+    const int s = e / per, r = e - s * per;
     const Range g = range_of(a, s);
-    reserve_ws(a.p, a.max_rows, a.ws).fate[e] = g.j0 + r <= g.j1 ? fate_of(a, s, g.j0 + r) : STAYS;
+    const int f = g.j0 + r <= g.j1 ? fate_of(a, s, g.j0 + r) : STAYS;
+    if ((threadIdx.x & 63) == 0) a.fate[e] = f;
 }
 
 // Sum over the workgroup's earlier threads, and over all of them.
@@ -154,25 +147,17 @@ __device__ __forceinline__ int2 block_scan(int v, int *lds) {
     return make_int2(before + sum - v, all);
 }
 
-// The books of one call, by one workgroup, a thread a stream.
-__global__ __launch_bounds__(kBookThreads) void reserve_kernel(ReserveArgs a, int per) {
-    __shared__ int lds[kBookThreads / 64], unserved;
-    const ReserveWs w = reserve_ws(a.p, a.max_rows, a.ws);
+// The lowest free pages, as many as are wanted, into `list`: how many there are.  A barrier has to follow.
+__device__ __forceinline__ int lowest_free(const PagesArgs &p, int wanted, int *list, int *lds) {
     const int t = threadIdx.x;
-    if (t == 0) unserved = a.p.streams;
-    // how many pages are wanted
-    int mine = 0;
-    for (long long e = t; e < (long long)a.p.streams * per; e += kBookThreads) mine += w.fate[e] <= SHARED;
-    const int wanted = block_scan(mine, lds).y;
-    // the lowest free ones, as many as that
     int found = 0;
-    for (int p0 = 0; p0 < a.p.n_pages && found < wanted; p0 += 4 * kBookThreads) {
+    for (int p0 = 0; p0 < p.n_pages && found < wanted; p0 += 4 * kBookThreads) {
         bool is[4];
         int n = 0;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int p = p0 + 4 * t + i;
-            is[i] = p < a.p.n_pages && a.p.refs[p] == 0;
+            const int page = p0 + 4 * t + i;
+            is[i] = page < p.n_pages && p.refs[page] == 0;
             n += is[i];
         }
         const int2 at = block_scan(n, lds);
@@ -180,11 +165,84 @@ __global__ __launch_bounds__(kBookThreads) void reserve_kernel(ReserveArgs a, in
 #pragma unroll
         for (int i = 0; i < 4; ++i)
             if (is[i]) {
-                if (k < wanted) w.free_pages[k] = p0 + 4 * t + i;
+                if (k < wanted) list[k] = p0 + 4 * t + i;
                 ++k;
             }
         found += at.y;
     }
+    return found;
+}
+
+// An entry's new page.
+__device__ __forceinline__ int4 take_page(const ReserveArgs &a, int s, int j, int j0, int fate, int page) {
+    int *entry = a.p.table + (size_t)s * a.p.table_stride + j;
+    int4 copy = make_int4(0, 0, 0, 0);
+    if (fate == SHARED) {
+        const int old = *entry;
+        atomicAdd(a.p.refs + old, -1);
+        if (j == j0) copy = make_int4(old, page, a.ctx_len[s] - j * a.p.page_size, 0);
+    }
+    a.p.refs[page] = 1;
+    *entry = page;
+    return copy;
+}
+
+// The books of one call of up to 1024 entries (streams times the pages that one of them can touch), by one workgroup, a thread
+// an entry: a chain of a few dependent loads.
+__global__ __launch_bounds__(kBookThreads) void reserve_small_kernel(ReserveArgs a, int per) {
+    __shared__ int lds[kBookThreads / 64], unserved, free_pages[kBookThreads], bad[kBookThreads];
+    __shared__ int2 entries[kBookThreads];  // page, place in the table
+    const int t = threadIdx.x, s = t / per, r = t - s * per;
+    const bool in = s < a.p.streams;
+    Range g{0, -1, false};
+    if (in) g = range_of(a, s);
+    const int j = g.j0 + r;
+    int e = -1, held = 0;
+    if (j <= g.j1) e = a.p.table[(size_t)s * a.p.table_stride + j];
+    if (e < 0 || e >= a.p.n_pages) e = -1;
+    if (e >= 0) held = a.p.refs[e];
+    entries[t] = make_int2(e, j);
+    bad[t] = 0;
+    if (t == 0) unserved = a.p.streams;
+    __syncthreads();
+    int fate = STAYS;
+    if (j <= g.j1 && e < 0) fate = MISSING;
+    if (held > 1) {
+        int earlier = 0, last = 0;
+        for (int o = 0; o < s * per; ++o)
+            if (entries[o].x == e && entries[o].y == j) {
+                ++earlier;
+                last = o;
+            }
+        fate = held - earlier > 1 ? SHARED : last / per;
+    }
+    const bool need = fate <= SHARED;
+    const int2 at = block_scan(need, lds);
+    const int found = lowest_free(a.p, at.y, free_pages, lds);
+    if (need && at.x >= found) atomicMin(&unserved, s);
+    __syncthreads();
+    if (in && (!g.ok || fate >= unserved || (need && s >= unserved))) bad[s] = 1;
+    __syncthreads();
+    if (!in) return;
+    const bool ok = !bad[s];
+    int4 copy = make_int4(0, 0, 0, 0);
+    if (ok && need) copy = take_page(a, s, j, g.j0, fate, free_pages[at.x]);
+    if (r == 0) {
+        a.ok[s] = ok;
+        a.copies[s] = copy;
+    }
+}
+
+// The same for more entries: what becomes of them is in the workspace, a thread a stream.
+__global__ __launch_bounds__(kBookThreads) void reserve_kernel(ReserveArgs a, int per) {
+    __shared__ int lds[kBookThreads / 64], unserved;
+    const int t = threadIdx.x;
+    if (t == 0) unserved = a.p.streams;
+    // how many pages are wanted
+    int mine = 0;
+    for (long long e = t; e < (long long)a.p.streams * per; e += kBookThreads) mine += a.fate[e] <= SHARED;
+    const int wanted = block_scan(mine, lds).y;
+    const int found = lowest_free(a.p, wanted, a.free_pages, lds);
     __syncthreads();  // (the list is read by other threads of this workgroup)
     // Streams in their order: those before the first that finds too few are served.
     int given = 0;
@@ -193,7 +251,7 @@ __global__ __launch_bounds__(kBookThreads) void reserve_kernel(ReserveArgs a, in
         int need = 0, left = -1;
         if (s < a.p.streams)
             for (int r = 0; r < per; ++r) {
-                const int f = w.fate[(size_t)s * per + r];
+                const int f = a.fate[(size_t)s * per + r];
                 need += f <= SHARED;
                 left = max(left, f);
             }
@@ -207,45 +265,40 @@ __global__ __launch_bounds__(kBookThreads) void reserve_kernel(ReserveArgs a, in
             if (ok && need > 0) {
                 int k = given + at.x;
                 for (int j = g.j0; j <= g.j1; ++j) {
-                    const int f = w.fate[(size_t)s * per + (j - g.j0)];
+                    const int f = a.fate[(size_t)s * per + (j - g.j0)];
                     if (f > SHARED) continue;
-                    int *entry = a.p.table + (size_t)s * a.p.table_stride + j;
-                    const int page = w.free_pages[k++];
-                    if (f == SHARED) {
-                        const int old = *entry;
-                        atomicAdd(a.p.refs + old, -1);
-                        if (j == g.j0) copy = make_int4(old, page, a.ctx_len[s] - j * a.p.page_size, 0);
-                    }
-                    a.p.refs[page] = 1;
-                    *entry = page;
+                    const int4 c = take_page(a, s, j, g.j0, f, a.free_pages[k++]);
+                    if (c.z > 0) copy = c;
                 }
             }
             a.ok[s] = ok;
-            w.copies[s] = copy;
+            a.copies[s] = copy;
         }
         given += at.y;
     }
 }
 
-// 16-byte pieces and scales of one head's first `slots` positions.
+// The first `slots` positions of one head of a page in one of the layers' K's and V's.  Memory bound: 72 streams' copies of half a
+// page of 32 layers x 8 heads x 128 int8, 69 MB, 31 us (4.4 TB/s).  A workgroup of all heads, whose pieces then lie at steps of a power
+// of two, took 50.
+template <bool SCALES>
 __global__ __launch_bounds__(kThreads) void copy_kernel(ReserveArgs a, KvLayers l) {
-    const int4 c = reserve_ws(a.p, a.max_rows, a.ws).copies[blockIdx.x];
+    // Neighbouring workgroups, which go to the 8 XCDs in turn, have one stream's pools: streams differ in what there is to do, and
+    // 64 of them side by side left some XCDs with nothing (50 us).
+    const int s = blockIdx.x / (2 * a.layers), pool = blockIdx.x - s * 2 * a.layers, layer = pool >> 1;
+    const int4 c = a.copies[s];
     if (c.z <= 0) return;
-    const int layer = blockIdx.y >> 1;
-    const bool is_v = blockIdx.y & 1;
-    char *pool = (char *)(is_v ? l.v[layer] : l.k[layer]);
+    const bool is_v = pool & 1;
+    const size_t from = ((size_t)c.x * a.heads + blockIdx.y) * a.p.page_size, to = ((size_t)c.y * a.heads + blockIdx.y) * a.p.page_size;
+    char *data = (char *)(is_v ? l.v[layer] : l.k[layer]);
+    const uint4 *x = (const uint4 *)(data + from * a.vec_bytes);
+    uint4 *y = (uint4 *)(data + to * a.vec_bytes);
     const int units = c.z * a.vec_bytes / 16;
-    const size_t head = (size_t)a.p.page_size * a.vec_bytes;
-    for (int h = blockIdx.z; h < a.heads; h += gridDim.z) {
-        const uint4 *from = (const uint4 *)(pool + ((size_t)c.x * a.heads + h) * head);
-        uint4 *to = (uint4 *)(pool + ((size_t)c.y * a.heads + h) * head);
-        for (int u = threadIdx.x; u < units; u += kThreads) to[u] = from[u];
-        if (a.scales) {
-            float *scale = is_v ? l.v_scale[layer] : l.k_scale[layer];
-            const float *fs = scale + ((size_t)c.x * a.heads + h) * a.p.page_size;
-            float *ts = scale + ((size_t)c.y * a.heads + h) * a.p.page_size;
-            for (int u = threadIdx.x; u < c.z; u += kThreads) ts[u] = fs[u];
-        }
+#pragma unroll 4
+    for (int u = threadIdx.x; u < units; u += kThreads) y[u] = x[u];
+    if constexpr (SCALES) {
+        float *scale = is_v ? l.v_scale[layer] : l.k_scale[layer];
+        for (int u = threadIdx.x; u < c.z; u += kThreads) scale[to + u] = scale[from + u];
     }
 }
 
@@ -260,7 +313,8 @@ template <bool SCALES>
 __global__ __launch_bounds__(kThreads) void compact_kernel(CompactArgs a, KvLayers l, int pools_each, int heads_each) {
     __shared__ size_t from[kTreeMax], to[kTreeMax];  // vectors of head 0
     __shared__ int moves;
-    const int s = blockIdx.x, t = threadIdx.x;
+    const int of_stream = (2 * a.layers + pools_each - 1) / pools_each;  // (neighbours have one stream's pools, as above)
+    const int s = blockIdx.x / of_stream, first_pool = (blockIdx.x - s * of_stream) * pools_each, t = threadIdx.x;
     if (t < 64) {
         const int r0 = a.row_start[s], r1 = a.row_start[s + 1], ctx = a.ctx_len[s];
         bool move = false;
@@ -291,9 +345,9 @@ __global__ __launch_bounds__(kThreads) void compact_kernel(CompactArgs a, KvLaye
     const int m = moves;
     if (m == 0) return;
     const int shift = __builtin_ctz(a.vec_bytes) - 4, per = 1 << shift, of_head = m << shift;  // 16-byte pieces
-    const int first = blockIdx.z * heads_each, last = min(first + heads_each, a.c.heads);
+    const int first = blockIdx.y * heads_each, last = min(first + heads_each, a.c.heads);
     const int group = max(1, kMovesPerThread * kThreads / of_head);  // heads at a time
-    for (int pool = blockIdx.y * pools_each; pool < min((int)(blockIdx.y + 1) * pools_each, 2 * a.layers); ++pool) {
+    for (int pool = first_pool; pool < min(first_pool + pools_each, 2 * a.layers); ++pool) {
         char *data = (char *)(pool & 1 ? l.v[pool >> 1] : l.k[pool >> 1]);
         float *scale = pool & 1 ? l.v_scale[pool >> 1] : l.k_scale[pool >> 1];
         for (int h0 = first; h0 < last; h0 += group) {
@@ -346,29 +400,43 @@ hipError_t launch_kv_fork(const ForkArgs &a, hipStream_t s) {
     return hipGetLastError();
 }
 
+// The workspace: copies [streams] (from page, to page, slots); the lowest free pages, and what becomes of each entry
+// [streams][pages of a stream].
 size_t reserve_workspace(const PagesArgs &p, int max_rows) {
-    return p.streams * (sizeof(int4) + 2 * sizeof(int) * (size_t)pages_of(max_rows, p.page_size));
+    const size_t n = (size_t)p.streams * pages_of(max_rows, p.page_size);
+    return p.streams * sizeof(int4) + (n <= kBookThreads ? 0 : 2 * sizeof(int) * n);
 }
 
-hipError_t launch_kv_reserve(const ReserveArgs &a, const KvLayers &l, hipStream_t s) {
-    const int per = pages_of(a.max_rows, a.p.page_size);
-    const long long n = (long long)a.p.streams * per;
+hipError_t launch_kv_reserve(ReserveArgs a, const KvLayers &l, hipStream_t s) {
+    const int per = pages_of(a.max_rows, a.p.page_size), n = a.p.streams * per;  // (within 2^27)
+    a.copies = (int4 *)a.ws;
+    a.free_pages = (int *)(a.copies + a.p.streams);
+    a.fate = a.free_pages + n;
     (void)hipGetLastError();
-    hipLaunchKernelGGL(fate_kernel, dim3((unsigned)((n + kThreads - 1) / kThreads)), dim3(kThreads), 0, s, a, n, per);
-    hipLaunchKernelGGL(reserve_kernel, dim3(1), dim3(kBookThreads), 0, s, a, per);
-    hipLaunchKernelGGL(copy_kernel, dim3(a.p.streams, 2 * a.layers, a.heads), dim3(kThreads), 0, s, a, l);
+    if (n <= kBookThreads) {
+        hipLaunchKernelGGL(reserve_small_kernel, dim3(1), dim3(kBookThreads), 0, s, a, per);
+    } else {
+        hipLaunchKernelGGL(fate_kernel, dim3((n + 3) / 4), dim3(kThreads), 0, s, a, n, per);
+        hipLaunchKernelGGL(reserve_kernel, dim3(1), dim3(kBookThreads), 0, s, a, per);
+    }
+    const dim3 grid(a.p.streams * 2 * a.layers, a.heads);
+    if (a.scales)
+        hipLaunchKernelGGL(copy_kernel<true>, grid, dim3(kThreads), 0, s, a, l);
+    else
+        hipLaunchKernelGGL(copy_kernel<false>, grid, dim3(kThreads), 0, s, a, l);
     return hipGetLastError();
 }
 
 hipError_t launch_kv_compact(const CompactArgs &a, const KvLayers &l, hipStream_t s) {
     (void)hipGetLastError();
-    // a workgroup all heads of a pool, of several pools where that leaves 2048, or fewer heads of one where streams are few
+    // As many heads as one pass takes, and two pools where that leaves 2048 workgroups (64 streams of 32 layers x 8 heads: 36 us, one pool
+    // 42, twice the heads 42, half of them 39); fewer heads where streams are few.
     const int pools = 2 * a.layers;
-    int pools_each = 1, parts = 1;
-    while (pools_each < 8 && (long long)a.c.streams * ((pools + 2 * pools_each - 1) / (2 * pools_each)) >= 2048) pools_each *= 2;
-    while (parts < a.c.heads && (long long)a.c.streams * pools * parts < 512) parts *= 2;
-    const int heads_each = (a.c.heads + parts - 1) / parts;
-    const dim3 grid(a.c.streams, (pools + pools_each - 1) / pools_each, (a.c.heads + heads_each - 1) / heads_each);
+    int heads_each = std::max(1, std::min(a.c.heads, kMovesPerThread * kThreads * 16 / (a.max_rows * a.vec_bytes)));
+    auto parts = [&] { return (a.c.heads + heads_each - 1) / heads_each; };
+    const int pools_each = (long long)a.c.streams * pools * parts() >= 4096 ? 2 : 1;
+    while (heads_each > 1 && (long long)a.c.streams * pools * parts() < 512) heads_each /= 2;
+    const dim3 grid(a.c.streams * ((pools + pools_each - 1) / pools_each), parts());
     if (quantised(a.c.dtype))
         hipLaunchKernelGGL(compact_kernel<true>, grid, dim3(kThreads), 0, s, a, l, pools_each, heads_each);
     else

@@ -128,9 +128,11 @@ struct ReserveArgs {
     int max_rows = 0;
     int *ok = nullptr;
     void *ws = nullptr;
+    int4 *copies = nullptr;  // parts of the workspace (set at the launch)
+    int *free_pages = nullptr, *fate = nullptr;
 };
 size_t reserve_workspace(const PagesArgs &p, int max_rows);
-hipError_t launch_kv_reserve(const ReserveArgs &a, const KvLayers &l, hipStream_t s);
+hipError_t launch_kv_reserve(ReserveArgs a, const KvLayers &l, hipStream_t s);
 
 struct CompactArgs {
     KvCacheArgs c;  // of one layer: its shape and the table
