@@ -36,7 +36,7 @@ struct Stat {
 };
 
 // 2^a for a <= 0, as 2^n 2^f with a polynomial through Chebyshev's nodes of |f| <= 1/2, within 2^-45; under
-// 2^-1000, and for NaN, it is 2^-1000.  n comes out of the low bits of a + 1.5 * 2^52 and goes into the exponent as an
+// 2^-1010, and for NaN, it is 2^-1010.  n comes out of the low bits of a + 1.5 * 2^52 and goes into the exponent as an
 // integer.
 template <int N>
 __device__ __forceinline__ void exp2_64(double (&a)[N]) {
@@ -46,7 +46,7 @@ __device__ __forceinline__ void exp2_64(double (&a)[N]) {
     double t[N], y[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        a[i] = fmax(a[i], -1000.0);
+        a[i] = fmax(a[i], -1010.0);
         t[i] = a[i] + magic;
         a[i] -= t[i] - magic;
         y[i] = 1.0205905320493103e-07;
@@ -58,22 +58,20 @@ __device__ __forceinline__ void exp2_64(double (&a)[N]) {
 #pragma unroll
     for (int i = 0; i < N; ++i) a[i] = __hiloint2double(__double2hiint(y[i]) + (__double2loint(t[i]) << 20), __double2loint(y[i]));
 }
-// e^{(x - m) / T}, k = log2(e) / T, and 0 for what is under 2^-1000, -inf among it.  The difference first: logits may be
-// far from 0.
+// e^{(x - m) / T}, k = log2(e) / T.  The difference first: logits may be far from 0.  -inf is 2^-1010, and what is under kNone of
+// the largest, a million of those together too, counts as nothing.
+constexpr double kNone = 0x1p-980;
 template <int N>
 __device__ __forceinline__ void weights(const float (&x)[N], float m, double k, double (&v)[N]) {
-    double a[N];
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = a[i] = ((double)x[i] - (double)m) * k;
+    for (int i = 0; i < N; ++i) v[i] = ((double)x[i] - (double)m) * k;
     exp2_64(v);
-#pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = a[i] >= -1000.0 ? v[i] : 0.0;
 }
-__device__ __forceinline__ double weight(float x, float m, double k) {
+__device__ __forceinline__ double weight(float x, float m, double k) {  // (0 for what counts as nothing)
     const float in[1] = {x};
     double v[1];
     weights<1>(in, m, k, v);
-    return v[0];
+    return v[0] > kNone ? v[0] : 0.0;
 }
 
 template <int M>
@@ -113,11 +111,17 @@ __device__ __forceinline__ void load_logits(const T *p, int e, int vocab, float 
 
 // The workspace: statistics [streams][max_rows][parts] of the target, then of the draft; the masses [streams][pieces] of the row
 // that is drawn from, and with a draft those of q and of (p - q)+; how many workgroups of a stream are done, in the second and the
-// third launch.
+// third launch; and what the draft's streams draw from.
+struct Draw {
+    float pm, qm;  // the row's largest logits
+    int row, mode;
+};
+enum { DRAW_NONE = 0, DRAW_P = 1, DRAW_REST = 2 };
 struct VerifyWs {
     Stat *p, *q;
     double *mass, *mass_q, *rest;
     int2 *done;
+    Draw *draw;
 };
 __host__ __device__ __forceinline__ VerifyWs verify_ws(int streams, int max_rows, int parts, bool draft, void *ws) {
     VerifyWs w;
@@ -128,6 +132,7 @@ __host__ __device__ __forceinline__ VerifyWs verify_ws(int streams, int max_rows
     w.mass_q = w.mass + m;
     w.rest = w.mass_q + (draft ? m : 0);
     w.done = (int2 *)(w.rest + (draft ? m : 0));
+    w.draw = (Draw *)(w.done + streams);
     return w;
 }
 
@@ -139,26 +144,14 @@ __device__ __forceinline__ int2 nodes_of(const VerifyArgs &a, int s) {
 
 // ---------------------------------------------------------------- all rows
 
-// One part of one row of the target (blockIdx.y 0) or the draft (1), a wave a piece: EPT values a lane, read V at a time.
+// One piece of a row, by one wave: EPT values a lane, read V at a time.  Lane 0's is right.
 template <class T, int EPT, bool GREEDY>
-__global__ __launch_bounds__(kThreads) void stat_kernel(VerifyArgs a, int parts) {
+__device__ __forceinline__ Stat piece_stat(const T *p, int c, int vocab, float inv_t) {
     constexpr int V = std::min<int>(16 / (int)sizeof(T), EPT);
-    __shared__ float lm[kWaves];
-    __shared__ int lb[kWaves];
-    __shared__ double ls[kWaves];
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const int at = blockIdx.x / parts, part = blockIdx.x - at * parts;
-    const int s = at / a.max_rows, node = at - s * a.max_rows;
-    const bool of_draft = blockIdx.y == 1;
-    const VerifyWs ws = verify_ws(a.streams, a.max_rows, parts, a.y != nullptr, a.ws);
-    if (node == 0 && part == 0 && !of_draft && threadIdx.x == 0) ws.done[s] = make_int2(0, 0);
-    const int2 rows = nodes_of(a, s);
-    if (node >= rows.y - of_draft) return;  // (nothing was drawn behind the last row)
-    const T *p = of_draft ? (const T *)a.y + (rows.x + node) * a.y_row : (const T *)a.x + (rows.x + node) * a.x_row;
-    const int base = (part * kWaves + w) * EPT * 64 + lane * V;
+    const int base = c * EPT * 64 + ((int)threadIdx.x & 63) * V;
     float x[EPT / V][V];
 #pragma unroll
-    for (int i = 0; i < EPT / V; ++i) load_logits<T, V>(p, base + i * 64 * V, a.vocab, x[i]);
+    for (int i = 0; i < EPT / V; ++i) load_logits<T, V>(p, base + i * 64 * V, vocab, x[i]);
     float m = -INFINITY;
     int best = 0x7fffffff;
 #pragma unroll
@@ -168,51 +161,57 @@ __global__ __launch_bounds__(kThreads) void stat_kernel(VerifyArgs a, int parts)
             if (GREEDY && x[i][j] > m) best = base + i * 64 * V + j;
             m = fmaxf(m, x[i][j]);
         }
-    if constexpr (GREEDY)
+    if constexpr (GREEDY) {
         wave_argmax(m, best);
-    else
+        return Stat{m, m > -INFINITY ? best : -1, 0.0};
+    } else {
         m = wave_max(m);
-    double sum = 0.0;
-    if constexpr (!GREEDY) {
         // half of the difference: that of a type's two ends stays within it
-        const float h = m == -INFINITY ? 0.0f : -0.5f * m, inv_t = of_draft ? a.draft_inv_t : a.inv_t;
+        const float h = m == -INFINITY ? 0.0f : -0.5f * m;
         float more[4] = {};
 #pragma unroll
         for (int i = 0; i < EPT / V; ++i)
 #pragma unroll
             for (int j = 0; j < V; ++j) more[j & 3] += __builtin_amdgcn_exp2f(fmaf(x[i][j], 0.5f, h) * inv_t * (float)(2.0 * kLog2e));
-        sum = wave_sum64(((double)more[0] + more[1]) + ((double)more[2] + more[3]));
+        return Stat{m, -1, wave_sum64(((double)more[0] + more[1]) + ((double)more[2] + more[3]))};
     }
-    if (lane == 0) {
-        lm[w] = m;
-        lb[w] = best;
-        ls[w] = sum;
-    }
+}
+
+// One part of one row of the target (blockIdx.y 0) or the draft (1).
+template <class T, int EPT, bool GREEDY>
+__global__ __launch_bounds__(kThreads) void stat_kernel(VerifyArgs a, int parts) {
+    __shared__ Stat ls[kWaves];
+    const int at = blockIdx.x / parts, part = blockIdx.x - at * parts;
+    const int s = at / a.max_rows, node = at - s * a.max_rows;
+    const bool of_draft = blockIdx.y == 1;
+    const VerifyWs ws = verify_ws(a.streams, a.max_rows, parts, a.y != nullptr, a.ws);
+    if (node == 0 && part == 0 && !of_draft && threadIdx.x == 0) ws.done[s] = make_int2(0, 0);
+    const int2 rows = nodes_of(a, s);
+    if (node >= rows.y - of_draft) return;  // (nothing was drawn behind the last row)
+    const T *p = of_draft ? (const T *)a.y + (rows.x + node) * a.y_row : (const T *)a.x + (rows.x + node) * a.x_row;
+    const float inv_t = of_draft ? a.draft_inv_t : a.inv_t;
+    const int w = threadIdx.x >> 6;
+    const Stat mine = piece_stat<T, EPT, GREEDY>(p, part * kWaves + w, a.vocab, inv_t);
+    if ((threadIdx.x & 63) == 0) ls[w] = mine;
     __syncthreads();
     if (threadIdx.x == 0) {
-        const double k = (double)(of_draft ? a.draft_inv_t : a.inv_t) * kLog2e;
+        const double k = (double)inv_t * kLog2e;
         Stat r{-INFINITY, -1, 0.0};
 #pragma unroll
         for (int i = 0; i < kWaves; ++i)
-            if (lm[i] > r.m) {
-                r.m = lm[i];
-                r.best = lb[i];
+            if (ls[i].m > r.m) {
+                r.m = ls[i].m;
+                r.best = ls[i].best;
             }
         if constexpr (!GREEDY)
 #pragma unroll
             for (int i = 0; i < kWaves; ++i)
-                if (!(ls[i] == 0.0)) r.s += lm[i] == r.m ? ls[i] : ls[i] * weight(lm[i], r.m, k);
+                if (!(ls[i].s == 0.0)) r.s += ls[i].m == r.m ? ls[i].s : ls[i].s * weight(ls[i].m, r.m, k);
         (of_draft ? ws.q : ws.p)[(size_t)at * parts + part] = r;
     }
 }
 
 // ---------------------------------------------------------------- the walk
-
-struct Draw {
-    Stat p, q;  // of the row
-    int row, mode;
-};
-enum { DRAW_NONE = 0, DRAW_P = 1, DRAW_REST = 2 };
 
 struct WalkLds {
     Stat p[kTreeMax], q[kTreeMax];
@@ -220,17 +219,12 @@ struct WalkLds {
     int gone[kTreeMax], n_gone;  // the children of the last node, all rejected
 };
 
-// The parts of a row together, by the 8 lanes that ask for it.
+// The parts of a row together, by 8 lanes; `mine` is the lane's first.
 template <bool GREEDY>
-__device__ __forceinline__ Stat row_stat(const Stat *c, int parts, double k) {
+__device__ __forceinline__ Stat row_stat(const Stat &mine, const Stat *c, int parts, double k) {
     const int l = threadIdx.x & 7;
-    float m = -INFINITY;
-    int best = 0x7fffffff;
-    double s = 0.0;
-    Stat mine{-INFINITY, -1, 0.0};
-    if (l < parts) mine = c[l];
-    m = mine.m;
-    if (GREEDY && m > -INFINITY) best = mine.best;
+    float m = mine.m;
+    int best = GREEDY && m > -INFINITY ? mine.best : 0x7fffffff;
     for (int i = l + 8; i < parts; i += 8) {
         if (GREEDY && c[i].m > m) best = c[i].best;
         m = fmaxf(m, c[i].m);
@@ -244,9 +238,10 @@ __device__ __forceinline__ Stat row_stat(const Stat *c, int parts, double k) {
         m = fmaxf(m, xshfl<4>(m));
         m = fmaxf(m, xshfl<2>(m));
         m = fmaxf(m, xshfl<1>(m));
-        if (!(mine.s == 0.0)) s = mine.s * weight(mine.m, m, k);
+        double s = 0.0;
+        if (!(mine.s == 0.0)) s = mine.m == m ? mine.s : mine.s * weight(mine.m, m, k);
         for (int i = l + 8; i < parts; i += 8)
-            if (!(c[i].s == 0.0)) s += c[i].s * weight(c[i].m, m, k);
+            if (!(c[i].s == 0.0)) s += c[i].m == m ? c[i].s : c[i].s * weight(c[i].m, m, k);
         s += xshfl64<4>(s);
         s += xshfl64<2>(s);
         s += xshfl64<1>(s);
@@ -256,12 +251,17 @@ __device__ __forceinline__ Stat row_stat(const Stat *c, int parts, double k) {
 
 __device__ __forceinline__ double uniform(double u) { return u < 1.0 ? (u > 0.0 ? u : 0.0) : 1.0; }  // (NaN: 1)
 
-// The walk of one stream, by one workgroup: the rows' sums by all threads, then a lane a node.  `writes`: whether this
-// workgroup leaves the outputs.
+// The walk of one stream, by one workgroup: the rows' sums by all threads, then a lane a node.  pp, qq: the stream's parts; `writes`:
+// whether this workgroup leaves the outputs.  Loads that do not wait for each other come first: the chain of them is most
+// of its time.
 template <class T, bool GREEDY>
-__device__ __forceinline__ void walk(const VerifyArgs &a, int s, int2 rows, const VerifyWs &ws, int parts, bool writes, WalkLds &lds) {
+__device__ __forceinline__ void walk(const VerifyArgs &a, int s, int2 rows, const Stat *pp, const Stat *qq, int parts, bool writes, WalkLds &lds) {
     const int t = threadIdx.x, n = rows.y;
     const bool drafted = a.y != nullptr;
+    const int all = GREEDY || !drafted ? a.max_rows : 2 * a.max_rows;  // the target's rows, then the draft's; what is past n is not used
+    auto row_at = [&](int i) { return (i < a.max_rows ? pp + (size_t)i * parts : qq + (size_t)(i - a.max_rows) * parts); };
+    Stat first{-INFINITY, -1, 0.0};
+    if ((t >> 3) < all && (t & 7) < parts) first = row_at(t >> 3)[t & 7];
     const double kp = (double)a.inv_t * kLog2e, kq = (double)a.draft_inv_t * kLog2e;
     // what a lane needs of its node, asked for early
     const bool in = t < n;
@@ -281,11 +281,11 @@ __device__ __forceinline__ void walk(const VerifyArgs &a, int s, int2 rows, cons
         lx = logit((const T *)a.x + (rows.x + of) * a.x_row + tok);
         if (drafted) ly = logit((const T *)a.y + (rows.x + of) * a.y_row + tok);
     }
-    const int all = GREEDY || !drafted ? n : 2 * n - 1;  // the target's rows, then the draft's
     for (int i = t >> 3; i < all; i += kThreads / 8) {
-        const bool q = i >= n;
-        const Stat r = row_stat<GREEDY>((q ? ws.q : ws.p) + ((size_t)s * a.max_rows + (q ? i - n : i)) * parts, parts, q ? kq : kp);
-        if ((t & 7) == 0) (q ? lds.q[i - n] : lds.p[i]) = r;
+        const bool q = i >= a.max_rows;
+        if (i >= kThreads / 8) first = (t & 7) < parts ? row_at(i)[t & 7] : Stat{-INFINITY, -1, 0.0};
+        const Stat r = row_stat<GREEDY>(first, row_at(i), parts, q ? kq : kp);
+        if ((t & 7) == 0) (q ? lds.q[i - a.max_rows] : lds.p[i]) = r;
     }
     __syncthreads();
     if (t < 64) {
@@ -338,7 +338,7 @@ __device__ __forceinline__ void walk(const VerifyArgs &a, int s, int2 rows, cons
             Stat ql{};
             if (drafted && cur < n - 1) ql = lds.q[cur];
             lds.n_gone = __popcll(children);
-            lds.draw = Draw{pl, ql, rows.x + cur, !(pl.s > 0.0) ? DRAW_NONE : (ql.s > 0.0 ? DRAW_REST : DRAW_P)};
+            lds.draw = Draw{pl.m, ql.m, rows.x + cur, !(pl.s > 0.0) ? DRAW_NONE : (ql.s > 0.0 ? DRAW_REST : DRAW_P)};
             if (writes) {
                 a.accepted[s] = __popcll(on) - 1;
                 if (GREEDY) a.next[s] = pl.best;
@@ -384,7 +384,7 @@ struct PickLds {
 };
 
 // Of values in order, N a thread: the first whose cumulative sum, on top of `before`, passes u of `whole` (or, whole < 0, of
-// their own sum), else the last above 0; -1 where there is none.  `before` becomes the sum in front of it, whole theirs.
+// their own sum), else the last that counts; -1 where there is none.  `before` becomes the sum in front of it, whole theirs.
 template <int N>
 __device__ __forceinline__ int pick_of(const double (&v)[N], double u, double &before, double &whole, PickLds &lds) {
     const int t = threadIdx.x;
@@ -402,7 +402,7 @@ __device__ __forceinline__ int pick_of(const double (&v)[N], double u, double &b
     double front = 0.0;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        if (v[i] > 0.0) {
+        if (v[i] > kNone) {
             last = t * N + i;
             if (found < 0) front = run;
             if (run + v[i] > aim && found < 0) found = t * N + i;
@@ -436,7 +436,7 @@ struct Weights {
     double kp, kq, ps = 1.0, qs = 1.0;  // ps, qs: 1 / sum
     bool rest = false;                  // (p - q)+
     __device__ __forceinline__ Weights(const VerifyArgs &a, const Draw &d)
-        : x((const T *)a.x + d.row * a.x_row), y((const T *)a.y + d.row * a.y_row), pm(d.p.m), qm(d.q.m), kp((double)a.inv_t * kLog2e),
+        : x((const T *)a.x + d.row * a.x_row), y((const T *)a.y + d.row * a.y_row), pm(d.pm), qm(d.qm), kp((double)a.inv_t * kLog2e),
           kq((double)a.draft_inv_t * kLog2e) {}
     // of N tokens from e on
     template <int N>
@@ -493,14 +493,14 @@ __device__ __forceinline__ double piece_mass(const Weights<T> &w, int vocab, int
     return wave_sum64(sum);
 }
 
-// The token drawn with u; mass: the pieces'.  -1 where they are all 0.
-template <class T, int EPT, class D>
-__device__ __forceinline__ int pick(const Weights<T> &w, const double *mass, int vocab, int pieces, double u, PickLds &lds, const D &drop) {
+// The token drawn with u; mass(c): the pieces'.  -1 where none counts.
+template <class T, int EPT, class M, class D>
+__device__ __forceinline__ int pick(const Weights<T> &w, const M &mass, int vocab, int pieces, double u, PickLds &lds, const D &drop) {
     constexpr int N = EPT * 64 / kThreads, NP = kMaxPieces / kThreads;
     const int t = threadIdx.x;
     double m[NP];
 #pragma unroll
-    for (int i = 0; i < NP; ++i) m[i] = t * NP + i < pieces ? get_mass(mass + t * NP + i) : 0.0;
+    for (int i = 0; i < NP; ++i) m[i] = t * NP + i < pieces ? mass(t * NP + i) : 0.0;
     double before = 0.0, whole = -1.0;
     const int c = pick_of<NP>(m, u, before, whole, lds);
     if (c < 0) return -1;
@@ -528,6 +528,26 @@ __device__ __forceinline__ bool last_of(int *done, int all, int *lds) {
     return *lds != 0;
 }
 
+// A stream without rows.
+__device__ __forceinline__ bool no_rows(const VerifyArgs &a, int s, int2 rows, bool writes) {
+    if (rows.y > 0) return false;
+    if (threadIdx.x == 0 && writes) {
+        a.accepted[s] = 0;
+        a.next[s] = -1;
+    }
+    return true;
+}
+
+// The other distribution of a row, as one to be weighed by itself.
+template <class T>
+__device__ __forceinline__ Weights<T> draft_of(const Weights<T> &w) {
+    Weights<T> q = w;
+    q.x = w.y;
+    q.pm = w.qm;
+    q.kp = w.kq;
+    return q;
+}
+
 // A workgroup for each part of a stream.  With a draft, what has to come from (p - q)+ is left to the next launch.
 template <class T, int EPT, bool DRAFT>
 __global__ __launch_bounds__(kThreads) void walk_kernel(VerifyArgs a, int pieces, int parts) {
@@ -536,40 +556,35 @@ __global__ __launch_bounds__(kThreads) void walk_kernel(VerifyArgs a, int pieces
     __shared__ int last;
     const int s = blockIdx.x / parts, part = blockIdx.x - s * parts, t = threadIdx.x;
     const int2 rows = nodes_of(a, s);
-    if (rows.y == 0) {
-        if (t == 0 && part == 0) {
-            a.accepted[s] = 0;
-            a.next[s] = -1;
-        }
+    const VerifyWs ws = verify_ws(a.streams, a.max_rows, parts, DRAFT, a.ws);
+    if (no_rows(a, s, rows, part == 0)) {
+        if (DRAFT && t == 0 && part == 0) ws.draw[s].mode = DRAW_NONE;
         return;
     }
-    const VerifyWs ws = verify_ws(a.streams, a.max_rows, parts, DRAFT, a.ws);
-    walk<T, false>(a, s, rows, ws, parts, part == 0, wl);
+    const double u = uniform(a.uniforms[rows.x]);
+    walk<T, false>(a, s, rows, ws.p + (size_t)s * a.max_rows * parts, ws.q + (size_t)s * a.max_rows * parts, parts, part == 0, wl);
     const Draw d = wl.draw;
+    if (DRAFT && t == 0 && part == 0) ws.draw[s] = d;
     if (d.mode == DRAW_NONE) {
         if (t == 0 && part == 0) a.next[s] = -1;
         return;
     }
     const int c = part * kWaves + (t >> 6);
-    Weights<T> w(a, d);
+    const Weights<T> w(a, d);
     double *mass = ws.mass + (size_t)s * parts * kWaves;
     const Drop drop{wl.gone, DRAFT ? 0 : wl.n_gone};
     if (c < pieces) {
         const double v = piece_mass<T, EPT>(w, a.vocab, c, drop);
         if ((t & 63) == 0) put_mass(mass + c, v);
         if (DRAFT && d.mode == DRAW_REST) {
-            Weights<T> q = w;
-            q.x = w.y;
-            q.pm = w.qm;
-            q.kp = w.kq;
-            const double vq = piece_mass<T, EPT>(q, a.vocab, c, KeepAll());
+            const double vq = piece_mass<T, EPT>(draft_of(w), a.vocab, c, KeepAll());
             if ((t & 63) == 0) put_mass(ws.mass_q + (size_t)s * parts * kWaves + c, vq);
         }
     }
     if (DRAFT && d.mode == DRAW_REST) return;
     if (!last_of(&ws.done[s].x, parts, &last)) return;
-    const double u = uniform(a.uniforms[rows.x]);
-    int got = pick<T, EPT>(w, mass, a.vocab, pieces, u, lds, drop);
+    auto masses = [&](int i) { return get_mass(mass + i); };
+    int got = pick<T, EPT>(w, masses, a.vocab, pieces, u, lds, drop);
     if (!DRAFT && got < 0) {  // nothing is left: p itself
         __syncthreads();
         for (int i = t >> 6; i < pieces; i += kWaves) {
@@ -578,24 +593,18 @@ __global__ __launch_bounds__(kThreads) void walk_kernel(VerifyArgs a, int pieces
         }
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
-        got = pick<T, EPT>(w, mass, a.vocab, pieces, u, lds, KeepAll());
+        got = pick<T, EPT>(w, masses, a.vocab, pieces, u, lds, KeepAll());
     }
     if (t == 0) a.next[s] = got;
 }
 
-template <class T, int EPT>
 __global__ __launch_bounds__(kThreads) void greedy_kernel(VerifyArgs a, int parts) {
     __shared__ WalkLds wl;
     const int s = blockIdx.x;
     const int2 rows = nodes_of(a, s);
-    if (rows.y == 0) {
-        if (threadIdx.x == 0) {
-            a.accepted[s] = 0;
-            a.next[s] = -1;
-        }
-        return;
-    }
-    walk<T, true>(a, s, rows, verify_ws(a.streams, a.max_rows, parts, false, a.ws), parts, true, wl);
+    if (no_rows(a, s, rows, true)) return;
+    const Stat *p = verify_ws(a.streams, a.max_rows, parts, false, a.ws).p + (size_t)s * a.max_rows * parts;
+    walk<float, true>(a, s, rows, p, p, parts, true, wl);  // (no logit is read)
 }
 
 // The draw behind a rejected token: a workgroup for each part of a stream has its masses of (p - q)+, the last one draws.
@@ -604,44 +613,102 @@ __global__ __launch_bounds__(kThreads) void rest_kernel(VerifyArgs a, int pieces
     __shared__ PickLds lds;
     __shared__ int last;
     const int s = blockIdx.x / parts, part = blockIdx.x - s * parts, t = threadIdx.x;
-    const int2 rows = nodes_of(a, s);
-    if (rows.y == 0) return;
     const VerifyWs ws = verify_ws(a.streams, a.max_rows, parts, true, a.ws);
-    const int node = a.accepted[s];  // (a chain's)
-    if (node >= rows.y - 1) return;
-    Draw d{};
-    d.row = rows.x + node;
-    // what the walk saw, once more
-    const size_t at = ((size_t)s * a.max_rows + node) * parts;
-    d.p = row_stat<false>(ws.p + at, parts, (double)a.inv_t * kLog2e);
-    d.q = row_stat<false>(ws.q + at, parts, (double)a.draft_inv_t * kLog2e);
-    if (!(d.p.s > 0.0) || !(d.q.s > 0.0)) return;
+    const double *mass = ws.mass + (size_t)s * parts * kWaves, *mass_q = ws.mass_q + (size_t)s * parts * kWaves;
+    const Draw d = ws.draw[s];
+    const int root = a.row_start[s];
+    if (d.mode != DRAW_REST) return;
+    const double u = uniform(a.uniforms[root]);
     Weights<T> w(a, d);
-    const double *mass = ws.mass + (size_t)s * parts * kWaves;
-    double *rest = ws.rest + (size_t)s * parts * kWaves;
     w.ps = 1.0 / sum_of(mass, pieces);
-    w.qs = 1.0 / sum_of(ws.mass_q + (size_t)s * parts * kWaves, pieces);
+    w.qs = 1.0 / sum_of(mass_q, pieces);
     w.rest = true;
+    double *rest = ws.rest + (size_t)s * parts * kWaves;
     const int c = part * kWaves + (t >> 6);
     if (c < pieces) {
         const double v = piece_mass<T, EPT>(w, a.vocab, c, KeepAll());
         if ((t & 63) == 0) put_mass(rest + c, v);
     }
     if (!last_of(&ws.done[s].y, parts, &last)) return;
-    const double u = uniform(a.uniforms[rows.x]);
-    int got = pick<T, EPT>(w, rest, a.vocab, pieces, u, lds, KeepAll());
+    int got = pick<T, EPT>(w, [&](int i) { return get_mass(rest + i); }, a.vocab, pieces, u, lds, KeepAll());
     if (got < 0) {  // nothing is left over: p itself
         __syncthreads();
         w.rest = false;
-        got = pick<T, EPT>(w, mass, a.vocab, pieces, u, lds, KeepAll());
+        got = pick<T, EPT>(w, [&](int i) { return mass[i]; }, a.vocab, pieces, u, lds, KeepAll());
     }
     if (t == 0) a.next[s] = got;
 }
 
+// All of it in one launch, a workgroup a stream, where its rows have no more than kSmallPieces pieces: the smallest calls are
+// launches and chains of loads.
+constexpr int kSmallPieces = 32, kSmallEpt = 16;
+template <class T, bool GREEDY>
+__global__ __launch_bounds__(kThreads) void small_kernel(VerifyArgs a, int pieces) {
+    constexpr int EPT = kSmallEpt;
+    __shared__ Stat p[kSmallPieces], q[kSmallPieces];
+    __shared__ double mass[kSmallPieces], mass_q[kSmallPieces];
+    __shared__ WalkLds wl;
+    __shared__ PickLds lds;
+    const int s = blockIdx.x, t = threadIdx.x, w = t >> 6;
+    const int2 rows = nodes_of(a, s);
+    if (no_rows(a, s, rows, true)) return;
+    const bool drafted = a.y != nullptr;
+    const int units = rows.y * pieces;
+    for (int i = w; i < units; i += kWaves) {
+        const int node = i / pieces, c = i - node * pieces;
+        const Stat m = piece_stat<T, EPT, GREEDY>((const T *)a.x + (rows.x + node) * a.x_row, c, a.vocab, a.inv_t);
+        if ((t & 63) == 0) p[i] = m;
+        if (drafted && node < rows.y - 1) {
+            const Stat n = piece_stat<T, EPT, GREEDY>((const T *)a.y + (rows.x + node) * a.y_row, c, a.vocab, a.draft_inv_t);
+            if ((t & 63) == 0) q[i] = n;
+        }
+    }
+    __syncthreads();
+    walk<T, GREEDY>(a, s, rows, p, q, pieces, true, wl);
+    if constexpr (!GREEDY) {
+        const Draw d = wl.draw;
+        int got = -1;
+        if (d.mode != DRAW_NONE) {
+            const double u = uniform(a.uniforms[rows.x]);
+            Weights<T> wt(a, d);
+            auto weigh = [&](const Weights<T> &x, double *to, const auto &drop) {
+                for (int c = w; c < pieces; c += kWaves) {
+                    const double v = piece_mass<T, EPT>(x, a.vocab, c, drop);
+                    if ((t & 63) == 0) to[c] = v;
+                }
+            };
+            const Drop drop{wl.gone, drafted ? 0 : wl.n_gone};
+            weigh(wt, mass, drop);
+            if (d.mode == DRAW_REST) {
+                weigh(draft_of(wt), mass_q, KeepAll());
+                __syncthreads();
+                wt.ps = 1.0 / sum_of(mass, pieces);
+                wt.qs = 1.0 / sum_of(mass_q, pieces);
+                wt.rest = true;
+                __syncthreads();
+                weigh(wt, mass, KeepAll());
+            }
+            __syncthreads();
+            got = pick<T, EPT>(wt, [&](int i) { return mass[i]; }, a.vocab, pieces, u, lds, drop);
+            if (got < 0) {  // nothing is left: p itself
+                wt.rest = false;
+                __syncthreads();
+                weigh(wt, mass, KeepAll());
+                __syncthreads();
+                got = pick<T, EPT>(wt, [&](int i) { return mass[i]; }, a.vocab, pieces, u, lds, KeepAll());
+            }
+        }
+        if (t == 0) a.next[s] = got;
+    }
+}
+
+// Whether a stream's rows are few and short enough for one workgroup.
+bool small(int max_rows, int vocab) { return max_rows * ((vocab + kSmallEpt * 64 - 1) / (kSmallEpt * 64)) <= kSmallPieces; }
+
 // Values of a lane of a piece: few while that fills the chip, many where the parts' sums would be much work themselves.
 int ept_of(int rows, int vocab) {
-    const int small = (vocab + 1023) / 1024;  // parts of 4 values a lane
-    if (small <= 16 && (long long)rows * small <= 1024) return 4;
+    const int few = (vocab + 1023) / 1024;  // parts of 4 values a lane
+    if (few <= 16 && (long long)rows * few <= 1024) return 4;
     return vocab <= 64 * 1024 ? 16 : 32;
 }
 int parts_of(int rows, int vocab) {
@@ -654,10 +721,9 @@ template <class T, int EPT>
 hipError_t verify_e(const VerifyArgs &a, hipStream_t s) {
     const int parts = parts_of(a.streams * a.max_rows, a.vocab), pieces = (a.vocab + EPT * 64 - 1) / (EPT * 64);
     const dim3 rows((unsigned)a.streams * a.max_rows * parts, a.y != nullptr ? 2 : 1), of_streams((unsigned)a.streams * parts);
-    (void)hipGetLastError();
     if (a.greedy) {
         hipLaunchKernelGGL((stat_kernel<T, EPT, true>), rows, dim3(kThreads), 0, s, a, parts);
-        hipLaunchKernelGGL((greedy_kernel<T, EPT>), dim3(a.streams), dim3(kThreads), 0, s, a, parts);
+        hipLaunchKernelGGL(greedy_kernel, dim3(a.streams), dim3(kThreads), 0, s, a, parts);
         return hipGetLastError();
     }
     hipLaunchKernelGGL((stat_kernel<T, EPT, false>), rows, dim3(kThreads), 0, s, a, parts);
@@ -672,6 +738,15 @@ hipError_t verify_e(const VerifyArgs &a, hipStream_t s) {
 
 template <class T>
 hipError_t verify_t(const VerifyArgs &a, hipStream_t s) {
+    (void)hipGetLastError();
+    if (small(a.max_rows, a.vocab)) {
+        const int pieces = (a.vocab + kSmallEpt * 64 - 1) / (kSmallEpt * 64);
+        if (a.greedy)
+            hipLaunchKernelGGL((small_kernel<T, true>), dim3(a.streams), dim3(kThreads), 0, s, a, pieces);
+        else
+            hipLaunchKernelGGL((small_kernel<T, false>), dim3(a.streams), dim3(kThreads), 0, s, a, pieces);
+        return hipGetLastError();
+    }
     switch (ept_of(a.streams * a.max_rows, a.vocab)) {
         case 4: return verify_e<T, 4>(a, s);
         case 16: return verify_e<T, 16>(a, s);
@@ -682,8 +757,9 @@ hipError_t verify_t(const VerifyArgs &a, hipStream_t s) {
 }  // namespace
 
 size_t verify_workspace(int streams, int max_rows, int vocab, bool draft) {
+    if (small(max_rows, vocab)) return 0;
     const VerifyWs w = verify_ws(streams, max_rows, parts_of(streams * max_rows, vocab), draft, nullptr);
-    return (size_t)(uintptr_t)(w.done + streams);
+    return (size_t)(uintptr_t)(w.draw + (draft ? streams : 0));
 }
 
 hipError_t launch_verify(const VerifyArgs &a, hipStream_t s) { return a.dtype == ELEM_F16 ? verify_t<__half>(a, s) : verify_t<float>(a, s); }

@@ -43,7 +43,7 @@ def _each(fn, ok, bad):
 def test_verify_refusals():
     L = lib.load()
     #     0  1    2        3     4  5  6    7  8  9     10 11 12 13   14   15 16 17 18 19 20       21
-    ok = [P, 100, lib.F32, None, 0, 8, 100, P, P, None, 2, 4, P, 1.0, 1.0, 0, P, P, P, P, 1 << 20, None]
+    ok = [P, 99999, lib.F32, None, 0, 8, 99999, P, P, None, 2, 4, P, 1.0, 1.0, 0, P, P, P, P, 1 << 20, None]
     _each(L.moss_hip_verify_tokens, ok, [
         (0, None, "null"), (7, None, "null"), (8, None, "null"), (16, None, "null"), (17, None, "null"), (18, None, "null"),
         (12, None, "uniforms"), (2, lib.I8, "dtype"), (1, -1, "negative"), (4, -1, "negative"), (1, (1 << 40) + 1, "2^40"), (5, -1, "rows"),
@@ -63,6 +63,7 @@ def test_verify_refusals():
         assert L.moss_hip_verify_tokens_workspace(3, 5, 130001, draft, C.byref(n)) == lib.OK
         sizes.append(n.value)
     assert 0 < sizes[0] < sizes[1]
+    assert L.moss_hip_verify_tokens_workspace(3, 5, 1024, 1, C.byref(n)) == lib.OK and n.value == 0  # (one launch holds all of it)
     nothing = list(ok)  # no streams: nothing to do
     nothing[10], nothing[19] = 0, None
     assert L.moss_hip_verify_tokens(*nothing) == lib.OK
