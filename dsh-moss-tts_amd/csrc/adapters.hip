@@ -6,12 +6,15 @@
 // Both products are matrix instructions with the weights as the one operand and a tile of 16 neighbouring rows as the
 // other, one of the adapters among them at a time, so a lane keeps one row throughout: what scales a row is one
 // number of the lane.  With one row of an adapter, 15 of 16 columns of a product idle; the instructions are still
-// fewer than the vector unit would need.  Few rows take one launch, a workgroup a tile, an adapter and a share of the
-// outputs, with t = A x kept on the chip; many rows take two, with t in the workspace.
+// fewer than the vector unit would need.  One launch: a workgroup takes a tile, one of the adapters among its rows and a
+// share of the outputs, and keeps t = A x on the chip.  (Two launches with t in memory were as fast at 8191 rows of 4096, 84 and
+// 86 us, 19 and 16 at 2896 of 768 -> 2304, and slower below: 84 and 39 at 1086 rows of 64 adapters.)
 //
 // Weights are fp16, laid out once in the order in which a wave's lanes hold them, so that a load is 1 KiB in one piece.
 // Rows go through LDS for the same reason: as an operand, lanes next to each other hold different rows, and 64 separate
-// accesses a load made the L1 the limit (20 of 33 us of the first product of 8191 rows of 4096).
+// accesses a load made the L1 the limit: 8191 fp16 rows of 4096 -> 4096, rank 64, took 129 us, now 86 (2.4 TB/s; a copy of
+// those sizes reaches 3.2).  What is left is that a workgroup's registers fill a compute unit, so that its two products
+// do not overlap with another's.  2896 fp32 rows of 768 -> 2304, rank 16: 16.3 us, 3.9 TB/s.  One row: 5.7 us, a chain of loads.
 //
 // fp16 rows are multiplied as they are.  32-bit rows, and t, go in as two fp16 numbers, hi + lo, 22 bits: of 128 columns of a
 // row (of all ranks of t) the largest is put at 2^14 by a power of two, which leaves 2^-39 of the largest as the
@@ -415,8 +418,11 @@ template <class X, class Y, int RK>
 hipError_t launch(const AdapterArgs &a, hipStream_t s) {
     (void)hipGetLastError();
     const int tiles = (a.rows + 15) / 16, groups = (a.out + 63) / 64;
+    // Workgroups for the adapters of a tile, and for shares of the outputs (each share forms t again), until there are 512. Most
+    // of them find no adapter left and end; 2048 of them took 23 us in place of 16 at 2896 rows, 256 56 in place of 39 at
+    // 1086 rows of 64 adapters.
     const int of_tile = std::min({16, a.rows, a.n + 1});
-    const int each = std::min(of_tile, std::max(2, 512 / tiles));  // workgroups for the adapters of a tile
+    const int each = std::min(of_tile, std::max(2, 512 / tiles));
     const int slices = std::min(std::max(1, 512 / (tiles * each)), std::max(1, groups / kSlices));
     const int outs = (groups + slices - 1) / slices * 64;
     hipLaunchKernelGGL((adapter_kernel<X, Y, RK>), dim3(tiles, each, (a.out + outs - 1) / outs), dim3(kThreads), 0, s, a, outs);

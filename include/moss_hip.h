@@ -344,14 +344,16 @@ int moss_hip_attn_decode_noalloc(const float *q, const void *k_cache, const void
 /* ---- Operators of a caller's own decoding loop -----------------------------------------
  * Rotary positions, a paged K/V cache that may hold 8-bit values, attention of one or more drafted
  * rows per stream over it, and the log probabilities that accept or reject what was drafted.  One
- * step of such a loop: rotate the queries (moss_hip_rope_rows), write the rows' keys and values
+ * step of such a loop: find room in the cache (moss_hip_kv_reserve), add each request's adapter to the shared
+ * projection (moss_hip_adapter_rows), rotate the queries (moss_hip_rope_rows), write the rows' keys and values
  * (moss_hip_kv_write, which rotates the keys on the way), attend (moss_hip_attn_tree), score the
- * drafted tokens under the logits (moss_hip_token_logprobs); then write the accepted rows once
- * more at their final positions.  The reference has none of these as calls of their own: its
+ * drafted tokens under the logits (moss_hip_token_logprobs) or accept and reject them (moss_hip_verify_tokens); then move the
+ * accepted rows to their final positions (moss_hip_kv_compact, or moss_hip_kv_write once more), and share, reorder or end
+ * streams (moss_hip_kv_fork).  The reference has none of these as calls of their own: its
  * rotation and cache write are part of its QKV step (csrc/src/llm.cpp:173-228), its cache is fp32
  * and its decode takes one row at a time.
  *
- * The calls allocate nothing, wait for nothing and keep nothing: they launch one or two kernels on
+ * The calls allocate nothing, wait for nothing and keep nothing: they launch one to three kernels on
  * `stream` and may be captured.  Every pointer inside the structs but the structs' own is a device
  * pointer of the device that is current at the call, and `stream` is a stream of that device.
  * Arrays read while a call's kernels run must not be changed meanwhile by work on other streams.  A
@@ -483,7 +485,8 @@ int moss_hip_token_logprobs_workspace(int rows, int vocab, int top_k, size_t *by
  *   greedy: accepted where it is the likeliest (of equal logits the lowest index; NaN is none), which also follows.
  * uniforms [rows]: u of each node, numbers of [0, 1) (others count as the nearest of 0 and 1, NaN as 1); row 0's draws the next token: the
  * first whose cumulative sum, in the order of the vocabulary, passes u times the whole.  Where nothing is left over,
- * it is drawn from p.  Probabilities are formed and summed in 64 bits.  greedy takes no uniforms and no draft_logits.
+ * it is drawn from p.  The row that is drawn from is weighed and summed in 64 bits (what is under 2^-980 of its largest counts as nothing); the sums
+ * that acceptance goes by are within 2^-18 of themselves.  The streams' row ranges lie apart.  greedy takes no uniforms and no draft_logits.
  *   accepted [streams]: drafted nodes accepted.
  *   path [rows]: entry row_start[s] + j is the node that the walk took as its j-th (0 first), -1 past the last: what
  *     moss_hip_kv_compact takes.  Rows of no stream, and a stream's rows past max_rows, stay as they were.

@@ -13,16 +13,20 @@ def softmax(x, inv_t):
     return e / e.sum()
 
 
+#: How near a number may come to a border: the sums that acceptance goes by are within 2^-18, a draw's are of 64 bits.
+ACCEPT, DRAW = 2.0 ** -18, 1e-10
+
+
 def _number(u):
     return 1.0 if math.isnan(u) else min(max(u, 0.0), 1.0)
 
 
 def _drawn(w, u):
     """The first index whose cumulative sum passes u of the whole, else the last with any weight; and how near the
-    pick was to a border, as a share of the whole."""
+    pick was to a border, in units of DRAW of the whole."""
     cdf = np.cumsum(w)
     aim = _number(u) * cdf[-1]
-    near = np.min(np.abs(cdf - aim)) / cdf[-1] if 0.0 < _number(u) < 1.0 else 1.0
+    near = np.min(np.abs(cdf - aim)) / cdf[-1] / DRAW if 0.0 < _number(u) < 1.0 else np.inf
     hit = np.nonzero((cdf > aim) & (w > 0))[0]
     return (int(hit[0]) if len(hit) else int(np.nonzero(w > 0)[0][-1])), near
 
@@ -37,12 +41,12 @@ def _parent(i, mask):
 
 
 def verify_stream(x, tok, u, y=None, mask=None, inv_t=1.0, draft_inv_t=1.0, greedy=False):
-    """(path, next token, margin) of one stream's rows."""
+    """(path, next token, margin) of one stream's rows.  A margin over 1 is safe."""
     n, vocab = x.shape
     if n == 0:
-        return [], -1, 1.0
+        return [], -1, np.inf
     parents = [_parent(i, mask) for i in range(n)]
-    path, near = [0], 1.0
+    path, near = [0], np.inf
     while True:
         cur = path[-1]
         row = np.asarray(x[cur], np.float64)
@@ -73,7 +77,7 @@ def verify_stream(x, tok, u, y=None, mask=None, inv_t=1.0, draft_inv_t=1.0, gree
                     continue
                 a, b = _number(u[i]) * max(left, 0.0), p[t]
             if a != 0.0 and b != 0.0 and a != b:
-                near = min(near, abs(a - b) / max(a, b))
+                near = min(near, abs(a - b) / max(a, b) / ACCEPT)
             if a < b:
                 taken = i
                 break
@@ -97,7 +101,7 @@ def verify_stream(x, tok, u, y=None, mask=None, inv_t=1.0, draft_inv_t=1.0, gree
 def verify(x, tok, start, u, max_rows, y=None, mask=None, inv_t=1.0, draft_inv_t=1.0, greedy=False, path=None):
     """(accepted, path, next tokens, margin); `path` is what it holds before."""
     streams = len(start) - 1
-    accepted, nxt, near = np.zeros(streams, np.int32), np.full(streams, -1, np.int32), 1.0
+    accepted, nxt, near = np.zeros(streams, np.int32), np.full(streams, -1, np.int32), np.inf
     path = np.array(path, np.int32)
     for s in range(streams):
         a, b = int(start[s]), int(start[s + 1])

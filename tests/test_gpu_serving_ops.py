@@ -1,8 +1,8 @@
 """The operators of a serving loop against plain sequential forms in 64 bits (GPU): verification of drafted tokens, pages that
 streams share, accepted rows moved to their positions, adapters beside a projection, and a run of all of them together.
 
-Decisions and moved bytes have to be equal.  Where a random number is compared with a probability, both sides form it in 64
-bits (errors of some 2^-50); each test makes sure that no number of its own lies within 1e-10 of a border."""
+Decisions and moved bytes have to be equal.  Where a random number is compared with a probability, the call's is off by up to
+2^-18 (acceptance) or some 2^-40 (draws); each test makes sure that no number of its own lies that near to a border."""
 import numpy as np
 import pytest
 
@@ -64,13 +64,13 @@ def _held(torch, z, dtype):
 
 
 def _check_verify(torch, x, tok, start, max_rows, u=None, y=None, mask=None, dtype=None, pad=0, inv_temperature=1.0,
-                  draft_inv_temperature=None, greedy=False, margin=1e-10):
+                  draft_inv_temperature=None, greedy=False):
     dtype = dtype or torch.float32
     got = _verify(torch, x, tok, start, max_rows, u, y, mask, dtype, pad, inv_temperature=inv_temperature,
                   draft_inv_temperature=draft_inv_temperature, greedy=greedy)
     *want, near = so.verify(_held(torch, x, dtype), tok, start, u, max_rows, None if y is None else _held(torch, y, dtype), mask, inv_temperature,
                             inv_temperature if draft_inv_temperature is None else draft_inv_temperature, greedy, path=np.full(len(tok), -7))
-    assert near > margin, near
+    assert near > 1, near
     for name, g, w in zip(("accepted", "path", "next"), got, want):
         assert np.array_equal(g, w), (name, g, w)
     return got
@@ -305,7 +305,7 @@ def test_verify_captured_and_streams(torch_gpu):
         g.replay()
         torch.cuda.synchronize()
         *want, near = so.verify(x, tok, start, u, 6, y, path=np.full(14, -7))
-        assert near > 1e-10
+        assert near > 1
         assert all(np.array_equal(o.cpu().numpy(), w) for o, w in zip(out, want))
         eager = _verify(torch, x, tok, start, 6, u, y=y)
         assert all(np.array_equal(e, w) for e, w in zip(eager, want))
@@ -772,7 +772,7 @@ def test_a_serving_loop(torch_gpu, cache):
         lib.kv_write(kv, k, v, i32(stream), i32(ctx[stream] + node), rope=rope, rope_pos=i32(pos))
         lib.verify_tokens(logits, i32(tok), i32(start), acc, path, nxt, tree, uniforms=_cu(torch, u), row_mask=_cu(torch, mask.view(np.int64)))
         *want, near = so.verify(logits.double().cpu().numpy(), tok, start, u, tree, mask=mask, path=np.zeros(start[-1]))
-        assert near > 1e-10 and np.array_equal(acc.cpu().numpy(), want[0]) and np.array_equal(path.cpu().numpy(), want[1])
+        assert near > 1 and np.array_equal(acc.cpu().numpy(), want[0]) and np.array_equal(path.cpu().numpy(), want[1])
         lib.kv_compact(ls, i32(start), i32(ctx), path, tree)
         for s in range(streams):
             said[s] += [(int(tok[start[s] + j]), int(voice[s])) for j in want[1][start[s]:start[s + 1]] if j >= 0]
