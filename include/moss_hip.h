@@ -544,7 +544,8 @@ int moss_hip_kv_compact(const moss_hip_kv_cache *layers, int n_layers, const int
  *   y[r] = base[r] + scale_a B_a (A_a x[r]),  a = adapter[r];  y[r] = base[r] for an adapter outside [0, n_adapters).
  * x [rows][cols] of x_dtype, base and y [rows][out] of y_dtype (F32 or F16), row strides in elements; y may be base itself (same
  * stride), and must not overlap x, or base otherwise.  Weights (fp16) and rows are multiplied exactly, but for 32-bit rows, and A x,
- * held to 22 bits and 2^-39 of the largest (in 128 neighbouring columns); sums are held in 32 bits and y is rounded once. */
+ * held to 22 bits and 2^-39 of the largest (in 128 neighbouring columns); sums are held in 32 bits and y is rounded once.  A row with an Inf or NaN is not finite under any adapter,
+ * one of rank 0 too. */
 typedef struct {
     void *a, *b;          /* the weights, of the sizes that moss_hip_adapter_sizes says, 16-byte aligned: filled by moss_hip_adapter_pack */
     const float *scale;   /* [n_adapters]; NULL: 1 */
