@@ -254,38 +254,49 @@ __device__ __forceinline__ Stat row_stat(const Stat &mine, const Stat *c, int pa
     }
 }
 
+
 __device__ __forceinline__ double uniform(double u) { return u < 1.0 ? (u > 0.0 ? u : 0.0) : 1.0; }  // (NaN: 1)
 
-// The walk of one stream, by one workgroup: the rows' sums by all threads, then a lane a node.  pp, qq: the stream's parts; `writes`:
-// whether this workgroup leaves the outputs.  Loads that do not wait for each other come first: the chain of them is most
-// of its time.
+// What a thread of the walk needs of its node, asked for before everything that does not wait for it.
+struct Node {
+    bool in, known;  // known: a child with a token of the vocabulary
+    int tok, parent;
+    double u;
+    float lx, ly;  // its token's logits behind the parent
+};
 template <class T, bool GREEDY>
-__device__ __forceinline__ void walk(const VerifyArgs &a, int s, int2 rows, const Stat *pp, const Stat *qq, int parts, bool writes, WalkLds &lds) {
+__device__ __forceinline__ Node node_of(const VerifyArgs &a, int2 rows) {
     const int t = threadIdx.x, n = rows.y;
-    const bool drafted = a.y != nullptr;
+    Node d{t < n, false, -1, t - 1, 0.0, -INFINITY, -INFINITY};
+    if (d.in) d.tok = a.tokens[rows.x + t];
+    if (d.in && a.row_mask != nullptr) {
+        const uint64_t mask = a.row_mask[rows.x + t], up = mask & ((1ull << t) - 1);
+        d.parent = (mask >> t & 1) && up ? 63 - __builtin_clzll(up) : -1;
+    }
+    if (!d.in || t == 0) d.parent = -1;
+    d.known = d.tok >= 0 && d.tok < a.vocab && d.parent >= 0;
+    if (!GREEDY && d.known) {
+        d.u = uniform(a.uniforms[rows.x + t]);
+        d.lx = logit((const T *)a.x + (rows.x + d.parent) * a.x_row + d.tok);
+        if (a.y != nullptr) d.ly = logit((const T *)a.y + (rows.x + d.parent) * a.y_row + d.tok);
+    }
+    return d;
+}
+
+// The walk of one stream, by one workgroup: the rows' sums by all threads, then a lane a node.  pp, qq: the stream's parts; `writes`:
+// whether this workgroup leaves the outputs.
+template <bool GREEDY>
+__device__ __forceinline__ void walk(const VerifyArgs &a, int s, int2 rows, const Node &d, const Stat *pp, const Stat *qq, int parts, bool writes, WalkLds &lds) {
+    const int t = threadIdx.x, n = rows.y;
+    const bool drafted = a.y != nullptr, in = d.in, known = d.known;
     const int all = GREEDY || !drafted ? a.max_rows : 2 * a.max_rows;  // the target's rows, then the draft's; what is past n is not used
     auto row_at = [&](int i) { return (i < a.max_rows ? pp + (size_t)i * parts : qq + (size_t)(i - a.max_rows) * parts); };
     Stat first{-INFINITY, -1, 0.0};
     if ((t >> 3) < all && (t & 7) < parts) first = row_at(t >> 3)[t & 7];
     const double kp = (double)a.inv_t * kLog2e, kq = (double)a.draft_inv_t * kLog2e;
-    // what a lane needs of its node, asked for early
-    const bool in = t < n;
-    const int tok = in ? a.tokens[rows.x + t] : -1;
-    int parent = t - 1;
-    if (in && a.row_mask != nullptr) {
-        const uint64_t mask = a.row_mask[rows.x + t], up = mask & ((1ull << t) - 1);
-        parent = (mask >> t & 1) && up ? 63 - __builtin_clzll(up) : -1;
-    }
-    if (!in || t == 0) parent = -1;
-    const int of = max(parent, 0);
-    const bool known = tok >= 0 && tok < a.vocab && parent >= 0;
-    double u = 0.0;
-    float lx = -INFINITY, ly = -INFINITY;
-    if (!GREEDY && known) {
-        u = uniform(a.uniforms[rows.x + t]);
-        lx = logit((const T *)a.x + (rows.x + of) * a.x_row + tok);
-        if (drafted) ly = logit((const T *)a.y + (rows.x + of) * a.y_row + tok);
-    }
+    const int tok = d.tok, parent = d.parent, of = max(parent, 0);
+    const double u = d.u;
+    const float lx = d.lx, ly = d.ly;
     for (int i = t >> 3; i < all; i += kThreads / 8) {
         const bool q = i >= a.max_rows;
         if (i >= kThreads / 8) first = (t & 7) < parts ? row_at(i)[t & 7] : Stat{-INFINITY, -1, 0.0};
@@ -312,7 +323,8 @@ __device__ __forceinline__ void walk(const VerifyArgs &a, int s, int2 rows, cons
                     for (int j = 1; j < n; ++j) {
                         const int pj = __builtin_amdgcn_readlane(parent, j), tj = __builtin_amdgcn_readlane(tok, j);
                         const bool aj = __builtin_amdgcn_readlane((int)again, j);
-                        const double bj = __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(prob), j), __builtin_amdgcn_readlane(__double2loint(prob), j));
+                        const double bj = __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(prob), j),
+                                                           __builtin_amdgcn_readlane(__double2loint(prob), j));
                         if (t > j && parent == pj && pj >= 0) {
                             again |= tok == tj;
                             if (!aj) left -= bj;
@@ -567,7 +579,8 @@ __global__ __launch_bounds__(kThreads) void walk_kernel(VerifyArgs a, int pieces
         return;
     }
     const double u = uniform(a.uniforms[rows.x]);
-    walk<T, false>(a, s, rows, ws.p + (size_t)s * a.max_rows * parts, ws.q + (size_t)s * a.max_rows * parts, parts, part == 0, wl);
+    const Node node = node_of<T, false>(a, rows);
+    walk<false>(a, s, rows, node, ws.p + (size_t)s * a.max_rows * parts, ws.q + (size_t)s * a.max_rows * parts, parts, part == 0, wl);
     const Draw d = wl.draw;
     if (DRAFT && t == 0 && part == 0) ws.draw[s] = d;
     if (d.mode == DRAW_NONE) {
@@ -609,7 +622,7 @@ __global__ __launch_bounds__(kThreads) void greedy_kernel(VerifyArgs a, int part
     const int2 rows = nodes_of(a, s);
     if (no_rows(a, s, rows, true)) return;
     const Stat *p = verify_ws(a.streams, a.max_rows, parts, false, a.ws).p + (size_t)s * a.max_rows * parts;
-    walk<float, true>(a, s, rows, p, p, parts, true, wl);  // (no logit is read)
+    walk<true>(a, s, rows, node_of<float, true>(a, rows), p, p, parts, true, wl);  // (no logit is read)
 }
 
 // The draw behind a rejected token: a workgroup for each part of a stream has its masses of (p - q)+, the last one draws.
@@ -658,6 +671,7 @@ __global__ __launch_bounds__(kThreads) void small_kernel(VerifyArgs a, int piece
     const int2 rows = nodes_of(a, s);
     if (no_rows(a, s, rows, true)) return;
     const bool drafted = a.y != nullptr;
+    const Node mine = node_of<T, GREEDY>(a, rows);
     const int units = rows.y * pieces;
     for (int i = w; i < units; i += kWaves) {
         const int node = i / pieces, c = i - node * pieces;
@@ -669,7 +683,7 @@ __global__ __launch_bounds__(kThreads) void small_kernel(VerifyArgs a, int piece
         }
     }
     __syncthreads();
-    walk<T, GREEDY>(a, s, rows, p, q, pieces, true, wl);
+    walk<GREEDY>(a, s, rows, mine, p, q, pieces, true, wl);
     if constexpr (!GREEDY) {
         const Draw d = wl.draw;
         int got = -1;
