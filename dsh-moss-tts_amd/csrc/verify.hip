@@ -17,7 +17,7 @@
 // that one again.  What is drawn from (p - q)+ needs the exact sums of p and q first, and gets its masses and its
 // draw in a third launch.  Which workgroup finishes last changes nothing but who draws.  Streams of few short rows take one launch.
 //
-// 24 chains of 9 over 130001 fp16 logits and the draft's: 27.7 us for all rows (4 TB/s), 18 for the walk and the two sums, 22 for
+// 24 chains of 9 over 130001 fp16 logits and the draft's: 27.5 us for all rows (4 TB/s), 17 for the walk and the two sums, 19 for
 // (p - q)+ and the draw, both of which are 64-bit exponentials on 3.1 million logits (6 us each at best) and a chain of
 // loads.  64 chains of 6 over 16384: 10 + 13 + 12.  16 trees of 27 over 16384: 7 + 17.  All rows in 64 bits took 50 us in place
 // of 28.
