@@ -676,7 +676,7 @@ mh::PagesArgs pages_args(const moss_hip_kv_pages *p) {
         throw Status(MOSS_HIP_EINVAL, "need table_stride > 0, streams * table_stride at most 2^26");
     if (p->page_size <= 0 || p->page_size % 16 || p->page_size > mh::kTreePageMax)
         throw Status(MOSS_HIP_EINVAL, "page_size must be a multiple of 16 and at most 32768");
-    if (p->n_pages <= 0) throw Status(MOSS_HIP_EINVAL, "need n_pages > 0");
+    if (p->n_pages <= 0 || p->n_pages > (1 << 30)) throw Status(MOSS_HIP_EINVAL, "need 0 < n_pages <= 2^30");
     mh::PagesArgs a;
     a.table = p->page_table;
     a.table_stride = p->table_stride;

@@ -509,7 +509,7 @@ typedef struct {
     int32_t *page_table; /* [streams][table_stride] */
     int table_stride, streams;
     int32_t *refs; /* [n_pages] */
-    int n_pages;
+    int n_pages;   /* at most 2^30 */
     int page_size; /* a multiple of 16, at most 32768 */
 } moss_hip_kv_pages;
 

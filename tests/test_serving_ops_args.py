@@ -71,7 +71,7 @@ def test_verify_refusals():
 
 BAD_PAGES = [(dict(streams=-1), "streams"), (dict(streams=65537), "streams"), (dict(table_stride=0), "table_stride"),
              (dict(streams=65536, table_stride=2048), "2^26"), (dict(page_size=0), "page_size"), (dict(page_size=40), "page_size"),
-             (dict(page_size=65536), "page_size"), (dict(n_pages=0), "n_pages")]
+             (dict(page_size=65536), "page_size"), (dict(n_pages=0), "n_pages"), (dict(n_pages=(1 << 30) + 1), "n_pages")]
 
 
 @pytest.mark.parametrize("kw,word", BAD_PAGES + [(dict(page_table=None), "null"), (dict(refs=None), "null")])
