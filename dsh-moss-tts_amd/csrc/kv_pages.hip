@@ -115,8 +115,8 @@ __device__ __forceinline__ int fate_of(const ReserveArgs &a, int s, int j) {
     return held - earlier > 1 ? SHARED : last;
 }
 
-// Pages that one stream's rows can touch.
-__host__ __device__ __forceinline__ int pages_of(int max_rows, int page_size) { return (max_rows + page_size - 2) / page_size + 1; }
+// Pages that one stream's rows can touch: those that max_rows positions can lie on, and no more than a stream has.
+int pages_of(const PagesArgs &p, int max_rows) { return (int)std::min<long long>(((long long)max_rows + p.page_size - 2) / p.page_size + 1, p.table_stride); }
 
 __global__ __launch_bounds__(kThreads) void fate_kernel(ReserveArgs a, int n, int per) {
     const int e = __builtin_amdgcn_readfirstlane(blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6));
@@ -404,12 +404,12 @@ hipError_t launch_kv_fork(const ForkArgs &a, hipStream_t s) {
 // The workspace: copies [streams] (from page, to page, slots); the lowest free pages, and what becomes of each entry
 // [streams][pages of a stream].
 size_t reserve_workspace(const PagesArgs &p, int max_rows) {
-    const size_t n = (size_t)p.streams * pages_of(max_rows, p.page_size);
+    const size_t n = (size_t)p.streams * pages_of(p, max_rows);
     return p.streams * sizeof(int4) + (n <= kBookThreads ? 0 : 2 * sizeof(int) * n);
 }
 
 hipError_t launch_kv_reserve(ReserveArgs a, const KvLayers &l, hipStream_t s) {
-    const int per = pages_of(a.max_rows, a.p.page_size), n = a.p.streams * per;  // (within 2^27)
+    const int per = pages_of(a.p, a.max_rows), n = a.p.streams * per;  // (within 2^26, as the table)
     a.copies = (int4 *)a.ws;
     a.free_pages = (int *)(a.copies + a.p.streams);
     a.fate = a.free_pages + n;
