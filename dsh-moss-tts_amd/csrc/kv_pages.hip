@@ -119,12 +119,12 @@ __device__ __forceinline__ int fate_of(const ReserveArgs &a, int s, int j) {
 int pages_of(const PagesArgs &p, int max_rows) { return (int)std::min<long long>(((long long)max_rows + p.page_size - 2) / p.page_size + 1, p.table_stride); }
 
 __global__ __launch_bounds__(kThreads) void fate_kernel(ReserveArgs a, int n, int per) {
-    const int e = __builtin_amdgcn_readfirstlane(blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6));
-    if (e >= n) return;
-    const int s = e / per, r = e - s * per;
-    const Range g = range_of(a, s);
-    const int f = g.j0 + r <= g.j1 ? fate_of(a, s, g.j0 + r) : STAYS;
-    if ((threadIdx.x & 63) == 0) a.fate[e] = f;
+    for (int e = __builtin_amdgcn_readfirstlane(blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6)); e < n; e += gridDim.x * (kThreads / 64)) {
+        const int s = e / per, r = e - s * per;
+        const Range g = range_of(a, s);
+        const int f = g.j0 + r <= g.j1 ? fate_of(a, s, g.j0 + r) : STAYS;
+        if ((threadIdx.x & 63) == 0) a.fate[e] = f;
+    }
 }
 
 // Sum over the workgroup's earlier threads, and over all of them.
@@ -396,6 +396,7 @@ hipError_t launch_kv_fork(const ForkArgs &a, hipStream_t s) {
     } else {
         const unsigned blocks = (unsigned)((n + kThreads - 1) / kThreads);
         hipLaunchKernelGGL(fork_read_kernel, dim3(blocks), dim3(kThreads), 0, s, a, n);
+        if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;  // (what follows trusts what it leaves)
         hipLaunchKernelGGL(fork_write_kernel, dim3(blocks), dim3(kThreads), 0, s, a, n);
     }
     return hipGetLastError();
@@ -417,9 +418,12 @@ hipError_t launch_kv_reserve(ReserveArgs a, const KvLayers &l, hipStream_t s) {
     if (n <= kBookThreads) {
         hipLaunchKernelGGL(reserve_small_kernel, dim3(1), dim3(kBookThreads), 0, s, a, per);
     } else {
-        hipLaunchKernelGGL(fate_kernel, dim3((n + 3) / 4), dim3(kThreads), 0, s, a, n, per);
+        // A wave an entry, of up to 2^26: those of 65536 workgroups take them in turn, as a grid holds fewer than 2^32 threads.
+        hipLaunchKernelGGL(fate_kernel, dim3(std::min((n + 3) / 4, 1 << 16)), dim3(kThreads), 0, s, a, n, per);
+        if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;  // (what follows trusts what it leaves)
         hipLaunchKernelGGL(reserve_kernel, dim3(1), dim3(kBookThreads), 0, s, a, per);
     }
+    if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
     const dim3 grid(a.p.streams * 2 * a.layers, a.heads);
     if (a.scales)
         hipLaunchKernelGGL(copy_kernel<true>, grid, dim3(kThreads), 0, s, a, l);

@@ -742,12 +742,15 @@ hipError_t verify_e(const VerifyArgs &a, hipStream_t s) {
     const dim3 rows((unsigned)a.streams * a.max_rows * parts, a.y != nullptr ? 2 : 1), of_streams((unsigned)a.streams * parts);
     if (a.greedy) {
         hipLaunchKernelGGL((stat_kernel<T, EPT, true>), rows, dim3(kThreads), 0, s, a, parts);
+        if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;  // (what follows trusts what it leaves)
         hipLaunchKernelGGL(greedy_kernel, dim3(a.streams), dim3(kThreads), 0, s, a, parts);
         return hipGetLastError();
     }
     hipLaunchKernelGGL((stat_kernel<T, EPT, false>), rows, dim3(kThreads), 0, s, a, parts);
+    if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
     if (a.y != nullptr) {
         hipLaunchKernelGGL((walk_kernel<T, EPT, true>), of_streams, dim3(kThreads), 0, s, a, pieces, parts);
+        if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
         hipLaunchKernelGGL((rest_kernel<T, EPT>), of_streams, dim3(kThreads), 0, s, a, pieces, parts);
     } else {
         hipLaunchKernelGGL((walk_kernel<T, EPT, false>), of_streams, dim3(kThreads), 0, s, a, pieces, parts);

@@ -1,0 +1,36 @@
+"""The serving-loop operators at the ends of the sizes that they take, and what their row ranges may hold (GPU)."""
+import numpy as np
+import pytest
+
+from mosship import lib
+from test_gpu_serving_ops import _cu, _layers, _pools
+
+pytestmark = pytest.mark.gpu
+
+
+def test_reserve_the_largest_table(torch_gpu):
+    """65536 streams of 1024 pages, any of which a call may touch: 2^26 entries, whose books take 2^26 waves.  Streams with
+    rows take the lowest free pages in their order; a shared page of the last one is copied."""
+    torch = torch_gpu
+    streams, stride, page, n_pages = 65536, 1024, 16, 64
+    print("largest table", flush=True)
+    pools = _pools(torch, np.random.default_rng(0), "i8", 1, n_pages, 1, page, 64)
+    table = torch.full((streams, stride), -1, dtype=torch.int32, device="cuda")
+    refs = np.zeros(n_pages, np.int32)
+    refs[[0, 2]] = 2, 1  # page 0 is that of the last two streams
+    table[-2:, 0] = 0
+    dr, ok = _cu(torch, refs), torch.full((streams,), -7, dtype=torch.int32, device="cuda")
+    n, ctx = np.zeros(streams, np.int64), np.zeros(streams, np.int32)
+    n[[0, 1, 30000, 65535]] = 20, 33, 16, 5
+    ctx[[30000, 65534, 65535]] = 1023 * 16, 7, 7
+    start = np.concatenate([[0], np.cumsum(n)]).astype(np.int32)
+    before = pools["k"].clone(), pools["ks"].clone()
+    lib.kv_reserve(lib.KVPages(table, dr, page), _layers(torch, pools, table), _cu(torch, start), _cu(torch, ctx), ok, 1023 * 16)
+    torch.cuda.synchronize()
+    want = {(0, 0): 1, (0, 1): 3, (1, 0): 4, (1, 1): 5, (1, 2): 6, (30000, 1023): 7, (65534, 0): 0, (65535, 0): 8}
+    at = (table >= 0).nonzero().tolist()
+    assert {(s, j): int(table[s, j]) for s, j in at} == want
+    refs[:9] = 1
+    assert np.array_equal(dr.cpu().numpy(), refs) and bool((ok == 1).all())
+    before[0][0, 8, :, :7], before[1][0, 8, :, :7] = before[0][0, 0, :, :7], before[1][0, 0, :, :7]
+    assert torch.equal(pools["k"], before[0]) and torch.equal(pools["ks"].view(torch.int32), before[1].view(torch.int32))
