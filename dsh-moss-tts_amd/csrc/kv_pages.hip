@@ -320,7 +320,7 @@ __global__ __launch_bounds__(kThreads) void compact_kernel(CompactArgs a, KvLaye
         const int r0 = a.row_start[s], r1 = a.row_start[s + 1], ctx = a.ctx_len[s];
         bool move = false;
         size_t src = 0, dst = 0;
-        if (r0 >= 0 && r1 <= a.rows && ctx >= 0 && t < min(r1 - r0, a.max_rows)) {
+        if (r0 >= 0 && r1 >= r0 && r1 <= a.rows && ctx >= 0 && t < min(r1 - r0, a.max_rows)) {  // (no difference leaves 32 bits)
             const int k = a.kept[r0 + t];
             if (k >= 0 && k < r1 - r0 && k != t) {
                 const unsigned ps = (unsigned)ctx + k, pd = (unsigned)ctx + t;  // (below 2^31 + 2^23)

@@ -34,3 +34,22 @@ def test_reserve_the_largest_table(torch_gpu):
     assert np.array_equal(dr.cpu().numpy(), refs) and bool((ok == 1).all())
     before[0][0, 8, :, :7], before[1][0, 8, :, :7] = before[0][0, 0, :, :7], before[1][0, 0, :, :7]
     assert torch.equal(pools["k"], before[0]) and torch.equal(pools["ks"].view(torch.int32), before[1].view(torch.int32))
+
+
+def test_compact_row_ranges_that_end_far_below_their_start(torch_gpu):
+    """A range whose length does not fit 32 bits is one of no rows, as any that ends before it starts: nothing moves, and nothing
+    behind the list is looked at (what follows it here would move rows)."""
+    torch = torch_gpu
+    print("compact row ranges", flush=True)
+    streams, page, n_pages, rows = 6, 16, 12, 40
+    pools = _pools(torch, np.random.default_rng(1), "e4m3", 2, n_pages, 2, page, 64)
+    table = _cu(torch, np.arange(n_pages, dtype=np.int32).reshape(streams, 2))
+    ls = _layers(torch, pools, table)
+    whole = (torch.arange(rows + 128, device="cuda", dtype=torch.int32) * 7 + 3) % 20
+    before = {k: v.view(torch.uint8).clone() for k, v in pools.items()}
+    low = -(2 ** 31)
+    # ranges of streams 0, 2 and 4 start within the rows and end at the lowest numbers; the others start below 0
+    start = _cu(torch, np.array([1, low, rows, low + 1, 39, low + 39, 0], np.int32))
+    lib.kv_compact(ls, start, torch.zeros(streams, dtype=torch.int32, device="cuda"), whole[:rows], 64)
+    torch.cuda.synchronize()
+    assert all(torch.equal(v.view(torch.uint8), before[k]) for k, v in pools.items())
