@@ -9,7 +9,8 @@
 // A draw compares u with as many borders as the vocabulary has tokens, and sums of 32-bit exponentials move each by up
 // to 2^-24: one draw in a hundred over 2^17 tokens.  So the row that is drawn from is weighed in 64 bits, at
 // 20 instructions of 8 cycles a logit; all others, of which only the sum is wanted, with the hardware's exponential (the sum's
-// error is some 2^-26 of it, and within 2^-18), which hides behind the reading.
+// error is some 2^-26 of it, and within 2^-18), which hides behind the reading.  Rows behind which a tree branches take 64 bits for
+// their sums too: 1 - p of a likely child leaves of such an error as many times more as it leaves less of the 1.
 //
 // A row is cut into pieces of a wave's values, four pieces a part.  First launch: every row, a workgroup a part, leaves each
 // part's maximum and sum.  Second: a workgroup for each part of a stream; each one walks by itself, weighs its part of the row that
@@ -147,11 +148,22 @@ __device__ __forceinline__ int2 nodes_of(const VerifyArgs &a, int s) {
     return r0 >= 0 && r1 >= r0 && r1 <= a.rows ? make_int2(r0, min(r1 - r0, a.max_rows)) : make_int2(0, 0);
 }
 
+// The parent of node t, -1: none (node 0, a mask without the node's own bit or without ancestors).
+__device__ __forceinline__ int parent_of(const VerifyArgs &a, int2 rows, int t) {
+    if (t == 0 || t >= rows.y) return -1;
+    if (a.row_mask == nullptr) return t - 1;
+    const uint64_t mask = a.row_mask[rows.x + t], up = mask & ((1ull << t) - 1);
+    return (mask >> t & 1) && up ? 63 - __builtin_clzll(up) : -1;
+}
+
 // ---------------------------------------------------------------- all rows
 
+// What is done for a row: GREEDY finds the largest, SUMS the sums with the hardware's exponential, EXACT those of marked rows in 64 bits.
+enum { GREEDY, SUMS, EXACT };
+
 // One piece of a row, by one wave: EPT values a lane, read V at a time.  Lane 0's is right.
-template <class T, int EPT, bool GREEDY>
-__device__ __forceinline__ Stat piece_stat(const T *p, int c, int vocab, float inv_t) {
+template <class T, int EPT, int HOW>
+__device__ __forceinline__ Stat piece_stat(const T *p, int c, int vocab, float inv_t, bool marked) {
     constexpr int V = std::min<int>(16 / (int)sizeof(T), EPT);
     const int base = c * EPT * 64 + ((int)threadIdx.x & 63) * V;
     float x[EPT / V][V];
@@ -163,10 +175,10 @@ __device__ __forceinline__ Stat piece_stat(const T *p, int c, int vocab, float i
     for (int i = 0; i < EPT / V; ++i)
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            if (GREEDY && x[i][j] > m) best = base + i * 64 * V + j;
+            if (HOW == GREEDY && x[i][j] > m) best = base + i * 64 * V + j;
             m = fmaxf(m, x[i][j]);
         }
-    if constexpr (GREEDY) {
+    if constexpr (HOW == GREEDY) {
         wave_argmax(m, best);
         return Stat{m, m > -INFINITY ? best : -1, 0.0};
     } else {
@@ -178,12 +190,27 @@ __device__ __forceinline__ Stat piece_stat(const T *p, int c, int vocab, float i
         for (int i = 0; i < EPT / V; ++i)
 #pragma unroll
             for (int j = 0; j < V; ++j) more[j & 3] += __builtin_amdgcn_exp2f(fmaf(x[i][j], 0.5f, h) * inv_t * (float)(2.0 * kLog2e));
-        return Stat{m, -1, wave_sum64(((double)more[0] + more[1]) + ((double)more[2] + more[3]))};
+        double sum = wave_sum64(((double)more[0] + more[1]) + ((double)more[2] + more[3]));
+        if constexpr (HOW == EXACT)
+            if (marked && sum > 0.0) {  // (neither NaN nor nothing)
+                sum = 0.0;
+#pragma unroll
+                for (int i = 0; i < EPT / V; ++i) {
+                    double v[V];
+                    weights<V>(x[i], m, (double)inv_t * kLog2e, v);
+#pragma unroll
+                    for (int j = 0; j < V; ++j) sum += v[j];
+                }
+                sum = wave_sum64(sum);
+            }
+        return Stat{m, -1, sum};
     }
 }
+// Whether node has several children; `parent` is the lane's node's.
+__device__ __forceinline__ bool branches(int parent, int node) { return __popcll(__ballot(parent == node)) > 1; }
 
 // One part of one row of the target (blockIdx.y 0) or the draft (1).
-template <class T, int EPT, bool GREEDY>
+template <class T, int EPT, int HOW>
 __global__ __launch_bounds__(kThreads) void stat_kernel(VerifyArgs a, int parts) {
     __shared__ Stat ls[kWaves];
     const int at = blockIdx.x / parts, part = blockIdx.x - at * parts;
@@ -196,7 +223,8 @@ __global__ __launch_bounds__(kThreads) void stat_kernel(VerifyArgs a, int parts)
     const T *p = of_draft ? (const T *)a.y + (rows.x + node) * a.y_row : (const T *)a.x + (rows.x + node) * a.x_row;
     const float inv_t = of_draft ? a.draft_inv_t : a.inv_t;
     const int w = threadIdx.x >> 6;
-    const Stat mine = piece_stat<T, EPT, GREEDY>(p, part * kWaves + w, a.vocab, inv_t);
+    const bool marked = HOW == EXACT && branches(parent_of(a, rows, threadIdx.x & 63), node);
+    const Stat mine = piece_stat<T, EPT, HOW>(p, part * kWaves + w, a.vocab, inv_t, marked);
     if ((threadIdx.x & 63) == 0) ls[w] = mine;
     __syncthreads();
     if (threadIdx.x == 0) {
@@ -208,7 +236,7 @@ __global__ __launch_bounds__(kThreads) void stat_kernel(VerifyArgs a, int parts)
                 r.m = ls[i].m;
                 r.best = ls[i].best;
             }
-        if constexpr (!GREEDY)
+        if constexpr (HOW != GREEDY)
 #pragma unroll
             for (int i = 0; i < kWaves; ++i)
                 if (!(ls[i].s == 0.0)) r.s += ls[i].m == r.m ? ls[i].s : ls[i].s * weight(ls[i].m, r.m, k);
@@ -225,16 +253,16 @@ struct WalkLds {
 };
 
 // The parts of a row together, by 8 lanes; `mine` is the lane's first.
-template <bool GREEDY>
+template <bool LARGEST>
 __device__ __forceinline__ Stat row_stat(const Stat &mine, const Stat *c, int parts, double k) {
     const int l = threadIdx.x & 7;
     float m = mine.m;
-    int best = GREEDY && m > -INFINITY ? mine.best : 0x7fffffff;
+    int best = LARGEST && m > -INFINITY ? mine.best : 0x7fffffff;
     for (int i = l + 8; i < parts; i += 8) {
-        if (GREEDY && c[i].m > m) best = c[i].best;
+        if (LARGEST && c[i].m > m) best = c[i].best;
         m = fmaxf(m, c[i].m);
     }
-    if constexpr (GREEDY) {
+    if constexpr (LARGEST) {
         argmax_step<4>(m, best);
         argmax_step<2>(m, best);
         argmax_step<1>(m, best);
@@ -264,18 +292,14 @@ struct Node {
     double u;
     float lx, ly;  // its token's logits behind the parent
 };
-template <class T, bool GREEDY>
+template <class T, bool LARGEST>
 __device__ __forceinline__ Node node_of(const VerifyArgs &a, int2 rows) {
     const int t = threadIdx.x, n = rows.y;
-    Node d{t < n, false, -1, t - 1, 0.0, -INFINITY, -INFINITY};
+    Node d{t < n, false, -1, -1, 0.0, -INFINITY, -INFINITY};
     if (d.in) d.tok = a.tokens[rows.x + t];
-    if (d.in && a.row_mask != nullptr) {
-        const uint64_t mask = a.row_mask[rows.x + t], up = mask & ((1ull << t) - 1);
-        d.parent = (mask >> t & 1) && up ? 63 - __builtin_clzll(up) : -1;
-    }
-    if (!d.in || t == 0) d.parent = -1;
+    d.parent = parent_of(a, rows, t);
     d.known = d.tok >= 0 && d.tok < a.vocab && d.parent >= 0;
-    if (!GREEDY && d.known) {
+    if (!LARGEST && d.known) {
         d.u = uniform(a.uniforms[rows.x + t]);
         d.lx = logit((const T *)a.x + (rows.x + d.parent) * a.x_row + d.tok);
         if (a.y != nullptr) d.ly = logit((const T *)a.y + (rows.x + d.parent) * a.y_row + d.tok);
@@ -285,11 +309,11 @@ __device__ __forceinline__ Node node_of(const VerifyArgs &a, int2 rows) {
 
 // The walk of one stream, by one workgroup: the rows' sums by all threads, then a lane a node.  pp, qq: the stream's parts; `writes`:
 // whether this workgroup leaves the outputs.
-template <bool GREEDY>
+template <bool LARGEST>
 __device__ __forceinline__ void walk(const VerifyArgs &a, int s, int2 rows, const Node &d, const Stat *pp, const Stat *qq, int parts, bool writes, WalkLds &lds) {
     const int t = threadIdx.x, n = rows.y;
     const bool drafted = a.y != nullptr, in = d.in, known = d.known;
-    const int all = GREEDY || !drafted ? a.max_rows : 2 * a.max_rows;  // the target's rows, then the draft's; what is past n is not used
+    const int all = LARGEST || !drafted ? a.max_rows : 2 * a.max_rows;  // the target's rows, then the draft's; what is past n is not used
     auto row_at = [&](int i) { return (i < a.max_rows ? pp + (size_t)i * parts : qq + (size_t)(i - a.max_rows) * parts); };
     Stat first{-INFINITY, -1, 0.0};
     if ((t >> 3) < all && (t & 7) < parts) first = row_at(t >> 3)[t & 7];
@@ -300,14 +324,14 @@ __device__ __forceinline__ void walk(const VerifyArgs &a, int s, int2 rows, cons
     for (int i = t >> 3; i < all; i += kThreads / 8) {
         const bool q = i >= a.max_rows;
         if (i >= kThreads / 8) first = (t & 7) < parts ? row_at(i)[t & 7] : Stat{-INFINITY, -1, 0.0};
-        const Stat r = row_stat<GREEDY>(first, row_at(i), parts, q ? kq : kp);
+        const Stat r = row_stat<LARGEST>(first, row_at(i), parts, q ? kq : kp);
         if ((t & 7) == 0) (q ? lds.q[i - a.max_rows] : lds.p[i]) = r;
     }
     __syncthreads();
     if (t < 64) {
         bool accept = false;
         const Stat p = lds.p[of];
-        if constexpr (GREEDY) {
+        if constexpr (LARGEST) {
             accept = known && tok == p.best;
         } else {
             double prob = 0.0;
@@ -347,7 +371,7 @@ __device__ __forceinline__ void walk(const VerifyArgs &a, int s, int2 rows, cons
             if (on >> t & 1) a.path[rows.x + __popcll(on & ((1ull << t) - 1))] = t;
             if (t >= taken) a.path[rows.x + t] = -1;
         }
-        const bool child = !GREEDY && !drafted && parent == cur && known;
+        const bool child = !LARGEST && !drafted && parent == cur && known;
         const uint64_t children = __ballot(child);
         if (child) lds.gone[__popcll(children & ((1ull << t) - 1))] = tok;
         if (t == 0) {
@@ -358,7 +382,7 @@ __device__ __forceinline__ void walk(const VerifyArgs &a, int s, int2 rows, cons
             lds.draw = Draw{pl.m, ql.m, rows.x + cur, !(pl.s > 0.0) ? DRAW_NONE : (ql.s > 0.0 ? DRAW_REST : DRAW_P)};
             if (writes) {
                 a.accepted[s] = __popcll(on) - 1;
-                if (GREEDY) a.next[s] = pl.best;
+                if (LARGEST) a.next[s] = pl.best;
             }
         }
     }
@@ -660,7 +684,7 @@ __global__ __launch_bounds__(kThreads) void rest_kernel(VerifyArgs a, int pieces
 // All of it in one launch, a workgroup a stream, where its rows have no more than kSmallPieces pieces: the smallest calls are
 // launches and chains of loads.
 constexpr int kSmallPieces = 32, kSmallEpt = 16;
-template <class T, bool GREEDY>
+template <class T, int HOW>
 __global__ __launch_bounds__(kThreads) void small_kernel(VerifyArgs a, int pieces) {
     constexpr int EPT = kSmallEpt;
     __shared__ Stat p[kSmallPieces], q[kSmallPieces];
@@ -671,20 +695,21 @@ __global__ __launch_bounds__(kThreads) void small_kernel(VerifyArgs a, int piece
     const int2 rows = nodes_of(a, s);
     if (no_rows(a, s, rows, true)) return;
     const bool drafted = a.y != nullptr;
-    const Node mine = node_of<T, GREEDY>(a, rows);
+    const Node mine = node_of<T, HOW == GREEDY>(a, rows);
+    const int parent = HOW == EXACT ? parent_of(a, rows, t & 63) : -1;
     const int units = rows.y * pieces;
     for (int i = w; i < units; i += kWaves) {
         const int node = i / pieces, c = i - node * pieces;
-        const Stat m = piece_stat<T, EPT, GREEDY>((const T *)a.x + (rows.x + node) * a.x_row, c, a.vocab, a.inv_t);
+        const Stat m = piece_stat<T, EPT, HOW>((const T *)a.x + (rows.x + node) * a.x_row, c, a.vocab, a.inv_t, HOW == EXACT && branches(parent, node));
         if ((t & 63) == 0) p[i] = m;
         if (drafted && node < rows.y - 1) {
-            const Stat n = piece_stat<T, EPT, GREEDY>((const T *)a.y + (rows.x + node) * a.y_row, c, a.vocab, a.draft_inv_t);
+            const Stat n = piece_stat<T, EPT, HOW>((const T *)a.y + (rows.x + node) * a.y_row, c, a.vocab, a.draft_inv_t, false);
             if ((t & 63) == 0) q[i] = n;
         }
     }
     __syncthreads();
-    walk<GREEDY>(a, s, rows, mine, p, q, pieces, true, wl);
-    if constexpr (!GREEDY) {
+    walk<HOW == GREEDY>(a, s, rows, mine, p, q, pieces, true, wl);
+    if constexpr (HOW != GREEDY) {
         const Draw d = wl.draw;
         int got = -1;
         if (d.mode != DRAW_NONE) {
@@ -741,12 +766,15 @@ hipError_t verify_e(const VerifyArgs &a, hipStream_t s) {
     const int parts = parts_of(a.streams * a.max_rows, a.vocab), pieces = (a.vocab + EPT * 64 - 1) / (EPT * 64);
     const dim3 rows((unsigned)a.streams * a.max_rows * parts, a.y != nullptr ? 2 : 1), of_streams((unsigned)a.streams * parts);
     if (a.greedy) {
-        hipLaunchKernelGGL((stat_kernel<T, EPT, true>), rows, dim3(kThreads), 0, s, a, parts);
+        hipLaunchKernelGGL((stat_kernel<T, EPT, GREEDY>), rows, dim3(kThreads), 0, s, a, parts);
         if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;  // (what follows trusts what it leaves)
         hipLaunchKernelGGL(greedy_kernel, dim3(a.streams), dim3(kThreads), 0, s, a, parts);
         return hipGetLastError();
     }
-    hipLaunchKernelGGL((stat_kernel<T, EPT, false>), rows, dim3(kThreads), 0, s, a, parts);
+    if (a.row_mask != nullptr)
+        hipLaunchKernelGGL((stat_kernel<T, EPT, EXACT>), rows, dim3(kThreads), 0, s, a, parts);
+    else
+        hipLaunchKernelGGL((stat_kernel<T, EPT, SUMS>), rows, dim3(kThreads), 0, s, a, parts);
     if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
     if (a.y != nullptr) {
         hipLaunchKernelGGL((walk_kernel<T, EPT, true>), of_streams, dim3(kThreads), 0, s, a, pieces, parts);
@@ -764,9 +792,11 @@ hipError_t verify_t(const VerifyArgs &a, hipStream_t s) {
     if (small(a.max_rows, a.vocab)) {
         const int pieces = (a.vocab + kSmallEpt * 64 - 1) / (kSmallEpt * 64);
         if (a.greedy)
-            hipLaunchKernelGGL((small_kernel<T, true>), dim3(a.streams), dim3(kThreads), 0, s, a, pieces);
+            hipLaunchKernelGGL((small_kernel<T, GREEDY>), dim3(a.streams), dim3(kThreads), 0, s, a, pieces);
+        else if (a.row_mask != nullptr)
+            hipLaunchKernelGGL((small_kernel<T, EXACT>), dim3(a.streams), dim3(kThreads), 0, s, a, pieces);
         else
-            hipLaunchKernelGGL((small_kernel<T, false>), dim3(a.streams), dim3(kThreads), 0, s, a, pieces);
+            hipLaunchKernelGGL((small_kernel<T, SUMS>), dim3(a.streams), dim3(kThreads), 0, s, a, pieces);
         return hipGetLastError();
     }
     switch (ept_of(a.streams * a.max_rows, a.vocab)) {

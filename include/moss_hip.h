@@ -486,7 +486,7 @@ int moss_hip_token_logprobs_workspace(int rows, int vocab, int top_k, size_t *by
  * uniforms [rows]: u of each node, numbers of [0, 1) (others count as the nearest of 0 and 1, NaN as 1); row 0's draws the next token: the
  * first whose cumulative sum, in the order of the vocabulary, passes u times the whole.  Where nothing is left over,
  * it is drawn from p.  The row that is drawn from is weighed and summed in 64 bits (what is under 2^-980 of its largest counts as nothing); the sums
- * that acceptance goes by are within 2^-18 of themselves.  The streams' row ranges lie apart.  greedy takes no uniforms and no draft_logits.
+ * that acceptance goes by are within 2^-18 of themselves, those of rows with several children, of whose p little may be left, within 2^-44.  The streams' row ranges lie apart.  greedy takes no uniforms and no draft_logits.
  *   accepted [streams]: drafted nodes accepted.
  *   path [rows]: entry row_start[s] + j is the node that the walk took as its j-th (0 first), -1 past the last: what
  *     moss_hip_kv_compact takes.  Rows of no stream, and a stream's rows past max_rows, stay as they were.
