@@ -970,7 +970,7 @@ int moss_hip_verify_tokens(const void *logits, int64_t row_stride, int dtype, co
         for (const float t : {inv_temperature, draft_inv_temperature})
             if (!(t > 0.0f) || !std::isfinite(t)) throw Status(MOSS_HIP_EINVAL, "inverse temperatures must be positive and finite");
         if (streams == 0) return;
-        check_workspace(workspace, workspace_bytes, mh::verify_workspace(streams, max_rows, vocab, draft_logits != nullptr), "moss_hip_verify_tokens");
+        check_workspace(workspace, workspace_bytes, mh::verify_need(streams, max_rows, vocab, draft_logits != nullptr), "moss_hip_verify_tokens");
         mh::VerifyArgs a;
         a.x = logits;
         a.y = draft_logits;

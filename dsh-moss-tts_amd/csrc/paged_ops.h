@@ -158,7 +158,8 @@ struct VerifyArgs {
     int *accepted = nullptr, *path = nullptr, *next = nullptr;
     void *ws = nullptr;
 };
-size_t verify_workspace(int streams, int max_rows, int vocab, bool draft);
+size_t verify_need(int streams, int max_rows, int vocab, bool draft);       // of a call
+size_t verify_workspace(int streams, int max_rows, int vocab, bool draft);  // of any call of no more streams and rows
 hipError_t launch_verify(const VerifyArgs &a, hipStream_t s);
 
 // ---- low-rank adapters beside a projection

@@ -750,9 +750,10 @@ __global__ __launch_bounds__(kThreads) void small_kernel(VerifyArgs a, int piece
 bool small(int max_rows, int vocab) { return max_rows * ((vocab + kSmallEpt * 64 - 1) / (kSmallEpt * 64)) <= kSmallPieces; }
 
 // Values of a lane of a piece: few while that fills the chip, many where the parts' sums would be much work themselves.
+constexpr int kFinePieces = 16, kFineRows = 1024;  // parts of 4 values a lane: most of a row, and of all rows
 int ept_of(int rows, int vocab) {
-    const int few = (vocab + 1023) / 1024;  // parts of 4 values a lane
-    if (few <= 16 && (long long)rows * few <= 1024) return 4;
+    const int few = (vocab + 1023) / 1024;
+    if (few <= kFinePieces && (long long)rows * few <= kFineRows) return 4;
     return vocab <= 64 * 1024 ? 16 : 32;
 }
 int parts_of(int rows, int vocab) {
@@ -808,10 +809,19 @@ hipError_t verify_t(const VerifyArgs &a, hipStream_t s) {
 
 }  // namespace
 
-size_t verify_workspace(int streams, int max_rows, int vocab, bool draft) {
+size_t verify_need(int streams, int max_rows, int vocab, bool draft) {
     if (small(max_rows, vocab)) return 0;
     const VerifyWs w = verify_ws(streams, max_rows, parts_of(streams * max_rows, vocab), draft, nullptr);
     return (size_t)(uintptr_t)(w.draw + (draft ? streams : 0));
+}
+// What calls of up to so many streams and rows need.  Few rows are cut finer (ept_of), so the most can be that of the largest call that
+// still is.
+size_t verify_workspace(int streams, int max_rows, int vocab, bool draft) {
+    size_t most = verify_need(streams, max_rows, vocab, draft);
+    const int few = (vocab + 1023) / 1024;
+    for (int r = 1; r <= max_rows && few <= kFinePieces; ++r)
+        if (const int s = std::min(streams, kFineRows / (few * r)); s > 0) most = std::max(most, verify_need(s, r, vocab, draft));
+    return most;
 }
 
 hipError_t launch_verify(const VerifyArgs &a, hipStream_t s) { return a.dtype == ELEM_F16 ? verify_t<__half>(a, s) : verify_t<float>(a, s); }

@@ -539,7 +539,7 @@ def token_logprobs(logits, tokens, logprob, entropy=None, top_ids=None, top_logp
 
 
 def verify_tokens_workspace(streams: int, max_rows: int, vocab: int, draft: bool = False) -> int:
-    """Bytes of workspace verify_tokens takes (draft: with draft_logits)."""
+    """Bytes of workspace verify_tokens takes (draft: with draft_logits) with this many streams and rows, or fewer."""
     n = C.c_size_t(0)
     check(load().moss_hip_verify_tokens_workspace(streams, max_rows, vocab, int(draft), C.byref(n)))
     return n.value

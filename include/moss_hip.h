@@ -494,7 +494,8 @@ int moss_hip_token_logprobs_workspace(int rows, int vocab, int top_k, size_t *by
  * -inf logits are ruled out.  A row with a NaN or +inf, or of nothing but -inf, is no distribution: no child of it is
  * accepted, and no token (-1) follows; a draft's row like that rejects its child and the next token is drawn from p.  A token
  * outside [0, vocab) is rejected.  Without rows, or with a row range not within [0, rows], a stream has accepted 0 and
- * next_token -1.  vocab <= 2^20.  workspace as above: moss_hip_verify_tokens_workspace bytes (draft: whether draft_logits are given). */
+ * next_token -1.  vocab <= 2^20.  workspace as above: moss_hip_verify_tokens_workspace bytes (draft: whether draft_logits are
+ * given), which are enough for any call of the same vocab with no more streams and max_rows, and with draft_logits or without where draft is 1. */
 int moss_hip_verify_tokens(const void *logits, int64_t row_stride, int dtype, const void *draft_logits, int64_t draft_stride,
                            int rows, int vocab, const int32_t *tokens, const int32_t *row_start, const uint64_t *row_mask,
                            int streams, int max_rows, const double *uniforms, float inv_temperature, float draft_inv_temperature,

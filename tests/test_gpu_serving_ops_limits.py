@@ -2,8 +2,9 @@
 import numpy as np
 import pytest
 
+import serving_oracle as so
 from mosship import lib
-from test_gpu_serving_ops import _cu, _layers, _pools
+from test_gpu_serving_ops import _cu, _draft, _layers, _pools
 
 pytestmark = pytest.mark.gpu
 
@@ -53,3 +54,27 @@ def test_compact_row_ranges_that_end_far_below_their_start(torch_gpu):
     lib.kv_compact(ls, start, torch.zeros(streams, dtype=torch.int32, device="cuda"), whole[:rows], 64)
     torch.cuda.synchronize()
     assert all(torch.equal(v.view(torch.uint8), before[k]) for k, v in pools.items())
+
+
+def test_verify_batches_that_shrink(torch_gpu):
+    """One workspace, of the bytes that the largest batch asks for, through batches of fewer streams and rows: all as by themselves."""
+    torch = torch_gpu
+    rng = np.random.default_rng(17)
+    vocab, most, rows = 16384, 17, 4
+    x, tok, _, start = _draft(rng, [rows] * most, vocab, True, near=0.9, peak=18.0)
+    y = (x + 0.5 * rng.standard_normal(x.shape)).astype(np.float32)
+    u = rng.random(len(tok))
+    size = lib.verify_tokens_workspace(most, rows, vocab, draft=True)
+    whole = torch.full((size + 8192,), 0xA5, dtype=torch.uint8, device="cuda")
+    for streams, max_rows, drafted in ((17, 4, True), (16, 4, True), (16, 4, False), (11, 4, True), (5, 3, True), (1, 4, True), (2, 2, True)):
+        print(f"shrink {streams} {max_rows} {drafted}", flush=True)
+        n = streams * rows
+        acc, nxt = (torch.empty(streams, dtype=torch.int32, device="cuda") for _ in range(2))
+        path = torch.full((n,), -7, dtype=torch.int32, device="cuda")
+        d = _cu(torch, y[:n]) if drafted else None
+        lib.verify_tokens(_cu(torch, x[:n]), _cu(torch, tok[:n]), _cu(torch, start[:streams + 1]), acc, path, nxt, max_rows,
+                          uniforms=_cu(torch, u[:n]), draft_logits=d, workspace=whole[4096:4096 + size])
+        *want, near = so.verify(x[:n], tok[:n], start[:streams + 1], u[:n], max_rows, y[:n] if drafted else None, path=np.full(n, -7))
+        assert near > 1
+        assert all(np.array_equal(g.cpu().numpy(), w) for g, w in zip((acc, path, nxt), want))
+    assert bool((whole[:4096] == 0xA5).all()) and bool((whole[4096 + size:] == 0xA5).all())
