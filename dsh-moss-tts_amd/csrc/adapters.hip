@@ -446,10 +446,19 @@ void adapter_sizes(const AdapterArgs &a, size_t *a_bytes, size_t *b_bytes) {
     *b_bytes = a.n * b_size(a.max_rank, a.out) * 2;
 }
 
-hipError_t launch_adapter_pack(const AdapterPackArgs &p, hipStream_t s) {
+hipError_t launch_adapter_pack(const AdapterPackArgs &all, hipStream_t s) {
     (void)hipGetLastError();
-    const int per_a = (int)(a_size(p.max_rank, p.cols) / 8), per_b = (int)(b_size(p.max_rank, p.out) / 8);
-    hipLaunchKernelGGL(pack_kernel, dim3((std::max(per_a, per_b) + 255) / 256, p.count), dim3(256), 0, s, p, per_a, per_b);
+    constexpr int kMost = 65535;  // of a grid's y
+    const int per_a = (int)(a_size(all.max_rank, all.cols) / 8), per_b = (int)(b_size(all.max_rank, all.out) / 8);
+    for (int from = 0; from < all.count; from += kMost) {
+        AdapterPackArgs p = all;
+        p.a = (const __half *)all.a + (size_t)from * all.max_rank * all.cols;
+        p.b = (const __half *)all.b + (size_t)from * all.out * all.max_rank;
+        if (all.rank != nullptr) p.rank = all.rank + from;
+        p.first = all.first + from;
+        p.count = std::min(all.count - from, kMost);
+        hipLaunchKernelGGL(pack_kernel, dim3((std::max(per_a, per_b) + 255) / 256, p.count), dim3(256), 0, s, p, per_a, per_b);
+    }
     return hipGetLastError();
 }
 

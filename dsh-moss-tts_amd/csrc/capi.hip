@@ -1090,8 +1090,8 @@ int moss_hip_adapter_pack(const moss_hip_adapters *adapters, int first, int coun
         const mh::AdapterArgs to = adapter_args(adapters);
         check_adapter_weights(to.a, to.b);
         check_adapter_weights(a, b);
-        if (first < 0 || count < 0 || count > to.n || first > to.n - count || count > 65535)
-            throw Status(MOSS_HIP_EINVAL, "need first, count >= 0 within the adapters, count at most 65535");
+        if (first < 0 || count < 0 || count > to.n || first > to.n - count)
+            throw Status(MOSS_HIP_EINVAL, "need first, count >= 0 within the adapters");
         if (count == 0) return;
         mh::AdapterPackArgs p;
         p.a = a;

@@ -4,7 +4,7 @@ import pytest
 
 import serving_oracle as so
 from mosship import lib
-from test_gpu_serving_ops import _cu, _draft, _layers, _pools
+from test_gpu_serving_ops import _adapter_want, _cu, _draft, _layers, _pools
 
 pytestmark = pytest.mark.gpu
 
@@ -78,3 +78,33 @@ def test_verify_batches_that_shrink(torch_gpu):
         assert near > 1
         assert all(np.array_equal(g.cpu().numpy(), w) for g, w in zip((acc, path, nxt), want))
     assert bool((whole[:4096] == 0xA5).all()) and bool((whole[4096 + size:] == 0xA5).all())
+
+
+def test_more_adapters_than_a_launch_packs(torch_gpu):
+    """70001 adapters, laid out at once and some of them replaced across the first 65535."""
+    torch = torch_gpu
+    print("many adapters", flush=True)
+    n, cols, out, rank = 70001, 32, 16, 16
+    g = torch.Generator(device="cuda").manual_seed(5)
+    a = (torch.randn(n, rank, cols, generator=g, device="cuda") * cols ** -0.5).half()
+    b = (torch.randn(n, out, rank, generator=g, device="cuda") * 0.3).half()
+    ranks = torch.randint(0, rank + 1, (n,), generator=g, device="cuda").to(torch.int32)
+    scale = torch.rand(n, generator=g, device="cuda") + 0.5
+    which = torch.tensor([0, 1, 65534, 65535, 65536, 69999, 70000, 70001, -1, 40000, 65533, 68000], dtype=torch.int32, device="cuda")
+    x, base = (torch.randn(which.numel(), w, generator=g, device="cuda") for w in (cols, out))
+    ad, y = lib.Adapters(a, b, ranks, scale), torch.empty(which.numel(), out, device="cuda")
+
+    def check():
+        lib.adapter_rows(x, ad, which, y, base=base)
+        used = which.cpu().numpy().astype(np.int64)
+        at = [int(i) if 0 <= i < n else 0 for i in used]
+        pick = lambda t: t[at].cpu().numpy()  # noqa: E731
+        rows = np.where((used >= 0) & (used < n), np.arange(len(used)), -1).astype(np.int32)
+        want, tol = _adapter_want(x.double().cpu().numpy(), base.double().cpu().numpy(), rows, pick(a), pick(b), pick(ranks), pick(scale), True)
+        assert (np.abs(y.double().cpu().numpy() - want) <= tol).all()
+    check()
+    first, count = 2, 69000
+    a[first:first + count] = a[first:first + count].flip(0)
+    ranks[first:first + count] = ranks[first:first + count].flip(0)
+    ad.set(first, a[first:first + count].contiguous(), b[first:first + count].contiguous(), ranks[first:first + count].contiguous())
+    check()
