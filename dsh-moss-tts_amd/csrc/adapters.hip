@@ -12,9 +12,15 @@
 //
 // Weights are fp16, laid out once in the order in which a wave's lanes hold them, so that a load is 1 KiB in one piece.
 // Rows go through LDS for the same reason: as an operand, lanes next to each other hold different rows, and 64 separate
-// accesses a load made the L1 the limit: 8191 fp16 rows of 4096 -> 4096, rank 64, took 129 us, now 86 (2.4 TB/s; a copy of
-// those sizes reaches 3.2).  What is left is that a workgroup's registers fill a compute unit, so that its two products
-// do not overlap with another's.  2896 fp32 rows of 768 -> 2304, rank 16: 16.3 us, 3.9 TB/s.  One row: 5.7 us, a chain of loads.
+// accesses a load made the L1 the limit: 8191 fp16 rows of 4096 -> 4096, rank 64, took 129 us, 86 through LDS, now 79 (2.5 TB/s of the
+// 201 MB that it reads and writes; a copy of 134 MB in tiles of 16 rows reaches 3.2).  What is left is that a workgroup's registers
+// fill a compute unit, so that its two products do not overlap with another's.  2896 fp32 rows of 768 -> 2304, rank 16: 13.9 us, 4.5
+// TB/s.  One row: 5.7 us, a chain of loads.
+//
+// No kernel keeps anything in scratch memory: weights are held as far as they have to run ahead, in places that the next ones take as
+// soon as they have been used; places in LDS are worked out anew for each tile; and the eight partial sums of t are added up once
+// where ranks are many.  Before that, 4260 fp32 rows that change between 5 adapters of rank 128, 768 -> 768, took 170 us, now 66; 7434 of 14,
+// 32 -> 544, 346, now 134.  Such rows read every adapter among 16 of them again for each 16.
 //
 // fp16 rows are multiplied as they are.  32-bit rows, and t, go in as two fp16 numbers, hi + lo, 22 bits: of 128 columns of a
 // row (of all ranks of t) the largest is put at 2^14 by a power of two, which leaves 2^-39 of the largest as the
@@ -22,6 +28,7 @@
 // than 8 of them go into one sum before it is added up in 32 bits with rounding.  A row's sums do not depend on where in a
 // tile it stands, nor on the other rows.
 #include <algorithm>
+#include <type_traits>
 
 #include "paged_ops.h"
 
@@ -42,6 +49,14 @@ __device__ __forceinline__ float get(T x) {
         return __half2float(x);
     else
         return x;
+}
+
+template <int N, int I = 0, class F>
+__device__ __forceinline__ void static_for(F &&f) {
+    if constexpr (I < N) {
+        f(std::integral_constant<int, I>{});
+        static_for<N, I + 1>(f);
+    }
 }
 
 union Frag {
@@ -74,6 +89,13 @@ __device__ __forceinline__ void split(const float (&x)[N], float up, Frag &hi, F
 __device__ __forceinline__ float row_max(float v) {  // over the lanes of one row
     v = fmaxf(v, xshfl<16>(v));
     return fmaxf(v, xshfl<32>(v));
+}
+// This thread's number, as one that the compiler does not know: places in LDS that follow from it are not held in registers from one
+// tile to the next, which took 60 of them.
+__device__ __forceinline__ int own_thread() {
+    int t = threadIdx.x;
+    asm volatile("" : "+v"(t));
+    return t;
 }
 // What lanes of this wave wrote to LDS can be read by others of it.
 __device__ __forceinline__ void wave_fence() {
@@ -117,6 +139,12 @@ __global__ __launch_bounds__(256) void pack_kernel(AdapterPackArgs p, int per_a,
     }
 }
 
+// A tile's rows of one adapter: row0 + r for the bits r of who.
+struct TileRows {
+    int64_t row0;
+    uint64_t who;
+};
+
 // ---------------------------------------------------------------- t = A x
 
 // 16 rows of 128 columns in LDS, one wave's: 16-byte pieces, piece c of row r at c ^ r of its 256 bytes, so that neither the
@@ -128,62 +156,61 @@ struct Tile {
     static constexpr int kBytes = 16 * kChunk * (int)sizeof(X);
     static __device__ __forceinline__ int at(int row, int piece) { return row * 16 * W + (piece & ~15) + ((piece ^ row) & 15); }
     // Lane l of load i: row and piece.
-    static __device__ __forceinline__ int row_of(int i) { return W == 1 ? 4 * i + ((threadIdx.x & 63) >> 4) : 2 * i + ((threadIdx.x & 63) >> 5); }
-    static __device__ __forceinline__ int piece_of() { return threadIdx.x & (16 * W - 1); }
+    static __device__ __forceinline__ int row_of(int lane, int i) { return W == 1 ? 4 * i + (lane >> 4) : 2 * i + (lane >> 5); }
+    static __device__ __forceinline__ int piece_of(int lane) { return lane & (16 * W - 1); }
 };
 
 template <class X, int RK>
 struct Shrink {
     using T = Tile<X>;
     static constexpr int W = T::W;
+    static constexpr int KB = std::min(RK, 2), R = std::min(RK, 4);  // 16s of ranks at a time, and whose weights are held
     const X *x[T::N];  // the rows of this lane's pieces
     const __half *w;
-    int cols;
+    int cols, lane;
 
-    __device__ __forceinline__ Shrink(const AdapterArgs &a, int id, int row0, uint64_t who) : cols(a.cols) {
-        const int some = __builtin_ctzll(who);  // rows of others are not read: their lanes read this one
+    __device__ __forceinline__ Shrink(const AdapterArgs &a, int id, const TileRows &rows, int own) : cols(a.cols), lane(own) {
+        const int some = __builtin_ctzll(rows.who);  // rows of others are not read: their lanes read this one
 #pragma unroll
         for (int i = 0; i < T::N; ++i) {
-            const int r = T::row_of(i);
-            x[i] = (const X *)a.x + (row0 + (who >> r & 1 ? r : some)) * a.x_row;
+            const int r = T::row_of(lane, i);
+            x[i] = (const X *)a.x + (rows.row0 + (rows.who >> r & 1 ? r : some)) * a.x_row;
         }
-        w = (const __half *)a.a + id * a_size(a.max_rank, a.cols) + 8 * (threadIdx.x & 63);
+        w = (const __half *)a.a + id * a_size(a.max_rank, a.cols) + 8 * lane;
     }
     __device__ __forceinline__ void load(int c, uint4 (&raw)[T::N]) const {
-        const int col = c + T::piece_of() * (8 / W);
+        const int col = c + T::piece_of(lane) * (8 / W);
 #pragma unroll
         for (int i = 0; i < T::N; ++i) {
             __builtin_memcpy(&raw[i], x[i] + min(col, cols - 8 / W), 16);
             if (col >= cols) raw[i] = uint4{};  // (of the last chunk)
         }
     }
-    // Chunks c, c + step, ... of the columns, into sum.  The rows' loads run a chunk ahead.
+    __device__ __forceinline__ void load_weights(int c, int k, Frag (&f)[4]) const {
+#pragma unroll
+        for (int s = 0; s < 4; ++s) f[s].u = *(const uint4 *)(w + ((size_t)min(c / 32 + s, cols / 32 - 1) * RK + k) * 512);
+    }
+    // Chunks c, c + step, ... of the columns, into sum.  The rows' loads run a chunk ahead, the weights' R 16s of ranks: all of a
+    // chunk's at rank 128 would be half of the registers.
     __device__ __forceinline__ void run(int c, int step, uint4 *lds, f32x4_t (&sum)[RK]) const {
         if (c >= cols) return;
-        const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
+        const int m = lane & 15, g = lane >> 4;
         uint4 raw[T::N];
+        Frag f[R][4];
         load(c, raw);
+#pragma unroll
+        for (int k = 0; k < R; ++k) load_weights(c, k, f[k]);
         while (true) {
-            Frag f[4][RK];
-#pragma unroll
-            for (int s = 0; s < 4; ++s)
-#pragma unroll
-                for (int k = 0; k < RK; ++k) f[s][k].u = *(const uint4 *)(w + ((size_t)min(c / 32 + s, cols / 32 - 1) * RK + k) * 512);
             wave_fence();  // (the last chunk has been read)
 #pragma unroll
-            for (int i = 0; i < T::N; ++i) lds[T::at(T::row_of(i), T::piece_of())] = raw[i];
+            for (int i = 0; i < T::N; ++i) lds[T::at(T::row_of(lane, i), T::piece_of(lane))] = raw[i];
             wave_fence();
             const int next = c + step;
-            if (next < cols) load(next, raw);
-            f32x4_t acc[RK] = {};
+            Frag hi[4], lo[4];
             float down = 1.0f;
             if constexpr (W == 1) {
 #pragma unroll
-                for (int s = 0; s < 4; ++s) {
-                    const Frag v{lds[T::at(m, 4 * s + g)]};
-#pragma unroll
-                    for (int k = 0; k < RK; ++k) acc[k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f[s][k].h, v.h, acc[k], 0, 0, 0);
-                }
+                for (int s = 0; s < 4; ++s) hi[s].u = lds[T::at(m, 4 * s + g)];
             } else {
                 float v[4][8], top = 0.0f;
 #pragma unroll
@@ -196,20 +223,30 @@ struct Shrink {
                 const Power p = power_of(row_max(top));
                 down = p.down;
 #pragma unroll
-                for (int s = 0; s < 4; ++s) {
-                    Frag hi, lo;
-                    split(v[s], p.up, hi, lo);
-#pragma unroll
-                    for (int k = 0; k < RK; ++k) {
-                        acc[k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f[s][k].h, hi.h, acc[k], 0, 0, 0);
-                        acc[k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f[s][k].h, lo.h, acc[k], 0, 0, 0);
-                    }
-                }
+                for (int s = 0; s < 4; ++s) split(v[s], p.up, hi[s], lo[s]);
             }
 #pragma unroll
-            for (int k = 0; k < RK; ++k)
+            for (int k0 = 0; k0 < RK; k0 += KB) {
+                if (k0 == RK - R && next < cols) load(next, raw);  // (behind the last weights of this chunk, which are waited for first)
+                f32x4_t acc[KB] = {};
 #pragma unroll
-                for (int i = 0; i < 4; ++i) sum[k][i] = fmaf(acc[k][i], down, sum[k][i]);
+                for (int s = 0; s < 4; ++s) {
+#pragma unroll
+                    for (int k = 0; k < KB; ++k) acc[k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f[(k0 + k) % R][s].h, hi[s].h, acc[k], 0, 0, 0);
+                    if constexpr (W == 2)
+#pragma unroll
+                        for (int k = 0; k < KB; ++k) acc[k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f[(k0 + k) % R][s].h, lo[s].h, acc[k], 0, 0, 0);
+                }
+#pragma unroll
+                for (int k = 0; k < KB; ++k) {
+                    if (k0 + k + R < RK)
+                        load_weights(c, k0 + k + R, f[(k0 + k) % R]);
+                    else if (next < cols)
+                        load_weights(next, k0 + k + R - RK, f[(k0 + k) % R]);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) sum[k0 + k][i] = fmaf(acc[k][i], down, sum[k0 + k][i]);
+                }
+            }
             if (next >= cols) break;
             c = next;
         }
@@ -225,8 +262,8 @@ struct Rows {
     Frag hi[KS], lo[KS];
     float factor;
     template <class Get>
-    __device__ __forceinline__ void set(float scale, Get &&get_t) {
-        const int g = (threadIdx.x & 63) >> 4;
+    __device__ __forceinline__ void set(float scale, int lane, Get &&get_t) {
+        const int g = lane >> 4;
         float v[KS][N], top = 0.0f;
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
@@ -247,52 +284,55 @@ template <class Y, int RK>
 struct Expand {
     static constexpr int KS = Rows<RK>::KS, F = RK == 1 ? 2 : 4 * KS;  // 16-byte loads of weights
     static constexpr int P = 16 / (int)sizeof(Y), N = 16 / P;          // outputs of a piece of y, pieces of a lane
-    struct In {
-        Frag f[F];
-        uint4 raw[N];
-    };
     const Y *base[N];
     Y *y[N];
     bool mine[N];
-    int out1;
+    int out1, lane;
     const __half *w;
 
-    static __device__ __forceinline__ int row_of(int i) { return (i * 64 + ((int)threadIdx.x & 63)) / (64 / P); }
-    static __device__ __forceinline__ int first() { return ((int)threadIdx.x & (64 / P - 1)) * P; }
-    __device__ __forceinline__ Expand(const AdapterArgs &a, int id, int64_t row0, uint64_t who, int end) : out1(end) {
+    __device__ __forceinline__ int row_of(int i) const { return (i * 64 + lane) / (64 / P); }
+    __device__ __forceinline__ int first() const { return (lane & (64 / P - 1)) * P; }
+    __device__ __forceinline__ Expand(const AdapterArgs &a, int id, const TileRows &rows, int end, int own) : out1(end), lane(own) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int r = row_of(i);
-            mine[i] = who >> r & 1;
-            base[i] = (const Y *)a.base + (row0 + r) * a.base_row + first();
-            y[i] = (Y *)a.y + (row0 + r) * a.y_row + first();
+            mine[i] = rows.who >> r & 1;
+            base[i] = (const Y *)a.base + (rows.row0 + r) * a.base_row + first();
+            y[i] = (Y *)a.y + (rows.row0 + r) * a.y_row + first();
         }
-        w = (const __half *)a.b + id * b_size(a.max_rank, a.out) + 8 * (threadIdx.x & 63);
+        w = (const __half *)a.b + id * b_size(a.max_rank, a.out) + 8 * lane;
     }
-    __device__ __forceinline__ void load(int o, In &in) const {
+    __device__ __forceinline__ void load_base(int o, uint4 (&raw)[N]) const {
 #pragma unroll
         for (int i = 0; i < N; ++i)
-            if (mine[i] && o + first() < out1) __builtin_memcpy(&in.raw[i], base[i] + o, 16);
-#pragma unroll
-        for (int i = 0; i < F; ++i) in.f[i].u = *(const uint4 *)(w + ((size_t)(o / 64) * F + i) * 512);
+            if (mine[i] && o + first() < out1) __builtin_memcpy(&raw[i], base[i] + o, 16);
     }
-    __device__ __forceinline__ void finish(int o, const Rows<RK> &t, const In &in, uint4 *lds) const {
-        const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
+    template <int FROM, int TO>
+    __device__ __forceinline__ void load_weights(int o, Frag (&f)[F]) const {
+#pragma unroll
+        for (int i = FROM; i < TO; ++i) f[i].u = *(const uint4 *)(w + ((size_t)(o / 64) * F + i) * 512);
+    }
+    // Group o; the weights of group `next` (none: -1) take the places of those that have been used.
+    __device__ __forceinline__ void finish(int o, int next, const Rows<RK> &t, Frag (&f)[F], const uint4 (&raw)[N], uint4 *lds) const {
+        const int m = lane & 15, g = lane >> 4;
         f32x4_t acc[4] = {};
         if constexpr (RK == 1) {
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-                acc[q] = __builtin_amdgcn_mfma_f32_16x16x16f16(in.f[q >> 1].q[q & 1], t.hi[0].q[0], acc[q], 0, 0, 0);
-                acc[q] = __builtin_amdgcn_mfma_f32_16x16x16f16(in.f[q >> 1].q[q & 1], t.lo[0].q[0], acc[q], 0, 0, 0);
+                acc[q] = __builtin_amdgcn_mfma_f32_16x16x16f16(f[q >> 1].q[q & 1], t.hi[0].q[0], acc[q], 0, 0, 0);
+                acc[q] = __builtin_amdgcn_mfma_f32_16x16x16f16(f[q >> 1].q[q & 1], t.lo[0].q[0], acc[q], 0, 0, 0);
             }
+            if (next >= 0) load_weights<0, F>(next, f);
         } else {
-#pragma unroll
-            for (int s = 0; s < KS; ++s)
+            static_for<KS>([&](auto step) {
+                constexpr int s = decltype(step)::value;
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
-                    acc[q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(in.f[4 * s + q].h, t.hi[s].h, acc[q], 0, 0, 0);
-                    acc[q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(in.f[4 * s + q].h, t.lo[s].h, acc[q], 0, 0, 0);
+                    acc[q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f[4 * s + q].h, t.hi[s].h, acc[q], 0, 0, 0);
+                    acc[q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f[4 * s + q].h, t.lo[s].h, acc[q], 0, 0, 0);
                 }
+                if (next >= 0) load_weights<4 * s, 4 * s + 4>(next, f);
+            });
         }
         wave_fence();  // (the last group has been read)
 #pragma unroll
@@ -307,7 +347,7 @@ struct Expand {
             if (!mine[i] || o + first() >= out1) continue;
             Y v[P];
             float d[P];
-            __builtin_memcpy(v, &in.raw[i], 16);
+            __builtin_memcpy(v, &raw[i], 16);
 #pragma unroll
             for (int j = 0; j < P / 4; ++j) {
                 const uint4 u = lds[16 * r + ((first() / 4 + j) ^ r)];
@@ -327,30 +367,32 @@ struct Expand {
     // Groups o, o + step, ...; the next one's loads run ahead.
     __device__ __forceinline__ void run(int o, int step, const Rows<RK> &t, uint4 *lds) const {
         if (o >= out1) return;
-        In in, next;
-        load(o, in);
+        Frag f[F];
+        uint4 raw[N], ahead[N];
+        load_base(o, raw);
+        load_weights<0, F>(o, f);
         while (true) {
-            const bool more = o + step < out1;
-            if (more) load(o + step, next);
-            finish(o, t, in, lds);
-            if (!more) break;
-            in = next;
-            o += step;
+            const int next = o + step < out1 ? o + step : -1;
+            if (next >= 0) load_base(next, ahead);
+            finish(o, next, t, f, raw, lds);
+            if (next < 0) break;
+            __builtin_memcpy(raw, ahead, sizeof(raw));
+            o = next;
         }
     }
 };
 
 // ---------------------------------------------------------------- tiles
 
-// Rows `who` without an adapter, or one of rank 0: y is base.
+// Rows without an adapter: y is base.
 template <class Y>
-__device__ __forceinline__ void copy_rows(const AdapterArgs &a, int64_t row0, int rows, uint64_t who, int out0, int out1) {
+__device__ __forceinline__ void copy_rows(const AdapterArgs &a, const TileRows &rows, int out0, int out1) {
     if (a.y == a.base) return;
     const int units = (out1 - out0) * (int)sizeof(Y) / 16;
-    for (int r = threadIdx.x >> 6; r < rows; r += blockDim.x >> 6) {
-        if (!(who >> r & 1)) continue;
-        const char *from = (const char *)((const Y *)a.base + (row0 + r) * a.base_row + out0);
-        char *to = (char *)((Y *)a.y + (row0 + r) * a.y_row + out0);
+    for (int r = threadIdx.x >> 6; r < 16; r += blockDim.x >> 6) {
+        if (!(rows.who >> r & 1)) continue;
+        const char *from = (const char *)((const Y *)a.base + (rows.row0 + r) * a.base_row + out0);
+        char *to = (char *)((Y *)a.y + (rows.row0 + r) * a.y_row + out0);
         for (int u = threadIdx.x & 63; u < units; u += 64) {
             uint4 v;
             __builtin_memcpy(&v, from + 16 * u, 16);
@@ -383,18 +425,17 @@ __device__ __forceinline__ float sum8(const float *p, int step) {
     return s;
 }
 
-// Both products of a tile of 16 rows (RK: ranks of 16), for outs_each outputs.
+// Both products of a tile of up to 16 rows of one adapter (RK: ranks of 16), for outputs out0 .. out1.
 template <class X, class Y, int RK>
-__global__ __launch_bounds__(kThreads) void adapter_kernel(AdapterArgs a, int outs_each) {
-    constexpr int kPart = kSlices * 16 * RK * kTPitch * 4, kTiles = kSlices * Tile<X>::kBytes;
-    __shared__ uint4 lds[std::max({kPart, kTiles, kSlices * 4096}) / 16];
-    float *part = (float *)lds;  // [slice][rank][row]
-    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), m = lane & 15, g = lane >> 4;
-    const int row0 = blockIdx.x * 16, out0 = blockIdx.z * outs_each, out1 = min(out0 + outs_each, a.out);
-    each_adapter(a, row0, 16, [&](int id, uint64_t who) {
-        if (id < 0) return copy_rows<Y>(a, row0, 16, who, out0, out1);
+struct Products {
+    static constexpr int kPart = kSlices * 16 * RK * kTPitch * 4, kTiles = kSlices * Tile<X>::kBytes;
+    static constexpr int kBytes = std::max({kPart, kTiles, kSlices * 4096});
+    static __device__ __forceinline__ void of(const AdapterArgs &a, int id, const TileRows &rows, int out0, int out1, uint4 *lds) {
+        if (id < 0) return copy_rows<Y>(a, rows, out0, out1);
+        float *part = (float *)lds;  // [slice][rank][row]
+        const int t = own_thread(), lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6), m = lane & 15, g = lane >> 4;
         f32x4_t sum[RK] = {};
-        const Shrink<X, RK> shrink(a, id, row0, who);
+        const Shrink<X, RK> shrink(a, id, rows, lane);
         __syncthreads();  // (the last adapter's outputs have left LDS)
         shrink.run(kChunk * w, kChunk * kSlices, lds + w * Tile<X>::kBytes / 16, sum);
         __syncthreads();
@@ -403,15 +444,36 @@ __global__ __launch_bounds__(kThreads) void adapter_kernel(AdapterArgs a, int ou
 #pragma unroll
             for (int i = 0; i < 4; ++i) part[(w * 16 * RK + 16 * k + 4 * g + i) * kTPitch + m] = sum[k][i];
         __syncthreads();
-        Rows<RK> t;
-        t.set(a.scale == nullptr ? 1.0f : a.scale[id], [&](int k, auto &v) {
+        // The slices' sums: of many ranks each by one thread, of few by every wave for itself, which saves a barrier.
+        constexpr int kSlice = 16 * RK * kTPitch;
+        constexpr bool kShared = RK >= 4;
+        if constexpr (kShared) {
 #pragma unroll
-            for (int i = 0; i < Rows<RK>::N; ++i) v[i] = sum8(part + (k + i) * kTPitch + m, 16 * RK * kTPitch);
+            for (int i = 0; i < 256 * RK / kThreads; ++i) {
+                float *p = part + (i * kThreads + t) / 16 * kTPitch + (t & 15);
+                *p = sum8(p, kSlice);
+            }
+            __syncthreads();
+        }
+        Rows<RK> tr;
+        tr.set(a.scale == nullptr ? 1.0f : a.scale[id], lane, [&](int k, auto &v) {
+#pragma unroll
+            for (int i = 0; i < Rows<RK>::N; ++i) {
+                const float *p = part + (k + i) * kTPitch + m;
+                v[i] = kShared ? *p : sum8(p, kSlice);
+            }
         });
         __syncthreads();
-        const Expand<Y, RK> expand(a, id, row0, who, out1);
-        expand.run(out0 + 64 * w, 64 * kSlices, t, lds + w * 256);
-    });
+        const Expand<Y, RK> expand(a, id, rows, out1, lane);
+        expand.run(out0 + 64 * w, 64 * kSlices, tr, lds + w * 256);
+    }
+};
+
+template <class X, class Y, int RK>
+__global__ __launch_bounds__(kThreads) void adapter_kernel(AdapterArgs a, int outs_each) {
+    __shared__ uint4 lds[Products<X, Y, RK>::kBytes / 16];
+    const int row0 = blockIdx.x * 16, out0 = blockIdx.z * outs_each, out1 = min(out0 + outs_each, a.out);
+    each_adapter(a, row0, 16, [&](int id, uint64_t who) { Products<X, Y, RK>::of(a, id, TileRows{row0, who}, out0, out1, lds); });
 }
 
 template <class X, class Y, int RK>
