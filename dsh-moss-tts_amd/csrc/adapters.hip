@@ -260,9 +260,9 @@ template <int RK>
 struct Rows {
     static constexpr int KS = (RK + 1) / 2, N = RK == 1 ? 4 : 8;  // elements of a lane in a step
     Frag hi[KS], lo[KS];
-    float factor;
+    float scale, down;
     template <class Get>
-    __device__ __forceinline__ void set(float scale, int lane, Get &&get_t) {
+    __device__ __forceinline__ void set(float by, int lane, Get &&get_t) {
         const int g = lane >> 4;
         float v[KS][N], top = 0.0f;
 #pragma unroll
@@ -272,7 +272,8 @@ struct Rows {
             for (int i = 0; i < N; ++i) top = fmaxf(top, fabsf(v[s][i]));
         }
         const Power p = power_of(row_max(top));
-        factor = p.down * scale;
+        scale = by;
+        down = p.down;
 #pragma unroll
         for (int s = 0; s < KS; ++s) split(v[s], p.up, hi[s], lo[s]);
     }
@@ -337,7 +338,7 @@ struct Expand {
         wave_fence();  // (the last group has been read)
 #pragma unroll
         for (int q = 0; q < 4; ++q) {  // outputs 16 q + 4 g .. of row m: piece 4 q + g of its 256 bytes, at that ^ m
-            f32x4_t v = acc[q] * t.factor;
+            f32x4_t v = acc[q] * t.scale * t.down;  // (the power of two last: it rounds only what leaves the range)
             lds[16 * m + ((4 * q + g) ^ m)] = __builtin_bit_cast(uint4, v);
         }
         wave_fence();
