@@ -9,8 +9,9 @@
 // A draw compares u with as many borders as the vocabulary has tokens, and sums of 32-bit exponentials move each by up
 // to 2^-24: one draw in a hundred over 2^17 tokens.  So the row that is drawn from is weighed in 64 bits, at
 // 20 instructions of 8 cycles a logit; all others, of which only the sum is wanted, with the hardware's exponential (the sum's
-// error is some 2^-26 of it, and within 2^-18), which hides behind the reading.  Rows behind which a tree branches take 64 bits for
-// their sums too: 1 - p of a likely child leaves of such an error as many times more as it leaves less of the 1.
+// error is some 2^-26 of it, and within 2^-18), which hides behind the reading.  Where a number then comes so near to the border of a
+// child that the walk asks about that such errors could decide, the walk stops for the sums of that row in 64 bits: one
+// question in 2^16, but many more behind likely children that were rejected, as what they leave of 1 is a small difference.
 //
 // A row is cut into pieces of a wave's values, four pieces a part.  First launch: every row, a workgroup a part, leaves each
 // part's maximum and sum.  Second: a workgroup for each part of a stream; each one walks by itself, weighs its part of the row that
@@ -20,7 +21,8 @@
 //
 // 24 chains of 9 over 130001 fp16 logits and the draft's: 27.5 us for all rows (4 TB/s), 17 for the walk and the two sums, 19 for
 // (p - q)+ and the draw, both of which are 64-bit exponentials on 3.1 million logits (6 us each at best) and a chain of
-// loads.  64 chains of 6 over 16384: 10 + 13 + 12.  16 trees of 27 over 16384: 7 + 17.  All rows in 64 bits took 50 us in place
+// loads, one after the other: the bound of a row's end is each lane's own, so a lane waits for every 16 bytes before it asks for
+// more.  64 chains of 6 over 16384: 10 + 13 + 12.  16 trees of 27 over 16384: 7 + 17.  All rows in 64 bits took 50 us in place
 // of 28.
 #include <algorithm>
 
@@ -41,7 +43,7 @@ struct Stat {
     double s;
 };
 
-// 2^a for a <= 0, as 2^n 2^f with a polynomial through Chebyshev's nodes of |f| <= 1/2, within 2^-45; under
+// 2^a for a <= 0, as 2^n 2^f with a polynomial through Chebyshev's nodes of |f| <= 1/2, within 2^-44.5; under
 // 2^-1010, and for NaN, it is 2^-1010.  n comes out of the low bits of a + 1.5 * 2^52 and goes into the exponent as an
 // integer.
 template <int N>
@@ -148,22 +150,11 @@ __device__ __forceinline__ int2 nodes_of(const VerifyArgs &a, int s) {
     return r0 >= 0 && r1 >= r0 && r1 <= a.rows ? make_int2(r0, min(r1 - r0, a.max_rows)) : make_int2(0, 0);
 }
 
-// The parent of node t, -1: none (node 0, a mask without the node's own bit or without ancestors).
-__device__ __forceinline__ int parent_of(const VerifyArgs &a, int2 rows, int t) {
-    if (t == 0 || t >= rows.y) return -1;
-    if (a.row_mask == nullptr) return t - 1;
-    const uint64_t mask = a.row_mask[rows.x + t], up = mask & ((1ull << t) - 1);
-    return (mask >> t & 1) && up ? 63 - __builtin_clzll(up) : -1;
-}
-
 // ---------------------------------------------------------------- all rows
 
-// What is done for a row: GREEDY finds the largest, SUMS the sums with the hardware's exponential, EXACT those of marked rows in 64 bits.
-enum { GREEDY, SUMS, EXACT };
-
 // One piece of a row, by one wave: EPT values a lane, read V at a time.  Lane 0's is right.
-template <class T, int EPT, int HOW>
-__device__ __forceinline__ Stat piece_stat(const T *p, int c, int vocab, float inv_t, bool marked) {
+template <class T, int EPT, bool GREEDY>
+__device__ __forceinline__ Stat piece_stat(const T *p, int c, int vocab, float inv_t) {
     constexpr int V = std::min<int>(16 / (int)sizeof(T), EPT);
     const int base = c * EPT * 64 + ((int)threadIdx.x & 63) * V;
     float x[EPT / V][V];
@@ -175,10 +166,10 @@ __device__ __forceinline__ Stat piece_stat(const T *p, int c, int vocab, float i
     for (int i = 0; i < EPT / V; ++i)
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            if (HOW == GREEDY && x[i][j] > m) best = base + i * 64 * V + j;
+            if (GREEDY && x[i][j] > m) best = base + i * 64 * V + j;
             m = fmaxf(m, x[i][j]);
         }
-    if constexpr (HOW == GREEDY) {
+    if constexpr (GREEDY) {
         wave_argmax(m, best);
         return Stat{m, m > -INFINITY ? best : -1, 0.0};
     } else {
@@ -190,27 +181,12 @@ __device__ __forceinline__ Stat piece_stat(const T *p, int c, int vocab, float i
         for (int i = 0; i < EPT / V; ++i)
 #pragma unroll
             for (int j = 0; j < V; ++j) more[j & 3] += __builtin_amdgcn_exp2f(fmaf(x[i][j], 0.5f, h) * inv_t * (float)(2.0 * kLog2e));
-        double sum = wave_sum64(((double)more[0] + more[1]) + ((double)more[2] + more[3]));
-        if constexpr (HOW == EXACT)
-            if (marked && sum > 0.0) {  // (neither NaN nor nothing)
-                sum = 0.0;
-#pragma unroll
-                for (int i = 0; i < EPT / V; ++i) {
-                    double v[V];
-                    weights<V>(x[i], m, (double)inv_t * kLog2e, v);
-#pragma unroll
-                    for (int j = 0; j < V; ++j) sum += v[j];
-                }
-                sum = wave_sum64(sum);
-            }
-        return Stat{m, -1, sum};
+        return Stat{m, -1, wave_sum64(((double)more[0] + more[1]) + ((double)more[2] + more[3]))};
     }
 }
-// Whether node has several children; `parent` is the lane's node's.
-__device__ __forceinline__ bool branches(int parent, int node) { return __popcll(__ballot(parent == node)) > 1; }
 
 // One part of one row of the target (blockIdx.y 0) or the draft (1).
-template <class T, int EPT, int HOW>
+template <class T, int EPT, bool GREEDY>
 __global__ __launch_bounds__(kThreads) void stat_kernel(VerifyArgs a, int parts) {
     __shared__ Stat ls[kWaves];
     const int at = blockIdx.x / parts, part = blockIdx.x - at * parts;
@@ -223,8 +199,7 @@ __global__ __launch_bounds__(kThreads) void stat_kernel(VerifyArgs a, int parts)
     const T *p = of_draft ? (const T *)a.y + (rows.x + node) * a.y_row : (const T *)a.x + (rows.x + node) * a.x_row;
     const float inv_t = of_draft ? a.draft_inv_t : a.inv_t;
     const int w = threadIdx.x >> 6;
-    const bool marked = HOW == EXACT && branches(parent_of(a, rows, threadIdx.x & 63), node);
-    const Stat mine = piece_stat<T, EPT, HOW>(p, part * kWaves + w, a.vocab, inv_t, marked);
+    const Stat mine = piece_stat<T, EPT, GREEDY>(p, part * kWaves + w, a.vocab, inv_t);
     if ((threadIdx.x & 63) == 0) ls[w] = mine;
     __syncthreads();
     if (threadIdx.x == 0) {
@@ -236,7 +211,7 @@ __global__ __launch_bounds__(kThreads) void stat_kernel(VerifyArgs a, int parts)
                 r.m = ls[i].m;
                 r.best = ls[i].best;
             }
-        if constexpr (HOW != GREEDY)
+        if constexpr (!GREEDY)
 #pragma unroll
             for (int i = 0; i < kWaves; ++i)
                 if (!(ls[i].s == 0.0)) r.s += ls[i].m == r.m ? ls[i].s : ls[i].s * weight(ls[i].m, r.m, k);
@@ -250,6 +225,8 @@ struct WalkLds {
     Stat p[kTreeMax], q[kTreeMax];
     Draw draw;
     int gone[kTreeMax], n_gone;  // the children of the last node, all rejected
+    int unsure;                  // the node whose children the walk cannot tell apart by these sums, -1: none
+    double part[kWaves];
 };
 
 // The parts of a row together, by 8 lanes; `mine` is the lane's first.
@@ -282,6 +259,29 @@ __device__ __forceinline__ Stat row_stat(const Stat &mine, const Stat *c, int pa
     }
 }
 
+// Sum of a row's weights in 64 bits, by the workgroup; every thread has it.
+template <class T>
+__device__ __forceinline__ double row_sum64(const T *p, int vocab, float m, double k, double (&part)[kWaves]) {
+    constexpr int V = 4;
+    double sum = 0.0;
+#pragma unroll 1
+    for (int e = threadIdx.x * V; e < vocab; e += kThreads * V) {
+        float x[V];
+        double v[V];
+        load_logits<T, V>(p, e, vocab, x);
+        weights<V>(x, m, k, v);
+#pragma unroll
+        for (int j = 0; j < V; ++j) sum += v[j];
+    }
+    sum = wave_sum64(sum);
+    __syncthreads();  // (the last row's have been read)
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = sum;
+    __syncthreads();
+    sum = 0.0;
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) sum += part[i];
+    return sum;
+}
 
 __device__ __forceinline__ double uniform(double u) { return u < 1.0 ? (u > 0.0 ? u : 0.0) : 1.0; }  // (NaN: 1)
 
@@ -295,9 +295,13 @@ struct Node {
 template <class T, bool LARGEST>
 __device__ __forceinline__ Node node_of(const VerifyArgs &a, int2 rows) {
     const int t = threadIdx.x, n = rows.y;
-    Node d{t < n, false, -1, -1, 0.0, -INFINITY, -INFINITY};
+    Node d{t < n, false, -1, t - 1, 0.0, -INFINITY, -INFINITY};
     if (d.in) d.tok = a.tokens[rows.x + t];
-    d.parent = parent_of(a, rows, t);
+    if (d.in && a.row_mask != nullptr) {
+        const uint64_t mask = a.row_mask[rows.x + t], up = mask & ((1ull << t) - 1);
+        d.parent = (mask >> t & 1) && up ? 63 - __builtin_clzll(up) : -1;
+    }
+    if (!d.in || t == 0) d.parent = -1;
     d.known = d.tok >= 0 && d.tok < a.vocab && d.parent >= 0;
     if (!LARGEST && d.known) {
         d.u = uniform(a.uniforms[rows.x + t]);
@@ -307,9 +311,47 @@ __device__ __forceinline__ Node node_of(const VerifyArgs &a, int2 rows) {
     return d;
 }
 
+// What decides a child: `number` < p(t), where number is u q(t), or u times what its elder siblings leave of 1.
+struct Choice {
+    bool accept;
+    bool unsure;  // the sums' errors could decide it
+};
+template <bool LARGEST>
+__device__ __forceinline__ Choice choice_of(const VerifyArgs &a, int n, const Node &d, const Stat &p, const Stat &q, double kp, double kq) {
+    // Errors of 2^-18 of each probability, twice over; of what is left they are as large as of what is gone.
+    constexpr double kNear = 0x1p-17;
+    if constexpr (LARGEST) return Choice{d.known && d.tok == p.best, false};
+    const int t = threadIdx.x, tok = d.tok, parent = d.parent;
+    double prob = 0.0, number = 0.0, gone = 0.0;
+    bool fine = d.known && p.s > 0.0;  // (not NaN)
+    if (fine) prob = weight(d.lx, p.m, kp) / p.s;
+    if (a.y != nullptr) {
+        fine &= q.s > 0.0;
+        if (fine) number = gone = d.u * (weight(d.ly, q.m, kq) / q.s);
+    } else {
+        double left = 1.0;
+        bool again = false;  // an elder sibling is the same token
+        if (a.row_mask != nullptr)
+            for (int j = 1; j < n; ++j) {
+                const int pj = __builtin_amdgcn_readlane(parent, j), tj = __builtin_amdgcn_readlane(tok, j);
+                const bool aj = __builtin_amdgcn_readlane((int)again, j);
+                const double bj = __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(prob), j),
+                                                   __builtin_amdgcn_readlane(__double2loint(prob), j));
+                if (t > j && parent == pj && pj >= 0) {
+                    again |= tok == tj;
+                    if (!aj) left -= bj;
+                }
+            }
+        fine &= !again;
+        number = d.u * (left > 0.0 ? left : 0.0);
+        gone = d.u * (1.0 - left);
+    }
+    return Choice{fine && number < prob, fine && prob > 0.0 && fabs(number - prob) <= kNear * (prob + gone)};
+}
+
 // The walk of one stream, by one workgroup: the rows' sums by all threads, then a lane a node.  pp, qq: the stream's parts; `writes`:
 // whether this workgroup leaves the outputs.
-template <bool LARGEST>
+template <class T, bool LARGEST>
 __device__ __forceinline__ void walk(const VerifyArgs &a, int s, int2 rows, const Node &d, const Stat *pp, const Stat *qq, int parts, bool writes, WalkLds &lds) {
     const int t = threadIdx.x, n = rows.y;
     const bool drafted = a.y != nullptr, in = d.in, known = d.known;
@@ -319,8 +361,6 @@ __device__ __forceinline__ void walk(const VerifyArgs &a, int s, int2 rows, cons
     if ((t >> 3) < all && (t & 7) < parts) first = row_at(t >> 3)[t & 7];
     const double kp = (double)a.inv_t * kLog2e, kq = (double)a.draft_inv_t * kLog2e;
     const int tok = d.tok, parent = d.parent, of = max(parent, 0);
-    const double u = d.u;
-    const float lx = d.lx, ly = d.ly;
     for (int i = t >> 3; i < all; i += kThreads / 8) {
         const bool q = i >= a.max_rows;
         if (i >= kThreads / 8) first = (t & 7) < parts ? row_at(i)[t & 7] : Stat{-INFINITY, -1, 0.0};
@@ -328,65 +368,56 @@ __device__ __forceinline__ void walk(const VerifyArgs &a, int s, int2 rows, cons
         if ((t & 7) == 0) (q ? lds.q[i - a.max_rows] : lds.p[i]) = r;
     }
     __syncthreads();
-    if (t < 64) {
-        bool accept = false;
-        const Stat p = lds.p[of];
-        if constexpr (LARGEST) {
-            accept = known && tok == p.best;
-        } else {
-            double prob = 0.0;
-            const bool fine = known && p.s > 0.0;  // (not NaN)
-            if (fine) prob = weight(lx, p.m, kp) / p.s;
-            if (drafted) {
-                const Stat q = lds.q[of];
-                if (fine && q.s > 0.0) accept = u * (weight(ly, q.m, kq) / q.s) < prob;
-            } else {
-                double left = 1.0;
-                bool again = false;  // an elder sibling is the same token
-                if (a.row_mask != nullptr)
-                    for (int j = 1; j < n; ++j) {
-                        const int pj = __builtin_amdgcn_readlane(parent, j), tj = __builtin_amdgcn_readlane(tok, j);
-                        const bool aj = __builtin_amdgcn_readlane((int)again, j);
-                        const double bj = __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(prob), j),
-                                                           __builtin_amdgcn_readlane(__double2loint(prob), j));
-                        if (t > j && parent == pj && pj >= 0) {
-                            again |= tok == tj;
-                            if (!aj) left -= bj;
-                        }
+    // From node to node by the first child that is accepted.
+    int cur = 0;
+    uint64_t on = 1, exact = 0;  // nodes on the path, and those whose rows' sums are of 64 bits
+    while (true) {
+        if (t < 64) {
+            const Choice c = choice_of<LARGEST>(a, n, d, lds.p[of], drafted ? lds.q[of] : Stat{}, kp, kq);
+            const uint64_t doubt = __ballot(c.unsure && !(exact >> of & 1)), stops = __ballot(c.accept) | doubt;
+            bool unsure = false;
+            while (const uint64_t next = __ballot(parent == cur) & stops) {
+                unsure = doubt >> __builtin_ctzll(next) & 1;
+                if (unsure) break;
+                cur = __builtin_ctzll(next);
+                on |= 1ull << cur;
+            }
+            if (!unsure) {
+                if (in && writes) {  // entry j of the path is the j-th node on it
+                    const int taken = __popcll(on);
+                    if (on >> t & 1) a.path[rows.x + __popcll(on & ((1ull << t) - 1))] = t;
+                    if (t >= taken) a.path[rows.x + t] = -1;
+                }
+                const bool child = !LARGEST && !drafted && parent == cur && known;
+                const uint64_t children = __ballot(child);
+                if (child) lds.gone[__popcll(children & ((1ull << t) - 1))] = tok;
+                if (t == 0) {
+                    const Stat pl = lds.p[cur];
+                    Stat ql{};
+                    if (drafted && cur < n - 1) ql = lds.q[cur];
+                    lds.n_gone = __popcll(children);
+                    lds.draw = Draw{pl.m, ql.m, rows.x + cur, !(pl.s > 0.0) ? DRAW_NONE : (ql.s > 0.0 ? DRAW_REST : DRAW_P)};
+                    if (writes) {
+                        a.accepted[s] = __popcll(on) - 1;
+                        if (LARGEST) a.next[s] = pl.best;
                     }
-                accept = !again && known && u * (left > 0.0 ? left : 0.0) < prob;
+                }
             }
+            if (!LARGEST && t == 0) lds.unsure = unsure ? cur : -1;
         }
-        // from node to node by the first child that is accepted
-        int cur = 0;
-        uint64_t on = 1;
-        while (true) {
-            const uint64_t next = __ballot(accept && parent == cur);
-            if (!next) break;
-            cur = __builtin_ctzll(next);
-            on |= 1ull << cur;
-        }
-        if (in && writes) {  // entry j of the path is the j-th node on it
-            const int taken = __popcll(on);
-            if (on >> t & 1) a.path[rows.x + __popcll(on & ((1ull << t) - 1))] = t;
-            if (t >= taken) a.path[rows.x + t] = -1;
-        }
-        const bool child = !LARGEST && !drafted && parent == cur && known;
-        const uint64_t children = __ballot(child);
-        if (child) lds.gone[__popcll(children & ((1ull << t) - 1))] = tok;
+        __syncthreads();
+        if (LARGEST || __builtin_expect(lds.unsure < 0, 1)) return;
+        const int row = lds.unsure;
+        const double sum = row_sum64((const T *)a.x + (rows.x + row) * a.x_row, a.vocab, lds.p[row].m, kp, lds.part);
+        double sum_q = 0.0;
+        if (drafted) sum_q = row_sum64((const T *)a.y + (rows.x + row) * a.y_row, a.vocab, lds.q[row].m, kq, lds.part);
         if (t == 0) {
-            const Stat pl = lds.p[cur];
-            Stat ql{};
-            if (drafted && cur < n - 1) ql = lds.q[cur];
-            lds.n_gone = __popcll(children);
-            lds.draw = Draw{pl.m, ql.m, rows.x + cur, !(pl.s > 0.0) ? DRAW_NONE : (ql.s > 0.0 ? DRAW_REST : DRAW_P)};
-            if (writes) {
-                a.accepted[s] = __popcll(on) - 1;
-                if (LARGEST) a.next[s] = pl.best;
-            }
+            lds.p[row].s = sum;
+            if (drafted) lds.q[row].s = sum_q;
         }
+        exact |= 1ull << row;
+        __syncthreads();
     }
-    __syncthreads();
 }
 
 // ---------------------------------------------------------------- the draw
@@ -604,7 +635,7 @@ __global__ __launch_bounds__(kThreads) void walk_kernel(VerifyArgs a, int pieces
     }
     const double u = uniform(a.uniforms[rows.x]);
     const Node node = node_of<T, false>(a, rows);
-    walk<false>(a, s, rows, node, ws.p + (size_t)s * a.max_rows * parts, ws.q + (size_t)s * a.max_rows * parts, parts, part == 0, wl);
+    walk<T, false>(a, s, rows, node, ws.p + (size_t)s * a.max_rows * parts, ws.q + (size_t)s * a.max_rows * parts, parts, part == 0, wl);
     const Draw d = wl.draw;
     if (DRAFT && t == 0 && part == 0) ws.draw[s] = d;
     if (d.mode == DRAW_NONE) {
@@ -646,7 +677,7 @@ __global__ __launch_bounds__(kThreads) void greedy_kernel(VerifyArgs a, int part
     const int2 rows = nodes_of(a, s);
     if (no_rows(a, s, rows, true)) return;
     const Stat *p = verify_ws(a.streams, a.max_rows, parts, false, a.ws).p + (size_t)s * a.max_rows * parts;
-    walk<true>(a, s, rows, node_of<float, true>(a, rows), p, p, parts, true, wl);  // (no logit is read)
+    walk<float, true>(a, s, rows, node_of<float, true>(a, rows), p, p, parts, true, wl);  // (no logit is read)
 }
 
 // The draw behind a rejected token: a workgroup for each part of a stream has its masses of (p - q)+, the last one draws.
@@ -684,7 +715,7 @@ __global__ __launch_bounds__(kThreads) void rest_kernel(VerifyArgs a, int pieces
 // All of it in one launch, a workgroup a stream, where its rows have no more than kSmallPieces pieces: the smallest calls are
 // launches and chains of loads.
 constexpr int kSmallPieces = 32, kSmallEpt = 16;
-template <class T, int HOW>
+template <class T, bool GREEDY>
 __global__ __launch_bounds__(kThreads) void small_kernel(VerifyArgs a, int pieces) {
     constexpr int EPT = kSmallEpt;
     __shared__ Stat p[kSmallPieces], q[kSmallPieces];
@@ -695,21 +726,20 @@ __global__ __launch_bounds__(kThreads) void small_kernel(VerifyArgs a, int piece
     const int2 rows = nodes_of(a, s);
     if (no_rows(a, s, rows, true)) return;
     const bool drafted = a.y != nullptr;
-    const Node mine = node_of<T, HOW == GREEDY>(a, rows);
-    const int parent = HOW == EXACT ? parent_of(a, rows, t & 63) : -1;
+    const Node mine = node_of<T, GREEDY>(a, rows);
     const int units = rows.y * pieces;
     for (int i = w; i < units; i += kWaves) {
         const int node = i / pieces, c = i - node * pieces;
-        const Stat m = piece_stat<T, EPT, HOW>((const T *)a.x + (rows.x + node) * a.x_row, c, a.vocab, a.inv_t, HOW == EXACT && branches(parent, node));
+        const Stat m = piece_stat<T, EPT, GREEDY>((const T *)a.x + (rows.x + node) * a.x_row, c, a.vocab, a.inv_t);
         if ((t & 63) == 0) p[i] = m;
         if (drafted && node < rows.y - 1) {
-            const Stat n = piece_stat<T, EPT, HOW>((const T *)a.y + (rows.x + node) * a.y_row, c, a.vocab, a.draft_inv_t, false);
+            const Stat n = piece_stat<T, EPT, GREEDY>((const T *)a.y + (rows.x + node) * a.y_row, c, a.vocab, a.draft_inv_t);
             if ((t & 63) == 0) q[i] = n;
         }
     }
     __syncthreads();
-    walk<HOW == GREEDY>(a, s, rows, mine, p, q, pieces, true, wl);
-    if constexpr (HOW != GREEDY) {
+    walk<T, GREEDY>(a, s, rows, mine, p, q, pieces, true, wl);
+    if constexpr (!GREEDY) {
         const Draw d = wl.draw;
         int got = -1;
         if (d.mode != DRAW_NONE) {
@@ -767,15 +797,12 @@ hipError_t verify_e(const VerifyArgs &a, hipStream_t s) {
     const int parts = parts_of(a.streams * a.max_rows, a.vocab), pieces = (a.vocab + EPT * 64 - 1) / (EPT * 64);
     const dim3 rows((unsigned)a.streams * a.max_rows * parts, a.y != nullptr ? 2 : 1), of_streams((unsigned)a.streams * parts);
     if (a.greedy) {
-        hipLaunchKernelGGL((stat_kernel<T, EPT, GREEDY>), rows, dim3(kThreads), 0, s, a, parts);
+        hipLaunchKernelGGL((stat_kernel<T, EPT, true>), rows, dim3(kThreads), 0, s, a, parts);
         if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;  // (what follows trusts what it leaves)
         hipLaunchKernelGGL(greedy_kernel, dim3(a.streams), dim3(kThreads), 0, s, a, parts);
         return hipGetLastError();
     }
-    if (a.row_mask != nullptr)
-        hipLaunchKernelGGL((stat_kernel<T, EPT, EXACT>), rows, dim3(kThreads), 0, s, a, parts);
-    else
-        hipLaunchKernelGGL((stat_kernel<T, EPT, SUMS>), rows, dim3(kThreads), 0, s, a, parts);
+    hipLaunchKernelGGL((stat_kernel<T, EPT, false>), rows, dim3(kThreads), 0, s, a, parts);
     if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
     if (a.y != nullptr) {
         hipLaunchKernelGGL((walk_kernel<T, EPT, true>), of_streams, dim3(kThreads), 0, s, a, pieces, parts);
@@ -793,11 +820,9 @@ hipError_t verify_t(const VerifyArgs &a, hipStream_t s) {
     if (small(a.max_rows, a.vocab)) {
         const int pieces = (a.vocab + kSmallEpt * 64 - 1) / (kSmallEpt * 64);
         if (a.greedy)
-            hipLaunchKernelGGL((small_kernel<T, GREEDY>), dim3(a.streams), dim3(kThreads), 0, s, a, pieces);
-        else if (a.row_mask != nullptr)
-            hipLaunchKernelGGL((small_kernel<T, EXACT>), dim3(a.streams), dim3(kThreads), 0, s, a, pieces);
+            hipLaunchKernelGGL((small_kernel<T, true>), dim3(a.streams), dim3(kThreads), 0, s, a, pieces);
         else
-            hipLaunchKernelGGL((small_kernel<T, SUMS>), dim3(a.streams), dim3(kThreads), 0, s, a, pieces);
+            hipLaunchKernelGGL((small_kernel<T, false>), dim3(a.streams), dim3(kThreads), 0, s, a, pieces);
         return hipGetLastError();
     }
     switch (ept_of(a.streams * a.max_rows, a.vocab)) {

@@ -482,17 +482,18 @@ int moss_hip_token_logprobs_workspace(int rows, int vocab, int top_k, size_t *by
  *   draft_logits NULL: the tokens were picked outright.  Of a node's children, in the order of their rows, c is accepted
  *     where u_c (1 - p of the different tokens rejected before it) < p(t_c); the token behind them is drawn from p without the
  *     rejected tokens.  A child whose token an earlier one had is rejected.
- *   greedy: accepted where it is the likeliest (of equal logits the lowest index; NaN is none), which also follows.
+ *   greedy: accepted where it is the likeliest (of equal logits the lowest index; NaN is none, +inf may be), which also follows.
  * uniforms [rows]: u of each node, numbers of [0, 1) (others count as the nearest of 0 and 1, NaN as 1); row 0's draws the next token: the
  * first whose cumulative sum, in the order of the vocabulary, passes u times the whole.  Where nothing is left over,
- * it is drawn from p.  The row that is drawn from is weighed and summed in 64 bits (what is under 2^-980 of its largest counts as nothing); the sums
- * that acceptance goes by are within 2^-18 of themselves, those of rows with several children, of whose p little may be left, within 2^-44.  The streams' row ranges lie apart.  greedy takes no uniforms and no draft_logits.
+ * it is drawn from p.  The row that is drawn from is weighed and summed in 64 bits (what is under 2^-980 of its largest counts as
+ * nothing); acceptance goes by 32-bit exponentials and, where their errors (2^-18 of a probability) could decide, by 64-bit ones, within
+ * 2^-44.  The streams' row ranges lie apart.  greedy takes no uniforms and no draft_logits.
  *   accepted [streams]: drafted nodes accepted.
  *   path [rows]: entry row_start[s] + j is the node that the walk took as its j-th (0 first), -1 past the last: what
  *     moss_hip_kv_compact takes.  Rows of no stream, and a stream's rows past max_rows, stay as they were.
  *   next_token [streams]: the token behind the last node of the path.
- * -inf logits are ruled out.  A row with a NaN or +inf, or of nothing but -inf, is no distribution: no child of it is
- * accepted, and no token (-1) follows; a draft's row like that rejects its child and the next token is drawn from p.  A token
+ * -inf logits are ruled out.  A row with a NaN or +inf (greedy: of NaN and -inf alone), or of nothing but -inf, is no distribution: no
+ * child of it is accepted, and no token (-1) follows; a draft's row like that rejects its child and the next token is drawn from p.  A token
  * outside [0, vocab) is rejected.  Without rows, or with a row range not within [0, rows], a stream has accepted 0 and
  * next_token -1.  vocab <= 2^20.  workspace as above: moss_hip_verify_tokens_workspace bytes (draft: whether draft_logits are
  * given), which are enough for any call of the same vocab with no more streams and max_rows, and with draft_logits or without where draft is 1. */

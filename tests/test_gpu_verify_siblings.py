@@ -1,4 +1,5 @@
-"""Trees of tokens picked outright whose likely siblings were rejected: what is left of the probability is a small difference (GPU)."""
+"""Decisions of the verification that come near their borders, and those behind likely siblings that were rejected, where what is left of the
+probability is a small difference (GPU)."""
 import numpy as np
 import pytest
 
@@ -41,3 +42,38 @@ def test_verify_behind_likely_siblings(torch_gpu, vocab, kids, dtype, left):
     for g, w in zip(got, want):
         assert np.array_equal(g, w)
     assert np.array_equal(got[0], (np.arange(streams) + 1) % 2)
+
+
+@pytest.mark.parametrize("vocab,rows", [(300, 6), (1024, 5), (9000, 6), (40000, 4), (130001, 5)])
+@pytest.mark.parametrize("dtype", ["float32", "float16"])
+@pytest.mark.parametrize("draft", [False, True])
+def test_verify_numbers_at_their_borders(torch_gpu, vocab, rows, dtype, draft):
+    """Numbers 2^-30 of themselves above or below the border of their child, several in one chain: probabilities are within 2^-44 there.
+    (Only what is accepted is compared: the draws' numbers come near to no border on purpose.)"""
+    torch = torch_gpu
+    print(f"borders {vocab} {dtype} {draft}", flush=True)
+    rng = np.random.default_rng(vocab + rows)
+    streams, dt = 24 if vocab < 50000 else 6, getattr(torch, dtype)
+    x = 2.0 * rng.standard_normal((streams * rows, vocab)).astype(np.float32)
+    tok = rng.integers(0, vocab, streams * rows).astype(np.int32)
+    x[np.arange(len(tok))[:-1], tok[1:]] += np.float32(12.0)
+    y = None
+    if draft:  # the draft is surer of its tokens than the target, so that every border is below 1
+        y = (x + 0.2 * rng.standard_normal(x.shape)).astype(np.float32)
+        y[np.arange(len(tok))[:-1], tok[1:]] += np.float32(3.0)
+    u, want = rng.random(len(tok)), np.zeros(streams, np.int64)
+    for s in range(streams):
+        stop = int(rng.integers(1, rows + 1))  # the first node that is rejected, or none
+        want[s] = stop - 1
+        for i in range(1, rows):
+            r = s * rows + i
+            p = so.softmax(_held(torch, x[r - 1:r], dt)[0], 0.8)[tok[r]]
+            border = p / (so.softmax(_held(torch, y[r - 1:r], dt)[0], 0.9)[tok[r]] if draft else 1.0)
+            assert 0 < border < 0.9999999
+            u[r] = border * (1.0 + (2.0 ** -30 if i >= stop else -(2.0 ** -30)))
+    start = (np.arange(streams + 1) * rows).astype(np.int32)
+    kw = dict(inv_temperature=0.8, draft_inv_temperature=0.9)
+    for mask in [None] if draft else [None, np.tile(np.array([(1 << i + 1) - 1 for i in range(rows)], np.uint64), streams)]:
+        acc, path, _ = _verify(torch, x, tok, start, rows, u, y=y, mask=mask, dtype=dt, **kw)
+        assert np.array_equal(acc, want)
+        assert np.array_equal(path.reshape(streams, rows), np.where(np.arange(rows) <= want[:, None], np.arange(rows), -1))
