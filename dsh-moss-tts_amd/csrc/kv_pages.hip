@@ -279,7 +279,8 @@ __global__ __launch_bounds__(kBookThreads) void reserve_kernel(ReserveArgs a, in
 }
 
 // The first `slots` positions of one head of a page in one of the layers' K's and V's.  Memory bound: 32 streams' copies of half a
-// page of 32 layers x 8 heads x 128 int8, 69 MB, 31 us (4.4 TB/s).  A workgroup of all heads, whose pieces then lie at steps of a power
+// page of 32 layers x 8 heads x 128 int8, 69 MB, 31 us (4.4 TB/s), a load of a thread at a time.  Where nothing is copied the workgroups
+// still start: 32768 at 64 streams of 32 layers x 8 heads, 8.5 us.  A workgroup of all heads, whose pieces then lie at steps of a power
 // of two, took 50.
 template <bool SCALES>
 __global__ __launch_bounds__(kThreads) void copy_kernel(ReserveArgs a, KvLayers l) {
@@ -304,12 +305,13 @@ __global__ __launch_bounds__(kThreads) void copy_kernel(ReserveArgs a, KvLayers 
 
 // ---------------------------------------------------------------- compact
 
-constexpr int kMovesPerThread = 8;  // 16-byte pieces in flight
+constexpr int kMovesPerThread = 8;  // 16-byte pieces, all of which are loaded before the first is stored
 
 // One workgroup: the rows of one stream in pools_each of the layers' K's and V's, heads_each heads.  The list of moves is made
 // once; then, pool by pool and a group of heads at a time, all rows of a head are in registers before the first is
 // stored, so any row may take any other's place.  64 streams, 12 rows each of 32 layers x 8 heads x 128 bytes and scales: 36 us,
-// 2.3 TB/s in pieces of 128 bytes whose heads lie at steps of a power of two.
+// 2.3 TB/s in pieces of 128 bytes whose heads lie at steps of a power of two.  The pieces lie in scratch memory (144 bytes a lane), so a
+// thread has one load in flight at a time.
 template <bool SCALES>
 __global__ __launch_bounds__(kThreads) void compact_kernel(CompactArgs a, KvLayers l, int pools_each, int heads_each) {
     __shared__ size_t from[kTreeMax], to[kTreeMax];  // vectors of head 0
