@@ -12,10 +12,10 @@
 //
 // Weights are fp16, laid out once in the order in which a wave's lanes hold them, so that a load is 1 KiB in one piece.
 // Rows go through LDS for the same reason: as an operand, lanes next to each other hold different rows, and 64 separate
-// accesses a load made the L1 the limit: 8191 fp16 rows of 4096 -> 4096, rank 64, took 129 us, 86 through LDS, now 79 (2.5 TB/s of the
+// accesses a load made the L1 the limit: 8191 fp16 rows of 4096 -> 4096, rank 64, took 129 us, 86 through LDS, now 77 (2.6 TB/s of the
 // 201 MB that it reads and writes; a copy of 134 MB in tiles of 16 rows reaches 3.2).  What is left is that a workgroup's registers
-// fill a compute unit, so that its two products do not overlap with another's.  2896 fp32 rows of 768 -> 2304, rank 16: 13.9 us, 4.5
-// TB/s.  One row: 5.7 us, a chain of loads.
+// fill a compute unit, so that its two products do not overlap with another's.  2896 fp32 rows of 768 -> 2304, rank 16: 13.8 us, 4.6
+// TB/s.  One row: 5.3 us, a chain of loads.
 //
 // No kernel keeps anything in scratch memory: weights are held as far as they have to run ahead, in places that the next ones take as
 // soon as they have been used; places in LDS are worked out anew for each tile; and the eight partial sums of t are added up once
@@ -164,6 +164,7 @@ template <class X, int RK>
 struct Shrink {
     using T = Tile<X>;
     static constexpr int W = T::W;
+    static constexpr bool kPeel = RK < 8;  // whether the last chunk has code of its own
     static constexpr int KB = std::min(RK, 2), R = std::min(RK, 4);  // 16s of ranks at a time, and whose weights are held
     const X *x[T::N];  // the rows of this lane's pieces
     const __half *w;
@@ -183,7 +184,7 @@ struct Shrink {
 #pragma unroll
         for (int i = 0; i < T::N; ++i) {
             __builtin_memcpy(&raw[i], x[i] + min(col, cols - 8 / W), 16);
-            if (col >= cols) raw[i] = uint4{};  // (of the last chunk)
+            if (!kPeel && col >= cols) raw[i] = uint4{};  // (of the last chunk; else in LDS, so that nothing waits here)
         }
     }
     __device__ __forceinline__ void load_weights(int c, int k, Frag (&f)[4]) const {
@@ -191,64 +192,72 @@ struct Shrink {
         for (int s = 0; s < 4; ++s) f[s].u = *(const uint4 *)(w + ((size_t)min(c / 32 + s, cols / 32 - 1) * RK + k) * 512);
     }
     // Chunks c, c + step, ... of the columns, into sum.  The rows' loads run a chunk ahead, the weights' R 16s of ranks: all of a
-    // chunk's at rank 128 would be half of the registers.
+    // chunk's at rank 128 would be half of the registers.  No load stands behind a branch, so that each is waited for by itself, but at rank
+    // 128, where a last chunk of its own takes too many registers (271 -> 286 us, 7784 fp32 rows of 3 adapters in turn, 4096 -> 4096).
     __device__ __forceinline__ void run(int c, int step, uint4 *lds, f32x4_t (&sum)[RK]) const {
         if (c >= cols) return;
-        const int m = lane & 15, g = lane >> 4;
         uint4 raw[T::N];
         Frag f[R][4];
         load(c, raw);
 #pragma unroll
         for (int k = 0; k < R; ++k) load_weights(c, k, f[k]);
-        while (true) {
-            wave_fence();  // (the last chunk has been read)
+        if constexpr (kPeel) {
+            for (; c + step < cols; c += step) chunk(c, c + step, true, lds, raw, f, sum);
+            chunk(c, c, false, lds, raw, f, sum);
+        } else {
+            for (; c < cols; c += step) chunk(c, c + step, c + step < cols, lds, raw, f, sum);
+        }
+    }
+    // Chunk c, and with `more` the loads of chunk next.
+    __device__ __forceinline__ void chunk(int c, int next, bool more, uint4 *lds, uint4 (&raw)[T::N], Frag (&f)[R][4], f32x4_t (&sum)[RK]) const {
+        const int m = lane & 15, g = lane >> 4;
+        if (kPeel && c + kChunk > cols && c + T::piece_of(lane) * (8 / W) >= cols)
 #pragma unroll
-            for (int i = 0; i < T::N; ++i) lds[T::at(T::row_of(lane, i), T::piece_of(lane))] = raw[i];
-            wave_fence();
-            const int next = c + step;
-            Frag hi[4], lo[4];
-            float down = 1.0f;
-            if constexpr (W == 1) {
+            for (int i = 0; i < T::N; ++i) raw[i] = uint4{};
+        wave_fence();  // (the last chunk has been read)
 #pragma unroll
-                for (int s = 0; s < 4; ++s) hi[s].u = lds[T::at(m, 4 * s + g)];
-            } else {
-                float v[4][8], top = 0.0f;
+        for (int i = 0; i < T::N; ++i) lds[T::at(T::row_of(lane, i), T::piece_of(lane))] = raw[i];
+        wave_fence();
+        Frag hi[4], lo[4];
+        float down = 1.0f;
+        if constexpr (W == 1) {
 #pragma unroll
-                for (int s = 0; s < 4; ++s) {
-                    const uint4 two[2] = {lds[T::at(m, 8 * s + 2 * g)], lds[T::at(m, 8 * s + 2 * g + 1)]};
-                    __builtin_memcpy(v[s], two, 32);
+            for (int s = 0; s < 4; ++s) hi[s].u = lds[T::at(m, 4 * s + g)];
+        } else {
+            float v[4][8], top = 0.0f;
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[s][i]));
-                }
-                const Power p = power_of(row_max(top));
-                down = p.down;
+            for (int s = 0; s < 4; ++s) {
+                const uint4 two[2] = {lds[T::at(m, 8 * s + 2 * g)], lds[T::at(m, 8 * s + 2 * g + 1)]};
+                __builtin_memcpy(v[s], two, 32);
 #pragma unroll
-                for (int s = 0; s < 4; ++s) split(v[s], p.up, hi[s], lo[s]);
+                for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[s][i]));
+            }
+            const Power p = power_of(row_max(top));
+            down = p.down;
+#pragma unroll
+            for (int s = 0; s < 4; ++s) split(v[s], p.up, hi[s], lo[s]);
+        }
+#pragma unroll
+        for (int k0 = 0; k0 < RK; k0 += KB) {
+            if (more && k0 == RK - R) load(next, raw);  // (behind the last weights of this chunk, which are waited for first)
+            f32x4_t acc[KB] = {};
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+#pragma unroll
+                for (int k = 0; k < KB; ++k) acc[k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f[(k0 + k) % R][s].h, hi[s].h, acc[k], 0, 0, 0);
+                if constexpr (W == 2)
+#pragma unroll
+                    for (int k = 0; k < KB; ++k) acc[k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f[(k0 + k) % R][s].h, lo[s].h, acc[k], 0, 0, 0);
             }
 #pragma unroll
-            for (int k0 = 0; k0 < RK; k0 += KB) {
-                if (k0 == RK - R && next < cols) load(next, raw);  // (behind the last weights of this chunk, which are waited for first)
-                f32x4_t acc[KB] = {};
+            for (int k = 0; k < KB; ++k) {
+                if (k0 + k + R < RK)
+                    load_weights(c, k0 + k + R, f[(k0 + k) % R]);
+                else if (more)
+                    load_weights(next, k0 + k + R - RK, f[(k0 + k) % R]);
 #pragma unroll
-                for (int s = 0; s < 4; ++s) {
-#pragma unroll
-                    for (int k = 0; k < KB; ++k) acc[k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f[(k0 + k) % R][s].h, hi[s].h, acc[k], 0, 0, 0);
-                    if constexpr (W == 2)
-#pragma unroll
-                        for (int k = 0; k < KB; ++k) acc[k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f[(k0 + k) % R][s].h, lo[s].h, acc[k], 0, 0, 0);
-                }
-#pragma unroll
-                for (int k = 0; k < KB; ++k) {
-                    if (k0 + k + R < RK)
-                        load_weights(c, k0 + k + R, f[(k0 + k) % R]);
-                    else if (next < cols)
-                        load_weights(next, k0 + k + R - RK, f[(k0 + k) % R]);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) sum[k0 + k][i] = fmaf(acc[k][i], down, sum[k0 + k][i]);
-                }
+                for (int i = 0; i < 4; ++i) sum[k0 + k][i] = fmaf(acc[k][i], down, sum[k0 + k][i]);
             }
-            if (next >= cols) break;
-            c = next;
         }
     }
 };
@@ -284,6 +293,7 @@ struct Rows {
 template <class Y, int RK>
 struct Expand {
     static constexpr int KS = Rows<RK>::KS, F = RK == 1 ? 2 : 4 * KS;  // 16-byte loads of weights
+    static constexpr bool kPeel = RK < 8;
     static constexpr int P = 16 / (int)sizeof(Y), N = 16 / P;          // outputs of a piece of y, pieces of a lane
     const Y *base[N];
     Y *y[N];
@@ -298,23 +308,24 @@ struct Expand {
         for (int i = 0; i < N; ++i) {
             const int r = row_of(i);
             mine[i] = rows.who >> r & 1;
-            base[i] = (const Y *)a.base + (rows.row0 + r) * a.base_row + first();
+            base[i] = (const Y *)a.base + (rows.row0 + (mine[i] ? r : __builtin_ctzll(rows.who))) * a.base_row;  // (others read that one)
             y[i] = (Y *)a.y + (rows.row0 + r) * a.y_row + first();
         }
         w = (const __half *)a.b + id * b_size(a.max_rank, a.out) + 8 * lane;
     }
     __device__ __forceinline__ void load_base(int o, uint4 (&raw)[N]) const {
+        const int at = min(o + first(), out1 - P);
 #pragma unroll
         for (int i = 0; i < N; ++i)
-            if (mine[i] && o + first() < out1) __builtin_memcpy(&raw[i], base[i] + o, 16);
+            if (kPeel || mine[i]) __builtin_memcpy(&raw[i], base[i] + at, 16);  // (rows of others only where it saves a branch)
     }
     template <int FROM, int TO>
     __device__ __forceinline__ void load_weights(int o, Frag (&f)[F]) const {
 #pragma unroll
         for (int i = FROM; i < TO; ++i) f[i].u = *(const uint4 *)(w + ((size_t)(o / 64) * F + i) * 512);
     }
-    // Group o; the weights of group `next` (none: -1) take the places of those that have been used.
-    __device__ __forceinline__ void finish(int o, int next, const Rows<RK> &t, Frag (&f)[F], const uint4 (&raw)[N], uint4 *lds) const {
+    // Group o; with `more`, the weights of group next take the places of those that have been used.
+    __device__ __forceinline__ void finish(int o, int next, bool more, const Rows<RK> &t, Frag (&f)[F], const uint4 (&raw)[N], uint4 *lds) const {
         const int m = lane & 15, g = lane >> 4;
         f32x4_t acc[4] = {};
         if constexpr (RK == 1) {
@@ -323,7 +334,7 @@ struct Expand {
                 acc[q] = __builtin_amdgcn_mfma_f32_16x16x16f16(f[q >> 1].q[q & 1], t.hi[0].q[0], acc[q], 0, 0, 0);
                 acc[q] = __builtin_amdgcn_mfma_f32_16x16x16f16(f[q >> 1].q[q & 1], t.lo[0].q[0], acc[q], 0, 0, 0);
             }
-            if (next >= 0) load_weights<0, F>(next, f);
+            if (more) load_weights<0, F>(next, f);
         } else {
             static_for<KS>([&](auto step) {
                 constexpr int s = decltype(step)::value;
@@ -332,7 +343,7 @@ struct Expand {
                     acc[q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f[4 * s + q].h, t.hi[s].h, acc[q], 0, 0, 0);
                     acc[q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f[4 * s + q].h, t.lo[s].h, acc[q], 0, 0, 0);
                 }
-                if (next >= 0) load_weights<4 * s, 4 * s + 4>(next, f);
+                if (more) load_weights<4 * s, 4 * s + 4>(next, f);
             });
         }
         wave_fence();  // (the last group has been read)
@@ -372,13 +383,20 @@ struct Expand {
         uint4 raw[N], ahead[N];
         load_base(o, raw);
         load_weights<0, F>(o, f);
-        while (true) {
-            const int next = o + step < out1 ? o + step : -1;
-            if (next >= 0) load_base(next, ahead);
-            finish(o, next, t, f, raw, lds);
-            if (next < 0) break;
-            __builtin_memcpy(raw, ahead, sizeof(raw));
-            o = next;
+        if constexpr (kPeel) {
+            for (; o + step < out1; o += step) {
+                load_base(o + step, ahead);
+                finish(o, o + step, true, t, f, raw, lds);
+                __builtin_memcpy(raw, ahead, sizeof(raw));
+            }
+            finish(o, o, false, t, f, raw, lds);
+        } else {
+            for (; o < out1; o += step) {
+                const bool more = o + step < out1;
+                if (more) load_base(o + step, ahead);
+                finish(o, o + step, more, t, f, raw, lds);
+                __builtin_memcpy(raw, ahead, sizeof(raw));
+            }
         }
     }
 };
@@ -488,7 +506,13 @@ hipError_t launch(const AdapterArgs &a, hipStream_t s) {
     const int each = std::min(of_tile, std::max(2, 512 / tiles));
     const int slices = std::min(std::max(1, 512 / (tiles * each)), std::max(1, groups / kSlices));
     const int outs = (groups + slices - 1) / slices * 64;
-    hipLaunchKernelGGL((adapter_kernel<X, Y, RK>), dim3(tiles, each, (a.out + outs - 1) / outs), dim3(kThreads), 0, s, a, outs);
+    // Two workgroups of fp16 kernels of up to 32 ranks fit a compute unit, and where there is about one for each, some share one while others
+    // have none.  More than half of the LDS keeps them apart: 3560 rows in runs, 4096 -> 4096, rank 32, 25.4 -> 20.6 us, in turn 43 -> 53; with
+    // more tiles it costs (8192 rows in runs 47 -> 53), with fewer, where more of a tile's workgroups have work, too (285 rows of
+    // 58 adapters 11 -> 16), and of up to 16 ranks rows in turn lose more (1221: 11.4 -> 16.5) than runs gain (21.6 -> 18.4).
+    constexpr bool kTwo = RK == 2 && sizeof(X) == 2 && sizeof(Y) == 2;
+    const unsigned spare = kTwo && each <= 2 && tiles <= 256 ? 82 * 1024 - Products<X, Y, RK>::kBytes : 0;
+    hipLaunchKernelGGL((adapter_kernel<X, Y, RK>), dim3(tiles, each, (a.out + outs - 1) / outs), dim3(kThreads), spare, s, a, outs);
     return hipGetLastError();
 }
 
